@@ -490,6 +490,113 @@ PRNN_API int prnn_gru_decode_x(const void* h, const void* x, const void* w, cons
                                void* out, const int* block_table, int B, int d, int d_in,
                                int n_heads, float cap, int has_cap, int dtype, void* stream);
 
+/* ---- Decayed linear attention --------------------------------------------
+ * Per head, with a state S (Dk x Dv, fp32) and a log decay g_t per token:
+ *   S_t = exp(g_t) S_{t-1} + k_t v_t^T,   o_t = scale q_t^T S_t.
+ * Arrays are given by strides (in elements; a head's values are contiguous) and may have fewer
+ * heads than H (dividing it): consecutive heads then share one.
+ *
+ * A batch is B sequences of T tokens, or (cu_seqlens, int32 on the device, n_seq + 1 offsets)
+ * one packed stream of T tokens with B = 1; offsets outside the stream are clamped into it.
+ * g: float32 (g_dtype 0) or the storage type; one per head where g_sb = g_st = 0.
+ * h0: rows of (H, Dk, Dv) floats, or NULL (zeros); sequence s starts from row s, or
+ * h0_table[s]; a row outside [0, h0_rows) is none (zeros).  state_out takes the final states in
+ * the same way (out_table, out_rows); it may be h0 itself if no two sequences share a row.
+ */
+typedef struct prnn_la_view {
+  const void* p;
+  long long sb, st, sh; /* strides: batch, token, head */
+  int heads;
+} prnn_la_view;
+
+typedef struct prnn_linear_attention_problem {
+  prnn_la_view q, k, v;
+  const void* g;
+  long long g_sb, g_st, g_sh;
+  const float* h0;
+  const int* h0_table;
+  const int* cu_seqlens;
+  int h0_rows, n_seq;
+  int B, T, H, Dk, Dv;
+  int g_dtype, dtype;
+  float scale;
+} prnn_linear_attention_problem;
+
+PRNN_API size_t
+prnn_linear_attention_workspace_size(const prnn_linear_attention_problem* problem);
+PRNN_API int prnn_linear_attention(const prnn_linear_attention_problem* problem,
+                                   const prnn_la_view* out, float* state_out, const int* out_table,
+                                   int out_rows, void* workspace, size_t workspace_bytes,
+                                   void* stream);
+
+/* Gradients for go = dL/do (strided) and gs = dL/dS_T (sequence, H, Dk, Dv; NULL: zero): dq,
+ * dk, dv (batch, token, heads of that array, width) in the storage type, dg (batch, token, H),
+ * or (H) where g is per head, in g's type (NULL: not wanted), dh0 like gs in float32 (NULL: not
+ * wanted; needed for dg where h0 is given).  No block table. */
+PRNN_API size_t prnn_linear_attention_backward_workspace_size(
+    const prnn_linear_attention_problem* problem, int decay_grad);
+PRNN_API int prnn_linear_attention_backward(const prnn_linear_attention_problem* problem,
+                                            const prnn_la_view* go, const float* gs, void* dq,
+                                            void* dk, void* dv, void* dg, float* dh0,
+                                            void* workspace, size_t workspace_bytes, void* stream);
+
+/* One token per row: the states (rows, H, Dk, Dv) advance in place, row b's at block_table[b]
+ * (NULL: b; outside [0, rows): from zeros, not kept).  *_sb, *_sh: strides between rows and
+ * heads; out is (B, H, Dv), contiguous. */
+PRNN_API int prnn_linear_attention_step(const void* q, long long q_sb, long long q_sh, int q_heads,
+                                        const void* k, long long k_sb, long long k_sh, int k_heads,
+                                        const void* v, long long v_sb, long long v_sh, int v_heads,
+                                        const void* g, long long g_sb, long long g_sh, int g_dtype,
+                                        float* state, const int* block_table, int rows, void* out,
+                                        int B, int H, int Dk, int Dv, float scale, int dtype,
+                                        void* stream);
+
+/* ---- Group norm, channels last --------------------------------------------
+ * x, gate, y (N, L, C), statistics over a sample's L tokens and a group's C / G channels (L = 1:
+ * per token).  y = act(z) with z = w (x - mean) rstd + b, or z act(gate) where gate is given.
+ * act: 0 none, 1 silu, 2 sigmoid.  w and b (C; NULL: ones, zeros) float32 or of x's type.
+ * stats: (N, G, 2) floats (mean, rstd) that the forward call writes and the backward call reads;
+ * not used (may be NULL) where L = 1 and a group is at most 256 accesses of 16 bytes (4 or 2
+ * bytes where alignment or an odd width allows no more).  The backward call's alignment of x,
+ * gate, gy, dx and dgate may differ from the forward call's only if stats is given. */
+PRNN_API size_t prnn_group_norm_workspace_size(int N, int L, int C, int G, int dtype,
+                                               int backward);
+PRNN_API int prnn_group_norm(const void* x, const void* w, const void* b, const void* gate,
+                             void* y, float* stats, int N, int L, int C, int G, float eps, int act,
+                             int w_dtype, int dtype, void* workspace, size_t workspace_bytes,
+                             void* stream);
+PRNN_API int prnn_group_norm_backward(const void* gy, const void* x, const void* w, const void* b,
+                                      const void* gate, const float* stats, void* dx, void* dw,
+                                      void* db, void* dgate, int N, int L, int C, int G, float eps,
+                                      int act, int w_dtype, int dtype, void* workspace,
+                                      size_t workspace_bytes, void* stream);
+
+/* ---- Pages of a state cache ------------------------------------------------
+ * A cache is one or several pools whose rows 0 .. slots - 1 belong together (a slot), and used
+ * (slots) int32: 0 = free.  Lists are int32 on the device; entries outside 0 .. slots - 1 are
+ * passed over.  Everything stays on the device: nothing waits for the host. */
+typedef struct prnn_pool {
+  void* p;
+  long long row_bytes;
+} prnn_pool;
+
+/* out[i] for i < n: the i-th lowest free slot, now used; -1 where none is left. */
+PRNN_API int prnn_pages_take(int* used, int slots, int* out, int n, void* stream);
+/* out[i]: a free slot (lowest first), now used, with a copy of slot parents[i] in every pool; -1
+ * where the parent is none or no slot is left.  scratch: n ints. */
+PRNN_API int prnn_pages_fork(int* used, int slots, const prnn_pool* pools, int n_pools,
+                             const int* parents, int* out, int n, int* scratch, void* stream);
+PRNN_API int prnn_pages_free(int* used, int slots, const int* list, int n, void* stream);
+/* Slot dst[i] of every pool gets slot src[i]; no dst may be another entry's src or dst. */
+PRNN_API int prnn_pages_copy(int slots, const prnn_pool* pools, int n_pools, const int* src,
+                             const int* dst, int n, void* stream);
+/* The live slots move into the lowest ones: the i-th lowest free slot below their number gets the
+ * i-th lowest live one above it.  tables[k] (lens[k] entries, in place): live slots become their
+ * new places, free ones -1.  live: their number (one int).  scratch: 2 slots + 1 ints. */
+PRNN_API int prnn_pages_compact(int* used, int slots, const prnn_pool* pools, int n_pools,
+                                int* const* tables, const int* lens, int n_tables, int* live,
+                                int* scratch, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

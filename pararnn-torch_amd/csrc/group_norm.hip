@@ -1,0 +1,933 @@
+// Group norm, channels last, with an activation or a gate:
+//
+//   h = (x - mean) rstd,  z = w h + b,   y = act(z)   or   y = z act(gate)
+//
+// with mean and rstd = (var + eps)^(-1/2) over a group of channels of one token, or over all
+// tokens of a sample.  Backward, with dz = dy act'(z) (gate: dy act(gate)), dh = w dz and the
+// means m1 = <dh>, m2 = <dh h> over the same elements:
+//
+//   dx = rstd (dh - m1 - h m2),  dw = sum dz h,  db = sum dz,  dgate = dy z act'(gate).
+//
+// Bound by memory: a token's group sits in a few lanes' registers, so the statistics, the
+// normalisation and in the backward pass all sums over the group come from one read of the
+// arrays.  The parameters' sums are kept per thread (a thread's channels stay the same from row
+// to row), then per workgroup, and are added up in a fixed order by a second kernel.
+//
+// Statistics and sums are fp32: two passes over registers for a token, running means and squared
+// deviations (joined by their exact combination rule) for a sample.
+#include <algorithm>
+
+#include "prnn_host.h"
+
+namespace prnn {
+namespace {
+
+enum { kActNone = 0, kActSilu = 1, kActSigmoid = 2 };
+
+struct NormArgs {
+  const void *x, *w, *b, *gate, *gy;
+  void *y, *dx, *dgate;
+  float* stats;      // (N, G) mean, rstd of samples
+  float* part;       // partial sums, see the kernels
+  float* part2;
+  size_t rows;       // tokens (token kernels)
+  int N, L, C, G, Cg;
+  int act, w_f32;    // w and b are float32
+  int lanes;         // lanes of a group: a power of two
+  int strips, strip_rows;
+  float eps;
+};
+
+__device__ __forceinline__ float act_of(int act, float z) {
+  if (act == kActNone) return z;
+  const float s = fsigmoid(z);
+  return act == kActSilu ? z * s : s;
+}
+// act(z) and act'(z)
+__device__ __forceinline__ void act_grad(int act, float z, float& f, float& d) {
+  if (act == kActNone) {
+    f = z;
+    d = 1.0f;
+    return;
+  }
+  const float s = fsigmoid(z);
+  // 1 - s as a sigmoid of its own: no cancellation for large z
+  const float c = fsigmoid(-z);
+  if (act == kActSilu) {
+    f = z * s;
+    d = s * fmaf(z, c, 1.0f);
+  } else {
+    f = s;
+    d = s * c;
+  }
+}
+
+// V consecutive elements (V * sizeof(T) bytes, aligned) as floats.
+template <typename T, int V>
+__device__ __forceinline__ void loadv(const T* p, float* v) {
+  if constexpr (V == 1) {
+    v[0] = to_f32(*p);
+  } else if constexpr (sizeof(T) == 4) {
+    typedef float f4 __attribute__((ext_vector_type(4)));
+    static_assert(V == 4, "");
+    const f4 q = *reinterpret_cast<const f4*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = q[i];
+  } else if constexpr (V == 2) {
+    const uint32_t q = *reinterpret_cast<const uint32_t*>(p);
+    v[0] = Narrow<T>::lo(q);
+    v[1] = Narrow<T>::hi(q);
+  } else {
+    static_assert(V == 8, "");
+    const uint4 q = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = Narrow<T>::lo(w[i]);
+      v[2 * i + 1] = Narrow<T>::hi(w[i]);
+    }
+  }
+}
+template <typename T, int V>
+__device__ __forceinline__ void storev(T* p, const float* v) {
+  if constexpr (V == 1) {
+    *p = from_f32<T>(v[0]);
+  } else if constexpr (sizeof(T) == 4) {
+    typedef float f4 __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<f4*>(p) = f4{v[0], v[1], v[2], v[3]};
+  } else if constexpr (V == 2) {
+    *reinterpret_cast<uint32_t*>(p) = Narrow<T>::pack(v[0], v[1]);
+  } else {
+    *reinterpret_cast<uint4*>(p) = uint4{Narrow<T>::pack(v[0], v[1]), Narrow<T>::pack(v[2], v[3]),
+                                         Narrow<T>::pack(v[4], v[5]), Narrow<T>::pack(v[6], v[7])};
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ float param(const void* p, int f32, int c, float none) {
+  if (p == nullptr) return none;
+  return f32 ? static_cast<const float*>(p)[c] : to_f32(static_cast<const T*>(p)[c]);
+}
+
+// Sum over the `lanes` lanes of a group (a power of two; every lane gets it).
+__device__ __forceinline__ float group_sum(float v, int lanes) {
+  for (int k = 1; k < lanes; k <<= 1) v += __shfl_xor(v, k);
+  return v;
+}
+
+// ---- statistics per token ----------------------------------------------------------------
+// Lanes are laid over a row's groups, `lanes` to a group, K vectors of V channels to a lane
+// (vector k of lane l: channels (k lanes + l) V); lanes behind a group's end idle.  Where a row
+// takes fewer than 256 lanes a workgroup works on several rows at a time.
+
+struct TokenPlace {
+  int row, rows_per, group, l;
+  bool on;
+};
+__device__ __forceinline__ TokenPlace token_place(const NormArgs& A) {
+  const int per_row = A.G * A.lanes;
+  TokenPlace p;
+  int u;
+  if (per_row <= 256) {
+    p.rows_per = 256 / per_row;
+    p.row = threadIdx.x / per_row;
+    u = threadIdx.x - p.row * per_row;
+    p.on = p.row < p.rows_per;
+  } else {
+    p.rows_per = 1;
+    p.row = 0;
+    u = blockIdx.y * 256 + threadIdx.x;
+    p.on = u < per_row;
+  }
+  p.group = u / A.lanes;
+  p.l = u - p.group * A.lanes;
+  return p;
+}
+
+template <typename T, int V, int K>
+__global__ __launch_bounds__(256) void norm_token_kernel(NormArgs A) {
+  const TokenPlace p = token_place(A);
+  const float inv = 1.0f / A.Cg;
+  float w[K][V], b[K][V];
+  bool in[K];
+  int ch[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = (k * A.lanes + p.l) * V;
+    in[k] = p.on && c < A.Cg;
+    ch[k] = in[k] ? p.group * A.Cg + c : 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      w[k][i] = in[k] ? param<T>(A.w, A.w_f32, ch[k] + i, 1.0f) : 0.0f;
+      b[k][i] = in[k] ? param<T>(A.b, A.w_f32, ch[k] + i, 0.0f) : 0.0f;
+    }
+  }
+  // all lanes of a wave stay in the loop: the sums are shuffles
+  for (size_t r0 = static_cast<size_t>(blockIdx.x) * p.rows_per; r0 < A.rows;
+       r0 += static_cast<size_t>(gridDim.x) * p.rows_per) {
+    const size_t row = r0 + p.row;
+    const bool live = p.on && row < A.rows;
+    const size_t at = row * A.C;
+    float x[K][V], g[K][V], s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const bool go = live && in[k];
+      if (go) {
+        loadv<T, V>(static_cast<const T*>(A.x) + at + ch[k], x[k]);
+        if (A.gate) loadv<T, V>(static_cast<const T*>(A.gate) + at + ch[k], g[k]);
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if (!go) x[k][i] = g[k][i] = 0.0f;
+        s += x[k][i];
+      }
+    }
+    const float mean = group_sum(s, A.lanes) * inv;
+    s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float d = in[k] ? x[k][i] - mean : 0.0f;
+        s = fmaf(d, d, s);
+      }
+    const float rstd = 1.0f / sqrtf(fmaf(group_sum(s, A.lanes), inv, A.eps));
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (!(live && in[k])) continue;
+      float y[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float z = fmaf(w[k][i], (x[k][i] - mean) * rstd, b[k][i]);
+        y[i] = A.gate ? z * act_of(A.act, g[k][i]) : act_of(A.act, z);
+      }
+      storev<T, V>(static_cast<T*>(A.y) + at + ch[k], y);
+    }
+  }
+}
+
+// part: [gridDim.x][2][C] sums of dz h and dz.
+template <typename T, int V, int K>
+__global__ __launch_bounds__(256) void norm_token_bwd_kernel(NormArgs A) {
+  __shared__ float red[256];
+  const TokenPlace p = token_place(A);
+  const float inv = 1.0f / A.Cg;
+  float w[K][V], b[K][V], dw[K][V], db[K][V];
+  bool in[K];
+  int ch[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = (k * A.lanes + p.l) * V;
+    in[k] = p.on && c < A.Cg;
+    ch[k] = in[k] ? p.group * A.Cg + c : 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      w[k][i] = in[k] ? param<T>(A.w, A.w_f32, ch[k] + i, 1.0f) : 0.0f;
+      b[k][i] = in[k] ? param<T>(A.b, A.w_f32, ch[k] + i, 0.0f) : 0.0f;
+      dw[k][i] = db[k][i] = 0.0f;
+    }
+  }
+  for (size_t r0 = static_cast<size_t>(blockIdx.x) * p.rows_per; r0 < A.rows;
+       r0 += static_cast<size_t>(gridDim.x) * p.rows_per) {
+    const size_t row = r0 + p.row;
+    const bool live = p.on && row < A.rows;
+    const size_t at = row * A.C;
+    float x[K][V], g[K][V], dz[K][V], s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const bool go = live && in[k];
+      if (go) {
+        loadv<T, V>(static_cast<const T*>(A.x) + at + ch[k], x[k]);
+        loadv<T, V>(static_cast<const T*>(A.gy) + at + ch[k], dz[k]);
+        if (A.gate) loadv<T, V>(static_cast<const T*>(A.gate) + at + ch[k], g[k]);
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if (!go) x[k][i] = g[k][i] = dz[k][i] = 0.0f;
+        s += x[k][i];
+      }
+    }
+    const float mean = group_sum(s, A.lanes) * inv;
+    s = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float d = in[k] ? x[k][i] - mean : 0.0f;
+        s = fmaf(d, d, s);
+      }
+    const float rstd = 1.0f / sqrtf(fmaf(group_sum(s, A.lanes), inv, A.eps));
+    float m1 = 0.0f, m2 = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const bool go = live && in[k];
+      float dg[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float h = go ? (x[k][i] - mean) * rstd : 0.0f;
+        const float z = fmaf(w[k][i], h, b[k][i]);
+        float f, d;
+        act_grad(A.act, A.gate ? g[k][i] : z, f, d);
+        if (A.gate) {
+          dg[i] = dz[k][i] * z * d;
+          dz[k][i] *= f;
+        } else {
+          dz[k][i] *= d;
+        }
+        x[k][i] = h;
+        if (go) {  // an idle lane adds nothing, whatever act gives there
+          dw[k][i] = fmaf(dz[k][i], h, dw[k][i]);
+          db[k][i] += dz[k][i];
+          const float dh = w[k][i] * dz[k][i];
+          m1 += dh;
+          m2 = fmaf(dh, h, m2);
+        }
+      }
+      if (go && A.gate) storev<T, V>(static_cast<T*>(A.dgate) + at + ch[k], dg);
+    }
+    m1 = group_sum(m1, A.lanes) * inv;
+    m2 = group_sum(m2, A.lanes) * inv;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      if (!(live && in[k])) continue;
+      float dx[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        dx[i] = rstd * (fmaf(w[k][i], dz[k][i], -m1) - x[k][i] * m2);
+      storev<T, V>(static_cast<T*>(A.dx) + at + ch[k], dx);
+    }
+  }
+  // the workgroup's rows, in their order
+  const int per_row = A.G * A.lanes;
+  float* out = A.part + static_cast<size_t>(blockIdx.x) * 2 * A.C;
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        const float mine = which ? db[k][i] : dw[k][i];
+        float sum = mine;
+        if (p.rows_per > 1) {
+          __syncthreads();
+          red[threadIdx.x] = mine;
+          __syncthreads();
+          if (p.row == 0)
+            for (int r = 1; r < p.rows_per; ++r) sum += red[r * per_row + threadIdx.x];
+        }
+        if (p.row == 0 && in[k]) out[which * A.C + ch[k] + i] = sum;
+      }
+}
+
+// dw and db from partial sums [parts][2][C]: 32 channels a workgroup, 8 lanes to a channel.
+template <typename T>
+__global__ __launch_bounds__(256) void norm_param_kernel(const float* __restrict__ part, int parts,
+                                                         int C, void* dw, void* db, int f32) {
+  __shared__ float red[8][33];
+  const int c0 = blockIdx.x * 32, c = c0 + threadIdx.x % 32, sub = threadIdx.x / 32;
+  const int which = blockIdx.y;
+  float s = 0.0f;
+  if (c < C)
+    for (int p = sub; p < parts; p += 8) s += part[(static_cast<size_t>(p) * 2 + which) * C + c];
+  red[sub][threadIdx.x % 32] = s;
+  __syncthreads();
+  void* out = which ? db : dw;
+  if (sub == 0 && c < C && out) {
+    for (int k = 1; k < 8; ++k) s += red[k][threadIdx.x];
+    if (f32)
+      static_cast<float*>(out)[c] = s;
+    else
+      static_cast<T*>(out)[c] = from_f32<T>(s);
+  }
+}
+
+// ---- statistics per sample ---------------------------------------------------------------
+// A sample (L tokens) is cut into strips of rows, one workgroup each.  Threads lie over the
+// channels, V to a thread, and over as many rows at a time as fit.
+
+struct SamplePlace {
+  int slots, rows_per, row, slot;
+  bool on;
+};
+template <int V>
+__device__ __forceinline__ SamplePlace sample_place(const NormArgs& A) {
+  SamplePlace p;
+  p.slots = A.C / V;
+  if (p.slots <= 256) {
+    p.rows_per = 256 / p.slots;
+    p.row = threadIdx.x / p.slots;
+    p.slot = threadIdx.x - p.row * p.slots;
+    p.on = p.row < p.rows_per;
+  } else {
+    p.rows_per = 1;
+    p.row = 0;
+    p.slot = threadIdx.x;
+    p.on = true;
+  }
+  return p;
+}
+
+// Sum over a workgroup of 256 (every thread gets it).
+__device__ __forceinline__ float block_sum(float v, float* red) {
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) v += __shfl_xor(v, k);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return red[0] + red[1] + red[2] + red[3];
+}
+
+// Statistics of strip `strip` of sample n, one group after another of those in the workgroup's
+// share: mean and squared deviations per thread and channel, then joined per group.
+// part: [N][strips][G][2].
+template <typename T, int V>
+__global__ __launch_bounds__(256) void norm_sample_stats_kernel(NormArgs A) {
+  extern __shared__ float lds[];  // [256][2 V] mean and squared deviations per thread
+  const int n = blockIdx.x / A.strips, strip = blockIdx.x - n * A.strips;
+  const SamplePlace p = sample_place<V>(A);
+  const int l0 = strip * A.strip_rows, l1 = min(A.L, l0 + A.strip_rows);
+  const T* x = static_cast<const T*>(A.x) + static_cast<size_t>(n) * A.L * A.C;
+  float* out = A.part + (static_cast<size_t>(n) * A.strips + strip) * A.G * 2;
+  // slots beyond 256 in rounds, a whole number of groups each
+  const int per_group = A.Cg / V;
+  const int groups_round = p.slots <= 256 ? A.G : max(1, 256 / per_group);
+  for (int g0 = 0; g0 < A.G; g0 += groups_round) {
+    const int gn = min(groups_round, A.G - g0);
+    if (p.slots > 256 && per_group > 256) {
+      // a group wider than the workgroup: its channels in turns, two passes over the strip
+      const size_t c0 = static_cast<size_t>(g0) * A.Cg;
+      float s = 0.0f;
+      for (int l = l0; l < l1; ++l)
+        for (int u = threadIdx.x; u < per_group; u += 256) {
+          float v[V];
+          loadv<T, V>(x + static_cast<size_t>(l) * A.C + c0 + u * V, v);
+#pragma unroll
+          for (int i = 0; i < V; ++i) s += v[i];
+        }
+      const float cnt = static_cast<float>(l1 - l0) * A.Cg;
+      const float mean = block_sum(s, lds) / cnt;
+      s = 0.0f;
+      for (int l = l0; l < l1; ++l)
+        for (int u = threadIdx.x; u < per_group; u += 256) {
+          float v[V];
+          loadv<T, V>(x + static_cast<size_t>(l) * A.C + c0 + u * V, v);
+#pragma unroll
+          for (int i = 0; i < V; ++i) s = fmaf(v[i] - mean, v[i] - mean, s);
+        }
+      s = block_sum(s, lds);
+      if (threadIdx.x == 0) {
+        out[2 * g0] = mean;
+        out[2 * g0 + 1] = s;
+      }
+      __syncthreads();
+      continue;
+    }
+    const int slot = p.slots <= 256 ? p.slot : g0 * per_group + threadIdx.x;
+    const bool on = p.slots <= 256 ? p.on : threadIdx.x < static_cast<unsigned>(gn * per_group);
+    float mean[V], m2[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) mean[i] = m2[i] = 0.0f;
+    float cnt = 0.0f;
+    if (on)
+      for (int l = l0 + p.row; l < l1; l += p.rows_per) {
+        float v[V];
+        loadv<T, V>(x + static_cast<size_t>(l) * A.C + slot * V, v);
+        cnt += 1.0f;
+        const float inv = frcp(cnt);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float d = v[i] - mean[i];
+          mean[i] = fmaf(d, inv, mean[i]);
+          m2[i] = fmaf(d, v[i] - mean[i], m2[i]);
+        }
+      }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      lds[threadIdx.x * 2 * V + 2 * i] = mean[i];
+      lds[threadIdx.x * 2 * V + 2 * i + 1] = m2[i];
+    }
+    __syncthreads();
+    // one wave per group: the mean of the means, then the deviations from it
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int g = wave; g < gn; g += 4) {
+      const int items = per_group * p.rows_per;
+      float s = 0.0f;
+      const float total = static_cast<float>(l1 - l0) * A.Cg;
+      for (int it = lane; it < items; it += 64) {
+        const int r = it / per_group, u = g * per_group + it - r * per_group;
+        const float c = static_cast<float>((l1 - l0 - r + p.rows_per - 1) / p.rows_per);
+        const float* e = &lds[(r * (p.slots <= 256 ? p.slots : 0) + u) * 2 * V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) s = fmaf(c, e[2 * i], s);
+      }
+#pragma unroll
+      for (int k = 1; k < 64; k <<= 1) s += __shfl_xor(s, k);
+      const float gm = s / total;
+      s = 0.0f;
+      for (int it = lane; it < items; it += 64) {
+        const int r = it / per_group, u = g * per_group + it - r * per_group;
+        const float c = static_cast<float>((l1 - l0 - r + p.rows_per - 1) / p.rows_per);
+        const float* e = &lds[(r * (p.slots <= 256 ? p.slots : 0) + u) * 2 * V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float d = e[2 * i] - gm;
+          s += fmaf(c * d, d, e[2 * i + 1]);
+        }
+      }
+#pragma unroll
+      for (int k = 1; k < 64; k <<= 1) s += __shfl_xor(s, k);
+      if (lane == 0) {
+        out[2 * (g0 + g)] = gm;
+        out[2 * (g0 + g) + 1] = s;
+      }
+    }
+  }
+}
+
+// Mean and rstd per (sample, group) from the strips.
+__global__ __launch_bounds__(256) void norm_sample_join_kernel(NormArgs A) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const long long id = static_cast<long long>(blockIdx.x) * 4 + wave;
+  if (id >= static_cast<long long>(A.N) * A.G) return;
+  const int n = static_cast<int>(id / A.G), g = static_cast<int>(id - static_cast<long long>(n) * A.G);
+  const float* e = A.part + static_cast<size_t>(n) * A.strips * A.G * 2 + 2 * g;
+  double s = 0.0;
+  for (int k = lane; k < A.strips; k += 64) {
+    const double c = min(A.strip_rows, A.L - k * A.strip_rows);
+    s += c * e[static_cast<size_t>(k) * A.G * 2];
+  }
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) s += __shfl_xor(s, k);
+  const double mean = s / A.L;
+  s = 0.0;
+  for (int k = lane; k < A.strips; k += 64) {
+    const double c = static_cast<double>(min(A.strip_rows, A.L - k * A.strip_rows)) * A.Cg;
+    const double d = e[static_cast<size_t>(k) * A.G * 2] - mean;
+    s += e[static_cast<size_t>(k) * A.G * 2 + 1] + c * d * d;
+  }
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) s += __shfl_xor(s, k);
+  if (lane == 0) {
+    const double var = s / (static_cast<double>(A.L) * A.Cg);
+    A.stats[2 * id] = static_cast<float>(mean);
+    A.stats[2 * id + 1] = static_cast<float>(1.0 / sqrt(var + A.eps));
+  }
+}
+
+// y of a strip.
+template <typename T, int V>
+__global__ __launch_bounds__(256) void norm_sample_apply_kernel(NormArgs A) {
+  const int n = blockIdx.x / A.strips, strip = blockIdx.x - n * A.strips;
+  const SamplePlace p = sample_place<V>(A);
+  const int l0 = strip * A.strip_rows, l1 = min(A.L, l0 + A.strip_rows);
+  const size_t base = static_cast<size_t>(n) * A.L * A.C;
+  if (!p.on) return;
+  for (int slot = p.slot; slot < p.slots; slot += 256) {
+    const int c = slot * V, g = c / A.Cg;
+    const float mean = A.stats[2 * (static_cast<size_t>(n) * A.G + g)];
+    const float rstd = A.stats[2 * (static_cast<size_t>(n) * A.G + g) + 1];
+    float w[V], b[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      w[i] = param<T>(A.w, A.w_f32, c + i, 1.0f);
+      b[i] = param<T>(A.b, A.w_f32, c + i, 0.0f);
+    }
+    for (int l = l0 + p.row; l < l1; l += p.rows_per) {
+      const size_t at = base + static_cast<size_t>(l) * A.C + c;
+      float x[V], gt[V], y[V];
+      loadv<T, V>(static_cast<const T*>(A.x) + at, x);
+      if (A.gate) loadv<T, V>(static_cast<const T*>(A.gate) + at, gt);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float z = fmaf(w[i], (x[i] - mean) * rstd, b[i]);
+        y[i] = A.gate ? z * act_of(A.act, gt[i]) : act_of(A.act, z);
+      }
+      storev<T, V>(static_cast<T*>(A.y) + at, y);
+    }
+    if (p.slots <= 256) break;
+  }
+}
+
+// Sums of dz h and dz of a strip per channel: part [N * strips][2][C]; dgate on the way.
+template <typename T, int V>
+__global__ __launch_bounds__(256) void norm_sample_bwd_sums_kernel(NormArgs A) {
+  __shared__ float red[256];
+  const int n = blockIdx.x / A.strips, strip = blockIdx.x - n * A.strips;
+  const SamplePlace p = sample_place<V>(A);
+  const int l0 = strip * A.strip_rows, l1 = min(A.L, l0 + A.strip_rows);
+  const size_t base = static_cast<size_t>(n) * A.L * A.C;
+  float* out = A.part + (static_cast<size_t>(n) * A.strips + strip) * 2 * A.C;
+  for (int s0 = 0; s0 < p.slots; s0 += 256) {
+    const int slot = p.slot + s0;
+    const bool on = p.on && slot < p.slots;
+    const int c = on ? slot * V : 0, g = c / A.Cg;
+    const float mean = A.stats[2 * (static_cast<size_t>(n) * A.G + g)];
+    const float rstd = A.stats[2 * (static_cast<size_t>(n) * A.G + g) + 1];
+    float w[V], b[V], dw[V], db[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      w[i] = param<T>(A.w, A.w_f32, c + i, 1.0f);
+      b[i] = param<T>(A.b, A.w_f32, c + i, 0.0f);
+      dw[i] = db[i] = 0.0f;
+    }
+    if (on)
+      for (int l = l0 + p.row; l < l1; l += p.rows_per) {
+        const size_t at = base + static_cast<size_t>(l) * A.C + c;
+        float x[V], gt[V], dz[V];
+        loadv<T, V>(static_cast<const T*>(A.x) + at, x);
+        loadv<T, V>(static_cast<const T*>(A.gy) + at, dz);
+        if (A.gate) loadv<T, V>(static_cast<const T*>(A.gate) + at, gt);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float h = (x[i] - mean) * rstd, z = fmaf(w[i], h, b[i]);
+          float f, d;
+          act_grad(A.act, A.gate ? gt[i] : z, f, d);
+          if (A.gate) {
+            gt[i] = dz[i] * z * d;
+            dz[i] *= f;
+          } else {
+            dz[i] *= d;
+          }
+          dw[i] = fmaf(dz[i], h, dw[i]);
+          db[i] += dz[i];
+        }
+        if (A.gate) storev<T, V>(static_cast<T*>(A.dgate) + at, gt);
+      }
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        const float mine = which ? db[i] : dw[i];
+        float sum = mine;
+        if (p.rows_per > 1) {
+          __syncthreads();
+          red[threadIdx.x] = mine;
+          __syncthreads();
+          if (p.row == 0)
+            for (int r = 1; r < p.rows_per; ++r) sum += red[r * p.slots + threadIdx.x];
+        }
+        if (p.row == 0 && on) out[which * A.C + c + i] = sum;
+      }
+  }
+}
+
+// m1 and m2 per (sample, group): part2 [N][G][2], one wave each.
+template <typename T>
+__global__ __launch_bounds__(256) void norm_sample_means_kernel(NormArgs A) {
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const long long id = static_cast<long long>(blockIdx.x) * 4 + wave;
+  if (id >= static_cast<long long>(A.N) * A.G) return;
+  const int n = static_cast<int>(id / A.G), g = static_cast<int>(id - static_cast<long long>(n) * A.G);
+  const float* e = A.part + static_cast<size_t>(n) * A.strips * 2 * A.C + g * A.Cg;
+  double m1 = 0.0, m2 = 0.0;
+  const long long items = static_cast<long long>(A.strips) * A.Cg;
+  for (long long it = lane; it < items; it += 64) {
+    const int k = static_cast<int>(it / A.Cg), c = static_cast<int>(it - static_cast<long long>(k) * A.Cg);
+    const float w = param<T>(A.w, A.w_f32, g * A.Cg + c, 1.0f);
+    m2 += static_cast<double>(w) * e[static_cast<size_t>(k) * 2 * A.C + c];
+    m1 += static_cast<double>(w) * e[static_cast<size_t>(k) * 2 * A.C + A.C + c];
+  }
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) {
+    m1 += __shfl_xor(m1, k);
+    m2 += __shfl_xor(m2, k);
+  }
+  if (lane == 0) {
+    const double inv = 1.0 / (static_cast<double>(A.L) * A.Cg);
+    A.part2[2 * id] = static_cast<float>(m1 * inv);
+    A.part2[2 * id + 1] = static_cast<float>(m2 * inv);
+  }
+}
+
+template <typename T, int V>
+__global__ __launch_bounds__(256) void norm_sample_dx_kernel(NormArgs A) {
+  const int n = blockIdx.x / A.strips, strip = blockIdx.x - n * A.strips;
+  const SamplePlace p = sample_place<V>(A);
+  const int l0 = strip * A.strip_rows, l1 = min(A.L, l0 + A.strip_rows);
+  const size_t base = static_cast<size_t>(n) * A.L * A.C;
+  if (!p.on) return;
+  for (int slot = p.slot; slot < p.slots; slot += 256) {
+    const int c = slot * V, g = c / A.Cg;
+    const size_t ng = static_cast<size_t>(n) * A.G + g;
+    const float mean = A.stats[2 * ng], rstd = A.stats[2 * ng + 1];
+    const float m1 = A.part2[2 * ng], m2 = A.part2[2 * ng + 1];
+    float w[V], b[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      w[i] = param<T>(A.w, A.w_f32, c + i, 1.0f);
+      b[i] = param<T>(A.b, A.w_f32, c + i, 0.0f);
+    }
+    for (int l = l0 + p.row; l < l1; l += p.rows_per) {
+      const size_t at = base + static_cast<size_t>(l) * A.C + c;
+      float x[V], gt[V], dz[V];
+      loadv<T, V>(static_cast<const T*>(A.x) + at, x);
+      loadv<T, V>(static_cast<const T*>(A.gy) + at, dz);
+      if (A.gate) loadv<T, V>(static_cast<const T*>(A.gate) + at, gt);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float h = (x[i] - mean) * rstd, z = fmaf(w[i], h, b[i]);
+        if (A.gate) {
+          dz[i] *= act_of(A.act, gt[i]);
+        } else {
+          float f, d;
+          act_grad(A.act, z, f, d);
+          dz[i] *= d;
+        }
+        x[i] = rstd * (fmaf(w[i], dz[i], -m1) - h * m2);
+      }
+      storev<T, V>(static_cast<T*>(A.dx) + at, x);
+    }
+    if (p.slots <= 256) break;
+  }
+}
+
+// ---- host ----------------------------------------------------------------------------------
+
+struct Plan {
+  bool token;
+  int V, K, lanes;       // token kernels
+  int blocks_x, blocks_y;
+  int strips, strip_rows;
+};
+
+// Elements of a 16-byte access; 2 where 16-bit channels come in pairs only; else 1.
+int vector_of(int dtype, int Cg, uintptr_t bits) {
+  const int size = dtype == PRNN_F32 ? 4 : 2;
+  const int v = 16 / size;
+  if (Cg % v == 0 && (bits & 15) == 0) return v;
+  if (size == 2 && Cg % 2 == 0 && (bits & 3) == 0) return 2;
+  return 1;
+}
+
+Plan plan(int N, int L, int Cg, int G, int dtype, uintptr_t bits, bool backward) {
+  Plan p{};
+  p.V = vector_of(dtype, Cg, bits);
+  // A token's group in one wave's registers: up to 64 lanes, 4 vectors each.
+  if (L == 1 && Cg <= 256 * p.V) {
+    p.token = true;
+    const int vecs = (Cg + p.V - 1) / p.V;
+    p.K = vecs <= 64 ? 1 : 4;
+    p.lanes = 1;
+    while (p.lanes * p.K < vecs) p.lanes <<= 1;
+    const int per_row = G * p.lanes;
+    const int rows_per = per_row <= 256 ? 256 / per_row : 1;
+    p.blocks_y = (per_row + 255) / 256;
+    const int need = (N + rows_per - 1) / rows_per;
+    // The backward pass keeps the parameters' sums per workgroup: about four workgroups a CU
+    // share the rows; the forward pass has nothing to keep.
+    const int most = backward ? std::max(1, 1024 / p.blocks_y) : 16384;
+    p.blocks_x = std::max(1, std::min(need, most));
+    return p;
+  }
+  // strips: enough workgroups for the chip, at least 8 rounds of rows each
+  const int slots = G * Cg / p.V, rows_per = slots <= 256 ? 256 / slots : 1;
+  const int want = std::max(1, 1024 / std::max(1, N));
+  p.strip_rows = std::max((L + want - 1) / want, 8 * rows_per);
+  p.strips = (L + p.strip_rows - 1) / p.strip_rows;
+  return p;
+}
+
+template <typename F>
+int with_vector(int V, F&& f) {
+  if (V == 8) return f(std::integral_constant<int, 8>{});
+  if (V == 4) return f(std::integral_constant<int, 4>{});
+  if (V == 2) return f(std::integral_constant<int, 2>{});
+  return f(std::integral_constant<int, 1>{});
+}
+
+// f(T, V) for the vectors that exist: 16 bytes, a pair of 16-bit elements, one element.
+template <typename F>
+int with_types(int dtype, int V, F&& f) {
+  return with_storage(dtype, [&](auto z) {
+    using T = decltype(z);
+    return with_vector(V, [&](auto v) -> int {
+      constexpr int n = decltype(v)::value;
+      if constexpr (n == 1 || (sizeof(T) == 4 ? n == 4 : n == 8 || n == 2))
+        return f(z, v);
+      else
+        return fail(PRNN_ERR_RUNTIME, "no vector of %d elements", n);
+    });
+  });
+}
+
+int check(const char* what, int N, int L, int C, int G, int act, int w_dtype, int dtype) {
+  if (int rc = check_dtype(dtype)) return rc;
+  if (w_dtype != PRNN_F32 && w_dtype != dtype)
+    return fail(PRNN_ERR_TYPE, "%s: weight and bias must be float32 or of x's type", what);
+  if (N < 0 || L < 0 || C < 1 || G < 1 || C % G)
+    return fail(PRNN_ERR_VALUE, "%s: N=%d, L=%d, C=%d, groups=%d", what, N, L, C, G);
+  if (act < 0 || act > 2) return fail(PRNN_ERR_VALUE, "%s: activation code %d", what, act);
+  return PRNN_OK;
+}
+
+uintptr_t bits_of(std::initializer_list<const void*> ps) {
+  uintptr_t b = 0;
+  for (const void* p : ps) b |= reinterpret_cast<uintptr_t>(p);
+  return b;
+}
+
+}  // namespace
+}  // namespace prnn
+
+using namespace prnn;
+
+extern "C" PRNN_API size_t prnn_group_norm_workspace_size(int N, int L, int C, int G, int dtype,
+                                                          int backward) {
+  if (N < 1 || L < 1 || C < 1 || G < 1 || C % G) return 0;
+  // the largest over the alignments that a call may turn out to have
+  size_t most = 0;
+  for (uintptr_t bits : {uintptr_t{0}, uintptr_t{4}, uintptr_t{2}}) {
+    const Plan p = plan(N, L, C / G, G, dtype, bits, backward != 0);
+    Carver c(nullptr);
+    if (p.token) {
+      if (backward) c.take(sizeof(float) * 2 * C * p.blocks_x);
+    } else if (!backward) {
+      c.take(sizeof(float) * 2 * G * p.strips * static_cast<size_t>(N));
+    } else {
+      c.take(sizeof(float) * 2 * C * p.strips * static_cast<size_t>(N));
+      c.take(sizeof(float) * 2 * G * static_cast<size_t>(N));
+    }
+    most = std::max(most, c.used);
+  }
+  return most;
+}
+
+extern "C" PRNN_API int prnn_group_norm(const void* x, const void* w, const void* b,
+                                        const void* gate, void* y, float* stats, int N, int L,
+                                        int C, int G, float eps, int act, int w_dtype, int dtype,
+                                        void* workspace, size_t bytes, void* stream) {
+  if (int rc = check("group_norm", N, L, C, G, act, w_dtype, dtype)) return rc;
+  if (N == 0 || L == 0) return PRNN_OK;
+  if (!x || !y) return fail(PRNN_ERR_VALUE, "group_norm: x and y must be non-null");
+  const Plan p = plan(N, L, C / G, G, dtype, bits_of({x, y, gate}), false);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  NormArgs a{};
+  a.x = x;
+  a.w = w;
+  a.b = b;
+  a.gate = gate;
+  a.y = y;
+  a.stats = stats;
+  a.rows = N;
+  a.N = N;
+  a.L = L;
+  a.C = C;
+  a.G = G;
+  a.Cg = C / G;
+  a.act = act;
+  a.w_f32 = w_dtype == PRNN_F32;
+  a.lanes = p.lanes;
+  a.strips = p.strips;
+  a.strip_rows = p.strip_rows;
+  a.eps = eps;
+  if (p.token)
+    return with_types(dtype, p.V, [&](auto z, auto v) {
+      using T = decltype(z);
+      constexpr int V = decltype(v)::value;
+      const dim3 grid(p.blocks_x, p.blocks_y);
+      if (p.K == 1)
+        norm_token_kernel<T, V, 1><<<grid, 256, 0, st>>>(a);
+      else
+        norm_token_kernel<T, V, 4><<<grid, 256, 0, st>>>(a);
+      PRNN_HIP(hipGetLastError());
+      return static_cast<int>(PRNN_OK);
+    });
+  if (!stats) return fail(PRNN_ERR_VALUE, "group_norm: statistics per sample need stats");
+  const size_t need = sizeof(float) * 2 * G * p.strips * static_cast<size_t>(N);
+  if (!workspace || bytes < need)
+    return fail(PRNN_ERR_VALUE, "group_norm: the workspace must hold %zu bytes", need);
+  a.part = static_cast<float*>(workspace);
+  return with_types(dtype, p.V, [&](auto z, auto v) {
+    using T = decltype(z);
+    constexpr int V = decltype(v)::value;
+    const dim3 grid(static_cast<unsigned>(p.strips) * N);
+    norm_sample_stats_kernel<T, V><<<grid, 256, 256 * 2 * V * sizeof(float), st>>>(a);
+    PRNN_HIP(hipGetLastError());
+    const unsigned joins = static_cast<unsigned>((1ll * N * G + 3) / 4);
+    norm_sample_join_kernel<<<joins, 256, 0, st>>>(a);
+    PRNN_HIP(hipGetLastError());
+    norm_sample_apply_kernel<T, V><<<grid, 256, 0, st>>>(a);
+    PRNN_HIP(hipGetLastError());
+    return static_cast<int>(PRNN_OK);
+  });
+}
+
+extern "C" PRNN_API int prnn_group_norm_backward(
+    const void* gy, const void* x, const void* w, const void* b, const void* gate,
+    const float* stats, void* dx, void* dw, void* db, void* dgate, int N, int L, int C, int G,
+    float eps, int act, int w_dtype, int dtype, void* workspace, size_t bytes, void* stream) {
+  if (int rc = check("group_norm backward", N, L, C, G, act, w_dtype, dtype)) return rc;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const bool any = N > 0 && L > 0;
+  if (any && (!gy || !x || !dx || (gate && !dgate)))
+    return fail(PRNN_ERR_VALUE, "group_norm backward: gy, x, dx (and dgate) must be non-null");
+  const Plan p = plan(std::max(N, 1), std::max(L, 1), C / G, G, dtype,
+                      bits_of({gy, x, gate, dx, dgate}), true);
+  Carver c(workspace);
+  float *part, *part2 = nullptr;
+  int parts;
+  if (p.token) {
+    parts = p.blocks_x;
+    part = static_cast<float*>(c.take(sizeof(float) * 2 * C * parts));
+  } else {
+    parts = p.strips * N;
+    part = static_cast<float*>(c.take(sizeof(float) * 2 * C * static_cast<size_t>(parts)));
+    part2 = static_cast<float*>(c.take(sizeof(float) * 2 * G * static_cast<size_t>(N)));
+  }
+  if (any && (!workspace || bytes < c.used))
+    return fail(PRNN_ERR_VALUE, "group_norm backward: the workspace must hold %zu bytes", c.used);
+  NormArgs a{};
+  a.x = x;
+  a.w = w;
+  a.b = b;
+  a.gate = gate;
+  a.gy = gy;
+  a.dx = dx;
+  a.dgate = dgate;
+  a.stats = const_cast<float*>(stats);
+  a.part = part;
+  a.part2 = part2;
+  a.rows = N;
+  a.N = N;
+  a.L = L;
+  a.C = C;
+  a.G = G;
+  a.Cg = C / G;
+  a.act = act;
+  a.w_f32 = w_dtype == PRNN_F32;
+  a.lanes = p.lanes;
+  a.strips = p.strips;
+  a.strip_rows = p.strip_rows;
+  a.eps = eps;
+  if (!any) parts = 0;
+  if (any && !p.token && !stats)
+    return fail(PRNN_ERR_VALUE, "group_norm backward: statistics per sample need stats");
+  return with_types(dtype, p.V, [&](auto z, auto v) {
+    using T = decltype(z);
+    constexpr int V = decltype(v)::value;
+    if (any && p.token) {
+      const dim3 grid(p.blocks_x, p.blocks_y);
+      if (p.K == 1)
+        norm_token_bwd_kernel<T, V, 1><<<grid, 256, 0, st>>>(a);
+      else
+        norm_token_bwd_kernel<T, V, 4><<<grid, 256, 0, st>>>(a);
+      PRNN_HIP(hipGetLastError());
+    } else if (any) {
+      const dim3 grid(static_cast<unsigned>(p.strips) * N);
+      norm_sample_bwd_sums_kernel<T, V><<<grid, 256, 0, st>>>(a);
+      PRNN_HIP(hipGetLastError());
+      const unsigned joins = static_cast<unsigned>((1ll * N * G + 3) / 4);
+      norm_sample_means_kernel<T><<<joins, 256, 0, st>>>(a);
+      PRNN_HIP(hipGetLastError());
+      norm_sample_dx_kernel<T, V><<<grid, 256, 0, st>>>(a);
+      PRNN_HIP(hipGetLastError());
+    }
+    if (dw || db) {
+      norm_param_kernel<T><<<dim3((C + 31) / 32, 2), 256, 0, st>>>(part, parts, C, dw, db,
+                                                                   a.w_f32);
+      PRNN_HIP(hipGetLastError());
+    }
+    return static_cast<int>(PRNN_OK);
+  });
+}

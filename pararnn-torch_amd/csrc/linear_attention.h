@@ -1,0 +1,209 @@
+// Decayed linear attention: what the walk kernels and their host code share.
+//
+// One head holds a state S (Dk x Dv) in fp32 and a log decay g_t per token:
+//
+//   S_t = exp(g_t) S_{t-1} + k_t v_t^T,      o_t = scale q_t^T S_t.
+//
+// The kernels walk a sequence in chunks with S in registers.  With G_i the running sum of g
+// inside a chunk (the chunk's first token included) and S the state before the chunk,
+//
+//   o_i = scale [ sum_{j <= i} exp(G_i - G_j) (q_i . k_j) v_j  +  exp(G_i) q_i^T S ]
+//   S'  = exp(G_last) S + sum_j exp(G_last - G_j) k_j v_j^T:
+//
+// four matrix products a chunk.  All three gradients are walks of the same form with the
+// arrays in other roles (x: the rows of the output, y and z: what the state is made of):
+//
+//             x   y   z    state            direction
+//   o     =   q   k   v    S                forward
+//   dq    =   go  v   k    S^T              forward
+//   dk    =   v   go  q    R^T              backward
+//   dv    =   k   q   go   R                backward
+//
+// where R_t = exp(g_{t+1}) R_{t+1} + scale q_t go_t^T is dL/dS_t; backwards the decay between
+// a token and the one walked before it is the later one's.  A sequence may be cut into pieces
+// that run side by side: a first pass forms every piece's own contribution to the state, a
+// small one joins them into the states at the pieces' starts.
+#pragma once
+
+#include <algorithm>
+
+#include "prnn_host.h"
+
+namespace prnn {
+
+constexpr int kLaMaxDim = 256;  // widest head (keys or values)
+
+struct LaView {
+  const void* p;
+  long long sb, st, sh;  // elements between batches, tokens, heads
+  int rep;               // consecutive heads that share one of this array
+  int vec;               // rows and base admit 16-byte accesses
+};
+
+// The decays: (B, T, H) by strides, or one per head (sb = st = 0); fp32 or the storage type.
+struct LaDecay {
+  const void* p;
+  long long sb, st, sh;
+  int dtype;
+};
+
+// How the tokens lie: B sequences of T tokens, or one packed stream with offsets cu.
+struct LaSeqs {
+  const int* cu;    // NULL: rectangular
+  int n_seq;
+  int T;            // tokens of a sequence (rectangular) or of the stream
+  int len;          // tokens of a piece at most
+  int pieces;       // upper bound of the pieces (the grid's)
+};
+
+// States at the ends of the walks: rows of H x Dk x Dv floats.
+struct LaState {
+  float* p;
+  const int* table;  // row of sequence s (NULL: s); outside [0, rows): none
+  int rows;
+};
+
+struct LaRole {
+  LaView x, y, z;
+  void* out;            // (batch, token, head, vd) by the strides below
+  long long o_sb, o_st, o_sh;
+  int out_f32;          // out holds floats (heads that are summed afterwards)
+  LaView dot;           // dots[token] = out . dot where dots is given
+  float* dots;          // [column tile][head][token of the whole batch]
+  int kd, vd;           // columns of x, y and of z, out
+  int sk, sv;           // strides of the state's kd and vd axes
+  int rev;
+  float p_scale, x_scale, u_scale;  // of the pairs, of the state's part, of what enters it
+  float* piece_state;   // [piece][head][Dk][Dv]: states before the pieces (NULL: not cut)
+  float* piece_decay;   // [piece][head]: a piece's whole log decay in the walk's direction
+  LaState init, last;   // given state; where the final one goes (p = NULL: none)
+};
+
+struct LaParams {
+  LaRole role[3];
+  LaDecay g;
+  LaSeqs seqs;
+  int H, Dk, Dv;
+  int tiles;            // column tiles of the widest role (the grid's)
+  int batch_tokens;     // tokens of the whole batch (dots' rows)
+};
+
+// A piece of a sequence: tokens [begin, end) of sequence [s0, s1).
+struct LaPiece {
+  int seq, begin, end, s0, s1;
+  bool first, last, alone;
+};
+
+// Sequence s of a packed stream starts at cu[s]; whatever the offsets hold, nothing outside
+// the stream is touched.
+__device__ __forceinline__ int la_offset(const LaSeqs& q, int s) {
+  const int v = q.cu[s];
+  return v < 0 ? 0 : v > q.T ? q.T : v;
+}
+
+// Piece p.  Rectangular: every sequence has ceil(T / len) of them.  Packed: the stream is cut
+// at multiples of len and at sequence heads, so sequence s starts with piece
+// s + floor(cu[s] / len); its last piece may be empty.
+__device__ __forceinline__ LaPiece la_piece(const LaSeqs& q, int p) {
+  LaPiece r;
+  if (q.cu == nullptr) {
+    const int n = q.T > q.len ? (q.T + q.len - 1) / q.len : 1;
+    r.seq = p / n;
+    const int i = p - r.seq * n;
+    r.s0 = 0;
+    r.s1 = q.T;
+    r.begin = i * q.len;
+    r.end = r.begin + q.len < q.T ? r.begin + q.len : q.T;
+    r.first = i == 0;
+    r.last = i == n - 1;
+  } else {
+    int lo = 0, hi = q.n_seq;  // the last s with s + cu[s] / len <= p
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (mid + la_offset(q, mid) / q.len <= p) lo = mid; else hi = mid;
+    }
+    r.seq = lo;
+    r.s0 = la_offset(q, lo);
+    r.s1 = la_offset(q, lo + 1);
+    if (r.s1 < r.s0) r.s1 = r.s0;
+    const int q0 = r.s0 / q.len;
+    const int i = p - lo - q0;
+    // the piece that holds the last token is the last one; behind it nothing is done
+    const int n = r.s1 > r.s0 ? (r.s1 - 1) / q.len - q0 + 1 : 1;
+    if (i < 0 || i >= n) {
+      r.begin = r.end = r.s1;
+      r.first = r.last = false;
+      r.alone = true;
+      return r;
+    }
+    const int b = (q0 + i) * q.len, e = b + q.len;
+    r.begin = b > r.s0 ? b : r.s0;
+    r.end = e < r.s1 ? e : r.s1;
+    r.first = i == 0;
+    r.last = i == n - 1;
+  }
+  r.alone = r.first && r.last;
+  return r;
+}
+
+// Row of sequence s, or NULL where there is none.
+__device__ __forceinline__ float* la_row(const LaState& st, int s, size_t row_floats) {
+  if (st.p == nullptr) return nullptr;
+  const int r = st.table ? st.table[s] : s;
+  return r < 0 || r >= st.rows ? nullptr : st.p + static_cast<size_t>(r) * row_floats;
+}
+
+// Log decay as it is used: below -104 the factor is zero in fp32 whatever the value (a -inf
+// that resets the state included), and sums stay finite; NaN stays NaN.
+__device__ __forceinline__ float la_clamp(float g) { return g < -104.0f ? -104.0f : g; }
+
+__device__ __forceinline__ float la_decay(const LaDecay& d, int b, int t, int h) {
+  const long long at = static_cast<long long>(b) * d.sb + static_cast<long long>(t) * d.st +
+                       static_cast<long long>(h) * d.sh;
+  float g;
+  if (d.dtype == PRNN_F32)
+    g = static_cast<const float*>(d.p)[at];
+  else if (d.dtype == PRNN_F16)
+    g = to_f32(static_cast<const f16*>(d.p)[at]);
+  else
+    g = to_f32(static_cast<const bf16*>(d.p)[at]);
+  return la_clamp(g);
+}
+
+// The log decay of a step of the walk that reaches token t: forwards g_t, backwards the next
+// token's (none behind the sequence's last token).
+__device__ __forceinline__ float la_step_decay(const LaDecay& d, int rev, const LaPiece& pc, int b,
+                                               int t, int h) {
+  if (!rev) return la_decay(d, b, t, h);
+  return t + 1 < pc.s1 ? la_decay(d, b, t + 1, h) : 0.0f;
+}
+
+// Batch and token of a stream position: rectangular sequences are batches of their own.
+__device__ __forceinline__ int la_batch(const LaSeqs& q, const LaPiece& pc) {
+  return q.cu ? 0 : pc.seq;
+}
+
+// First piece of sequence s and their number.
+__device__ __forceinline__ void la_pieces_of(const LaSeqs& q, int s, int& p0, int& n) {
+  if (q.cu == nullptr) {
+    n = q.T > q.len ? (q.T + q.len - 1) / q.len : 1;
+    p0 = s * n;
+  } else {
+    const int s0 = la_offset(q, s), s1 = la_offset(q, s + 1);
+    p0 = s + s0 / q.len;
+    n = s1 > s0 ? (s1 - 1) / q.len - s0 / q.len + 1 : 1;
+  }
+}
+
+inline int la_widest(const LaParams& p, int roles) {
+  int vd = 0;
+  for (int i = 0; i < roles; ++i) vd = std::max(vd, p.role[i].vd);
+  return vd;
+}
+
+// The walks of `roles` roles of `p`, or (state_only) their pieces' own contributions to the
+// states.  *_tile_cols: columns of z that a workgroup takes where the widest role has vd.
+int la_walk_f32(LaParams p, int roles, bool state_only, int dtype, hipStream_t stream);
+int la_f32_tile_cols(int vd);
+
+}  // namespace prnn

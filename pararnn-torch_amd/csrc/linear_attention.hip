@@ -1,0 +1,527 @@
+// Decayed linear attention: the small kernels around the walks and the C entry points.
+//
+// * la_join_kernel: states before a cut sequence's pieces from the pieces' own contributions;
+// * la_decay_grad_kernel: the log decays' gradient.  dL/dg_t = exp(g_t) <S_{t-1}, R_t> is the
+//   flow from all earlier tokens to t and later ones; from one token to the next it gains what
+//   token t hands on and loses what it receives, so it is a running sum of
+//   k_t . dk_t - q_t . dq_t (both formed in fp32 by the walks), begun at <S_0, dL/dS_0>;
+// * la_head_sum_kernel: gradients of shared heads, summed in a fixed order.
+#include "linear_attention.h"
+
+namespace prnn {
+namespace {
+
+// ---- states before the pieces ------------------------------------------------------------
+
+struct JoinArgs {
+  LaSeqs seqs;
+  float* state[2];
+  const float* decay[2];
+  LaState init[2];
+  int rev[2];
+  int H, DD;
+};
+
+__global__ __launch_bounds__(256) void la_join_kernel(JoinArgs A, int seq_blocks) {
+  const int role = blockIdx.z, h = blockIdx.y;
+  const int seq = blockIdx.x / seq_blocks;
+  const int e = (blockIdx.x - seq * seq_blocks) * 256 + threadIdx.x;
+  int p0, n;
+  la_pieces_of(A.seqs, seq, p0, n);
+  if (n < 2 || e >= A.DD) return;
+  const size_t row = static_cast<size_t>(A.H) * A.DD;
+  const size_t at = static_cast<size_t>(h) * A.DD + e;
+  const float* init = la_row(A.init[role], seq, row);
+  float S = init ? init[at] : 0.0f;
+  for (int i = 0; i < n; ++i) {
+    const size_t p = p0 + (A.rev[role] ? n - 1 - i : i);
+    float* w = A.state[role] + p * row + at;
+    const float U = i + 1 < n ? *w : 0.0f;
+    const float d = i + 1 < n ? A.decay[role][p * A.H + h] : 0.0f;
+    *w = S;
+    S = fmaf(fexp(d), S, U);
+  }
+}
+
+// ---- gradient of the log decays --------------------------------------------------------
+
+struct DecayGradArgs {
+  LaSeqs seqs;
+  const float* q_dots;  // [tile][head][token]
+  const float* k_dots;
+  int tiles, H, DD, batch_tokens;
+  LaState h0;
+  const float* dh0;     // rows of sequences
+  int g_dtype;
+  void* dg;             // (token, H) of g's type, or NULL
+  float* per_seq;       // (sequence, H) sums for decays per head, or NULL
+};
+
+__global__ __launch_bounds__(256) void la_decay_grad_kernel(DecayGradArgs A) {
+  __shared__ double s_wave[4];
+  const int h = blockIdx.y, seq = blockIdx.x, tid = threadIdx.x;
+  const int lane = tid & 63, wave = tid >> 6;
+  int t0, n;
+  if (A.seqs.cu) {
+    t0 = la_offset(A.seqs, seq);
+    n = la_offset(A.seqs, seq + 1) - t0;
+  } else {
+    t0 = seq * A.seqs.T;
+    n = A.seqs.T;
+  }
+  // <S_0, dL/dS_0>
+  double begin = 0.0;
+  const size_t row = static_cast<size_t>(A.H) * A.DD;
+  const float* s0 = la_row(A.h0, seq, row);
+  if (s0) {
+    s0 += static_cast<size_t>(h) * A.DD;
+    const float* d0 = A.dh0 + seq * row + static_cast<size_t>(h) * A.DD;
+    double d = 0.0;
+    for (int e = tid; e < A.DD; e += 256) d += static_cast<double>(s0[e]) * d0[e];
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) d += __shfl_xor(d, k);
+    if (lane == 0) s_wave[wave] = d;
+    __syncthreads();
+    begin = s_wave[0] + s_wave[1] + s_wave[2] + s_wave[3];
+    __syncthreads();
+  }
+  double flow = begin, total = 0.0;
+  constexpr int kEach = 4;
+  for (int base = 0; base < n; base += 256 * kEach) {
+    double d[kEach], sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int t = base + tid * kEach + i;
+      double x = 0.0;
+      if (t < n)
+        for (int k = 0; k < A.tiles; ++k) {
+          const size_t at = (static_cast<size_t>(k) * A.H + h) * A.batch_tokens + t0 + t;
+          x += static_cast<double>(A.k_dots[at]) - A.q_dots[at];
+        }
+      d[i] = sum;  // what came before within the thread's tokens
+      sum += x;
+    }
+    double run = sum;
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) {
+      const double o = __shfl_up(run, k);
+      if (lane >= k) run += o;
+    }
+    if (lane == 63) s_wave[wave] = run;
+    __syncthreads();
+    double before = flow + run - sum, all = 0.0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) before += s_wave[w];
+      all += s_wave[w];
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int t = base + tid * kEach + i;
+      if (t >= n) continue;
+      const float v = static_cast<float>(before + d[i]);
+      total += v;
+      if (A.dg) {
+        const size_t at = (static_cast<size_t>(t0) + t) * A.H + h;
+        if (A.g_dtype == PRNN_F32)
+          static_cast<float*>(A.dg)[at] = v;
+        else if (A.g_dtype == PRNN_F16)
+          static_cast<f16*>(A.dg)[at] = from_f32<f16>(v);
+        else
+          static_cast<bf16*>(A.dg)[at] = from_f32<bf16>(v);
+      }
+    }
+    flow += all;
+    __syncthreads();
+  }
+  if (A.per_seq) {
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) total += __shfl_xor(total, k);
+    if (lane == 0) s_wave[wave] = total;
+    __syncthreads();
+    if (tid == 0)
+      A.per_seq[static_cast<size_t>(seq) * A.H + h] =
+          static_cast<float>(s_wave[0] + s_wave[1] + s_wave[2] + s_wave[3]);
+  }
+}
+
+__global__ void la_decay_sum_kernel(const float* __restrict__ per_seq, void* dg, int g_dtype,
+                                    int n_seq, int H) {
+  const int h = blockIdx.x * blockDim.x + threadIdx.x;
+  if (h >= H) return;
+  double d = 0.0;
+  for (int s = 0; s < n_seq; ++s) d += per_seq[static_cast<size_t>(s) * H + h];
+  const float v = static_cast<float>(d);
+  if (g_dtype == PRNN_F32)
+    static_cast<float*>(dg)[h] = v;
+  else if (g_dtype == PRNN_F16)
+    static_cast<f16*>(dg)[h] = from_f32<f16>(v);
+  else
+    static_cast<bf16*>(dg)[h] = from_f32<bf16>(v);
+}
+
+// ---- gradients of shared heads ---------------------------------------------------------
+
+struct HeadSumArgs {
+  const float* src[3];  // (token, H, D)
+  void* dst[3];         // (token, H / rep, D)
+  int rep[3], D[3];
+  int H;
+  size_t tokens;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void la_head_sum_kernel(HeadSumArgs A) {
+  const int k = blockIdx.y;
+  if (A.src[k] == nullptr) return;
+  const int D = A.D[k], rep = A.rep[k], heads = A.H / rep;
+  const size_t n = A.tokens * heads * D, stride = static_cast<size_t>(gridDim.x) * 256;
+  for (size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += stride) {
+    const size_t d = i % D, th = i / D, hh = th % heads, t = th / heads;
+    const float* s = A.src[k] + (t * A.H + hh * rep) * D + d;
+    float v = 0.0f;
+    for (int r = 0; r < rep; ++r) v += s[static_cast<size_t>(r) * D];
+    static_cast<T*>(A.dst[k])[i] = from_f32<T>(v);
+  }
+}
+
+// ---- host ------------------------------------------------------------------------------
+
+using Problem = prnn_linear_attention_problem;
+
+LaView view(const prnn_la_view& v, int H, int dtype) {
+  LaView r{v.p, v.sb, v.st, v.sh, 1, 0};
+  if (v.heads > 0) r.rep = H / v.heads;
+  const long long size = dtype == PRNN_F32 ? 4 : 2;
+  const long long bytes = static_cast<long long>(reinterpret_cast<uintptr_t>(v.p)) |
+                          v.sb * size | v.st * size | v.sh * size;
+  r.vec = (bytes & 15) == 0;
+  return r;
+}
+
+int check(const Problem* a) {
+  if (a == nullptr) return fail(PRNN_ERR_VALUE, "the problem must be non-null");
+  if (int rc = check_dtype(a->dtype)) return rc;
+  if (a->g_dtype != PRNN_F32 && a->g_dtype != a->dtype)
+    return fail(PRNN_ERR_TYPE, "log_decay must be float32 or of the storage type");
+  if (a->H < 1 || a->H > 65535) return fail(PRNN_ERR_VALUE, "H=%d is not in 1 .. 65535", a->H);
+  if (a->Dk < 1 || a->Dk > kLaMaxDim || a->Dv < 1 || a->Dv > kLaMaxDim)
+    return fail(PRNN_ERR_VALUE, "head widths (%d, %d) are not in 1 .. %d", a->Dk, a->Dv, kLaMaxDim);
+  if (a->B < 0 || a->T < 0 || (a->cu_seqlens ? a->n_seq < 1 || a->B != 1 : a->n_seq != 0))
+    return fail(PRNN_ERR_VALUE, "B=%d, T=%d, n_seq=%d do not describe a batch", a->B, a->T,
+                a->n_seq);
+  if (static_cast<long long>(a->B) * a->T > (1ll << 30))
+    return fail(PRNN_ERR_VALUE, "%lld tokens are more than 2^30", 1ll * a->B * a->T);
+  for (const prnn_la_view* v : {&a->q, &a->k, &a->v})
+    if (v->heads < 1 || a->H % v->heads)
+      return fail(PRNN_ERR_VALUE, "%d heads do not divide H=%d", v->heads, a->H);
+  if (static_cast<long long>(a->B) * a->T > 0)
+    for (const void* p : {a->q.p, a->k.p, a->v.p, a->g})
+      if (p == nullptr) return fail(PRNN_ERR_VALUE, "q, k, v and log_decay must be non-null");
+  if (a->h0 && a->h0_rows < 0) return fail(PRNN_ERR_VALUE, "h0_rows=%d", a->h0_rows);
+  return PRNN_OK;
+}
+
+int sequences(const Problem& a) { return a.cu_seqlens ? a.n_seq : a.B; }
+
+// How long the pieces are.  Walks of whole sequences read every array once; cut ones read k
+// and v once more and move a state a piece, so a sequence is cut only as far as the chip has
+// workgroups to spare (about kLaTarget run at a time), and never below kLaLeast tokens.
+constexpr int kLaTarget = 1024, kLaLeast = 256;
+
+LaSeqs cut(const Problem& a, int tiles_and_roles) {
+  LaSeqs s{a.cu_seqlens, sequences(a), a.T, 1, 0};
+  const long long work = 1ll * a.B * a.T * a.H * tiles_and_roles;
+  long long len = (work + kLaTarget - 1) / kLaTarget;
+  len = std::max<long long>(kLaLeast, (len + 63) / 64 * 64);
+  if (len >= a.T) {
+    s.len = a.T + 1;  // every sequence whole
+    s.pieces = s.n_seq;
+  } else {
+    s.len = static_cast<int>(len);
+    s.pieces = a.cu_seqlens ? s.n_seq + a.T / s.len
+                            : a.B * ((a.T + s.len - 1) / s.len);
+  }
+  return s;
+}
+
+bool is_cut(const LaSeqs& s) { return s.len <= s.T; }
+
+LaDecay decay_of(const Problem& a) { return LaDecay{a.g, a.g_sb, a.g_st, a.g_sh, a.g_dtype}; }
+
+// Scratch of either direction.  `roles`: states that are kept per piece (forward 1,
+// backward 2).
+struct Scratch {
+  float* state[2];
+  float* decay[2];
+  float* dots[2];
+  float* heads[3];
+  float* per_seq;
+  size_t bytes;
+};
+
+int walk_cols(const Problem& a, int vd) { return la_f32_tile_cols(vd); }
+
+int walk(const LaParams& p, int roles, bool state_only, const Problem& a, hipStream_t st) {
+  return la_walk_f32(p, roles, state_only, a.dtype, st);
+}
+
+int tiles_of(const Problem& a, int vd) {
+  const int c = walk_cols(a, vd);
+  return (vd + c - 1) / c;
+}
+
+LaSeqs forward_cut(const Problem& a) { return cut(a, tiles_of(a, a.Dv)); }
+LaSeqs backward_cut(const Problem& a) {
+  return cut(a, 3 * tiles_of(a, std::max(a.Dk, a.Dv)));
+}
+
+Scratch carve(void* ws, const Problem& a, bool backward, bool decay_grad) {
+  Carver c(ws);
+  Scratch s{};
+  const LaSeqs q = backward ? backward_cut(a) : forward_cut(a);
+  const size_t dd = static_cast<size_t>(a.Dk) * a.Dv;
+  const size_t tokens = static_cast<size_t>(a.B) * a.T;
+  for (int i = 0; i < (backward ? 2 : 1); ++i)
+    if (is_cut(q)) {
+      s.state[i] = static_cast<float*>(c.take(4 * dd * a.H * q.pieces));
+      s.decay[i] = static_cast<float*>(c.take(4 * static_cast<size_t>(a.H) * q.pieces));
+    }
+  if (backward) {
+    if (decay_grad) {
+      const size_t tiles = tiles_of(a, std::max(a.Dk, a.Dv));
+      for (float*& d : s.dots) d = static_cast<float*>(c.take(4 * tiles * a.H * tokens));
+      s.per_seq = static_cast<float*>(c.take(4 * static_cast<size_t>(a.H) * sequences(a)));
+    }
+    const int heads[3] = {a.q.heads, a.k.heads, a.v.heads}, D[3] = {a.Dk, a.Dk, a.Dv};
+    for (int i = 0; i < 3; ++i)
+      if (heads[i] != a.H)
+        s.heads[i] = static_cast<float*>(c.take(4 * tokens * a.H * D[i]));
+  }
+  s.bytes = c.used;
+  return s;
+}
+
+int check_ws(size_t need, const void* ws, size_t bytes) {
+  if (need && (ws == nullptr || bytes < need || (reinterpret_cast<uintptr_t>(ws) & 255)))
+    return fail(PRNN_ERR_VALUE, "the workspace must hold %zu bytes, 256-byte aligned (got %zu)",
+                need, bytes);
+  return PRNN_OK;
+}
+
+int join(const LaParams& p, const Scratch& s, const LaState* init, const int* rev, int roles,
+         hipStream_t st) {
+  JoinArgs j{};
+  j.seqs = p.seqs;
+  j.H = p.H;
+  j.DD = p.Dk * p.Dv;
+  for (int i = 0; i < roles; ++i) {
+    j.state[i] = s.state[i];
+    j.decay[i] = s.decay[i];
+    j.init[i] = init[i];
+    j.rev[i] = rev[i];
+  }
+  const int blocks = (j.DD + 255) / 256;
+  la_join_kernel<<<dim3(static_cast<unsigned>(p.seqs.n_seq) * blocks, p.H, roles), 256, 0, st>>>(
+      j, blocks);
+  PRNN_HIP(hipGetLastError());
+  return PRNN_OK;
+}
+
+LaParams params(const Problem& a, const LaSeqs& q) {
+  LaParams p{};
+  p.g = decay_of(a);
+  p.seqs = q;
+  p.H = a.H;
+  p.Dk = a.Dk;
+  p.Dv = a.Dv;
+  p.batch_tokens = a.B * a.T;
+  return p;
+}
+
+LaState initial(const Problem& a) {
+  return LaState{const_cast<float*>(a.h0), a.h0_table, a.h0_rows};
+}
+
+int forward(const Problem& a, const prnn_la_view& out, float* state_out, const int* out_table,
+            int out_rows, void* ws, hipStream_t st) {
+  const Scratch s = carve(ws, a, false, false);
+  LaParams p = params(a, forward_cut(a));
+  LaRole& r = p.role[0];
+  r.x = view(a.q, a.H, a.dtype);
+  r.y = view(a.k, a.H, a.dtype);
+  r.z = view(a.v, a.H, a.dtype);
+  r.out = const_cast<void*>(out.p);
+  r.o_sb = out.sb;
+  r.o_st = out.st;
+  r.o_sh = out.sh;
+  r.kd = a.Dk;
+  r.vd = a.Dv;
+  r.sk = a.Dv;
+  r.sv = 1;
+  r.p_scale = r.x_scale = a.scale;
+  r.u_scale = 1.0f;
+  r.piece_state = s.state[0];
+  r.piece_decay = s.decay[0];
+  r.init = initial(a);
+  r.last = LaState{state_out, out_table, out_rows};
+  if (is_cut(p.seqs)) {
+    if (int rc = walk(p, 1, true, a, st)) return rc;
+    const int rev = 0;
+    if (int rc = join(p, s, &r.init, &rev, 1, st)) return rc;
+  }
+  return walk(p, 1, false, a, st);
+}
+
+int backward(const Problem& a, const prnn_la_view& go, const float* gs, void* dq, void* dk,
+             void* dv, void* dg, float* dh0, void* ws, hipStream_t st) {
+  const Scratch s = carve(ws, a, true, dg != nullptr);
+  LaParams p = params(a, backward_cut(a));
+  const LaView q = view(a.q, a.H, a.dtype), k = view(a.k, a.H, a.dtype),
+               v = view(a.v, a.H, a.dtype), o = view(go, a.H, a.dtype);
+  const LaState init = initial(a), fin{const_cast<float*>(gs), nullptr, sequences(a)};
+  const LaView none{nullptr, 0, 0, 0, 1, 1};
+  auto role = [&](LaView x, LaView y, LaView z, int kd, int vd, bool transposed, int rev) {
+    LaRole r{};
+    r.x = x;
+    r.y = y;
+    r.z = z;
+    r.kd = kd;
+    r.vd = vd;
+    r.sk = transposed ? 1 : a.Dv;
+    r.sv = transposed ? a.Dv : 1;
+    r.rev = rev;
+    r.p_scale = a.scale;
+    r.x_scale = rev ? 1.0f : a.scale;
+    r.u_scale = rev ? a.scale : 1.0f;
+    r.piece_state = s.state[rev];
+    r.piece_decay = s.decay[rev];
+    r.init = rev ? fin : init;
+    r.dot = none;
+    return r;
+  };
+  if (is_cut(p.seqs)) {
+    p.role[0] = role(none, k, v, a.Dk, a.Dv, false, 0);
+    p.role[1] = role(none, q, o, a.Dk, a.Dv, false, 1);
+    if (int rc = walk(p, 2, true, a, st)) return rc;
+    const LaState inits[2] = {init, fin};
+    const int rev[2] = {0, 1};
+    if (int rc = join(p, s, inits, rev, 2, st)) return rc;
+  }
+  p.role[0] = role(o, v, k, a.Dv, a.Dk, true, 0);
+  p.role[1] = role(v, o, q, a.Dv, a.Dk, true, 1);
+  p.role[2] = role(k, q, o, a.Dk, a.Dv, false, 1);
+  void* outs[3] = {dq, dk, dv};
+  const int D[3] = {a.Dk, a.Dk, a.Dv}, heads[3] = {a.q.heads, a.k.heads, a.v.heads};
+  HeadSumArgs hs{};
+  bool sums = false;
+  for (int i = 0; i < 3; ++i) {
+    LaRole& r = p.role[i];
+    r.out_f32 = s.heads[i] != nullptr;
+    r.out = r.out_f32 ? s.heads[i] : outs[i];
+    r.o_sh = D[i];
+    r.o_st = static_cast<long long>(a.H) * D[i];
+    r.o_sb = r.o_st * a.T;
+    hs.src[i] = s.heads[i];
+    hs.dst[i] = outs[i];
+    hs.rep[i] = a.H / heads[i];
+    hs.D[i] = D[i];
+    sums = sums || s.heads[i];
+  }
+  p.role[2].last = LaState{dh0, nullptr, sequences(a)};
+  if (dg) {
+    p.role[0].dot = q;
+    p.role[0].dots = s.dots[0];
+    p.role[1].dot = k;
+    p.role[1].dots = s.dots[1];
+  }
+  if (int rc = walk(p, 3, false, a, st)) return rc;
+  const size_t tokens = static_cast<size_t>(a.B) * a.T;
+  if (sums && tokens) {
+    hs.H = a.H;
+    hs.tokens = tokens;
+    const size_t most = tokens * a.H * std::max(a.Dk, a.Dv);
+    const unsigned blocks = static_cast<unsigned>(std::min<size_t>((most + 1023) / 1024, 4096));
+    if (int rc = with_storage(a.dtype, [&](auto z) {
+          la_head_sum_kernel<decltype(z)><<<dim3(blocks, 3), 256, 0, st>>>(hs);
+          PRNN_HIP(hipGetLastError());
+          return static_cast<int>(PRNN_OK);
+        }))
+      return rc;
+  }
+  if (dg) {
+    DecayGradArgs d{};
+    d.seqs = p.seqs;
+    d.q_dots = s.dots[0];
+    d.k_dots = s.dots[1];
+    const int cols = walk_cols(a, std::max(a.Dk, a.Dv));
+    d.tiles = (a.Dk + cols - 1) / cols;
+    d.H = a.H;
+    d.DD = a.Dk * a.Dv;
+    d.batch_tokens = static_cast<int>(tokens);
+    d.h0 = init;
+    d.dh0 = dh0;
+    d.g_dtype = a.g_dtype;
+    const bool per_head = a.g_sb == 0 && a.g_st == 0;
+    d.dg = per_head ? nullptr : dg;
+    d.per_seq = per_head ? s.per_seq : nullptr;
+    const int n_seq = sequences(a);
+    if (n_seq > 0) {
+      la_decay_grad_kernel<<<dim3(n_seq, a.H), 256, 0, st>>>(d);
+      PRNN_HIP(hipGetLastError());
+    }
+    if (per_head) {
+      la_decay_sum_kernel<<<(a.H + 63) / 64, 64, 0, st>>>(s.per_seq, dg, a.g_dtype, n_seq, a.H);
+      PRNN_HIP(hipGetLastError());
+    }
+  }
+  return PRNN_OK;
+}
+
+}  // namespace
+}  // namespace prnn
+
+using namespace prnn;
+
+extern "C" PRNN_API size_t
+prnn_linear_attention_workspace_size(const prnn_linear_attention_problem* a) {
+  if (check(a)) return 0;
+  return carve(nullptr, *a, false, false).bytes;
+}
+
+extern "C" PRNN_API int prnn_linear_attention(const prnn_linear_attention_problem* a,
+                                              const prnn_la_view* out, float* state_out,
+                                              const int* out_table, int out_rows, void* workspace,
+                                              size_t bytes, void* stream) {
+  if (int rc = check(a)) return rc;
+  if (out == nullptr || (out->p == nullptr && 1ll * a->B * a->T > 0))
+    return fail(PRNN_ERR_VALUE, "out must be non-null");
+  if (sequences(*a) == 0) return PRNN_OK;
+  if (int rc = check_ws(carve(nullptr, *a, false, false).bytes, workspace, bytes)) return rc;
+  return forward(*a, *out, state_out, out_table, out_rows, workspace,
+                 static_cast<hipStream_t>(stream));
+}
+
+extern "C" PRNN_API size_t prnn_linear_attention_backward_workspace_size(
+    const prnn_linear_attention_problem* a, int decay_grad) {
+  if (check(a)) return 0;
+  return carve(nullptr, *a, true, decay_grad != 0).bytes;
+}
+
+extern "C" PRNN_API int prnn_linear_attention_backward(
+    const prnn_linear_attention_problem* a, const prnn_la_view* go, const float* gs, void* dq,
+    void* dk, void* dv, void* dg, float* dh0, void* workspace, size_t bytes, void* stream) {
+  if (int rc = check(a)) return rc;
+  const bool any = 1ll * a->B * a->T > 0;
+  if (go == nullptr || (any && (!go->p || !dq || !dk || !dv)))
+    return fail(PRNN_ERR_VALUE, "go, dq, dk and dv must be non-null");
+  if (a->h0_table) return fail(PRNN_ERR_VALUE, "a block table has no gradient");
+  if (a->h0 && a->h0_rows < sequences(*a))
+    return fail(PRNN_ERR_VALUE, "h0 has %d rows for %d sequences", a->h0_rows, sequences(*a));
+  if (dg && a->h0 && !dh0)
+    return fail(PRNN_ERR_VALUE, "the decays' gradient with an initial state needs dh0");
+  if (sequences(*a) == 0 && !(dg && a->g_sb == 0 && a->g_st == 0)) return PRNN_OK;
+  if (int rc = check_ws(carve(nullptr, *a, true, dg != nullptr).bytes, workspace, bytes)) return rc;
+  if (sequences(*a) == 0) return PRNN_OK;
+  return backward(*a, *go, gs, dq, dk, dv, dg, dh0, workspace, static_cast<hipStream_t>(stream));
+}

@@ -1,0 +1,162 @@
+// Decayed linear attention, one token: S <- exp(g) S + k v^T in place, o = scale q^T S.
+//
+// Bound by the state's traffic (read once, written once: 8 bytes an element against 4 flops).
+// A workgroup takes TJ columns of one head's state: L lanes of four columns side by side, the
+// rows spread over 256 / L groups of lanes, so every access is 16 bytes a lane and a thread has
+// all its rows' loads in flight before the first is used.
+#include "linear_attention.h"
+
+namespace prnn {
+namespace {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+
+struct StepArgs {
+  LaView q, k, v;
+  LaDecay g;
+  void* out;
+  long long o_sb, o_sh;
+  float* state;
+  const int* table;
+  int rows;
+  int H, Dk, Dv;
+  float scale;
+};
+
+// L lanes x 4 columns; U rows of a thread at a time.
+template <typename T, int L, bool VEC>
+__global__ __launch_bounds__(256) void la_step_kernel(StepArgs A) {
+  constexpr int G = 256 / L;  // rows at a time
+  constexpr int U = 8;
+  __shared__ float sq[kLaMaxDim], sk[kLaMaxDim];
+  __shared__ __align__(16) float so[G * L * 4];
+  const int tid = threadIdx.x, lane = tid % L, grp = tid / L;
+  const int h = blockIdx.y, b = blockIdx.z;
+  const int c0 = (blockIdx.x * L + lane) * 4;
+  const int r = A.table ? A.table[b] : b;
+  const bool kept = r >= 0 && r < A.rows;
+  float* S = A.state + (static_cast<size_t>(kept ? r : 0) * A.H + h) * A.Dk * A.Dv;
+  const T* q = static_cast<const T*>(A.q.p) + b * A.q.sb + (h / A.q.rep) * A.q.sh;
+  const T* k = static_cast<const T*>(A.k.p) + b * A.k.sb + (h / A.k.rep) * A.k.sh;
+  const T* v = static_cast<const T*>(A.v.p) + b * A.v.sb + (h / A.v.rep) * A.v.sh;
+  for (int i = tid; i < A.Dk; i += 256) {
+    sq[i] = to_f32(q[i]);
+    sk[i] = to_f32(k[i]);
+  }
+  const float a = fexp(la_decay(A.g, b, 0, h));
+  f4 vv = {0, 0, 0, 0};
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    if (c0 + c < A.Dv) vv[c] = to_f32(v[c0 + c]);
+  f4 o = {0, 0, 0, 0};
+  bool synced = false;
+  for (int i0 = grp; i0 < A.Dk || !synced; i0 += G * U) {
+    f4 s[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * G;
+      s[u] = f4{0, 0, 0, 0};
+      if (kept && i < A.Dk) {
+        if (VEC) {
+          if (c0 < A.Dv) s[u] = *reinterpret_cast<const f4*>(S + static_cast<size_t>(i) * A.Dv + c0);
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (c0 + c < A.Dv) s[u][c] = S[static_cast<size_t>(i) * A.Dv + c0 + c];
+        }
+      }
+    }
+    if (!synced) {
+      __syncthreads();
+      synced = true;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * G;
+      if (i >= A.Dk) continue;
+      const float ki = sk[i], qi = sq[i];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        s[u][c] = fmaf(a, s[u][c], ki * vv[c]);
+        o[c] = fmaf(qi, s[u][c], o[c]);
+      }
+      if (kept) {
+        if (VEC) {
+          if (c0 < A.Dv) *reinterpret_cast<f4*>(S + static_cast<size_t>(i) * A.Dv + c0) = s[u];
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (c0 + c < A.Dv) S[static_cast<size_t>(i) * A.Dv + c0 + c] = s[u][c];
+        }
+      }
+    }
+  }
+  *reinterpret_cast<f4*>(&so[tid * 4]) = o;
+  __syncthreads();
+  // column j of the tile: the groups' sums in their order
+  for (int j = tid; j < 4 * L; j += 256) {
+    float x = 0.0f;
+#pragma unroll
+    for (int g = 0; g < G; ++g) x += so[g * 4 * L + j];
+    const int col = blockIdx.x * 4 * L + j;
+    if (col < A.Dv)
+      static_cast<T*>(A.out)[b * A.o_sb + h * A.o_sh + col] = from_f32<T>(x * A.scale);
+  }
+}
+
+template <typename T, int L>
+int launch(const StepArgs& a, int B, bool vec, hipStream_t st) {
+  const dim3 grid((a.Dv + 4 * L - 1) / (4 * L), a.H, B);
+  if (vec)
+    la_step_kernel<T, L, true><<<grid, 256, 0, st>>>(a);
+  else
+    la_step_kernel<T, L, false><<<grid, 256, 0, st>>>(a);
+  PRNN_HIP(hipGetLastError());
+  return PRNN_OK;
+}
+
+}  // namespace
+}  // namespace prnn
+
+using namespace prnn;
+
+extern "C" PRNN_API int prnn_linear_attention_step(
+    const void* q, long long q_sb, long long q_sh, int q_heads, const void* k, long long k_sb,
+    long long k_sh, int k_heads, const void* v, long long v_sb, long long v_sh, int v_heads,
+    const void* g, long long g_sb, long long g_sh, int g_dtype, float* state,
+    const int* block_table, int rows, void* out, int B, int H, int Dk, int Dv, float scale,
+    int dtype, void* stream) {
+  if (int rc = check_dtype(dtype)) return rc;
+  if (g_dtype != PRNN_F32 && g_dtype != dtype)
+    return fail(PRNN_ERR_TYPE, "log_decay must be float32 or of the storage type");
+  if (B < 0 || B > 65535 || H < 1 || H > 65535)
+    return fail(PRNN_ERR_VALUE, "B=%d, H=%d are not in 0 .. 65535", B, H);
+  if (Dk < 1 || Dk > kLaMaxDim || Dv < 1 || Dv > kLaMaxDim)
+    return fail(PRNN_ERR_VALUE, "head widths (%d, %d) are not in 1 .. %d", Dk, Dv, kLaMaxDim);
+  for (int heads : {q_heads, k_heads, v_heads})
+    if (heads < 1 || H % heads)
+      return fail(PRNN_ERR_VALUE, "%d heads do not divide H=%d", heads, H);
+  if (B == 0) return PRNN_OK;
+  if (!q || !k || !v || !g || !state || !out)
+    return fail(PRNN_ERR_VALUE, "q, k, v, log_decay, state and out must be non-null");
+  StepArgs a{};
+  a.q = LaView{q, q_sb, 0, q_sh, H / q_heads, 0};
+  a.k = LaView{k, k_sb, 0, k_sh, H / k_heads, 0};
+  a.v = LaView{v, v_sb, 0, v_sh, H / v_heads, 0};
+  a.g = LaDecay{g, g_sb, 0, g_sh, g_dtype};
+  a.out = out;
+  a.o_sb = static_cast<long long>(H) * Dv;
+  a.o_sh = Dv;
+  a.state = state;
+  a.table = block_table;
+  a.rows = rows;
+  a.H = H;
+  a.Dk = Dk;
+  a.Dv = Dv;
+  a.scale = scale;
+  const bool vec = Dv % 4 == 0 && (reinterpret_cast<uintptr_t>(state) & 15) == 0;
+  return with_storage(dtype, [&](auto z) {
+    using T = decltype(z);
+    return launch<T, 16>(a, B, vec, static_cast<hipStream_t>(stream));
+  });
+}

@@ -17,6 +17,8 @@ from pararnn_amd.config import (
     NewtonStats,
     compile_safe_config,
 )
+from pararnn_amd.group_norm import group_norm
+from pararnn_amd.linear_attention import linear_attention, linear_attention_step
 from pararnn_amd.newton import (
     auto_newton_iters,
     fused_newton,
@@ -26,6 +28,14 @@ from pararnn_amd.newton import (
 )
 from pararnn_amd.layers import ParaRNN
 from pararnn_amd.ops import newton_gru_head_fused, newton_slstm_fused, slstm_init_fused
+from pararnn_amd.pages import (
+    compact_pages,
+    copy_pages,
+    fork_pages,
+    free_pages,
+    take_pages,
+)
+from pararnn_amd.ragged import PackedSequences
 from pararnn_amd.sequential import sequential_apply
 from pararnn_amd.verify import (
     AgreementError,
@@ -43,6 +53,7 @@ __all__ = [
     "NewtonConfig",
     "NewtonDivergenceError",
     "NewtonStats",
+    "PackedSequences",
     "ParaGRU",
     "ParaRNN",
     "ParaSLSTM",
@@ -50,9 +61,16 @@ __all__ = [
     "can_decode_step",
     "decode_step",
     "decode_wx",
+    "compact_pages",
     "compile_safe_config",
+    "copy_pages",
     "default_agreement_atol",
+    "fork_pages",
+    "free_pages",
     "fused_newton",
+    "group_norm",
+    "linear_attention",
+    "linear_attention_step",
     "newton_apply",
     "newton_gru_head_fused",
     "newton_slstm_fused",
@@ -60,5 +78,6 @@ __all__ = [
     "slstm_auto_picard",
     "slstm_init_fused",
     "slstm_picard_next",
+    "take_pages",
     "verify_agreement",
 ]

@@ -20,7 +20,7 @@ PRNN_OK = 0
 PRNN_ERR_VALUE = 1
 PRNN_ERR_TYPE = 2
 PRNN_ERR_RUNTIME = 3
-ABI_VERSION = 14
+ABI_VERSION = 15
 
 class BlockMove(ctypes.Structure):
     """``prnn_block_move``."""
@@ -29,11 +29,40 @@ class BlockMove(ctypes.Structure):
                 ("matrix", ctypes.c_int), ("elem_bytes", ctypes.c_int)]
 
 
+class LaView(ctypes.Structure):
+    """``prnn_la_view``."""
+
+    _fields_ = [("p", ctypes.c_void_p), ("sb", ctypes.c_longlong), ("st", ctypes.c_longlong),
+                ("sh", ctypes.c_longlong), ("heads", ctypes.c_int)]
+
+
+class LaProblem(ctypes.Structure):
+    """``prnn_linear_attention_problem``."""
+
+    _fields_ = [("q", LaView), ("k", LaView), ("v", LaView), ("g", ctypes.c_void_p),
+                ("g_sb", ctypes.c_longlong), ("g_st", ctypes.c_longlong),
+                ("g_sh", ctypes.c_longlong), ("h0", ctypes.c_void_p),
+                ("h0_table", ctypes.c_void_p), ("cu_seqlens", ctypes.c_void_p),
+                *((n, ctypes.c_int) for n in ("h0_rows", "n_seq", "B", "T", "H", "Dk", "Dv",
+                                              "g_dtype", "dtype")),
+                ("scale", ctypes.c_float)]
+
+
+class Pool(ctypes.Structure):
+    """``prnn_pool``."""
+
+    _fields_ = [("p", ctypes.c_void_p), ("row_bytes", ctypes.c_longlong)]
+
+
 # name -> (restype, argtypes); mirrors include/pararnn_amd.h
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _F = ctypes.c_float
 _S = ctypes.c_size_t
+_L = ctypes.c_longlong
+_LAP = ctypes.POINTER(LaProblem)
+_LAV = ctypes.POINTER(LaView)
+_PP = ctypes.POINTER(Pool)
 SIGNATURES: dict[str, tuple] = {
     "prnn_abi_version": (_I, []),
     "prnn_last_error": (ctypes.c_char_p, []),
@@ -118,6 +147,25 @@ SIGNATURES: dict[str, tuple] = {
         _I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _F, _F, _I, _I, _P]),
     "prnn_gru_decode_x": (
         _I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I, _P]),
+    "prnn_linear_attention_workspace_size": (_S, [_LAP]),
+    "prnn_linear_attention": (_I, [_LAP, _LAV, _P, _P, _I, _P, _S, _P]),
+    "prnn_linear_attention_backward_workspace_size": (_S, [_LAP, _I]),
+    "prnn_linear_attention_backward": (
+        _I, [_LAP, _LAV, _P, _P, _P, _P, _P, _P, _P, _S, _P]),
+    "prnn_linear_attention_step": (
+        _I, [_P, _L, _L, _I, _P, _L, _L, _I, _P, _L, _L, _I, _P, _L, _L, _I, _P, _P, _I, _P,
+             _I, _I, _I, _I, _F, _I, _P]),
+    "prnn_group_norm_workspace_size": (_S, [_I, _I, _I, _I, _I, _I]),
+    "prnn_group_norm": (
+        _I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I, _I, _P, _S, _P]),
+    "prnn_group_norm_backward": (
+        _I, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I, _I, _P, _S, _P]),
+    "prnn_pages_take": (_I, [_P, _I, _P, _I, _P]),
+    "prnn_pages_fork": (_I, [_P, _I, _PP, _I, _P, _P, _I, _P, _P]),
+    "prnn_pages_free": (_I, [_P, _I, _P, _I, _P]),
+    "prnn_pages_copy": (_I, [_I, _PP, _I, _P, _P, _I, _P]),
+    "prnn_pages_compact": (
+        _I, [_P, _I, _PP, _I, ctypes.POINTER(_P), ctypes.POINTER(_I), _I, _P, _P, _P]),
 }
 
 _lock = threading.Lock()

@@ -1,0 +1,145 @@
+"""Group norm, channels last, with an activation or a gate: the norm behind a token mixer.
+
+    z = weight * (x - mean) * rstd + bias        y = act(z)     or     y = z * act(gate)
+
+per group of consecutive channels of ``x`` ``(..., C)``; the statistics run over one token's group
+(``over="token"``, what a causal model uses) or over all tokens of a sample (``over="sample"``: all
+dimensions between the first and the last).  float32, bfloat16 and float16; arithmetic, statistics
+and the parameters' gradient sums are float32, each result is rounded once.  Sums run in a fixed
+order.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch import Tensor
+
+from pararnn_amd import _lib
+from pararnn_amd.linear_attention import _on
+from pararnn_amd.ops import _DTYPES, _ptr, _stream, _validate, _workspace
+
+_ACTIVATIONS = {None: 0, "silu": 1, "sigmoid": 2}
+
+
+def _shape(x: Tensor, over: str) -> tuple[int, int, int]:
+    """(N, L, C): L tokens share their statistics."""
+    c = x.shape[-1]
+    if over == "token":
+        return x.numel() // c, 1, c
+    n = x.shape[0] if x.dim() > 1 else 1
+    return n, (x.numel() // (n * c) if n else 0), c
+
+
+def _forward(x, weight, bias, gate, groups, eps, act, over):
+    n, length, c = _shape(x, over)
+    lib = _lib.load()
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    code = _DTYPES[x.dtype]
+    w_code = code if weight is None and bias is None else _DTYPES[(bias if weight is None
+                                                                   else weight).dtype]
+    need = lib.prnn_group_norm_workspace_size(n, length, c, groups, code, 0)
+    ws = stats = None
+    if need:  # statistics per sample, or groups too wide for a wave
+        ws = _workspace(need, x.device)
+        stats = torch.empty(n, groups, 2, dtype=torch.float32, device=x.device)
+    with _on(x.device):
+        rc = lib.prnn_group_norm(
+            x.data_ptr(), _ptr(weight), _ptr(bias), _ptr(gate), y.data_ptr(), _ptr(stats), n,
+            length, c, groups, eps, act, w_code, code, _ptr(ws), need, _stream(x.device))
+    _lib.check(rc, "group_norm")
+    return y, stats
+
+
+class _GroupNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, gate, groups, eps, act, over):
+        y, stats = _forward(x, weight, bias, gate, groups, eps, act, over)
+        ctx.save_for_backward(x, weight, bias, gate, stats)
+        ctx.args = (groups, eps, act, over)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        x, weight, bias, gate, stats = ctx.saved_tensors
+        groups, eps, act, over = ctx.args
+        n, length, c = _shape(x, over)
+        lib, dev = _lib.load(), x.device
+        if gy.dtype != x.dtype:
+            gy = gy.to(x.dtype)
+        gy = gy.contiguous()
+        if gy.data_ptr() % 16:
+            gy = gy.clone()
+        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        dgate = None if gate is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
+        dw = None if weight is None else torch.empty_like(weight)
+        db = None if bias is None else torch.empty_like(bias)
+        code = _DTYPES[x.dtype]
+        w_code = code if weight is None and bias is None else _DTYPES[(bias if weight is None
+                                                                       else weight).dtype]
+        need = lib.prnn_group_norm_workspace_size(n, length, c, groups, code, 1)
+        ws = _workspace(need, dev)
+        with _on(dev):
+            rc = lib.prnn_group_norm_backward(
+                gy.data_ptr(), x.data_ptr(), _ptr(weight), _ptr(bias), _ptr(gate), _ptr(stats),
+                dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(dgate), n, length, c, groups, eps, act,
+                w_code, code, ws.data_ptr(), ws.numel(), _stream(dev))
+        _lib.check(rc, "group_norm backward")
+        need_in = ctx.needs_input_grad
+        return (dx if need_in[0] else None, dw, db, dgate, None, None, None, None)
+
+
+def group_norm(x: Tensor, num_groups: int, weight: Tensor | None = None,
+               bias: Tensor | None = None, *, gate: Tensor | None = None,
+               activation: str | None = None, over: str = "token", eps: float = 1e-5) -> Tensor:
+    """Group norm of ``x`` ``(..., C)``, channels last, in ``x``'s type.
+
+    ``num_groups`` divides ``C``.  ``weight`` and ``bias`` ``(C,)``: float32 or ``x``'s type (ones
+    and zeros without).  ``activation``: ``None``, ``"silu"`` or ``"sigmoid"``, applied to the
+    normalised values, or, where ``gate`` (like ``x``) is given, to the gate that multiplies them.
+    ``over``: ``"token"`` or ``"sample"`` (``x`` ``(N, ..., C)``).  Differentiable in all tensors.
+    """
+    what = "group_norm"
+    _validate(what, x, gate)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"{what}: x must be (..., C), got {tuple(x.shape)}")
+    c = x.shape[-1]
+    if num_groups < 1 or c % num_groups:
+        raise ValueError(f"{what}: {num_groups} groups do not divide C={c}")
+    if gate is not None and gate.shape != x.shape:
+        raise ValueError(f"{what}: gate {tuple(gate.shape)} != x {tuple(x.shape)}")
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"{what}: activation must be None, 'silu' or 'sigmoid', got "
+                         f"{activation!r}")
+    if over not in ("token", "sample"):
+        raise ValueError(f"{what}: over must be 'token' or 'sample', got {over!r}")
+    if not eps >= 0:
+        raise ValueError(f"{what}: eps must be >= 0, got {eps!r}")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        if t.device != x.device:
+            raise RuntimeError(f"{what}: tensors on different devices ({t.device} vs {x.device})")
+        if t.dtype != x.dtype and t.dtype != torch.float32:
+            raise TypeError(f"{what}: {name} must be float32 or {x.dtype}, got {t.dtype}")
+        if t.shape != (c,):
+            raise ValueError(f"{what}: {name} shape {tuple(t.shape)} != {(c,)}")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise TypeError(f"{what}: dtype mismatch {weight.dtype} vs {bias.dtype}")
+    if x.numel() // c >= 1 << 31:
+        raise ValueError(f"{what}: x has {x.numel() // c} tokens, more than 2^31 - 1")
+
+    def flat(t):
+        # as the kernels read it: contiguous, from a 16-byte boundary
+        if t is None:
+            return None
+        t = t.contiguous()
+        return t.clone() if t.data_ptr() % 16 else t
+
+    x, gate = flat(x), flat(gate)
+    weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
+    act = _ACTIVATIONS[activation]
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (x, weight, bias, gate)):
+        return _GroupNorm.apply(x, weight, bias, gate, int(num_groups), float(eps), act, over)
+    return _forward(x, weight, bias, gate, int(num_groups), float(eps), act, over)[0]

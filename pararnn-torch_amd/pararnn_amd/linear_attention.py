@@ -1,0 +1,345 @@
+"""Linear attention with a decay per head: whole sequences, their gradients, single tokens.
+
+For every head, with a state ``S`` ``(Dk, Dv)`` held in float32 and a log decay ``g_t``:
+
+    S_t = exp(g_t) S_{t-1} + k_t v_t^T,        o_t = scale q_t^T S_t.
+
+``linear_attention`` runs prompts and training sequences in the chunked form (matrix products
+inside a chunk, the state from chunk to chunk), ``linear_attention_step`` one token per session
+on a state or a pool of states, in place.  Both keep the state in the same layout, so a prompt's
+final state is what decoding goes on from; it lies next to the recurrent cells' states in a
+serving program and is paged in the same way (``block_table``).
+
+Layouts: ``q`` ``(B, T, Hq, Dk)``, ``k`` ``(B, T, Hk, Dk)``, ``v`` ``(B, T, Hv, Dv)`` with any
+strides whose last one is 1 (views of one fused projection are read as they are).  ``H`` is the
+largest of the head counts and of the decay's; each count divides it, and consecutive heads share
+an array that has fewer.  Widths up to 256.  float32, bfloat16 and float16; arithmetic and states
+are float32 (bfloat16 products take bfloat16 operands, see the kernels), results are rounded
+once.  Results do not depend on the order in which workgroups run: no atomics.
+"""
+
+from __future__ import annotations
+
+import contextlib
+import ctypes
+
+import torch
+from torch import Tensor
+
+from pararnn_amd import _lib
+from pararnn_amd.ops import _DTYPES, _ptr, _stream, _validate, _workspace
+from pararnn_amd.ragged import PackedSequences
+
+
+def _on(dev: torch.device):
+    """Makes ``dev`` the current device where it is not."""
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
+
+
+def _rows(t: Tensor) -> Tensor:
+    """``t`` with its heads' values side by side."""
+    return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _view(t: Tensor) -> _lib.LaView:
+    return _lib.LaView(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2), t.shape[2])
+
+
+def _heads(what: str, *counts: int) -> int:
+    h = max(counts)
+    for n in counts:
+        if n < 1 or h % n:
+            raise ValueError(f"{what}: head counts {counts} do not divide {h}")
+    return h
+
+
+def _decay_code(what: str, g: Tensor, q: Tensor) -> int:
+    if g.device != q.device:
+        raise RuntimeError(f"{what}: tensors on different devices ({g.device} vs {q.device})")
+    if g.dtype != q.dtype and g.dtype != torch.float32:
+        raise TypeError(f"{what}: log_decay must be float32 or {q.dtype}, got {g.dtype}")
+    return _DTYPES[g.dtype]
+
+
+def _check_state(what: str, name: str, t: Tensor, q: Tensor, tail: tuple[int, ...],
+                 rows: int | None) -> None:
+    if t.device != q.device:
+        raise RuntimeError(f"{what}: tensors on different devices ({t.device} vs {q.device})")
+    if t.dtype != torch.float32:
+        raise TypeError(f"{what}: {name} must be float32, got {t.dtype}")
+    if t.dim() != 4 or tuple(t.shape[1:]) != tail or (rows is not None and t.shape[0] != rows):
+        want = ("C" if rows is None else rows, *tail)
+        raise ValueError(f"{what}: {name} shape {tuple(t.shape)} != {want}")
+
+
+def _check_table(what: str, table: Tensor, rows: int, dev: torch.device) -> Tensor:
+    if table.dim() != 1 or table.numel() != rows:
+        raise ValueError(f"{what}: block_table must be ({rows},), got {tuple(table.shape)}")
+    if table.dtype == torch.int32 and table.device == dev and table.is_contiguous():
+        return table
+    if table.is_floating_point() or table.is_complex():
+        raise TypeError(f"{what}: block_table must be whole numbers, got {table.dtype}")
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{what} under graph capture needs a contiguous int32 block_table on "
+                           "the state's device")
+    return table.to(device=dev, dtype=torch.int32).contiguous()
+
+
+class _Problem:
+    """A checked call: the C problem and the tensors that it points to."""
+
+    def __init__(self, q: Tensor, k: Tensor, v: Tensor, g: Tensor, h0: Tensor | None,
+                 table: Tensor | None, packed: PackedSequences | None, scale: float | None):
+        what = "linear_attention"
+        code = _validate(what, q, k, v)
+        for n, t in (("q", q), ("k", k), ("v", v)):
+            if t.dim() != 4:
+                raise ValueError(f"{what}: {n} must be (B, T, heads, width), got "
+                                 f"{tuple(t.shape)}")
+        batch, time = q.shape[:2]
+        if k.shape[:2] != (batch, time) or v.shape[:2] != (batch, time):
+            raise ValueError(f"{what}: q, k and v disagree on (B, T): {tuple(q.shape[:2])}, "
+                             f"{tuple(k.shape[:2])}, {tuple(v.shape[:2])}")
+        if q.shape[3] != k.shape[3]:
+            raise ValueError(f"{what}: q has width {q.shape[3]}, k {k.shape[3]}")
+        g_code = _decay_code(what, g, q)
+        if g.dim() not in (1, 3) or (g.dim() == 3 and g.shape[:2] != (batch, time)):
+            raise ValueError(f"{what}: log_decay must be (H,) or (B, T, H), got "
+                             f"{tuple(g.shape)}")
+        heads = _heads(what, q.shape[2], k.shape[2], v.shape[2])
+        if g.shape[-1] != heads:
+            if g.shape[-1] % heads:
+                raise ValueError(f"{what}: log_decay has {g.shape[-1]} heads, q, k and v have "
+                                 f"{heads}")
+            heads = _heads(what, q.shape[2], k.shape[2], v.shape[2], g.shape[-1])
+        self.q, self.k, self.v, self.g = _rows(q), _rows(k), _rows(v), g
+        dk, dv = q.shape[3], v.shape[3]
+        if not 1 <= dk <= 256 or not 1 <= dv <= 256:
+            raise ValueError(f"{what}: head widths ({dk}, {dv}) are not in 1 .. 256")
+        self.dims = (batch, time, heads, dk, dv)
+        self.sequences = batch
+        self.offsets = None
+        if packed is not None:
+            if batch != 1:
+                raise ValueError(f"{what}: cu_seqlens packs q with batch=1, got batch={batch}")
+            if packed.tokens != time:
+                raise ValueError(f"cu_seqlens[-1] must equal time={time}, got {packed.tokens}")
+            self.sequences = packed.sequences
+            self.offsets = packed.offsets(q.device)
+        self.table = None
+        if table is not None:
+            if h0 is None:
+                raise ValueError("block_table needs h0 as a pool (C, ...)")
+            self.table = _check_table(what, table, self.sequences, q.device)
+        self.h0 = None
+        if h0 is not None:
+            _check_state(what, "h0", h0, q, (heads, dk, dv),
+                         None if table is not None else self.sequences)
+            self.h0 = h0.contiguous()
+        self.scale = float(dk ** -0.5 if scale is None else scale)
+        at = g.stride() if g.dim() == 3 else (0, 0, g.stride(0))
+        if g.dim() == 3 and time * batch > 0 and at[0] == 0 and at[1] == 0:
+            self.g = g.contiguous()  # expanded, not per head: the gradient's layout tells them apart
+            at = self.g.stride()
+        self.c = _lib.LaProblem(
+            _view(self.q), _view(self.k), _view(self.v), self.g.data_ptr(), *at,
+            None if self.h0 is None else self.h0.data_ptr(),
+            None if self.table is None else self.table.data_ptr(),
+            None if self.offsets is None else self.offsets.data_ptr(),
+            0 if self.h0 is None else self.h0.shape[0],
+            0 if packed is None else self.sequences, batch, time, heads, dk, dv, g_code, code,
+            self.scale)
+
+
+def _forward(p: _Problem, state_out: Tensor | None, table: Tensor | None) -> Tensor:
+    batch, time, heads, _, dv = p.dims
+    lib, dev = _lib.load(), p.q.device
+    out = p.q.new_empty(batch, time, heads, dv)
+    with _on(dev):
+        need = lib.prnn_linear_attention_workspace_size(ctypes.byref(p.c))
+        ws = _workspace(need, dev) if need else None
+        view = _view(out)
+        rc = lib.prnn_linear_attention(
+            ctypes.byref(p.c), ctypes.byref(view), _ptr(state_out), _ptr(table),
+            0 if state_out is None else state_out.shape[0], _ptr(ws), need, _stream(dev))
+    _lib.check(rc, "linear_attention")
+    return out
+
+
+def _backward(p: _Problem, go: Tensor, gs: Tensor | None, need_g: bool, need_h0: bool):
+    lib, dev = _lib.load(), p.q.device
+    go = _rows(go)
+    gs = None if gs is None else gs.contiguous()
+    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (p.q, p.k, p.v))
+    dg = torch.empty(p.g.shape, dtype=p.g.dtype, device=dev) if need_g else None
+    dh0 = None
+    if p.h0 is not None and (need_g or need_h0):
+        dh0 = torch.empty_like(p.h0)
+    with _on(dev):
+        need = lib.prnn_linear_attention_backward_workspace_size(ctypes.byref(p.c), int(need_g))
+        ws = _workspace(need, dev) if need else None
+        view = _view(go)
+        rc = lib.prnn_linear_attention_backward(
+            ctypes.byref(p.c), ctypes.byref(view), _ptr(gs), _ptr(dq), _ptr(dk), _ptr(dv),
+            _ptr(dg), _ptr(dh0), _ptr(ws), need, _stream(dev))
+    _lib.check(rc, "linear_attention backward")
+    return dq, dk, dv, dg, dh0
+
+
+class _LinearAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, g, h0, packed, scale, want_state):
+        p = _Problem(q, k, v, g, h0, None, packed, scale)
+        _, _, heads, dk, dv = p.dims
+        state = q.new_empty(p.sequences, heads, dk, dv, dtype=torch.float32) if want_state else None
+        out = _forward(p, state, None)
+        ctx.save_for_backward(q, k, v, g, h0)
+        ctx.packed, ctx.scale = packed, scale
+        ctx.set_materialize_grads(False)
+        return out, state
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, go, gs):
+        q, k, v, g, h0 = ctx.saved_tensors
+        if go is None and gs is None:
+            return (None,) * 8
+        p = _Problem(q, k, v, g, h0, None, ctx.packed, ctx.scale)
+        if go is None:
+            go = q.new_zeros(1).expand(*p.dims[:3], p.dims[4])
+        if go.dtype != q.dtype:
+            go = go.to(q.dtype)
+        need = ctx.needs_input_grad
+        dq, dk, dv, dg, dh0 = _backward(p, go, gs, need[3], need[4])
+        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dg,
+                dh0 if need[4] else None, None, None, None)
+
+
+def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, *,
+                     scale: float | None = None, h0: Tensor | None = None,
+                     cu_seqlens: Tensor | PackedSequences | None = None,
+                     block_table: Tensor | None = None, state_out: Tensor | None = None,
+                     return_state: bool = False) -> Tensor | tuple[Tensor, Tensor]:
+    """Linear attention over whole sequences; ``(B, T, H, Dv)`` in ``q``'s type.
+
+    ``log_decay``: ``(H,)``, fixed per head, or ``(B, T, H)``, per token; at most zero in use
+    (``-inf`` forgets the state), float32 or ``q``'s type.  ``scale`` defaults to ``Dk ** -0.5``.
+    ``h0`` ``(B, H, Dk, Dv)`` float32: the states to go on from (zeros without).
+
+    ``cu_seqlens`` packs ``S`` sequences into ``(1, N, ...)``; every one starts from its own
+    ``h0`` row.  A tensor is checked at each call (a copy from the device); a
+    :class:`PackedSequences` was checked when it was made.
+
+    ``return_state=True`` also returns the final states ``(sequences, H, Dk, Dv)``.  Gradients of
+    the output and of the returned states flow to ``q``, ``k``, ``v``, ``log_decay`` and ``h0``.
+
+    Serving: with ``block_table`` ``(sequences,)`` ``h0`` is a pool ``(C, H, Dk, Dv)`` and
+    sequence ``s`` starts from row ``block_table[s]`` (a negative entry: from zeros).
+    ``state_out`` takes the final states: ``(sequences, H, Dk, Dv)``, or with a block table a pool
+    whose named rows are overwritten (``h0`` itself is allowed: no two sequences may then name
+    one row).  Neither has a gradient.
+    """
+    packed = cu_seqlens
+    if packed is not None and not isinstance(packed, PackedSequences):
+        packed = PackedSequences(packed)
+    grads = torch.is_grad_enabled() and any(
+        t is not None and t.requires_grad for t in (q, k, v, log_decay, h0))
+    if grads and block_table is None and state_out is None:
+        out, state = _LinearAttention.apply(q, k, v, log_decay, h0, packed, scale, return_state)
+        return (out, state) if return_state else out
+    if grads:
+        raise RuntimeError("linear_attention: block_table and state_out are inference-only; call "
+                           "it under torch.no_grad()")
+    p = _Problem(q, k, v, log_decay, h0, block_table, packed, scale)
+    _, _, heads, dk, dv = p.dims
+    dest, table = None, None
+    if state_out is not None:
+        if return_state:
+            raise ValueError("linear_attention: state_out and return_state exclude each other")
+        _check_state("linear_attention", "state_out", state_out, q, (heads, dk, dv),
+                     p.sequences if p.table is None else None)
+        if not state_out.is_contiguous():
+            raise ValueError("linear_attention: state_out must be contiguous")
+        dest, table = state_out, p.table
+    elif return_state:
+        dest = q.new_empty(p.sequences, heads, dk, dv, dtype=torch.float32)
+    out = _forward(p, dest, table)
+    return (out, dest) if return_state else out
+
+
+def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, state: Tensor, *,
+                          scale: float | None = None, block_table: Tensor | None = None,
+                          out: Tensor | None = None) -> Tensor:
+    """One token for every row; ``state`` ``(B, H, Dk, Dv)`` float32 advances in place.
+
+    ``q`` ``(B, Hq, Dk)``, ``k`` ``(B, Hk, Dk)``, ``v`` ``(B, Hv, Dv)`` (a time axis of 1 after
+    ``B`` is allowed on all of them), ``log_decay`` ``(H,)`` or ``(B, H)``.  Returns
+    ``(B, H, Dv)`` in ``q``'s type (with the time axis if ``q`` has it), in ``out`` where given.
+    With ``block_table`` ``(B,)`` ``state`` is a pool ``(C, H, Dk, Dv)`` and row ``b`` works on
+    slot ``block_table[b]``; a slot outside the pool (-1) is an idle row: it starts from zeros and
+    nothing is kept.  No two rows may name one slot.  No autograd.  With contiguous operands and
+    ``out=`` it allocates nothing and can be captured in a HIP graph.
+    """
+    what = "linear_attention_step"
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                    or log_decay.requires_grad or state.requires_grad):
+        raise RuntimeError(f"{what} has no autograd; call it under torch.no_grad()")
+    timed = q.dim() == 4
+    if timed:
+        if q.shape[1] != 1 or k.dim() != 4 or k.shape[1] != 1 or v.dim() != 4 or v.shape[1] != 1:
+            raise ValueError(f"{what} takes one token per row, got q {tuple(q.shape)}")
+        q, k, v = q[:, 0], k[:, 0], v[:, 0]
+        if log_decay.dim() == 3:
+            if log_decay.shape[1] != 1:
+                raise ValueError(f"{what}: log_decay must be (H,) or (B, H), got "
+                                 f"{tuple(log_decay.shape)}")
+            log_decay = log_decay[:, 0]
+    code = _validate(what, q, k, v)
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise ValueError(f"{what}: q, k and v must be (B, heads, width), got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)}, {tuple(v.shape)}")
+    (batch, hq, dk), (bk, hk, dk2), (bv, hv, dv) = q.shape, k.shape, v.shape
+    if bk != batch or bv != batch or dk2 != dk:
+        raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)} and v "
+                         f"{tuple(v.shape)} do not fit")
+    g_code = _decay_code(what, log_decay, q)
+    heads = log_decay.shape[-1] if log_decay.dim() else 0
+    if _heads(what, hq, hk, hv, heads) != heads:
+        raise ValueError(f"{what}: log_decay has {heads} heads, q, k and v have "
+                         f"{max(hq, hk, hv)}")
+    if log_decay.dim() == 1:
+        g_sb, g_sh = 0, log_decay.stride(0)
+    elif log_decay.dim() == 2 and log_decay.shape[0] == batch:
+        g_sb, g_sh = log_decay.stride()
+    else:
+        raise ValueError(f"{what}: log_decay must be (H,) or (B, H), got "
+                         f"{tuple(log_decay.shape)}")
+    dev = q.device
+    _check_state(what, "state", state, q, (heads, dk, dv), None if block_table is not None
+                 else batch)
+    if not state.is_contiguous():
+        raise ValueError(f"{what}: state must be contiguous (it is advanced in place)")
+    table = None if block_table is None else _check_table(what, block_table, batch, dev)
+    q, k, v = _rows(q), _rows(k), _rows(v)
+    if out is None:
+        res = q.new_empty(batch, heads, dv)
+    else:
+        if out.shape != ((batch, 1, heads, dv) if timed else (batch, heads, dv)):
+            raise ValueError(f"{what}: out {tuple(out.shape)} != {(batch, heads, dv)}")
+        if out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
+            raise ValueError(f"{what}: out must be contiguous, of q's type and on its device")
+        res = out
+    lib = _lib.load()
+    with _on(dev):
+        rc = lib.prnn_linear_attention_step(
+            q.data_ptr(), q.stride(0), q.stride(1), hq, k.data_ptr(), k.stride(0), k.stride(1),
+            hk, v.data_ptr(), v.stride(0), v.stride(1), hv, log_decay.data_ptr(), g_sb, g_sh,
+            g_code, state.data_ptr(), None if table is None else table.data_ptr(),
+            state.shape[0], res.data_ptr(), batch, heads, dk, dv,
+            dk ** -0.5 if scale is None else scale, code, _stream(dev))
+    _lib.check(rc, what)
+    if out is not None:
+        return out
+    return res[:, None] if timed else res

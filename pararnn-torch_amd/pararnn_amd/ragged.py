@@ -84,6 +84,39 @@ def validate_cu_seqlens(cu_seqlens: Tensor, time: int,
     return cs
 
 
+class PackedSequences:
+    """The offsets of a packed batch, checked once: what a program makes of a batch's
+    ``cu_seqlens`` and hands to every layer and step that runs on it, so that none of them has
+    to copy the offsets from the device to look at them.
+
+    ``cu_seqlens`` ``(S+1,)``: ``[0] = 0``, none below the one before it (a sequence may be
+    empty); on the host or on a GPU.  The handle keeps int32 copies on the devices that used it.
+    """
+
+    def __init__(self, cu_seqlens: Tensor):
+        if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2:
+            raise ValueError(f"cu_seqlens must be (S+1,), got {tuple(cu_seqlens.shape)}")
+        if cu_seqlens.is_floating_point() or cu_seqlens.is_complex():
+            raise TypeError(f"cu_seqlens must be whole numbers, got {cu_seqlens.dtype}")
+        host = cu_seqlens.detach().to("cpu", torch.long)
+        if int(host[0]) != 0:
+            raise ValueError(f"cu_seqlens[0] must be 0, got {int(host[0])}")
+        if bool((host[1:] < host[:-1]).any()):
+            raise ValueError("cu_seqlens must not decrease")
+        if int(host[-1]) >= 1 << 30:
+            raise ValueError(f"a packed batch holds fewer than 2^30 tokens, got {int(host[-1])}")
+        self.sequences = int(host.numel()) - 1
+        self.tokens = int(host[-1])
+        self._on = {torch.device("cpu"): host.to(torch.int32)}
+
+    def offsets(self, device: torch.device) -> Tensor:
+        """The int32 offsets on ``device``."""
+        got = self._on.get(device)
+        if got is None:
+            got = self._on[device] = self._on[torch.device("cpu")].to(device)
+        return got
+
+
 def longest_sequence(cs: Tensor, time: int) -> int:
     """Length of the longest sequence of checked offsets (no copy from the
     device when they are the last ones checked)."""

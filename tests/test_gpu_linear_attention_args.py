@@ -1,0 +1,125 @@
+"""Refusals of the linear-attention layer's operators on GPU tensors: each before any launch."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+
+
+def _t(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype, device=DEV)
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(q=lambda: _t(1, 6, 2)), ValueError),
+    (dict(k=lambda: _t(1, 5, 2, 8)), ValueError),
+    (dict(k=lambda: _t(1, 6, 2, 9)), ValueError),
+    (dict(k=lambda: _t(1, 6, 3, 8)), ValueError),
+    (dict(v=lambda: _t(1, 6, 2, 300)), ValueError),
+    (dict(v=lambda: _t(1, 6, 2, 8, dtype=torch.bfloat16)), TypeError),
+    (dict(q=lambda: _t(1, 6, 2, 8, dtype=torch.float64)), TypeError),
+    (dict(g=lambda: _t(1, 6, 2, dtype=torch.bfloat16)), TypeError),
+    (dict(g=lambda: _t(1, 7, 2)), ValueError),
+    (dict(g=lambda: _t(3)), ValueError),
+    (dict(g=lambda: torch.zeros(2)), RuntimeError),
+    (dict(h0=lambda: _t(2, 2, 8, 8)), ValueError),
+    (dict(h0=lambda: _t(1, 2, 8, 8, dtype=torch.bfloat16)), TypeError),
+    (dict(cu_seqlens=lambda: torch.tensor([0, 5])), ValueError),
+    (dict(cu_seqlens=lambda: torch.tensor([0, 4, 3, 6])), ValueError),
+    (dict(block_table=lambda: torch.tensor([0])), ValueError),
+    (dict(h0=lambda: _t(4, 2, 8, 8), block_table=lambda: torch.tensor([0, 1])), ValueError),
+    (dict(h0=lambda: _t(4, 2, 8, 8), block_table=lambda: torch.tensor([0.0])), TypeError),
+    (dict(state_out=lambda: _t(1, 2, 8, 9)), ValueError),
+    (dict(state_out=lambda: _t(1, 2, 8, 16)[..., ::2]), ValueError),
+])
+def test_linear_attention_refuses(change, error):
+    from pararnn_amd import linear_attention
+
+    args = dict(q=_t(1, 6, 2, 8), k=_t(1, 6, 2, 8), v=_t(1, 6, 2, 8), g=_t(1, 6, 2))
+    args.update({n: f() for n, f in change.items()})
+    first = [args.pop(n) for n in "qkvg"]
+    with pytest.raises(error):
+        linear_attention(*first, **args)
+
+
+def test_linear_attention_refuses_gradients_where_there_are_none():
+    from pararnn_amd import linear_attention, linear_attention_step
+
+    q = _t(1, 6, 2, 8).requires_grad_(True)
+    with pytest.raises(RuntimeError, match="inference"):
+        linear_attention(q, q, q, _t(2), h0=_t(3, 2, 8, 8), block_table=torch.tensor([1]))
+    with pytest.raises(RuntimeError, match="autograd"):
+        linear_attention_step(q[:, 0], q[:, 0], q[:, 0], _t(2), _t(1, 2, 8, 8))
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(q=lambda: _t(2, 2, 2, 8)), ValueError),
+    (dict(k=lambda: _t(3, 2, 8)), ValueError),
+    (dict(v=lambda: _t(2, 3, 8)), ValueError),
+    (dict(g=lambda: _t(2, 3)), ValueError),
+    (dict(g=lambda: _t(3, 2)), ValueError),
+    (dict(state=lambda: _t(1, 2, 8, 8)), ValueError),
+    (dict(state=lambda: _t(2, 2, 8, 8, dtype=torch.bfloat16)), TypeError),
+    (dict(state=lambda: _t(2, 2, 8, 16)[..., ::2]), ValueError),
+    (dict(block_table=lambda: torch.tensor([0, 1, 2])), ValueError),
+    (dict(out=lambda: _t(2, 2, 9)), ValueError),
+    (dict(out=lambda: _t(2, 2, 8, dtype=torch.bfloat16)), ValueError),
+])
+def test_step_refuses(change, error):
+    from pararnn_amd import linear_attention_step
+
+    args = dict(q=_t(2, 2, 8), k=_t(2, 2, 8), v=_t(2, 2, 8), g=_t(2, 2), state=_t(2, 2, 8, 8))
+    args.update({n: f() for n, f in change.items()})
+    first = [args.pop(n) for n in ("q", "k", "v", "g", "state")]
+    with pytest.raises(error):
+        linear_attention_step(*first, **args)
+
+
+@pytest.mark.parametrize("kw,error", [
+    (dict(num_groups=3), ValueError), (dict(num_groups=0), ValueError),
+    (dict(weight=lambda: _t(7)), ValueError),
+    (dict(weight=lambda: _t(8, dtype=torch.bfloat16)), TypeError),
+    (dict(weight=lambda: torch.zeros(8)), RuntimeError),
+    (dict(gate=lambda: _t(4, 7)), ValueError),
+    (dict(gate=lambda: _t(4, 8, dtype=torch.bfloat16)), TypeError),
+    (dict(activation="relu"), ValueError), (dict(over="time"), ValueError),
+    (dict(eps=-1.0), ValueError),
+])
+def test_group_norm_refuses(kw, error):
+    from pararnn_amd import group_norm
+
+    kw = {n: f() if callable(f) else f for n, f in kw.items()}
+    with pytest.raises(error):
+        group_norm(_t(4, 8), kw.pop("num_groups", 2), **kw)
+
+
+def test_pages_refuse():
+    from pararnn_amd import compact_pages, copy_pages, fork_pages, free_pages, take_pages
+
+    used, pool = _t(4, dtype=torch.int32), _t(4, 3)
+    with pytest.raises(TypeError):
+        take_pages(_t(4), 1)
+    with pytest.raises(ValueError):
+        take_pages(used, -1)
+    with pytest.raises(ValueError):
+        take_pages(_t(8, dtype=torch.int32)[::2], 1)
+    with pytest.raises(ValueError):
+        fork_pages(used, [pool, _t(5, 3)], torch.tensor([0]))
+    with pytest.raises(TypeError):
+        fork_pages(used, pool, torch.tensor([0.0]))
+    with pytest.raises(ValueError):
+        fork_pages(used, _t(4, 6)[:, ::2], torch.tensor([0]))
+    with pytest.raises(ValueError):
+        free_pages(used, torch.tensor([[0]]))
+    with pytest.raises(ValueError):
+        copy_pages(pool, torch.tensor([0]), torch.tensor([1, 2]))
+    with pytest.raises(ValueError):
+        copy_pages([], torch.tensor([0]), torch.tensor([1]))
+    with pytest.raises(TypeError):
+        compact_pages(used, pool, [_t(3, dtype=torch.int64)])
+    with pytest.raises(ValueError):
+        compact_pages(used, pool, [_t(6, dtype=torch.int32)[::2]])
+    with pytest.raises(RuntimeError):
+        compact_pages(used, pool, [torch.zeros(3, dtype=torch.int32)])
