@@ -205,5 +205,9 @@ inline int la_widest(const LaParams& p, int roles) {
 // states.  *_tile_cols: columns of z that a workgroup takes where the widest role has vd.
 int la_walk_f32(LaParams p, int roles, bool state_only, int dtype, hipStream_t stream);
 int la_f32_tile_cols(int vd);
+// bf16 storage with widths in multiples of 8 and rows that admit 16-byte accesses (x, y, z, dot)
+// or 8-byte ones (out).
+int la_walk_bf16(LaParams p, int roles, bool state_only, bool fine, hipStream_t stream);
+int la_bf16_tile_cols(int vd);
 
 }  // namespace prnn

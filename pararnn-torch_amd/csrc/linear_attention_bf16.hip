@@ -1,0 +1,483 @@
+// Decayed linear attention, the walk for bf16 storage on v_mfma_f32_32x32x16_bf16: chunks of 64
+// tokens, 32 columns of the state per wave.
+//
+// Everything is formed transposed, so that what one product leaves in registers is the next one's
+// operand as it is.  The instruction's result has lane l hold column l % 32 and rows
+// 8 b + 4 (l / 32) + r; its operands have lane l hold row (or column) l % 32 and 8 places of the
+// contraction.  The order of a contraction is free, so a lane's 8 places are the rows
+// {4 (l / 32) + r, 8 + 4 (l / 32) + r} of 16:
+//   pairs^T = y x^T    (a tile per wave, handed round through LDS as whole operands)
+//   out^T   = S^T x^T + z^T pairs^T
+//   S      <- tot S + y^T (w z)
+// x lies in LDS with its columns in that order (one 16-byte read per operand), y and z as they
+// come, read across tokens by the transposing LDS load.
+//
+// Roundings to bf16: the pairs' weights and the state where they are operands (S itself stays
+// fp32); what enters the state, w z, is split into three bf16 parts, 24 bits: the state is an
+// fp32 result.  FINE splits the weights and the state into two parts as well (16 bits), for the
+// backward pass, where the decays' gradient adds up differences of the results.
+#include "linear_attention.h"
+
+namespace prnn {
+namespace {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s4 lds_s4;
+
+constexpr int kC = 64;  // tokens per chunk
+
+__device__ __forceinline__ f16v mfma(b8 a, b8 b, f16v c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// Bytes of an LDS row.  x and y are read 16 bytes a lane down 16 rows (an odd number of 16-byte
+// units lets them fall into different banks) and y and z 64 bytes along 4 rows (z: exactly 64
+// bytes apart; y's rows overlap by a quarter, a two-way conflict in those banks).
+constexpr int row_xy(int cols) { return cols >= 128 ? cols * 2 + 48 : cols * 2 + 16; }
+constexpr int row_z(int cols) { return cols == 32 ? 64 : cols * 2 + 64; }
+
+// Two transposing loads: this lane's column (c0 + lane % 32) at 8 tokens of the 16 from t0.
+// `at`: the tile with this lane's share of the address, across_share.
+template <int RB>
+__device__ __forceinline__ int across_share(int lane) {
+  const int i = lane & 15, g = lane >> 4;
+  return (4 * (g >> 1) + (i >> 2)) * RB + (16 * (g & 1) + 4 * (i & 3)) * 2;
+}
+template <int RB>
+__device__ __forceinline__ b8 load_across(const char* at, int t0, int c0) {
+  union {
+    s4 h[2];
+    b8 v;
+  } r;
+  r.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + t0 * RB + c0 * 2));
+  r.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + (t0 + 8) * RB + c0 * 2));
+  return r.v;
+}
+
+__device__ __forceinline__ b8 pack8(const float* x) {
+  union {
+    uint32_t w[4];
+    b8 v;
+  } r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.w[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+  return r.v;
+}
+// x as bf16, and what that leaves of it in x.
+__device__ __forceinline__ b8 split8(float* x) {
+  union {
+    uint32_t w[4];
+    b8 v;
+  } r;
+  r.v = pack8(x);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] -= lo_bf16(r.w[i]);
+    x[2 * i + 1] -= hi_bf16(r.w[i]);
+  }
+  return r.v;
+}
+
+template <int KD, int W, bool STATE_ONLY, bool FINE>
+__global__ __launch_bounds__(64 * W, (KD >= 256 || (W == 1 && KD >= 128)) ? 1 : 2)
+void la_walk_bf16_kernel(LaParams P) {
+  constexpr int NT = 64 * W, VT = 32 * W;
+  constexpr int UX = KD / 8, UZ = VT / 8;      // 16-byte units of a row
+  constexpr int NX = kC * UX / NT, NZ = kC * UZ / NT;
+  constexpr int KT = KD / 32;                  // 32-row tiles of the state
+  constexpr int RX = row_xy(KD), RZ = row_z(VT);
+  constexpr int KX = STATE_ONLY ? 0 : kC * RX;
+  constexpr int KP = STATE_ONLY ? 0 : 3 * 2 * 64 * 16 * (FINE ? 2 : 1);
+  __shared__ __align__(16) char sx[KX ? KX : 16];
+  __shared__ __align__(16) char sy[kC * RX];
+  __shared__ __align__(16) char sz[kC * RZ];
+  __shared__ __align__(16) char sp[KP ? KP : 16];
+  __shared__ __align__(16) float sG[kC], se[kC], sw[kC];
+  __shared__ float sdot[W][kC], s_tot, s_sum;
+  __shared__ int s_stop[2];
+
+  const LaRole& R = P.role[blockIdx.z];
+  const int h = blockIdx.y;
+  const int tile = blockIdx.x % P.tiles, piece = blockIdx.x / P.tiles;
+  if (tile * VT >= R.vd) return;
+  const LaPiece pc = la_piece(P.seqs, piece);
+  if (STATE_ONLY) {
+    // the piece that a walk ends with hands its state to none
+    if (pc.alone || (R.rev ? pc.first : pc.last)) return;
+  } else if (pc.begin >= pc.end && !pc.first) {
+    return;  // no piece (an empty sequence is one, it hands its state on)
+  }
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int l32 = lane & 31, half = lane >> 5;
+  const int b = la_batch(P.seqs, pc);
+  const int col0 = tile * VT;
+  const int col = col0 + 32 * wave + l32;  // this lane's column of the state
+  const size_t row_floats = static_cast<size_t>(P.H) * P.Dk * P.Dv;
+  const size_t head_floats = static_cast<size_t>(h) * P.Dk * P.Dv;
+
+  // ---- the state before the piece
+  f16v S[KT];
+#pragma unroll
+  for (int t = 0; t < KT; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) S[t][r] = 0.0f;
+  if (!STATE_ONLY) {
+    const float* src = nullptr;
+    if (R.piece_state && !pc.alone)
+      src = R.piece_state + static_cast<size_t>(piece) * row_floats + head_floats;
+    else if (const float* row = la_row(R.init, pc.seq, row_floats))
+      src = row + head_floats;
+    if (src && col < R.vd) {
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int i = 32 * t + 8 * (r >> 2) + 4 * half + (r & 3);
+          if (i < R.kd) S[t][r] = src[static_cast<size_t>(i) * R.sk + static_cast<size_t>(col) * R.sv];
+        }
+    }
+  }
+
+  const int n_tok = pc.end - pc.begin;
+  float sum_decay = 0.0f;
+  auto token = [&](int i) { return R.rev ? pc.end - 1 - i : pc.begin + i; };
+
+  // A thread's loads of an array are rows apart by a constant number: one pointer, which moves on
+  // by a chunk at a time.
+  constexpr int DX = NT / UX, DZ = NT / UZ;
+  const int rowx = tid / UX, cx = (tid % UX) * 8, rowz = tid / UZ, cz = col0 + (tid % UZ) * 8;
+  const long long dir = R.rev ? -1 : 1;
+  const long long stx = dir * R.x.st, sty = dir * R.y.st, stz = dir * R.z.st;
+  const bf16* px = static_cast<const bf16*>(R.x.p) + b * R.x.sb + (h / R.x.rep) * R.x.sh +
+                   token(rowx) * R.x.st + cx;
+  const bf16* py = static_cast<const bf16*>(R.y.p) + b * R.y.sb + (h / R.y.rep) * R.y.sh +
+                   token(rowx) * R.y.st + cx;
+  const bf16* pz = static_cast<const bf16*>(R.z.p) + b * R.z.sb + (h / R.z.rep) * R.z.sh +
+                   token(rowz) * R.z.st + cz;
+  auto move_on = [&](int by) {
+    if (!STATE_ONLY) px += by * stx;
+    py += by * sty;
+    pz += by * stz;
+  };
+  const bool inx = cx < R.kd, inz = cz < R.vd;
+  u4 rx[STATE_ONLY ? 1 : NX], ry[NX], rz[NZ];
+  float rg = 0.0f;
+  auto fetch = [&](int base) {
+#pragma unroll
+    for (int k = 0; k < NX; ++k) {
+      const bool in = inx && base + rowx + k * DX < n_tok;
+      if (!STATE_ONLY) {
+        rx[k] = u4{0, 0, 0, 0};
+        if (in) rx[k] = *reinterpret_cast<const u4*>(px + k * DX * stx);
+      }
+      ry[k] = u4{0, 0, 0, 0};
+      if (in) ry[k] = *reinterpret_cast<const u4*>(py + k * DX * sty);
+    }
+#pragma unroll
+    for (int k = 0; k < NZ; ++k) {
+      rz[k] = u4{0, 0, 0, 0};
+      if (inz && base + rowz + k * DZ < n_tok)
+        rz[k] = *reinterpret_cast<const u4*>(pz + k * DZ * stz);
+    }
+    move_on(kC);
+    rg = wave == 0 && base + lane < n_tok
+             ? la_step_decay(P.g, R.rev, pc, b, token(base + lane), h) : 0.0f;
+  };
+  // Decays of the chunk's first `n` tokens: running sums in fp64, so that what is left of the
+  // whole keeps its digits.
+  auto decays = [&](float g, int n) {
+    double G = lane < n ? g : 0.0f;
+#pragma unroll
+    for (int d = 1; d < kC; d <<= 1) {
+      const double o = __shfl_up(G, d);
+      if (lane >= d) G += o;
+    }
+    const double last = __shfl(G, kC - 1);
+    sG[lane] = static_cast<float>(G);
+    se[lane] = fexp(static_cast<float>(G)) * R.x_scale;
+    sw[lane] = fexp(static_cast<float>(last - G)) * R.u_scale;
+    if (lane == 0) {
+      s_tot = fexp(static_cast<float>(last));
+      s_sum = static_cast<float>(last);
+    }
+  };
+  if (tid < 2) s_stop[tid] = kC;
+  if (n_tok > 0) fetch(0);
+  __syncthreads();
+
+  int next = 0;
+  for (int base = 0, turn = 0; base < n_tok; base = next, turn ^= 1) {
+    // x: columns 0-3 | 8-11 and 4-7 | 12-15 of every 16 side by side
+    const int ox = rowx * RX + (tid % UX >> 1) * 32 + (tid & 1) * 8;
+#pragma unroll
+    for (int k = 0; k < NX; ++k) {
+      if (!STATE_ONLY) {
+        *reinterpret_cast<uint2*>(sx + ox + k * DX * RX) = uint2{rx[k][0], rx[k][1]};
+        *reinterpret_cast<uint2*>(sx + ox + 16 + k * DX * RX) = uint2{rx[k][2], rx[k][3]};
+      }
+      *reinterpret_cast<u4*>(sy + (rowx + k * DX) * RX + cx * 2) = ry[k];
+    }
+#pragma unroll
+    for (int k = 0; k < NZ; ++k) {
+      *reinterpret_cast<u4*>(sz + (rowz + k * DZ) * RZ + (tid % UZ) * 16) = rz[k];
+      // an exponent of ones: infinity or NaN
+      uint32_t bad = 0;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) bad |= (rz[k][q] & 0x7f807f80u) + 0x00800080u;
+      if ((bad & 0x80008000u) && rowz + k * DZ > 0) atomicMin(&s_stop[turn], rowz + k * DZ);
+    }
+    const float g_here = rg;
+    if (wave == 0) decays(rg, kC);
+    next = base + kC;
+    if (next < n_tok) fetch(next);
+    __syncthreads();
+    if (tid == 0) s_stop[turn ^ 1] = kC;
+    const int stop = s_stop[turn];
+    if (stop < kC) {
+      // A masked pair is an exact zero, but zero times an infinity or NaN of a later token is
+      // not: where z holds one behind the chunk's first token (rare), the chunk ends before it
+      // and the next one begins there.
+      for (int e = tid; e < (kC - stop) * (RX / 16); e += NT)
+        *reinterpret_cast<u4*>(sy + stop * RX + e * 16) = u4{0, 0, 0, 0};
+      for (int e = tid; e < (kC - stop) * (RZ / 16); e += NT)
+        *reinterpret_cast<u4*>(sz + stop * RZ + e * 16) = u4{0, 0, 0, 0};
+      if (wave == 0) decays(g_here, stop);
+      if (next < n_tok) move_on(-kC);
+      move_on(stop - kC);
+      next = base + stop;
+      if (next < n_tok) fetch(next);
+      __syncthreads();
+    }
+    const int n_here = min(n_tok, next) - base;  // tokens of this chunk
+
+    f16v O[2];
+    if (!STATE_ONLY) {
+      // ---- the chunk's pairs: tiles (out rows, earlier rows) (0,0), (1,0), (1,1)
+      for (int id = wave; id < 3; id += W) {
+        const int it = id > 0, jt = id > 1;
+        f16v acc;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
+        const int i = 32 * it + l32;
+        const char* yr = sy + (32 * jt + l32) * RX + 8 * half;
+        const char* xr = sx + i * RX + 16 * half;
+#pragma unroll
+        for (int k = 0; k < KD / 16; ++k) {
+          union {
+            uint2 h[2];
+            b8 v;
+          } y;
+          y.h[0] = *reinterpret_cast<const uint2*>(yr + 32 * k);
+          y.h[1] = *reinterpret_cast<const uint2*>(yr + 32 * k + 16);
+          acc = mfma(y.v, *reinterpret_cast<const b8*>(xr + 32 * k), acc);
+        }
+        const float Gi = sG[i];
+        float w[16];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int j0 = 32 * jt + 8 * q + 4 * half;
+          const f4 Gj = *reinterpret_cast<const f4*>(&sG[j0]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            w[4 * q + r] = j0 + r <= i ? acc[4 * q + r] * (R.p_scale * fexp(Gi - Gj[r])) : 0.0f;
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          b8* at = reinterpret_cast<b8*>(sp) + (id * 2 + s) * 64 + lane;
+          if (FINE) {
+            at[0] = split8(w + 8 * s);
+            at[3 * 2 * 64] = pack8(w + 8 * s);
+          } else {
+            at[0] = pack8(w + 8 * s);
+          }
+        }
+      }
+      // ---- the state's part of the output
+#pragma unroll
+      for (int it = 0; it < 2; ++it)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) O[it][r] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < KD / 16; ++k) {
+        float x[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) x[q] = S[k / 2][8 * (k & 1) + q];
+        const b8 s0 = FINE ? split8(x) : pack8(x);
+        const b8 s1 = FINE ? pack8(x) : s0;
+#pragma unroll
+        for (int it = 0; it < 2; ++it) {
+          const b8 xr = *reinterpret_cast<const b8*>(sx + (32 * it + l32) * RX + 16 * half + 32 * k);
+          O[it] = mfma(s0, xr, O[it]);
+          if (FINE) O[it] = mfma(s1, xr, O[it]);
+        }
+      }
+#pragma unroll
+      for (int it = 0; it < 2; ++it) {
+        const float e = se[32 * it + l32];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) O[it][r] *= e;
+      }
+      __syncthreads();
+    }
+
+    union Z8 {
+      uint32_t w[4];
+      b8 v;
+    };
+    Z8 zf[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) zf[t].v = load_across<RZ>(sz + wave * 64 + across_share<RZ>(lane), 16 * t, 0);
+
+    if (!STATE_ONLY) {
+      // ---- the chunk's own part
+      auto pairs = [&](int id, int s, int lo) {
+        return reinterpret_cast<const b8*>(sp)[((lo * 3 + id) * 2 + s) * 64 + lane];
+      };
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        O[1] = mfma(zf[s].v, pairs(1, s, 0), O[1]);
+        if (FINE) O[1] = mfma(zf[s].v, pairs(1, s, 1), O[1]);
+      }
+#pragma unroll
+      for (int it = 0; it < 2; ++it)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          O[it] = mfma(zf[2 * it + s].v, pairs(2 * it, s, 0), O[it]);
+          if (FINE) O[it] = mfma(zf[2 * it + s].v, pairs(2 * it, s, 1), O[it]);
+        }
+      // ---- out: lane l has token l % 32 of a tile and four columns side by side
+#pragma unroll
+      for (int it = 0; it < 2; ++it) {
+        const int i = 32 * it + l32;
+        const bool in = i < n_here;
+        const long long t = token(in ? base + i : 0);
+        const long long at = b * R.o_sb + t * R.o_st + h * R.o_sh;
+        const bf16* dp = static_cast<const bf16*>(R.dot.p) + b * R.dot.sb + t * R.dot.st +
+                         (h / R.dot.rep) * R.dot.sh;
+        float d = 0.0f;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int c4 = col0 + 32 * wave + 8 * q + 4 * half;
+          const float v[4] = {O[it][4 * q], O[it][4 * q + 1], O[it][4 * q + 2], O[it][4 * q + 3]};
+          if (!in || c4 >= R.vd) continue;
+          if (R.out_f32)
+            *reinterpret_cast<f4*>(static_cast<float*>(R.out) + at + c4) = f4{v[0], v[1], v[2], v[3]};
+          else
+            *reinterpret_cast<uint2*>(static_cast<bf16*>(R.out) + at + c4) =
+                uint2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+          if (R.dots) {
+            const uint2 w = *reinterpret_cast<const uint2*>(dp + c4);
+            d = fmaf(v[0], lo_bf16(w.x), d);
+            d = fmaf(v[1], hi_bf16(w.x), d);
+            d = fmaf(v[2], lo_bf16(w.y), d);
+            d = fmaf(v[3], hi_bf16(w.y), d);
+          }
+        }
+        if (R.dots) {
+          d += __shfl_xor(d, 32);
+          if (half == 0) sdot[wave][i] = d;
+        }
+      }
+    }
+
+    // ---- the state behind the chunk
+    const float tot = s_tot;
+    sum_decay += s_sum;
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) S[t][r] *= tot;
+#pragma unroll
+    for (int ts = 0; ts < 4; ++ts) {
+      float x[8];
+      const f4 w0 = *reinterpret_cast<const f4*>(&sw[16 * ts + 4 * half]);
+      const f4 w1 = *reinterpret_cast<const f4*>(&sw[16 * ts + 8 + 4 * half]);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        x[q] = (q & 1 ? hi_bf16(zf[ts].w[q / 2]) : lo_bf16(zf[ts].w[q / 2])) * w0[q];
+        x[4 + q] = (q & 1 ? hi_bf16(zf[ts].w[2 + q / 2]) : lo_bf16(zf[ts].w[2 + q / 2])) * w1[q];
+      }
+      const b8 z0 = split8(x), z1 = split8(x), z2 = pack8(x);
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        const b8 y = load_across<RX>(sy + across_share<RX>(lane), 16 * ts, 32 * t);
+        S[t] = mfma(y, z0, S[t]);
+        S[t] = mfma(y, z1, S[t]);
+        S[t] = mfma(y, z2, S[t]);
+      }
+    }
+    __syncthreads();
+    if (!STATE_ONLY && R.dots && tid < n_here) {
+      float d = 0.0f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) d += sdot[w][tid];
+      const size_t at = P.seqs.cu ? token(base + tid)
+                                  : static_cast<size_t>(b) * P.seqs.T + token(base + tid);
+      R.dots[(static_cast<size_t>(tile) * P.H + h) * P.batch_tokens + at] = d;
+    }
+  }
+
+  // ---- the state behind the piece
+  float* dst = nullptr;
+  float f = 1.0f;
+  if (STATE_ONLY) {
+    dst = R.piece_state + static_cast<size_t>(piece) * row_floats + head_floats;
+    if (tile == 0 && tid == 0) R.piece_decay[static_cast<size_t>(piece) * P.H + h] = sum_decay;
+  } else if (R.rev ? pc.first : pc.last) {
+    if (float* row = la_row(R.last, pc.seq, row_floats)) dst = row + head_floats;
+    // backwards the first token's decay lies between its R and the initial state's gradient
+    if (R.rev && pc.s1 > pc.s0) f = fexp(la_decay(P.g, b, pc.s0, h));
+  }
+  if (dst && col < R.vd) {
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int i = 32 * t + 8 * (r >> 2) + 4 * half + (r & 3);
+        if (i < R.kd)
+          dst[static_cast<size_t>(i) * R.sk + static_cast<size_t>(col) * R.sv] = S[t][r] * f;
+      }
+  }
+}
+
+template <int KD, int W>
+int launch(const LaParams& p, int roles, bool state_only, bool fine, hipStream_t stream) {
+  const dim3 grid(static_cast<unsigned>(p.seqs.pieces) * p.tiles, p.H, roles), block(64 * W);
+  if (state_only)
+    la_walk_bf16_kernel<KD, W, true, false><<<grid, block, 0, stream>>>(p);
+  else if (fine)
+    la_walk_bf16_kernel<KD, W, false, true><<<grid, block, 0, stream>>>(p);
+  else
+    la_walk_bf16_kernel<KD, W, false, false><<<grid, block, 0, stream>>>(p);
+  PRNN_HIP(hipGetLastError());
+  return PRNN_OK;
+}
+
+template <int KD>
+int launch_kd(const LaParams& p, int roles, bool state_only, bool fine, hipStream_t stream) {
+  const int cols = la_bf16_tile_cols(la_widest(p, roles));
+  if (cols == 32) return launch<KD, 1>(p, roles, state_only, fine, stream);
+  if (cols == 64) return launch<KD, 2>(p, roles, state_only, fine, stream);
+  return launch<KD, 4>(p, roles, state_only, fine, stream);
+}
+
+}  // namespace
+
+int la_bf16_tile_cols(int vd) { return vd <= 32 ? 32 : vd <= 64 ? 64 : 128; }
+
+int la_walk_bf16(LaParams p, int roles, bool state_only, bool fine, hipStream_t stream) {
+  const int vd = la_widest(p, roles), cols = la_bf16_tile_cols(vd);
+  p.tiles = (vd + cols - 1) / cols;
+  int kd = 0;
+  for (int i = 0; i < roles; ++i) kd = std::max(kd, p.role[i].kd);
+  if (kd <= 32) return launch_kd<32>(p, roles, state_only, fine, stream);
+  if (kd <= 64) return launch_kd<64>(p, roles, state_only, fine, stream);
+  if (kd <= 128) return launch_kd<128>(p, roles, state_only, fine, stream);
+  return launch_kd<256>(p, roles, state_only, fine, stream);
+}
+
+}  // namespace prnn

@@ -43,6 +43,19 @@ def _rows(t: Tensor) -> Tensor:
     return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
 
 
+def _tiles(t: Tensor) -> Tensor:
+    """``t`` as the walks read it.  Which walk runs goes by type and widths alone, so that equal
+    values give equal bits: the bfloat16 one (widths in eights) reads 16 bytes at a time, and rows
+    that do not lie for that (a view of a fused projection with an odd offset) are copied."""
+    t = _rows(t)
+    if t.dtype != torch.bfloat16 or t.shape[-1] % 8:
+        return t
+    sb, st, sh, _ = t.stride()
+    if (sb | st | sh) % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 def _view(t: Tensor) -> _lib.LaView:
     return _lib.LaView(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2), t.shape[2])
 
@@ -114,7 +127,7 @@ class _Problem:
                 raise ValueError(f"{what}: log_decay has {g.shape[-1]} heads, q, k and v have "
                                  f"{heads}")
             heads = _heads(what, q.shape[2], k.shape[2], v.shape[2], g.shape[-1])
-        self.q, self.k, self.v, self.g = _rows(q), _rows(k), _rows(v), g
+        self.q, self.k, self.v, self.g = _tiles(q), _tiles(k), _tiles(v), g
         dk, dv = q.shape[3], v.shape[3]
         if not 1 <= dk <= 256 or not 1 <= dv <= 256:
             raise ValueError(f"{what}: head widths ({dk}, {dv}) are not in 1 .. 256")
@@ -170,7 +183,7 @@ def _forward(p: _Problem, state_out: Tensor | None, table: Tensor | None) -> Ten
 
 def _backward(p: _Problem, go: Tensor, gs: Tensor | None, need_g: bool, need_h0: bool):
     lib, dev = _lib.load(), p.q.device
-    go = _rows(go)
+    go = _tiles(go)
     gs = None if gs is None else gs.contiguous()
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (p.q, p.k, p.v))
     dg = torch.empty(p.g.shape, dtype=p.g.dtype, device=dev) if need_g else None
