@@ -33,6 +33,7 @@ struct NormArgs {
   size_t rows;       // tokens (token kernels)
   int N, L, C, G, Cg;
   int act, w_f32;    // w and b are float32
+  int w_vec;         // and lie on 16-byte boundaries
   int lanes;         // lanes of a group: a power of two
   int strips, strip_rows;
   float eps;
@@ -109,6 +110,26 @@ __device__ __forceinline__ float param(const void* p, int f32, int c, float none
   return f32 ? static_cast<const float*>(p)[c] : to_f32(static_cast<const T*>(p)[c]);
 }
 
+// V consecutive parameters; c is a multiple of V, so where x's channels admit vectors and the
+// parameters' rows lie alike (vec) these do too.
+template <typename T, int V>
+__device__ __forceinline__ void params(const void* p, int f32, int vec, int c, float none,
+                                       float* v) {
+  if (p != nullptr && vec) {
+    if (!f32) {
+      loadv<T, V>(static_cast<const T*>(p) + c, v);
+      return;
+    }
+    if constexpr (V >= 4) {
+#pragma unroll
+      for (int i = 0; i < V; i += 4) loadv<float, 4>(static_cast<const float*>(p) + c + i, v + i);
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = param<T>(p, f32, c + i, none);
+}
+
 // Sum over the `lanes` lanes of a group (a power of two; every lane gets it).
 __device__ __forceinline__ float group_sum(float v, int lanes) {
   for (int k = 1; k < lanes; k <<= 1) v += __shfl_xor(v, k);
@@ -156,11 +177,8 @@ __global__ __launch_bounds__(256) void norm_token_kernel(NormArgs A) {
     const int c = (k * A.lanes + p.l) * V;
     in[k] = p.on && c < A.Cg;
     ch[k] = in[k] ? p.group * A.Cg + c : 0;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      w[k][i] = in[k] ? param<T>(A.w, A.w_f32, ch[k] + i, 1.0f) : 0.0f;
-      b[k][i] = in[k] ? param<T>(A.b, A.w_f32, ch[k] + i, 0.0f) : 0.0f;
-    }
+    params<T, V>(A.w, A.w_f32, A.w_vec, ch[k], 1.0f, w[k]);
+    params<T, V>(A.b, A.w_f32, A.w_vec, ch[k], 0.0f, b[k]);
   }
   // all lanes of a wave stay in the loop: the sums are shuffles
   for (size_t r0 = static_cast<size_t>(blockIdx.x) * p.rows_per; r0 < A.rows;
@@ -220,12 +238,10 @@ __global__ __launch_bounds__(256) void norm_token_bwd_kernel(NormArgs A) {
     const int c = (k * A.lanes + p.l) * V;
     in[k] = p.on && c < A.Cg;
     ch[k] = in[k] ? p.group * A.Cg + c : 0;
+    params<T, V>(A.w, A.w_f32, A.w_vec, ch[k], 1.0f, w[k]);
+    params<T, V>(A.b, A.w_f32, A.w_vec, ch[k], 0.0f, b[k]);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      w[k][i] = in[k] ? param<T>(A.w, A.w_f32, ch[k] + i, 1.0f) : 0.0f;
-      b[k][i] = in[k] ? param<T>(A.b, A.w_f32, ch[k] + i, 0.0f) : 0.0f;
-      dw[k][i] = db[k][i] = 0.0f;
-    }
+    for (int i = 0; i < V; ++i) dw[k][i] = db[k][i] = 0.0f;
   }
   for (size_t r0 = static_cast<size_t>(blockIdx.x) * p.rows_per; r0 < A.rows;
        r0 += static_cast<size_t>(gridDim.x) * p.rows_per) {
@@ -319,21 +335,31 @@ __global__ __launch_bounds__(256) void norm_token_bwd_kernel(NormArgs A) {
       }
 }
 
-// dw and db from partial sums [parts][2][C]: 32 channels a workgroup, 8 lanes to a channel.
+// dw and db from partial sums [parts][2][C]: 32 channels a workgroup, 32 lanes to a channel, each
+// with 8 loads under way.
 template <typename T>
-__global__ __launch_bounds__(256) void norm_param_kernel(const float* __restrict__ part, int parts,
-                                                         int C, void* dw, void* db, int f32) {
-  __shared__ float red[8][33];
-  const int c0 = blockIdx.x * 32, c = c0 + threadIdx.x % 32, sub = threadIdx.x / 32;
+__global__ __launch_bounds__(1024) void norm_param_kernel(const float* __restrict__ part, int parts,
+                                                          int C, void* dw, void* db, int f32) {
+  __shared__ float red[32][33];
+  const int l = threadIdx.x & 31, sub = threadIdx.x >> 5, c = blockIdx.x * 32 + l;
   const int which = blockIdx.y;
   float s = 0.0f;
-  if (c < C)
-    for (int p = sub; p < parts; p += 8) s += part[(static_cast<size_t>(p) * 2 + which) * C + c];
-  red[sub][threadIdx.x % 32] = s;
+  if (c < C) {
+    const float* p = part + static_cast<size_t>(which) * C + c;
+    for (int k = sub; k < parts; k += 256) {
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        v[i] = k + 32 * i < parts ? p[static_cast<size_t>(k + 32 * i) * 2 * C] : 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += v[i];
+    }
+  }
+  red[sub][l] = s;
   __syncthreads();
   void* out = which ? db : dw;
   if (sub == 0 && c < C && out) {
-    for (int k = 1; k < 8; ++k) s += red[k][threadIdx.x];
+    for (int k = 1; k < 32; ++k) s += red[k][l];
     if (f32)
       static_cast<float*>(out)[c] = s;
     else
@@ -528,11 +554,8 @@ __global__ __launch_bounds__(256) void norm_sample_apply_kernel(NormArgs A) {
     const float mean = A.stats[2 * (static_cast<size_t>(n) * A.G + g)];
     const float rstd = A.stats[2 * (static_cast<size_t>(n) * A.G + g) + 1];
     float w[V], b[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      w[i] = param<T>(A.w, A.w_f32, c + i, 1.0f);
-      b[i] = param<T>(A.b, A.w_f32, c + i, 0.0f);
-    }
+    params<T, V>(A.w, A.w_f32, A.w_vec, c, 1.0f, w);
+    params<T, V>(A.b, A.w_f32, A.w_vec, c, 0.0f, b);
     for (int l = l0 + p.row; l < l1; l += p.rows_per) {
       const size_t at = base + static_cast<size_t>(l) * A.C + c;
       float x[V], gt[V], y[V];
@@ -565,12 +588,10 @@ __global__ __launch_bounds__(256) void norm_sample_bwd_sums_kernel(NormArgs A) {
     const float mean = A.stats[2 * (static_cast<size_t>(n) * A.G + g)];
     const float rstd = A.stats[2 * (static_cast<size_t>(n) * A.G + g) + 1];
     float w[V], b[V], dw[V], db[V];
+    params<T, V>(A.w, A.w_f32, A.w_vec, c, 1.0f, w);
+    params<T, V>(A.b, A.w_f32, A.w_vec, c, 0.0f, b);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      w[i] = param<T>(A.w, A.w_f32, c + i, 1.0f);
-      b[i] = param<T>(A.b, A.w_f32, c + i, 0.0f);
-      dw[i] = db[i] = 0.0f;
-    }
+    for (int i = 0; i < V; ++i) dw[i] = db[i] = 0.0f;
     if (on)
       for (int l = l0 + p.row; l < l1; l += p.rows_per) {
         const size_t at = base + static_cast<size_t>(l) * A.C + c;
@@ -653,11 +674,8 @@ __global__ __launch_bounds__(256) void norm_sample_dx_kernel(NormArgs A) {
     const float mean = A.stats[2 * ng], rstd = A.stats[2 * ng + 1];
     const float m1 = A.part2[2 * ng], m2 = A.part2[2 * ng + 1];
     float w[V], b[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      w[i] = param<T>(A.w, A.w_f32, c + i, 1.0f);
-      b[i] = param<T>(A.b, A.w_f32, c + i, 0.0f);
-    }
+    params<T, V>(A.w, A.w_f32, A.w_vec, c, 1.0f, w);
+    params<T, V>(A.b, A.w_f32, A.w_vec, c, 0.0f, b);
     for (int l = l0 + p.row; l < l1; l += p.rows_per) {
       const size_t at = base + static_cast<size_t>(l) * A.C + c;
       float x[V], gt[V], dz[V];
@@ -714,9 +732,9 @@ Plan plan(int N, int L, int Cg, int G, int dtype, uintptr_t bits, bool backward)
     const int rows_per = per_row <= 256 ? 256 / per_row : 1;
     p.blocks_y = (per_row + 255) / 256;
     const int need = (N + rows_per - 1) / rows_per;
-    // The backward pass keeps the parameters' sums per workgroup: about four workgroups a CU
-    // share the rows; the forward pass has nothing to keep.
-    const int most = backward ? std::max(1, 1024 / p.blocks_y) : 16384;
+    // A workgroup reads its parameters once (backward: keeps their sums) and goes on from row to
+    // row: about eight a CU forward, four backward, where a partial sum each is written.
+    const int most = std::max(1, (backward ? 1024 : 2048) / p.blocks_y);
     p.blocks_x = std::max(1, std::min(need, most));
     return p;
   }
@@ -817,6 +835,7 @@ extern "C" PRNN_API int prnn_group_norm(const void* x, const void* w, const void
   a.Cg = C / G;
   a.act = act;
   a.w_f32 = w_dtype == PRNN_F32;
+  a.w_vec = (bits_of({w, b}) & 15) == 0;
   a.lanes = p.lanes;
   a.strips = p.strips;
   a.strip_rows = p.strip_rows;
@@ -896,6 +915,7 @@ extern "C" PRNN_API int prnn_group_norm_backward(
   a.Cg = C / G;
   a.act = act;
   a.w_f32 = w_dtype == PRNN_F32;
+  a.w_vec = (bits_of({w, b}) & 15) == 0;
   a.lanes = p.lanes;
   a.strips = p.strips;
   a.strip_rows = p.strip_rows;
@@ -924,7 +944,7 @@ extern "C" PRNN_API int prnn_group_norm_backward(
       PRNN_HIP(hipGetLastError());
     }
     if (dw || db) {
-      norm_param_kernel<T><<<dim3((C + 31) / 32, 2), 256, 0, st>>>(part, parts, C, dw, db,
+      norm_param_kernel<T><<<dim3((C + 31) / 32, 2), 1024, 0, st>>>(part, parts, C, dw, db,
                                                                    a.w_f32);
       PRNN_HIP(hipGetLastError());
     }

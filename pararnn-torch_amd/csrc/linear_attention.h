@@ -40,6 +40,11 @@ struct LaView {
   int vec;               // rows and base admit 16-byte accesses
 };
 
+// Chunks' rows are read by 32-bit offsets.
+constexpr bool la_stride_fits(long long st, int size) {
+  return (st < 0 ? -st : st) * size <= (1 << 24);
+}
+
 // The decays: (B, T, H) by strides, or one per head (sb = st = 0); fp32 or the storage type.
 struct LaDecay {
   const void* p;
@@ -157,30 +162,44 @@ __device__ __forceinline__ float* la_row(const LaState& st, int s, size_t row_fl
 // that resets the state included), and sums stay finite; NaN stays NaN.
 __device__ __forceinline__ float la_clamp(float g) { return g < -104.0f ? -104.0f : g; }
 
-__device__ __forceinline__ float la_decay(const LaDecay& d, int b, int t, int h) {
+// A decay as it is stored, and its value: a load's bits are looked at only when they are used,
+// or the wave would wait for everything that it loaded before.
+__device__ __forceinline__ uint32_t la_decay_bits(const LaDecay& d, int b, int t, int h) {
   const long long at = static_cast<long long>(b) * d.sb + static_cast<long long>(t) * d.st +
                        static_cast<long long>(h) * d.sh;
-  float g;
-  if (d.dtype == PRNN_F32)
-    g = static_cast<const float*>(d.p)[at];
-  else if (d.dtype == PRNN_F16)
-    g = to_f32(static_cast<const f16*>(d.p)[at]);
-  else
-    g = to_f32(static_cast<const bf16*>(d.p)[at]);
-  return la_clamp(g);
+  return d.dtype == PRNN_F32 ? static_cast<const uint32_t*>(d.p)[at]
+                             : static_cast<const uint16_t*>(d.p)[at];
+}
+__device__ __forceinline__ float la_decay_value(const LaDecay& d, uint32_t bits) {
+  return la_clamp(d.dtype == PRNN_F32   ? __uint_as_float(bits)
+                  : d.dtype == PRNN_F16 ? Narrow<f16>::val(bits)
+                                        : Narrow<bf16>::val(bits));
+}
+__device__ __forceinline__ float la_decay(const LaDecay& d, int b, int t, int h) {
+  return la_decay_value(d, la_decay_bits(d, b, t, h));
 }
 
 // The log decay of a step of the walk that reaches token t: forwards g_t, backwards the next
-// token's (none behind the sequence's last token).
-__device__ __forceinline__ float la_step_decay(const LaDecay& d, int rev, const LaPiece& pc, int b,
-                                               int t, int h) {
-  if (!rev) return la_decay(d, b, t, h);
-  return t + 1 < pc.s1 ? la_decay(d, b, t + 1, h) : 0.0f;
+// token's (none, and zero bits are a zero of every type, behind the sequence's last token).
+__device__ __forceinline__ uint32_t la_step_decay(const LaDecay& d, int rev, const LaPiece& pc,
+                                                  int b, int t, int h) {
+  if (!rev) return la_decay_bits(d, b, t, h);
+  return t + 1 < pc.s1 ? la_decay_bits(d, b, t + 1, h) : 0u;
 }
 
-// Batch and token of a stream position: rectangular sequences are batches of their own.
+// Batch of a piece: rectangular sequences are batches of their own.
 __device__ __forceinline__ int la_batch(const LaSeqs& q, const LaPiece& pc) {
   return q.cu ? 0 : pc.seq;
+}
+
+// A head's rows of an array: a buffer resource at the lowest row of a chunk of C tokens of the
+// walk, and byte offsets in it (la_stride_fits).
+template <int C>
+__device__ __forceinline__ rsrc_t la_rows(const LaView& v, int size, int b, int h, int rev,
+                                          int begin, int end, int base) {
+  const long long t = rev ? static_cast<long long>(end) - base - C : static_cast<long long>(begin) + base;
+  return make_rsrc(static_cast<const char*>(v.p) + (b * v.sb + (h / v.rep) * v.sh + t * v.st) * size,
+                   0x7fffffffu);
 }
 
 // First piece of sequence s and their number.

@@ -32,14 +32,26 @@ __global__ __launch_bounds__(256) void la_join_kernel(JoinArgs A, int seq_blocks
   const size_t row = static_cast<size_t>(A.H) * A.DD;
   const size_t at = static_cast<size_t>(h) * A.DD + e;
   const float* init = la_row(A.init[role], seq, row);
+  const int dir = A.rev[role] ? -1 : 1, from = A.rev[role] ? p0 + n - 1 : p0;
   float S = init ? init[at] : 0.0f;
-  for (int i = 0; i < n; ++i) {
-    const size_t p = p0 + (A.rev[role] ? n - 1 - i : i);
-    float* w = A.state[role] + p * row + at;
-    const float U = i + 1 < n ? *w : 0.0f;
-    const float d = i + 1 < n ? A.decay[role][p * A.H + h] : 0.0f;
-    *w = S;
-    S = fmaf(fexp(d), S, U);
+  // the contributions of 16 pieces are under way before the first is added
+  constexpr int kAhead = 16;
+  for (int i0 = 0; i0 < n; i0 += kAhead) {
+    float U[kAhead], d[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const size_t p = from + dir * (i0 + i);
+      const bool more = i0 + i + 1 < n;  // the last piece hands on to none
+      U[i] = more ? A.state[role][p * row + at] : 0.0f;
+      d[i] = more ? A.decay[role][p * A.H + h] : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (i0 + i >= n) break;
+      const size_t p = from + dir * (i0 + i);
+      A.state[role][p * row + at] = S;
+      S = fmaf(fexp(d[i]), S, U[i]);
+    }
   }
 }
 
@@ -218,6 +230,12 @@ int check(const Problem* a) {
   if (static_cast<long long>(a->B) * a->T > 0)
     for (const void* p : {a->q.p, a->k.p, a->v.p, a->g})
       if (p == nullptr) return fail(PRNN_ERR_VALUE, "q, k, v and log_decay must be non-null");
+  const int size = a->dtype == PRNN_F32 ? 4 : 2;
+  for (const prnn_la_view* v : {&a->q, &a->k, &a->v})
+    if (!la_stride_fits(v->st, size))
+      return fail(PRNN_ERR_VALUE, "tokens %lld elements apart are too far (16 MiB)", v->st);
+  if (!la_stride_fits(1ll * a->H * std::max(a->Dk, a->Dv), 4))
+    return fail(PRNN_ERR_VALUE, "H=%d heads of (%d, %d) are too wide", a->H, a->Dk, a->Dv);
   if (a->h0 && a->h0_rows < 0) return fail(PRNN_ERR_VALUE, "h0_rows=%d", a->h0_rows);
   return PRNN_OK;
 }
@@ -513,6 +531,8 @@ extern "C" PRNN_API int prnn_linear_attention(const prnn_linear_attention_proble
   if (int rc = check(a)) return rc;
   if (out == nullptr || (out->p == nullptr && 1ll * a->B * a->T > 0))
     return fail(PRNN_ERR_VALUE, "out must be non-null");
+  if (!la_stride_fits(out->st, a->dtype == PRNN_F32 ? 4 : 2))
+    return fail(PRNN_ERR_VALUE, "tokens %lld elements apart are too far (16 MiB)", out->st);
   if (sequences(*a) == 0) return PRNN_OK;
   if (int rc = check_ws(need(*a, false, false), workspace, bytes)) return rc;
   return forward(*a, *out, state_out, out_table, out_rows, workspace,
@@ -532,6 +552,8 @@ extern "C" PRNN_API int prnn_linear_attention_backward(
   const bool any = 1ll * a->B * a->T > 0;
   if (go == nullptr || (any && (!go->p || !dq || !dk || !dv)))
     return fail(PRNN_ERR_VALUE, "go, dq, dk and dv must be non-null");
+  if (!la_stride_fits(go->st, a->dtype == PRNN_F32 ? 4 : 2))
+    return fail(PRNN_ERR_VALUE, "tokens %lld elements apart are too far (16 MiB)", go->st);
   if (a->h0_table) return fail(PRNN_ERR_VALUE, "a block table has no gradient");
   if (a->h0 && a->h0_rows < sequences(*a))
     return fail(PRNN_ERR_VALUE, "h0 has %d rows for %d sequences", a->h0_rows, sequences(*a));

@@ -25,6 +25,7 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s4 lds_s4;
 
@@ -131,13 +132,15 @@ void la_walk_bf16_kernel(LaParams P) {
       src = R.piece_state + static_cast<size_t>(piece) * row_floats + head_floats;
     else if (const float* row = la_row(R.init, pc.seq, row_floats))
       src = row + head_floats;
-    if (src && col < R.vd) {
+    if (src) {
+      const rsrc_t rs = make_rsrc(src, static_cast<uint32_t>(P.Dk * P.Dv) * 4);
 #pragma unroll
       for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const int i = 32 * t + 8 * (r >> 2) + 4 * half + (r & 3);
-          if (i < R.kd) S[t][r] = src[static_cast<size_t>(i) * R.sk + static_cast<size_t>(col) * R.sv];
+          const uint32_t o = static_cast<uint32_t>(i * R.sk + col * R.sv) * 4;
+          S[t][r] = ldb<float>(rs, i < R.kd && col < R.vd ? o : kOOB, 0);
         }
     }
   }
@@ -146,51 +149,46 @@ void la_walk_bf16_kernel(LaParams P) {
   float sum_decay = 0.0f;
   auto token = [&](int i) { return R.rev ? pc.end - 1 - i : pc.begin + i; };
 
-  // A thread's loads of an array are rows apart by a constant number: one pointer, which moves on
-  // by a chunk at a time.
+  // A thread's loads of an array are rows apart by a constant number.  What lies outside the
+  // piece or the width is read as zero (an offset outside the resource).
   constexpr int DX = NT / UX, DZ = NT / UZ;
   const int rowx = tid / UX, cx = (tid % UX) * 8, rowz = tid / UZ, cz = col0 + (tid % UZ) * 8;
-  const long long dir = R.rev ? -1 : 1;
-  const long long stx = dir * R.x.st, sty = dir * R.y.st, stz = dir * R.z.st;
-  const bf16* px = static_cast<const bf16*>(R.x.p) + b * R.x.sb + (h / R.x.rep) * R.x.sh +
-                   token(rowx) * R.x.st + cx;
-  const bf16* py = static_cast<const bf16*>(R.y.p) + b * R.y.sb + (h / R.y.rep) * R.y.sh +
-                   token(rowx) * R.y.st + cx;
-  const bf16* pz = static_cast<const bf16*>(R.z.p) + b * R.z.sb + (h / R.z.rep) * R.z.sh +
-                   token(rowz) * R.z.st + cz;
-  auto move_on = [&](int by) {
-    if (!STATE_ONLY) px += by * stx;
-    py += by * sty;
-    pz += by * stz;
-  };
   const bool inx = cx < R.kd, inz = cz < R.vd;
+  const int stx = static_cast<int>(R.x.st) * 2, sty = static_cast<int>(R.y.st) * 2,
+            stz = static_cast<int>(R.z.st) * 2;
+  const int fx = R.rev ? kC - 1 - rowx : rowx, fz = R.rev ? kC - 1 - rowz : rowz;
+  const int ahead = R.rev ? -1 : 1;
   u4 rx[STATE_ONLY ? 1 : NX], ry[NX], rz[NZ];
-  float rg = 0.0f;
+  uint32_t rg = 0;
   auto fetch = [&](int base) {
+    const int left = n_tok - base;
+    if (wave == 0)
+      rg = lane < left ? la_step_decay(P.g, R.rev, pc, b, token(base + lane), h) : 0u;
+    if (!STATE_ONLY) {
+      const rsrc_t bx = la_rows<kC>(R.x, 2, b, h, R.rev, pc.begin, pc.end, base);
+#pragma unroll
+      for (int k = 0; k < NX; ++k) {
+        const uint32_t o = (fx + ahead * k * DX) * stx + cx * 2;
+        rx[k] = __builtin_amdgcn_raw_buffer_load_b128(bx, inx && rowx + k * DX < left ? o : kOOB, 0, 0);
+      }
+    }
+    const rsrc_t by = la_rows<kC>(R.y, 2, b, h, R.rev, pc.begin, pc.end, base);
 #pragma unroll
     for (int k = 0; k < NX; ++k) {
-      const bool in = inx && base + rowx + k * DX < n_tok;
-      if (!STATE_ONLY) {
-        rx[k] = u4{0, 0, 0, 0};
-        if (in) rx[k] = *reinterpret_cast<const u4*>(px + k * DX * stx);
-      }
-      ry[k] = u4{0, 0, 0, 0};
-      if (in) ry[k] = *reinterpret_cast<const u4*>(py + k * DX * sty);
+      const uint32_t o = (fx + ahead * k * DX) * sty + cx * 2;
+      ry[k] = __builtin_amdgcn_raw_buffer_load_b128(by, inx && rowx + k * DX < left ? o : kOOB, 0, 0);
     }
+    const rsrc_t bz = la_rows<kC>(R.z, 2, b, h, R.rev, pc.begin, pc.end, base);
 #pragma unroll
     for (int k = 0; k < NZ; ++k) {
-      rz[k] = u4{0, 0, 0, 0};
-      if (inz && base + rowz + k * DZ < n_tok)
-        rz[k] = *reinterpret_cast<const u4*>(pz + k * DZ * stz);
+      const uint32_t o = (fz + ahead * k * DZ) * stz + cz * 2;
+      rz[k] = __builtin_amdgcn_raw_buffer_load_b128(bz, inz && rowz + k * DZ < left ? o : kOOB, 0, 0);
     }
-    move_on(kC);
-    rg = wave == 0 && base + lane < n_tok
-             ? la_step_decay(P.g, R.rev, pc, b, token(base + lane), h) : 0.0f;
   };
   // Decays of the chunk's first `n` tokens: running sums in fp64, so that what is left of the
   // whole keeps its digits.
-  auto decays = [&](float g, int n) {
-    double G = lane < n ? g : 0.0f;
+  auto decays = [&](uint32_t bits, int n) {
+    double G = lane < n ? la_decay_value(P.g, bits) : 0.0f;
 #pragma unroll
     for (int d = 1; d < kC; d <<= 1) {
       const double o = __shfl_up(G, d);
@@ -230,7 +228,7 @@ void la_walk_bf16_kernel(LaParams P) {
       for (int q = 0; q < 4; ++q) bad |= (rz[k][q] & 0x7f807f80u) + 0x00800080u;
       if ((bad & 0x80008000u) && rowz + k * DZ > 0) atomicMin(&s_stop[turn], rowz + k * DZ);
     }
-    const float g_here = rg;
+    const uint32_t g_here = rg;
     if (wave == 0) decays(rg, kC);
     next = base + kC;
     if (next < n_tok) fetch(next);
@@ -246,8 +244,6 @@ void la_walk_bf16_kernel(LaParams P) {
       for (int e = tid; e < (kC - stop) * (RZ / 16); e += NT)
         *reinterpret_cast<u4*>(sz + stop * RZ + e * 16) = u4{0, 0, 0, 0};
       if (wave == 0) decays(g_here, stop);
-      if (next < n_tok) move_on(-kC);
-      move_on(stop - kC);
       next = base + stop;
       if (next < n_tok) fetch(next);
       __syncthreads();
@@ -350,34 +346,45 @@ void la_walk_bf16_kernel(LaParams P) {
           if (FINE) O[it] = mfma(zf[2 * it + s].v, pairs(2 * it, s, 1), O[it]);
         }
       // ---- out: lane l has token l % 32 of a tile and four columns side by side
+      const LaView ov{R.out, R.o_sb, R.o_st, R.o_sh, 1, 1};
+      const int so = R.out_f32 ? 4 : 2;
+      const rsrc_t bo = la_rows<kC>(ov, so, b, h, R.rev, pc.begin, pc.end, base);
+      rsrc_t bd = bo;
+      if (FINE && R.dots) bd = la_rows<kC>(R.dot, 2, b, h, R.rev, pc.begin, pc.end, base);
 #pragma unroll
       for (int it = 0; it < 2; ++it) {
-        const int i = 32 * it + l32;
-        const bool in = i < n_here;
-        const long long t = token(in ? base + i : 0);
-        const long long at = b * R.o_sb + t * R.o_st + h * R.o_sh;
-        const bf16* dp = static_cast<const bf16*>(R.dot.p) + b * R.dot.sb + t * R.dot.st +
-                         (h / R.dot.rep) * R.dot.sh;
-        float d = 0.0f;
+        const int i = 32 * it + l32, row = R.rev ? kC - 1 - i : i;
+        const int c4 = col0 + 32 * wave + 4 * half;
+        const uint32_t at = (row * static_cast<int>(R.o_st) + c4) * so;
+        u2 dv[4];
+        if (FINE && R.dots)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const uint32_t o = (row * static_cast<int>(R.dot.st) + c4 + 8 * q) * 2;
+            dv[q] = __builtin_amdgcn_raw_buffer_load_b64(
+                bd, i < n_here && c4 + 8 * q < R.vd ? o : kOOB, 0, 0);
+          }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const int c4 = col0 + 32 * wave + 8 * q + 4 * half;
+          const uint32_t o = i < n_here && c4 + 8 * q < R.vd ? at + 8 * q * so : kOOB;
           const float v[4] = {O[it][4 * q], O[it][4 * q + 1], O[it][4 * q + 2], O[it][4 * q + 3]};
-          if (!in || c4 >= R.vd) continue;
           if (R.out_f32)
-            *reinterpret_cast<f4*>(static_cast<float*>(R.out) + at + c4) = f4{v[0], v[1], v[2], v[3]};
+            __builtin_amdgcn_raw_buffer_store_b128(
+                u4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
+                   __float_as_uint(v[3])}, bo, o, 0, 0);
           else
-            *reinterpret_cast<uint2*>(static_cast<bf16*>(R.out) + at + c4) =
-                uint2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-          if (R.dots) {
-            const uint2 w = *reinterpret_cast<const uint2*>(dp + c4);
-            d = fmaf(v[0], lo_bf16(w.x), d);
-            d = fmaf(v[1], hi_bf16(w.x), d);
-            d = fmaf(v[2], lo_bf16(w.y), d);
-            d = fmaf(v[3], hi_bf16(w.y), d);
-          }
+            __builtin_amdgcn_raw_buffer_store_b64(
+                u2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])}, bo, o, 0, 0);
         }
-        if (R.dots) {
+        if (FINE && R.dots) {
+          float d = 0.0f;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            d = fmaf(O[it][4 * q], lo_bf16(dv[q][0]), d);
+            d = fmaf(O[it][4 * q + 1], hi_bf16(dv[q][0]), d);
+            d = fmaf(O[it][4 * q + 2], lo_bf16(dv[q][1]), d);
+            d = fmaf(O[it][4 * q + 3], hi_bf16(dv[q][1]), d);
+          }
           d += __shfl_xor(d, 32);
           if (half == 0) sdot[wave][i] = d;
         }
@@ -411,7 +418,7 @@ void la_walk_bf16_kernel(LaParams P) {
       }
     }
     __syncthreads();
-    if (!STATE_ONLY && R.dots && tid < n_here) {
+    if (FINE && R.dots && tid < n_here) {
       float d = 0.0f;
 #pragma unroll
       for (int w = 0; w < W; ++w) d += sdot[w][tid];
@@ -432,14 +439,15 @@ void la_walk_bf16_kernel(LaParams P) {
     // backwards the first token's decay lies between its R and the initial state's gradient
     if (R.rev && pc.s1 > pc.s0) f = fexp(la_decay(P.g, b, pc.s0, h));
   }
-  if (dst && col < R.vd) {
+  if (dst) {
+    const rsrc_t rs = make_rsrc(dst, static_cast<uint32_t>(P.Dk * P.Dv) * 4);
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int i = 32 * t + 8 * (r >> 2) + 4 * half + (r & 3);
-        if (i < R.kd)
-          dst[static_cast<size_t>(i) * R.sk + static_cast<size_t>(col) * R.sv] = S[t][r] * f;
+        const uint32_t o = static_cast<uint32_t>(i * R.sk + col * R.sv) * 4;
+        stb<float>(rs, i < R.kd && col < R.vd ? o : kOOB, 0, S[t][r] * f);
       }
   }
 }

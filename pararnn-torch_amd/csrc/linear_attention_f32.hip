@@ -23,41 +23,40 @@ __device__ __forceinline__ float exp_diff(double a, double b) {
   return fexp(static_cast<float>(a - b));
 }
 
+// Four elements of a row as they are stored (raw), from a buffer or one by one; zeros outside.
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 template <typename T>
-__device__ __forceinline__ f4 load4(const T* p, int left, bool vec);
-template <>
-__device__ __forceinline__ f4 load4<float>(const float* p, int left, bool vec) {
-  if (vec && left >= 4) return *reinterpret_cast<const f4*>(p);
-  f4 v = {0, 0, 0, 0};
+struct Raw {
+  using type = u2;
+  static __device__ __forceinline__ u2 load(rsrc_t r, uint32_t o, int left, bool vec) {
+    if (vec) return __builtin_amdgcn_raw_buffer_load_b64(r, left >= 4 ? o : kOOB, 0, 0);
+    uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (i < left) v[i] = p[i];
-  return v;
-}
-template <typename T>
-__device__ __forceinline__ f4 load4_16(const T* p, int left, bool vec) {
-  f4 v = {0, 0, 0, 0};
-  if (vec && left >= 4) {
-    const uint2 w = *reinterpret_cast<const uint2*>(p);
-    v[0] = Narrow<T>::lo(w.x);
-    v[1] = Narrow<T>::hi(w.x);
-    v[2] = Narrow<T>::lo(w.y);
-    v[3] = Narrow<T>::hi(w.y);
-    return v;
+    for (int i = 0; i < 4; ++i)
+      w[i] = __builtin_amdgcn_raw_buffer_load_b16(r, i < left ? o + 2 * i : kOOB, 0, 0);
+    return u2{(w[0] & 0xffffu) | w[1] << 16, (w[2] & 0xffffu) | w[3] << 16};
   }
+  static __device__ __forceinline__ f4 value(u2 w) {
+    return f4{Narrow<T>::lo(w[0]), Narrow<T>::hi(w[0]), Narrow<T>::lo(w[1]), Narrow<T>::hi(w[1])};
+  }
+};
+template <>
+struct Raw<float> {
+  using type = u4;
+  static __device__ __forceinline__ u4 load(rsrc_t r, uint32_t o, int left, bool vec) {
+    if (vec) return __builtin_amdgcn_raw_buffer_load_b128(r, left >= 4 ? o : kOOB, 0, 0);
+    u4 w;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (i < left) v[i] = to_f32(p[i]);
-  return v;
-}
-template <>
-__device__ __forceinline__ f4 load4<bf16>(const bf16* p, int left, bool vec) {
-  return load4_16(p, left, vec);
-}
-template <>
-__device__ __forceinline__ f4 load4<f16>(const f16* p, int left, bool vec) {
-  return load4_16(p, left, vec);
-}
+    for (int i = 0; i < 4; ++i)
+      w[i] = __builtin_amdgcn_raw_buffer_load_b32(r, i < left ? o + 4 * i : kOOB, 0, 0);
+    return w;
+  }
+  static __device__ __forceinline__ f4 value(u4 w) {
+    return f4{__uint_as_float(w[0]), __uint_as_float(w[1]), __uint_as_float(w[2]),
+              __uint_as_float(w[3])};
+  }
+};
 
 // KT: 32-column blocks of x and y (padded with zeros); W: waves, 16 columns of z each.
 template <typename T, int KT, int W, bool STATE_ONLY>
@@ -109,46 +108,57 @@ __global__ __launch_bounds__(64 * W) void la_walk_f32_kernel(LaParams P) {
     else if (const float* row = la_row(R.init, pc.seq, row_floats))
       src = row + head_floats;
     if (src) {
+      const rsrc_t rs = make_rsrc(src, static_cast<uint32_t>(P.Dk * P.Dv) * 4);
 #pragma unroll
       for (int t = 0; t < 2 * KT; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int i = 16 * t + 4 * q4 + r;
-          if (i < R.kd && col < R.vd) S[t][r] = src[static_cast<size_t>(i) * R.sk + static_cast<size_t>(col) * R.sv];
+          const uint32_t o = static_cast<uint32_t>(i * R.sk + col * R.sv) * 4;
+          S[t][r] = ldb<float>(rs, i < R.kd && col < R.vd ? o : kOOB, 0);
         }
     }
   }
 
-  const T* xb = static_cast<const T*>(R.x.p) + b * R.x.sb + (h / R.x.rep) * R.x.sh;
-  const T* yb = static_cast<const T*>(R.y.p) + b * R.y.sb + (h / R.y.rep) * R.y.sh;
-  const T* zb = static_cast<const T*>(R.z.p) + b * R.z.sb + (h / R.z.rep) * R.z.sh;
   const int n_tok = pc.end - pc.begin;
   const int chunks = (n_tok + kC - 1) / kC;
   float sum_decay = 0.0f;
 
-  f4 rx[STATE_ONLY ? 1 : NX], ry[NX], rz[NZ];
-  float rg = 0.0f;
+  // A thread's loads of an array are rows apart by a constant number; what lies outside the
+  // piece or the width is read as zero (an offset outside the resource).
+  using raw = typename Raw<T>::type;
+  constexpr int SZ = sizeof(T);
+  constexpr int UX = KD / 4, UZ = 4 * W, DX = NT / UX, DZ = NT / UZ;
+  const int rowx = tid / UX, cx = (tid % UX) * 4, rowz = tid / UZ, cz = col0 + (tid % UZ) * 4;
+  const int fx = R.rev ? kC - 1 - rowx : rowx, fz = R.rev ? kC - 1 - rowz : rowz;
+  const int ahead = R.rev ? -1 : 1;
+  const int stx = static_cast<int>(R.x.st) * SZ, sty = static_cast<int>(R.y.st) * SZ,
+            stz = static_cast<int>(R.z.st) * SZ;
+  raw rx[STATE_ONLY ? 1 : NX], ry[NX], rz[NZ];
+  uint32_t rg = 0;
   // token of local index i of the walk
   auto token = [&](int i) { return R.rev ? pc.end - 1 - i : pc.begin + i; };
   auto fetch = [&](int c) {
-    const int base = c * kC;
+    const int base = c * kC, left = n_tok - base;
+    if (wave == 0)
+      rg = lane < min(left, kC) ? la_step_decay(P.g, R.rev, pc, b, token(base + lane), h) : 0u;
+    if (!STATE_ONLY) {
+      const rsrc_t bx = la_rows<kC>(R.x, SZ, b, h, R.rev, pc.begin, pc.end, base);
 #pragma unroll
-    for (int k = 0; k < NX; ++k) {
-      const int e = (tid + k * NT) * 4, row = e / KD, cc = e % KD;
-      const bool in = base + row < n_tok && cc < R.kd;
-      const long long t = token(base + row);
-      if (!STATE_ONLY) rx[k] = in ? load4<T>(xb + t * R.x.st + cc, R.kd - cc, R.x.vec) : f4{0, 0, 0, 0};
-      ry[k] = in ? load4<T>(yb + t * R.y.st + cc, R.kd - cc, R.y.vec) : f4{0, 0, 0, 0};
+      for (int k = 0; k < NX; ++k)
+        rx[k] = Raw<T>::load(bx, (fx + ahead * k * DX) * stx + cx * SZ,
+                             rowx + k * DX < left ? R.kd - cx : 0, R.x.vec && R.kd % 4 == 0);
     }
+    const rsrc_t by = la_rows<kC>(R.y, SZ, b, h, R.rev, pc.begin, pc.end, base);
 #pragma unroll
-    for (int k = 0; k < NZ; ++k) {
-      const int e = (tid + k * NT) * 4, row = e / (16 * W), cc = col0 + e % (16 * W);
-      const bool in = base + row < n_tok && cc < R.vd;
-      const long long t = token(base + row);
-      rz[k] = in ? load4<T>(zb + t * R.z.st + cc, R.vd - cc, R.z.vec) : f4{0, 0, 0, 0};
-    }
-    rg = lane < kC && base + lane < n_tok
-             ? la_step_decay(P.g, R.rev, pc, b, token(base + lane), h) : 0.0f;
+    for (int k = 0; k < NX; ++k)
+      ry[k] = Raw<T>::load(by, (fx + ahead * k * DX) * sty + cx * SZ,
+                           rowx + k * DX < left ? R.kd - cx : 0, R.y.vec && R.kd % 4 == 0);
+    const rsrc_t bz = la_rows<kC>(R.z, SZ, b, h, R.rev, pc.begin, pc.end, base);
+#pragma unroll
+    for (int k = 0; k < NZ; ++k)
+      rz[k] = Raw<T>::load(bz, (fz + ahead * k * DZ) * stz + cz * SZ,
+                           rowz + k * DZ < left ? R.vd - cz : 0, R.z.vec && R.vd % 4 == 0);
   };
   fetch(0);
 
@@ -156,18 +166,16 @@ __global__ __launch_bounds__(64 * W) void la_walk_f32_kernel(LaParams P) {
     const int base = c * kC;
 #pragma unroll
     for (int k = 0; k < NX; ++k) {
-      const int e = (tid + k * NT) * 4, row = e / KD, cc = e % KD;
-      if (!STATE_ONLY) *reinterpret_cast<f4*>(&sx[row * XS + cc]) = rx[k];
-      *reinterpret_cast<f4*>(&sy[row * XS + cc]) = ry[k];
+      const int o = (rowx + k * DX) * XS + cx;
+      if (!STATE_ONLY) *reinterpret_cast<f4*>(&sx[o]) = Raw<T>::value(rx[k]);
+      *reinterpret_cast<f4*>(&sy[o]) = Raw<T>::value(ry[k]);
     }
 #pragma unroll
-    for (int k = 0; k < NZ; ++k) {
-      const int e = (tid + k * NT) * 4, row = e / (16 * W), cc = e % (16 * W);
-      *reinterpret_cast<f4*>(&sz[row * ZS + cc]) = rz[k];
-    }
+    for (int k = 0; k < NZ; ++k)
+      *reinterpret_cast<f4*>(&sz[(rowz + k * DZ) * ZS + (tid % UZ) * 4]) = Raw<T>::value(rz[k]);
     if (wave == 0) {
       // running sums of the decays in fp64: differences of nearby ones keep their digits
-      double G = rg;
+      double G = la_decay_value(P.g, rg);
 #pragma unroll
       for (int d = 1; d < kC; d <<= 1) {
         const double o = __shfl_up(G, d);
@@ -340,13 +348,14 @@ __global__ __launch_bounds__(64 * W) void la_walk_f32_kernel(LaParams P) {
     if (R.rev && pc.s1 > pc.s0) f = fexp(la_decay(P.g, b, pc.s0, h));
   }
   if (dst) {
+    const rsrc_t rs = make_rsrc(dst, static_cast<uint32_t>(P.Dk * P.Dv) * 4);
 #pragma unroll
     for (int t = 0; t < 2 * KT; ++t)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int i = 16 * t + 4 * q4 + r;
-        if (i < R.kd && col < R.vd)
-          dst[static_cast<size_t>(i) * R.sk + static_cast<size_t>(col) * R.sv] = S[t][r] * f;
+        const uint32_t o = static_cast<uint32_t>(i * R.sk + col * R.sv) * 4;
+        stb<float>(rs, i < R.kd && col < R.vd ? o : kOOB, 0, S[t][r] * f);
       }
   }
 }

@@ -10,6 +10,7 @@ namespace prnn {
 namespace {
 
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 struct StepArgs {
   LaView q, k, v;
@@ -23,19 +24,39 @@ struct StepArgs {
   float scale;
 };
 
-// L lanes x 4 columns; U rows of a thread at a time.
-template <typename T, int L, bool VEC>
+// L lanes x 4 columns, U rows of a thread at a time; one row of the next U is under way while
+// these are worked on.  What lies outside the head is read as zero and not written (an offset
+// outside the resource).
+template <typename T, int L, int U, bool VEC>
 __global__ __launch_bounds__(256) void la_step_kernel(StepArgs A) {
   constexpr int G = 256 / L;  // rows at a time
-  constexpr int U = 8;
   __shared__ float sq[kLaMaxDim], sk[kLaMaxDim];
-  __shared__ __align__(16) float so[G * L * 4];
+  __shared__ __align__(16) float so[256 * 4];
   const int tid = threadIdx.x, lane = tid % L, grp = tid / L;
   const int h = blockIdx.y, b = blockIdx.z;
   const int c0 = (blockIdx.x * L + lane) * 4;
   const int r = A.table ? A.table[b] : b;
   const bool kept = r >= 0 && r < A.rows;
-  float* S = A.state + (static_cast<size_t>(kept ? r : 0) * A.H + h) * A.Dk * A.Dv;
+  const rsrc_t S = make_rsrc(
+      A.state + (static_cast<size_t>(kept ? r : 0) * A.H + h) * A.Dk * A.Dv,
+      kept ? static_cast<uint32_t>(A.Dk * A.Dv) * 4 : 0u);
+  auto offset = [&](int i, int c) {
+    return i < A.Dk && c0 + c < A.Dv ? static_cast<uint32_t>(i * A.Dv + c0 + c) * 4 : kOOB;
+  };
+  auto load = [&](f4* s, int i0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * G;
+      if (VEC) {
+        s[u] = __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(S, offset(i, 0), 0, 0));
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s[u][c] = ldb<float>(S, offset(i, c), 0);
+      }
+    }
+  };
+  f4 s[U];
+  load(s, grp);
   const T* q = static_cast<const T*>(A.q.p) + b * A.q.sb + (h / A.q.rep) * A.q.sh;
   const T* k = static_cast<const T*>(A.k.p) + b * A.k.sb + (h / A.k.rep) * A.k.sh;
   const T* v = static_cast<const T*>(A.v.p) + b * A.v.sb + (h / A.v.rep) * A.v.sh;
@@ -49,47 +70,28 @@ __global__ __launch_bounds__(256) void la_step_kernel(StepArgs A) {
   for (int c = 0; c < 4; ++c)
     if (c0 + c < A.Dv) vv[c] = to_f32(v[c0 + c]);
   f4 o = {0, 0, 0, 0};
-  bool synced = false;
-  for (int i0 = grp; i0 < A.Dk || !synced; i0 += G * U) {
-    f4 s[U];
+  __syncthreads();
+  for (int i0 = grp; i0 < A.Dk; i0 += G * U) {
+    f4 n[U];
+    load(n, i0 + G * U);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = i0 + u * G;
-      s[u] = f4{0, 0, 0, 0};
-      if (kept && i < A.Dk) {
-        if (VEC) {
-          if (c0 < A.Dv) s[u] = *reinterpret_cast<const f4*>(S + static_cast<size_t>(i) * A.Dv + c0);
-        } else {
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (c0 + c < A.Dv) s[u][c] = S[static_cast<size_t>(i) * A.Dv + c0 + c];
-        }
-      }
-    }
-    if (!synced) {
-      __syncthreads();
-      synced = true;
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * G;
-      if (i >= A.Dk) continue;
-      const float ki = sk[i], qi = sq[i];
+      const float ki = i < A.Dk ? sk[i] : 0.0f, qi = i < A.Dk ? sq[i] : 0.0f;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         s[u][c] = fmaf(a, s[u][c], ki * vv[c]);
-        o[c] = fmaf(qi, s[u][c], o[c]);
+        if (i < A.Dk) o[c] = fmaf(qi, s[u][c], o[c]);
       }
-      if (kept) {
-        if (VEC) {
-          if (c0 < A.Dv) *reinterpret_cast<f4*>(S + static_cast<size_t>(i) * A.Dv + c0) = s[u];
-        } else {
+      if (VEC) {
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u4, s[u]), S, offset(i, 0), 0, 0);
+      } else {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (c0 + c < A.Dv) S[static_cast<size_t>(i) * A.Dv + c0 + c] = s[u][c];
-        }
+        for (int c = 0; c < 4; ++c) stb<float>(S, offset(i, c), 0, s[u][c]);
       }
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u) s[u] = n[u];
   }
   *reinterpret_cast<f4*>(&so[tid * 4]) = o;
   __syncthreads();
@@ -104,13 +106,13 @@ __global__ __launch_bounds__(256) void la_step_kernel(StepArgs A) {
   }
 }
 
-template <typename T, int L>
+template <typename T, int L, int U>
 int launch(const StepArgs& a, int B, bool vec, hipStream_t st) {
   const dim3 grid((a.Dv + 4 * L - 1) / (4 * L), a.H, B);
   if (vec)
-    la_step_kernel<T, L, true><<<grid, 256, 0, st>>>(a);
+    la_step_kernel<T, L, U, true><<<grid, 256, 0, st>>>(a);
   else
-    la_step_kernel<T, L, false><<<grid, 256, 0, st>>>(a);
+    la_step_kernel<T, L, U, false><<<grid, 256, 0, st>>>(a);
   PRNN_HIP(hipGetLastError());
   return PRNN_OK;
 }
@@ -157,6 +159,11 @@ extern "C" PRNN_API int prnn_linear_attention_step(
   const bool vec = Dv % 4 == 0 && (reinterpret_cast<uintptr_t>(state) & 15) == 0;
   return with_storage(dtype, [&](auto z) {
     using T = decltype(z);
-    return launch<T, 16>(a, B, vec, static_cast<hipStream_t>(stream));
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    // whole rows of a head side by side where there are enough of them, narrow tiles (more
+    // workgroups) for few
+    if (Dv <= 32 || 1ll * B * H < 128) return launch<T, 8, 4>(a, B, vec, st);
+    if (Dv <= 64) return launch<T, 16, 4>(a, B, vec, st);
+    return launch<T, 32, 8>(a, B, vec, st);
   });
 }

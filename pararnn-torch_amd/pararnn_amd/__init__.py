@@ -8,6 +8,7 @@ ops are registered as ``torch.library`` custom ops under the reference's
 names (``pararnn::newton_slstm_fused``, ``pararnn::newton_gru_head_fused``).
 """
 
+from pararnn_amd.attention import linear_attention, linear_attention_step
 from pararnn_amd.cells import ParaGRU, ParaSLSTM
 from pararnn_amd.decode import can_decode_step, decode_step, decode_wx
 from pararnn_amd.config import (
@@ -17,8 +18,6 @@ from pararnn_amd.config import (
     NewtonStats,
     compile_safe_config,
 )
-from pararnn_amd.group_norm import group_norm
-from pararnn_amd.linear_attention import linear_attention, linear_attention_step
 from pararnn_amd.newton import (
     auto_newton_iters,
     fused_newton,
@@ -27,6 +26,7 @@ from pararnn_amd.newton import (
     slstm_picard_next,
 )
 from pararnn_amd.layers import ParaRNN
+from pararnn_amd.norm import group_norm
 from pararnn_amd.ops import newton_gru_head_fused, newton_slstm_fused, slstm_init_fused
 from pararnn_amd.pages import (
     compact_pages,

@@ -20,22 +20,29 @@ once.  Results do not depend on the order in which workgroups run: no atomics.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 
 import torch
 from torch import Tensor
 
 from pararnn_amd import _lib
-from pararnn_amd.ops import _DTYPES, _ptr, _stream, _validate, _workspace
+from pararnn_amd.ops import _DTYPES, _validate, _workspace
 from pararnn_amd.ragged import PackedSequences
 
 
-def _on(dev: torch.device):
-    """Makes ``dev`` the current device where it is not."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(dev)
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+
+
+def _enqueue(fn, dev: torch.device, *args) -> int:
+    """``fn(*args, stream)`` with ``dev`` as the current device and its current stream.  Small calls
+    are bound by the host: the stream object that ``torch.cuda.current_stream`` builds and a guard
+    for a device that is current already take 3 us of a step's 12."""
+    index = dev.index
+    if index == _current_device():
+        return fn(*args, _raw_stream(index))
+    with torch.cuda.device(dev):
+        return fn(*args, _raw_stream(index))
 
 
 def _rows(t: Tensor) -> Tensor:
@@ -48,6 +55,8 @@ def _tiles(t: Tensor) -> Tensor:
     values give equal bits: the bfloat16 one (widths in eights) reads 16 bytes at a time, and rows
     that do not lie for that (a view of a fused projection with an odd offset) are copied."""
     t = _rows(t)
+    if abs(t.stride(1)) * t.element_size() > 1 << 24:  # the kernels' offsets inside a chunk
+        t = t.contiguous()
     if t.dtype != torch.bfloat16 or t.shape[-1] % 8:
         return t
     sb, st, sh, _ = t.stride()
@@ -98,6 +107,10 @@ def _check_table(what: str, table: Tensor, rows: int, dev: torch.device) -> Tens
         raise RuntimeError(f"{what} under graph capture needs a contiguous int32 block_table on "
                            "the state's device")
     return table.to(device=dev, dtype=torch.int32).contiguous()
+
+
+def _at(t: Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
 
 
 class _Problem:
@@ -152,37 +165,51 @@ class _Problem:
                          None if table is not None else self.sequences)
             self.h0 = h0.contiguous()
         self.scale = float(dk ** -0.5 if scale is None else scale)
+        self.codes = (g_code, code)
+        self._fill()
+
+    def _fill(self) -> None:
+        g, batch, time = self.g, self.dims[0], self.dims[1]
         at = g.stride() if g.dim() == 3 else (0, 0, g.stride(0))
-        if g.dim() == 3 and time * batch > 0 and at[0] == 0 and at[1] == 0:
-            self.g = g.contiguous()  # expanded, not per head: the gradient's layout tells them apart
-            at = self.g.stride()
+        if at[0] == 0 and at[1] == 0 and g.dim() == 3 and time * batch > 0:
+            # expanded, not per head: the gradient's layout tells them apart
+            g = self.g = g.contiguous()
+            at = g.stride()
         self.c = _lib.LaProblem(
-            _view(self.q), _view(self.k), _view(self.v), self.g.data_ptr(), *at,
-            None if self.h0 is None else self.h0.data_ptr(),
-            None if self.table is None else self.table.data_ptr(),
-            None if self.offsets is None else self.offsets.data_ptr(),
-            0 if self.h0 is None else self.h0.shape[0],
-            0 if packed is None else self.sequences, batch, time, heads, dk, dv, g_code, code,
-            self.scale)
+            _view(self.q), _view(self.k), _view(self.v), g.data_ptr(), *at, _at(self.h0),
+            _at(self.table), _at(self.offsets), 0 if self.h0 is None else self.h0.shape[0],
+            0 if self.offsets is None else self.sequences, *self.dims, *self.codes, self.scale)
+
+    def again(self, q: Tensor, k: Tensor, v: Tensor, g: Tensor, h0: Tensor | None) -> _Problem:
+        """The same checked call on tensors like those it was made of (backward)."""
+        p = object.__new__(_Problem)
+        p.q, p.k, p.v, p.g = _tiles(q), _tiles(k), _tiles(v), g
+        p.h0 = None if h0 is None else h0.contiguous()
+        p.dims, p.codes, p.scale = self.dims, self.codes, self.scale
+        p.sequences, p.offsets, p.table = self.sequences, self.offsets, None
+        p._fill()
+        return p
+
+    def forget(self) -> _Problem:
+        """Keeps what was checked, not the tensors."""
+        self.q = self.k = self.v = self.g = self.h0 = self.c = None
+        return self
 
 
 def _forward(p: _Problem, state_out: Tensor | None, table: Tensor | None) -> Tensor:
     batch, time, heads, _, dv = p.dims
-    lib, dev = _lib.load(), p.q.device
+    lib, dev, c = _lib.load(), p.q.device, ctypes.byref(p.c)
     out = p.q.new_empty(batch, time, heads, dv)
-    with _on(dev):
-        need = lib.prnn_linear_attention_workspace_size(ctypes.byref(p.c))
-        ws = _workspace(need, dev) if need else None
-        view = _view(out)
-        rc = lib.prnn_linear_attention(
-            ctypes.byref(p.c), ctypes.byref(view), _ptr(state_out), _ptr(table),
-            0 if state_out is None else state_out.shape[0], _ptr(ws), need, _stream(dev))
+    need = lib.prnn_linear_attention_workspace_size(c)
+    ws = _workspace(need, dev) if need else None
+    rc = _enqueue(lib.prnn_linear_attention, dev, c, ctypes.byref(_view(out)), _at(state_out),
+                  _at(table), 0 if state_out is None else state_out.shape[0], _at(ws), need)
     _lib.check(rc, "linear_attention")
     return out
 
 
 def _backward(p: _Problem, go: Tensor, gs: Tensor | None, need_g: bool, need_h0: bool):
-    lib, dev = _lib.load(), p.q.device
+    lib, dev, c = _lib.load(), p.q.device, ctypes.byref(p.c)
     go = _tiles(go)
     gs = None if gs is None else gs.contiguous()
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (p.q, p.k, p.v))
@@ -190,13 +217,10 @@ def _backward(p: _Problem, go: Tensor, gs: Tensor | None, need_g: bool, need_h0:
     dh0 = None
     if p.h0 is not None and (need_g or need_h0):
         dh0 = torch.empty_like(p.h0)
-    with _on(dev):
-        need = lib.prnn_linear_attention_backward_workspace_size(ctypes.byref(p.c), int(need_g))
-        ws = _workspace(need, dev) if need else None
-        view = _view(go)
-        rc = lib.prnn_linear_attention_backward(
-            ctypes.byref(p.c), ctypes.byref(view), _ptr(gs), _ptr(dq), _ptr(dk), _ptr(dv),
-            _ptr(dg), _ptr(dh0), _ptr(ws), need, _stream(dev))
+    need = lib.prnn_linear_attention_backward_workspace_size(c, int(need_g))
+    ws = _workspace(need, dev) if need else None
+    rc = _enqueue(lib.prnn_linear_attention_backward, dev, c, ctypes.byref(_view(go)), _at(gs),
+                  dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _at(dg), _at(dh0), _at(ws), need)
     _lib.check(rc, "linear_attention backward")
     return dq, dk, dv, dg, dh0
 
@@ -209,7 +233,7 @@ class _LinearAttention(torch.autograd.Function):
         state = q.new_empty(p.sequences, heads, dk, dv, dtype=torch.float32) if want_state else None
         out = _forward(p, state, None)
         ctx.save_for_backward(q, k, v, g, h0)
-        ctx.packed, ctx.scale = packed, scale
+        ctx.call = p.forget()
         ctx.set_materialize_grads(False)
         return out, state
 
@@ -219,7 +243,7 @@ class _LinearAttention(torch.autograd.Function):
         q, k, v, g, h0 = ctx.saved_tensors
         if go is None and gs is None:
             return (None,) * 8
-        p = _Problem(q, k, v, g, h0, None, ctx.packed, ctx.scale)
+        p = ctx.call.again(q, k, v, g, h0)
         if go is None:
             go = q.new_zeros(1).expand(*p.dims[:3], p.dims[4])
         if go.dtype != q.dtype:
@@ -344,14 +368,12 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
         if out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
             raise ValueError(f"{what}: out must be contiguous, of q's type and on its device")
         res = out
-    lib = _lib.load()
-    with _on(dev):
-        rc = lib.prnn_linear_attention_step(
-            q.data_ptr(), q.stride(0), q.stride(1), hq, k.data_ptr(), k.stride(0), k.stride(1),
-            hk, v.data_ptr(), v.stride(0), v.stride(1), hv, log_decay.data_ptr(), g_sb, g_sh,
-            g_code, state.data_ptr(), None if table is None else table.data_ptr(),
-            state.shape[0], res.data_ptr(), batch, heads, dk, dv,
-            dk ** -0.5 if scale is None else scale, code, _stream(dev))
+    rc = _enqueue(
+        _lib.load().prnn_linear_attention_step, dev,
+        q.data_ptr(), q.stride(0), q.stride(1), hq, k.data_ptr(), k.stride(0), k.stride(1), hk,
+        v.data_ptr(), v.stride(0), v.stride(1), hv, log_decay.data_ptr(), g_sb, g_sh, g_code,
+        state.data_ptr(), None if table is None else table.data_ptr(), state.shape[0],
+        res.data_ptr(), batch, heads, dk, dv, dk ** -0.5 if scale is None else scale, code)
     _lib.check(rc, what)
     if out is not None:
         return out

@@ -11,12 +11,14 @@ order.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 from torch import Tensor
 
 from pararnn_amd import _lib
-from pararnn_amd.linear_attention import _on
-from pararnn_amd.ops import _DTYPES, _ptr, _stream, _validate, _workspace
+from pararnn_amd.attention import _at, _enqueue
+from pararnn_amd.ops import _DTYPES, _validate, _workspace
 
 _ACTIVATIONS = {None: 0, "silu": 1, "sigmoid": 2}
 
@@ -30,22 +32,24 @@ def _shape(x: Tensor, over: str) -> tuple[int, int, int]:
     return n, (x.numel() // (n * c) if n else 0), c
 
 
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(n: int, length: int, c: int, groups: int, code: int, backward: int) -> int:
+    return _lib.load().prnn_group_norm_workspace_size(n, length, c, groups, code, backward)
+
+
 def _forward(x, weight, bias, gate, groups, eps, act, over):
     n, length, c = _shape(x, over)
-    lib = _lib.load()
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x)
     code = _DTYPES[x.dtype]
-    w_code = code if weight is None and bias is None else _DTYPES[(bias if weight is None
-                                                                   else weight).dtype]
-    need = lib.prnn_group_norm_workspace_size(n, length, c, groups, code, 0)
+    w = bias if weight is None else weight
+    need = _workspace_bytes(n, length, c, groups, code, 0)
     ws = stats = None
     if need:  # statistics per sample, or groups too wide for a wave
         ws = _workspace(need, x.device)
         stats = torch.empty(n, groups, 2, dtype=torch.float32, device=x.device)
-    with _on(x.device):
-        rc = lib.prnn_group_norm(
-            x.data_ptr(), _ptr(weight), _ptr(bias), _ptr(gate), y.data_ptr(), _ptr(stats), n,
-            length, c, groups, eps, act, w_code, code, _ptr(ws), need, _stream(x.device))
+    rc = _enqueue(_lib.load().prnn_group_norm, x.device, x.data_ptr(), _at(weight), _at(bias),
+                  _at(gate), y.data_ptr(), _at(stats), n, length, c, groups, eps, act,
+                  code if w is None else _DTYPES[w.dtype], code, _at(ws), need)
     _lib.check(rc, "group_norm")
     return y, stats
 
@@ -64,26 +68,24 @@ class _GroupNorm(torch.autograd.Function):
         x, weight, bias, gate, stats = ctx.saved_tensors
         groups, eps, act, over = ctx.args
         n, length, c = _shape(x, over)
-        lib, dev = _lib.load(), x.device
+        dev = x.device
         if gy.dtype != x.dtype:
             gy = gy.to(x.dtype)
         gy = gy.contiguous()
         if gy.data_ptr() % 16:
             gy = gy.clone()
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        dgate = None if gate is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
+        dx = torch.empty_like(x)
+        dgate = None if gate is None else torch.empty_like(x)
         dw = None if weight is None else torch.empty_like(weight)
         db = None if bias is None else torch.empty_like(bias)
         code = _DTYPES[x.dtype]
-        w_code = code if weight is None and bias is None else _DTYPES[(bias if weight is None
-                                                                       else weight).dtype]
-        need = lib.prnn_group_norm_workspace_size(n, length, c, groups, code, 1)
+        w = bias if weight is None else weight
+        need = _workspace_bytes(n, length, c, groups, code, 1)
         ws = _workspace(need, dev)
-        with _on(dev):
-            rc = lib.prnn_group_norm_backward(
-                gy.data_ptr(), x.data_ptr(), _ptr(weight), _ptr(bias), _ptr(gate), _ptr(stats),
-                dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(dgate), n, length, c, groups, eps, act,
-                w_code, code, ws.data_ptr(), ws.numel(), _stream(dev))
+        rc = _enqueue(_lib.load().prnn_group_norm_backward, dev, gy.data_ptr(), x.data_ptr(),
+                      _at(weight), _at(bias), _at(gate), _at(stats), dx.data_ptr(), _at(dw),
+                      _at(db), _at(dgate), n, length, c, groups, eps, act,
+                      code if w is None else _DTYPES[w.dtype], code, ws.data_ptr(), ws.numel())
         _lib.check(rc, "group_norm backward")
         need_in = ctx.needs_input_grad
         return (dx if need_in[0] else None, dw, db, dgate, None, None, None, None)

@@ -20,8 +20,7 @@ import torch
 from torch import Tensor
 
 from pararnn_amd import _lib
-from pararnn_amd.linear_attention import _on
-from pararnn_amd.ops import _ptr, _stream
+from pararnn_amd.attention import _enqueue
 
 
 def _used(what: str, used: Tensor) -> Tensor:
@@ -74,9 +73,8 @@ def take_pages(used: Tensor, n: int) -> Tensor:
     if n < 0:
         raise ValueError(f"take_pages: n must be >= 0, got {n!r}")
     out = torch.empty(n, dtype=torch.int32, device=dev)
-    with _on(dev):
-        rc = _lib.load().prnn_pages_take(used.data_ptr(), used.shape[0], _ptr(out), n,
-                                         _stream(dev))
+    rc = _enqueue(_lib.load().prnn_pages_take, dev, used.data_ptr(), used.shape[0],
+                  out.data_ptr(), n)
     _lib.check(rc, "take_pages")
     return out
 
@@ -90,10 +88,8 @@ def fork_pages(used: Tensor, pools: Sequence[Tensor] | Tensor, parents: Tensor) 
     parents = _list("fork_pages", "parents", parents, dev)
     n = parents.shape[0]
     both = torch.empty(2, n, dtype=torch.int32, device=dev)
-    with _on(dev):
-        rc = _lib.load().prnn_pages_fork(used.data_ptr(), used.shape[0], rows, n_pools,
-                                         parents.data_ptr(), both.data_ptr(), n,
-                                         both.data_ptr() + 4 * n, _stream(dev))
+    rc = _enqueue(_lib.load().prnn_pages_fork, dev, used.data_ptr(), used.shape[0], rows, n_pools,
+                  parents.data_ptr(), both.data_ptr(), n, both.data_ptr() + 4 * n)
     _lib.check(rc, "fork_pages")
     return both[0]
 
@@ -102,9 +98,8 @@ def free_pages(used: Tensor, slots: Tensor) -> None:
     """Gives ``slots`` ``(n,)`` back; entries that are no slots are passed over."""
     dev = _used("free_pages", used).device
     slots = _list("free_pages", "slots", slots, dev)
-    with _on(dev):
-        rc = _lib.load().prnn_pages_free(used.data_ptr(), used.shape[0], slots.data_ptr(),
-                                         slots.shape[0], _stream(dev))
+    rc = _enqueue(_lib.load().prnn_pages_free, dev, used.data_ptr(), used.shape[0],
+                  slots.data_ptr(), slots.shape[0])
     _lib.check(rc, "free_pages")
 
 
@@ -118,9 +113,8 @@ def copy_pages(pools: Sequence[Tensor] | Tensor, src: Tensor, dst: Tensor) -> No
     dst = _list("copy_pages", "dst", dst, dev)
     if src.shape != dst.shape:
         raise ValueError(f"copy_pages: src {tuple(src.shape)} != dst {tuple(dst.shape)}")
-    with _on(dev):
-        rc = _lib.load().prnn_pages_copy(slots, rows, n_pools, src.data_ptr(), dst.data_ptr(),
-                                         src.shape[0], _stream(dev))
+    rc = _enqueue(_lib.load().prnn_pages_copy, dev, slots, rows, n_pools, src.data_ptr(),
+                  dst.data_ptr(), src.shape[0])
     _lib.check(rc, "copy_pages")
 
 
@@ -146,9 +140,7 @@ def compact_pages(used: Tensor, pools: Sequence[Tensor] | Tensor,
     scratch = torch.empty(2 + 2 * used.shape[0], dtype=torch.int32, device=dev)
     ptrs = (ctypes.c_void_p * max(1, n))(*(t.data_ptr() for t in tables))
     lens = (ctypes.c_int * max(1, n))(*(t.numel() for t in tables))
-    with _on(dev):
-        rc = _lib.load().prnn_pages_compact(
-            used.data_ptr(), used.shape[0], rows, n_pools, ptrs, lens, n, scratch.data_ptr(),
-            scratch.data_ptr() + 4, _stream(dev))
+    rc = _enqueue(_lib.load().prnn_pages_compact, dev, used.data_ptr(), used.shape[0], rows,
+                  n_pools, ptrs, lens, n, scratch.data_ptr(), scratch.data_ptr() + 4)
     _lib.check(rc, what)
     return scratch[0]
