@@ -90,6 +90,7 @@ struct LaParams {
   LaSeqs seqs;
   int H, Dk, Dv;
   int tiles;            // column tiles of the widest role (the grid's)
+  int roles, near;      // near: consecutive heads that share arrays
   int batch_tokens;     // tokens of the whole batch (dots' rows)
 };
 
@@ -179,17 +180,15 @@ __device__ __forceinline__ float la_decay(const LaDecay& d, int b, int t, int h)
   return la_decay_value(d, la_decay_bits(d, b, t, h));
 }
 
-// The log decay of a step of the walk that reaches token t: forwards g_t, backwards the next
-// token's (none, and zero bits are a zero of every type, behind the sequence's last token).
-__device__ __forceinline__ uint32_t la_step_decay(const LaDecay& d, int rev, const LaPiece& pc,
-                                                  int b, int t, int h) {
-  if (!rev) return la_decay_bits(d, b, t, h);
-  return t + 1 < pc.s1 ? la_decay_bits(d, b, t + 1, h) : 0u;
-}
-
 // Batch of a piece: rectangular sequences are batches of their own.
 __device__ __forceinline__ int la_batch(const LaSeqs& q, const LaPiece& pc) {
   return q.cu ? 0 : pc.seq;
+}
+
+// A byte offset in a buffer, or one outside it.  Arithmetic and not a choice: the compiler turns
+// `in ? offset : kOOB` around a load into two branches with a load each.
+__device__ __forceinline__ uint32_t la_in(bool in, uint32_t offset) {
+  return offset | (static_cast<uint32_t>(!in) << 31);
 }
 
 // A head's rows of an array: a buffer resource at the lowest row of a chunk of C tokens of the
@@ -202,6 +201,33 @@ __device__ __forceinline__ rsrc_t la_rows(const LaView& v, int size, int b, int 
                    0x7fffffffu);
 }
 
+// The decays of C tokens of the walk from local index base, lane i's in place: forwards g of the
+// token that a step reaches, backwards the next token's (none, and zero bits are a zero of every
+// type, behind the sequence's last token and outside the piece).  Nothing here is a branch, and
+// either width is loaded, one of them from an empty buffer: behind a branch the wave would wait
+// for the load as soon as the ways meet, and with it for all loads before.
+struct LaBits {
+  uint32_t wide, narrow;
+  __device__ __forceinline__ uint32_t get() const { return wide | narrow; }
+};
+template <int C>
+__device__ __forceinline__ LaBits la_step_decays(const LaDecay& d, int rev, const LaPiece& pc,
+                                                   int b, int h, int base, int lane) {
+  const int size = d.dtype == PRNN_F32 ? 4 : 2;
+  const int left = pc.end - pc.begin - base;
+  // lowest token of the C (backwards: behind the lowest that is walked)
+  const int low = rev ? pc.end - base - C + 1 : pc.begin + base;
+  const int row = rev ? C - 1 - lane : lane;
+  const bool in = (lane < left) & (lane < C) & (low + row < pc.s1);
+  const char* p = static_cast<const char*>(d.p) +
+                  (b * d.sb + static_cast<long long>(low) * d.st + h * d.sh) * size;
+  const uint32_t o = la_in(in, static_cast<uint32_t>(row * static_cast<int>(d.st)) * size);
+  LaBits bits;
+  bits.wide = __builtin_amdgcn_raw_buffer_load_b32(make_rsrc(p, size == 4 ? 0x7fffffffu : 0u), o, 0, 0);
+  bits.narrow = __builtin_amdgcn_raw_buffer_load_b16(make_rsrc(p, size == 4 ? 0u : 0x7fffffffu), o, 0, 0);
+  return bits;
+}
+
 // First piece of sequence s and their number.
 __device__ __forceinline__ void la_pieces_of(const LaSeqs& q, int s, int& p0, int& n) {
   if (q.cu == nullptr) {
@@ -212,6 +238,34 @@ __device__ __forceinline__ void la_pieces_of(const LaSeqs& q, int s, int& p0, in
     p0 = s + s0 / q.len;
     n = s1 > s0 ? (s1 - 1) / q.len - s0 / q.len + 1 : 1;
   }
+}
+
+// Where a workgroup of the walks works.  Workgroups go to the 8 XCDs in turn, each with an L2 of
+// its own, so those that read the same rows (the roles and column tiles of a piece, and the heads
+// that share arrays) are 8 apart and next to each other on one XCD.
+struct LaPlace {
+  int role, tile, piece, h;
+  bool any;
+};
+__device__ __forceinline__ LaPlace la_place(const LaParams& p) {
+  const int same = p.roles * p.tiles * p.near;
+  const int group = blockIdx.x / (8 * same), in = blockIdx.x - group * 8 * same;
+  int sub = in >> 3;
+  const int item = group * 8 + (in & 7);  // piece and the first of `near` heads
+  const int heads = p.H / p.near;
+  LaPlace r;
+  r.piece = item / heads;
+  r.h = (item - r.piece * heads) * p.near;
+  const int k = sub / p.near;
+  r.h += sub - k * p.near;
+  r.role = k / p.tiles;
+  r.tile = k - r.role * p.tiles;
+  r.any = r.piece < p.seqs.pieces;
+  return r;
+}
+inline unsigned la_grid(const LaParams& p) {
+  const long long items = 1ll * p.seqs.pieces * (p.H / p.near);
+  return static_cast<unsigned>((items + 7) / 8 * 8 * p.roles * p.tiles * p.near);
 }
 
 inline int la_widest(const LaParams& p, int roles) {

@@ -234,6 +234,8 @@ int check(const Problem* a) {
   for (const prnn_la_view* v : {&a->q, &a->k, &a->v})
     if (!la_stride_fits(v->st, size))
       return fail(PRNN_ERR_VALUE, "tokens %lld elements apart are too far (16 MiB)", v->st);
+  if (!la_stride_fits(a->g_st, 4))
+    return fail(PRNN_ERR_VALUE, "decays %lld elements apart are too far (16 MiB)", a->g_st);
   if (!la_stride_fits(1ll * a->H * std::max(a->Dk, a->Dv), 4))
     return fail(PRNN_ERR_VALUE, "H=%d heads of (%d, %d) are too wide", a->H, a->Dk, a->Dv);
   if (a->h0 && a->h0_rows < 0) return fail(PRNN_ERR_VALUE, "h0_rows=%d", a->h0_rows);
@@ -369,6 +371,11 @@ LaParams params(const Problem& a, const LaSeqs& q) {
   p.Dk = a.Dk;
   p.Dv = a.Dv;
   p.batch_tokens = a.B * a.T;
+  // heads that share q, k or v: up to 8 of them side by side
+  const int shared = a.H / std::min({a.q.heads, a.k.heads, a.v.heads});
+  p.near = 1;
+  for (int n = 2; n <= 8; ++n)
+    if (shared % n == 0) p.near = n;
   return p;
 }
 

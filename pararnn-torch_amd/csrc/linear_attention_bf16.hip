@@ -35,11 +35,15 @@ __device__ __forceinline__ f16v mfma(b8 a, b8 b, f16v c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-// Bytes of an LDS row.  x and y are read 16 bytes a lane down 16 rows (an odd number of 16-byte
-// units lets them fall into different banks) and y and z 64 bytes along 4 rows (z: exactly 64
-// bytes apart; y's rows overlap by a quarter, a two-way conflict in those banks).
-constexpr int row_xy(int cols) { return cols >= 128 ? cols * 2 + 48 : cols * 2 + 16; }
-constexpr int row_z(int cols) { return cols == 32 ? 64 : cols * 2 + 64; }
+// LDS rows.  x is read 16 bytes a lane down 16 rows: its 16-byte units are exchanged by the row's
+// number so that these fall into different banks.  y and z are also read 64 bytes along 4 rows,
+// for which a pad does (y's four windows overlap by a quarter or a half: two-way conflicts there).
+template <int U>
+__device__ __forceinline__ int exchange_x(int row) {
+  return (U >= 16 ? row & 15 : U == 8 ? (row >> 1) & 7 : (row >> 2) & 3) << 4;
+}
+constexpr int row_y(int cols) { return cols >= 128 ? cols * 2 + 48 : cols * 2 + 16; }
+constexpr int row_z(int cols) { return cols == 32 ? 64 : cols == 64 ? 144 : cols * 2 + 48; }
 
 // Two transposing loads: this lane's column (c0 + lane % 32) at 8 tokens of the 16 from t0.
 // `at`: the tile with this lane's share of the address, across_share.
@@ -83,27 +87,44 @@ __device__ __forceinline__ b8 split8(float* x) {
   return r.v;
 }
 
+// Inclusive running sum over the wave's lanes: rows of 16 by shifts, then the rows' last lanes
+// handed on.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_add(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ float scan_up(float v) {
+  v = dpp_add<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+  v = dpp_add<0x112, 0xf>(v);
+  v = dpp_add<0x114, 0xf>(v);
+  v = dpp_add<0x118, 0xf>(v);
+  v = dpp_add<0x142, 0xa>(v);  // lane 15 of a row to the next (rows 1 and 3)
+  v = dpp_add<0x143, 0xc>(v);  // lane 31 to rows 2 and 3
+  return v;
+}
+
 template <int KD, int W, bool STATE_ONLY, bool FINE>
-__global__ __launch_bounds__(64 * W, (KD >= 256 || (W == 1 && KD >= 128)) ? 1 : 2)
+__global__ __launch_bounds__(64 * W, (KD >= 256 || (W < 4 && KD >= 128)) ? 1 : 2)
 void la_walk_bf16_kernel(LaParams P) {
   constexpr int NT = 64 * W, VT = 32 * W;
   constexpr int UX = KD / 8, UZ = VT / 8;      // 16-byte units of a row
   constexpr int NX = kC * UX / NT, NZ = kC * UZ / NT;
   constexpr int KT = KD / 32;                  // 32-row tiles of the state
-  constexpr int RX = row_xy(KD), RZ = row_z(VT);
+  constexpr int RX = KD * 2, RY = row_y(KD), RZ = row_z(VT);
   constexpr int KX = STATE_ONLY ? 0 : kC * RX;
   constexpr int KP = STATE_ONLY ? 0 : 3 * 2 * 64 * 16 * (FINE ? 2 : 1);
   __shared__ __align__(16) char sx[KX ? KX : 16];
-  __shared__ __align__(16) char sy[kC * RX];
+  __shared__ __align__(16) char sy[kC * RY];
   __shared__ __align__(16) char sz[kC * RZ];
   __shared__ __align__(16) char sp[KP ? KP : 16];
   __shared__ __align__(16) float sG[kC], se[kC], sw[kC];
   __shared__ float sdot[W][kC], s_tot, s_sum;
   __shared__ int s_stop[2];
 
-  const LaRole& R = P.role[blockIdx.z];
-  const int h = blockIdx.y;
-  const int tile = blockIdx.x % P.tiles, piece = blockIdx.x / P.tiles;
+  const LaPlace place = la_place(P);
+  if (!place.any) return;
+  const LaRole& R = P.role[place.role];
+  const int h = place.h, tile = place.tile, piece = place.piece;
   if (tile * VT >= R.vd) return;
   const LaPiece pc = la_piece(P.seqs, piece);
   if (STATE_ONLY) {
@@ -119,6 +140,65 @@ void la_walk_bf16_kernel(LaParams P) {
   const int col = col0 + 32 * wave + l32;  // this lane's column of the state
   const size_t row_floats = static_cast<size_t>(P.H) * P.Dk * P.Dv;
   const size_t head_floats = static_cast<size_t>(h) * P.Dk * P.Dv;
+
+  const int n_tok = pc.end - pc.begin;
+  float sum_decay = 0.0f;
+  auto token = [&](int i) { return R.rev ? pc.end - 1 - i : pc.begin + i; };
+
+  // A thread's loads of an array are rows apart by a constant number.  What lies outside the
+  // piece or the width is read as zero (an offset outside the resource).
+  constexpr int DX = NT / UX, DZ = NT / UZ;
+  const int rowx = tid / UX, cx = (tid % UX) * 8, rowz = tid / UZ, cz = col0 + (tid % UZ) * 8;
+  const bool inx = cx < R.kd, inz = cz < R.vd;
+  const int stx = static_cast<int>(R.x.st) * 2, sty = static_cast<int>(R.y.st) * 2,
+            stz = static_cast<int>(R.z.st) * 2;
+  const int fx = R.rev ? kC - 1 - rowx : rowx, fz = R.rev ? kC - 1 - rowz : rowz;
+  const int ahead = R.rev ? -1 : 1;
+  u4 rx[STATE_ONLY ? 1 : NX], ry[NX], rz[NZ];
+  LaBits rg{0, 0};
+  auto fetch = [&](int base) {
+    const int left = n_tok - base;
+    rg = la_step_decays<kC>(P.g, R.rev, pc, b, h, base, lane);
+    if (!STATE_ONLY) {
+      const rsrc_t bx = la_rows<kC>(R.x, 2, b, h, R.rev, pc.begin, pc.end, base);
+#pragma unroll
+      for (int k = 0; k < NX; ++k) {
+        const uint32_t o = (fx + ahead * k * DX) * stx + cx * 2;
+        rx[k] = __builtin_amdgcn_raw_buffer_load_b128(bx, la_in(inx & (rowx + k * DX < left), o), 0, 0);
+      }
+    }
+    const rsrc_t by = la_rows<kC>(R.y, 2, b, h, R.rev, pc.begin, pc.end, base);
+#pragma unroll
+    for (int k = 0; k < NX; ++k) {
+      const uint32_t o = (fx + ahead * k * DX) * sty + cx * 2;
+      ry[k] = __builtin_amdgcn_raw_buffer_load_b128(by, la_in(inx & (rowx + k * DX < left), o), 0, 0);
+    }
+    const rsrc_t bz = la_rows<kC>(R.z, 2, b, h, R.rev, pc.begin, pc.end, base);
+#pragma unroll
+    for (int k = 0; k < NZ; ++k) {
+      const uint32_t o = (fz + ahead * k * DZ) * stz + cz * 2;
+      rz[k] = __builtin_amdgcn_raw_buffer_load_b128(bz, la_in(inz & (rowz + k * DZ < left), o), 0, 0);
+    }
+  };
+  // Decays of the chunk's first `n` tokens: running sums from the front for the pairs and the
+  // state's part, from the back for what enters the state, so that each weight that counts is the
+  // exponential of a short sum.
+  auto decays = [&](uint32_t bits, int n) {
+    const float g = lane < n ? la_decay_value(P.g, bits) : 0.0f;
+    const float G = scan_up(g);
+    const float last = __shfl(G, kC - 1);
+    const float back = scan_up(__shfl(g, kC - 1 - lane));  // lane l: the sum of the last l + 1
+    const float behind = __shfl(back, (kC - 2 - lane) & 63);
+    sG[lane] = G;
+    se[lane] = fexp(G) * R.x_scale;
+    sw[lane] = lane == kC - 1 ? R.u_scale : fexp(behind) * R.u_scale;
+    if (lane == 0) {
+      s_tot = fexp(last);
+      s_sum = last;
+    }
+  };
+  if (tid < 2) s_stop[tid] = kC;
+  fetch(0);
 
   // ---- the state before the piece
   f16v S[KT];
@@ -140,98 +220,56 @@ void la_walk_bf16_kernel(LaParams P) {
         for (int r = 0; r < 16; ++r) {
           const int i = 32 * t + 8 * (r >> 2) + 4 * half + (r & 3);
           const uint32_t o = static_cast<uint32_t>(i * R.sk + col * R.sv) * 4;
-          S[t][r] = ldb<float>(rs, i < R.kd && col < R.vd ? o : kOOB, 0);
+          S[t][r] = ldb<float>(rs, la_in((i < R.kd) & (col < R.vd), o), 0);
         }
     }
   }
-
-  const int n_tok = pc.end - pc.begin;
-  float sum_decay = 0.0f;
-  auto token = [&](int i) { return R.rev ? pc.end - 1 - i : pc.begin + i; };
-
-  // A thread's loads of an array are rows apart by a constant number.  What lies outside the
-  // piece or the width is read as zero (an offset outside the resource).
-  constexpr int DX = NT / UX, DZ = NT / UZ;
-  const int rowx = tid / UX, cx = (tid % UX) * 8, rowz = tid / UZ, cz = col0 + (tid % UZ) * 8;
-  const bool inx = cx < R.kd, inz = cz < R.vd;
-  const int stx = static_cast<int>(R.x.st) * 2, sty = static_cast<int>(R.y.st) * 2,
-            stz = static_cast<int>(R.z.st) * 2;
-  const int fx = R.rev ? kC - 1 - rowx : rowx, fz = R.rev ? kC - 1 - rowz : rowz;
-  const int ahead = R.rev ? -1 : 1;
-  u4 rx[STATE_ONLY ? 1 : NX], ry[NX], rz[NZ];
-  uint32_t rg = 0;
-  auto fetch = [&](int base) {
-    const int left = n_tok - base;
-    if (wave == 0)
-      rg = lane < left ? la_step_decay(P.g, R.rev, pc, b, token(base + lane), h) : 0u;
-    if (!STATE_ONLY) {
-      const rsrc_t bx = la_rows<kC>(R.x, 2, b, h, R.rev, pc.begin, pc.end, base);
-#pragma unroll
-      for (int k = 0; k < NX; ++k) {
-        const uint32_t o = (fx + ahead * k * DX) * stx + cx * 2;
-        rx[k] = __builtin_amdgcn_raw_buffer_load_b128(bx, inx && rowx + k * DX < left ? o : kOOB, 0, 0);
-      }
-    }
-    const rsrc_t by = la_rows<kC>(R.y, 2, b, h, R.rev, pc.begin, pc.end, base);
-#pragma unroll
-    for (int k = 0; k < NX; ++k) {
-      const uint32_t o = (fx + ahead * k * DX) * sty + cx * 2;
-      ry[k] = __builtin_amdgcn_raw_buffer_load_b128(by, inx && rowx + k * DX < left ? o : kOOB, 0, 0);
-    }
-    const rsrc_t bz = la_rows<kC>(R.z, 2, b, h, R.rev, pc.begin, pc.end, base);
-#pragma unroll
-    for (int k = 0; k < NZ; ++k) {
-      const uint32_t o = (fz + ahead * k * DZ) * stz + cz * 2;
-      rz[k] = __builtin_amdgcn_raw_buffer_load_b128(bz, inz && rowz + k * DZ < left ? o : kOOB, 0, 0);
-    }
-  };
-  // Decays of the chunk's first `n` tokens: running sums in fp64, so that what is left of the
-  // whole keeps its digits.
-  auto decays = [&](uint32_t bits, int n) {
-    double G = lane < n ? la_decay_value(P.g, bits) : 0.0f;
-#pragma unroll
-    for (int d = 1; d < kC; d <<= 1) {
-      const double o = __shfl_up(G, d);
-      if (lane >= d) G += o;
-    }
-    const double last = __shfl(G, kC - 1);
-    sG[lane] = static_cast<float>(G);
-    se[lane] = fexp(static_cast<float>(G)) * R.x_scale;
-    sw[lane] = fexp(static_cast<float>(last - G)) * R.u_scale;
-    if (lane == 0) {
-      s_tot = fexp(static_cast<float>(last));
-      s_sum = static_cast<float>(last);
-    }
-  };
-  if (tid < 2) s_stop[tid] = kC;
-  if (n_tok > 0) fetch(0);
   __syncthreads();
 
   int next = 0;
   for (int base = 0, turn = 0; base < n_tok; base = next, turn ^= 1) {
     // x: columns 0-3 | 8-11 and 4-7 | 12-15 of every 16 side by side
-    const int ox = rowx * RX + (tid % UX >> 1) * 32 + (tid & 1) * 8;
 #pragma unroll
     for (int k = 0; k < NX; ++k) {
+      const int row = rowx + k * DX;
       if (!STATE_ONLY) {
-        *reinterpret_cast<uint2*>(sx + ox + k * DX * RX) = uint2{rx[k][0], rx[k][1]};
-        *reinterpret_cast<uint2*>(sx + ox + 16 + k * DX * RX) = uint2{rx[k][2], rx[k][3]};
+        const int o = row * RX + (tid & 1) * 8, u = (tid % UX >> 1) * 32, f = exchange_x<UX>(row);
+        *reinterpret_cast<u2*>(sx + o + (u ^ f)) = u2{rx[k][0], rx[k][1]};
+        *reinterpret_cast<u2*>(sx + o + ((u | 16) ^ f)) = u2{rx[k][2], rx[k][3]};
       }
-      *reinterpret_cast<u4*>(sy + (rowx + k * DX) * RX + cx * 2) = ry[k];
+      *reinterpret_cast<u4*>(sy + row * RY + cx * 2) = ry[k];
     }
+    int stop_here = kC;
 #pragma unroll
-    for (int k = 0; k < NZ; ++k) {
+    for (int k = NZ - 1; k >= 0; --k) {
       *reinterpret_cast<u4*>(sz + (rowz + k * DZ) * RZ + (tid % UZ) * 16) = rz[k];
       // an exponent of ones: infinity or NaN
       uint32_t bad = 0;
 #pragma unroll
       for (int q = 0; q < 4; ++q) bad |= (rz[k][q] & 0x7f807f80u) + 0x00800080u;
-      if ((bad & 0x80008000u) && rowz + k * DZ > 0) atomicMin(&s_stop[turn], rowz + k * DZ);
+      if ((bad & 0x80008000u) && rowz + k * DZ > 0) stop_here = rowz + k * DZ;
     }
-    const uint32_t g_here = rg;
-    if (wave == 0) decays(rg, kC);
+    if (stop_here < kC) atomicMin(&s_stop[turn], stop_here);
+    const uint32_t g_here = rg.get();
+    if (wave == 0) decays(rg.get(), kC);
+    // the rows that the output is multiplied with, ahead of the next chunk's: what is waited for
+    // first is loaded first
+    u2 dv[2][4];
+    if (FINE) {
+      const rsrc_t bd = la_rows<kC>(R.dot, 2, b, h, R.rev, pc.begin, pc.end, base);
+#pragma unroll
+      for (int it = 0; it < 2; ++it) {
+        const int i = 32 * it + l32, row = R.rev ? kC - 1 - i : i;
+        const int c4 = col0 + 32 * wave + 4 * half;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          dv[it][q] = __builtin_amdgcn_raw_buffer_load_b64(
+              bd, la_in((R.dots != nullptr) & (base + i < n_tok) & (c4 + 8 * q < R.vd),
+                        (row * static_cast<int>(R.dot.st) + c4 + 8 * q) * 2), 0, 0);
+      }
+    }
     next = base + kC;
-    if (next < n_tok) fetch(next);
+    fetch(next);  // behind the piece's end nothing is loaded; a branch would be waited at
     __syncthreads();
     if (tid == 0) s_stop[turn ^ 1] = kC;
     const int stop = s_stop[turn];
@@ -239,13 +277,13 @@ void la_walk_bf16_kernel(LaParams P) {
       // A masked pair is an exact zero, but zero times an infinity or NaN of a later token is
       // not: where z holds one behind the chunk's first token (rare), the chunk ends before it
       // and the next one begins there.
-      for (int e = tid; e < (kC - stop) * (RX / 16); e += NT)
-        *reinterpret_cast<u4*>(sy + stop * RX + e * 16) = u4{0, 0, 0, 0};
+      for (int e = tid; e < (kC - stop) * (RY / 16); e += NT)
+        *reinterpret_cast<u4*>(sy + stop * RY + e * 16) = u4{0, 0, 0, 0};
       for (int e = tid; e < (kC - stop) * (RZ / 16); e += NT)
         *reinterpret_cast<u4*>(sz + stop * RZ + e * 16) = u4{0, 0, 0, 0};
       if (wave == 0) decays(g_here, stop);
       next = base + stop;
-      if (next < n_tok) fetch(next);
+      fetch(next);
       __syncthreads();
     }
     const int n_here = min(n_tok, next) - base;  // tokens of this chunk
@@ -259,8 +297,9 @@ void la_walk_bf16_kernel(LaParams P) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
         const int i = 32 * it + l32;
-        const char* yr = sy + (32 * jt + l32) * RX + 8 * half;
-        const char* xr = sx + i * RX + 16 * half;
+        const char* yr = sy + (32 * jt + l32) * RY + 8 * half;
+        const char* xr = sx + i * RX;
+        const int f = exchange_x<UX>(i) ^ (16 * half);
 #pragma unroll
         for (int k = 0; k < KD / 16; ++k) {
           union {
@@ -269,17 +308,20 @@ void la_walk_bf16_kernel(LaParams P) {
           } y;
           y.h[0] = *reinterpret_cast<const uint2*>(yr + 32 * k);
           y.h[1] = *reinterpret_cast<const uint2*>(yr + 32 * k + 16);
-          acc = mfma(y.v, *reinterpret_cast<const b8*>(xr + 32 * k), acc);
+          acc = mfma(y.v, *reinterpret_cast<const b8*>(xr + (f ^ 32 * k)), acc);
         }
         const float Gi = sG[i];
+        // the mask as bits, not as a choice: the compiler would branch round every exponential
+        const int before = 32 * jt + 4 * half - i - 1;
         float w[16];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const int j0 = 32 * jt + 8 * q + 4 * half;
-          const f4 Gj = *reinterpret_cast<const f4*>(&sG[j0]);
+          const f4 Gj = *reinterpret_cast<const f4*>(&sG[32 * jt + 8 * q + 4 * half]);
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            w[4 * q + r] = j0 + r <= i ? acc[4 * q + r] * (R.p_scale * fexp(Gi - Gj[r])) : 0.0f;
+            w[4 * q + r] = __int_as_float(
+                __float_as_int(acc[4 * q + r] * (R.p_scale * fexp(Gi - Gj[r]))) &
+                ((before + 8 * q + r) >> 31));
         }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
@@ -306,7 +348,8 @@ void la_walk_bf16_kernel(LaParams P) {
         const b8 s1 = FINE ? pack8(x) : s0;
 #pragma unroll
         for (int it = 0; it < 2; ++it) {
-          const b8 xr = *reinterpret_cast<const b8*>(sx + (32 * it + l32) * RX + 16 * half + 32 * k);
+          const b8 xr = *reinterpret_cast<const b8*>(
+              sx + (32 * it + l32) * RX + (exchange_x<UX>(l32) ^ (16 * half) ^ (32 * k)));
           O[it] = mfma(s0, xr, O[it]);
           if (FINE) O[it] = mfma(s1, xr, O[it]);
         }
@@ -349,24 +392,26 @@ void la_walk_bf16_kernel(LaParams P) {
       const LaView ov{R.out, R.o_sb, R.o_st, R.o_sh, 1, 1};
       const int so = R.out_f32 ? 4 : 2;
       const rsrc_t bo = la_rows<kC>(ov, so, b, h, R.rev, pc.begin, pc.end, base);
-      rsrc_t bd = bo;
-      if (FINE && R.dots) bd = la_rows<kC>(R.dot, 2, b, h, R.rev, pc.begin, pc.end, base);
 #pragma unroll
       for (int it = 0; it < 2; ++it) {
         const int i = 32 * it + l32, row = R.rev ? kC - 1 - i : i;
         const int c4 = col0 + 32 * wave + 4 * half;
         const uint32_t at = (row * static_cast<int>(R.o_st) + c4) * so;
-        u2 dv[4];
-        if (FINE && R.dots)
+        if (FINE) {
+          float d = 0.0f;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const uint32_t o = (row * static_cast<int>(R.dot.st) + c4 + 8 * q) * 2;
-            dv[q] = __builtin_amdgcn_raw_buffer_load_b64(
-                bd, i < n_here && c4 + 8 * q < R.vd ? o : kOOB, 0, 0);
+            d = fmaf(O[it][4 * q], lo_bf16(dv[it][q][0]), d);
+            d = fmaf(O[it][4 * q + 1], hi_bf16(dv[it][q][0]), d);
+            d = fmaf(O[it][4 * q + 2], lo_bf16(dv[it][q][1]), d);
+            d = fmaf(O[it][4 * q + 3], hi_bf16(dv[it][q][1]), d);
           }
+          d += __shfl_xor(d, 32);
+          if (half == 0) sdot[wave][i] = d;
+        }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const uint32_t o = i < n_here && c4 + 8 * q < R.vd ? at + 8 * q * so : kOOB;
+          const uint32_t o = la_in((i < n_here) & (c4 + 8 * q < R.vd), at + 8 * q * so);
           const float v[4] = {O[it][4 * q], O[it][4 * q + 1], O[it][4 * q + 2], O[it][4 * q + 3]};
           if (R.out_f32)
             __builtin_amdgcn_raw_buffer_store_b128(
@@ -375,18 +420,6 @@ void la_walk_bf16_kernel(LaParams P) {
           else
             __builtin_amdgcn_raw_buffer_store_b64(
                 u2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])}, bo, o, 0, 0);
-        }
-        if (FINE && R.dots) {
-          float d = 0.0f;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            d = fmaf(O[it][4 * q], lo_bf16(dv[q][0]), d);
-            d = fmaf(O[it][4 * q + 1], hi_bf16(dv[q][0]), d);
-            d = fmaf(O[it][4 * q + 2], lo_bf16(dv[q][1]), d);
-            d = fmaf(O[it][4 * q + 3], hi_bf16(dv[q][1]), d);
-          }
-          d += __shfl_xor(d, 32);
-          if (half == 0) sdot[wave][i] = d;
         }
       }
     }
@@ -411,7 +444,7 @@ void la_walk_bf16_kernel(LaParams P) {
       const b8 z0 = split8(x), z1 = split8(x), z2 = pack8(x);
 #pragma unroll
       for (int t = 0; t < KT; ++t) {
-        const b8 y = load_across<RX>(sy + across_share<RX>(lane), 16 * ts, 32 * t);
+        const b8 y = load_across<RY>(sy + across_share<RY>(lane), 16 * ts, 32 * t);
         S[t] = mfma(y, z0, S[t]);
         S[t] = mfma(y, z1, S[t]);
         S[t] = mfma(y, z2, S[t]);
@@ -447,14 +480,14 @@ void la_walk_bf16_kernel(LaParams P) {
       for (int r = 0; r < 16; ++r) {
         const int i = 32 * t + 8 * (r >> 2) + 4 * half + (r & 3);
         const uint32_t o = static_cast<uint32_t>(i * R.sk + col * R.sv) * 4;
-        stb<float>(rs, i < R.kd && col < R.vd ? o : kOOB, 0, S[t][r] * f);
+        stb<float>(rs, la_in((i < R.kd) & (col < R.vd), o), 0, S[t][r] * f);
       }
   }
 }
 
 template <int KD, int W>
-int launch(const LaParams& p, int roles, bool state_only, bool fine, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(p.seqs.pieces) * p.tiles, p.H, roles), block(64 * W);
+int launch(const LaParams& p, bool state_only, bool fine, hipStream_t stream) {
+  const unsigned grid = la_grid(p), block = 64 * W;
   if (state_only)
     la_walk_bf16_kernel<KD, W, true, false><<<grid, block, 0, stream>>>(p);
   else if (fine)
@@ -468,9 +501,9 @@ int launch(const LaParams& p, int roles, bool state_only, bool fine, hipStream_t
 template <int KD>
 int launch_kd(const LaParams& p, int roles, bool state_only, bool fine, hipStream_t stream) {
   const int cols = la_bf16_tile_cols(la_widest(p, roles));
-  if (cols == 32) return launch<KD, 1>(p, roles, state_only, fine, stream);
-  if (cols == 64) return launch<KD, 2>(p, roles, state_only, fine, stream);
-  return launch<KD, 4>(p, roles, state_only, fine, stream);
+  if (cols == 32) return launch<KD, 1>(p, state_only, fine, stream);
+  if (cols == 64) return launch<KD, 2>(p, state_only, fine, stream);
+  return launch<KD, 4>(p, state_only, fine, stream);
 }
 
 }  // namespace
@@ -480,6 +513,7 @@ int la_bf16_tile_cols(int vd) { return vd <= 32 ? 32 : vd <= 64 ? 64 : 128; }
 int la_walk_bf16(LaParams p, int roles, bool state_only, bool fine, hipStream_t stream) {
   const int vd = la_widest(p, roles), cols = la_bf16_tile_cols(vd);
   p.tiles = (vd + cols - 1) / cols;
+  p.roles = roles;
   int kd = 0;
   for (int i = 0; i < roles; ++i) kd = std::max(kd, p.role[i].kd);
   if (kd <= 32) return launch_kd<32>(p, roles, state_only, fine, stream);

@@ -30,11 +30,11 @@ template <typename T>
 struct Raw {
   using type = u2;
   static __device__ __forceinline__ u2 load(rsrc_t r, uint32_t o, int left, bool vec) {
-    if (vec) return __builtin_amdgcn_raw_buffer_load_b64(r, left >= 4 ? o : kOOB, 0, 0);
+    if (vec) return __builtin_amdgcn_raw_buffer_load_b64(r, la_in(left >= 4, o), 0, 0);
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      w[i] = __builtin_amdgcn_raw_buffer_load_b16(r, i < left ? o + 2 * i : kOOB, 0, 0);
+      w[i] = __builtin_amdgcn_raw_buffer_load_b16(r, la_in(i < left, o + 2 * i), 0, 0);
     return u2{(w[0] & 0xffffu) | w[1] << 16, (w[2] & 0xffffu) | w[3] << 16};
   }
   static __device__ __forceinline__ f4 value(u2 w) {
@@ -45,11 +45,11 @@ template <>
 struct Raw<float> {
   using type = u4;
   static __device__ __forceinline__ u4 load(rsrc_t r, uint32_t o, int left, bool vec) {
-    if (vec) return __builtin_amdgcn_raw_buffer_load_b128(r, left >= 4 ? o : kOOB, 0, 0);
+    if (vec) return __builtin_amdgcn_raw_buffer_load_b128(r, la_in(left >= 4, o), 0, 0);
     u4 w;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      w[i] = __builtin_amdgcn_raw_buffer_load_b32(r, i < left ? o + 4 * i : kOOB, 0, 0);
+      w[i] = __builtin_amdgcn_raw_buffer_load_b32(r, la_in(i < left, o + 4 * i), 0, 0);
     return w;
   }
   static __device__ __forceinline__ f4 value(u4 w) {
@@ -76,11 +76,11 @@ __global__ __launch_bounds__(64 * W) void la_walk_f32_kernel(LaParams P) {
   __shared__ float se[kC], sw[kC], sdot[W][kC];
   __shared__ float s_tot, s_sum;
 
-  const LaRole& R = P.role[blockIdx.z];
-  const int h = blockIdx.y;
+  const LaPlace at = la_place(P);
+  if (!at.any) return;
+  const LaRole& R = P.role[at.role];
+  const int h = at.h, tile = at.tile, piece = at.piece;
   const int tiles = (R.vd + 16 * W - 1) / (16 * W);
-  const int tile = blockIdx.x % P.tiles;
-  const int piece = blockIdx.x / P.tiles;
   if (tile >= tiles) return;
   const LaPiece pc = la_piece(P.seqs, piece);
   if (STATE_ONLY) {
@@ -115,7 +115,7 @@ __global__ __launch_bounds__(64 * W) void la_walk_f32_kernel(LaParams P) {
         for (int r = 0; r < 4; ++r) {
           const int i = 16 * t + 4 * q4 + r;
           const uint32_t o = static_cast<uint32_t>(i * R.sk + col * R.sv) * 4;
-          S[t][r] = ldb<float>(rs, i < R.kd && col < R.vd ? o : kOOB, 0);
+          S[t][r] = ldb<float>(rs, la_in((i < R.kd) & (col < R.vd), o), 0);
         }
     }
   }
@@ -135,13 +135,12 @@ __global__ __launch_bounds__(64 * W) void la_walk_f32_kernel(LaParams P) {
   const int stx = static_cast<int>(R.x.st) * SZ, sty = static_cast<int>(R.y.st) * SZ,
             stz = static_cast<int>(R.z.st) * SZ;
   raw rx[STATE_ONLY ? 1 : NX], ry[NX], rz[NZ];
-  uint32_t rg = 0;
+  LaBits rg{0, 0};
   // token of local index i of the walk
   auto token = [&](int i) { return R.rev ? pc.end - 1 - i : pc.begin + i; };
   auto fetch = [&](int c) {
     const int base = c * kC, left = n_tok - base;
-    if (wave == 0)
-      rg = lane < min(left, kC) ? la_step_decay(P.g, R.rev, pc, b, token(base + lane), h) : 0u;
+    rg = la_step_decays<kC>(P.g, R.rev, pc, b, h, base, lane);
     if (!STATE_ONLY) {
       const rsrc_t bx = la_rows<kC>(R.x, SZ, b, h, R.rev, pc.begin, pc.end, base);
 #pragma unroll
@@ -175,7 +174,7 @@ __global__ __launch_bounds__(64 * W) void la_walk_f32_kernel(LaParams P) {
       *reinterpret_cast<f4*>(&sz[(rowz + k * DZ) * ZS + (tid % UZ) * 4]) = Raw<T>::value(rz[k]);
     if (wave == 0) {
       // running sums of the decays in fp64: differences of nearby ones keep their digits
-      double G = la_decay_value(P.g, rg);
+      double G = la_decay_value(P.g, rg.get());
 #pragma unroll
       for (int d = 1; d < kC; d <<= 1) {
         const double o = __shfl_up(G, d);
@@ -192,7 +191,7 @@ __global__ __launch_bounds__(64 * W) void la_walk_f32_kernel(LaParams P) {
         s_sum = static_cast<float>(last);
       }
     }
-    if (c + 1 < chunks) fetch(c + 1);
+    fetch(c + 1);  // behind the piece's end nothing is loaded; a branch would be waited at
     __syncthreads();
 
     // ---- the chunk's pairs, masked and decayed: quadrants (0,0), (1,0), (1,1)
@@ -290,11 +289,11 @@ __global__ __launch_bounds__(64 * W) void la_walk_f32_kernel(LaParams P) {
           const bool in = base + i < n_tok && col < R.vd;
           const long long t = token(base + i);
           if (in) {
-            const long long at = b * R.o_sb + t * R.o_st + h * R.o_sh + col;
+            const long long o = b * R.o_sb + t * R.o_st + h * R.o_sh + col;
             if (R.out_f32)
-              static_cast<float*>(R.out)[at] = O[mi][r];
+              static_cast<float*>(R.out)[o] = O[mi][r];
             else
-              static_cast<T*>(R.out)[at] = from_f32<T>(O[mi][r]);
+              static_cast<T*>(R.out)[o] = from_f32<T>(O[mi][r]);
           }
           if (R.dots) {
             float d = 0.0f;
@@ -330,9 +329,9 @@ __global__ __launch_bounds__(64 * W) void la_walk_f32_kernel(LaParams P) {
       float d = 0.0f;
 #pragma unroll
       for (int w = 0; w < W; ++w) d += sdot[w][tid];
-      const size_t at = P.seqs.cu ? token(base + tid)
+      const size_t row = P.seqs.cu ? token(base + tid)
                                   : static_cast<size_t>(b) * P.seqs.T + token(base + tid);
-      R.dots[(static_cast<size_t>(tile) * P.H + h) * P.batch_tokens + at] = d;
+      R.dots[(static_cast<size_t>(tile) * P.H + h) * P.batch_tokens + row] = d;
     }
   }
 
@@ -355,14 +354,14 @@ __global__ __launch_bounds__(64 * W) void la_walk_f32_kernel(LaParams P) {
       for (int r = 0; r < 4; ++r) {
         const int i = 16 * t + 4 * q4 + r;
         const uint32_t o = static_cast<uint32_t>(i * R.sk + col * R.sv) * 4;
-        stb<float>(rs, i < R.kd && col < R.vd ? o : kOOB, 0, S[t][r] * f);
+        stb<float>(rs, la_in((i < R.kd) & (col < R.vd), o), 0, S[t][r] * f);
       }
   }
 }
 
 template <typename T, int KT, int W>
-int launch(const LaParams& p, int roles, bool state_only, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(p.seqs.pieces) * p.tiles, p.H, roles), block(64 * W);
+int launch(const LaParams& p, bool state_only, hipStream_t stream) {
+  const unsigned grid = la_grid(p), block = 64 * W;
   if (state_only)
     la_walk_f32_kernel<T, KT, W, true><<<grid, block, 0, stream>>>(p);
   else
@@ -374,8 +373,8 @@ int launch(const LaParams& p, int roles, bool state_only, hipStream_t stream) {
 template <typename T, int KT>
 int launch_kt(const LaParams& p, int roles, bool state_only, hipStream_t stream) {
   return la_f32_tile_cols(la_widest(p, roles)) == 32
-             ? launch<T, KT, 2>(p, roles, state_only, stream)
-             : launch<T, KT, 4>(p, roles, state_only, stream);
+             ? launch<T, KT, 2>(p, state_only, stream)
+             : launch<T, KT, 4>(p, state_only, stream);
 }
 
 }  // namespace
@@ -386,6 +385,7 @@ int la_f32_tile_cols(int vd) { return vd <= 32 ? 32 : 64; }
 int la_walk_f32(LaParams p, int roles, bool state_only, int dtype, hipStream_t stream) {
   const int vd = la_widest(p, roles), cols = la_f32_tile_cols(vd);
   p.tiles = (vd + cols - 1) / cols;
+  p.roles = roles;
   int kd = 0;
   for (int i = 0; i < roles; ++i) kd = std::max(kd, p.role[i].kd);
   return with_storage(dtype, [&](auto z) {
