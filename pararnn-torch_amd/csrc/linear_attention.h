@@ -78,6 +78,7 @@ struct LaRole {
   int kd, vd;           // columns of x, y and of z, out
   int sk, sv;           // strides of the state's kd and vd axes
   int rev;
+  int exact;            // the final state is a result: all of its 24 bits count
   float p_scale, x_scale, u_scale;  // of the pairs, of the state's part, of what enters it
   float* piece_state;   // [piece][head][Dk][Dv]: states before the pieces (NULL: not cut)
   float* piece_decay;   // [piece][head]: a piece's whole log decay in the walk's direction
@@ -278,8 +279,8 @@ inline int la_widest(const LaParams& p, int roles) {
 // states.  *_tile_cols: columns of z that a workgroup takes where the widest role has vd.
 int la_walk_f32(LaParams p, int roles, bool state_only, int dtype, hipStream_t stream);
 int la_f32_tile_cols(int vd);
-// bf16 storage with widths in multiples of 8 and rows that admit 16-byte accesses (x, y, z, dot)
-// or 8-byte ones (out).
+// bf16 storage with widths in multiples of 8, rows that admit 16-byte accesses (x, y, z, dot) or
+// 8-byte ones (out), and tokens at least a row apart, in ascending order.
 int la_walk_bf16(LaParams p, int roles, bool state_only, bool fine, hipStream_t stream);
 int la_bf16_tile_cols(int vd);
 

@@ -22,35 +22,52 @@ struct JoinArgs {
   int H, DD;
 };
 
+// V floats of the state a thread; the contributions of kAhead pieces are under way before the
+// first is added (from empty buffers behind the last: a branch would be waited at).
+template <int V>
 __global__ __launch_bounds__(256) void la_join_kernel(JoinArgs A, int seq_blocks) {
+  typedef uint32_t vec __attribute__((ext_vector_type(V)));
+  constexpr int kAhead = 8;
   const int role = blockIdx.z, h = blockIdx.y;
   const int seq = blockIdx.x / seq_blocks;
-  const int e = (blockIdx.x - seq * seq_blocks) * 256 + threadIdx.x;
+  const int e = ((blockIdx.x - seq * seq_blocks) * 256 + threadIdx.x) * V;
   int p0, n;
   la_pieces_of(A.seqs, seq, p0, n);
   if (n < 2 || e >= A.DD) return;
   const size_t row = static_cast<size_t>(A.H) * A.DD;
-  const size_t at = static_cast<size_t>(h) * A.DD + e;
+  const size_t at = static_cast<size_t>(h) * A.DD;
   const float* init = la_row(A.init[role], seq, row);
   const int dir = A.rev[role] ? -1 : 1, from = A.rev[role] ? p0 + n - 1 : p0;
-  float S = init ? init[at] : 0.0f;
-  // the contributions of 16 pieces are under way before the first is added
-  constexpr int kAhead = 16;
+  float S[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) S[v] = init ? init[at + e + v] : 0.0f;
   for (int i0 = 0; i0 < n; i0 += kAhead) {
-    float U[kAhead], d[kAhead];
+    vec U[kAhead];
+    float d[kAhead];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const size_t p = from + dir * (i0 + i);
       const bool more = i0 + i + 1 < n;  // the last piece hands on to none
-      U[i] = more ? A.state[role][p * row + at] : 0.0f;
-      d[i] = more ? A.decay[role][p * A.H + h] : 0.0f;
+      const size_t p = from + dir * min(i0 + i, n - 1);
+      const rsrc_t r = make_rsrc(A.state[role] + p * row + at, more ? A.DD * 4u : 0u);
+      if constexpr (V == 4)
+        U[i] = __builtin_amdgcn_raw_buffer_load_b128(r, e * 4, 0, 0);
+      else
+        U[i] = __builtin_amdgcn_raw_buffer_load_b32(r, e * 4, 0, 0);
+      d[i] = A.decay[role][p * A.H + h];
     }
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       if (i0 + i >= n) break;
       const size_t p = from + dir * (i0 + i);
-      A.state[role][p * row + at] = S;
-      S = fmaf(fexp(d[i]), S, U[i]);
+      float* w = A.state[role] + p * row + at + e;
+      const float f = fexp(d[i]);
+      vec s;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        s[v] = __float_as_uint(S[v]);
+        S[v] = fmaf(f, S[v], __uint_as_float(U[i][v]));
+      }
+      *reinterpret_cast<vec*>(w) = s;
     }
   }
 }
@@ -201,13 +218,15 @@ __global__ __launch_bounds__(256) void la_head_sum_kernel(HeadSumArgs A) {
 
 using Problem = prnn_linear_attention_problem;
 
-LaView view(const prnn_la_view& v, int H, int dtype) {
-  LaView r{v.p, v.sb, v.st, v.sh, 1, 0};
+// D: the array's width.  A lone token's stride is what suits the walks.
+LaView view(const prnn_la_view& v, const Problem& a, int D) {
+  const int H = a.H, dtype = a.dtype;
+  LaView r{v.p, v.sb, a.T > 1 ? v.st : D, v.sh, 1, 0};
   if (v.heads > 0) r.rep = H / v.heads;
   const long long size = dtype == PRNN_F32 ? 4 : 2;
   const long long bytes = static_cast<long long>(reinterpret_cast<uintptr_t>(v.p)) |
-                          v.sb * size | v.st * size | v.sh * size;
-  r.vec = (bytes & 15) == 0;
+                          r.sb * size | r.st * size | r.sh * size;
+  r.vec = (bytes & 15) == 0 && r.st >= D;
   return r;
 }
 
@@ -247,7 +266,7 @@ int sequences(const Problem& a) { return a.cu_seqlens ? a.n_seq : a.B; }
 // How long the pieces are.  Walks of whole sequences read every array once; cut ones read k
 // and v once more and move a state a piece, so a sequence is cut only as far as the chip has
 // workgroups to spare (about kLaTarget run at a time), and never below kLaLeast tokens.
-constexpr int kLaTarget = 1024, kLaLeast = 256;
+constexpr int kLaTarget = 1536, kLaLeast = 256;
 
 LaSeqs cut(const Problem& a, int tiles_and_roles) {
   LaSeqs s{a.cu_seqlens, sequences(a), a.T, 1, 0};
@@ -284,9 +303,8 @@ struct Scratch {
 // 16-byte accesses.  What is odd takes the fp32 walk, about a third as fast at width 64.
 bool on_bf16(const Problem& a, const prnn_la_view* other) {
   if (a.dtype != PRNN_BF16 || a.Dk % 8 || a.Dv % 8) return false;
-  for (const prnn_la_view* v : {&a.q, &a.k, &a.v, other})
-    if (v && !view(*v, a.H, a.dtype).vec) return false;
-  return true;
+  return view(a.q, a, a.Dk).vec && view(a.k, a, a.Dk).vec && view(a.v, a, a.Dv).vec &&
+         view(*other, a, a.Dv).vec;
 }
 
 struct Walks {
@@ -356,9 +374,13 @@ int join(const LaParams& p, const Scratch& s, const LaState* init, const int* re
     j.init[i] = init[i];
     j.rev[i] = rev[i];
   }
-  const int blocks = (j.DD + 255) / 256;
-  la_join_kernel<<<dim3(static_cast<unsigned>(p.seqs.n_seq) * blocks, p.H, roles), 256, 0, st>>>(
-      j, blocks);
+  const bool vec = j.DD % 4 == 0;
+  const int blocks = (j.DD / (vec ? 4 : 1) + 255) / 256;
+  const dim3 grid(static_cast<unsigned>(p.seqs.n_seq) * blocks, p.H, roles);
+  if (vec)
+    la_join_kernel<4><<<grid, 256, 0, st>>>(j, blocks);
+  else
+    la_join_kernel<1><<<grid, 256, 0, st>>>(j, blocks);
   PRNN_HIP(hipGetLastError());
   return PRNN_OK;
 }
@@ -389,13 +411,14 @@ int forward(const Problem& a, const prnn_la_view& out, float* state_out, const i
   const Scratch s = carve(ws, a, w, false, false);
   LaParams p = params(a, forward_cut(a, w));
   LaRole& r = p.role[0];
-  r.x = view(a.q, a.H, a.dtype);
-  r.y = view(a.k, a.H, a.dtype);
-  r.z = view(a.v, a.H, a.dtype);
+  r.x = view(a.q, a, a.Dk);
+  r.y = view(a.k, a, a.Dk);
+  r.z = view(a.v, a, a.Dv);
   r.out = const_cast<void*>(out.p);
   r.o_sb = out.sb;
-  r.o_st = out.st;
+  r.o_st = a.T > 1 ? out.st : a.Dv;
   r.o_sh = out.sh;
+  r.exact = 1;  // asked for or not: the output has the same bits
   r.kd = a.Dk;
   r.vd = a.Dv;
   r.sk = a.Dv;
@@ -419,8 +442,8 @@ int backward(const Problem& a, const prnn_la_view& go, const float* gs, void* dq
   const Walks w{on_bf16(a, &go), a.dtype};
   const Scratch s = carve(ws, a, w, true, dg != nullptr);
   LaParams p = params(a, backward_cut(a, w));
-  const LaView q = view(a.q, a.H, a.dtype), k = view(a.k, a.H, a.dtype),
-               v = view(a.v, a.H, a.dtype), o = view(go, a.H, a.dtype);
+  const LaView q = view(a.q, a, a.Dk), k = view(a.k, a, a.Dk), v = view(a.v, a, a.Dv),
+               o = view(go, a, a.Dv);
   const LaState init = initial(a), fin{const_cast<float*>(gs), nullptr, sequences(a)};
   const LaView none{nullptr, 0, 0, 0, 1, 1};
   auto role = [&](LaView x, LaView y, LaView z, int kd, int vd, bool transposed, int rev) {
@@ -433,6 +456,7 @@ int backward(const Problem& a, const prnn_la_view& go, const float* gs, void* dq
     r.sk = transposed ? 1 : a.Dv;
     r.sv = transposed ? a.Dv : 1;
     r.rev = rev;
+    r.exact = rev && dh0 != nullptr;
     r.p_scale = a.scale;
     r.x_scale = rev ? 1.0f : a.scale;
     r.u_scale = rev ? a.scale : 1.0f;

@@ -13,8 +13,8 @@
 // come, read across tokens by the transposing LDS load.
 //
 // Roundings to bf16: the pairs' weights and the state where they are operands (S itself stays
-// fp32); what enters the state, w z, is split into three bf16 parts, 24 bits: the state is an
-// fp32 result.  FINE splits the weights and the state into two parts as well (16 bits), for the
+// fp32); what enters the state, w z, is split into three bf16 parts, 24 bits, where the state is an
+// fp32 result, and into two where it only goes on to be rounded.  FINE splits the weights and the state into two parts as well (16 bits), for the
 // backward pass, where the decays' gradient adds up differences of the results.
 #include "linear_attention.h"
 
@@ -145,41 +145,58 @@ void la_walk_bf16_kernel(LaParams P) {
   float sum_decay = 0.0f;
   auto token = [&](int i) { return R.rev ? pc.end - 1 - i : pc.begin + i; };
 
-  // A thread's loads of an array are rows apart by a constant number.  What lies outside the
-  // piece or the width is read as zero (an offset outside the resource).
-  constexpr int DX = NT / UX, DZ = NT / UZ;
+  // An array's rows of a chunk are a window of 64 in memory, walked through by one pointer.  A
+  // buffer over the window's rows that belong to the piece leaves the others, and columns behind
+  // the width, outside: they are read as zero and not written, without a comparison.
+  constexpr int DX = NT / UX, DZ = NT / UZ;  // rows between a thread's loads
   const int rowx = tid / UX, cx = (tid % UX) * 8, rowz = tid / UZ, cz = col0 + (tid % UZ) * 8;
-  const bool inx = cx < R.kd, inz = cz < R.vd;
+  const int ahead = R.rev ? -1 : 1;
+  const int low = R.rev ? pc.end - kC : pc.begin;
+  auto window = [&](const LaView& v, int size) {
+    return static_cast<const char*>(v.p) +
+           (b * v.sb + (h / v.rep) * v.sh + static_cast<long long>(low) * v.st) * size;
+  };
   const int stx = static_cast<int>(R.x.st) * 2, sty = static_cast<int>(R.y.st) * 2,
             stz = static_cast<int>(R.z.st) * 2;
+  const char *px = STATE_ONLY ? nullptr : window(R.x, 2), *py = window(R.y, 2),
+             *pz = window(R.z, 2);
   const int fx = R.rev ? kC - 1 - rowx : rowx, fz = R.rev ? kC - 1 - rowz : rowz;
-  const int ahead = R.rev ? -1 : 1;
+  const uint32_t vx = la_in(cx < R.kd, fx * stx + cx * 2), vy = la_in(cx < R.kd, fx * sty + cx * 2),
+                 vz = la_in(cz < R.vd, fz * stz + cz * 2);
   u4 rx[STATE_ONLY ? 1 : NX], ry[NX], rz[NZ];
   LaBits rg{0, 0};
   auto fetch = [&](int base) {
-    const int left = n_tok - base;
+    const int have = max(0, min(n_tok - base, kC)), cut = R.rev ? kC - have : 0;
     rg = la_step_decays<kC>(P.g, R.rev, pc, b, h, base, lane);
     if (!STATE_ONLY) {
-      const rsrc_t bx = la_rows<kC>(R.x, 2, b, h, R.rev, pc.begin, pc.end, base);
+      const rsrc_t bx = make_rsrc(px + static_cast<long long>(cut) * stx, have * stx);
 #pragma unroll
-      for (int k = 0; k < NX; ++k) {
-        const uint32_t o = (fx + ahead * k * DX) * stx + cx * 2;
-        rx[k] = __builtin_amdgcn_raw_buffer_load_b128(bx, la_in(inx & (rowx + k * DX < left), o), 0, 0);
-      }
+      for (int k = 0; k < NX; ++k)
+        rx[k] = __builtin_amdgcn_raw_buffer_load_b128(bx, vx + (ahead * k * DX - cut) * stx, 0, 0);
+      px += ahead * kC * static_cast<long long>(stx);
     }
-    const rsrc_t by = la_rows<kC>(R.y, 2, b, h, R.rev, pc.begin, pc.end, base);
+    const rsrc_t by = make_rsrc(py + static_cast<long long>(cut) * sty, have * sty);
 #pragma unroll
-    for (int k = 0; k < NX; ++k) {
-      const uint32_t o = (fx + ahead * k * DX) * sty + cx * 2;
-      ry[k] = __builtin_amdgcn_raw_buffer_load_b128(by, la_in(inx & (rowx + k * DX < left), o), 0, 0);
-    }
-    const rsrc_t bz = la_rows<kC>(R.z, 2, b, h, R.rev, pc.begin, pc.end, base);
+    for (int k = 0; k < NX; ++k)
+      ry[k] = __builtin_amdgcn_raw_buffer_load_b128(by, vy + (ahead * k * DX - cut) * sty, 0, 0);
+    py += ahead * kC * static_cast<long long>(sty);
+    const rsrc_t bz = make_rsrc(pz + static_cast<long long>(cut) * stz, have * stz);
 #pragma unroll
-    for (int k = 0; k < NZ; ++k) {
-      const uint32_t o = (fz + ahead * k * DZ) * stz + cz * 2;
-      rz[k] = __builtin_amdgcn_raw_buffer_load_b128(bz, la_in(inz & (rowz + k * DZ < left), o), 0, 0);
-    }
+    for (int k = 0; k < NZ; ++k)
+      rz[k] = __builtin_amdgcn_raw_buffer_load_b128(bz, vz + (ahead * k * DZ - cut) * stz, 0, 0);
+    pz += ahead * kC * static_cast<long long>(stz);
   };
+  auto move_on = [&](int by) {
+    if (!STATE_ONLY) px += ahead * by * static_cast<long long>(stx);
+    py += ahead * by * static_cast<long long>(sty);
+    pz += ahead * by * static_cast<long long>(stz);
+  };
+  // the output and the rows that it is multiplied with, one window behind
+  const int so = R.out_f32 ? 4 : 2, sto = static_cast<int>(R.o_st) * so,
+            std_ = static_cast<int>(R.dot.st) * 2;
+  const char *po = nullptr, *pd = nullptr;
+  if (!STATE_ONLY) po = window(LaView{R.out, R.o_sb, R.o_st, R.o_sh, 1, 1}, so);
+  if (FINE) pd = window(R.dot, 2);
   // Decays of the chunk's first `n` tokens: running sums from the front for the pairs and the
   // state's part, from the back for what enters the state, so that each weight that counts is the
   // exponential of a short sum.
@@ -255,17 +272,17 @@ void la_walk_bf16_kernel(LaParams P) {
     // the rows that the output is multiplied with, ahead of the next chunk's: what is waited for
     // first is loaded first
     u2 dv[2][4];
+    const int c4 = col0 + 32 * wave + 4 * half;  // first of this lane's columns of out
     if (FINE) {
-      const rsrc_t bd = la_rows<kC>(R.dot, 2, b, h, R.rev, pc.begin, pc.end, base);
+      const int have = R.dots ? min(n_tok - base, kC) : 0, cut = R.rev ? kC - have : 0;
+      const rsrc_t bd = make_rsrc(pd + static_cast<long long>(cut) * std_, have * std_);
 #pragma unroll
       for (int it = 0; it < 2; ++it) {
-        const int i = 32 * it + l32, row = R.rev ? kC - 1 - i : i;
-        const int c4 = col0 + 32 * wave + 4 * half;
+        const int i = 32 * it + l32, row = (R.rev ? kC - 1 - i : i) - cut;
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           dv[it][q] = __builtin_amdgcn_raw_buffer_load_b64(
-              bd, la_in((R.dots != nullptr) & (base + i < n_tok) & (c4 + 8 * q < R.vd),
-                        (row * static_cast<int>(R.dot.st) + c4 + 8 * q) * 2), 0, 0);
+              bd, la_in(c4 + 8 * q < R.vd, 0) | (row * std_ + (c4 + 8 * q) * 2), 0, 0);
       }
     }
     next = base + kC;
@@ -283,6 +300,7 @@ void la_walk_bf16_kernel(LaParams P) {
         *reinterpret_cast<u4*>(sz + stop * RZ + e * 16) = u4{0, 0, 0, 0};
       if (wave == 0) decays(g_here, stop);
       next = base + stop;
+      move_on(stop - 2 * kC);  // two windows on already
       fetch(next);
       __syncthreads();
     }
@@ -389,14 +407,14 @@ void la_walk_bf16_kernel(LaParams P) {
           if (FINE) O[it] = mfma(zf[2 * it + s].v, pairs(2 * it, s, 1), O[it]);
         }
       // ---- out: lane l has token l % 32 of a tile and four columns side by side
-      const LaView ov{R.out, R.o_sb, R.o_st, R.o_sh, 1, 1};
-      const int so = R.out_f32 ? 4 : 2;
-      const rsrc_t bo = la_rows<kC>(ov, so, b, h, R.rev, pc.begin, pc.end, base);
+      const int cut = R.rev ? kC - n_here : 0;
+      const rsrc_t bo = make_rsrc(po + static_cast<long long>(cut) * sto, n_here * sto);
+      po += ahead * (next - base) * static_cast<long long>(sto);
+      if (FINE) pd += ahead * (next - base) * static_cast<long long>(std_);
 #pragma unroll
       for (int it = 0; it < 2; ++it) {
-        const int i = 32 * it + l32, row = R.rev ? kC - 1 - i : i;
-        const int c4 = col0 + 32 * wave + 4 * half;
-        const uint32_t at = (row * static_cast<int>(R.o_st) + c4) * so;
+        const int i = 32 * it + l32, row = (R.rev ? kC - 1 - i : i) - cut;
+        const uint32_t at = row * sto + c4 * so;
         if (FINE) {
           float d = 0.0f;
 #pragma unroll
@@ -411,7 +429,7 @@ void la_walk_bf16_kernel(LaParams P) {
         }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const uint32_t o = la_in((i < n_here) & (c4 + 8 * q < R.vd), at + 8 * q * so);
+          const uint32_t o = la_in(c4 + 8 * q < R.vd, 0) | (at + 8 * q * so);
           const float v[4] = {O[it][4 * q], O[it][4 * q + 1], O[it][4 * q + 2], O[it][4 * q + 3]};
           if (R.out_f32)
             __builtin_amdgcn_raw_buffer_store_b128(
@@ -447,7 +465,7 @@ void la_walk_bf16_kernel(LaParams P) {
         const b8 y = load_across<RY>(sy + across_share<RY>(lane), 16 * ts, 32 * t);
         S[t] = mfma(y, z0, S[t]);
         S[t] = mfma(y, z1, S[t]);
-        S[t] = mfma(y, z2, S[t]);
+        if (R.exact) S[t] = mfma(y, z2, S[t]);
       }
     }
     __syncthreads();

@@ -53,14 +53,16 @@ def _rows(t: Tensor) -> Tensor:
 def _tiles(t: Tensor) -> Tensor:
     """``t`` as the walks read it.  Which walk runs goes by type and widths alone, so that equal
     values give equal bits: the bfloat16 one (widths in eights) reads 16 bytes at a time, and rows
-    that do not lie for that (a view of a fused projection with an odd offset) are copied."""
+    that do not lie for that (a view of a fused projection with an odd offset, a row expanded over
+    time) are copied."""
     t = _rows(t)
     if abs(t.stride(1)) * t.element_size() > 1 << 24:  # the kernels' offsets inside a chunk
         t = t.contiguous()
     if t.dtype != torch.bfloat16 or t.shape[-1] % 8:
         return t
     sb, st, sh, _ = t.stride()
-    if (sb | st | sh) % 8 == 0 and t.data_ptr() % 16 == 0:
+    if (sb | st | sh) % 8 == 0 and t.data_ptr() % 16 == 0 and (st >= t.shape[-1]
+                                                               or t.shape[1] == 1):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
