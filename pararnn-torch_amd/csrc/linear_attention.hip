@@ -501,7 +501,8 @@ int backward(const Problem& a, const prnn_la_view& go, const float* gs, void* dq
     p.role[1].dot = k;
     p.role[1].dots = s.dots[1];
   }
-  if (int rc = w.run(p, 3, false, true, st)) return rc;
+  // the decays' gradient adds up differences of the results: they are formed finer for it
+  if (int rc = w.run(p, 3, false, dg != nullptr, st)) return rc;
   const size_t tokens = static_cast<size_t>(a.B) * a.T;
   if (sums && tokens) {
     hs.H = a.H;

@@ -206,7 +206,7 @@ void la_walk_bf16_kernel(LaParams P) {
     const float last = __shfl(G, kC - 1);
     const float back = scan_up(__shfl(g, kC - 1 - lane));  // lane l: the sum of the last l + 1
     const float behind = __shfl(back, (kC - 2 - lane) & 63);
-    sG[lane] = G;
+    sG[lane] = G * 1.4426950408889634f;
     se[lane] = fexp(G) * R.x_scale;
     sw[lane] = lane == kC - 1 ? R.u_scale : fexp(behind) * R.u_scale;
     if (lane == 0) {
@@ -214,6 +214,7 @@ void la_walk_bf16_kernel(LaParams P) {
       s_sum = last;
     }
   };
+  const float log_scale = __builtin_amdgcn_logf(fabsf(R.p_scale));  // to base 2; -inf for 0
   if (tid < 2) s_stop[tid] = kC;
   fetch(0);
 
@@ -267,26 +268,8 @@ void la_walk_bf16_kernel(LaParams P) {
       if ((bad & 0x80008000u) && rowz + k * DZ > 0) stop_here = rowz + k * DZ;
     }
     if (stop_here < kC) atomicMin(&s_stop[turn], stop_here);
-    const uint32_t g_here = rg.get();
     if (wave == 0) decays(rg.get(), kC);
-    // the rows that the output is multiplied with, ahead of the next chunk's: what is waited for
-    // first is loaded first
-    u2 dv[2][4];
-    const int c4 = col0 + 32 * wave + 4 * half;  // first of this lane's columns of out
-    if (FINE) {
-      const int have = R.dots ? min(n_tok - base, kC) : 0, cut = R.rev ? kC - have : 0;
-      const rsrc_t bd = make_rsrc(pd + static_cast<long long>(cut) * std_, have * std_);
-#pragma unroll
-      for (int it = 0; it < 2; ++it) {
-        const int i = 32 * it + l32, row = (R.rev ? kC - 1 - i : i) - cut;
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-          dv[it][q] = __builtin_amdgcn_raw_buffer_load_b64(
-              bd, la_in(c4 + 8 * q < R.vd, 0) | (row * std_ + (c4 + 8 * q) * 2), 0, 0);
-      }
-    }
     next = base + kC;
-    fetch(next);  // behind the piece's end nothing is loaded; a branch would be waited at
     __syncthreads();
     if (tid == 0) s_stop[turn ^ 1] = kC;
     const int stop = s_stop[turn];
@@ -298,15 +281,17 @@ void la_walk_bf16_kernel(LaParams P) {
         *reinterpret_cast<u4*>(sy + stop * RY + e * 16) = u4{0, 0, 0, 0};
       for (int e = tid; e < (kC - stop) * (RZ / 16); e += NT)
         *reinterpret_cast<u4*>(sz + stop * RZ + e * 16) = u4{0, 0, 0, 0};
-      if (wave == 0) decays(g_here, stop);
+      if (wave == 0) decays(rg.get(), stop);
       next = base + stop;
-      move_on(stop - 2 * kC);  // two windows on already
-      fetch(next);
+      move_on(stop - kC);
       __syncthreads();
     }
     const int n_here = min(n_tok, next) - base;  // tokens of this chunk
+    if (STATE_ONLY) fetch(next);
 
     f16v O[2];
+    u2 dv[2][4];
+    const int c4 = col0 + 32 * wave + 4 * half;  // first of this lane's columns of out
     if (!STATE_ONLY) {
       // ---- the chunk's pairs: tiles (out rows, earlier rows) (0,0), (1,0), (1,1)
       for (int id = wave; id < 3; id += W) {
@@ -328,18 +313,25 @@ void la_walk_bf16_kernel(LaParams P) {
           y.h[1] = *reinterpret_cast<const uint2*>(yr + 32 * k + 16);
           acc = mfma(y.v, *reinterpret_cast<const b8*>(xr + (f ^ 32 * k)), acc);
         }
-        const float Gi = sG[i];
-        // the mask as bits, not as a choice: the compiler would branch round every exponential
-        const int before = 32 * jt + 4 * half - i - 1;
+        // weights: exponentials to base 2, the scale among them
+        const float Gi = sG[i] + log_scale;
+        // Not to be known before: as masks of its own kept over the walk it costs two lane reads
+        // an element.
+        int before = 32 * jt + 4 * half - i;
+        asm volatile("" : "+v"(before));
         float w[16];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const f4 Gj = *reinterpret_cast<const f4*>(&sG[32 * jt + 8 * q + 4 * half]);
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            w[4 * q + r] = __int_as_float(
-                __float_as_int(acc[4 * q + r] * (R.p_scale * fexp(Gi - Gj[r]))) &
-                ((before + 8 * q + r) >> 31));
+          for (int r = 0; r < 4; ++r) {
+            const float e = acc[4 * q + r] * __builtin_amdgcn_exp2f(Gi - Gj[r]);
+            w[4 * q + r] = before <= -(8 * q + r) ? e : 0.0f;
+          }
+        }
+        if (R.p_scale < 0.0f) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) w[r] = -w[r];
         }
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
@@ -352,6 +344,22 @@ void la_walk_bf16_kernel(LaParams P) {
           }
         }
       }
+      // The rows that the output is multiplied with, then the next chunk's: what is waited for first is
+      // loaded first, and nothing before the registers of the pairs are free.  Behind the piece's end
+      // nothing is loaded; a branch would be waited at.
+      if (FINE) {
+        const int have = R.dots ? min(n_tok - base, kC) : 0, cut = R.rev ? kC - have : 0;
+        const rsrc_t bd = make_rsrc(pd + static_cast<long long>(cut) * std_, have * std_);
+  #pragma unroll
+        for (int it = 0; it < 2; ++it) {
+          const int i = 32 * it + l32, row = (R.rev ? kC - 1 - i : i) - cut;
+  #pragma unroll
+          for (int q = 0; q < 4; ++q)
+            dv[it][q] = __builtin_amdgcn_raw_buffer_load_b64(
+                bd, la_in(c4 + 8 * q < R.vd, 0) | (row * std_ + (c4 + 8 * q) * 2), 0, 0);
+        }
+      }
+      fetch(next);
       // ---- the state's part of the output
 #pragma unroll
       for (int it = 0; it < 2; ++it)
@@ -459,13 +467,24 @@ void la_walk_bf16_kernel(LaParams P) {
         x[q] = (q & 1 ? hi_bf16(zf[ts].w[q / 2]) : lo_bf16(zf[ts].w[q / 2])) * w0[q];
         x[4 + q] = (q & 1 ? hi_bf16(zf[ts].w[2 + q / 2]) : lo_bf16(zf[ts].w[2 + q / 2])) * w1[q];
       }
-      const b8 z0 = split8(x), z1 = split8(x), z2 = pack8(x);
+      const b8 z0 = split8(x);
+      if ((!FINE && !STATE_ONLY) || R.exact) {
+        const b8 z1 = split8(x), z2 = pack8(x);
 #pragma unroll
-      for (int t = 0; t < KT; ++t) {
-        const b8 y = load_across<RY>(sy + across_share<RY>(lane), 16 * ts, 32 * t);
-        S[t] = mfma(y, z0, S[t]);
-        S[t] = mfma(y, z1, S[t]);
-        if (R.exact) S[t] = mfma(y, z2, S[t]);
+        for (int t = 0; t < KT; ++t) {
+          const b8 y = load_across<RY>(sy + across_share<RY>(lane), 16 * ts, 32 * t);
+          S[t] = mfma(y, z0, S[t]);
+          S[t] = mfma(y, z1, S[t]);
+          S[t] = mfma(y, z2, S[t]);
+        }
+      } else {
+        const b8 z1 = pack8(x);
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+          const b8 y = load_across<RY>(sy + across_share<RY>(lane), 16 * ts, 32 * t);
+          S[t] = mfma(y, z0, S[t]);
+          S[t] = mfma(y, z1, S[t]);
+        }
       }
     }
     __syncthreads();
