@@ -1,10 +1,13 @@
 // Decayed linear attention: the small kernels around the walks and the C entry points.
 //
 // * la_join_kernel: states before a cut sequence's pieces from the pieces' own contributions;
-// * la_decay_grad_kernel: the log decays' gradient.  dL/dg_t = exp(g_t) <S_{t-1}, R_t> is the
-//   flow from all earlier tokens to t and later ones; from one token to the next it gains what
-//   token t hands on and loses what it receives, so it is a running sum of
-//   k_t . dk_t - q_t . dq_t (both formed in fp32 by the walks), begun at <S_0, dL/dS_0>;
+// * la_flow_kernel, la_decay_grad_kernel: the log decays' gradient.  dL/dg_t = exp(g_t)
+//   <S_{t-1}, R_t> is the flow from all earlier tokens to t and later ones; from one token to the
+//   next it gains what token t hands on and loses what it receives, so it is a running sum of
+//   k_t . dk_t - q_t . dq_t (both formed in fp32 by the walks).  The flow itself stays bounded
+//   while the sum's roundings add up, so the sum is tied at both ends of a sequence (<S_0,
+//   dL/dS_0> and <S_T, dL/dS_T>, zero without states) and, in the fp32 walks, of every piece,
+//   whose states are there; what it misses the end by is taken back along the way;
 // * la_head_sum_kernel: gradients of shared heads, summed in a fixed order.
 #include "linear_attention.h"
 
@@ -75,60 +78,94 @@ __global__ __launch_bounds__(256) void la_join_kernel(JoinArgs A, int seq_blocks
 // ---- gradient of the log decays --------------------------------------------------------
 
 struct DecayGradArgs {
-  LaSeqs seqs;
+  LaSeqs seqs;          // the parts that are tied at their ends: pieces, or whole sequences
+  LaDecay g;
   const float* q_dots;  // [tile][head][token]
   const float* k_dots;
   int tiles, H, DD, batch_tokens;
   LaState h0;
-  const float* dh0;     // rows of sequences
+  const float *dh0, *last, *gs;          // rows of sequences: dL/dS_0, S_T, dL/dS_T
+  const float *state, *adjoint;          // [piece][head][DD] before the pieces, either direction
+  float *flow, *flow_end;                // (piece, H) at the parts' first tokens, (sequence, H)
   int g_dtype;
   void* dg;             // (token, H) of g's type, or NULL
-  float* per_seq;       // (sequence, H) sums for decays per head, or NULL
+  float* per_part;      // (piece, H) sums for decays per head, or NULL
 };
+
+// Sum over a workgroup of 256, in every thread.
+__device__ __forceinline__ double block_sum(double v, double* lds) {
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) v += __shfl_xor(v, k);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return lds[0] + lds[1] + lds[2] + lds[3];
+}
+__device__ __forceinline__ double block_dot(const float* a, const float* b, int n, double* lds) {
+  double d = 0.0;
+  for (int e = threadIdx.x; e < n; e += 256) d += static_cast<double>(a[e]) * b[e];
+  return block_sum(d, lds);
+}
+
+__global__ __launch_bounds__(256) void la_flow_kernel(DecayGradArgs A) {
+  __shared__ double lds[4];
+  const int p = blockIdx.x, h = blockIdx.y;
+  const LaPiece pc = la_piece(A.seqs, p);
+  if (pc.begin >= pc.end) return;
+  const size_t row = static_cast<size_t>(A.H) * A.DD, head = static_cast<size_t>(h) * A.DD;
+  double begin = 0.0;
+  if (pc.first) {
+    if (const float* s0 = la_row(A.h0, pc.seq, row))
+      begin = block_dot(s0 + head, A.dh0 + pc.seq * row + head, A.DD, lds);
+  } else {
+    // the adjoint before the piece that lies ahead is that of this piece's first token
+    begin = block_dot(A.state + p * row + head, A.adjoint + (p - 1) * row + head, A.DD, lds) *
+            fexp(la_decay(A.g, la_batch(A.seqs, pc), pc.begin, h));
+  }
+  double end = 0.0;
+  if (pc.last && A.gs)
+    end = block_dot(A.last + pc.seq * row + head, A.gs + pc.seq * row + head, A.DD, lds);
+  if (threadIdx.x == 0) {
+    A.flow[static_cast<size_t>(p) * A.H + h] = static_cast<float>(begin);
+    if (pc.last) A.flow_end[static_cast<size_t>(pc.seq) * A.H + h] = static_cast<float>(end);
+  }
+}
 
 __global__ __launch_bounds__(256) void la_decay_grad_kernel(DecayGradArgs A) {
   __shared__ double s_wave[4];
-  const int h = blockIdx.y, seq = blockIdx.x, tid = threadIdx.x;
-  const int lane = tid & 63, wave = tid >> 6;
-  int t0, n;
-  if (A.seqs.cu) {
-    t0 = la_offset(A.seqs, seq);
-    n = la_offset(A.seqs, seq + 1) - t0;
-  } else {
-    t0 = seq * A.seqs.T;
-    n = A.seqs.T;
-  }
-  // <S_0, dL/dS_0>
-  double begin = 0.0;
-  const size_t row = static_cast<size_t>(A.H) * A.DD;
-  const float* s0 = la_row(A.h0, seq, row);
-  if (s0) {
-    s0 += static_cast<size_t>(h) * A.DD;
-    const float* d0 = A.dh0 + seq * row + static_cast<size_t>(h) * A.DD;
-    double d = 0.0;
-    for (int e = tid; e < A.DD; e += 256) d += static_cast<double>(s0[e]) * d0[e];
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1) d += __shfl_xor(d, k);
-    if (lane == 0) s_wave[wave] = d;
-    __syncthreads();
-    begin = s_wave[0] + s_wave[1] + s_wave[2] + s_wave[3];
-    __syncthreads();
-  }
-  double flow = begin, total = 0.0;
   constexpr int kEach = 4;
+  const int h = blockIdx.y, p = blockIdx.x, tid = threadIdx.x;
+  const int lane = tid & 63, wave = tid >> 6;
+  const LaPiece pc = la_piece(A.seqs, p);
+  const size_t ph = static_cast<size_t>(p) * A.H + h;
+  const int n = pc.end - pc.begin;
+  if (n <= 0) {
+    if (A.per_part && tid == 0) A.per_part[ph] = 0.0f;
+    return;
+  }
+  const size_t t0 = A.seqs.cu ? pc.begin : static_cast<size_t>(pc.seq) * A.seqs.T + pc.begin;
+  auto step = [&](int t) {  // what the flow gains behind token t
+    double x = 0.0;
+    for (int k = 0; k < A.tiles; ++k) {
+      const size_t at = (static_cast<size_t>(k) * A.H + h) * A.batch_tokens + t0 + t;
+      x += static_cast<double>(A.k_dots[at]) - A.q_dots[at];
+    }
+    return x;
+  };
+  const double begin = A.flow[ph];
+  const double end = pc.last ? A.flow_end[static_cast<size_t>(pc.seq) * A.H + h] : A.flow[ph + A.H];
+  double all = 0.0;
+  for (int t = tid; t < n; t += 256) all += step(t);
+  all = block_sum(all, s_wave);
+  const double miss = (begin + all - end) / n;  // per token
+  double flow = begin, total = 0.0;
   for (int base = 0; base < n; base += 256 * kEach) {
     double d[kEach], sum = 0.0;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       const int t = base + tid * kEach + i;
-      double x = 0.0;
-      if (t < n)
-        for (int k = 0; k < A.tiles; ++k) {
-          const size_t at = (static_cast<size_t>(k) * A.H + h) * A.batch_tokens + t0 + t;
-          x += static_cast<double>(A.k_dots[at]) - A.q_dots[at];
-        }
       d[i] = sum;  // what came before within the thread's tokens
-      sum += x;
+      sum += t < n ? step(t) : 0.0;
     }
     double run = sum;
 #pragma unroll
@@ -136,22 +173,23 @@ __global__ __launch_bounds__(256) void la_decay_grad_kernel(DecayGradArgs A) {
       const double o = __shfl_up(run, k);
       if (lane >= k) run += o;
     }
+    __syncthreads();
     if (lane == 63) s_wave[wave] = run;
     __syncthreads();
-    double before = flow + run - sum, all = 0.0;
+    double before = flow + run - sum;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       if (w < wave) before += s_wave[w];
-      all += s_wave[w];
+      flow += s_wave[w];
     }
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       const int t = base + tid * kEach + i;
       if (t >= n) continue;
-      const float v = static_cast<float>(before + d[i]);
+      const float v = static_cast<float>(before + d[i] - miss * t);
       total += v;
       if (A.dg) {
-        const size_t at = (static_cast<size_t>(t0) + t) * A.H + h;
+        const size_t at = (t0 + t) * A.H + h;
         if (A.g_dtype == PRNN_F32)
           static_cast<float*>(A.dg)[at] = v;
         else if (A.g_dtype == PRNN_F16)
@@ -160,26 +198,22 @@ __global__ __launch_bounds__(256) void la_decay_grad_kernel(DecayGradArgs A) {
           static_cast<bf16*>(A.dg)[at] = from_f32<bf16>(v);
       }
     }
-    flow += all;
-    __syncthreads();
   }
-  if (A.per_seq) {
-#pragma unroll
-    for (int k = 1; k < 64; k <<= 1) total += __shfl_xor(total, k);
-    if (lane == 0) s_wave[wave] = total;
-    __syncthreads();
-    if (tid == 0)
-      A.per_seq[static_cast<size_t>(seq) * A.H + h] =
-          static_cast<float>(s_wave[0] + s_wave[1] + s_wave[2] + s_wave[3]);
+  if (A.per_part) {
+    total = block_sum(total, s_wave);
+    if (tid == 0) A.per_part[ph] = static_cast<float>(total);
   }
 }
 
-__global__ void la_decay_sum_kernel(const float* __restrict__ per_seq, void* dg, int g_dtype,
-                                    int n_seq, int H) {
-  const int h = blockIdx.x * blockDim.x + threadIdx.x;
-  if (h >= H) return;
+// One wave per head: the parts' sums in a fixed order.
+__global__ __launch_bounds__(64) void la_decay_sum_kernel(const float* __restrict__ per_part,
+                                                          void* dg, int g_dtype, int parts, int H) {
+  const int h = blockIdx.x;
   double d = 0.0;
-  for (int s = 0; s < n_seq; ++s) d += per_seq[static_cast<size_t>(s) * H + h];
+  for (int s = threadIdx.x; s < parts; s += 64) d += per_part[static_cast<size_t>(s) * H + h];
+#pragma unroll
+  for (int k = 1; k < 64; k <<= 1) d += __shfl_xor(d, k);
+  if (threadIdx.x) return;
   const float v = static_cast<float>(d);
   if (g_dtype == PRNN_F32)
     static_cast<float*>(dg)[h] = v;
@@ -266,13 +300,13 @@ int sequences(const Problem& a) { return a.cu_seqlens ? a.n_seq : a.B; }
 // How long the pieces are.  Walks of whole sequences read every array once; cut ones read k
 // and v once more and move a state a piece, so a sequence is cut only as far as the chip has
 // workgroups to spare (about kLaTarget run at a time), and never below kLaLeast tokens.
-constexpr int kLaTarget = 1536, kLaLeast = 256;
+constexpr int kLaTarget = 1536, kLaLeast = 256, kLaLeastF32 = 128;
 
-LaSeqs cut(const Problem& a, int tiles_and_roles) {
+LaSeqs cut(const Problem& a, bool bf16, int tiles_and_roles) {
   LaSeqs s{a.cu_seqlens, sequences(a), a.T, 1, 0};
   const long long work = 1ll * a.B * a.T * a.H * tiles_and_roles;
   long long len = (work + kLaTarget - 1) / kLaTarget;
-  len = std::max<long long>(kLaLeast, (len + 63) / 64 * 64);
+  len = std::max<long long>(bf16 ? kLaLeast : kLaLeastF32, (len + 63) / 64 * 64);
   if (len >= a.T) {
     s.len = a.T + 1;  // every sequence whole
     s.pieces = s.n_seq;
@@ -295,7 +329,7 @@ struct Scratch {
   float* decay[2];
   float* dots[2];
   float* heads[3];
-  float* per_seq;
+  float *last, *flow, *flow_end, *per_part;
   size_t bytes;
 };
 
@@ -318,9 +352,9 @@ struct Walks {
   }
 };
 
-LaSeqs forward_cut(const Problem& a, const Walks& w) { return cut(a, w.tiles(a.Dv)); }
+LaSeqs forward_cut(const Problem& a, const Walks& w) { return cut(a, w.bf16, w.tiles(a.Dv)); }
 LaSeqs backward_cut(const Problem& a, const Walks& w) {
-  return cut(a, 3 * w.tiles(std::max(a.Dk, a.Dv)));
+  return cut(a, w.bf16, 3 * w.tiles(std::max(a.Dk, a.Dv)));
 }
 
 Scratch carve(void* ws, const Problem& a, const Walks& w, bool backward, bool decay_grad) {
@@ -338,7 +372,11 @@ Scratch carve(void* ws, const Problem& a, const Walks& w, bool backward, bool de
     if (decay_grad) {
       const size_t tiles = w.tiles(std::max(a.Dk, a.Dv));
       for (float*& d : s.dots) d = static_cast<float*>(c.take(4 * tiles * a.H * tokens));
-      s.per_seq = static_cast<float*>(c.take(4 * static_cast<size_t>(a.H) * sequences(a)));
+      const size_t seqs = sequences(a);
+      s.last = static_cast<float*>(c.take(4 * dd * a.H * seqs));
+      s.flow = static_cast<float*>(c.take(4 * static_cast<size_t>(a.H) * (q.pieces + 1)));
+      s.flow_end = static_cast<float*>(c.take(4 * static_cast<size_t>(a.H) * seqs));
+      s.per_part = static_cast<float*>(c.take(4 * static_cast<size_t>(a.H) * q.pieces));
     }
     const int heads[3] = {a.q.heads, a.k.heads, a.v.heads}, D[3] = {a.Dk, a.Dk, a.Dv};
     for (int i = 0; i < 3; ++i)
@@ -496,6 +534,8 @@ int backward(const Problem& a, const prnn_la_view& go, const float* gs, void* dq
   }
   p.role[2].last = LaState{dh0, nullptr, sequences(a)};
   if (dg) {
+    // the final state, for the flow into it
+    if (gs) p.role[0].last = LaState{s.last, nullptr, sequences(a)};
     p.role[0].dot = q;
     p.role[0].dots = s.dots[0];
     p.role[1].dot = k;
@@ -519,6 +559,12 @@ int backward(const Problem& a, const prnn_la_view& go, const float* gs, void* dq
   if (dg) {
     DecayGradArgs d{};
     d.seqs = p.seqs;
+    if (w.bf16) {
+      // 16-bit results: tying whole sequences is enough
+      d.seqs.len = a.T + 1;
+      d.seqs.pieces = sequences(a);
+    }
+    d.g = p.g;
     d.q_dots = s.dots[0];
     d.k_dots = s.dots[1];
     const int cols = w.cols(std::max(a.Dk, a.Dv));
@@ -528,17 +574,23 @@ int backward(const Problem& a, const prnn_la_view& go, const float* gs, void* dq
     d.batch_tokens = static_cast<int>(tokens);
     d.h0 = init;
     d.dh0 = dh0;
+    d.last = s.last;
+    d.gs = gs;
+    d.state = s.state[0];
+    d.adjoint = s.state[1];
+    d.flow = s.flow;
+    d.flow_end = s.flow_end;
     d.g_dtype = a.g_dtype;
     const bool per_head = a.g_sb == 0 && a.g_st == 0;
     d.dg = per_head ? nullptr : dg;
-    d.per_seq = per_head ? s.per_seq : nullptr;
-    const int n_seq = sequences(a);
-    if (n_seq > 0) {
-      la_decay_grad_kernel<<<dim3(n_seq, a.H), 256, 0, st>>>(d);
-      PRNN_HIP(hipGetLastError());
-    }
+    d.per_part = per_head ? s.per_part : nullptr;
+    const dim3 grid(d.seqs.pieces, a.H);
+    la_flow_kernel<<<grid, 256, 0, st>>>(d);
+    PRNN_HIP(hipGetLastError());
+    la_decay_grad_kernel<<<grid, 256, 0, st>>>(d);
+    PRNN_HIP(hipGetLastError());
     if (per_head) {
-      la_decay_sum_kernel<<<(a.H + 63) / 64, 64, 0, st>>>(s.per_seq, dg, a.g_dtype, n_seq, a.H);
+      la_decay_sum_kernel<<<a.H, 64, 0, st>>>(s.per_part, dg, a.g_dtype, d.seqs.pieces, a.H);
       PRNN_HIP(hipGetLastError());
     }
   }
@@ -591,8 +643,7 @@ extern "C" PRNN_API int prnn_linear_attention_backward(
     return fail(PRNN_ERR_VALUE, "h0 has %d rows for %d sequences", a->h0_rows, sequences(*a));
   if (dg && a->h0 && !dh0)
     return fail(PRNN_ERR_VALUE, "the decays' gradient with an initial state needs dh0");
-  if (sequences(*a) == 0 && !(dg && a->g_sb == 0 && a->g_st == 0)) return PRNN_OK;
+  if (sequences(*a) == 0) return PRNN_OK;  // (an empty batch's decays per head: the caller's zeros)
   if (int rc = check_ws(need(*a, true, dg != nullptr), workspace, bytes)) return rc;
-  if (sequences(*a) == 0) return PRNN_OK;
   return backward(*a, *go, gs, dq, dk, dv, dg, dh0, workspace, static_cast<hipStream_t>(stream));
 }

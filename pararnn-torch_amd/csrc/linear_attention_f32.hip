@@ -18,9 +18,34 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 
 constexpr int kC = 32;  // tokens per chunk
 
-// exp(x) of a difference formed in fp64
-__device__ __forceinline__ float exp_diff(double a, double b) {
-  return fexp(static_cast<float>(a - b));
+// 2^x of a difference formed in fp64
+__device__ __forceinline__ float exp2_diff(double a, double b) {
+  return __builtin_amdgcn_exp2f(static_cast<float>(a - b));
+}
+
+// Lane i of a row of 16 gets lane i's neighbour's value by a DPP control (0 where there is none).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_add(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(u), CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), CTRL, ROWS, 0xf, false);
+  return v + __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+// Inclusive running sum over lanes 0 .. 31.
+__device__ __forceinline__ double scan_up(double v) {
+  v = dpp_add<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+  v = dpp_add<0x112, 0xf>(v);
+  v = dpp_add<0x114, 0xf>(v);
+  v = dpp_add<0x118, 0xf>(v);
+  return dpp_add<0x142, 0xa>(v);  // lane 15 to the next row
+}
+// Sum over a row of 16 lanes, in every lane: rotations by 8, 4, 2, 1.
+template <int CTRL>
+__device__ __forceinline__ float rot_add(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float row_sum(float v) {
+  return rot_add<0x121>(rot_add<0x122>(rot_add<0x124>(rot_add<0x128>(v))));
 }
 
 // Four elements of a row as they are stored (raw), from a buffer or one by one; zeros outside.
@@ -29,13 +54,20 @@ typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 template <typename T>
 struct Raw {
   using type = u2;
-  static __device__ __forceinline__ u2 load(rsrc_t r, uint32_t o, int left, bool vec) {
-    if (vec) return __builtin_amdgcn_raw_buffer_load_b64(r, la_in(left >= 4, o), 0, 0);
+  template <bool VEC>
+  static __device__ __forceinline__ u2 load(rsrc_t r, uint32_t o, int left) {
+    if (VEC) return __builtin_amdgcn_raw_buffer_load_b64(r, la_in(left >= 4, o), 0, 0);
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       w[i] = __builtin_amdgcn_raw_buffer_load_b16(r, la_in(i < left, o + 2 * i), 0, 0);
     return u2{(w[0] & 0xffffu) | w[1] << 16, (w[2] & 0xffffu) | w[3] << 16};
+  }
+  static __device__ __forceinline__ float one(rsrc_t r, uint32_t o) { return ldb<T>(r, o, 0); }
+  static __device__ __forceinline__ bool bad(u2 w) {
+    constexpr uint32_t kOnes = std::is_same_v<T, f16> ? 0x7c007c00u : 0x7f807f80u;
+    constexpr uint32_t kStep = std::is_same_v<T, f16> ? 0x04000400u : 0x00800080u;
+    return ((((w[0] & kOnes) + kStep) | ((w[1] & kOnes) + kStep)) & 0x80008000u) != 0;
   }
   static __device__ __forceinline__ f4 value(u2 w) {
     return f4{Narrow<T>::lo(w[0]), Narrow<T>::hi(w[0]), Narrow<T>::lo(w[1]), Narrow<T>::hi(w[1])};
@@ -44,13 +76,21 @@ struct Raw {
 template <>
 struct Raw<float> {
   using type = u4;
-  static __device__ __forceinline__ u4 load(rsrc_t r, uint32_t o, int left, bool vec) {
-    if (vec) return __builtin_amdgcn_raw_buffer_load_b128(r, la_in(left >= 4, o), 0, 0);
+  template <bool VEC>
+  static __device__ __forceinline__ u4 load(rsrc_t r, uint32_t o, int left) {
+    if (VEC) return __builtin_amdgcn_raw_buffer_load_b128(r, la_in(left >= 4, o), 0, 0);
     u4 w;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       w[i] = __builtin_amdgcn_raw_buffer_load_b32(r, la_in(i < left, o + 4 * i), 0, 0);
     return w;
+  }
+  static __device__ __forceinline__ float one(rsrc_t r, uint32_t o) { return ldb<float>(r, o, 0); }
+  static __device__ __forceinline__ bool bad(u4 w) {
+    uint32_t b = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b |= (w[i] & 0x7f800000u) + 0x00800000u;
+    return (b & 0x80000000u) != 0;
   }
   static __device__ __forceinline__ f4 value(u4 w) {
     return f4{__uint_as_float(w[0]), __uint_as_float(w[1]), __uint_as_float(w[2]),
@@ -58,30 +98,35 @@ struct Raw<float> {
   }
 };
 
-// KT: 32-column blocks of x and y (padded with zeros); W: waves, 16 columns of z each.
-template <typename T, int KT, int W, bool STATE_ONLY>
+constexpr int low_power(int n) { return n < 2 ? 1 : 2 * low_power(n / 2); }
+
+// KT: 32-column blocks of x and y (padded with zeros); W: waves, 16 columns of z each; VEC: rows
+// of x, y and z admit accesses of four elements.
+template <typename T, int KT, int W, bool VEC, bool STATE_ONLY>
 __global__ __launch_bounds__(64 * W) void la_walk_f32_kernel(LaParams P) {
   constexpr int KD = 32 * KT;
   constexpr int NT = 64 * W;
   constexpr int XS = KD + 4;       // row strides in floats: 16 rows of 16-byte reads and
   constexpr int ZS = 16 * W + 4;   // 4 rows, 4 apart, of 16 words each fall into different banks
   constexpr int PS = kC + 4;
-  constexpr int NX = kC * KD / 4 / NT;       // 16-byte loads of x (and y) per thread
-  constexpr int NZ = kC * 16 * W / 4 / NT;   // of z: 2
+  constexpr int UX = KD / 4, UZ = 4 * W;                     // units of four in a row
+  constexpr int DX = std::min(kC, low_power(NT / UX)), DZ = NT / UZ;  // rows that a round takes
+  constexpr int NX = kC / DX, NZ = kC / DZ;
   __shared__ __align__(16) float sx[STATE_ONLY ? 4 : kC * XS];
   __shared__ __align__(16) float sy[kC * XS];
   __shared__ __align__(16) float sz[kC * ZS];
   __shared__ __align__(16) float sp[STATE_ONLY ? 4 : kC * PS];
-  __shared__ double sG[kC];
-  __shared__ float se[kC], sw[kC], sdot[W][kC];
-  __shared__ float s_tot, s_sum;
+  __shared__ __align__(16) double sG[kC];
+  __shared__ __align__(16) float se[kC], sw[kC];
+  __shared__ float sdot[W][kC], s_tot, s_sum;
+  __shared__ int s_stop[2];
 
-  const LaPlace at = la_place(P);
-  if (!at.any) return;
-  const LaRole& R = P.role[at.role];
-  const int h = at.h, tile = at.tile, piece = at.piece;
-  const int tiles = (R.vd + 16 * W - 1) / (16 * W);
-  if (tile >= tiles) return;
+  const LaPlace place = la_place(P);
+  if (!place.any) return;
+  const LaRole& R = P.role[place.role];
+  const int h = place.h, tile = place.tile, piece = place.piece;
+  const int col0 = tile * 16 * W;            // first column of the workgroup
+  if (col0 >= R.vd) return;
   const LaPiece pc = la_piece(P.seqs, piece);
   if (STATE_ONLY) {
     // the piece that a walk ends with hands its state to none
@@ -92,10 +137,66 @@ __global__ __launch_bounds__(64 * W) void la_walk_f32_kernel(LaParams P) {
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   const int l16 = lane & 15, q4 = lane >> 4;
   const int b = la_batch(P.seqs, pc);
-  const int col0 = tile * 16 * W;            // first column of the workgroup
   const int col = col0 + 16 * wave + l16;    // this lane's column of the state and of out
   const size_t row_floats = static_cast<size_t>(P.H) * P.Dk * P.Dv;
   const size_t head_floats = static_cast<size_t>(h) * P.Dk * P.Dv;
+  const int n_tok = pc.end - pc.begin;
+  float sum_decay = 0.0f;
+  // token of local index i of the walk
+  auto token = [&](int i) { return R.rev ? pc.end - 1 - i : pc.begin + i; };
+
+  // A thread's loads of an array are rows apart by a constant number; what lies outside the
+  // piece or the width is read as zero (an offset outside the resource).
+  using raw = typename Raw<T>::type;
+  constexpr int SZ = sizeof(T);
+  const int rowx = tid / UX, cx = (tid % UX) * 4, rowz = tid / UZ, cz = (tid % UZ) * 4;
+  const bool loads_x = rowx < DX;  // all threads but where a row's units are no power of two
+  const int widthx = loads_x ? R.kd - cx : 0, widthz = R.vd - col0 - cz;
+  const int fx = R.rev ? kC - 1 - rowx : rowx, fz = R.rev ? kC - 1 - rowz : rowz;
+  const int ahead = R.rev ? -1 : 1;
+  const int stx = static_cast<int>(R.x.st) * SZ, sty = static_cast<int>(R.y.st) * SZ,
+            stz = static_cast<int>(R.z.st) * SZ;
+  raw rx[STATE_ONLY ? 1 : NX], ry[NX], rz[NZ];
+  LaBits rg{0, 0};
+  auto fetch = [&](int base) {
+    const int left = n_tok - base;
+    rg = la_step_decays<kC>(P.g, R.rev, pc, b, h, base, lane);
+    if (!STATE_ONLY) {
+      const rsrc_t bx = la_rows<kC>(R.x, SZ, b, h, R.rev, pc.begin, pc.end, base);
+#pragma unroll
+      for (int k = 0; k < NX; ++k)
+        rx[k] = Raw<T>::template load<VEC>(bx, (fx + ahead * k * DX) * stx + cx * SZ,
+                                           rowx + k * DX < left ? widthx : 0);
+    }
+    const rsrc_t by = la_rows<kC>(R.y, SZ, b, h, R.rev, pc.begin, pc.end, base);
+#pragma unroll
+    for (int k = 0; k < NX; ++k)
+      ry[k] = Raw<T>::template load<VEC>(by, (fx + ahead * k * DX) * sty + cx * SZ,
+                                         rowx + k * DX < left ? widthx : 0);
+    const rsrc_t bz = la_rows<kC>(R.z, SZ, b, h, R.rev, pc.begin, pc.end, base);
+#pragma unroll
+    for (int k = 0; k < NZ; ++k)
+      rz[k] = Raw<T>::template load<VEC>(bz, (fz + ahead * k * DZ) * stz + (col0 + cz) * SZ,
+                                         rowz + k * DZ < left ? widthz : 0);
+  };
+  // Decays of the chunk's first n tokens, to base 2: running sums in fp64, so that differences of
+  // nearby ones keep their digits.
+  auto decays = [&](uint32_t bits, int n) {
+    const float g = lane < n ? la_decay_value(P.g, bits) : 0.0f;
+    const double G = scan_up(g * 1.4426950408889634);
+    const double last = __shfl(G, kC - 1);
+    if (lane < kC) {
+      sG[lane] = G;
+      se[lane] = exp2_diff(G, 0.0) * R.x_scale;
+      sw[lane] = exp2_diff(last, G) * R.u_scale;
+    }
+    if (lane == 0) {
+      s_tot = exp2_diff(last, 0.0);
+      s_sum = static_cast<float>(last * 0.6931471805599453);
+    }
+  };
+  if (tid < 2) s_stop[tid] = kC;
+  fetch(0);
 
   // ---- the state before the piece
   f4 S[2 * KT];
@@ -119,86 +220,48 @@ __global__ __launch_bounds__(64 * W) void la_walk_f32_kernel(LaParams P) {
         }
     }
   }
+  __syncthreads();
 
-  const int n_tok = pc.end - pc.begin;
-  const int chunks = (n_tok + kC - 1) / kC;
-  float sum_decay = 0.0f;
-
-  // A thread's loads of an array are rows apart by a constant number; what lies outside the
-  // piece or the width is read as zero (an offset outside the resource).
-  using raw = typename Raw<T>::type;
-  constexpr int SZ = sizeof(T);
-  constexpr int UX = KD / 4, UZ = 4 * W, DX = NT / UX, DZ = NT / UZ;
-  const int rowx = tid / UX, cx = (tid % UX) * 4, rowz = tid / UZ, cz = col0 + (tid % UZ) * 4;
-  const int fx = R.rev ? kC - 1 - rowx : rowx, fz = R.rev ? kC - 1 - rowz : rowz;
-  const int ahead = R.rev ? -1 : 1;
-  const int stx = static_cast<int>(R.x.st) * SZ, sty = static_cast<int>(R.y.st) * SZ,
-            stz = static_cast<int>(R.z.st) * SZ;
-  raw rx[STATE_ONLY ? 1 : NX], ry[NX], rz[NZ];
-  LaBits rg{0, 0};
-  // token of local index i of the walk
-  auto token = [&](int i) { return R.rev ? pc.end - 1 - i : pc.begin + i; };
-  auto fetch = [&](int c) {
-    const int base = c * kC, left = n_tok - base;
-    rg = la_step_decays<kC>(P.g, R.rev, pc, b, h, base, lane);
-    if (!STATE_ONLY) {
-      const rsrc_t bx = la_rows<kC>(R.x, SZ, b, h, R.rev, pc.begin, pc.end, base);
-#pragma unroll
-      for (int k = 0; k < NX; ++k)
-        rx[k] = Raw<T>::load(bx, (fx + ahead * k * DX) * stx + cx * SZ,
-                             rowx + k * DX < left ? R.kd - cx : 0, R.x.vec && R.kd % 4 == 0);
-    }
-    const rsrc_t by = la_rows<kC>(R.y, SZ, b, h, R.rev, pc.begin, pc.end, base);
-#pragma unroll
-    for (int k = 0; k < NX; ++k)
-      ry[k] = Raw<T>::load(by, (fx + ahead * k * DX) * sty + cx * SZ,
-                           rowx + k * DX < left ? R.kd - cx : 0, R.y.vec && R.kd % 4 == 0);
-    const rsrc_t bz = la_rows<kC>(R.z, SZ, b, h, R.rev, pc.begin, pc.end, base);
-#pragma unroll
-    for (int k = 0; k < NZ; ++k)
-      rz[k] = Raw<T>::load(bz, (fz + ahead * k * DZ) * stz + cz * SZ,
-                           rowz + k * DZ < left ? R.vd - cz : 0, R.z.vec && R.vd % 4 == 0);
-  };
-  fetch(0);
-
-  for (int c = 0; c < chunks; ++c) {
-    const int base = c * kC;
+  int next = 0;
+  for (int base = 0, turn = 0; base < n_tok; base = next, turn ^= 1) {
 #pragma unroll
     for (int k = 0; k < NX; ++k) {
       const int o = (rowx + k * DX) * XS + cx;
-      if (!STATE_ONLY) *reinterpret_cast<f4*>(&sx[o]) = Raw<T>::value(rx[k]);
-      *reinterpret_cast<f4*>(&sy[o]) = Raw<T>::value(ry[k]);
-    }
-#pragma unroll
-    for (int k = 0; k < NZ; ++k)
-      *reinterpret_cast<f4*>(&sz[(rowz + k * DZ) * ZS + (tid % UZ) * 4]) = Raw<T>::value(rz[k]);
-    if (wave == 0) {
-      // running sums of the decays in fp64: differences of nearby ones keep their digits
-      double G = la_decay_value(P.g, rg.get());
-#pragma unroll
-      for (int d = 1; d < kC; d <<= 1) {
-        const double o = __shfl_up(G, d);
-        if (lane >= d) G += o;
-      }
-      const double last = __shfl(G, kC - 1);
-      if (lane < kC) {
-        sG[lane] = G;
-        se[lane] = fexp(static_cast<float>(G));
-        sw[lane] = exp_diff(last, G) * R.u_scale;
-      }
-      if (lane == 0) {
-        s_tot = fexp(static_cast<float>(last));
-        s_sum = static_cast<float>(last);
+      if (loads_x) {
+        if (!STATE_ONLY) *reinterpret_cast<f4*>(&sx[o]) = Raw<T>::value(rx[k]);
+        *reinterpret_cast<f4*>(&sy[o]) = Raw<T>::value(ry[k]);
       }
     }
-    fetch(c + 1);  // behind the piece's end nothing is loaded; a branch would be waited at
+    int stop_here = kC;
+#pragma unroll
+    for (int k = NZ - 1; k >= 0; --k) {
+      *reinterpret_cast<f4*>(&sz[(rowz + k * DZ) * ZS + cz]) = Raw<T>::value(rz[k]);
+      if (Raw<T>::bad(rz[k]) && rowz + k * DZ > 0) stop_here = rowz + k * DZ;
+    }
+    if (stop_here < kC) atomicMin(&s_stop[turn], stop_here);
+    if (wave == 0) decays(rg.get(), kC);
+    next = base + kC;
     __syncthreads();
+    if (tid == 0) s_stop[turn ^ 1] = kC;
+    const int stop = s_stop[turn];
+    if (stop < kC) {
+      // A masked pair is an exact zero, but zero times an infinity or NaN of a later token is
+      // not: where z holds one behind the chunk's first token (rare), the chunk ends before it
+      // and the next one begins there.
+      for (int e = stop * XS + tid; e < kC * XS; e += NT) sy[e] = 0.0f;
+      for (int e = stop * ZS + tid; e < kC * ZS; e += NT) sz[e] = 0.0f;
+      if (wave == 0) decays(rg.get(), stop);
+      next = base + stop;
+      __syncthreads();
+    }
+    const int n_here = min(n_tok, next) - base;  // tokens of this chunk
 
     // ---- the chunk's pairs, masked and decayed: quadrants (0,0), (1,0), (1,1)
+    float dv[2][4];
     if (!STATE_ONLY) {
       for (int id = wave; id < 3; id += W) {
         const int mi = id > 0, ni = id > 1;
-        f4 acc = {0, 0, 0, 0};
+        f4 acc[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
         const float* xr = &sx[(16 * mi + l16) * XS + 4 * q4];
         const float* yr = &sy[(16 * ni + l16) * XS + 4 * q4];
 #pragma unroll
@@ -207,18 +270,35 @@ __global__ __launch_bounds__(64 * W) void la_walk_f32_kernel(LaParams P) {
           const f4 bb = *reinterpret_cast<const f4*>(yr + 16 * t);
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], bb[r], acc, 0, 0, 0);
+            acc[r & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], bb[r], acc[r & 1], 0, 0, 0);
         }
         const int n = 16 * ni + l16;
         const double Gn = sG[n];
+        // not to be known before, or its masks are kept over the walk
+        int after = n - 16 * mi - 4 * q4;
+        asm volatile("" : "+v"(after));
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int m = 16 * mi + 4 * q4 + r;
-          sp[m * PS + n] = n <= m ? acc[r] * (R.p_scale * exp_diff(sG[m], Gn)) : 0.0f;
+          const float w = (acc[0][r] + acc[1][r]) * (R.p_scale * exp2_diff(sG[m], Gn));
+          sp[m * PS + n] = after <= r ? w : 0.0f;
         }
       }
-      __syncthreads();
+      // The rows that the output is multiplied with, then the next chunk's: what is waited for
+      // first is loaded first.  Behind the piece's end nothing is loaded; a branch would be
+      // waited at.
+      const rsrc_t bd = la_rows<kC>(R.dot, SZ, b, h, R.rev, pc.begin, pc.end, base);
+#pragma unroll
+      for (int mi = 0; mi < 2; ++mi)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int i = 16 * mi + 4 * q4 + r, row = R.rev ? kC - 1 - i : i;
+          dv[mi][r] = Raw<T>::one(bd, la_in((R.dots != nullptr) & (i < n_here) & (col < R.vd),
+                                            (row * static_cast<int>(R.dot.st) + col) * SZ));
+        }
     }
+    fetch(next);
+    if (!STATE_ONLY) __syncthreads();
 
     float zr[2][4];
 #pragma unroll
@@ -230,78 +310,47 @@ __global__ __launch_bounds__(64 * W) void la_walk_f32_kernel(LaParams P) {
     if (!STATE_ONLY) {
       f4 O[2] = {f4{0, 0, 0, 0}, f4{0, 0, 0, 0}};
 #pragma unroll
-      for (int t = 0; t < 2 * KT; ++t)
+      for (int t = 0; t < 2 * KT; ++t) {
+        const f4 a0 = *reinterpret_cast<const f4*>(&sx[l16 * XS + 16 * t + 4 * q4]);
+        const f4 a1 = *reinterpret_cast<const f4*>(&sx[(16 + l16) * XS + 16 * t + 4 * q4]);
 #pragma unroll
-        for (int mi = 0; mi < 2; ++mi) {
-          const f4 a = *reinterpret_cast<const f4*>(&sx[(16 * mi + l16) * XS + 16 * t + 4 * q4]);
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            O[mi] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], S[t][r], O[mi], 0, 0, 0);
+        for (int r = 0; r < 4; ++r) {
+          O[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(a0[r], S[t][r], O[0], 0, 0, 0);
+          O[1] = __builtin_amdgcn_mfma_f32_16x16x4f32(a1[r], S[t][r], O[1], 0, 0, 0);
         }
+      }
 #pragma unroll
       for (int mi = 0; mi < 2; ++mi) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) O[mi][r] *= R.x_scale * se[16 * mi + 4 * q4 + r];
+        const f4 e = *reinterpret_cast<const f4*>(&se[16 * mi + 4 * q4]);
+        O[mi] *= e;
       }
-      // A masked pair is an exact zero, but zero times an infinity or NaN of a later token is
-      // not: rows before a column's first such value (rare) are formed without it.
-      f4 clean[2] = {O[0], O[1]};
-      float bad = 0.0f;
+      const f4 p0 = *reinterpret_cast<const f4*>(&sp[l16 * PS + 4 * q4]);
+      const f4 p1 = *reinterpret_cast<const f4*>(&sp[(16 + l16) * PS + 4 * q4]);
+      const f4 p2 = *reinterpret_cast<const f4*>(&sp[(16 + l16) * PS + 16 + 4 * q4]);
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int s = 0; s < 4; ++s) bad = fmaf(zr[u][s], 0.0f, bad);
-      const bool rare = __any(bad != 0.0f);
-      int first = kC;
-      if (rare) {
-#pragma unroll
-        for (int u = 1; u >= 0; --u)
-#pragma unroll
-          for (int s = 3; s >= 0; --s)
-            if (zr[u][s] * 0.0f != 0.0f) first = 16 * u + 4 * q4 + s;
-        first = min(first, __shfl_xor(first, 16));
-        first = min(first, __shfl_xor(first, 32));
+      for (int s = 0; s < 4; ++s) {
+        O[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(p0[s], zr[0][s], O[0], 0, 0, 0);
+        O[1] = __builtin_amdgcn_mfma_f32_16x16x4f32(p1[s], zr[0][s], O[1], 0, 0, 0);
       }
 #pragma unroll
-      for (int mi = 0; mi < 2; ++mi)
-#pragma unroll
-        for (int u = 0; u <= mi; ++u) {
-          const f4 a = *reinterpret_cast<const f4*>(&sp[(16 * mi + l16) * PS + 16 * u + 4 * q4]);
-#pragma unroll
-          for (int s = 0; s < 4; ++s) {
-            O[mi] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[s], zr[u][s], O[mi], 0, 0, 0);
-            if (rare)
-              clean[mi] = __builtin_amdgcn_mfma_f32_16x16x4f32(
-                  a[s], 16 * u + 4 * q4 + s < first ? zr[u][s] : 0.0f, clean[mi], 0, 0, 0);
-          }
-        }
-      if (rare)
-#pragma unroll
-        for (int mi = 0; mi < 2; ++mi)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (16 * mi + 4 * q4 + r < first) O[mi][r] = clean[mi][r];
+      for (int s = 0; s < 4; ++s)
+        O[1] = __builtin_amdgcn_mfma_f32_16x16x4f32(p2[s], zr[1][s], O[1], 0, 0, 0);
+      const int so = R.out_f32 ? 4 : SZ;
+      const rsrc_t bo = la_rows<kC>(LaView{R.out, R.o_sb, R.o_st, R.o_sh, 1, 1}, so, b, h, R.rev,
+                                    pc.begin, pc.end, base);
 #pragma unroll
       for (int mi = 0; mi < 2; ++mi)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int i = 16 * mi + 4 * q4 + r;
-          const bool in = base + i < n_tok && col < R.vd;
-          const long long t = token(base + i);
-          if (in) {
-            const long long o = b * R.o_sb + t * R.o_st + h * R.o_sh + col;
-            if (R.out_f32)
-              static_cast<float*>(R.out)[o] = O[mi][r];
-            else
-              static_cast<T*>(R.out)[o] = from_f32<T>(O[mi][r]);
-          }
+          const int i = 16 * mi + 4 * q4 + r, row = R.rev ? kC - 1 - i : i;
+          const uint32_t o = la_in((i < n_here) & (col < R.vd),
+                                   (row * static_cast<int>(R.o_st) + col) * so);
+          if (R.out_f32)
+            stb<float>(bo, o, 0, O[mi][r]);
+          else
+            stb<T>(bo, o, 0, O[mi][r]);
           if (R.dots) {
-            float d = 0.0f;
-            if (in)
-              d = O[mi][r] * to_f32(static_cast<const T*>(R.dot.p)[b * R.dot.sb + t * R.dot.st +
-                                                                   (h / R.dot.rep) * R.dot.sh + col]);
-#pragma unroll
-            for (int k = 1; k < 16; k <<= 1) d += __shfl_xor(d, k);
+            const float d = row_sum(O[mi][r] * dv[mi][r]);
             if (l16 == 0) sdot[wave][i] = d;
           }
         }
@@ -311,26 +360,31 @@ __global__ __launch_bounds__(64 * W) void la_walk_f32_kernel(LaParams P) {
     const float tot = s_tot;
     sum_decay += s_sum;
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int u = 0; u < 2; ++u) {
+      const f4 w = *reinterpret_cast<const f4*>(&sw[16 * u + 4 * q4]);
 #pragma unroll
-      for (int s = 0; s < 4; ++s) zr[u][s] *= sw[16 * u + 4 * q4 + s];
+      for (int s = 0; s < 4; ++s) zr[u][s] *= w[s];
+    }
 #pragma unroll
-    for (int t = 0; t < 2 * KT; ++t) {
-      S[t] *= tot;
+    for (int t = 0; t < 2 * KT; ++t) S[t] *= tot;
+    // two tiles at a time: their chains of products run side by side
+#pragma unroll
+    for (int t = 0; t < 2 * KT; t += 2)
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int s = 0; s < 4; ++s)
-          S[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(sy[(16 * u + 4 * q4 + s) * XS + 16 * t + l16],
-                                                      zr[u][s], S[t], 0, 0, 0);
-    }
+        for (int s = 0; s < 4; ++s) {
+          const float* y = &sy[(16 * u + 4 * q4 + s) * XS + 16 * t + l16];
+          S[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(y[0], zr[u][s], S[t], 0, 0, 0);
+          S[t + 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(y[16], zr[u][s], S[t + 1], 0, 0, 0);
+        }
     __syncthreads();
-    if (!STATE_ONLY && R.dots && tid < kC && base + tid < n_tok) {
+    if (!STATE_ONLY && R.dots && tid < n_here) {
       float d = 0.0f;
 #pragma unroll
       for (int w = 0; w < W; ++w) d += sdot[w][tid];
       const size_t row = P.seqs.cu ? token(base + tid)
-                                  : static_cast<size_t>(b) * P.seqs.T + token(base + tid);
+                                   : static_cast<size_t>(b) * P.seqs.T + token(base + tid);
       R.dots[(static_cast<size_t>(tile) * P.H + h) * P.batch_tokens + row] = d;
     }
   }
@@ -359,28 +413,35 @@ __global__ __launch_bounds__(64 * W) void la_walk_f32_kernel(LaParams P) {
   }
 }
 
-template <typename T, int KT, int W>
+template <typename T, int KT, int W, bool VEC>
 int launch(const LaParams& p, bool state_only, hipStream_t stream) {
   const unsigned grid = la_grid(p), block = 64 * W;
   if (state_only)
-    la_walk_f32_kernel<T, KT, W, true><<<grid, block, 0, stream>>>(p);
+    la_walk_f32_kernel<T, KT, W, VEC, true><<<grid, block, 0, stream>>>(p);
   else
-    la_walk_f32_kernel<T, KT, W, false><<<grid, block, 0, stream>>>(p);
+    la_walk_f32_kernel<T, KT, W, VEC, false><<<grid, block, 0, stream>>>(p);
   PRNN_HIP(hipGetLastError());
   return PRNN_OK;
 }
 
 template <typename T, int KT>
 int launch_kt(const LaParams& p, int roles, bool state_only, hipStream_t stream) {
-  return la_f32_tile_cols(la_widest(p, roles)) == 32
-             ? launch<T, KT, 2>(p, state_only, stream)
-             : launch<T, KT, 4>(p, state_only, stream);
+  bool vec = true;
+  for (int i = 0; i < roles; ++i) {
+    const LaRole& r = p.role[i];
+    vec = vec && (state_only || r.x.vec) && r.y.vec && r.z.vec && r.kd % 4 == 0 && r.vd % 4 == 0;
+  }
+  if (la_f32_tile_cols(la_widest(p, roles)) == 32)
+    return vec ? launch<T, KT, 2, true>(p, state_only, stream)
+               : launch<T, KT, 2, false>(p, state_only, stream);
+  return vec ? launch<T, KT, 4, true>(p, state_only, stream)
+             : launch<T, KT, 4, false>(p, state_only, stream);
 }
 
 }  // namespace
 
-// two waves where all columns fit in 32, else four
-int la_f32_tile_cols(int vd) { return vd <= 32 ? 32 : 64; }
+// four waves, or two where four would leave half of them without columns
+int la_f32_tile_cols(int vd) { return (vd + 63) / 64 * 64 - vd >= 32 ? 32 : 64; }
 
 int la_walk_f32(LaParams p, int roles, bool state_only, int dtype, hipStream_t stream) {
   const int vd = la_widest(p, roles), cols = la_f32_tile_cols(vd);
@@ -392,6 +453,7 @@ int la_walk_f32(LaParams p, int roles, bool state_only, int dtype, hipStream_t s
     using T = decltype(z);
     if (kd <= 32) return launch_kt<T, 1>(p, roles, state_only, stream);
     if (kd <= 64) return launch_kt<T, 2>(p, roles, state_only, stream);
+    if (kd <= 96) return launch_kt<T, 3>(p, roles, state_only, stream);
     if (kd <= 128) return launch_kt<T, 4>(p, roles, state_only, stream);
     return launch_kt<T, 8>(p, roles, state_only, stream);
   });

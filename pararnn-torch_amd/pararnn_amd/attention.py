@@ -215,7 +215,8 @@ def _backward(p: _Problem, go: Tensor, gs: Tensor | None, need_g: bool, need_h0:
     go = _tiles(go)
     gs = None if gs is None else gs.contiguous()
     dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (p.q, p.k, p.v))
-    dg = torch.empty(p.g.shape, dtype=p.g.dtype, device=dev) if need_g else None
+    make = torch.empty if p.sequences else torch.zeros
+    dg = make(p.g.shape, dtype=p.g.dtype, device=dev) if need_g else None
     dh0 = None
     if p.h0 is not None and (need_g or need_h0):
         dh0 = torch.empty_like(p.h0)
