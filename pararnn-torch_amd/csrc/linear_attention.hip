@@ -1,7 +1,7 @@
 // Decayed linear attention: the small kernels around the walks and the C entry points.
 //
 // * la_join_kernel: states before a cut sequence's pieces from the pieces' own contributions;
-// * la_flow_kernel, la_decay_grad_kernel: the log decays' gradient.  dL/dg_t = exp(g_t)
+// * la_decay_grad_kernel: the log decays' gradient.  dL/dg_t = exp(g_t)
 //   <S_{t-1}, R_t> is the flow from all earlier tokens to t and later ones; from one token to the
 //   next it gains what token t hands on and loses what it receives, so it is a running sum of
 //   k_t . dk_t - q_t . dq_t (both formed in fp32 by the walks).  The flow itself stays bounded
@@ -86,7 +86,6 @@ struct DecayGradArgs {
   LaState h0;
   const float *dh0, *last, *gs;          // rows of sequences: dL/dS_0, S_T, dL/dS_T
   const float *state, *adjoint;          // [piece][head][DD] before the pieces, either direction
-  float *flow, *flow_end;                // (piece, H) at the parts' first tokens, (sequence, H)
   int g_dtype;
   void* dg;             // (token, H) of g's type, or NULL
   float* per_part;      // (piece, H) sums for decays per head, or NULL
@@ -107,28 +106,13 @@ __device__ __forceinline__ double block_dot(const float* a, const float* b, int 
   return block_sum(d, lds);
 }
 
-__global__ __launch_bounds__(256) void la_flow_kernel(DecayGradArgs A) {
-  __shared__ double lds[4];
-  const int p = blockIdx.x, h = blockIdx.y;
-  const LaPiece pc = la_piece(A.seqs, p);
-  if (pc.begin >= pc.end) return;
+// The flow at the first token of part p of a sequence: its state with the adjoint of that token,
+// which is the one before the part that lies ahead.
+__device__ __forceinline__ double flow_at(const DecayGradArgs& A, const LaPiece& pc, int p,
+                                          int begin, int h, double* lds) {
   const size_t row = static_cast<size_t>(A.H) * A.DD, head = static_cast<size_t>(h) * A.DD;
-  double begin = 0.0;
-  if (pc.first) {
-    if (const float* s0 = la_row(A.h0, pc.seq, row))
-      begin = block_dot(s0 + head, A.dh0 + pc.seq * row + head, A.DD, lds);
-  } else {
-    // the adjoint before the piece that lies ahead is that of this piece's first token
-    begin = block_dot(A.state + p * row + head, A.adjoint + (p - 1) * row + head, A.DD, lds) *
-            fexp(la_decay(A.g, la_batch(A.seqs, pc), pc.begin, h));
-  }
-  double end = 0.0;
-  if (pc.last && A.gs)
-    end = block_dot(A.last + pc.seq * row + head, A.gs + pc.seq * row + head, A.DD, lds);
-  if (threadIdx.x == 0) {
-    A.flow[static_cast<size_t>(p) * A.H + h] = static_cast<float>(begin);
-    if (pc.last) A.flow_end[static_cast<size_t>(pc.seq) * A.H + h] = static_cast<float>(end);
-  }
+  return block_dot(A.state + p * row + head, A.adjoint + (p - 1) * row + head, A.DD, lds) *
+         fexp(la_decay(A.g, la_batch(A.seqs, pc), begin, h));
 }
 
 __global__ __launch_bounds__(256) void la_decay_grad_kernel(DecayGradArgs A) {
@@ -152,8 +136,17 @@ __global__ __launch_bounds__(256) void la_decay_grad_kernel(DecayGradArgs A) {
     }
     return x;
   };
-  const double begin = A.flow[ph];
-  const double end = pc.last ? A.flow_end[static_cast<size_t>(pc.seq) * A.H + h] : A.flow[ph + A.H];
+  const size_t row = static_cast<size_t>(A.H) * A.DD;
+  const size_t head = pc.seq * row + static_cast<size_t>(h) * A.DD;
+  double begin = 0.0, end = 0.0;
+  if (!pc.first)
+    begin = flow_at(A, pc, p, pc.begin, h, s_wave);
+  else if (const float* s0 = la_row(A.h0, pc.seq, row))
+    begin = block_dot(s0 + static_cast<size_t>(h) * A.DD, A.dh0 + head, A.DD, s_wave);
+  if (!pc.last)
+    end = flow_at(A, pc, p + 1, pc.end, h, s_wave);
+  else if (A.gs)
+    end = block_dot(A.last + head, A.gs + head, A.DD, s_wave);
   double all = 0.0;
   for (int t = tid; t < n; t += 256) all += step(t);
   all = block_sum(all, s_wave);
@@ -329,7 +322,7 @@ struct Scratch {
   float* decay[2];
   float* dots[2];
   float* heads[3];
-  float *last, *flow, *flow_end, *per_part;
+  float *last, *per_part;
   size_t bytes;
 };
 
@@ -374,8 +367,6 @@ Scratch carve(void* ws, const Problem& a, const Walks& w, bool backward, bool de
       for (float*& d : s.dots) d = static_cast<float*>(c.take(4 * tiles * a.H * tokens));
       const size_t seqs = sequences(a);
       s.last = static_cast<float*>(c.take(4 * dd * a.H * seqs));
-      s.flow = static_cast<float*>(c.take(4 * static_cast<size_t>(a.H) * (q.pieces + 1)));
-      s.flow_end = static_cast<float*>(c.take(4 * static_cast<size_t>(a.H) * seqs));
       s.per_part = static_cast<float*>(c.take(4 * static_cast<size_t>(a.H) * q.pieces));
     }
     const int heads[3] = {a.q.heads, a.k.heads, a.v.heads}, D[3] = {a.Dk, a.Dk, a.Dv};
@@ -578,15 +569,11 @@ int backward(const Problem& a, const prnn_la_view& go, const float* gs, void* dq
     d.gs = gs;
     d.state = s.state[0];
     d.adjoint = s.state[1];
-    d.flow = s.flow;
-    d.flow_end = s.flow_end;
     d.g_dtype = a.g_dtype;
     const bool per_head = a.g_sb == 0 && a.g_st == 0;
     d.dg = per_head ? nullptr : dg;
     d.per_part = per_head ? s.per_part : nullptr;
     const dim3 grid(d.seqs.pieces, a.H);
-    la_flow_kernel<<<grid, 256, 0, st>>>(d);
-    PRNN_HIP(hipGetLastError());
     la_decay_grad_kernel<<<grid, 256, 0, st>>>(d);
     PRNN_HIP(hipGetLastError());
     if (per_head) {

@@ -55,20 +55,22 @@ def _tiles(t: Tensor) -> Tensor:
     values give equal bits: the bfloat16 one (widths in eights) reads 16 bytes at a time, and rows
     that do not lie for that (a view of a fused projection with an odd offset, a row expanded over
     time) are copied."""
-    t = _rows(t)
-    if abs(t.stride(1)) * t.element_size() > 1 << 24:  # the kernels' offsets inside a chunk
+    sb, st, sh, sd = t.stride()
+    width = t.shape[3]
+    # at most 16 MiB between tokens: the kernels' offsets inside a chunk
+    if (sd != 1 and width != 1) or st > 1 << 22:
         t = t.contiguous()
-    if t.dtype != torch.bfloat16 or t.shape[-1] % 8:
+        sb, st, sh, _ = t.stride()
+    if t.dtype is not torch.bfloat16 or width % 8:
         return t
-    sb, st, sh, _ = t.stride()
-    if (sb | st | sh) % 8 == 0 and t.data_ptr() % 16 == 0 and (st >= t.shape[-1]
-                                                               or t.shape[1] == 1):
+    if (sb | st | sh) % 8 == 0 and t.data_ptr() % 16 == 0 and (st >= width or t.shape[1] == 1):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
 def _view(t: Tensor) -> _lib.LaView:
-    return _lib.LaView(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2), t.shape[2])
+    sb, st, sh, _ = t.stride()
+    return _lib.LaView(t.data_ptr(), sb, st, sh, t.shape[2])
 
 
 def _heads(what: str, *counts: int) -> int:
@@ -121,29 +123,33 @@ class _Problem:
     def __init__(self, q: Tensor, k: Tensor, v: Tensor, g: Tensor, h0: Tensor | None,
                  table: Tensor | None, packed: PackedSequences | None, scale: float | None):
         what = "linear_attention"
-        code = _validate(what, q, k, v)
+        code = _DTYPES.get(q.dtype)
+        # the quick look first: calls of small sizes are bound by the host
+        if not (code is not None and q.is_cuda and k.dtype is q.dtype and v.dtype is q.dtype
+                and k.device == q.device and v.device == q.device):
+            code = _validate(what, q, k, v)
         for n, t in (("q", q), ("k", k), ("v", v)):
             if t.dim() != 4:
                 raise ValueError(f"{what}: {n} must be (B, T, heads, width), got "
                                  f"{tuple(t.shape)}")
-        batch, time = q.shape[:2]
-        if k.shape[:2] != (batch, time) or v.shape[:2] != (batch, time):
-            raise ValueError(f"{what}: q, k and v disagree on (B, T): {tuple(q.shape[:2])}, "
-                             f"{tuple(k.shape[:2])}, {tuple(v.shape[:2])}")
-        if q.shape[3] != k.shape[3]:
-            raise ValueError(f"{what}: q has width {q.shape[3]}, k {k.shape[3]}")
+        (batch, time, hq, dk), (bk, tk, hk, dk2), (bv, tv, hv, dv) = q.shape, k.shape, v.shape
+        if bk != batch or bv != batch or tk != time or tv != time:
+            raise ValueError(f"{what}: q, k and v disagree on (B, T): {(batch, time)}, "
+                             f"{(bk, tk)}, {(bv, tv)}")
+        if dk2 != dk:
+            raise ValueError(f"{what}: q has width {dk}, k {dk2}")
         g_code = _decay_code(what, g, q)
         if g.dim() not in (1, 3) or (g.dim() == 3 and g.shape[:2] != (batch, time)):
             raise ValueError(f"{what}: log_decay must be (H,) or (B, T, H), got "
                              f"{tuple(g.shape)}")
-        heads = _heads(what, q.shape[2], k.shape[2], v.shape[2])
+        heads = max(hq, hk, hv, g.shape[-1])
+        if heads < 1 or (hq != heads and (hq < 1 or heads % hq)) or (
+                hk != heads and (hk < 1 or heads % hk)) or (
+                hv != heads and (hv < 1 or heads % hv)):
+            raise ValueError(f"{what}: head counts {(hq, hk, hv)} do not divide {heads}")
         if g.shape[-1] != heads:
-            if g.shape[-1] % heads:
-                raise ValueError(f"{what}: log_decay has {g.shape[-1]} heads, q, k and v have "
-                                 f"{heads}")
-            heads = _heads(what, q.shape[2], k.shape[2], v.shape[2], g.shape[-1])
+            raise ValueError(f"{what}: log_decay has {g.shape[-1]} heads, q, k and v have {heads}")
         self.q, self.k, self.v, self.g = _tiles(q), _tiles(k), _tiles(v), g
-        dk, dv = q.shape[3], v.shape[3]
         if not 1 <= dk <= 256 or not 1 <= dv <= 256:
             raise ValueError(f"{what}: head widths ({dk}, {dv}) are not in 1 .. 256")
         self.dims = (batch, time, heads, dk, dv)
