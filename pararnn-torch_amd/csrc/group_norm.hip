@@ -371,6 +371,9 @@ __global__ __launch_bounds__(1024) void norm_param_kernel(const float* __restric
 // A sample (L tokens) is cut into strips of rows, one workgroup each.  Threads lie over the
 // channels, V to a thread, and over as many rows at a time as fit.
 
+constexpr int kJoinGroups = 64;  // groups of a sample whose sums every workgroup forms itself
+constexpr int kRows = 4;         // rows of a thread under way at a time
+
 struct SamplePlace {
   int slots, rows_per, row, slot;
   bool on;
@@ -455,16 +458,22 @@ __global__ __launch_bounds__(256) void norm_sample_stats_kernel(NormArgs A) {
     for (int i = 0; i < V; ++i) mean[i] = m2[i] = 0.0f;
     float cnt = 0.0f;
     if (on)
-      for (int l = l0 + p.row; l < l1; l += p.rows_per) {
-        float v[V];
-        loadv<T, V>(x + static_cast<size_t>(l) * A.C + slot * V, v);
-        cnt += 1.0f;
-        const float inv = frcp(cnt);
+      for (int l = l0 + p.row; l < l1; l += kRows * p.rows_per) {
+        float v[kRows][V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float d = v[i] - mean[i];
-          mean[i] = fmaf(d, inv, mean[i]);
-          m2[i] = fmaf(d, v[i] - mean[i], m2[i]);
+        for (int k = 0; k < kRows; ++k)
+          loadv<T, V>(x + static_cast<size_t>(min(l + k * p.rows_per, l1 - 1)) * A.C + slot * V, v[k]);
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) {
+          if (l + k * p.rows_per >= l1) break;
+          cnt += 1.0f;
+          const float inv = frcp(cnt);
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float d = v[k][i] - mean[i];
+            mean[i] = fmaf(d, inv, mean[i]);
+            m2[i] = fmaf(d, v[k][i] - mean[i], m2[i]);
+          }
         }
       }
     __syncthreads();
@@ -511,71 +520,123 @@ __global__ __launch_bounds__(256) void norm_sample_stats_kernel(NormArgs A) {
   }
 }
 
-// Mean and rstd per (sample, group) from the strips.
+// Mean and rstd of a (sample, group) from its strips, by the 8 lanes of a thread's share.
+__device__ __forceinline__ double sum_8(double v) {
+#pragma unroll
+  for (int k = 1; k < 8; k <<= 1) v += __shfl_xor(v, k);
+  return v;
+}
+__device__ __forceinline__ void join_group(const NormArgs& A, int n, int g, bool on,
+                                           float& mean_out, float& rstd_out) {
+  const float2* e = reinterpret_cast<const float2*>(A.part) + static_cast<size_t>(n) * A.strips * A.G + g;
+  const int strips = on ? A.strips : 0, sub = threadIdx.x & 7;
+  // sums of means and of squares in fp64: one pass, 8 strips a lane under way
+  double s1 = 0.0, s2 = 0.0;
+  for (int k0 = sub; k0 < strips; k0 += 64) {
+    float2 v[8];  // mean, squared deviations
+    float c[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int k = k0 + 8 * i;
+      v[i] = float2{0.0f, 0.0f};
+      if (k < strips) v[i] = e[static_cast<size_t>(k) * A.G];
+      c[i] = k < strips ? static_cast<float>(min(A.strip_rows, A.L - k * A.strip_rows)) : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const double m = v[i].x, cm = c[i] * m;
+      s1 += cm;
+      s2 += v[i].y + cm * m * A.Cg;
+    }
+  }
+  const double mean = sum_8(s1) / A.L;
+  const double var = sum_8(s2) / (static_cast<double>(A.L) * A.Cg) - mean * mean;
+  mean_out = static_cast<float>(mean);
+  rstd_out = static_cast<float>(1.0 / sqrt((var > 0.0 ? var : var == var ? 0.0 : var) + A.eps));
+}
+
+// The same for every (sample, group): 32 a workgroup.
 __global__ __launch_bounds__(256) void norm_sample_join_kernel(NormArgs A) {
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const long long id = static_cast<long long>(blockIdx.x) * 4 + wave;
-  if (id >= static_cast<long long>(A.N) * A.G) return;
-  const int n = static_cast<int>(id / A.G), g = static_cast<int>(id - static_cast<long long>(n) * A.G);
-  const float* e = A.part + static_cast<size_t>(n) * A.strips * A.G * 2 + 2 * g;
-  double s = 0.0;
-  for (int k = lane; k < A.strips; k += 64) {
-    const double c = min(A.strip_rows, A.L - k * A.strip_rows);
-    s += c * e[static_cast<size_t>(k) * A.G * 2];
-  }
-#pragma unroll
-  for (int k = 1; k < 64; k <<= 1) s += __shfl_xor(s, k);
-  const double mean = s / A.L;
-  s = 0.0;
-  for (int k = lane; k < A.strips; k += 64) {
-    const double c = static_cast<double>(min(A.strip_rows, A.L - k * A.strip_rows)) * A.Cg;
-    const double d = e[static_cast<size_t>(k) * A.G * 2] - mean;
-    s += e[static_cast<size_t>(k) * A.G * 2 + 1] + c * d * d;
-  }
-#pragma unroll
-  for (int k = 1; k < 64; k <<= 1) s += __shfl_xor(s, k);
-  if (lane == 0) {
-    const double var = s / (static_cast<double>(A.L) * A.Cg);
-    A.stats[2 * id] = static_cast<float>(mean);
-    A.stats[2 * id + 1] = static_cast<float>(1.0 / sqrt(var + A.eps));
+  const long long id = static_cast<long long>(blockIdx.x) * 32 + (threadIdx.x >> 3);
+  const bool on = id < static_cast<long long>(A.N) * A.G;
+  const int n = on ? static_cast<int>(id / A.G) : 0;
+  const int g = on ? static_cast<int>(id - static_cast<long long>(n) * A.G) : 0;
+  float mean, rstd;
+  join_group(A, n, g, on, mean, rstd);
+  if (on && (threadIdx.x & 7) == 0) {
+    A.stats[2 * id] = mean;
+    A.stats[2 * id + 1] = rstd;
   }
 }
 
-// y of a strip.
-template <typename T, int V>
+// y of a strip.  JOIN: every workgroup forms its sample's statistics from the strips' itself (the
+// first one keeps them for the backward pass): with few groups that is cheaper than a launch.
+template <typename T, int V, bool JOIN>
 __global__ __launch_bounds__(256) void norm_sample_apply_kernel(NormArgs A) {
+  __shared__ float s_stats[JOIN ? 2 * kJoinGroups : 2];
   const int n = blockIdx.x / A.strips, strip = blockIdx.x - n * A.strips;
   const SamplePlace p = sample_place<V>(A);
+  if (JOIN) {
+    for (int g0 = 0; g0 < A.G; g0 += 32) {
+      const int g = g0 + (threadIdx.x >> 3);
+      const bool on = g < A.G;
+      float mean, rstd;
+      join_group(A, n, on ? g : 0, on, mean, rstd);
+      if (on && (threadIdx.x & 7) == 0) {
+        s_stats[2 * g] = mean;
+        s_stats[2 * g + 1] = rstd;
+        if (strip == 0) {
+          A.stats[2 * (static_cast<size_t>(n) * A.G + g)] = mean;
+          A.stats[2 * (static_cast<size_t>(n) * A.G + g) + 1] = rstd;
+        }
+      }
+    }
+    __syncthreads();
+  }
   const int l0 = strip * A.strip_rows, l1 = min(A.L, l0 + A.strip_rows);
   const size_t base = static_cast<size_t>(n) * A.L * A.C;
   if (!p.on) return;
   for (int slot = p.slot; slot < p.slots; slot += 256) {
     const int c = slot * V, g = c / A.Cg;
-    const float mean = A.stats[2 * (static_cast<size_t>(n) * A.G + g)];
-    const float rstd = A.stats[2 * (static_cast<size_t>(n) * A.G + g) + 1];
+    const float* st = JOIN ? &s_stats[2 * g] : &A.stats[2 * (static_cast<size_t>(n) * A.G + g)];
+    const float mean = st[0], rstd = st[1];
     float w[V], b[V];
     params<T, V>(A.w, A.w_f32, A.w_vec, c, 1.0f, w);
     params<T, V>(A.b, A.w_f32, A.w_vec, c, 0.0f, b);
-    for (int l = l0 + p.row; l < l1; l += p.rows_per) {
-      const size_t at = base + static_cast<size_t>(l) * A.C + c;
-      float x[V], gt[V], y[V];
-      loadv<T, V>(static_cast<const T*>(A.x) + at, x);
-      if (A.gate) loadv<T, V>(static_cast<const T*>(A.gate) + at, gt);
+    // kRows rows under way at a time
+    for (int l = l0 + p.row; l < l1; l += kRows * p.rows_per) {
+      float x[kRows][V], gt[kRows][V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float z = fmaf(w[i], (x[i] - mean) * rstd, b[i]);
-        y[i] = A.gate ? z * act_of(A.act, gt[i]) : act_of(A.act, z);
+      for (int k = 0; k < kRows; ++k) {
+        const int r = min(l + k * p.rows_per, l1 - 1);
+        const size_t at = base + static_cast<size_t>(r) * A.C + c;
+        loadv<T, V>(static_cast<const T*>(A.x) + at, x[k]);
+        if (A.gate) loadv<T, V>(static_cast<const T*>(A.gate) + at, gt[k]);
       }
-      storev<T, V>(static_cast<T*>(A.y) + at, y);
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) {
+        if (l + k * p.rows_per >= l1) break;
+        const size_t at = base + static_cast<size_t>(l + k * p.rows_per) * A.C + c;
+        float y[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float z = fmaf(w[i], (x[k][i] - mean) * rstd, b[i]);
+          y[i] = A.gate ? z * act_of(A.act, gt[k][i]) : act_of(A.act, z);
+        }
+        storev<T, V>(static_cast<T*>(A.y) + at, y);
+      }
     }
     if (p.slots <= 256) break;
   }
 }
 
-// Sums of dz h and dz of a strip per channel: part [N * strips][2][C]; dgate on the way.
-template <typename T, int V>
+// Sums of dz h and dz of a strip per channel: part [N * strips][2][C]; dgate on the way.  JOIN
+// (all channels in the workgroup at once): also those of dh h and dh per group, part2
+// [N * strips][2][G].
+template <typename T, int V, bool JOIN>
 __global__ __launch_bounds__(256) void norm_sample_bwd_sums_kernel(NormArgs A) {
   __shared__ float red[256];
+  __shared__ float s_ch[JOIN ? 2 * 256 * V : 2];
   const int n = blockIdx.x / A.strips, strip = blockIdx.x - n * A.strips;
   const SamplePlace p = sample_place<V>(A);
   const int l0 = strip * A.strip_rows, l1 = min(A.L, l0 + A.strip_rows);
@@ -593,27 +654,37 @@ __global__ __launch_bounds__(256) void norm_sample_bwd_sums_kernel(NormArgs A) {
 #pragma unroll
     for (int i = 0; i < V; ++i) dw[i] = db[i] = 0.0f;
     if (on)
-      for (int l = l0 + p.row; l < l1; l += p.rows_per) {
-        const size_t at = base + static_cast<size_t>(l) * A.C + c;
-        float x[V], gt[V], dz[V];
-        loadv<T, V>(static_cast<const T*>(A.x) + at, x);
-        loadv<T, V>(static_cast<const T*>(A.gy) + at, dz);
-        if (A.gate) loadv<T, V>(static_cast<const T*>(A.gate) + at, gt);
+      for (int l = l0 + p.row; l < l1; l += kRows * p.rows_per) {
+        float xs[kRows][V], gs[kRows][V], ys[kRows][V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float h = (x[i] - mean) * rstd, z = fmaf(w[i], h, b[i]);
-          float f, d;
-          act_grad(A.act, A.gate ? gt[i] : z, f, d);
-          if (A.gate) {
-            gt[i] = dz[i] * z * d;
-            dz[i] *= f;
-          } else {
-            dz[i] *= d;
-          }
-          dw[i] = fmaf(dz[i], h, dw[i]);
-          db[i] += dz[i];
+        for (int k = 0; k < kRows; ++k) {
+          const int r = min(l + k * p.rows_per, l1 - 1);
+          const size_t at = base + static_cast<size_t>(r) * A.C + c;
+          loadv<T, V>(static_cast<const T*>(A.x) + at, xs[k]);
+          loadv<T, V>(static_cast<const T*>(A.gy) + at, ys[k]);
+          if (A.gate) loadv<T, V>(static_cast<const T*>(A.gate) + at, gs[k]);
         }
-        if (A.gate) storev<T, V>(static_cast<T*>(A.dgate) + at, gt);
+#pragma unroll
+        for (int k = 0; k < kRows; ++k) {
+          if (l + k * p.rows_per >= l1) break;
+          const size_t at = base + static_cast<size_t>(l + k * p.rows_per) * A.C + c;
+          float *x = xs[k], *gt = gs[k], *dz = ys[k];
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            const float h = (x[i] - mean) * rstd, z = fmaf(w[i], h, b[i]);
+            float f, d;
+            act_grad(A.act, A.gate ? gt[i] : z, f, d);
+            if (A.gate) {
+              gt[i] = dz[i] * z * d;
+              dz[i] *= f;
+            } else {
+              dz[i] *= d;
+            }
+            dw[i] = fmaf(dz[i], h, dw[i]);
+            db[i] += dz[i];
+          }
+          if (A.gate) storev<T, V>(static_cast<T*>(A.dgate) + at, gt);
+        }
       }
 #pragma unroll
     for (int i = 0; i < V; ++i)
@@ -628,8 +699,21 @@ __global__ __launch_bounds__(256) void norm_sample_bwd_sums_kernel(NormArgs A) {
           if (p.row == 0)
             for (int r = 1; r < p.rows_per; ++r) sum += red[r * p.slots + threadIdx.x];
         }
-        if (p.row == 0 && on) out[which * A.C + c + i] = sum;
+        if (p.row == 0 && on) {
+          out[which * A.C + c + i] = sum;
+          if (JOIN) s_ch[which * 256 * V + c + i] = w[i] * sum;
+        }
       }
+    if (JOIN) {
+      __syncthreads();
+      for (int k = threadIdx.x; k < 2 * A.G; k += 256) {
+        const int which = k / A.G, gg = k - which * A.G;
+        const float* e = &s_ch[which * 256 * V + gg * A.Cg];
+        float sum = 0.0f;
+        for (int i = 0; i < A.Cg; ++i) sum += e[i];
+        A.part2[(static_cast<size_t>(n) * A.strips + strip) * 2 * A.G + k] = sum;
+      }
+    }
   }
 }
 
@@ -661,10 +745,33 @@ __global__ __launch_bounds__(256) void norm_sample_means_kernel(NormArgs A) {
   }
 }
 
-template <typename T, int V>
+// dx of a strip.  JOIN: m1 and m2 of the sample's groups from the strips' sums, in every workgroup.
+template <typename T, int V, bool JOIN>
 __global__ __launch_bounds__(256) void norm_sample_dx_kernel(NormArgs A) {
+  __shared__ float s_m[JOIN ? 2 * kJoinGroups : 2];
   const int n = blockIdx.x / A.strips, strip = blockIdx.x - n * A.strips;
   const SamplePlace p = sample_place<V>(A);
+  if (JOIN) {
+    for (int k0 = 0; k0 < 2 * A.G; k0 += 32) {
+      const int k = k0 + (threadIdx.x >> 3);
+      const int strips = k < 2 * A.G ? A.strips : 0;
+      double s = 0.0;
+      for (int i0 = threadIdx.x & 7; i0 < strips; i0 += 64) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int i = i0 + 8 * j;
+          v[j] = i < strips ? A.part2[(static_cast<size_t>(n) * A.strips + i) * 2 * A.G + k] : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s += v[j];
+      }
+      s = sum_8(s);
+      if (strips && (threadIdx.x & 7) == 0)
+        s_m[k] = static_cast<float>(s / (static_cast<double>(A.L) * A.Cg));
+    }
+    __syncthreads();
+  }
   const int l0 = strip * A.strip_rows, l1 = min(A.L, l0 + A.strip_rows);
   const size_t base = static_cast<size_t>(n) * A.L * A.C;
   if (!p.on) return;
@@ -672,29 +779,39 @@ __global__ __launch_bounds__(256) void norm_sample_dx_kernel(NormArgs A) {
     const int c = slot * V, g = c / A.Cg;
     const size_t ng = static_cast<size_t>(n) * A.G + g;
     const float mean = A.stats[2 * ng], rstd = A.stats[2 * ng + 1];
-    const float m1 = A.part2[2 * ng], m2 = A.part2[2 * ng + 1];
+    const float m1 = JOIN ? s_m[A.G + g] : A.part2[2 * ng], m2 = JOIN ? s_m[g] : A.part2[2 * ng + 1];
     float w[V], b[V];
     params<T, V>(A.w, A.w_f32, A.w_vec, c, 1.0f, w);
     params<T, V>(A.b, A.w_f32, A.w_vec, c, 0.0f, b);
-    for (int l = l0 + p.row; l < l1; l += p.rows_per) {
-      const size_t at = base + static_cast<size_t>(l) * A.C + c;
-      float x[V], gt[V], dz[V];
-      loadv<T, V>(static_cast<const T*>(A.x) + at, x);
-      loadv<T, V>(static_cast<const T*>(A.gy) + at, dz);
-      if (A.gate) loadv<T, V>(static_cast<const T*>(A.gate) + at, gt);
+    for (int l = l0 + p.row; l < l1; l += kRows * p.rows_per) {
+      float xs[kRows][V], gs[kRows][V], ys[kRows][V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float h = (x[i] - mean) * rstd, z = fmaf(w[i], h, b[i]);
-        if (A.gate) {
-          dz[i] *= act_of(A.act, gt[i]);
-        } else {
-          float f, d;
-          act_grad(A.act, z, f, d);
-          dz[i] *= d;
-        }
-        x[i] = rstd * (fmaf(w[i], dz[i], -m1) - h * m2);
+      for (int k = 0; k < kRows; ++k) {
+        const int r = min(l + k * p.rows_per, l1 - 1);
+        const size_t at = base + static_cast<size_t>(r) * A.C + c;
+        loadv<T, V>(static_cast<const T*>(A.x) + at, xs[k]);
+        loadv<T, V>(static_cast<const T*>(A.gy) + at, ys[k]);
+        if (A.gate) loadv<T, V>(static_cast<const T*>(A.gate) + at, gs[k]);
       }
-      storev<T, V>(static_cast<T*>(A.dx) + at, x);
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) {
+        if (l + k * p.rows_per >= l1) break;
+        const size_t at = base + static_cast<size_t>(l + k * p.rows_per) * A.C + c;
+        float *x = xs[k], *gt = gs[k], *dz = ys[k];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float h = (x[i] - mean) * rstd, z = fmaf(w[i], h, b[i]);
+          if (A.gate) {
+            dz[i] *= act_of(A.act, gt[i]);
+          } else {
+            float f, d;
+            act_grad(A.act, z, f, d);
+            dz[i] *= d;
+          }
+          x[i] = rstd * (fmaf(w[i], dz[i], -m1) - h * m2);
+        }
+        storev<T, V>(static_cast<T*>(A.dx) + at, x);
+      }
     }
     if (p.slots <= 256) break;
   }
@@ -738,10 +855,10 @@ Plan plan(int N, int L, int Cg, int G, int dtype, uintptr_t bits, bool backward)
     p.blocks_x = std::max(1, std::min(need, most));
     return p;
   }
-  // strips: enough workgroups for the chip, at least 8 rounds of rows each
+  // strips: enough workgroups for the chip, each of at least kRows rounds of rows
   const int slots = G * Cg / p.V, rows_per = slots <= 256 ? 256 / slots : 1;
-  const int want = std::max(1, 1024 / std::max(1, N));
-  p.strip_rows = std::max((L + want - 1) / want, 8 * rows_per);
+  const int want = std::max(1, 512 / std::max(1, N));
+  p.strip_rows = std::max((L + want - 1) / want, kRows * rows_per);
   p.strips = (L + p.strip_rows - 1) / p.strip_rows;
   return p;
 }
@@ -804,7 +921,7 @@ extern "C" PRNN_API size_t prnn_group_norm_workspace_size(int N, int L, int C, i
       c.take(sizeof(float) * 2 * G * p.strips * static_cast<size_t>(N));
     } else {
       c.take(sizeof(float) * 2 * C * p.strips * static_cast<size_t>(N));
-      c.take(sizeof(float) * 2 * G * static_cast<size_t>(N));
+      c.take(sizeof(float) * 2 * G * p.strips * static_cast<size_t>(N));
     }
     most = std::max(most, c.used);
   }
@@ -863,10 +980,13 @@ extern "C" PRNN_API int prnn_group_norm(const void* x, const void* w, const void
     const dim3 grid(static_cast<unsigned>(p.strips) * N);
     norm_sample_stats_kernel<T, V><<<grid, 256, 256 * 2 * V * sizeof(float), st>>>(a);
     PRNN_HIP(hipGetLastError());
-    const unsigned joins = static_cast<unsigned>((1ll * N * G + 3) / 4);
-    norm_sample_join_kernel<<<joins, 256, 0, st>>>(a);
-    PRNN_HIP(hipGetLastError());
-    norm_sample_apply_kernel<T, V><<<grid, 256, 0, st>>>(a);
+    if (G <= kJoinGroups) {
+      norm_sample_apply_kernel<T, V, true><<<grid, 256, 0, st>>>(a);
+    } else {
+      norm_sample_join_kernel<<<static_cast<unsigned>((1ll * N * G + 31) / 32), 256, 0, st>>>(a);
+      PRNN_HIP(hipGetLastError());
+      norm_sample_apply_kernel<T, V, false><<<grid, 256, 0, st>>>(a);
+    }
     PRNN_HIP(hipGetLastError());
     return static_cast<int>(PRNN_OK);
   });
@@ -892,7 +1012,7 @@ extern "C" PRNN_API int prnn_group_norm_backward(
   } else {
     parts = p.strips * N;
     part = static_cast<float*>(c.take(sizeof(float) * 2 * C * static_cast<size_t>(parts)));
-    part2 = static_cast<float*>(c.take(sizeof(float) * 2 * G * static_cast<size_t>(N)));
+    part2 = static_cast<float*>(c.take(sizeof(float) * 2 * G * static_cast<size_t>(parts)));
   }
   if (any && (!workspace || bytes < c.used))
     return fail(PRNN_ERR_VALUE, "group_norm backward: the workspace must hold %zu bytes", c.used);
@@ -935,12 +1055,18 @@ extern "C" PRNN_API int prnn_group_norm_backward(
       PRNN_HIP(hipGetLastError());
     } else if (any) {
       const dim3 grid(static_cast<unsigned>(p.strips) * N);
-      norm_sample_bwd_sums_kernel<T, V><<<grid, 256, 0, st>>>(a);
-      PRNN_HIP(hipGetLastError());
-      const unsigned joins = static_cast<unsigned>((1ll * N * G + 3) / 4);
-      norm_sample_means_kernel<T><<<joins, 256, 0, st>>>(a);
-      PRNN_HIP(hipGetLastError());
-      norm_sample_dx_kernel<T, V><<<grid, 256, 0, st>>>(a);
+      if (G <= kJoinGroups && C / V <= 256) {
+        norm_sample_bwd_sums_kernel<T, V, true><<<grid, 256, 0, st>>>(a);
+        PRNN_HIP(hipGetLastError());
+        norm_sample_dx_kernel<T, V, true><<<grid, 256, 0, st>>>(a);
+      } else {
+        norm_sample_bwd_sums_kernel<T, V, false><<<grid, 256, 0, st>>>(a);
+        PRNN_HIP(hipGetLastError());
+        norm_sample_means_kernel<T>
+            <<<static_cast<unsigned>((1ll * N * G + 3) / 4), 256, 0, st>>>(a);
+        PRNN_HIP(hipGetLastError());
+        norm_sample_dx_kernel<T, V, false><<<grid, 256, 0, st>>>(a);
+      }
       PRNN_HIP(hipGetLastError());
     }
     if (dw || db) {

@@ -102,7 +102,10 @@ def group_norm(x: Tensor, num_groups: int, weight: Tensor | None = None,
     ``over``: ``"token"`` or ``"sample"`` (``x`` ``(N, ..., C)``).  Differentiable in all tensors.
     """
     what = "group_norm"
-    _validate(what, x, gate)
+    # the quick look first: calls of small sizes are bound by the host
+    if not (x.is_cuda and x.dtype in _DTYPES
+            and (gate is None or (gate.dtype is x.dtype and gate.device == x.device))):
+        _validate(what, x, gate)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"{what}: x must be (..., C), got {tuple(x.shape)}")
     c = x.shape[-1]
