@@ -104,7 +104,7 @@ __device__ __forceinline__ float scan_up(float v) {
 }
 
 template <int KD, int W, bool STATE_ONLY, bool FINE>
-__global__ __launch_bounds__(64 * W, (KD >= 256 || (W < 4 && KD >= 128)) ? 1 : 2)
+__global__ __launch_bounds__(64 * W, (KD >= 256 || (W < 4 && KD >= 128) || (W == 1 && KD >= 64)) ? 1 : 2)
 void la_walk_bf16_kernel(LaParams P) {
   constexpr int NT = 64 * W, VT = 32 * W;
   constexpr int UX = KD / 8, UZ = VT / 8;      // 16-byte units of a row

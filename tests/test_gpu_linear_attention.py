@@ -357,3 +357,54 @@ def test_no_tokens_no_rows():
     assert linear_attention_step(empty, empty, empty, empty[..., 0], state).shape == (0, 2, 8)
     out = linear_attention(empty[:, None], empty[:, None], empty[:, None], empty[:, None, :, 0])
     assert out.shape == (0, 1, 2, 8)
+
+
+def test_offsets_beyond_32_bits():
+    """A pool and arrays of more than 2^32 bytes: the last slots and tokens are right."""
+    from pararnn_amd import linear_attention, linear_attention_step
+
+    slots, H, D = 17000, 4, 128  # 256 KiB a slot, 4.15 GiB
+    pool = torch.empty(slots, H, D, D, device=DEV)
+    table = torch.tensor([slots - 1, 3, 16385], dtype=torch.int32, device=DEV)
+    q, k, v, g, h0, _, _ = _inputs(3, 1, (H, H, H), D, D, BF16, "token", 5)
+    pool[table.long()] = h0.to(DEV)
+    out = linear_attention_step(*(x[:, 0].to(DEV) for x in (q, k, v, g)), pool, block_table=table)
+    o64, s64 = O.linear_attention(*(x.double() for x in (q, k, v, g)), h0.double())
+    assert _rel(out, o64[:, 0]) <= TOL[BF16] and _rel(pool[table.long()], s64) <= TOL[F32]
+    del pool
+    T, H = (1 << 20) + 70, 33  # 2^31 and more elements of q and out
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    q = torch.randn(1, T, H, 64, device=DEV, dtype=BF16, generator=gen)
+    k, v = (torch.randn(1, T, 1, 64, device=DEV, dtype=BF16, generator=gen) for _ in range(2))
+    g = torch.full((1, T, H), -0.1, device=DEV, dtype=BF16)
+    g[:, T - 100] = float("-inf")  # what follows stands on its own
+    with torch.no_grad():
+        out = linear_attention(q, k, v, g)
+        tail = [x[:, T - 100:].cpu().double() for x in (q, k, v, g)]
+    o64, _ = O.linear_attention(*tail)
+    assert _rel(out[:, T - 100:], o64) <= TOL[BF16]
+
+
+def test_shared_decay_and_lone_strides():
+    """A decay expanded over batch and time has the gradient of an expanded tensor; one token whose
+    strides are odd; keys expanded over time."""
+    from pararnn_amd import linear_attention
+
+    for dtype in (F32, BF16):
+        q, k, v, _, _, go, _ = (t.to(DEV) for t in _inputs(2, 70, (2, 2, 2), 64, 64, dtype, "token", 3))
+        head = torch.tensor([-0.1, -0.02], device=DEV, dtype=dtype).requires_grad_(True)
+        got = torch.autograd.grad(linear_attention(q, k, v, head.expand(2, 70, 2)), head, go)[0]
+        leaf = head.detach().double().cpu().requires_grad_(True)
+        o64, _ = O.linear_attention(*(x.double().cpu() for x in (q, k, v)), leaf)
+        want = torch.autograd.grad(o64, leaf, go.double().cpu())[0]
+        # summed over the batch in its own type by autograd: one rounding more in 16 bits
+        assert _rel(got, want) <= (TOL_G[dtype] if dtype == F32 else 2 * TOL_G[dtype])
+        with torch.no_grad():
+            one = torch.randn(2, 3, 2, 64, device=DEV).to(dtype)[:, 1:2]
+            a = linear_attention(one, one, one, head)
+            b = linear_attention(*(one.contiguous(),) * 3, head)
+            assert torch.equal(a, b)
+            wide = k[:, :1].expand(2, 70, 2, 64)
+            assert torch.equal(linear_attention(q, wide, v, head),
+                               linear_attention(q, wide.contiguous(), v, head))
+

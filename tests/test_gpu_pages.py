@@ -177,3 +177,23 @@ def test_a_serving_step_in_a_graph():
         assert sorted(table.tolist()) == list(range(n))
         assert torch.equal(pool[table.long()], want_pool)
         torch.cuda.synchronize()
+
+
+def test_slots_beyond_32_bits():
+    """Pools of more than 2^32 bytes: slots at the far end move and are copied like others."""
+    from pararnn_amd import compact_pages, copy_pages, fork_pages
+
+    slots, n = 4200, 1 << 18  # 1 MiB a slot, 4.1 GiB
+    pool = torch.empty(slots, n, device=DEV)
+    used = torch.zeros(slots, dtype=torch.int32, device=DEV)
+    live = torch.tensor([1, 4097, 4199], device=DEV)
+    used[live] = 1
+    pool[live] = torch.arange(3.0, device=DEV)[:, None] + torch.rand(n, device=DEV)
+    want = pool[live].clone()
+    copy_pages(pool, live[2:], torch.tensor([4198]))
+    assert torch.equal(pool[4198], want[2])
+    table = live.to(torch.int32)
+    assert fork_pages(used, pool, table[2:]).tolist() == [0]
+    assert torch.equal(pool[0], want[2])
+    assert int(compact_pages(used, pool, [table])) == 4
+    assert table.tolist() == [1, 2, 3] and torch.equal(pool[1:4], want)
