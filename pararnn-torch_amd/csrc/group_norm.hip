@@ -371,7 +371,9 @@ __global__ __launch_bounds__(1024) void norm_param_kernel(const float* __restric
 // A sample (L tokens) is cut into strips of rows, one workgroup each.  Threads lie over the
 // channels, V to a thread, and over as many rows at a time as fit.
 
-constexpr int kJoinGroups = 64;  // groups of a sample whose sums every workgroup forms itself
+// Groups of a sample whose sums every workgroup forms itself.  A training step of 8 x 2047 tokens of
+// 256 fp32 channels: 48 us against 51 with launches of their own for 32 groups, 61 against 56 for 64.
+constexpr int kJoinGroups = 32;
 constexpr int kRows = 4;         // rows of a thread under way at a time
 
 struct SamplePlace {

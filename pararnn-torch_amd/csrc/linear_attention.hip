@@ -290,27 +290,6 @@ int check(const Problem* a) {
 
 int sequences(const Problem& a) { return a.cu_seqlens ? a.n_seq : a.B; }
 
-// How long the pieces are.  Walks of whole sequences read every array once; cut ones read k
-// and v once more and move a state a piece, so a sequence is cut only as far as the chip has
-// workgroups to spare (about kLaTarget run at a time), and never below kLaLeast tokens.
-constexpr int kLaTarget = 1536, kLaLeast = 256, kLaLeastF32 = 128;
-
-LaSeqs cut(const Problem& a, bool bf16, int tiles_and_roles) {
-  LaSeqs s{a.cu_seqlens, sequences(a), a.T, 1, 0};
-  const long long work = 1ll * a.B * a.T * a.H * tiles_and_roles;
-  long long len = (work + kLaTarget - 1) / kLaTarget;
-  len = std::max<long long>(bf16 ? kLaLeast : kLaLeastF32, (len + 63) / 64 * 64);
-  if (len >= a.T) {
-    s.len = a.T + 1;  // every sequence whole
-    s.pieces = s.n_seq;
-  } else {
-    s.len = static_cast<int>(len);
-    s.pieces = a.cu_seqlens ? s.n_seq + a.T / s.len
-                            : a.B * ((a.T + s.len - 1) / s.len);
-  }
-  return s;
-}
-
 bool is_cut(const LaSeqs& s) { return s.len <= s.T; }
 
 LaDecay decay_of(const Problem& a) { return LaDecay{a.g, a.g_sb, a.g_st, a.g_sh, a.g_dtype}; }
@@ -327,7 +306,9 @@ struct Scratch {
 };
 
 // Whether the walks run on the bf16 matrix instructions: bf16 storage whose widths and rows admit
-// 16-byte accesses.  What is odd takes the fp32 walk, about a third as fast at width 64.
+// 16-byte accesses.  What is odd takes the fp32 walk: 8 x 2048 tokens of 16 heads of (64, 64) 62 us
+// on bf16 instructions and 140 in fp32, a training step 245 and 472, 4 x 2048 of (128, 128) 77 and
+// 223, of (32, 32) 42 and 65.
 bool on_bf16(const Problem& a, const prnn_la_view* other) {
   if (a.dtype != PRNN_BF16 || a.Dk % 8 || a.Dv % 8) return false;
   return view(a.q, a, a.Dk).vec && view(a.k, a, a.Dk).vec && view(a.v, a, a.Dv).vec &&
@@ -345,9 +326,52 @@ struct Walks {
   }
 };
 
-LaSeqs forward_cut(const Problem& a, const Walks& w) { return cut(a, w.bf16, w.tiles(a.Dv)); }
+// How long the pieces are, a multiple of 64 tokens.  Time in microseconds, measured on single
+// sequences of 2048 and 8192 tokens in pieces of 64 .. 1024:
+// * a piece's tokens come one after another, twice (its own contribution, then the walk): 0.085 a
+//   token on bf16 instructions, 0.17 in fp32; two thirds of that for a sequence that is not cut;
+// * the join takes a sequence's pieces one after another: 0.12 a piece;
+// * a state per piece and direction is written, read, written and read: 16 bytes an element at
+//   5.3 MB per us;
+// * two launches more than without a cut: 8.
+// So pieces are as long as makes the first equal to what falls with their length, unless the
+// chip has workgroups enough with longer ones: about 8 waves a CU on bf16 instructions, 16 in
+// fp32, run at a time.  Lengths of 64, 256 and 1024 and this rule's, us, heads of (64, 64) in bf16:
+// 2 x 512 tokens of 4 heads 19, 33, 31 and 19; 2048 of 4 heads 23, 33, 92 and 23, their training
+// step 60, 81, 218 and 60; 16384 of 8 heads 86, 55, 97 and 53, their training step 285, 206, 288
+// and 198; 8 x 2048 of 16 heads 97, 65, 99 and 64; 32 x 300 of 4 heads 29, 36, 23 and 23 (whole).
+LaSeqs cut(const Problem& a, const Walks& w, int widest, int roles, int states) {
+  LaSeqs s{a.cu_seqlens, sequences(a), a.T, 1, 0};
+  const double serial = w.bf16 ? 0.085 : 0.17, per_piece = 0.12, bytes_us = 5.3e6, launches = 8.0;
+  const double tokens = 1.0 * a.B * a.T;
+  // packed sequences' lengths are not known here: some are twice the mean
+  const double longest = a.cu_seqlens ? std::min(tokens, 2.0 * tokens / std::max(1, a.n_seq)) : a.T;
+  const double falls = per_piece * longest + 16.0 * states * a.Dk * a.Dv * a.H * tokens / bytes_us;
+  long long len = std::max(1ll, std::llround(std::sqrt(falls / serial) / 64)) * 64;
+  if (serial * longest * 2 / 3 <= serial * len + falls / len + launches) len = 1ll + a.T;
+  const long long waves = w.cols(widest) / (w.bf16 ? 32 : 16);
+  const long long most = (w.bf16 ? 2048 : 4096) / waves;  // workgroups that run at a time
+  const long long fill = (1ll * a.B * a.T * a.H * roles * w.tiles(widest) + most - 1) / most;
+  if (len < fill) {
+    // a batch's sequences in equal pieces, no more than run at a time
+    const long long n = a.cu_seqlens ? 1 : std::max(1ll, a.T / fill);
+    len = std::max(fill, a.cu_seqlens ? 0ll : (a.T + n - 1) / n);
+    len = (len + 63) / 64 * 64;
+  }
+  if (len >= a.T) {
+    s.len = a.T + 1;  // every sequence whole
+    s.pieces = s.n_seq;
+  } else {
+    s.len = static_cast<int>(len);
+    s.pieces = a.cu_seqlens ? s.n_seq + a.T / s.len
+                            : a.B * ((a.T + s.len - 1) / s.len);
+  }
+  return s;
+}
+
+LaSeqs forward_cut(const Problem& a, const Walks& w) { return cut(a, w, a.Dv, 1, 1); }
 LaSeqs backward_cut(const Problem& a, const Walks& w) {
-  return cut(a, w.bf16, 3 * w.tiles(std::max(a.Dk, a.Dv)));
+  return cut(a, w, std::max(a.Dk, a.Dv), 3, 2);
 }
 
 Scratch carve(void* ws, const Problem& a, const Walks& w, bool backward, bool decay_grad) {
