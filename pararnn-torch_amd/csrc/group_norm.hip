@@ -898,6 +898,13 @@ int check(const char* what, int N, int L, int C, int G, int act, int w_dtype, in
   return PRNN_OK;
 }
 
+// The launches of statistics per sample.
+int check_strips(const Plan& p, int N, int G) {
+  if (p.token) return PRNN_OK;
+  if (int rc = check_grid("group_norm", 1ll * p.strips * N, 256)) return rc;
+  return check_grid("group_norm", (1ll * N * G + 3) / 4, 256);
+}
+
 uintptr_t bits_of(std::initializer_list<const void*> ps) {
   uintptr_t b = 0;
   for (const void* p : ps) b |= reinterpret_cast<uintptr_t>(p);
@@ -938,6 +945,7 @@ extern "C" PRNN_API int prnn_group_norm(const void* x, const void* w, const void
   if (N == 0 || L == 0) return PRNN_OK;
   if (!x || !y) return fail(PRNN_ERR_VALUE, "group_norm: x and y must be non-null");
   const Plan p = plan(N, L, C / G, G, dtype, bits_of({x, y, gate}), false);
+  if (int rc = check_strips(p, N, G)) return rc;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   NormArgs a{};
   a.x = x;
@@ -1005,6 +1013,7 @@ extern "C" PRNN_API int prnn_group_norm_backward(
     return fail(PRNN_ERR_VALUE, "group_norm backward: gy, x, dx (and dgate) must be non-null");
   const Plan p = plan(std::max(N, 1), std::max(L, 1), C / G, G, dtype,
                       bits_of({gy, x, gate, dx, dgate}), true);
+  if (int rc = check_strips(p, N, G)) return rc;
   Carver c(workspace);
   float *part, *part2 = nullptr;
   int parts;

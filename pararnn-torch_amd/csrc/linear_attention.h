@@ -264,9 +264,9 @@ __device__ __forceinline__ LaPlace la_place(const LaParams& p) {
   r.any = r.piece < p.seqs.pieces;
   return r;
 }
-inline unsigned la_grid(const LaParams& p) {
+inline long long la_grid(const LaParams& p) {
   const long long items = 1ll * p.seqs.pieces * (p.H / p.near);
-  return static_cast<unsigned>((items + 7) / 8 * 8 * p.roles * p.tiles * p.near);
+  return (items + 7) / 8 * 8 * p.roles * p.tiles * p.near;
 }
 
 inline int la_widest(const LaParams& p, int roles) {

@@ -429,6 +429,7 @@ int join(const LaParams& p, const Scratch& s, const LaState* init, const int* re
   }
   const bool vec = j.DD % 4 == 0;
   const int blocks = (j.DD / (vec ? 4 : 1) + 255) / 256;
+  if (int rc = check_grid("linear_attention", 1ll * p.seqs.n_seq * blocks, 256)) return rc;
   const dim3 grid(static_cast<unsigned>(p.seqs.n_seq) * blocks, p.H, roles);
   if (vec)
     la_join_kernel<4><<<grid, 256, 0, st>>>(j, blocks);
@@ -597,6 +598,7 @@ int backward(const Problem& a, const prnn_la_view& go, const float* gs, void* dq
     const bool per_head = a.g_sb == 0 && a.g_st == 0;
     d.dg = per_head ? nullptr : dg;
     d.per_part = per_head ? s.per_part : nullptr;
+    if (int rc = check_grid("linear_attention", d.seqs.pieces, 256)) return rc;
     const dim3 grid(d.seqs.pieces, a.H);
     la_decay_grad_kernel<<<grid, 256, 0, st>>>(d);
     PRNN_HIP(hipGetLastError());

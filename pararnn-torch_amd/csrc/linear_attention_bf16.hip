@@ -524,7 +524,9 @@ void la_walk_bf16_kernel(LaParams P) {
 
 template <int KD, int W>
 int launch(const LaParams& p, bool state_only, bool fine, hipStream_t stream) {
-  const unsigned grid = la_grid(p), block = 64 * W;
+  const int block = 64 * W;
+  if (int rc = check_grid("linear_attention", la_grid(p), block)) return rc;
+  const unsigned grid = la_grid(p);
   if (state_only)
     la_walk_bf16_kernel<KD, W, true, false><<<grid, block, 0, stream>>>(p);
   else if (fine)

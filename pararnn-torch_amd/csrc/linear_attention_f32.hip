@@ -415,7 +415,9 @@ __global__ __launch_bounds__(64 * W) void la_walk_f32_kernel(LaParams P) {
 
 template <typename T, int KT, int W, bool VEC>
 int launch(const LaParams& p, bool state_only, hipStream_t stream) {
-  const unsigned grid = la_grid(p), block = 64 * W;
+  const int block = 64 * W;
+  if (int rc = check_grid("linear_attention", la_grid(p), block)) return rc;
+  const unsigned grid = la_grid(p);
   if (state_only)
     la_walk_f32_kernel<T, KT, W, VEC, true><<<grid, block, 0, stream>>>(p);
   else

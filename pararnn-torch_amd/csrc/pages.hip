@@ -250,8 +250,9 @@ int copy(const prnn_pool* pools, int n_pools, int slots, const int* src, const i
     const Pools P = some_pools(pools, n_pools, first);
     if (P.n == 0) continue;
     const long long per = P.parts[P.n - 1];
-    // a launch holds fewer than 2^31 workgroups
-    const int most = static_cast<int>(std::min<long long>(n, ((1ll << 31) - 1) / per));
+    // a launch holds fewer than 2^32 threads
+    if (int rc = check_grid("copy of pages", per, 256)) return rc;
+    const int most = static_cast<int>(std::min<long long>(n, 0xffffffffll / 256 / per));
     for (int i = 0; i < n; i += most) {
       const int m = std::min(most, n - i);
       pages_copy_kernel<<<static_cast<unsigned>(m * per), 256, 0, st>>>(P, slots, src + i, dst + i,

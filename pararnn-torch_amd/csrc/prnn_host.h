@@ -50,6 +50,14 @@ inline int hip_fail(hipError_t e, const char* what) {
     if (e_ != hipSuccess) return prnn::hip_fail(e_, #call); \
   } while (0)
 
+// A launch's threads along a dimension are counted in 32 bits.
+inline int check_grid(const char* what, long long groups, int block) {
+  if (groups * block > 0xffffffffll)
+    return fail(PRNN_ERR_VALUE, "%s: %lld workgroups of %d threads are too many for a launch", what,
+                groups, block);
+  return PRNN_OK;
+}
+
 // Bump allocator over the caller's workspace; every block 256-byte aligned.
 struct Carver {
   char* base;

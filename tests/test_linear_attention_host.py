@@ -74,3 +74,29 @@ def test_c_entries_refuse_before_any_device_work():
                                0, None) == _lib.PRNN_ERR_VALUE
     assert lib.prnn_pages_take(None, 4, None, 1, None) == _lib.PRNN_ERR_VALUE
     assert lib.prnn_pages_take(None, -1, None, 1, None) == _lib.PRNN_ERR_VALUE
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="made-up addresses: without a device only")
+def test_c_entries_refuse_grids_that_pass_32_bits():
+    import ctypes
+    import os
+
+    from pararnn_amd import _lib
+
+    if not os.path.exists(_lib.lib_path()):
+        pytest.skip("library not built")
+    lib = _lib.load()
+    view = _lib.LaView(256, 8, 8, 8, 64)
+    # 2^20 single tokens of 64 heads: 2^26 workgroups of 64 threads at least
+    p = _lib.LaProblem(view, view, view, 256, 64, 64, 1, None, None, None, 0, 0, 1 << 20, 1, 64, 8,
+                       8, 0, 0, 1.0)
+    args = (ctypes.byref(p), ctypes.byref(view), None, None, 0, None, 0, None)
+    assert lib.prnn_linear_attention(*args) == _lib.PRNN_ERR_VALUE
+    assert b"too many for a launch" in lib.prnn_last_error()
+    for n, groups in ((1 << 24, 1), (1 << 20, 64)):
+        rc = lib.prnn_group_norm(256, None, None, None, 256, None, n, 2, 64, groups, 1e-5, 0, 0, 0,
+                                 256, 1 << 40, None)
+        assert rc == _lib.PRNN_ERR_VALUE and b"too many for a launch" in lib.prnn_last_error()
+    pool = (_lib.Pool * 1)(_lib.Pool(256, 1 << 39))
+    rc = lib.prnn_pages_copy(1, pool, 1, 256, 256, 1, None)
+    assert rc == _lib.PRNN_ERR_VALUE and b"too many for a launch" in lib.prnn_last_error()
