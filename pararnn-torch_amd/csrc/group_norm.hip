@@ -165,6 +165,8 @@ __device__ __forceinline__ TokenPlace token_place(const NormArgs& A) {
   return p;
 }
 
+// 16384 tokens of 1024 bf16 channels in 16 groups with a gate: 20.3 us, 4.96 TB/s (a large copy:
+// 5.14); 32 tokens 4.0 us, a launch's own time.
 template <typename T, int V, int K>
 __global__ __launch_bounds__(256) void norm_token_kernel(NormArgs A) {
   const TokenPlace p = token_place(A);
@@ -224,7 +226,8 @@ __global__ __launch_bounds__(256) void norm_token_kernel(NormArgs A) {
   }
 }
 
-// part: [gridDim.x][2][C] sums of dz h and dz.
+// part: [gridDim.x][2][C] sums of dz h and dz.  The same 16384 tokens: 38.4 us, 4.4 TB/s, and 4.1 us
+// for the parameters' sums.
 template <typename T, int V, int K>
 __global__ __launch_bounds__(256) void norm_token_bwd_kernel(NormArgs A) {
   __shared__ float red[256];
@@ -336,7 +339,7 @@ __global__ __launch_bounds__(256) void norm_token_bwd_kernel(NormArgs A) {
 }
 
 // dw and db from partial sums [parts][2][C]: 32 channels a workgroup, 32 lanes to a channel, each
-// with 8 loads under way.
+// with 8 loads under way.  A thousand partial sums of 1024 channels: 4.1 us, 8 MB.
 template <typename T>
 __global__ __launch_bounds__(1024) void norm_param_kernel(const float* __restrict__ part, int parts,
                                                           int C, void* dw, void* db, int f32) {
@@ -369,10 +372,15 @@ __global__ __launch_bounds__(1024) void norm_param_kernel(const float* __restric
 
 // ---- statistics per sample ---------------------------------------------------------------
 // A sample (L tokens) is cut into strips of rows, one workgroup each.  Threads lie over the
-// channels, V to a thread, and over as many rows at a time as fit.
+// channels, V to a thread, and over as many rows at a time as fit.  8 x 2047 tokens of 256 fp32
+// channels in 32 groups (16.8 MB an array): statistics 7.7 us, y 9.2, sums 9.9, dx 14.1,
+// parameters 4.0: each a few dependent rounds of rows behind a launch, 2.2 to 3.6 TB/s.  Samples of
+// 16384 tokens: 35 for the statistics (one array), y 45 (two), sums 54 (two), dx 68 (three), 3.9 to
+// 6.0 TB/s with what the last-level cache still holds.
 
 // Groups of a sample whose sums every workgroup forms itself.  A training step of 8 x 2047 tokens of
-// 256 fp32 channels: 48 us against 51 with launches of their own for 32 groups, 61 against 56 for 64.
+// 256 fp32 channels: 42 us against 45 with launches of their own for 32 groups, 40 against 48 for 16, and with 64 groups
+// (before both got faster) 61 against 56.
 constexpr int kJoinGroups = 32;
 constexpr int kRows = 4;         // rows of a thread under way at a time
 
@@ -406,6 +414,13 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
   __syncthreads();
   return red[0] + red[1] + red[2] + red[3];
+}
+
+// Lanes of a sum over `items` values: a power of two.
+__device__ __forceinline__ int lanes_for(int items) {
+  int lanes = 1;
+  while (lanes < 64 && lanes < items) lanes <<= 1;
+  return lanes;
 }
 
 // Statistics of strip `strip` of sample n, one group after another of those in the workgroup's
@@ -460,13 +475,14 @@ __global__ __launch_bounds__(256) void norm_sample_stats_kernel(NormArgs A) {
     for (int i = 0; i < V; ++i) mean[i] = m2[i] = 0.0f;
     float cnt = 0.0f;
     if (on)
-      for (int l = l0 + p.row; l < l1; l += kRows * p.rows_per) {
-        float v[kRows][V];
+      for (int l = l0 + p.row; l < l1; l += 2 * kRows * p.rows_per) {
+        // one array alone: twice the rows for as many bytes under way
+        float v[2 * kRows][V];
 #pragma unroll
-        for (int k = 0; k < kRows; ++k)
+        for (int k = 0; k < 2 * kRows; ++k)
           loadv<T, V>(x + static_cast<size_t>(min(l + k * p.rows_per, l1 - 1)) * A.C + slot * V, v[k]);
 #pragma unroll
-        for (int k = 0; k < kRows; ++k) {
+        for (int k = 0; k < 2 * kRows; ++k) {
           if (l + k * p.rows_per >= l1) break;
           cnt += 1.0f;
           const float inv = frcp(cnt);
@@ -485,24 +501,24 @@ __global__ __launch_bounds__(256) void norm_sample_stats_kernel(NormArgs A) {
       lds[threadIdx.x * 2 * V + 2 * i + 1] = m2[i];
     }
     __syncthreads();
-    // one wave per group: the mean of the means, then the deviations from it
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int g = wave; g < gn; g += 4) {
-      const int items = per_group * p.rows_per;
+    // some lanes per group: the mean of the means, then the deviations from it
+    const int items = per_group * p.rows_per, lanes = lanes_for(items);
+    const int lane = threadIdx.x & (lanes - 1);
+    const float total = static_cast<float>(l1 - l0) * A.Cg;
+    for (int at = 0; at < gn; at += 256 / lanes) {
+      const int g = at + threadIdx.x / lanes, n_items = g < gn ? items : 0;
       float s = 0.0f;
-      const float total = static_cast<float>(l1 - l0) * A.Cg;
-      for (int it = lane; it < items; it += 64) {
+      for (int it = lane; it < n_items; it += lanes) {
         const int r = it / per_group, u = g * per_group + it - r * per_group;
         const float c = static_cast<float>((l1 - l0 - r + p.rows_per - 1) / p.rows_per);
         const float* e = &lds[(r * (p.slots <= 256 ? p.slots : 0) + u) * 2 * V];
 #pragma unroll
         for (int i = 0; i < V; ++i) s = fmaf(c, e[2 * i], s);
       }
-#pragma unroll
-      for (int k = 1; k < 64; k <<= 1) s += __shfl_xor(s, k);
+      for (int k = 1; k < lanes; k <<= 1) s += __shfl_xor(s, k);
       const float gm = s / total;
       s = 0.0f;
-      for (int it = lane; it < items; it += 64) {
+      for (int it = lane; it < n_items; it += lanes) {
         const int r = it / per_group, u = g * per_group + it - r * per_group;
         const float c = static_cast<float>((l1 - l0 - r + p.rows_per - 1) / p.rows_per);
         const float* e = &lds[(r * (p.slots <= 256 ? p.slots : 0) + u) * 2 * V];
@@ -512,9 +528,8 @@ __global__ __launch_bounds__(256) void norm_sample_stats_kernel(NormArgs A) {
           s += fmaf(c * d, d, e[2 * i + 1]);
         }
       }
-#pragma unroll
-      for (int k = 1; k < 64; k <<= 1) s += __shfl_xor(s, k);
-      if (lane == 0) {
+      for (int k = 1; k < lanes; k <<= 1) s += __shfl_xor(s, k);
+      if (lane == 0 && g < gn) {
         out[2 * (g0 + g)] = gm;
         out[2 * (g0 + g) + 1] = s;
       }
@@ -637,7 +652,7 @@ __global__ __launch_bounds__(256) void norm_sample_apply_kernel(NormArgs A) {
 // [N * strips][2][G].
 template <typename T, int V, bool JOIN>
 __global__ __launch_bounds__(256) void norm_sample_bwd_sums_kernel(NormArgs A) {
-  __shared__ float red[256];
+  __shared__ float red[2 * V][256];
   __shared__ float s_ch[JOIN ? 2 * 256 * V : 2];
   const int n = blockIdx.x / A.strips, strip = blockIdx.x - n * A.strips;
   const SamplePlace p = sample_place<V>(A);
@@ -688,62 +703,97 @@ __global__ __launch_bounds__(256) void norm_sample_bwd_sums_kernel(NormArgs A) {
           if (A.gate) storev<T, V>(static_cast<T*>(A.dgate) + at, gt);
         }
       }
+    if (p.rows_per > 1) {  // all slots at once: one round
 #pragma unroll
-    for (int i = 0; i < V; ++i)
+      for (int i = 0; i < V; ++i) {
+        red[i][threadIdx.x] = dw[i];
+        red[V + i][threadIdx.x] = db[i];
+      }
+      __syncthreads();
+      if (p.row == 0)
+        for (int r = 1; r < p.rows_per; ++r)
 #pragma unroll
-      for (int which = 0; which < 2; ++which) {
-        const float mine = which ? db[i] : dw[i];
-        float sum = mine;
-        if (p.rows_per > 1) {
-          __syncthreads();
-          red[threadIdx.x] = mine;
-          __syncthreads();
-          if (p.row == 0)
-            for (int r = 1; r < p.rows_per; ++r) sum += red[r * p.slots + threadIdx.x];
-        }
-        if (p.row == 0 && on) {
-          out[which * A.C + c + i] = sum;
-          if (JOIN) s_ch[which * 256 * V + c + i] = w[i] * sum;
+          for (int i = 0; i < V; ++i) {
+            dw[i] += red[i][r * p.slots + threadIdx.x];
+            db[i] += red[V + i][r * p.slots + threadIdx.x];
+          }
+    }
+    if (p.row == 0 && on)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        out[c + i] = dw[i];
+        out[A.C + c + i] = db[i];
+        if (JOIN) {
+          s_ch[c + i] = w[i] * dw[i];
+          s_ch[256 * V + c + i] = w[i] * db[i];
         }
       }
     if (JOIN) {
       __syncthreads();
-      for (int k = threadIdx.x; k < 2 * A.G; k += 256) {
-        const int which = k / A.G, gg = k - which * A.G;
-        const float* e = &s_ch[which * 256 * V + gg * A.Cg];
+      const int lanes = lanes_for(A.Cg), lane = threadIdx.x & (lanes - 1);
+      for (int at = 0; at < 2 * A.G; at += 256 / lanes) {
+        const int k = at + threadIdx.x / lanes, which = k / A.G, gg = k - which * A.G;
         float sum = 0.0f;
-        for (int i = 0; i < A.Cg; ++i) sum += e[i];
-        A.part2[(static_cast<size_t>(n) * A.strips + strip) * 2 * A.G + k] = sum;
+        if (k < 2 * A.G)
+          for (int i = lane; i < A.Cg; i += lanes) sum += s_ch[which * 256 * V + gg * A.Cg + i];
+        for (int s = 1; s < lanes; s <<= 1) sum += __shfl_xor(sum, s);
+        if (k < 2 * A.G && lane == 0)
+          A.part2[(static_cast<size_t>(n) * A.strips + strip) * 2 * A.G + k] = sum;
       }
     }
   }
 }
 
-// m1 and m2 per (sample, group): part2 [N][G][2], one wave each.
+// m1 and m2 of a (sample, group), part2 [N][G][2], from the strips' sums per channel: lanes over
+// the group's channels and as many strips at a time as fit, 4 of them under way.
 template <typename T>
-__global__ __launch_bounds__(256) void norm_sample_means_kernel(NormArgs A) {
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const long long id = static_cast<long long>(blockIdx.x) * 4 + wave;
-  if (id >= static_cast<long long>(A.N) * A.G) return;
-  const int n = static_cast<int>(id / A.G), g = static_cast<int>(id - static_cast<long long>(n) * A.G);
+__global__ __launch_bounds__(1024) void norm_sample_means_kernel(NormArgs A) {
+  __shared__ double red[2][16];
+  const int id = blockIdx.x, n = id / A.G, g = id - n * A.G;
   const float* e = A.part + static_cast<size_t>(n) * A.strips * 2 * A.C + g * A.Cg;
+  int lanes = 1;
+  while (lanes < static_cast<int>(blockDim.x) && lanes < A.Cg) lanes <<= 1;
+  const int k0 = threadIdx.x / lanes, step = blockDim.x / lanes;
   double m1 = 0.0, m2 = 0.0;
-  const long long items = static_cast<long long>(A.strips) * A.Cg;
-  for (long long it = lane; it < items; it += 64) {
-    const int k = static_cast<int>(it / A.Cg), c = static_cast<int>(it - static_cast<long long>(k) * A.Cg);
+  for (int c = threadIdx.x - k0 * lanes; c < A.Cg; c += lanes) {
     const float w = param<T>(A.w, A.w_f32, g * A.Cg + c, 1.0f);
-    m2 += static_cast<double>(w) * e[static_cast<size_t>(k) * 2 * A.C + c];
-    m1 += static_cast<double>(w) * e[static_cast<size_t>(k) * 2 * A.C + A.C + c];
+    double s1 = 0.0, s2 = 0.0;
+    for (int k = k0; k < A.strips; k += 4 * step) {
+      float a[4], b[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int kk = min(k + i * step, A.strips - 1);
+        a[i] = e[static_cast<size_t>(kk) * 2 * A.C + c];
+        b[i] = e[static_cast<size_t>(kk) * 2 * A.C + A.C + c];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (k + i * step < A.strips) {
+          s2 += a[i];
+          s1 += b[i];
+        }
+    }
+    m2 += w * s2;
+    m1 += w * s1;
   }
 #pragma unroll
   for (int k = 1; k < 64; k <<= 1) {
     m1 += __shfl_xor(m1, k);
     m2 += __shfl_xor(m2, k);
   }
-  if (lane == 0) {
+  if ((threadIdx.x & 63) == 0) {
+    red[0][threadIdx.x >> 6] = m1;
+    red[1][threadIdx.x >> 6] = m2;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int k = 1; k < static_cast<int>(blockDim.x) / 64; ++k) {
+      m1 += red[0][k];
+      m2 += red[1][k];
+    }
     const double inv = 1.0 / (static_cast<double>(A.L) * A.Cg);
-    A.part2[2 * id] = static_cast<float>(m1 * inv);
-    A.part2[2 * id + 1] = static_cast<float>(m2 * inv);
+    A.part2[2 * static_cast<size_t>(id)] = static_cast<float>(m1 * inv);
+    A.part2[2 * static_cast<size_t>(id) + 1] = static_cast<float>(m2 * inv);
   }
 }
 
@@ -852,12 +902,14 @@ Plan plan(int N, int L, int Cg, int G, int dtype, uintptr_t bits, bool backward)
     p.blocks_y = (per_row + 255) / 256;
     const int need = (N + rows_per - 1) / rows_per;
     // A workgroup reads its parameters once (backward: keeps their sums) and goes on from row to
-    // row: about eight a CU forward, four backward, where a partial sum each is written.
+    // row: about eight a CU forward, four backward, where a partial sum each is written.  A training
+    // step of 16384 tokens of 1024 channels: 63 us, with half as many 70, with twice as many 67.
     const int most = std::max(1, (backward ? 1024 : 2048) / p.blocks_y);
     p.blocks_x = std::max(1, std::min(need, most));
     return p;
   }
-  // strips: enough workgroups for the chip, each of at least kRows rounds of rows
+  // strips: enough workgroups for the chip, each of at least kRows rounds of rows.  512 of them:
+  // 42 us for a training step of 8 x 2047 tokens of 256 channels; 256: 45; 1024: 52.
   const int slots = G * Cg / p.V, rows_per = slots <= 256 ? 256 / slots : 1;
   const int want = std::max(1, 512 / std::max(1, N));
   p.strip_rows = std::max((L + want - 1) / want, kRows * rows_per);
@@ -902,7 +954,7 @@ int check(const char* what, int N, int L, int C, int G, int act, int w_dtype, in
 int check_strips(const Plan& p, int N, int G) {
   if (p.token) return PRNN_OK;
   if (int rc = check_grid("group_norm", 1ll * p.strips * N, 256)) return rc;
-  return check_grid("group_norm", (1ll * N * G + 3) / 4, 256);
+  return check_grid("group_norm", 1ll * N * G, 64);  // (sample, group): a wave at least
 }
 
 uintptr_t bits_of(std::initializer_list<const void*> ps) {
@@ -1073,8 +1125,12 @@ extern "C" PRNN_API int prnn_group_norm_backward(
       } else {
         norm_sample_bwd_sums_kernel<T, V, false><<<grid, 256, 0, st>>>(a);
         PRNN_HIP(hipGetLastError());
-        norm_sample_means_kernel<T>
-            <<<static_cast<unsigned>((1ll * N * G + 3) / 4), 256, 0, st>>>(a);
+        // A thread per 16 sums.  8 samples of one group of 2048 channels, 131072 sums each: 26 us;
+        // in 32 groups 4.8.  A wave each took some 140 us for one group of 256 channels.
+        int block = 64;
+        while (block < 1024 && block * 16ll < 1ll * p.strips * (C / G)) block *= 2;
+        if (int rc = check_grid("group_norm backward", 1ll * N * G, block)) return rc;
+        norm_sample_means_kernel<T><<<N * G, block, 0, st>>>(a);
         PRNN_HIP(hipGetLastError());
         norm_sample_dx_kernel<T, V, false><<<grid, 256, 0, st>>>(a);
       }

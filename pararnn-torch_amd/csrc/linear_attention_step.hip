@@ -3,7 +3,10 @@
 // Bound by the state's traffic (read once, written once: 8 bytes an element against 4 flops).
 // A workgroup takes TJ columns of one head's state: L lanes of four columns side by side, the
 // rows spread over 256 / L groups of lanes, so every access is 16 bytes a lane and a thread has
-// all its rows' loads in flight before the first is used.
+// U of its rows' loads in flight, and the next U's while these are worked on.
+//
+// 256 sessions of 16 heads of (128, 128) on a pool: 112 us, 4.8 TB/s (a large copy: 5.1); one
+// session of 8 heads of (64, 64): 4.5 us on the GPU, a launch's own time.
 #include "linear_attention.h"
 
 namespace prnn {
@@ -24,8 +27,7 @@ struct StepArgs {
   float scale;
 };
 
-// L lanes x 4 columns, U rows of a thread at a time; one row of the next U is under way while
-// these are worked on.  What lies outside the head is read as zero and not written (an offset
+// L lanes x 4 columns, U rows of a thread at a time.  What lies outside the head is read as zero and not written (an offset
 // outside the resource).
 template <typename T, int L, int U, bool VEC>
 __global__ __launch_bounds__(256) void la_step_kernel(StepArgs A) {
@@ -160,10 +162,13 @@ extern "C" PRNN_API int prnn_linear_attention_step(
   return with_storage(dtype, [&](auto z) {
     using T = decltype(z);
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    // whole rows of a head side by side where there are enough of them, narrow tiles (more
-    // workgroups) for few
-    if (Dv <= 32 || 1ll * B * H < 128) return launch<T, 8, 4>(a, B, vec, st);
-    if (Dv <= 64) return launch<T, 16, 4>(a, B, vec, st);
+    // Narrow tiles (more workgroups) for few heads, whole rows of a head side by side for many.
+    // Of 8, 16 and 32 lanes, us: (128, 128) 64 heads 4.4, 4.9, 6.2; 128 heads 5.1, 5.6, 6.8; 256
+    // heads 7.6, 7.0, 7.6; 512 heads 11.0, 9.9, 9.8; 4096 heads 93, 85, 81.  (64, 64) 8 heads 3.8,
+    // 3.8, 4.8; 512 heads 5.9, 5.0, 5.8; 4096 heads 29, 25, 30.  (32, 32) 4096 heads 13, 13, 20.
+    const long long heads = 1ll * B * H;
+    if (Dv <= 32 || heads <= 128) return launch<T, 8, 4>(a, B, vec, st);
+    if (Dv <= 64 || heads < 512) return launch<T, 16, 4>(a, B, vec, st);
     return launch<T, 32, 8>(a, B, vec, st);
   });
 }

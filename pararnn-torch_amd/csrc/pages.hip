@@ -2,8 +2,10 @@
 //
 // Which slot goes where is one workgroup's work: a running count over the `used` flags (4 a
 // thread, 4096 a round), so that the k-th wanted slot is the k-th lowest free one whatever the
-// timing.  The pools' data then moves in a launch of its own, a workgroup per 16 KB, bound by
-// memory: every byte is read once and written once.
+// timing: two launches would cost more than one workgroup's rounds (2048 slots: taking 300 of them
+// 4.7 us, planning a compaction 6.0, most of it the launch).  The pools' data then moves in a launch
+// of its own, a workgroup per 16 KB, bound by memory: every byte is read once and written once, 252
+// MB of slots of 512 KB in 55 us, 4.5 TB/s (a large copy: 5.1); 8 slots of 128 KB take 8.3 us.
 #include <algorithm>
 
 #include "prnn_host.h"
@@ -151,8 +153,8 @@ __global__ __launch_bounds__(256) void pages_copy_kernel(Pools P, int slots,
   copy_entry(P, s, d, blockIdx.x - i * per);
 }
 
-// scratch: [0] moves, [1 .. slots] new place of every slot, then the movers (slots / 2 + 1) and
-// the holes below them, as many.
+// scratch: [0] moves, [1 .. slots] new place of every slot, then the movers (slots / 2 at most)
+// and the holes below them, as many.
 __global__ __launch_bounds__(kPlan) void pages_plan_kernel(int* used, int slots, int* live,
                                                            int* scratch) {
   __shared__ int lds[kPlan / 64];
