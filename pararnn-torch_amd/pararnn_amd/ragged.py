@@ -108,12 +108,21 @@ class PackedSequences:
         self.sequences = int(host.numel()) - 1
         self.tokens = int(host[-1])
         self._on = {torch.device("cpu"): host.to(torch.int32)}
+        self._streams: set[tuple[int, int]] = set()  # (device index, stream) that use a copy
 
     def offsets(self, device: torch.device) -> Tensor:
-        """The int32 offsets on ``device``."""
+        """The int32 offsets on ``device``, for work on its current stream."""
         got = self._on.get(device)
         if got is None:
             got = self._on[device] = self._on[torch.device("cpu")].to(device)
+        if device.type == "cuda":
+            index = got.device.index
+            key = index, torch._C._cuda_getCurrentRawStream(index)
+            if key not in self._streams and not torch.cuda.is_current_stream_capturing():
+                # the copy is the handle's own: its memory must outlast this stream's work on it
+                # even where the program drops the handle first
+                got.record_stream(torch.cuda.current_stream(device))
+                self._streams.add(key)
         return got
 
 

@@ -123,3 +123,28 @@ def test_pages_refuse():
         compact_pages(used, pool, [_t(6, dtype=torch.int32)[::2]])
     with pytest.raises(RuntimeError):
         compact_pages(used, pool, [torch.zeros(3, dtype=torch.int32)])
+
+
+def test_packed_offsets_outlast_work_on_another_stream():
+    """A handle dropped while a side stream has yet to read its offsets: their memory is not handed
+    out before (what would lie there, all sequences empty, is valid too)."""
+    from pararnn_amd import PackedSequences, linear_attention
+
+    g = torch.Generator().manual_seed(5)
+    n = 4096
+    q = torch.randn(1, n, 2, 16, generator=g).to(DEV)
+    a = -torch.rand(1, n, 2, generator=g).to(DEV)
+    cu = torch.arange(0, n + 1, 16)
+    with torch.no_grad():
+        want, state = linear_attention(q, q, q, a, cu_seqlens=cu, return_state=True)
+        side = torch.cuda.Stream()
+        packed = PackedSequences(cu)
+        linear_attention(q, q, q, a, cu_seqlens=packed)  # the copy belongs to this stream
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)
+            got, late = linear_attention(q, q, q, a, cu_seqlens=packed, return_state=True)
+        del packed
+        others = [torch.zeros(cu.numel(), dtype=torch.int32, device=DEV) for _ in range(64)]
+        torch.cuda.synchronize()
+    assert torch.equal(got, want) and torch.equal(late, state) and len(others) == 64
