@@ -18,9 +18,11 @@
 // state into two parts as well (16 bits), for the backward pass, where the decays' gradient adds
 // up differences of the results.
 //
-// Bound by the issue of vector instructions (scaling, splitting and packing between the products:
-// 850 to 1000 a wave and chunk of 64 against some 60 matrix instructions) at the two or three
-// waves a SIMD that the state leaves registers for.  16384 tokens of 8 heads of (128, 128): the
+// Bound by the chain inside a chunk at the two or three waves a SIMD that the state leaves registers
+// for: between the products stand 770 (forward) to 910 (backward) vector instructions a wave and
+// chunk of 64 at (64, 64) against 44 to 50 matrix instructions (scaling, splitting, packing); in the backward
+// walk they take 27 % of a wave's cycles, waits for LDS, memory and barriers 44 %, and the matrix
+// units are busy for 14 % of the time.  16384 tokens of 8 heads of (128, 128): the
 // pieces' contributions 27 us (67 MB of k and v, 2.4 TB/s), the walk 43 (134 MB, 3.1 TB/s).  8 x
 // 2048 tokens of 16 heads of (64, 64): 31 and 36, backward with all gradients 31 and 116.  Chunks
 // of 32 (half the work on pairs, twice the scalings of the state) were as fast: 28 and 34, 28 and
