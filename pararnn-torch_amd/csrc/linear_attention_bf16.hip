@@ -98,6 +98,58 @@ __device__ __forceinline__ b8 split8(float* x) {
   return r.v;
 }
 
+// Upper half of a's lanes for the lower half of b's; odd rows of 16 lanes for even ones.
+__device__ __forceinline__ void swap_halves(uint32_t& a, uint32_t& b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  a = r[0];
+  b = r[1];
+}
+__device__ __forceinline__ void swap_rows(uint32_t& a, uint32_t& b) {
+  const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+  a = r[0];
+  b = r[1];
+}
+// A tile of 32 tokens and 32 columns in 16 bits.  As a product leaves it, p: lane l has token l % 32
+// and columns 8 q + 4 (l / 32) + {0 .. 3} in p[q].  As rows lie in memory, u: lane l has columns
+// 8 (l / 16) + {0 .. 7} of tokens l % 16 in u[0] and 16 + l % 16 in u[1], so that an access of 16
+// bytes a lane takes whole 64 bytes of 16 rows, not 16 bytes of 32.
+__device__ __forceinline__ void to_rows(u2* p, u4* u) {
+#pragma unroll
+  for (int w = 0; w < 2; ++w)
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      uint32_t a = p[q][w], b = p[q + 2][w];
+      swap_halves(a, b);
+      p[q][w] = a;
+      p[q + 2][w] = b;
+    }
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    uint32_t a = p[w & 2][w & 1], b = p[(w & 2) + 1][w & 1];
+    swap_rows(a, b);
+    u[0][w] = a;
+    u[1][w] = b;
+  }
+}
+__device__ __forceinline__ void from_rows(const u4* u, u2* p) {
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    uint32_t a = u[0][w], b = u[1][w];
+    swap_rows(a, b);
+    p[w & 2][w & 1] = a;
+    p[(w & 2) + 1][w & 1] = b;
+  }
+#pragma unroll
+  for (int w = 0; w < 2; ++w)
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      uint32_t a = p[q][w], b = p[q + 2][w];
+      swap_halves(a, b);
+      p[q][w] = a;
+      p[q + 2][w] = b;
+    }
+}
+
 // Inclusive running sum over the wave's lanes: rows of 16 by shifts, then the rows' last lanes
 // handed on.
 template <int CTRL, int ROWS>
@@ -301,8 +353,9 @@ void la_walk_bf16_kernel(LaParams P) {
     if (STATE_ONLY) fetch(next);
 
     f16v O[2];
-    u2 dv[2][4];
-    const int c4 = col0 + 32 * wave + 4 * half;  // first of this lane's columns of out
+    u4 dv[2][2];
+    const int c4 = col0 + 32 * wave + 4 * half;           // first of this lane's columns of out
+    const int c8 = col0 + 32 * wave + 8 * (lane >> 4);    // and of its rows in memory
     if (!STATE_ONLY) {
       // ---- the chunk's pairs: tiles (out rows, earlier rows) (0,0), (1,0), (1,1)
       for (int id = wave; id < 3; id += W) {
@@ -361,14 +414,14 @@ void la_walk_bf16_kernel(LaParams P) {
       if (FINE) {
         const int have = R.dots ? min(n_tok - base, kC) : 0, cut = R.rev ? kC - have : 0;
         const rsrc_t bd = make_rsrc(pd + static_cast<long long>(cut) * std_, have * std_);
-  #pragma unroll
-        for (int it = 0; it < 2; ++it) {
-          const int i = 32 * it + l32, row = (R.rev ? kC - 1 - i : i) - cut;
-  #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            dv[it][q] = __builtin_amdgcn_raw_buffer_load_b64(
-                bd, la_in(c4 + 8 * q < R.vd, 0) | (row * std_ + (c4 + 8 * q) * 2), 0, 0);
-        }
+#pragma unroll
+        for (int it = 0; it < 2; ++it)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int i = 32 * it + 16 * u + (lane & 15), row = (R.rev ? kC - 1 - i : i) - cut;
+            dv[it][u] = __builtin_amdgcn_raw_buffer_load_b128(
+                bd, la_in(c8 < R.vd, 0) | (row * std_ + c8 * 2), 0, 0);
+          }
       }
       fetch(next);
       // ---- the state's part of the output
@@ -425,38 +478,50 @@ void la_walk_bf16_kernel(LaParams P) {
           O[it] = mfma(zf[2 * it + s].v, pairs(2 * it, s, 0), O[it]);
           if (FINE) O[it] = mfma(zf[2 * it + s].v, pairs(2 * it, s, 1), O[it]);
         }
-      // ---- out: lane l has token l % 32 of a tile and four columns side by side
+      // ---- out
       const int cut = R.rev ? kC - n_here : 0;
       const rsrc_t bo = make_rsrc(po + static_cast<long long>(cut) * sto, n_here * sto);
       po += ahead * (next - base) * static_cast<long long>(sto);
       if (FINE) pd += ahead * (next - base) * static_cast<long long>(std_);
 #pragma unroll
       for (int it = 0; it < 2; ++it) {
-        const int i = 32 * it + l32, row = (R.rev ? kC - 1 - i : i) - cut;
-        const uint32_t at = row * sto + c4 * so;
         if (FINE) {
+          u2 r[4];
+          from_rows(dv[it], r);
           float d = 0.0f;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            d = fmaf(O[it][4 * q], lo_bf16(dv[it][q][0]), d);
-            d = fmaf(O[it][4 * q + 1], hi_bf16(dv[it][q][0]), d);
-            d = fmaf(O[it][4 * q + 2], lo_bf16(dv[it][q][1]), d);
-            d = fmaf(O[it][4 * q + 3], hi_bf16(dv[it][q][1]), d);
+            d = fmaf(O[it][4 * q], lo_bf16(r[q][0]), d);
+            d = fmaf(O[it][4 * q + 1], hi_bf16(r[q][0]), d);
+            d = fmaf(O[it][4 * q + 2], lo_bf16(r[q][1]), d);
+            d = fmaf(O[it][4 * q + 3], hi_bf16(r[q][1]), d);
           }
           d += __shfl_xor(d, 32);
-          if (half == 0) sdot[wave][i] = d;
+          if (half == 0) sdot[wave][32 * it + l32] = d;
         }
+        if (R.out_f32) {
+          const int i = 32 * it + l32, row = (R.rev ? kC - 1 - i : i) - cut;
+          const uint32_t at = row * sto + c4 * 4;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const uint32_t o = la_in(c4 + 8 * q < R.vd, 0) | (at + 8 * q * so);
-          const float v[4] = {O[it][4 * q], O[it][4 * q + 1], O[it][4 * q + 2], O[it][4 * q + 3]};
-          if (R.out_f32)
+          for (int q = 0; q < 4; ++q)
             __builtin_amdgcn_raw_buffer_store_b128(
-                u4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]),
-                   __float_as_uint(v[3])}, bo, o, 0, 0);
-          else
-            __builtin_amdgcn_raw_buffer_store_b64(
-                u2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])}, bo, o, 0, 0);
+                u4{__float_as_uint(O[it][4 * q]), __float_as_uint(O[it][4 * q + 1]),
+                   __float_as_uint(O[it][4 * q + 2]), __float_as_uint(O[it][4 * q + 3])},
+                bo, la_in(c4 + 8 * q < R.vd, 0) | (at + 32 * q), 0, 0);
+        } else {
+          u2 p[4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            p[q] = u2{pack_bf16x2(O[it][4 * q], O[it][4 * q + 1]),
+                      pack_bf16x2(O[it][4 * q + 2], O[it][4 * q + 3])};
+          u4 u[2];
+          to_rows(p, u);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int i = 32 * it + 16 * k + (lane & 15), row = (R.rev ? kC - 1 - i : i) - cut;
+            __builtin_amdgcn_raw_buffer_store_b128(
+                u[k], bo, la_in(c8 < R.vd, 0) | (row * sto + c8 * 2), 0, 0);
+          }
         }
       }
     }
