@@ -103,8 +103,19 @@ __device__ __forceinline__ double block_sum(double v, double* lds) {
   return lds[0] + lds[1] + lds[2] + lds[3];
 }
 __device__ __forceinline__ double block_dot(const float* a, const float* b, int n, double* lds) {
+  constexpr int kAhead = 8;  // loads under way, from empty places behind the end
+  const rsrc_t ra = make_rsrc(a, n * 4u), rb = make_rsrc(b, n * 4u);
   double d = 0.0;
-  for (int e = threadIdx.x; e < n; e += 256) d += static_cast<double>(a[e]) * b[e];
+  for (int e = threadIdx.x; e < n; e += 256 * kAhead) {
+    float x[kAhead], y[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      x[i] = ldb<float>(ra, (e + 256 * i) * 4u, 0);
+      y[i] = ldb<float>(rb, (e + 256 * i) * 4u, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) d += static_cast<double>(x[i]) * y[i];
+  }
   return block_sum(d, lds);
 }
 
@@ -118,8 +129,8 @@ __device__ __forceinline__ double flow_at(const DecayGradArgs& A, const LaPiece&
 }
 
 // A workgroup per part and head.  The dots are read twice (their sum first, to tie the end), the
-// second time from the L2; 8 x 2048 tokens of 16 heads take 8.6 us, a chain of reductions in fp64,
-// with two states a part (1001 tokens x 3, 6 heads of (48, 72)) 13.4.
+// second time from the L2; 8 x 2048 tokens of 16 heads take 7.0 us, a chain of reductions in fp64,
+// with two products of states a part (1001 tokens x 3, 6 heads of (48, 72)) 7.5.
 __global__ __launch_bounds__(256) void la_decay_grad_kernel(DecayGradArgs A) {
   __shared__ double s_wave[4];
   constexpr int kEach = 4;
@@ -133,13 +144,24 @@ __global__ __launch_bounds__(256) void la_decay_grad_kernel(DecayGradArgs A) {
     return;
   }
   const size_t t0 = A.seqs.cu ? pc.begin : static_cast<size_t>(pc.seq) * A.seqs.T + pc.begin;
-  auto step = [&](int t) {  // what the flow gains behind token t
-    double x = 0.0;
+  // what the flow gains behind tokens base + t, base + t + stride, ..: all loads before the first
+  // sum, zeros behind the part's end
+  auto steps = [&](double* x, int base, int t, int stride) {
+    const uint32_t bytes = min(n - base, 256 * kEach) * 4u;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) x[i] = 0.0;
     for (int k = 0; k < A.tiles; ++k) {
-      const size_t at = (static_cast<size_t>(k) * A.H + h) * A.batch_tokens + t0 + t;
-      x += static_cast<double>(A.k_dots[at]) - A.q_dots[at];
+      const size_t at = (static_cast<size_t>(k) * A.H + h) * A.batch_tokens + t0 + base;
+      const rsrc_t rk = make_rsrc(A.k_dots + at, bytes), rq = make_rsrc(A.q_dots + at, bytes);
+      float u[kEach], v[kEach];
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        u[i] = ldb<float>(rk, (t + i * stride) * 4u, 0);
+        v[i] = ldb<float>(rq, (t + i * stride) * 4u, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) x[i] += static_cast<double>(u[i]) - v[i];
     }
-    return x;
   };
   const size_t row = static_cast<size_t>(A.H) * A.DD;
   const size_t head = pc.seq * row + static_cast<size_t>(h) * A.DD;
@@ -153,17 +175,22 @@ __global__ __launch_bounds__(256) void la_decay_grad_kernel(DecayGradArgs A) {
   else if (A.gs)
     end = block_dot(A.last + head, A.gs + head, A.DD, s_wave);
   double all = 0.0;
-  for (int t = tid; t < n; t += 256) all += step(t);
+  for (int base = 0; base < n; base += 256 * kEach) {
+    double x[kEach];
+    steps(x, base, tid, 256);
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) all += x[i];
+  }
   all = block_sum(all, s_wave);
   const double miss = (begin + all - end) / n;  // per token
   double flow = begin, total = 0.0;
   for (int base = 0; base < n; base += 256 * kEach) {
-    double d[kEach], sum = 0.0;
+    double x[kEach], d[kEach], sum = 0.0;
+    steps(x, base, tid * kEach, 1);
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const int t = base + tid * kEach + i;
       d[i] = sum;  // what came before within the thread's tokens
-      sum += t < n ? step(t) : 0.0;
+      sum += x[i];
     }
     double run = sum;
 #pragma unroll
