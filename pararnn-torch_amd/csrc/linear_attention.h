@@ -59,6 +59,8 @@ struct LaSeqs {
   int T;            // tokens of a sequence (rectangular) or of the stream
   int len;          // tokens of a piece at most
   int pieces;       // upper bound of the pieces (the grid's)
+  int sub;          // tokens between the states that are formed first: divides len
+  int span;         // tokens of a walk's piece: len, or where those states are formed more
 };
 
 // States at the ends of the walks: rows of H x Dk x Dv floats.
@@ -80,7 +82,7 @@ struct LaRole {
   int rev;
   int exact;            // the final state is a result: all of its 24 bits count
   float p_scale, x_scale, u_scale;  // of the pairs, of the state's part, of what enters it
-  float* piece_state;   // [piece][head][Dk][Dv]: states before the pieces (NULL: not cut)
+  float* piece_state;   // [la_state_row][head][Dk][Dv]: states before the pieces (NULL: not cut)
   float* piece_decay;   // [piece][head]: a piece's whole log decay in the walk's direction
   LaState init, last;   // given state; where the final one goes (p = NULL: none)
 };
@@ -151,6 +153,12 @@ __device__ __forceinline__ LaPiece la_piece(const LaSeqs& q, int p) {
   }
   r.alone = r.first && r.last;
   return r;
+}
+
+// Row of the states (one every `sub` tokens, numbered like pieces of that length) before, and
+// backwards behind, the part of sequence s that token t lies in.
+__device__ __forceinline__ int la_state_row(const LaSeqs& q, int s, int t) {
+  return (q.cu ? s : s * ((q.T + q.sub - 1) / q.sub)) + t / q.sub;
 }
 
 // Row of sequence s, or NULL where there is none.

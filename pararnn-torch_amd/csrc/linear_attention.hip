@@ -39,10 +39,17 @@ __global__ __launch_bounds__(256) void la_join_kernel(JoinArgs A, int seq_blocks
   int p0, n;
   la_pieces_of(A.seqs, seq, p0, n);
   if (n < 2 || e >= A.DD) return;
+  // parts in the walk's order up to the one that its last piece starts with
+  const int s0 = A.seqs.cu ? la_offset(A.seqs, seq) : 0;
+  const int s1 = A.seqs.cu ? la_offset(A.seqs, seq + 1) : A.seqs.T;
+  const int per = A.seqs.span / A.seqs.sub, behind = n, c0 = s0 / A.seqs.sub;
+  n = A.rev[role] ? n - ((s0 / A.seqs.span + 1) * per - 1 - c0)
+                  : (s1 - 1) / A.seqs.span * per - c0 + 1;
+  if (n < 2) return;  // the walk has one piece
   const size_t row = static_cast<size_t>(A.H) * A.DD;
   const size_t at = static_cast<size_t>(h) * A.DD;
   const float* init = la_row(A.init[role], seq, row);
-  const int dir = A.rev[role] ? -1 : 1, from = A.rev[role] ? p0 + n - 1 : p0;
+  const int dir = A.rev[role] ? -1 : 1, from = A.rev[role] ? p0 + behind - 1 : p0;
   float S[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) S[v] = init ? init[at + e + v] : 0.0f;
@@ -87,7 +94,7 @@ struct DecayGradArgs {
   int tiles, H, DD, batch_tokens;
   LaState h0;
   const float *dh0, *last, *gs;          // rows of sequences: dL/dS_0, S_T, dL/dS_T
-  const float *state, *adjoint;          // [piece][head][DD] before the pieces, either direction
+  const float *state, *adjoint;          // the walks' states, either direction
   int g_dtype;
   void* dg;             // (token, H) of g's type, or NULL
   float* per_part;      // (piece, H) sums for decays per head, or NULL
@@ -119,12 +126,13 @@ __device__ __forceinline__ double block_dot(const float* a, const float* b, int 
   return block_sum(d, lds);
 }
 
-// The flow at the first token of part p of a sequence: its state with the adjoint of that token,
-// which is the one before the part that lies ahead.
-__device__ __forceinline__ double flow_at(const DecayGradArgs& A, const LaPiece& pc, int p,
-                                          int begin, int h, double* lds) {
+// The flow at the first token of a part: its state with the adjoint of that token, which is the one
+// behind the part before.
+__device__ __forceinline__ double flow_at(const DecayGradArgs& A, const LaPiece& pc, int begin,
+                                          int h, double* lds) {
   const size_t row = static_cast<size_t>(A.H) * A.DD, head = static_cast<size_t>(h) * A.DD;
-  return block_dot(A.state + p * row + head, A.adjoint + (p - 1) * row + head, A.DD, lds) *
+  return block_dot(A.state + la_state_row(A.seqs, pc.seq, begin) * row + head,
+                   A.adjoint + la_state_row(A.seqs, pc.seq, begin - 1) * row + head, A.DD, lds) *
          fexp(la_decay(A.g, la_batch(A.seqs, pc), begin, h));
 }
 
@@ -167,11 +175,11 @@ __global__ __launch_bounds__(256) void la_decay_grad_kernel(DecayGradArgs A) {
   const size_t head = pc.seq * row + static_cast<size_t>(h) * A.DD;
   double begin = 0.0, end = 0.0;
   if (!pc.first)
-    begin = flow_at(A, pc, p, pc.begin, h, s_wave);
+    begin = flow_at(A, pc, pc.begin, h, s_wave);
   else if (const float* s0 = la_row(A.h0, pc.seq, row))
     begin = block_dot(s0 + static_cast<size_t>(h) * A.DD, A.dh0 + head, A.DD, s_wave);
   if (!pc.last)
-    end = flow_at(A, pc, p + 1, pc.end, h, s_wave);
+    end = flow_at(A, pc, pc.end, h, s_wave);
   else if (A.gs)
     end = block_dot(A.last + head, A.gs + head, A.DD, s_wave);
   double all = 0.0;
@@ -374,14 +382,29 @@ struct Walks {
 // 2 x 512 tokens of 4 heads 19, 33, 31 and 19; 2048 of 4 heads 23, 33, 92 and 23, their training
 // step 60, 81, 218 and 60; 16384 of 8 heads 86, 55, 97 and 53, their training step 285, 206, 288
 // and 198; 8 x 2048 of 16 heads 97, 65, 99 and 64; 32 x 300 of 4 heads 29, 36, 23 and 23 (whole).
+//
+// Pieces that are longer for that get their states from the contributions of shorter parts, of the
+// length above: a training step of 8 x 2048 tokens of 16 heads 214 us, with parts as long as the
+// pieces 228.  A piece that a walk ends with has no contribution formed.
+LaSeqs pieces(const Problem& a, long long len, long long sub, long long span) {
+  LaSeqs s{a.cu_seqlens, sequences(a), a.T, a.T + 1, sequences(a), a.T + 1, a.T + 1};
+  if (len < a.T) {
+    s.len = static_cast<int>(len);
+    s.sub = static_cast<int>(sub);
+    s.span = static_cast<int>(span);
+    s.pieces = a.cu_seqlens ? s.n_seq + a.T / s.len : a.B * ((a.T + s.len - 1) / s.len);
+  }
+  return s;
+}
+
 LaSeqs cut(const Problem& a, const Walks& w, int widest, int roles, int states) {
-  LaSeqs s{a.cu_seqlens, sequences(a), a.T, 1, 0};
   const double serial = w.bf16 ? 0.085 : 0.17, per_piece = 0.12, bytes_us = 5.3e6, launches = 8.0;
   const double tokens = 1.0 * a.B * a.T;
   // packed sequences' lengths are not known here: some are twice the mean
   const double longest = a.cu_seqlens ? std::min(tokens, 2.0 * tokens / std::max(1, a.n_seq)) : a.T;
   const double falls = per_piece * longest + 16.0 * states * a.Dk * a.Dv * a.H * tokens / bytes_us;
-  long long len = std::max(1ll, std::llround(std::sqrt(falls / serial) / 64)) * 64;
+  const long long best = std::max(1ll, std::llround(std::sqrt(falls / serial) / 64)) * 64;
+  long long len = best;
   if (serial * longest * 2 / 3 <= serial * len + falls / len + launches) len = 1ll + a.T;
   const long long waves = w.cols(widest) / (w.bf16 ? 32 : 16);
   const long long most = (w.bf16 ? 2048 : 4096) / waves;  // workgroups that run at a time
@@ -392,15 +415,15 @@ LaSeqs cut(const Problem& a, const Walks& w, int widest, int roles, int states) 
     len = std::max(fill, a.cu_seqlens ? 0ll : (a.T + n - 1) / n);
     len = (len + 63) / 64 * 64;
   }
-  if (len >= a.T) {
-    s.len = a.T + 1;  // every sequence whole
-    s.pieces = s.n_seq;
-  } else {
-    s.len = static_cast<int>(len);
-    s.pieces = a.cu_seqlens ? s.n_seq + a.T / s.len
-                            : a.B * ((a.T + s.len - 1) / s.len);
-  }
-  return s;
+  if (len >= a.T) return pieces(a, len, len, len);  // every sequence whole
+  long long n = std::max(1ll, len / best);
+  while (len % (64 * n)) --n;
+  return pieces(a, len, len / n, len);
+}
+
+// The parts whose contributions to the states are formed.
+LaSeqs parts_of(const Problem& a, const LaSeqs& s) {
+  return is_cut(s) ? pieces(a, s.sub, s.sub, s.span) : s;
 }
 
 LaSeqs forward_cut(const Problem& a, const Walks& w) { return cut(a, w, a.Dv, 1, 1); }
@@ -416,8 +439,9 @@ Scratch carve(void* ws, const Problem& a, const Walks& w, bool backward, bool de
   const size_t tokens = static_cast<size_t>(a.B) * a.T;
   for (int i = 0; i < (backward ? 2 : 1); ++i)
     if (is_cut(q)) {
-      s.state[i] = static_cast<float*>(c.take(4 * dd * a.H * q.pieces));
-      s.decay[i] = static_cast<float*>(c.take(4 * static_cast<size_t>(a.H) * q.pieces));
+      const size_t rows = parts_of(a, q).pieces;
+      s.state[i] = static_cast<float*>(c.take(4 * dd * a.H * rows));
+      s.decay[i] = static_cast<float*>(c.take(4 * a.H * rows));
     }
   if (backward) {
     if (decay_grad) {
@@ -518,9 +542,12 @@ int forward(const Problem& a, const prnn_la_view& out, float* state_out, const i
   r.init = initial(a);
   r.last = LaState{state_out, out_table, out_rows};
   if (is_cut(p.seqs)) {
+    const LaSeqs walked = p.seqs;
+    p.seqs = parts_of(a, walked);
     if (int rc = w.run(p, 1, true, false, st)) return rc;
     const int rev = 0;
     if (int rc = join(p, s, &r.init, &rev, 1, st)) return rc;
+    p.seqs = walked;
   }
   return w.run(p, 1, false, false, st);
 }
@@ -555,12 +582,15 @@ int backward(const Problem& a, const prnn_la_view& go, const float* gs, void* dq
     return r;
   };
   if (is_cut(p.seqs)) {
+    const LaSeqs walked = p.seqs;
+    p.seqs = parts_of(a, walked);
     p.role[0] = role(none, k, v, a.Dk, a.Dv, false, 0);
     p.role[1] = role(none, q, o, a.Dk, a.Dv, false, 1);
     if (int rc = w.run(p, 2, true, false, st)) return rc;
     const LaState inits[2] = {init, fin};
     const int rev[2] = {0, 1};
     if (int rc = join(p, s, inits, rev, 2, st)) return rc;
+    p.seqs = walked;
   }
   p.role[0] = role(o, v, k, a.Dv, a.Dk, true, 0);
   p.role[1] = role(v, o, q, a.Dv, a.Dk, true, 1);

@@ -23,10 +23,10 @@
 // chunk of 64 at (64, 64) against 44 to 50 matrix instructions (scaling, splitting, packing); in the backward
 // walk they take 27 % of a wave's cycles, waits for LDS, memory and barriers 44 %, and the matrix
 // units are busy for 14 % of the time.  16384 tokens of 8 heads of (128, 128): the
-// pieces' contributions 27 us (67 MB of k and v, 2.4 TB/s), the walk 43 (134 MB, 3.1 TB/s).  8 x
-// 2048 tokens of 16 heads of (64, 64): 31 and 36, backward with all gradients 31 and 116.  Chunks
-// of 32 (half the work on pairs, twice the scalings of the state) were as fast: 28 and 34, 28 and
-// 148 (143 then), and 5 % slower on a packed batch.
+// pieces' contributions 27 us (67 MB of k and v, 2.4 TB/s), the walk 42 (134 MB, 3.2 TB/s).  8 x
+// 2048 tokens of 16 heads of (64, 64): 21 and 34, backward with all gradients 21 and 112.  Chunks
+// of 32 (half the work on pairs, twice the scalings of the state) were no faster: 34 forward for
+// 36 then, 148 backward for 143, and 5 % slower on a packed batch.
 #include "linear_attention.h"
 
 namespace prnn {
@@ -191,8 +191,9 @@ void la_walk_bf16_kernel(LaParams P) {
   if (tile * VT >= R.vd) return;
   const LaPiece pc = la_piece(P.seqs, piece);
   if (STATE_ONLY) {
-    // the piece that a walk ends with hands its state to none
-    if (pc.alone || (R.rev ? pc.first : pc.last)) return;
+    // a part of the piece that the walk ends with hands its state to none
+    const int at = pc.begin / P.seqs.span;
+    if (pc.alone || at == (R.rev ? pc.s0 : pc.s1 - 1) / P.seqs.span) return;
   } else if (pc.begin >= pc.end && !pc.first) {
     return;  // no piece (an empty sequence is one, it hands its state on)
   }
@@ -290,7 +291,8 @@ void la_walk_bf16_kernel(LaParams P) {
   if (!STATE_ONLY) {
     const float* src = nullptr;
     if (R.piece_state && !pc.alone)
-      src = R.piece_state + static_cast<size_t>(piece) * row_floats + head_floats;
+      src = R.piece_state + head_floats +
+            la_state_row(P.seqs, pc.seq, R.rev ? pc.end - 1 : pc.begin) * row_floats;
     else if (const float* row = la_row(R.init, pc.seq, row_floats))
       src = row + head_floats;
     if (src) {

@@ -134,8 +134,9 @@ __global__ __launch_bounds__(64 * W) void la_walk_f32_kernel(LaParams P) {
   if (col0 >= R.vd) return;
   const LaPiece pc = la_piece(P.seqs, piece);
   if (STATE_ONLY) {
-    // the piece that a walk ends with hands its state to none
-    if (pc.alone || (R.rev ? pc.first : pc.last)) return;
+    // a part of the piece that the walk ends with hands its state to none
+    const int at = pc.begin / P.seqs.span;
+    if (pc.alone || at == (R.rev ? pc.s0 : pc.s1 - 1) / P.seqs.span) return;
   } else if (pc.begin >= pc.end && !pc.first) {
     return;  // no piece (an empty sequence is one, it hands its state on)
   }
@@ -210,7 +211,8 @@ __global__ __launch_bounds__(64 * W) void la_walk_f32_kernel(LaParams P) {
   if (!STATE_ONLY) {
     const float* src = nullptr;
     if (R.piece_state && !pc.alone)
-      src = R.piece_state + static_cast<size_t>(piece) * row_floats + head_floats;
+      src = R.piece_state + head_floats +
+            la_state_row(P.seqs, pc.seq, R.rev ? pc.end - 1 : pc.begin) * row_floats;
     else if (const float* row = la_row(R.init, pc.seq, row_floats))
       src = row + head_floats;
     if (src) {

@@ -408,3 +408,27 @@ def test_shared_decay_and_lone_strides():
             assert torch.equal(linear_attention(q, wide, v, head),
                                linear_attention(q, wide.contiguous(), v, head))
 
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("cu", [None, [0, 2900, 2901, 2901, 4303, 6000]], ids=["batch", "packed"])
+def test_pieces_of_several_parts(cu, dtype):
+    """So many narrow heads that pieces are as long as the chip's workgroups ask for, three times
+    what the states' contributions are formed for."""
+    from pararnn_amd import linear_attention
+
+    B, T, S = (1, cu[-1], len(cu) - 1) if cu else (3, 2000, 3)
+    print(f"case pieces of several parts {cu} {dtype}", flush=True)
+    q, k, v, g, h0, go, gs = _inputs(B, T, (16, 8, 16), 16, 16, dtype, "token", 11, seqs=S)
+    exact = [t.double().requires_grad_(True) for t in (q, k, v, g, h0)]
+    o64, s64 = O.linear_attention(*exact, cu=cu)
+    want = torch.autograd.grad([o64, s64], exact, [go.double(), gs.double()])
+    mine = [t.to(DEV).requires_grad_(True) for t in (q, k, v, g, h0)]
+    out, state = linear_attention(*mine[:4], h0=mine[4], return_state=True,
+                                  cu_seqlens=torch.tensor(cu) if cu else None)
+    got = torch.autograd.grad([out, state], mine, [go.to(DEV), gs.to(DEV)])
+    assert _rel(out, o64) <= TOL[dtype] and _rel(state, s64) <= TOL[F32]
+    for name, x, y in zip(("dq", "dk", "dv", "dg", "dh0"), got, want):
+        e = _rel(x, y)
+        print(f"  {name} {e:.1e}", flush=True)
+        assert e <= (TOL[F32] if name == "dh0" else TOL_G[dtype] if name == "dg" else TOL[dtype]), name
