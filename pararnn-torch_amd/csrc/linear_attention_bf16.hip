@@ -21,12 +21,12 @@
 // Bound by the chain inside a chunk at the two or three waves a SIMD that the state leaves registers
 // for: between the products stand 770 (forward) to 910 (backward) vector instructions a wave and
 // chunk of 64 at (64, 64) against 44 to 50 matrix instructions (scaling, splitting, packing); in the backward
-// walk they take 27 % of a wave's cycles, waits for LDS, memory and barriers 44 %, and the matrix
+// walk they take 29 % of a wave's cycles, waits for LDS, memory and barriers 43 %, and the matrix
 // units are busy for 14 % of the time.  16384 tokens of 8 heads of (128, 128): the
 // pieces' contributions 27 us (67 MB of k and v, 2.4 TB/s), the walk 42 (134 MB, 3.2 TB/s).  8 x
 // 2048 tokens of 16 heads of (64, 64): 21 and 34, backward with all gradients 21 and 112.  Chunks
-// of 32 (half the work on pairs, twice the scalings of the state) were no faster: 34 forward for
-// 36 then, 148 backward for 143, and 5 % slower on a packed batch.
+// of 32 (half the work on pairs, twice the scalings of the state, two buffers and one barrier) were
+// no faster: 34 forward, 134 backward, contributions on a packed batch 28 for 24.
 #include "linear_attention.h"
 
 namespace prnn {
