@@ -17,7 +17,7 @@ import torch
 from torch import Tensor
 
 from pararnn_amd import _lib
-from pararnn_amd.attention import _at, _enqueue
+from pararnn_amd.attention import _at, _enqueue, _once
 from pararnn_amd.ops import _DTYPES, _validate, _workspace
 
 _ACTIVATIONS = {None: 0, "silu": 1, "sigmoid": 2}
@@ -32,42 +32,54 @@ def _shape(x: Tensor, over: str) -> tuple[int, int, int]:
     return n, (x.numel() // (n * c) if n else 0), c
 
 
+def _flat(t: Tensor | None) -> Tensor | None:
+    """As the kernels read it: contiguous, from a 16-byte boundary."""
+    if t is None:
+        return None
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
 @functools.lru_cache(maxsize=256)
 def _workspace_bytes(n: int, length: int, c: int, groups: int, code: int, backward: int) -> int:
     return _lib.load().prnn_group_norm_workspace_size(n, length, c, groups, code, backward)
 
 
-def _forward(x, weight, bias, gate, groups, eps, act, over):
-    n, length, c = _shape(x, over)
-    y = torch.empty_like(x)
+def _codes(x, weight, bias, groups, eps, act, over) -> tuple:
+    """The C entries' numbers: N, L, C, groups, eps, act and the types of w and x."""
     code = _DTYPES[x.dtype]
     w = bias if weight is None else weight
+    return (*_shape(x, over), groups, eps, act, code if w is None else _DTYPES[w.dtype], code)
+
+
+def _forward(x, weight, bias, gate, codes):
+    n, length, c, groups, _, _, _, code = codes
+    y = torch.empty_like(x)
     need = _workspace_bytes(n, length, c, groups, code, 0)
     ws = stats = None
     if need:  # statistics per sample, or groups too wide for a wave
         ws = _workspace(need, x.device)
         stats = torch.empty(n, groups, 2, dtype=torch.float32, device=x.device)
     rc = _enqueue(_lib.load().prnn_group_norm, x.device, x.data_ptr(), _at(weight), _at(bias),
-                  _at(gate), y.data_ptr(), _at(stats), n, length, c, groups, eps, act,
-                  code if w is None else _DTYPES[w.dtype], code, _at(ws), need)
+                  _at(gate), y.data_ptr(), _at(stats), *codes, _at(ws), need)
     _lib.check(rc, "group_norm")
     return y, stats
 
 
 class _GroupNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, gate, groups, eps, act, over):
-        y, stats = _forward(x, weight, bias, gate, groups, eps, act, over)
+    def forward(ctx, x, weight, bias, gate, codes):
+        y, stats = _forward(x, weight, bias, gate, codes)
         ctx.save_for_backward(x, weight, bias, gate, stats)
-        ctx.args = (groups, eps, act, over)
+        ctx.codes = codes
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, gy):
         x, weight, bias, gate, stats = ctx.saved_tensors
-        groups, eps, act, over = ctx.args
-        n, length, c = _shape(x, over)
+        codes = ctx.codes
+        n, length, c, groups, _, _, _, code = codes
         dev = x.device
         if gy.dtype != x.dtype:
             gy = gy.to(x.dtype)
@@ -78,17 +90,13 @@ class _GroupNorm(torch.autograd.Function):
         dgate = None if gate is None else torch.empty_like(x)
         dw = None if weight is None else torch.empty_like(weight)
         db = None if bias is None else torch.empty_like(bias)
-        code = _DTYPES[x.dtype]
-        w = bias if weight is None else weight
         need = _workspace_bytes(n, length, c, groups, code, 1)
         ws = _workspace(need, dev)
         rc = _enqueue(_lib.load().prnn_group_norm_backward, dev, gy.data_ptr(), x.data_ptr(),
                       _at(weight), _at(bias), _at(gate), _at(stats), dx.data_ptr(), _at(dw),
-                      _at(db), _at(dgate), n, length, c, groups, eps, act,
-                      code if w is None else _DTYPES[w.dtype], code, ws.data_ptr(), ws.numel())
+                      _at(db), _at(dgate), *codes, ws.data_ptr(), ws.numel())
         _lib.check(rc, "group_norm backward")
-        need_in = ctx.needs_input_grad
-        return (dx if need_in[0] else None, dw, db, dgate, None, None, None, None)
+        return dx if ctx.needs_input_grad[0] else None, dw, db, dgate, None
 
 
 def group_norm(x: Tensor, num_groups: int, weight: Tensor | None = None,
@@ -134,17 +142,13 @@ def group_norm(x: Tensor, num_groups: int, weight: Tensor | None = None,
     if x.numel() // c >= 1 << 31:
         raise ValueError(f"{what}: x has {x.numel() // c} tokens, more than 2^31 - 1")
 
-    def flat(t):
-        # as the kernels read it: contiguous, from a 16-byte boundary
-        if t is None:
-            return None
-        t = t.contiguous()
-        return t.clone() if t.data_ptr() % 16 else t
-
-    x, gate = flat(x), flat(gate)
-    weight, bias = (None if t is None else t.contiguous() for t in (weight, bias))
-    act = _ACTIVATIONS[activation]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (x, weight, bias, gate)):
-        return _GroupNorm.apply(x, weight, bias, gate, int(num_groups), float(eps), act, over)
-    return _forward(x, weight, bias, gate, int(num_groups), float(eps), act, over)[0]
+    x, gate = _flat(x), _flat(gate)
+    weight = None if weight is None else weight.contiguous()
+    bias = None if bias is None else bias.contiguous()
+    codes = _codes(x, weight, bias, int(num_groups), float(eps), _ACTIVATIONS[activation], over)
+    if torch.is_grad_enabled() and (x.requires_grad
+                                    or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)
+                                    or (gate is not None and gate.requires_grad)):
+        return _GroupNorm.apply(x, weight, bias, gate, codes)
+    return _forward(x, weight, bias, gate, codes)[0]

@@ -148,3 +148,18 @@ def test_packed_offsets_outlast_work_on_another_stream():
         others = [torch.zeros(cu.numel(), dtype=torch.int32, device=DEV) for _ in range(64)]
         torch.cuda.synchronize()
     assert torch.equal(got, want) and torch.equal(late, state) and len(others) == 64
+
+
+def test_gradients_are_differentiable_once():
+    """A graph of the gradients can be asked for; a second derivative is refused, not wrong."""
+    from pararnn_amd import group_norm, linear_attention
+
+    g = torch.Generator().manual_seed(9)
+    q = torch.randn(1, 20, 2, 8, generator=g).to(DEV).requires_grad_(True)
+    a = -torch.rand(1, 20, 2, generator=g).to(DEV)
+    for y in (linear_attention(q, q, q, a), group_norm(q.flatten(-2), 2)):
+        plain = torch.autograd.grad(y.square().sum(), q, retain_graph=True)[0]
+        again = torch.autograd.grad(y.square().sum(), q, create_graph=True)[0]
+        assert torch.equal(plain, again)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            again.sum().backward()
