@@ -520,6 +520,8 @@ typedef struct prnn_linear_attention_problem {
   int B, T, H, Dk, Dv;
   int g_dtype, dtype;
   float scale;
+  int longest; /* packed: tokens of the longest sequence, 0 where that is not known (how the work is
+                * cut goes by it, the result does not) */
 } prnn_linear_attention_problem;
 
 PRNN_API size_t

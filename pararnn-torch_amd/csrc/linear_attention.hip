@@ -400,8 +400,9 @@ LaSeqs pieces(const Problem& a, long long len, long long sub, long long span) {
 LaSeqs cut(const Problem& a, const Walks& w, int widest, int roles, int states) {
   const double serial = w.bf16 ? 0.085 : 0.17, per_piece = 0.12, bytes_us = 5.3e6, launches = 8.0;
   const double tokens = 1.0 * a.B * a.T;
-  // packed sequences' lengths are not known here: some are twice the mean
-  const double longest = a.cu_seqlens ? std::min(tokens, 2.0 * tokens / std::max(1, a.n_seq)) : a.T;
+  // packed sequences of unknown lengths: one may be all there is (100 of 60 tokens, 8 heads of (64,
+  // 64): 11 us where that is known, 42 where not)
+  const double longest = a.cu_seqlens && a.longest > 0 ? std::min(a.longest, a.T) : a.T;
   const double falls = per_piece * longest + 16.0 * states * a.Dk * a.Dv * a.H * tokens / bytes_us;
   const long long best = std::max(1ll, std::llround(std::sqrt(falls / serial) / 64)) * 64;
   long long len = best;
@@ -415,7 +416,7 @@ LaSeqs cut(const Problem& a, const Walks& w, int widest, int roles, int states) 
     len = std::max(fill, a.cu_seqlens ? 0ll : (a.T + n - 1) / n);
     len = (len + 63) / 64 * 64;
   }
-  if (len >= a.T) return pieces(a, len, len, len);  // every sequence whole
+  if (len >= longest) return pieces(a, 1ll + a.T, 0, 0);  // every sequence whole
   long long n = std::max(1ll, len / best);
   while (len % (64 * n)) --n;
   return pieces(a, len, len / n, len);

@@ -45,7 +45,7 @@ class LaProblem(ctypes.Structure):
                 ("h0_table", ctypes.c_void_p), ("cu_seqlens", ctypes.c_void_p),
                 *((n, ctypes.c_int) for n in ("h0_rows", "n_seq", "B", "T", "H", "Dk", "Dv",
                                               "g_dtype", "dtype")),
-                ("scale", ctypes.c_float)]
+                ("scale", ctypes.c_float), ("longest", ctypes.c_int)]
 
 
 class Pool(ctypes.Structure):

@@ -167,14 +167,14 @@ class _Problem:
             raise ValueError(f"{what}: head widths ({dk}, {dv}) are not in 1 .. 256")
         self.dims = (batch, time, heads, dk, dv)
         self.sequences = batch
-        self.offsets = None
+        self.offsets, self.longest = None, 0
         if packed is not None:
             if batch != 1:
                 raise ValueError(f"{what}: cu_seqlens packs q with batch=1, got batch={batch}")
             if packed.tokens != time:
                 raise ValueError(f"cu_seqlens[-1] must equal time={time}, got {packed.tokens}")
             self.sequences = packed.sequences
-            self.offsets = packed.offsets(q.device)
+            self.offsets, self.longest = packed.offsets(q.device), packed.longest
         self.table = None
         if table is not None:
             if h0 is None:
@@ -199,7 +199,8 @@ class _Problem:
         self.c = _lib.LaProblem(
             _view(self.q), _view(self.k), _view(self.v), g.data_ptr(), *at, _at(self.h0),
             _at(self.table), _at(self.offsets), 0 if self.h0 is None else self.h0.shape[0],
-            0 if self.offsets is None else self.sequences, *self.dims, *self.codes, self.scale)
+            0 if self.offsets is None else self.sequences, *self.dims, *self.codes, self.scale,
+            self.longest)
 
     def again(self, q: Tensor, k: Tensor, v: Tensor, g: Tensor, h0: Tensor | None) -> _Problem:
         """The same checked call on tensors like those it was made of (backward)."""
@@ -208,6 +209,7 @@ class _Problem:
         p.h0 = None if h0 is None else h0.contiguous()
         p.dims, p.codes, p.scale = self.dims, self.codes, self.scale
         p.sequences, p.offsets, p.table = self.sequences, self.offsets, None
+        p.longest = self.longest
         p._fill()
         return p
 

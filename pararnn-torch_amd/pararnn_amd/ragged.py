@@ -107,6 +107,7 @@ class PackedSequences:
             raise ValueError(f"a packed batch holds fewer than 2^30 tokens, got {int(host[-1])}")
         self.sequences = int(host.numel()) - 1
         self.tokens = int(host[-1])
+        self.longest = int((host[1:] - host[:-1]).max())
         self._on = {torch.device("cpu"): host.to(torch.int32)}
         self._streams: set[tuple[int, int]] = set()  # (device index, stream) that use a copy
 
