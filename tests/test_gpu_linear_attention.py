@@ -432,3 +432,24 @@ def test_pieces_of_several_parts(cu, dtype):
         e = _rel(x, y)
         print(f"  {name} {e:.1e}", flush=True)
         assert e <= (TOL[F32] if name == "dh0" else TOL_G[dtype] if name == "dg" else TOL[dtype]), name
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_one_long_sequence_among_short_ones(dtype):
+    """Cut for the long one's sake; told or not, the longest length changes no more than the order of
+    sums: twice the tolerance between two results that are each within it."""
+    from pararnn_amd import PackedSequences, linear_attention
+
+    cu = torch.tensor([0] + [20] * 10 + [1500] + [3] * 7).cumsum(0)
+    S, N = cu.numel() - 1, int(cu[-1])
+    q, k, v, g, h0, go, gs = _inputs(1, N, (2, 2, 2), 32, 64, dtype, "token", 13, seqs=S)
+    o64, s64 = O.linear_attention(*(t.double() for t in (q, k, v, g, h0)), cu=cu.tolist())
+    mine = [t.to(DEV) for t in (q, k, v, g)]
+    with torch.no_grad():
+        packed = PackedSequences(cu)
+        assert packed.longest == 1500
+        out, state = linear_attention(*mine, h0=h0.to(DEV), cu_seqlens=packed, return_state=True)
+        packed.longest = 0  # not known
+        other, last = linear_attention(*mine, h0=h0.to(DEV), cu_seqlens=packed, return_state=True)
+    assert _rel(out, o64) <= TOL[dtype] and _rel(state, s64) <= TOL[F32]
+    assert _rel(other, out) <= 2 * TOL[dtype] and _rel(last, state) <= 2 * TOL[F32]

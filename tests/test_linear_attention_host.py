@@ -100,3 +100,11 @@ def test_c_entries_refuse_grids_that_pass_32_bits():
     pool = (_lib.Pool * 1)(_lib.Pool(256, 1 << 39))
     rc = lib.prnn_pages_copy(1, pool, 1, 256, 256, 1, None)
     assert rc == _lib.PRNN_ERR_VALUE and b"too many for a launch" in lib.prnn_last_error()
+
+
+def test_packed_sequences_know_their_longest():
+    from pararnn_amd import PackedSequences
+
+    for cu, longest in (([0, 3, 3, 10], 7), ([0, 0], 0), ([0, 5], 5), ([0, 1, 2, 3], 1)):
+        packed = PackedSequences(torch.tensor(cu))
+        assert (packed.longest, packed.tokens, packed.sequences) == (longest, cu[-1], len(cu) - 1)
