@@ -289,7 +289,8 @@ int la_walk_f32(LaParams p, int roles, bool state_only, int dtype, hipStream_t s
 int la_f32_tile_cols(int vd);
 // bf16 storage with widths in multiples of 8, rows that admit 16-byte accesses (x, y, z, dot) or
 // 8-byte ones (out), and tokens at least a row apart, in ascending order.
-int la_walk_bf16(LaParams p, int roles, bool state_only, bool fine, hipStream_t stream);
+// dots: some role has dots.
+int la_walk_bf16(LaParams p, int roles, bool state_only, bool dots, hipStream_t stream);
 int la_bf16_tile_cols(int vd);
 
 }  // namespace prnn

@@ -362,8 +362,8 @@ struct Walks {
   int dtype;
   int cols(int vd) const { return bf16 ? la_bf16_tile_cols(vd) : la_f32_tile_cols(vd); }
   int tiles(int vd) const { return (vd + cols(vd) - 1) / cols(vd); }
-  int run(const LaParams& p, int roles, bool state_only, bool fine, hipStream_t st) const {
-    return bf16 ? la_walk_bf16(p, roles, state_only, fine, st)
+  int run(const LaParams& p, int roles, bool state_only, bool dots, hipStream_t st) const {
+    return bf16 ? la_walk_bf16(p, roles, state_only, dots, st)
                 : la_walk_f32(p, roles, state_only, dtype, st);
   }
 };
@@ -622,7 +622,6 @@ int backward(const Problem& a, const prnn_la_view& go, const float* gs, void* dq
     p.role[1].dot = k;
     p.role[1].dots = s.dots[1];
   }
-  // the decays' gradient adds up differences of the results: they are formed finer for it
   if (int rc = w.run(p, 3, false, dg != nullptr, st)) return rc;
   const size_t tokens = static_cast<size_t>(a.B) * a.T;
   if (sums && tokens) {
