@@ -4,10 +4,12 @@
 // * la_decay_grad_kernel: the log decays' gradient.  dL/dg_t = exp(g_t)
 //   <S_{t-1}, R_t> is the flow from all earlier tokens to t and later ones; from one token to the
 //   next it gains what token t hands on and loses what it receives, so it is a running sum of
-//   k_t . dk_t - q_t . dq_t (both formed in fp32 by the walks).  The flow itself stays bounded
-//   while the sum's roundings add up, so the sum is tied at both ends of a sequence (<S_0,
-//   dL/dS_0> and <S_T, dL/dS_T>, zero without states) and, in the fp32 walks, of every piece,
-//   whose states are there; what it misses the end by is taken back along the way;
+//   k_t . dk_t - q_t . dq_t (both formed in fp32 by the walks).  What a token hands to itself,
+//   scale (q_t . k_t)(v_t . go_t), is in both and in neither here: behind a strong decay the flow is a
+//   small part of it (exp(-12) of it and less, which fp32 differences of the whole would lose).  The
+//   flow itself stays bounded while the sum's roundings add up, so the sum is tied at both ends of a
+//   sequence (<S_0, dL/dS_0> and <S_T, dL/dS_T>, zero without states) and of every piece, whose
+//   states are there; what it misses the end by is taken back along the way;
 // * la_head_sum_kernel: gradients of shared heads, summed in a fixed order.
 #include "linear_attention.h"
 
@@ -194,6 +196,10 @@ __global__ __launch_bounds__(256) void la_decay_grad_kernel(DecayGradArgs A) {
   double flow = begin, total = 0.0;
   for (int base = 0; base < n; base += 256 * kEach) {
     double x[kEach], d[kEach], sum = 0.0;
+    uint32_t g[kEach];  // decays, loaded ahead too (the last token's behind the end)
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      g[i] = la_decay_bits(A.g, la_batch(A.seqs, pc), min(pc.begin + base + tid * kEach + i, pc.end - 1), h);
     steps(x, base, tid * kEach, 1);
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
@@ -219,7 +225,9 @@ __global__ __launch_bounds__(256) void la_decay_grad_kernel(DecayGradArgs A) {
     for (int i = 0; i < kEach; ++i) {
       const int t = base + tid * kEach + i;
       if (t >= n) continue;
-      const float v = static_cast<float>(before + d[i] - miss * t);
+      // nothing comes through a factor that is zero
+      const float v = la_decay_value(A.g, g[i]) <= -104.0f ? 0.0f
+                          : static_cast<float>(before + d[i] - miss * t);
       total += v;
       if (A.dg) {
         const size_t at = (t0 + t) * A.H + h;
@@ -639,11 +647,6 @@ int backward(const Problem& a, const prnn_la_view& go, const float* gs, void* dq
   if (dg) {
     DecayGradArgs d{};
     d.seqs = p.seqs;
-    if (w.bf16) {
-      // 16-bit results: tying whole sequences is enough
-      d.seqs.len = a.T + 1;
-      d.seqs.pieces = sequences(a);
-    }
     d.g = p.g;
     d.q_dots = s.dots[0];
     d.k_dots = s.dots[1];

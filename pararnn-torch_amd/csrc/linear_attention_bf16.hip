@@ -99,6 +99,9 @@ __device__ __forceinline__ b8 split8(float* x) {
   return r.v;
 }
 
+// By value: of two elements of an array the compiler would make one with a variable index.
+__device__ __forceinline__ float pick(bool b, float x, float y) { return b ? x : y; }
+
 // Upper half of a's lanes for the lower half of b's; odd rows of 16 lanes for even ones.
 __device__ __forceinline__ void swap_halves(uint32_t& a, uint32_t& b) {
   const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
@@ -182,7 +185,7 @@ void la_walk_bf16_kernel(LaParams P) {
   __shared__ __align__(16) char sz[kC * RZ];
   __shared__ __align__(16) char sp[KP ? KP : 16];
   __shared__ __align__(16) float sG[kC], se[kC], sw[kC];
-  __shared__ float sdot[W][kC], s_tot, s_sum;
+  __shared__ float sdot[W][kC], s_own[DOTS ? kC : 1], s_tot, s_sum;
   __shared__ int s_stop[2];
 
   const LaPlace place = la_place(P);
@@ -262,6 +265,9 @@ void la_walk_bf16_kernel(LaParams P) {
   const char *po = nullptr, *pd = nullptr;
   if (!STATE_ONLY) po = window(LaView{R.out, R.o_sb, R.o_st, R.o_sh, 1, 1}, so);
   if (DOTS) pd = window(R.dot, 2);
+  // Dots leave out a token's pair with itself (linear_attention.hip): its part of the output is added
+  // behind them.
+  const bool dots = DOTS && R.dots != nullptr;
   // Decays of the chunk's first `n` tokens: running sums from the front for the pairs and the
   // state's part, from the back for what enters the state, so that each weight that counts is the
   // exponential of a short sum.
@@ -381,10 +387,20 @@ void la_walk_bf16_kernel(LaParams P) {
           acc = mfma(y.v, *reinterpret_cast<const b8*>(xr + (f ^ 32 * k)), acc);
         }
         // weights: exponentials to base 2, the scale among them
+        if (dots && it == jt) {
+          // element 4 q + r with 8 q + 4 half + r = l32
+          float a[8], c[4];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) a[e] = pick(l32 & 1, acc[2 * e + 1], acc[2 * e]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) c[e] = pick(l32 & 2, a[2 * e + 1], a[2 * e]);
+          const float d = pick(l32 & 16, pick(l32 & 8, c[3], c[2]), pick(l32 & 8, c[1], c[0]));
+          if ((l32 >> 2 & 1) == half) s_own[i] = R.p_scale * d;
+        }
         const float Gi = sG[i] + log_scale;
         // Not to be known before: as masks of its own kept over the walk it costs two lane reads
         // an element.
-        int before = 32 * jt + 4 * half - i;
+        int before = 32 * jt + 4 * half - i + dots;
         asm volatile("" : "+v"(before));
         float w[16];
 #pragma unroll
@@ -411,7 +427,7 @@ void la_walk_bf16_kernel(LaParams P) {
       // loaded first, and nothing before the registers of the pairs are free.  Behind the piece's end
       // nothing is loaded; a branch would be waited at.
       if (DOTS) {
-        const int have = R.dots ? min(n_tok - base, kC) : 0, cut = R.rev ? kC - have : 0;
+        const int have = dots ? min(n_tok - base, kC) : 0, cut = R.rev ? kC - have : 0;
         const rsrc_t bd = make_rsrc(pd + static_cast<long long>(cut) * std_, have * std_);
 #pragma unroll
         for (int it = 0; it < 2; ++it)
@@ -496,6 +512,18 @@ void la_walk_bf16_kernel(LaParams P) {
           }
           d += __shfl_xor(d, 32);
           if (half == 0) sdot[wave][32 * it + l32] = d;
+          if (dots) {
+            const float own = s_own[32 * it + l32];
+            const char* zr = sz + (32 * it + l32) * RZ + wave * 64 + 8 * half;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const u2 z = *reinterpret_cast<const u2*>(zr + 16 * q);
+              O[it][4 * q] = fmaf(own, lo_bf16(z[0]), O[it][4 * q]);
+              O[it][4 * q + 1] = fmaf(own, hi_bf16(z[0]), O[it][4 * q + 1]);
+              O[it][4 * q + 2] = fmaf(own, lo_bf16(z[1]), O[it][4 * q + 2]);
+              O[it][4 * q + 3] = fmaf(own, hi_bf16(z[1]), O[it][4 * q + 3]);
+            }
+          }
         }
         if (R.out_f32) {
           const int i = 32 * it + l32, row = (R.rev ? kC - 1 - i : i) - cut;
@@ -562,7 +590,7 @@ void la_walk_bf16_kernel(LaParams P) {
       }
     }
     __syncthreads();
-    if (DOTS && R.dots && tid < n_here) {
+    if (dots && tid < n_here) {
       float d = 0.0f;
 #pragma unroll
       for (int w = 0; w < W; ++w) d += sdot[w][tid];

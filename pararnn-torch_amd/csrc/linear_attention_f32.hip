@@ -122,7 +122,7 @@ __global__ __launch_bounds__(64 * W) void la_walk_f32_kernel(LaParams P) {
   __shared__ __align__(16) float sz[kC * ZS];
   __shared__ __align__(16) float sp[STATE_ONLY ? 4 : kC * PS];
   __shared__ __align__(16) double sG[kC];
-  __shared__ __align__(16) float se[kC], sw[kC];
+  __shared__ __align__(16) float se[kC], sw[kC], s_own[STATE_ONLY ? 4 : kC];
   __shared__ float sdot[W][kC], s_tot, s_sum;
   __shared__ int s_stop[2];
 
@@ -263,7 +263,8 @@ __global__ __launch_bounds__(64 * W) void la_walk_f32_kernel(LaParams P) {
     }
     const int n_here = min(n_tok, next) - base;  // tokens of this chunk
 
-    // ---- the chunk's pairs, masked and decayed: quadrants (0,0), (1,0), (1,1)
+    // ---- the chunk's pairs, masked and decayed: quadrants (0,0), (1,0), (1,1).  Dots leave out a
+    // token's pair with itself (linear_attention.hip): its part of the output is added behind them.
     float dv[2][4];
     if (!STATE_ONLY) {
       for (int id = wave; id < 3; id += W) {
@@ -288,7 +289,8 @@ __global__ __launch_bounds__(64 * W) void la_walk_f32_kernel(LaParams P) {
         for (int r = 0; r < 4; ++r) {
           const int m = 16 * mi + 4 * q4 + r;
           const float w = (acc[0][r] + acc[1][r]) * (R.p_scale * exp2_diff(sG[m], Gn));
-          sp[m * PS + n] = after <= r ? w : 0.0f;
+          sp[m * PS + n] = after + (R.dots != nullptr) <= r ? w : 0.0f;
+          if (mi == ni && after == r) s_own[m] = w;
         }
       }
       // The rows that the output is multiplied with, then the next chunk's: what is waited for
@@ -346,7 +348,17 @@ __global__ __launch_bounds__(64 * W) void la_walk_f32_kernel(LaParams P) {
       const rsrc_t bo = la_rows<kC>(LaView{R.out, R.o_sb, R.o_st, R.o_sh, 1, 1}, so, b, h, R.rev,
                                     pc.begin, pc.end, base);
 #pragma unroll
-      for (int mi = 0; mi < 2; ++mi)
+      for (int mi = 0; mi < 2; ++mi) {
+        if (R.dots) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float d = row_sum(O[mi][r] * dv[mi][r]);
+            if (l16 == 0) sdot[wave][16 * mi + 4 * q4 + r] = d;
+          }
+          const f4 own = *reinterpret_cast<const f4*>(&s_own[16 * mi + 4 * q4]);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) O[mi][r] = fmaf(own[r], zr[mi][r], O[mi][r]);
+        }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int i = 16 * mi + 4 * q4 + r, row = R.rev ? kC - 1 - i : i;
@@ -356,11 +368,8 @@ __global__ __launch_bounds__(64 * W) void la_walk_f32_kernel(LaParams P) {
             stb<float>(bo, o, 0, O[mi][r]);
           else
             stb<T>(bo, o, 0, O[mi][r]);
-          if (R.dots) {
-            const float d = row_sum(O[mi][r] * dv[mi][r]);
-            if (l16 == 0) sdot[wave][i] = d;
-          }
         }
+      }
     }
 
     // ---- the state behind the chunk
