@@ -558,9 +558,9 @@ PRNN_API int prnn_linear_attention_step(const void* q, long long q_sb, long long
  * per token).  y = act(z) with z = w (x - mean) rstd + b, or z act(gate) where gate is given.
  * act: 0 none, 1 silu, 2 sigmoid.  w and b (C; NULL: ones, zeros) float32 or of x's type.
  * stats: (N, G, 2) floats (mean, rstd) that the forward call writes and the backward call reads;
- * not used (may be NULL) where L = 1 and a group is at most 256 accesses of 16 bytes (4 or 2
+ * not needed (may be NULL) where L = 1 and a group is at most 256 accesses of 16 bytes (4 or 2
  * bytes where alignment or an odd width allows no more).  The backward call's alignment of x,
- * gate, gy, dx and dgate may differ from the forward call's only if stats is given. */
+ * gate, gy, dx and dgate may differ from the forward call's only if stats is given to both. */
 PRNN_API size_t prnn_group_norm_workspace_size(int N, int L, int C, int G, int dtype,
                                                int backward);
 PRNN_API int prnn_group_norm(const void* x, const void* w, const void* b, const void* gate,

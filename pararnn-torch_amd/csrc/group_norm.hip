@@ -27,7 +27,7 @@ enum { kActNone = 0, kActSilu = 1, kActSigmoid = 2 };
 struct NormArgs {
   const void *x, *w, *b, *gate, *gy;
   void *y, *dx, *dgate;
-  float* stats;      // (N, G) mean, rstd of samples
+  float* stats;      // (N, G) mean, rstd (tokens: where wanted)
   float* part;       // partial sums, see the kernels
   float* part2;
   size_t rows;       // tokens (token kernels)
@@ -212,6 +212,11 @@ __global__ __launch_bounds__(256) void norm_token_kernel(NormArgs A) {
         s = fmaf(d, d, s);
       }
     const float rstd = 1.0f / sqrtf(fmaf(group_sum(s, A.lanes), inv, A.eps));
+    if (A.stats && live && p.l == 0) {
+      float* st = A.stats + 2 * (row * A.G + p.group);
+      st[0] = mean;
+      st[1] = rstd;
+    }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       if (!(live && in[k])) continue;
