@@ -494,7 +494,8 @@ PRNN_API int prnn_gru_decode_x(const void* h, const void* x, const void* w, cons
  * Per head, with a state S (Dk x Dv, fp32) and a log decay g_t per token:
  *   S_t = exp(g_t) S_{t-1} + k_t v_t^T,   o_t = scale q_t^T S_t.
  * Arrays are given by strides (in elements; a head's values are contiguous) and may have fewer
- * heads than H (dividing it): consecutive heads then share one.  Tokens lie at most 16 MiB apart.
+ * heads than H (dividing it): consecutive heads then share one.  Tokens lie in ascending order, at
+ * most 16 MiB apart (stride 0: one for all).
  *
  * A batch is B sequences of T tokens, or (cu_seqlens, int32 on the device, n_seq + 1 offsets)
  * one packed stream of T tokens with B = 1; offsets outside the stream are clamped into it.

@@ -40,10 +40,8 @@ struct LaView {
   int vec;               // rows and base admit 16-byte accesses
 };
 
-// Chunks' rows are read by 32-bit offsets.
-constexpr bool la_stride_fits(long long st, int size) {
-  return (st < 0 ? -st : st) * size <= (1 << 24);
-}
+// Chunks' rows are read by unsigned 32-bit offsets from the lowest token's.
+constexpr bool la_stride_fits(long long st, int size) { return st >= 0 && st <= (1 << 24) / size; }
 
 // The decays: (B, T, H) by strides, or one per head (sb = st = 0); fp32 or the storage type.
 struct LaDecay {

@@ -306,6 +306,8 @@ LaView view(const prnn_la_view& v, const Problem& a, int D) {
   return r;
 }
 
+constexpr char kTokens[] = "tokens %lld elements apart do not lie 0 bytes to 16 MiB apart";
+
 int check(const Problem* a) {
   if (a == nullptr) return fail(PRNN_ERR_VALUE, "the problem must be non-null");
   if (int rc = check_dtype(a->dtype)) return rc;
@@ -328,9 +330,9 @@ int check(const Problem* a) {
   const int size = a->dtype == PRNN_F32 ? 4 : 2;
   for (const prnn_la_view* v : {&a->q, &a->k, &a->v})
     if (!la_stride_fits(v->st, size))
-      return fail(PRNN_ERR_VALUE, "tokens %lld elements apart are too far (16 MiB)", v->st);
+      return fail(PRNN_ERR_VALUE, kTokens, v->st);
   if (!la_stride_fits(a->g_st, 4))
-    return fail(PRNN_ERR_VALUE, "decays %lld elements apart are too far (16 MiB)", a->g_st);
+    return fail(PRNN_ERR_VALUE, "decays %lld elements apart do not lie 0 bytes to 16 MiB apart", a->g_st);
   if (!la_stride_fits(1ll * a->H * std::max(a->Dk, a->Dv), 4))
     return fail(PRNN_ERR_VALUE, "H=%d heads of (%d, %d) are too wide", a->H, a->Dk, a->Dv);
   if (a->h0 && a->h0_rows < 0) return fail(PRNN_ERR_VALUE, "h0_rows=%d", a->h0_rows);
@@ -696,7 +698,7 @@ extern "C" PRNN_API int prnn_linear_attention(const prnn_linear_attention_proble
   if (out == nullptr || (out->p == nullptr && 1ll * a->B * a->T > 0))
     return fail(PRNN_ERR_VALUE, "out must be non-null");
   if (!la_stride_fits(out->st, a->dtype == PRNN_F32 ? 4 : 2))
-    return fail(PRNN_ERR_VALUE, "tokens %lld elements apart are too far (16 MiB)", out->st);
+    return fail(PRNN_ERR_VALUE, kTokens, out->st);
   if (sequences(*a) == 0) return PRNN_OK;
   if (int rc = check_ws(need(*a, false, false), workspace, bytes)) return rc;
   return forward(*a, *out, state_out, out_table, out_rows, workspace,
@@ -717,7 +719,7 @@ extern "C" PRNN_API int prnn_linear_attention_backward(
   if (go == nullptr || (any && (!go->p || !dq || !dk || !dv)))
     return fail(PRNN_ERR_VALUE, "go, dq, dk and dv must be non-null");
   if (!la_stride_fits(go->st, a->dtype == PRNN_F32 ? 4 : 2))
-    return fail(PRNN_ERR_VALUE, "tokens %lld elements apart are too far (16 MiB)", go->st);
+    return fail(PRNN_ERR_VALUE, kTokens, go->st);
   if (a->h0_table) return fail(PRNN_ERR_VALUE, "a block table has no gradient");
   if (a->h0 && a->h0_rows < sequences(*a))
     return fail(PRNN_ERR_VALUE, "h0 has %d rows for %d sequences", a->h0_rows, sequences(*a));
