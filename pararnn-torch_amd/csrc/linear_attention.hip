@@ -306,7 +306,12 @@ LaView view(const prnn_la_view& v, const Problem& a, int D) {
   return r;
 }
 
-constexpr char kTokens[] = "tokens %lld elements apart do not lie 0 bytes to 16 MiB apart";
+// The stride of an only token is never used.
+int check_tokens(const Problem& a, long long st) {
+  if (a.T > 1 && !la_stride_fits(st, a.dtype == PRNN_F32 ? 4 : 2))
+    return fail(PRNN_ERR_VALUE, "tokens %lld elements apart do not lie 0 bytes to 16 MiB apart", st);
+  return PRNN_OK;
+}
 
 int check(const Problem* a) {
   if (a == nullptr) return fail(PRNN_ERR_VALUE, "the problem must be non-null");
@@ -327,11 +332,9 @@ int check(const Problem* a) {
   if (static_cast<long long>(a->B) * a->T > 0)
     for (const void* p : {a->q.p, a->k.p, a->v.p, a->g})
       if (p == nullptr) return fail(PRNN_ERR_VALUE, "q, k, v and log_decay must be non-null");
-  const int size = a->dtype == PRNN_F32 ? 4 : 2;
   for (const prnn_la_view* v : {&a->q, &a->k, &a->v})
-    if (!la_stride_fits(v->st, size))
-      return fail(PRNN_ERR_VALUE, kTokens, v->st);
-  if (!la_stride_fits(a->g_st, 4))
+    if (int rc = check_tokens(*a, v->st)) return rc;
+  if (a->T > 1 && !la_stride_fits(a->g_st, 4))
     return fail(PRNN_ERR_VALUE, "decays %lld elements apart do not lie 0 bytes to 16 MiB apart", a->g_st);
   if (!la_stride_fits(1ll * a->H * std::max(a->Dk, a->Dv), 4))
     return fail(PRNN_ERR_VALUE, "H=%d heads of (%d, %d) are too wide", a->H, a->Dk, a->Dv);
@@ -697,8 +700,7 @@ extern "C" PRNN_API int prnn_linear_attention(const prnn_linear_attention_proble
   if (int rc = check(a)) return rc;
   if (out == nullptr || (out->p == nullptr && 1ll * a->B * a->T > 0))
     return fail(PRNN_ERR_VALUE, "out must be non-null");
-  if (!la_stride_fits(out->st, a->dtype == PRNN_F32 ? 4 : 2))
-    return fail(PRNN_ERR_VALUE, kTokens, out->st);
+  if (int rc = check_tokens(*a, out->st)) return rc;
   if (sequences(*a) == 0) return PRNN_OK;
   if (int rc = check_ws(need(*a, false, false), workspace, bytes)) return rc;
   return forward(*a, *out, state_out, out_table, out_rows, workspace,
@@ -718,8 +720,7 @@ extern "C" PRNN_API int prnn_linear_attention_backward(
   const bool any = 1ll * a->B * a->T > 0;
   if (go == nullptr || (any && (!go->p || !dq || !dk || !dv)))
     return fail(PRNN_ERR_VALUE, "go, dq, dk and dv must be non-null");
-  if (!la_stride_fits(go->st, a->dtype == PRNN_F32 ? 4 : 2))
-    return fail(PRNN_ERR_VALUE, kTokens, go->st);
+  if (int rc = check_tokens(*a, go->st)) return rc;
   if (a->h0_table) return fail(PRNN_ERR_VALUE, "a block table has no gradient");
   if (a->h0 && a->h0_rows < sequences(*a))
     return fail(PRNN_ERR_VALUE, "h0 has %d rows for %d sequences", a->h0_rows, sequences(*a));

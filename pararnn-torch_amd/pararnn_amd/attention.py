@@ -69,14 +69,16 @@ def _tiles(t: Tensor) -> Tensor:
     that do not lie for that (a view of a fused projection with an odd offset, a row expanded over
     time) are copied."""
     sb, st, sh, sd = t.stride()
-    width = t.shape[3]
+    time, width = t.shape[1], t.shape[3]
+    if time == 1:
+        st = width  # whatever it is, the kernels do not use it
     # at most 16 MiB between tokens: the kernels' offsets inside a chunk
     if (sd != 1 and width != 1) or st > 1 << 22:
         t = t.contiguous()
         sb, st, sh, _ = t.stride()
     if t.dtype is not torch.bfloat16 or width % 8:
         return t
-    if (sb | st | sh) % 8 == 0 and t.data_ptr() % 16 == 0 and (st >= width or t.shape[1] == 1):
+    if (sb | st | sh) % 8 == 0 and t.data_ptr() % 16 == 0 and st >= width:
         return t
     return t.clone(memory_format=torch.contiguous_format)
 

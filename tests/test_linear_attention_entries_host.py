@@ -51,3 +51,10 @@ def test_tokens_in_descending_order_are_refused():
     # a problem like these, but ascending, is not refused (what fails then is the missing device)
     for call in (_forward, _backward):
         assert call(_problem()) == _lib.PRNN_ERR_RUNTIME
+
+
+def test_an_only_tokens_stride_does_not_matter():
+    far = 1 << 40
+    p = _problem(_view(st=far), _view(st=-far), _view(st=far), g_st=far, B=3, T=1)
+    for call in (_forward, _backward):
+        assert call(p, _view(st=far)) == _lib.PRNN_ERR_RUNTIME  # not refused: no device
