@@ -6,8 +6,8 @@
   back a fixed number of steps later), packed ragged sequences;
 * serving: ragged prompts in one call, their final states written to the slots of a state pool,
   then a token at a time with ``linear_attention_step``; a session is forked, others end and their
-  slots are freed, the pool is compacted, and the served tokens are checked against one pass over
-  the whole sequences.
+  slots are freed, the pool is compacted, a new session takes one of the slots, and the served tokens
+  are checked against one pass over the whole sequences.
 """
 
 from __future__ import annotations
@@ -119,8 +119,9 @@ def serve(model: Model, tokens: int, device: str, seed: int = 1, new: int = 12) 
 
     table = take_pages(used, len(lens))
     cu = torch.tensor([0, *torch.tensor(lens).cumsum(0).tolist()])
-    logits = model(torch.cat(prompts)[None].to(device), PackedSequences(cu), h0=pool,
-                   block_table=table, state_out=pool)
+    # new sessions start from zeros, whatever their slots hold, and leave their states there
+    logits = model(torch.cat(prompts)[None].to(device), PackedSequences(cu), block_table=table,
+                   state_out=pool)
     last = logits[0, cu[1:].to(device) - 1]
     texts, seen = [p.tolist() for p in prompts], [[] for _ in lens]
     for step in range(new):
@@ -136,6 +137,13 @@ def serve(model: Model, tokens: int, device: str, seed: int = 1, new: int = 12) 
             live = compact_pages(used, [pool], [table])
             assert int(live) == table.numel() and int(table.max()) < table.numel()
             texts, seen, last = texts[2:], seen[2:], last[2:]
+        if step == 9:  # another session begins, on a slot that one of those has left
+            prompt = torch.randint(0, tokens, (23,), generator=gen)
+            slot = take_pages(used, 1)
+            logits = model(prompt[None].to(device), block_table=slot, state_out=pool)
+            table, last = torch.cat([table, slot]), torch.cat([last, logits[:, -1]])
+            texts.append(prompt.tolist())
+            seen.append([])
         ids = last.argmax(-1)
         if step == 4:
             ids[-1] = (ids[-1] + 1) % tokens  # the fork goes its own way

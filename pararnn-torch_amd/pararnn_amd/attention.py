@@ -115,15 +115,15 @@ def _check_state(what: str, name: str, t: Tensor, q: Tensor, tail: tuple[int, ..
         raise ValueError(f"{what}: {name} shape {tuple(t.shape)} != {want}")
 
 
-def _check_table(what: str, table: Tensor, rows: int, dev: torch.device) -> Tensor:
+def _check_table(what: str, name: str, table: Tensor, rows: int, dev: torch.device) -> Tensor:
     if table.dim() != 1 or table.numel() != rows:
-        raise ValueError(f"{what}: block_table must be ({rows},), got {tuple(table.shape)}")
+        raise ValueError(f"{what}: {name} must be ({rows},), got {tuple(table.shape)}")
     if table.dtype == torch.int32 and table.device == dev and table.is_contiguous():
         return table
     if table.is_floating_point() or table.is_complex():
-        raise TypeError(f"{what}: block_table must be whole numbers, got {table.dtype}")
+        raise TypeError(f"{what}: {name} must be whole numbers, got {table.dtype}")
     if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError(f"{what} under graph capture needs a contiguous int32 block_table on "
+        raise RuntimeError(f"{what} under graph capture needs a contiguous int32 {name} on "
                            "the state's device")
     return table.to(device=dev, dtype=torch.int32).contiguous()
 
@@ -177,11 +177,8 @@ class _Problem:
                 raise ValueError(f"cu_seqlens[-1] must equal time={time}, got {packed.tokens}")
             self.sequences = packed.sequences
             self.offsets, self.longest = packed.offsets(q.device), packed.longest
-        self.table = None
-        if table is not None:
-            if h0 is None:
-                raise ValueError("block_table needs h0 as a pool (C, ...)")
-            self.table = _check_table(what, table, self.sequences, q.device)
+        self.table = None if table is None else _check_table(what, "block_table", table,
+                                                             self.sequences, q.device)
         self.h0 = None
         if h0 is not None:
             _check_state(what, "h0", h0, q, (heads, dk, dv),
@@ -284,6 +281,7 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, *,
                      scale: float | None = None, h0: Tensor | None = None,
                      cu_seqlens: Tensor | PackedSequences | None = None,
                      block_table: Tensor | None = None, state_out: Tensor | None = None,
+                     state_table: Tensor | None = None,
                      return_state: bool = False) -> Tensor | tuple[Tensor, Tensor]:
     """Linear attention over whole sequences; ``(B, T, H, Dv)`` in ``q``'s type.
 
@@ -299,33 +297,47 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, *,
     the output and of the returned states flow to ``q``, ``k``, ``v``, ``log_decay`` and ``h0``.
 
     Serving: with ``block_table`` ``(sequences,)`` ``h0`` is a pool ``(C, H, Dk, Dv)`` and
-    sequence ``s`` starts from row ``block_table[s]`` (a negative entry: from zeros).
-    ``state_out`` takes the final states: ``(sequences, H, Dk, Dv)``, or with a block table a pool
-    whose named rows are overwritten (``h0`` itself is allowed: no two sequences may then name
-    one row).  Neither has a gradient.
+    sequence ``s`` starts from row ``block_table[s]`` (an entry that is no row, -1: from zeros).
+    ``state_out`` takes the final states: ``(sequences, H, Dk, Dv)``, or with a table a pool whose
+    named rows are overwritten: those of ``state_table`` where given, or of ``block_table``.  A pool
+    row keeps its last session's state, so a new session's prompt goes without ``h0``
+    (``block_table=slots, state_out=pool``: zeros in, the final state to its slot), and next to
+    others that go on (``h0=pool``) has -1 in ``block_table`` and its slot in ``state_table``.
+    ``state_out`` may be ``h0`` itself if no row that one sequence writes is read or written by
+    another.  None of these has a gradient.
     """
     packed = cu_seqlens
     if packed is not None and not isinstance(packed, PackedSequences):
         packed = PackedSequences(packed)
     grads = torch.is_grad_enabled() and any(
         t is not None and t.requires_grad for t in (q, k, v, log_decay, h0))
+    if block_table is not None and h0 is None and (state_out is None or state_table is not None):
+        raise ValueError("block_table needs h0, or without a state_table state_out, as a pool "
+                         "(C, ...)")
+    if state_table is not None and state_out is None:
+        raise ValueError("state_table needs state_out as a pool (C, ...)")
     if grads and block_table is None and state_out is None:
         out, state = _LinearAttention.apply(q, k, v, log_decay, h0, packed, scale, return_state)
         return (out, state) if return_state else out
     if grads:
         raise RuntimeError("linear_attention: block_table and state_out are inference-only; call "
                            "it under torch.no_grad()")
-    p = _Problem(q, k, v, log_decay, h0, block_table, packed, scale)
+    p = _Problem(q, k, v, log_decay, h0, None if h0 is None else block_table, packed, scale)
     _, _, heads, dk, dv = p.dims
     dest, table = None, None
     if state_out is not None:
         if return_state:
             raise ValueError("linear_attention: state_out and return_state exclude each other")
+        if state_table is not None:
+            table = _check_table("linear_attention", "state_table", state_table, p.sequences, q.device)
+        elif block_table is not None:
+            table = p.table if p.table is not None else _check_table(
+                "linear_attention", "block_table", block_table, p.sequences, q.device)
         _check_state("linear_attention", "state_out", state_out, q, (heads, dk, dv),
-                     p.sequences if p.table is None else None)
+                     p.sequences if table is None else None)
         if not state_out.is_contiguous():
             raise ValueError("linear_attention: state_out must be contiguous")
-        dest, table = state_out, p.table
+        dest = state_out
     elif return_state:
         dest = q.new_empty(p.sequences, heads, dk, dv, dtype=torch.float32)
     out = _forward(p, dest, table)
@@ -384,7 +396,7 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
                  else batch)
     if not state.is_contiguous():
         raise ValueError(f"{what}: state must be contiguous (it is advanced in place)")
-    table = None if block_table is None else _check_table(what, block_table, batch, dev)
+    table = None if block_table is None else _check_table(what, "block_table", block_table, batch, dev)
     q, k, v = _rows(q), _rows(k), _rows(v)
     if out is None:
         res = q.new_empty(batch, heads, dv)

@@ -68,7 +68,10 @@ def _pools(what: str, pools: Sequence[Tensor] | Tensor, slots: int | None, dev):
 
 
 def take_pages(used: Tensor, n: int) -> Tensor:
-    """The ``n`` lowest free slots, now used, ``(n,)`` int32; -1 where none is left."""
+    """The ``n`` lowest free slots, now used, ``(n,)`` int32; -1 where none is left.  The pools are
+    not touched: a slot's rows still hold what its last session left, so a new session's prompt
+    starts without them (``linear_attention`` without ``h0``), and one that starts with a single
+    token clears them first."""
     dev = _used("take_pages", used).device
     if n < 0:
         raise ValueError(f"take_pages: n must be >= 0, got {n!r}")

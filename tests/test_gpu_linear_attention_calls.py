@@ -42,3 +42,70 @@ def test_one_token_of_a_time_major_layout(dtype):
     for x, y in zip(torch.autograd.grad(out, major, time_major(go)),
                     torch.autograd.grad(want, dense, go)):
         assert torch.equal(x, y)
+
+
+def _rel(got, want):
+    got, want = got.detach().double().cpu(), want.detach().double().cpu()
+    assert got.shape == want.shape
+    return float((got - want).norm() / want.norm())
+
+
+def _prompts(lens, dtype, H=2, D=32, seed=1):
+    n = sum(lens)
+    q, k, v = (_t(1, n, H, D, dtype=dtype, seed=seed + i, scale=0.5) for i in range(3))
+    g = -_t(1, n, H, dtype=dtype, seed=seed + 7).abs() / 4
+    cu = [0]
+    for x in lens:
+        cu.append(cu[-1] + x)
+    return q, k, v, g, cu
+
+
+@pytest.mark.parametrize("lens", [[40, 1, 90], [700, 30, 900]], ids=["whole", "cut"])
+def test_new_sessions_on_used_slots(lens):
+    """A slot keeps the state of the session that had it: a new one starts from zeros all the same, alone
+    and next to sessions that go on.  float32, the tests' tolerance of states."""
+    from pararnn_amd import free_pages, linear_attention, take_pages
+
+    q, k, v, g, cu = _prompts(lens, F32)
+    pool = _t(6, 2, 32, 32, seed=5)
+    used = torch.ones(6, dtype=torch.int32, device=DEV)
+    free_pages(used, torch.tensor([4, 1, 2]))
+    slots = take_pages(used, 3)
+    assert slots.tolist() == [1, 2, 4]
+    before = pool.clone()
+    o64, s64 = O.linear_attention(*(x.double().cpu() for x in (q, k, v, g)), cu=cu)
+    with torch.no_grad():
+        out = linear_attention(q, k, v, g, cu_seqlens=torch.tensor(cu), block_table=slots,
+                               state_out=pool)
+    assert _rel(out, o64) <= 2.7e-6 and _rel(pool[slots.long()], s64) <= 2.7e-6
+    assert torch.equal(pool[[0, 3, 5]], before[[0, 3, 5]])
+
+    # the first and the last go on, the second gives its slot to a new one; in place
+    now = pool.clone()
+    h0 = torch.stack([now[1], torch.zeros_like(now[0]), now[4]])
+    o64, s64 = O.linear_attention(*(x.double().cpu() for x in (q, k, v, g)), h0.double().cpu(), cu=cu)
+    with torch.no_grad():
+        out = linear_attention(q, k, v, g, h0=pool, cu_seqlens=torch.tensor(cu),
+                               block_table=torch.tensor([1, -1, 4]), state_out=pool,
+                               state_table=torch.tensor([1, 2, 4]))
+    assert _rel(out, o64) <= 2.7e-6 and _rel(pool[[1, 2, 4]], s64) <= 2.7e-6
+    assert torch.equal(pool[[0, 3, 5]], before[[0, 3, 5]])
+
+
+def test_state_tables_refuse():
+    from pararnn_amd import linear_attention
+
+    q, k, v, g, _ = _prompts([8], F32)
+    pool, one = _t(4, 2, 32, 32), torch.tensor([2])
+    with pytest.raises(ValueError, match="state_out"):
+        linear_attention(q, k, v, g, block_table=one)
+    with pytest.raises(ValueError, match="block_table"):
+        linear_attention(q, k, v, g, block_table=one, state_out=pool, state_table=one)
+    with pytest.raises(ValueError, match="state_out"):
+        linear_attention(q, k, v, g, h0=pool, block_table=one, state_table=one)
+    with pytest.raises(ValueError, match="state_table"):
+        linear_attention(q, k, v, g, state_out=pool, state_table=torch.tensor([1, 2]))
+    with pytest.raises(ValueError, match="state_out"):
+        linear_attention(q, k, v, g, state_out=pool)  # four rows for one sequence
+    with pytest.raises(RuntimeError, match="inference"):
+        linear_attention(q.requires_grad_(True), k, v, g, block_table=one, state_out=pool)
