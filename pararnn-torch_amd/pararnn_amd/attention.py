@@ -115,17 +115,29 @@ def _check_state(what: str, name: str, t: Tensor, q: Tensor, tail: tuple[int, ..
         raise ValueError(f"{what}: {name} shape {tuple(t.shape)} != {want}")
 
 
+_INTS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
+
+
+def _slots(what: str, name: str, t: Tensor, dev: torch.device) -> Tensor:
+    """A list of slots as the kernels read it: int32, contiguous, on ``dev``."""
+    if t.dtype not in _INTS:
+        raise TypeError(f"{what}: {name} must be whole numbers, got {t.dtype}")
+    if t.dim() != 1:
+        raise ValueError(f"{what}: {name} must be one-dimensional, got {tuple(t.shape)}")
+    if t.dtype is torch.int32 and t.device == dev and t.is_contiguous():
+        return t
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{what} under graph capture needs a contiguous int32 {name} on the "
+                           "device of what it names")
+    if t.dtype is torch.int64:
+        t = t.clamp(-1, (1 << 31) - 1)  # what int32 cannot hold names no slot either
+    return t.to(device=dev, dtype=torch.int32).contiguous()
+
+
 def _check_table(what: str, name: str, table: Tensor, rows: int, dev: torch.device) -> Tensor:
     if table.dim() != 1 or table.numel() != rows:
         raise ValueError(f"{what}: {name} must be ({rows},), got {tuple(table.shape)}")
-    if table.dtype == torch.int32 and table.device == dev and table.is_contiguous():
-        return table
-    if table.is_floating_point() or table.is_complex():
-        raise TypeError(f"{what}: {name} must be whole numbers, got {table.dtype}")
-    if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError(f"{what} under graph capture needs a contiguous int32 {name} on "
-                           "the state's device")
-    return table.to(device=dev, dtype=torch.int32).contiguous()
+    return _slots(what, name, table, dev)
 
 
 def _at(t: Tensor | None) -> int | None:

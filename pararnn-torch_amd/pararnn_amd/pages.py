@@ -20,7 +20,7 @@ import torch
 from torch import Tensor
 
 from pararnn_amd import _lib
-from pararnn_amd.attention import _enqueue
+from pararnn_amd.attention import _enqueue, _slots
 
 
 def _used(what: str, used: Tensor) -> Tensor:
@@ -31,21 +31,6 @@ def _used(what: str, used: Tensor) -> Tensor:
     if used.dim() != 1 or not used.is_contiguous():
         raise ValueError(f"{what}: used must be (slots,) and contiguous, got {tuple(used.shape)}")
     return used
-
-
-def _list(what: str, name: str, t: Tensor, dev: torch.device) -> Tensor:
-    if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
-        raise TypeError(f"{what}: {name} must be whole numbers, got {t.dtype}")
-    if t.dim() != 1:
-        raise ValueError(f"{what}: {name} must be one-dimensional, got {tuple(t.shape)}")
-    if t.dtype == torch.int32 and t.device == dev and t.is_contiguous():
-        return t
-    if torch.cuda.is_current_stream_capturing():
-        raise RuntimeError(f"{what} under graph capture needs a contiguous int32 {name} on the "
-                           "pools' device")
-    if t.dtype == torch.int64:
-        t = t.clamp(-1, (1 << 31) - 1)  # what int32 cannot hold names no slot either
-    return t.to(device=dev, dtype=torch.int32).contiguous()
 
 
 def _pools(what: str, pools: Sequence[Tensor] | Tensor, slots: int | None, dev):
@@ -88,7 +73,7 @@ def fork_pages(used: Tensor, pools: Sequence[Tensor] | Tensor, parents: Tensor) 
     which no slot is left, gets -1."""
     dev = _used("fork_pages", used).device
     rows, n_pools, _, _ = _pools("fork_pages", pools, used.shape[0], dev)
-    parents = _list("fork_pages", "parents", parents, dev)
+    parents = _slots("fork_pages", "parents", parents, dev)
     n = parents.shape[0]
     both = torch.empty(2, n, dtype=torch.int32, device=dev)
     rc = _enqueue(_lib.load().prnn_pages_fork, dev, used.data_ptr(), used.shape[0], rows, n_pools,
@@ -100,7 +85,7 @@ def fork_pages(used: Tensor, pools: Sequence[Tensor] | Tensor, parents: Tensor) 
 def free_pages(used: Tensor, slots: Tensor) -> None:
     """Gives ``slots`` ``(n,)`` back; entries that are no slots are passed over."""
     dev = _used("free_pages", used).device
-    slots = _list("free_pages", "slots", slots, dev)
+    slots = _slots("free_pages", "slots", slots, dev)
     rc = _enqueue(_lib.load().prnn_pages_free, dev, used.data_ptr(), used.shape[0],
                   slots.data_ptr(), slots.shape[0])
     _lib.check(rc, "free_pages")
@@ -112,8 +97,8 @@ def copy_pages(pools: Sequence[Tensor] | Tensor, src: Tensor, dst: Tensor) -> No
     rows, n_pools, slots, dev = _pools("copy_pages", pools, None, None)
     if dev is None:
         raise ValueError("copy_pages needs a pool")
-    src = _list("copy_pages", "src", src, dev)
-    dst = _list("copy_pages", "dst", dst, dev)
+    src = _slots("copy_pages", "src", src, dev)
+    dst = _slots("copy_pages", "dst", dst, dev)
     if src.shape != dst.shape:
         raise ValueError(f"copy_pages: src {tuple(src.shape)} != dst {tuple(dst.shape)}")
     rc = _enqueue(_lib.load().prnn_pages_copy, dev, slots, rows, n_pools, src.data_ptr(),

@@ -109,3 +109,41 @@ def test_state_tables_refuse():
         linear_attention(q, k, v, g, state_out=pool)  # four rows for one sequence
     with pytest.raises(RuntimeError, match="inference"):
         linear_attention(q.requires_grad_(True), k, v, g, block_table=one, state_out=pool)
+
+
+def test_tables_name_no_slot_beyond_32_bits():
+    """Entries of 64 bits that 32 cannot hold are idle rows, not the slot that is left of them."""
+    from pararnn_amd import linear_attention, linear_attention_step
+
+    pool = _t(6, 2, 32, 32, seed=5)
+    table = torch.tensor([(1 << 32) + 3, 2, -(1 << 40), 1 << 32])
+    q, k, v = (_t(4, 5, 2, 32, seed=i) for i in range(3))
+    g = -_t(4, 5, 2).abs()
+    for call in ("prompt", "step"):
+        mine = pool.clone()
+        with torch.no_grad():
+            if call == "prompt":
+                out = linear_attention(q, k, v, g, h0=mine, block_table=table, state_out=mine)
+                zeros = linear_attention(q, k, v, g)
+            else:
+                first = [x[:, 0] for x in (q, k, v, g)]
+                out = linear_attention_step(*first, mine, block_table=table)
+                zeros = linear_attention_step(*first, torch.zeros(4, 2, 32, 32, device=DEV))
+        assert torch.equal(out[[0, 2, 3]], zeros[[0, 2, 3]]), call
+        assert not torch.equal(mine[2], pool[2]), call
+        assert torch.equal(mine[[0, 1, 3, 4, 5]], pool[[0, 1, 3, 4, 5]]), call
+
+
+def test_masks_are_no_tables():
+    from pararnn_amd import free_pages, linear_attention, linear_attention_step
+
+    pool = _t(2, 2, 32, 32)
+    q, g = _t(2, 3, 2, 32), -_t(2, 3, 2).abs()
+    mask = torch.tensor([True, False])
+    with torch.no_grad():
+        with pytest.raises(TypeError, match="whole numbers"):
+            linear_attention(q, q, q, g, h0=pool, block_table=mask)
+        with pytest.raises(TypeError, match="whole numbers"):
+            linear_attention_step(q[:, 0], q[:, 0], q[:, 0], g[:, 0], pool, block_table=mask)
+    with pytest.raises(TypeError, match="whole numbers"):
+        free_pages(torch.ones(2, dtype=torch.int32, device=DEV), mask)
