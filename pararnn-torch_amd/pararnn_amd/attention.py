@@ -25,6 +25,7 @@ import functools
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from pararnn_amd import _lib
 from pararnn_amd.ops import _DTYPES, _validate, _workspace
@@ -56,6 +57,15 @@ def _once(fn):
         return guarded(ctx, *grads) if torch.is_grad_enabled() else fn(ctx, *grads)
 
     return backward
+
+
+def _no_tangents(what: str, *tensors: Tensor | None) -> None:
+    """Refuses forward-mode duals: the kernels would drop their tangents unnoticed."""
+    if forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what} has no forward-mode derivative")
 
 
 def _rows(t: Tensor) -> Tensor:
@@ -318,6 +328,7 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, *,
     ``state_out`` may be ``h0`` itself if no row that one sequence writes is read or written by
     another.  None of these has a gradient.
     """
+    _no_tangents("linear_attention", q, k, v, log_decay, h0)
     packed = cu_seqlens
     if packed is not None and not isinstance(packed, PackedSequences):
         packed = PackedSequences(packed)
@@ -373,6 +384,7 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or log_decay.requires_grad or state.requires_grad):
         raise RuntimeError(f"{what} has no autograd; call it under torch.no_grad()")
+    _no_tangents(what, q, k, v, log_decay, state)
     timed = q.dim() == 4
     if timed:
         if q.shape[1] != 1 or k.dim() != 4 or k.shape[1] != 1 or v.dim() != 4 or v.shape[1] != 1:

@@ -17,7 +17,7 @@ import torch
 from torch import Tensor
 
 from pararnn_amd import _lib
-from pararnn_amd.attention import _at, _enqueue, _once
+from pararnn_amd.attention import _at, _enqueue, _no_tangents, _once
 from pararnn_amd.ops import _DTYPES, _validate, _workspace
 
 _ACTIVATIONS = {None: 0, "silu": 1, "sigmoid": 2}
@@ -142,6 +142,7 @@ def group_norm(x: Tensor, num_groups: int, weight: Tensor | None = None,
     if x.numel() // c >= 1 << 31:
         raise ValueError(f"{what}: x has {x.numel() // c} tokens, more than 2^31 - 1")
 
+    _no_tangents(what, x, weight, bias, gate)
     x, gate = _flat(x), _flat(gate)
     weight = None if weight is None else weight.contiguous()
     bias = None if bias is None else bias.contiguous()

@@ -147,3 +147,23 @@ def test_masks_are_no_tables():
             linear_attention_step(q[:, 0], q[:, 0], q[:, 0], g[:, 0], pool, block_table=mask)
     with pytest.raises(TypeError, match="whole numbers"):
         free_pages(torch.ones(2, dtype=torch.int32, device=DEV), mask)
+
+
+def test_forward_mode_is_refused():
+    """A dual tensor's tangent would be dropped without a word."""
+    from torch.autograd import forward_ad
+
+    from pararnn_amd import group_norm, linear_attention, linear_attention_step
+
+    q, g, state = _t(1, 6, 2, 32), -_t(1, 6, 2).abs(), _t(1, 2, 32, 32)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(q, torch.ones_like(q))
+        for call in (lambda: linear_attention(q, dual, q, g),
+                     lambda: linear_attention(q, q, q, g, h0=forward_ad.make_dual(state, state)),
+                     lambda: linear_attention_step(dual[:, 0], q[:, 0], q[:, 0], g[:, 0], state),
+                     lambda: group_norm(dual.flatten(-2), 2),
+                     lambda: group_norm(q.flatten(-2), 2, gate=dual.flatten(-2))):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                    call()
+        assert linear_attention(q, q, q, g).shape == q.shape  # no dual among them
