@@ -68,6 +68,17 @@ def _no_tangents(what: str, *tensors: Tensor | None) -> None:
             raise RuntimeError(f"{what} has no forward-mode derivative")
 
 
+def _writes(what: str, *tensors: Tensor) -> None:
+    """Tells autograd that a call is about to write ``tensors`` in place, which it cannot see: a
+    backward pass that saved one of them must not read the new values unnoticed."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise RuntimeError(f"{what} writes in place and has no autograd; call it under "
+                                   "torch.no_grad()")
+    torch.autograd.graph.increment_version(tensors)
+
+
 def _rows(t: Tensor) -> Tensor:
     """``t`` with its heads' values side by side."""
     return t if t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
@@ -360,6 +371,7 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, *,
                      p.sequences if table is None else None)
         if not state_out.is_contiguous():
             raise ValueError("linear_attention: state_out must be contiguous")
+        _writes("linear_attention", state_out)
         dest = state_out
     elif return_state:
         dest = q.new_empty(p.sequences, heads, dk, dv, dtype=torch.float32)
@@ -430,6 +442,8 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
         if out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
             raise ValueError(f"{what}: out must be contiguous, of q's type and on its device")
         res = out
+        _writes(what, out)
+    _writes(what, state)
     rc = _enqueue(
         _lib.load().prnn_linear_attention_step, dev,
         q.data_ptr(), q.stride(0), q.stride(1), hq, k.data_ptr(), k.stride(0), k.stride(1), hk,

@@ -20,7 +20,7 @@ import torch
 from torch import Tensor
 
 from pararnn_amd import _lib
-from pararnn_amd.attention import _enqueue, _slots
+from pararnn_amd.attention import _enqueue, _slots, _writes
 
 
 def _used(what: str, used: Tensor) -> Tensor:
@@ -49,7 +49,7 @@ def _pools(what: str, pools: Sequence[Tensor] | Tensor, slots: int | None, dev):
     rows = (_lib.Pool * max(1, len(pools)))(*(
         _lib.Pool(p.data_ptr(), p.numel() // p.shape[0] * p.element_size() if p.shape[0] else 0)
         for p in pools))
-    return rows, len(pools), slots, dev
+    return pools, rows, slots, dev
 
 
 def take_pages(used: Tensor, n: int) -> Tensor:
@@ -61,6 +61,7 @@ def take_pages(used: Tensor, n: int) -> Tensor:
     if n < 0:
         raise ValueError(f"take_pages: n must be >= 0, got {n!r}")
     out = torch.empty(n, dtype=torch.int32, device=dev)
+    _writes("take_pages", used)
     rc = _enqueue(_lib.load().prnn_pages_take, dev, used.data_ptr(), used.shape[0],
                   out.data_ptr(), n)
     _lib.check(rc, "take_pages")
@@ -72,11 +73,12 @@ def fork_pages(used: Tensor, pools: Sequence[Tensor] | Tensor, parents: Tensor) 
     of the parent's row in every pool; ``(n,)`` int32.  An entry that is no slot (-1), and one for
     which no slot is left, gets -1."""
     dev = _used("fork_pages", used).device
-    rows, n_pools, _, _ = _pools("fork_pages", pools, used.shape[0], dev)
+    pools, rows, _, _ = _pools("fork_pages", pools, used.shape[0], dev)
     parents = _slots("fork_pages", "parents", parents, dev)
+    _writes("fork_pages", used, *pools)
     n = parents.shape[0]
     both = torch.empty(2, n, dtype=torch.int32, device=dev)
-    rc = _enqueue(_lib.load().prnn_pages_fork, dev, used.data_ptr(), used.shape[0], rows, n_pools,
+    rc = _enqueue(_lib.load().prnn_pages_fork, dev, used.data_ptr(), used.shape[0], rows, len(pools),
                   parents.data_ptr(), both.data_ptr(), n, both.data_ptr() + 4 * n)
     _lib.check(rc, "fork_pages")
     return both[0]
@@ -86,6 +88,7 @@ def free_pages(used: Tensor, slots: Tensor) -> None:
     """Gives ``slots`` ``(n,)`` back; entries that are no slots are passed over."""
     dev = _used("free_pages", used).device
     slots = _slots("free_pages", "slots", slots, dev)
+    _writes("free_pages", used)
     rc = _enqueue(_lib.load().prnn_pages_free, dev, used.data_ptr(), used.shape[0],
                   slots.data_ptr(), slots.shape[0])
     _lib.check(rc, "free_pages")
@@ -94,14 +97,15 @@ def free_pages(used: Tensor, slots: Tensor) -> None:
 def copy_pages(pools: Sequence[Tensor] | Tensor, src: Tensor, dst: Tensor) -> None:
     """Row ``dst[i]`` of every pool gets row ``src[i]``.  No ``dst`` may be another entry's ``src``
     or ``dst``; an entry with either outside the pool is passed over."""
-    rows, n_pools, slots, dev = _pools("copy_pages", pools, None, None)
+    pools, rows, slots, dev = _pools("copy_pages", pools, None, None)
     if dev is None:
         raise ValueError("copy_pages needs a pool")
     src = _slots("copy_pages", "src", src, dev)
     dst = _slots("copy_pages", "dst", dst, dev)
     if src.shape != dst.shape:
         raise ValueError(f"copy_pages: src {tuple(src.shape)} != dst {tuple(dst.shape)}")
-    rc = _enqueue(_lib.load().prnn_pages_copy, dev, slots, rows, n_pools, src.data_ptr(),
+    _writes("copy_pages", *pools)
+    rc = _enqueue(_lib.load().prnn_pages_copy, dev, slots, rows, len(pools), src.data_ptr(),
                   dst.data_ptr(), src.shape[0])
     _lib.check(rc, "copy_pages")
 
@@ -115,7 +119,7 @@ def compact_pages(used: Tensor, pools: Sequence[Tensor] | Tensor,
     stays."""
     what = "compact_pages"
     dev = _used(what, used).device
-    rows, n_pools, _, _ = _pools(what, pools, used.shape[0], dev)
+    pools, rows, _, _ = _pools(what, pools, used.shape[0], dev)
     tables = [tables] if isinstance(tables, Tensor) else list(tables)
     for t in tables:
         if t.device != dev:
@@ -124,11 +128,12 @@ def compact_pages(used: Tensor, pools: Sequence[Tensor] | Tensor,
             raise TypeError(f"{what}: tables must be int32, got {t.dtype}")
         if not t.is_contiguous():
             raise ValueError(f"{what}: tables must be contiguous (they are changed in place)")
+    _writes(what, used, *pools, *tables)
     n = len(tables)
     scratch = torch.empty(2 + 2 * used.shape[0], dtype=torch.int32, device=dev)
     ptrs = (ctypes.c_void_p * max(1, n))(*(t.data_ptr() for t in tables))
     lens = (ctypes.c_int * max(1, n))(*(t.numel() for t in tables))
     rc = _enqueue(_lib.load().prnn_pages_compact, dev, used.data_ptr(), used.shape[0], rows,
-                  n_pools, ptrs, lens, n, scratch.data_ptr(), scratch.data_ptr() + 4)
+                  len(pools), ptrs, lens, n, scratch.data_ptr(), scratch.data_ptr() + 4)
     _lib.check(rc, what)
     return scratch[0]

@@ -167,3 +167,42 @@ def test_forward_mode_is_refused():
                 with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
                     call()
         assert linear_attention(q, q, q, g).shape == q.shape  # no dual among them
+
+
+def test_writes_in_place_are_seen_by_autograd():
+    """What saved a state that a call then overwrites refuses its backward pass; what a call would write
+    in place does not require a gradient."""
+    from pararnn_amd import (compact_pages, copy_pages, fork_pages, free_pages, linear_attention,
+                             linear_attention_step, take_pages)
+
+    q, g = _t(2, 6, 2, 32), -_t(2, 6, 2).abs()
+    one, first = torch.tensor([0]), [q[:, 0], q[:, 0], q[:, 0], g[:, 0]]
+    dest = torch.empty(2, 2, 32, device=DEV)
+    used = torch.ones(2, dtype=torch.int32, device=DEV)
+    used[1] = 0
+
+    def writers(state, used):
+        return {
+            "prompt": lambda: linear_attention(q, q, q, g, state_out=state),
+            "step": lambda: linear_attention_step(*first, state),
+            "fork": lambda: fork_pages(used, state, one),
+            "copy": lambda: copy_pages(state, one, one + 1),
+            "compact": lambda: compact_pages(used, state)}
+
+    for name in writers(None, None):
+        leaf = q.clone().requires_grad_(True)
+        state = _t(2, 2, 32, 32)
+        y = linear_attention(leaf, q, q, g, h0=state).square().sum()
+        with torch.no_grad():
+            writers(state, used.clone())[name]()
+        with pytest.raises(RuntimeError, match="inplace"):
+            y.backward()
+        with pytest.raises(RuntimeError, match="no_grad"):
+            writers(_t(2, 2, 32, 32).requires_grad_(True), used.clone())[name]()
+    table = torch.zeros(1, dtype=torch.int32, device=DEV)
+    for t, call in ((dest, lambda: linear_attention_step(*first, _t(2, 2, 32, 32), out=dest)),
+                    (used, lambda: take_pages(used, 1)), (used, lambda: free_pages(used, one)),
+                    (table, lambda: compact_pages(used, _t(2, 3), table))):
+        before = t._version
+        call()
+        assert t._version > before
