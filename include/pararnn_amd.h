@@ -586,7 +586,8 @@ typedef struct prnn_pool {
 /* out[i] for i < n: the i-th lowest free slot, now used; -1 where none is left. */
 PRNN_API int prnn_pages_take(int* used, int slots, int* out, int n, void* stream);
 /* out[i]: a free slot (lowest first), now used, with a copy of slot parents[i] in every pool; -1
- * where the parent is none or no slot is left.  scratch: n ints. */
+ * where the parent is none in use or no slot is left.  parents, out and scratch (n ints) do not
+ * overlap. */
 PRNN_API int prnn_pages_fork(int* used, int slots, const prnn_pool* pools, int n_pools,
                              const int* parents, int* out, int n, int* scratch, void* stream);
 PRNN_API int prnn_pages_free(int* used, int slots, const int* list, int n, void* stream);

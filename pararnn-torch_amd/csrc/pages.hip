@@ -73,17 +73,21 @@ __global__ __launch_bounds__(kPlan) void pages_take_kernel(int* used, int slots,
   for (int i = got + threadIdx.x; i < n; i += kPlan) out[i] = -1;
 }
 
-// scratch: the slots taken, in order.
+// scratch: the slots taken, in order.  A parent is a slot in use before the call: a free one could be
+// handed out as another entry's child and be read and written by one launch.
 __global__ __launch_bounds__(kPlan) void pages_fork_kernel(int* used, int slots,
                                                            const int* __restrict__ parents,
                                                            int* out, int n, int* scratch) {
   __shared__ int lds[kPlan / 64];
-  // how many entries have a parent
+  // how many entries have a parent (0 in out until they are told their child)
   int want = 0;
   for (int base = 0; base < n; base += kPlan) {
     const int i = base + threadIdx.x;
+    const int p = i < n ? parents[i] : -1;
+    const bool has = p >= 0 && p < slots && used[p] != 0;
+    if (i < n) out[i] = has ? 0 : -1;
     int total;
-    block_rank(i < n && parents[i] >= 0 && parents[i] < slots, lds, total);
+    block_rank(has, lds, total);
     want += total;
   }
   const int got = take_lowest(used, slots, scratch, want, lds);
@@ -91,10 +95,10 @@ __global__ __launch_bounds__(kPlan) void pages_fork_kernel(int* used, int slots,
   int first = 0;
   for (int base = 0; base < n; base += kPlan) {
     const int i = base + threadIdx.x;
-    const bool has = i < n && parents[i] >= 0 && parents[i] < slots;
+    const bool has = i < n && out[i] == 0;
     int total;
     const int rank = block_rank(has, lds, total) + first;
-    if (i < n) out[i] = has && rank < got ? scratch[rank] : -1;
+    if (has) out[i] = rank < got ? scratch[rank] : -1;
     first += total;
   }
 }

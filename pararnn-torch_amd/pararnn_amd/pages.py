@@ -70,8 +70,8 @@ def take_pages(used: Tensor, n: int) -> Tensor:
 
 def fork_pages(used: Tensor, pools: Sequence[Tensor] | Tensor, parents: Tensor) -> Tensor:
     """For every entry of ``parents`` ``(n,)`` a free slot of its own, lowest first, holding a copy
-    of the parent's row in every pool; ``(n,)`` int32.  An entry that is no slot (-1), and one for
-    which no slot is left, gets -1."""
+    of the parent's row in every pool; ``(n,)`` int32.  An entry that is no slot in use (-1, a free
+    one), and one for which no slot is left, gets -1."""
     dev = _used("fork_pages", used).device
     pools, rows, _, _ = _pools("fork_pages", pools, used.shape[0], dev)
     parents = _slots("fork_pages", "parents", parents, dev)
