@@ -595,8 +595,8 @@ PRNN_API int prnn_pages_free(int* used, int slots, const int* list, int n, void*
 PRNN_API int prnn_pages_copy(int slots, const prnn_pool* pools, int n_pools, const int* src,
                              const int* dst, int n, void* stream);
 /* The live slots move into the lowest ones: the i-th lowest free slot below their number gets the
- * i-th lowest live one above it.  tables[k] (lens[k] entries, in place): live slots become their
- * new places, free ones -1.  live: their number (one int).  scratch: 2 slots + 1 ints. */
+ * i-th lowest live one above it.  tables[k] (lens[k] entries, in place, none overlapping another):
+ * live slots become their new places, free ones -1.  live: their number (one int).  scratch: 2 slots + 1 ints. */
 PRNN_API int prnn_pages_compact(int* used, int slots, const prnn_pool* pools, int n_pools,
                                 int* const* tables, const int* lens, int n_tables, int* live,
                                 int* scratch, void* stream);

@@ -128,11 +128,15 @@ def compact_pages(used: Tensor, pools: Sequence[Tensor] | Tensor,
             raise TypeError(f"{what}: tables must be int32, got {t.dtype}")
         if not t.is_contiguous():
             raise ValueError(f"{what}: tables must be contiguous (they are changed in place)")
+    # a table given twice is one table: renamed twice, its moved entries would name free slots
+    spans = sorted({(t.data_ptr(), t.numel()) for t in tables if t.numel()})
+    if any(a + 4 * n > b for (a, n), (b, _) in zip(spans, spans[1:])):
+        raise ValueError(f"{what}: tables must not overlap")
     _writes(what, used, *pools, *tables)
-    n = len(tables)
+    n = len(spans)
     scratch = torch.empty(2 + 2 * used.shape[0], dtype=torch.int32, device=dev)
-    ptrs = (ctypes.c_void_p * max(1, n))(*(t.data_ptr() for t in tables))
-    lens = (ctypes.c_int * max(1, n))(*(t.numel() for t in tables))
+    ptrs = (ctypes.c_void_p * max(1, n))(*(p for p, _ in spans))
+    lens = (ctypes.c_int * max(1, n))(*(k for _, k in spans))
     rc = _enqueue(_lib.load().prnn_pages_compact, dev, used.data_ptr(), used.shape[0], rows,
                   len(pools), ptrs, lens, n, scratch.data_ptr(), scratch.data_ptr() + 4)
     _lib.check(rc, what)

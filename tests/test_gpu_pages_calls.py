@@ -33,3 +33,20 @@ def test_free_slots_have_no_children(slots, n):
         if k >= 0:
             want[k] = pool[p]
     assert torch.equal(data.cpu(), want)
+
+
+def test_one_table_of_several_layers():
+    """The same table for every layer is renamed once; tables that share a part are refused."""
+    from pararnn_amd import compact_pages
+
+    used = torch.tensor([0, 1, 0, 1, 1, 0], dtype=torch.int32, device=DEV)
+    pool = torch.arange(6.0, device=DEV)[:, None].repeat(1, 8)
+    table = torch.tensor([4, 1, 3], dtype=torch.int32, device=DEV)
+    assert int(compact_pages(used, pool, [table, table, table.view(3, 1)])) == 3
+    assert sorted(table.tolist()) == [0, 1, 2]
+    assert pool[table.long(), 0].tolist() == [4.0, 1.0, 3.0]
+    both = torch.tensor([0, 1, 2, 2], dtype=torch.int32, device=DEV)
+    with pytest.raises(ValueError, match="overlap"):
+        compact_pages(used, pool, [both[:3], both[2:]])
+    compact_pages(used, pool, [both[:2], both[2:], both[:0]])
+    assert both.tolist() == [0, 1, 2, 2]
