@@ -34,7 +34,7 @@ from torch import Tensor, nn
 
 from pararnn_amd.config import NewtonConfig, NewtonStats
 from pararnn_amd.newton import newton_apply
-from pararnn_amd.ragged import validate_cu_seqlens
+from pararnn_amd.ragged import PackedSequences, validate_cu_seqlens
 from pararnn_amd.sequential import sequential_apply
 
 log = logging.getLogger("pararnn_amd.layers")
@@ -249,7 +249,7 @@ class ParaRNN(nn.Module):
         self,
         x: Tensor,
         h0: Tensor | Sequence[Tensor] | None = None,
-        cu_seqlens: Tensor | None = None,
+        cu_seqlens: Tensor | PackedSequences | None = None,
     ) -> Tensor | tuple[Tensor, Tensor]:
         """``output`` (and, with ``return_hidden``, the final layer's last state)."""
         shapes = [CellShape.of(c) for c in self.layers]
@@ -265,7 +265,8 @@ class ParaRNN(nn.Module):
         if cu_seqlens is not None:
             if rows != 1:
                 raise ValueError(f"cu_seqlens needs x packed as batch 1, got batch {rows}")
-            packed = validate_cu_seqlens(cu_seqlens, seq.shape[1])
+            on = seq.device if isinstance(cu_seqlens, PackedSequences) else None
+            packed = validate_cu_seqlens(cu_seqlens, seq.shape[1], on)
             rows = int(packed.numel()) - 1
         starts = self._initial_states(h0, rows, shapes)
 

@@ -36,6 +36,7 @@ from torch import Tensor, nn
 from pararnn_amd import determinism, ops
 from pararnn_amd.cells import SLSTM_HIDDEN, ParaGRU, ParaSLSTM
 from pararnn_amd.ragged import (
+    PackedSequences,
     RaggedPlan,
     gather_h0,
     packed_in_kernel,
@@ -444,7 +445,7 @@ def newton_apply(
     *,
     h0: Tensor | None = None,
     stats: NewtonStats | None = None,
-    cu_seqlens: Tensor | None = None,
+    cu_seqlens: Tensor | PackedSequences | None = None,
     block_table: Tensor | None = None,
 ) -> Tensor:
     """Solve ``F(H) = 0`` with Newton + parallel scan on the GPU (newton/__init__.py:212-324).
@@ -461,6 +462,8 @@ def newton_apply(
         )
     if cu_seqlens is not None:
         _check_ragged_args(x, config)
+        if isinstance(cu_seqlens, PackedSequences):
+            cu_seqlens = validate_cu_seqlens(cu_seqlens, x.shape[1], x.device)
     config = _resolve_backend(cell, x, config)
     params = tuple(cell.parameters())
     needs_grad = torch.is_grad_enabled() and (

@@ -56,11 +56,21 @@ def packed_in_kernel() -> bool:
     return os.environ.get("PARARNN_AMD_PACKED", "1") != "0"
 
 
-def validate_cu_seqlens(cu_seqlens: Tensor, time: int,
+def validate_cu_seqlens(cu_seqlens: Tensor | PackedSequences, time: int,
                         device: torch.device | None = None) -> Tensor:
     """``(S+1,)`` exclusive prefix with ``[0] = 0``, last = ``time``, strictly increasing
-    (layout.py:93-104); returned as int64 on ``device`` (default: where it is)."""
+    (layout.py:93-104); returned as int64 on ``device`` (default: where it is; a handle's: the
+    host)."""
     global _checked
+    if isinstance(cu_seqlens, PackedSequences):
+        if cu_seqlens.tokens != time:
+            raise ValueError(f"cu_seqlens[-1] must equal time={time}, got {cu_seqlens.tokens}")
+        if cu_seqlens.shortest < 1:
+            raise ValueError("cu_seqlens must be strictly increasing")
+        cs = cu_seqlens.offsets(device or torch.device("cpu"), torch.long)
+        if not _known(_checked, cs, time):
+            _checked = ((weakref.ref(cs), cs._version),), int(time), cu_seqlens.longest
+        return cs
     if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 2:
         raise ValueError(f"cu_seqlens must be (S+1,), got {tuple(cu_seqlens.shape)}")
     cs = cu_seqlens.to(dtype=torch.long, device=device or cu_seqlens.device)
@@ -90,7 +100,9 @@ class PackedSequences:
     to copy the offsets from the device to look at them.
 
     ``cu_seqlens`` ``(S+1,)``: ``[0] = 0``, none below the one before it (a sequence may be
-    empty); on the host or on a GPU.  The handle keeps int32 copies on the devices that used it.
+    empty; the recurrent cells refuse such a batch); on the host or on a GPU.  The handle keeps
+    copies on the devices that used it; a captured graph reads them, so it must not outlive the
+    handle.
     """
 
     def __init__(self, cu_seqlens: Tensor):
@@ -107,18 +119,21 @@ class PackedSequences:
             raise ValueError(f"a packed batch holds fewer than 2^30 tokens, got {int(host[-1])}")
         self.sequences = int(host.numel()) - 1
         self.tokens = int(host[-1])
-        self.longest = int((host[1:] - host[:-1]).max())
-        self._on = {torch.device("cpu"): host.to(torch.int32)}
-        self._streams: set[tuple[int, int]] = set()  # (device index, stream) that use a copy
+        lengths = host[1:] - host[:-1]
+        self.longest, self.shortest = int(lengths.max()), int(lengths.min())
+        cpu = torch.device("cpu")
+        self._on = {(cpu, torch.int32): host.to(torch.int32), (cpu, torch.long): host.clone()}
+        # (device index, type, stream) that use a copy
+        self._streams: set[tuple[int, torch.dtype, int]] = set()
 
-    def offsets(self, device: torch.device) -> Tensor:
-        """The int32 offsets on ``device``, for work on its current stream."""
-        got = self._on.get(device)
+    def offsets(self, device: torch.device, dtype: torch.dtype = torch.int32) -> Tensor:
+        """The offsets (int32 or int64) on ``device``, for work on its current stream."""
+        got = self._on.get((device, dtype))
         if got is None:
-            got = self._on[device] = self._on[torch.device("cpu")].to(device)
+            got = self._on[device, dtype] = self._on[torch.device("cpu"), dtype].to(device)
         if device.type == "cuda":
             index = got.device.index
-            key = index, torch._C._cuda_getCurrentRawStream(index)
+            key = index, dtype, torch._C._cuda_getCurrentRawStream(index)
             if key not in self._streams and not torch.cuda.is_current_stream_capturing():
                 # the copy is the handle's own: its memory must outlast this stream's work on it
                 # even where the program drops the handle first
