@@ -411,6 +411,14 @@ __device__ __forceinline__ SamplePlace sample_place(const NormArgs& A) {
   return p;
 }
 
+// Rows of a strip: unsigned, so that a step behind the last of 2^31 - 1 does not wrap.
+__device__ __forceinline__ unsigned strip_begin(const NormArgs& A, int strip) {
+  return static_cast<unsigned>(strip) * A.strip_rows;
+}
+__device__ __forceinline__ unsigned strip_end(const NormArgs& A, unsigned begin) {
+  return min(static_cast<unsigned>(A.L), begin + A.strip_rows);
+}
+
 // Sum over a workgroup of 256 (every thread gets it).
 __device__ __forceinline__ float block_sum(float v, float* red) {
 #pragma unroll
@@ -436,7 +444,7 @@ __global__ __launch_bounds__(256) void norm_sample_stats_kernel(NormArgs A) {
   extern __shared__ float lds[];  // [256][2 V] mean and squared deviations per thread
   const int n = blockIdx.x / A.strips, strip = blockIdx.x - n * A.strips;
   const SamplePlace p = sample_place<V>(A);
-  const int l0 = strip * A.strip_rows, l1 = min(A.L, l0 + A.strip_rows);
+  const unsigned l0 = strip_begin(A, strip), l1 = strip_end(A, l0);
   const T* x = static_cast<const T*>(A.x) + static_cast<size_t>(n) * A.L * A.C;
   float* out = A.part + (static_cast<size_t>(n) * A.strips + strip) * A.G * 2;
   // slots beyond 256 in rounds, a whole number of groups each
@@ -448,7 +456,7 @@ __global__ __launch_bounds__(256) void norm_sample_stats_kernel(NormArgs A) {
       // a group wider than the workgroup: its channels in turns, two passes over the strip
       const size_t c0 = static_cast<size_t>(g0) * A.Cg;
       float s = 0.0f;
-      for (int l = l0; l < l1; ++l)
+      for (unsigned l = l0; l < l1; ++l)
         for (int u = threadIdx.x; u < per_group; u += 256) {
           float v[V];
           loadv<T, V>(x + static_cast<size_t>(l) * A.C + c0 + u * V, v);
@@ -458,7 +466,7 @@ __global__ __launch_bounds__(256) void norm_sample_stats_kernel(NormArgs A) {
       const float cnt = static_cast<float>(l1 - l0) * A.Cg;
       const float mean = block_sum(s, lds) / cnt;
       s = 0.0f;
-      for (int l = l0; l < l1; ++l)
+      for (unsigned l = l0; l < l1; ++l)
         for (int u = threadIdx.x; u < per_group; u += 256) {
           float v[V];
           loadv<T, V>(x + static_cast<size_t>(l) * A.C + c0 + u * V, v);
@@ -480,7 +488,7 @@ __global__ __launch_bounds__(256) void norm_sample_stats_kernel(NormArgs A) {
     for (int i = 0; i < V; ++i) mean[i] = m2[i] = 0.0f;
     float cnt = 0.0f;
     if (on)
-      for (int l = l0 + p.row; l < l1; l += 2 * kRows * p.rows_per) {
+      for (unsigned l = l0 + p.row; l < l1; l += 2 * kRows * p.rows_per) {
         // one array alone: twice the rows for as many bytes under way
         float v[2 * kRows][V];
 #pragma unroll
@@ -509,13 +517,14 @@ __global__ __launch_bounds__(256) void norm_sample_stats_kernel(NormArgs A) {
     // some lanes per group: the mean of the means, then the deviations from it
     const int items = per_group * p.rows_per, lanes = lanes_for(items);
     const int lane = threadIdx.x & (lanes - 1);
-    const float total = static_cast<float>(l1 - l0) * A.Cg;
+    const int n_rows = l1 - l0;
+    const float total = static_cast<float>(n_rows) * A.Cg;
     for (int at = 0; at < gn; at += 256 / lanes) {
       const int g = at + threadIdx.x / lanes, n_items = g < gn ? items : 0;
       float s = 0.0f;
       for (int it = lane; it < n_items; it += lanes) {
         const int r = it / per_group, u = g * per_group + it - r * per_group;
-        const float c = static_cast<float>((l1 - l0 - r + p.rows_per - 1) / p.rows_per);
+        const float c = static_cast<float>((n_rows - r + p.rows_per - 1) / p.rows_per);
         const float* e = &lds[(r * (p.slots <= 256 ? p.slots : 0) + u) * 2 * V];
 #pragma unroll
         for (int i = 0; i < V; ++i) s = fmaf(c, e[2 * i], s);
@@ -525,7 +534,7 @@ __global__ __launch_bounds__(256) void norm_sample_stats_kernel(NormArgs A) {
       s = 0.0f;
       for (int it = lane; it < n_items; it += lanes) {
         const int r = it / per_group, u = g * per_group + it - r * per_group;
-        const float c = static_cast<float>((l1 - l0 - r + p.rows_per - 1) / p.rows_per);
+        const float c = static_cast<float>((n_rows - r + p.rows_per - 1) / p.rows_per);
         const float* e = &lds[(r * (p.slots <= 256 ? p.slots : 0) + u) * 2 * V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -615,7 +624,7 @@ __global__ __launch_bounds__(256) void norm_sample_apply_kernel(NormArgs A) {
     }
     __syncthreads();
   }
-  const int l0 = strip * A.strip_rows, l1 = min(A.L, l0 + A.strip_rows);
+  const unsigned l0 = strip_begin(A, strip), l1 = strip_end(A, l0);
   const size_t base = static_cast<size_t>(n) * A.L * A.C;
   if (!p.on) return;
   for (int slot = p.slot; slot < p.slots; slot += 256) {
@@ -626,11 +635,11 @@ __global__ __launch_bounds__(256) void norm_sample_apply_kernel(NormArgs A) {
     params<T, V>(A.w, A.w_f32, A.w_vec, c, 1.0f, w);
     params<T, V>(A.b, A.w_f32, A.w_vec, c, 0.0f, b);
     // kRows rows under way at a time
-    for (int l = l0 + p.row; l < l1; l += kRows * p.rows_per) {
+    for (unsigned l = l0 + p.row; l < l1; l += kRows * p.rows_per) {
       float x[kRows][V], gt[kRows][V];
 #pragma unroll
       for (int k = 0; k < kRows; ++k) {
-        const int r = min(l + k * p.rows_per, l1 - 1);
+        const unsigned r = min(l + k * p.rows_per, l1 - 1);
         const size_t at = base + static_cast<size_t>(r) * A.C + c;
         loadv<T, V>(static_cast<const T*>(A.x) + at, x[k]);
         if (A.gate) loadv<T, V>(static_cast<const T*>(A.gate) + at, gt[k]);
@@ -661,7 +670,7 @@ __global__ __launch_bounds__(256) void norm_sample_bwd_sums_kernel(NormArgs A) {
   __shared__ float s_ch[JOIN ? 2 * 256 * V : 2];
   const int n = blockIdx.x / A.strips, strip = blockIdx.x - n * A.strips;
   const SamplePlace p = sample_place<V>(A);
-  const int l0 = strip * A.strip_rows, l1 = min(A.L, l0 + A.strip_rows);
+  const unsigned l0 = strip_begin(A, strip), l1 = strip_end(A, l0);
   const size_t base = static_cast<size_t>(n) * A.L * A.C;
   float* out = A.part + (static_cast<size_t>(n) * A.strips + strip) * 2 * A.C;
   for (int s0 = 0; s0 < p.slots; s0 += 256) {
@@ -676,11 +685,11 @@ __global__ __launch_bounds__(256) void norm_sample_bwd_sums_kernel(NormArgs A) {
 #pragma unroll
     for (int i = 0; i < V; ++i) dw[i] = db[i] = 0.0f;
     if (on)
-      for (int l = l0 + p.row; l < l1; l += kRows * p.rows_per) {
+      for (unsigned l = l0 + p.row; l < l1; l += kRows * p.rows_per) {
         float xs[kRows][V], gs[kRows][V], ys[kRows][V];
 #pragma unroll
         for (int k = 0; k < kRows; ++k) {
-          const int r = min(l + k * p.rows_per, l1 - 1);
+          const unsigned r = min(l + k * p.rows_per, l1 - 1);
           const size_t at = base + static_cast<size_t>(r) * A.C + c;
           loadv<T, V>(static_cast<const T*>(A.x) + at, xs[k]);
           loadv<T, V>(static_cast<const T*>(A.gy) + at, ys[k]);
@@ -829,7 +838,7 @@ __global__ __launch_bounds__(256) void norm_sample_dx_kernel(NormArgs A) {
     }
     __syncthreads();
   }
-  const int l0 = strip * A.strip_rows, l1 = min(A.L, l0 + A.strip_rows);
+  const unsigned l0 = strip_begin(A, strip), l1 = strip_end(A, l0);
   const size_t base = static_cast<size_t>(n) * A.L * A.C;
   if (!p.on) return;
   for (int slot = p.slot; slot < p.slots; slot += 256) {
@@ -840,11 +849,11 @@ __global__ __launch_bounds__(256) void norm_sample_dx_kernel(NormArgs A) {
     float w[V], b[V];
     params<T, V>(A.w, A.w_f32, A.w_vec, c, 1.0f, w);
     params<T, V>(A.b, A.w_f32, A.w_vec, c, 0.0f, b);
-    for (int l = l0 + p.row; l < l1; l += kRows * p.rows_per) {
+    for (unsigned l = l0 + p.row; l < l1; l += kRows * p.rows_per) {
       float xs[kRows][V], gs[kRows][V], ys[kRows][V];
 #pragma unroll
       for (int k = 0; k < kRows; ++k) {
-        const int r = min(l + k * p.rows_per, l1 - 1);
+        const unsigned r = min(l + k * p.rows_per, l1 - 1);
         const size_t at = base + static_cast<size_t>(r) * A.C + c;
         loadv<T, V>(static_cast<const T*>(A.x) + at, xs[k]);
         loadv<T, V>(static_cast<const T*>(A.gy) + at, ys[k]);
@@ -905,7 +914,7 @@ Plan plan(int N, int L, int Cg, int G, int dtype, uintptr_t bits, bool backward)
     const int per_row = G * p.lanes;
     const int rows_per = per_row <= 256 ? 256 / per_row : 1;
     p.blocks_y = (per_row + 255) / 256;
-    const int need = (N + rows_per - 1) / rows_per;
+    const int need = static_cast<int>((1ll * N + rows_per - 1) / rows_per);
     // A workgroup reads its parameters once (backward: keeps their sums) and goes on from row to
     // row: about eight a CU forward, four backward, where a partial sum each is written.  A training
     // step of 16384 tokens of 1024 channels: 63 us, with half as many 70, with twice as many 67.
@@ -917,8 +926,8 @@ Plan plan(int N, int L, int Cg, int G, int dtype, uintptr_t bits, bool backward)
   // 42 us for a training step of 8 x 2047 tokens of 256 channels; 256: 45; 1024: 52.
   const int slots = G * Cg / p.V, rows_per = slots <= 256 ? 256 / slots : 1;
   const int want = std::max(1, 512 / std::max(1, N));
-  p.strip_rows = std::max((L + want - 1) / want, kRows * rows_per);
-  p.strips = (L + p.strip_rows - 1) / p.strip_rows;
+  p.strip_rows = std::max(static_cast<int>((1ll * L + want - 1) / want), kRows * rows_per);
+  p.strips = static_cast<int>((1ll * L + p.strip_rows - 1) / p.strip_rows);
   return p;
 }
 
