@@ -577,7 +577,8 @@ PRNN_API int prnn_group_norm_backward(const void* gy, const void* x, const void*
 /* ---- Pages of a state cache ------------------------------------------------
  * A cache is one or several pools whose rows 0 .. slots - 1 belong together (a slot), and used
  * (slots) int32: 0 = free.  Lists are int32 on the device; entries outside 0 .. slots - 1 are
- * passed over.  Everything stays on the device: nothing waits for the host. */
+ * passed over.  At most 2^30 slots and entries of a list.  Everything stays on the device: nothing
+ * waits for the host. */
 typedef struct prnn_pool {
   void* p;
   long long row_bytes;

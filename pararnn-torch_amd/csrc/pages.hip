@@ -223,6 +223,9 @@ __global__ __launch_bounds__(256) void pages_move_kernel(Pools P, Tables T, int 
   }
 }
 
+// Entries of lists, as of slots: a workgroup's step past the last does not wrap.
+bool list_fits(int n) { return n >= 0 && n <= (1 << 30); }
+
 int check_cache(const char* what, const int* used, int slots, const prnn_pool* pools,
                 int n_pools) {
   if (slots < 0 || slots > (1 << 30))
@@ -276,7 +279,7 @@ using namespace prnn;
 
 extern "C" PRNN_API int prnn_pages_take(int* used, int slots, int* out, int n, void* stream) {
   if (int rc = check_cache("pages_take", used, slots, nullptr, 0)) return rc;
-  if (n < 0 || (n > 0 && out == nullptr)) return fail(PRNN_ERR_VALUE, "pages_take: n=%d", n);
+  if (!list_fits(n) || (n > 0 && out == nullptr)) return fail(PRNN_ERR_VALUE, "pages_take: n=%d", n);
   if (n == 0) return PRNN_OK;
   pages_take_kernel<<<1, kPlan, 0, static_cast<hipStream_t>(stream)>>>(used, slots, out, n);
   PRNN_HIP(hipGetLastError());
@@ -287,8 +290,8 @@ extern "C" PRNN_API int prnn_pages_fork(int* used, int slots, const prnn_pool* p
                                         const int* parents, int* out, int n, int* scratch,
                                         void* stream) {
   if (int rc = check_cache("pages_fork", used, slots, pools, n_pools)) return rc;
-  if (n < 0 || (n > 0 && (!parents || !out || !scratch)))
-    return fail(PRNN_ERR_VALUE, "pages_fork: parents, out and scratch must be non-null");
+  if (!list_fits(n) || (n > 0 && (!parents || !out || !scratch)))
+    return fail(PRNN_ERR_VALUE, "pages_fork: n=%d, parents, out and scratch must be non-null", n);
   if (n == 0) return PRNN_OK;
   const hipStream_t st = static_cast<hipStream_t>(stream);
   pages_fork_kernel<<<1, kPlan, 0, st>>>(used, slots, parents, out, n, scratch);
@@ -299,7 +302,7 @@ extern "C" PRNN_API int prnn_pages_fork(int* used, int slots, const prnn_pool* p
 extern "C" PRNN_API int prnn_pages_free(int* used, int slots, const int* list, int n,
                                         void* stream) {
   if (int rc = check_cache("pages_free", used, slots, nullptr, 0)) return rc;
-  if (n < 0 || (n > 0 && list == nullptr)) return fail(PRNN_ERR_VALUE, "pages_free: n=%d", n);
+  if (!list_fits(n) || (n > 0 && list == nullptr)) return fail(PRNN_ERR_VALUE, "pages_free: n=%d", n);
   if (n == 0) return PRNN_OK;
   pages_free_kernel<<<(n + 255) / 256, 256, 0, static_cast<hipStream_t>(stream)>>>(used, slots,
                                                                                   list, n);
@@ -311,8 +314,8 @@ extern "C" PRNN_API int prnn_pages_copy(int slots, const prnn_pool* pools, int n
                                         const int* src, const int* dst, int n, void* stream) {
   int none = 0;
   if (int rc = check_cache("pages_copy", &none, slots, pools, n_pools)) return rc;
-  if (n < 0 || (n > 0 && (!src || !dst)))
-    return fail(PRNN_ERR_VALUE, "pages_copy: src and dst must be non-null");
+  if (!list_fits(n) || (n > 0 && (!src || !dst)))
+    return fail(PRNN_ERR_VALUE, "pages_copy: n=%d, src and dst must be non-null", n);
   if (n == 0 || slots == 0) return PRNN_OK;
   return copy(pools, n_pools, slots, src, dst, n, static_cast<hipStream_t>(stream));
 }
@@ -324,7 +327,7 @@ extern "C" PRNN_API int prnn_pages_compact(int* used, int slots, const prnn_pool
   if (n_tables < 0 || (n_tables > 0 && (!tables || !lens)) || !live || !scratch)
     return fail(PRNN_ERR_VALUE, "pages_compact: tables, live and scratch must be non-null");
   for (int i = 0; i < n_tables; ++i)
-    if (lens[i] < 0 || (lens[i] > 0 && !tables[i]))
+    if (!list_fits(lens[i]) || (lens[i] > 0 && !tables[i]))
       return fail(PRNN_ERR_VALUE, "pages_compact: table %d", i);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   pages_plan_kernel<<<1, kPlan, 0, st>>>(used, slots, live, scratch);

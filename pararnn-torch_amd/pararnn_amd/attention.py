@@ -134,6 +134,9 @@ def _check_state(what: str, name: str, t: Tensor, q: Tensor, tail: tuple[int, ..
     if t.dim() != 4 or tuple(t.shape[1:]) != tail or (rows is not None and t.shape[0] != rows):
         want = ("C" if rows is None else rows, *tail)
         raise ValueError(f"{what}: {name} shape {tuple(t.shape)} != {want}")
+    # counts go to the kernels in 32 bits
+    if t.shape[0] >= 1 << 31:
+        raise ValueError(f"{what}: {name} has {t.shape[0]} rows, more than 2^31 - 1")
 
 
 _INTS = (torch.int32, torch.int64, torch.int16, torch.int8, torch.uint8)
@@ -145,6 +148,8 @@ def _slots(what: str, name: str, t: Tensor, dev: torch.device) -> Tensor:
         raise TypeError(f"{what}: {name} must be whole numbers, got {t.dtype}")
     if t.dim() != 1:
         raise ValueError(f"{what}: {name} must be one-dimensional, got {tuple(t.shape)}")
+    if t.shape[0] > 1 << 30:
+        raise ValueError(f"{what}: {name} has {t.shape[0]} entries, more than 2^30")
     if t.dtype is torch.int32 and t.device == dev and t.is_contiguous():
         return t
     if torch.cuda.is_current_stream_capturing():
@@ -186,6 +191,8 @@ class _Problem:
                              f"{(bk, tk)}, {(bv, tv)}")
         if dk2 != dk:
             raise ValueError(f"{what}: q has width {dk}, k {dk2}")
+        if max(batch, 1) * max(time, 1) > 1 << 30:
+            raise ValueError(f"{what}: {batch} x {time} tokens are more than 2^30")
         g_code = _decay_code(what, g, q)
         if g.dim() not in (1, 3) or (g.dim() == 3 and g.shape[:2] != (batch, time)):
             raise ValueError(f"{what}: log_decay must be (H,) or (B, T, H), got "
@@ -415,6 +422,8 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
     if bk != batch or bv != batch or dk2 != dk:
         raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)} and v "
                          f"{tuple(v.shape)} do not fit")
+    if batch > 65535:
+        raise ValueError(f"{what}: {batch} rows are more than 65535")
     g_code = _decay_code(what, log_decay, q)
     heads = log_decay.shape[-1] if log_decay.dim() else 0
     if _heads(what, hq, hk, hv, heads) != heads:

@@ -139,8 +139,8 @@ def group_norm(x: Tensor, num_groups: int, weight: Tensor | None = None,
             raise ValueError(f"{what}: {name} shape {tuple(t.shape)} != {(c,)}")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise TypeError(f"{what}: dtype mismatch {weight.dtype} vs {bias.dtype}")
-    if x.numel() // c >= 1 << 31:
-        raise ValueError(f"{what}: x has {x.numel() // c} tokens, more than 2^31 - 1")
+    if x.numel() // c >= 1 << 31 or c >= 1 << 31:
+        raise ValueError(f"{what}: x has {x.numel() // c} tokens of {c} channels, more than 2^31 - 1")
 
     _no_tangents(what, x, weight, bias, gate)
     x, gate = _flat(x), _flat(gate)

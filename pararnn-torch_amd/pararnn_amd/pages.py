@@ -30,6 +30,8 @@ def _used(what: str, used: Tensor) -> Tensor:
         raise TypeError(f"{what}: used must be int32, got {used.dtype}")
     if used.dim() != 1 or not used.is_contiguous():
         raise ValueError(f"{what}: used must be (slots,) and contiguous, got {tuple(used.shape)}")
+    if used.shape[0] > 1 << 30:
+        raise ValueError(f"{what}: {used.shape[0]} slots are more than 2^30")
     return used
 
 
@@ -46,6 +48,8 @@ def _pools(what: str, pools: Sequence[Tensor] | Tensor, slots: int | None, dev):
         if slots is not None and p.shape[0] != slots:
             raise ValueError(f"{what}: a pool has {p.shape[0]} slots, not {slots}")
         dev, slots = p.device, p.shape[0]
+        if slots > 1 << 30:
+            raise ValueError(f"{what}: {slots} slots are more than 2^30")
     rows = (_lib.Pool * max(1, len(pools)))(*(
         _lib.Pool(p.data_ptr(), p.numel() // p.shape[0] * p.element_size() if p.shape[0] else 0)
         for p in pools))
@@ -58,8 +62,8 @@ def take_pages(used: Tensor, n: int) -> Tensor:
     starts without them (``linear_attention`` without ``h0``), and one that starts with a single
     token clears them first."""
     dev = _used("take_pages", used).device
-    if n < 0:
-        raise ValueError(f"take_pages: n must be >= 0, got {n!r}")
+    if not 0 <= n <= 1 << 30:
+        raise ValueError(f"take_pages: n must be in 0 .. 2^30, got {n!r}")
     out = torch.empty(n, dtype=torch.int32, device=dev)
     _writes("take_pages", used)
     rc = _enqueue(_lib.load().prnn_pages_take, dev, used.data_ptr(), used.shape[0],
@@ -128,6 +132,8 @@ def compact_pages(used: Tensor, pools: Sequence[Tensor] | Tensor,
             raise TypeError(f"{what}: tables must be int32, got {t.dtype}")
         if not t.is_contiguous():
             raise ValueError(f"{what}: tables must be contiguous (they are changed in place)")
+        if t.numel() > 1 << 30:
+            raise ValueError(f"{what}: a table has {t.numel()} entries, more than 2^30")
     # a table given twice is one table: renamed twice, its moved entries would name free slots
     spans = sorted({(t.data_ptr(), t.numel()) for t in tables if t.numel()})
     if any(a + 4 * n > b for (a, n), (b, _) in zip(spans, spans[1:])):
