@@ -36,8 +36,8 @@ constexpr int kLaMaxDim = 256;  // widest head (keys or values)
 struct LaView {
   const void* p;
   long long sb, st, sh;  // elements between batches, tokens, heads
-  int rep;               // consecutive heads that share one of this array
-  int vec;               // rows and base admit 16-byte accesses
+  int rep = 1;           // consecutive heads that share one of this array
+  int vec = 0;           // rows and base admit 16-byte accesses
 };
 
 // Chunks' rows are read by unsigned 32-bit offsets from the lowest token's.
