@@ -499,7 +499,7 @@ void la_walk_bf16_kernel(LaParams P) {
       if (DOTS) pd += ahead * (next - base) * static_cast<long long>(std_);
 #pragma unroll
       for (int it = 0; it < 2; ++it) {
-        if (DOTS) {
+        if (dots) {
           u2 r[4];
           from_rows(dv[it], r);
           float d = 0.0f;
@@ -512,17 +512,15 @@ void la_walk_bf16_kernel(LaParams P) {
           }
           d += __shfl_xor(d, 32);
           if (half == 0) sdot[wave][32 * it + l32] = d;
-          if (dots) {
-            const float own = s_own[32 * it + l32];
-            const char* zr = sz + (32 * it + l32) * RZ + wave * 64 + 8 * half;
+          const float own = s_own[32 * it + l32];
+          const char* zr = sz + (32 * it + l32) * RZ + wave * 64 + 8 * half;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const u2 z = *reinterpret_cast<const u2*>(zr + 16 * q);
-              O[it][4 * q] = fmaf(own, lo_bf16(z[0]), O[it][4 * q]);
-              O[it][4 * q + 1] = fmaf(own, hi_bf16(z[0]), O[it][4 * q + 1]);
-              O[it][4 * q + 2] = fmaf(own, lo_bf16(z[1]), O[it][4 * q + 2]);
-              O[it][4 * q + 3] = fmaf(own, hi_bf16(z[1]), O[it][4 * q + 3]);
-            }
+          for (int q = 0; q < 4; ++q) {
+            const u2 z = *reinterpret_cast<const u2*>(zr + 16 * q);
+            O[it][4 * q] = fmaf(own, lo_bf16(z[0]), O[it][4 * q]);
+            O[it][4 * q + 1] = fmaf(own, hi_bf16(z[0]), O[it][4 * q + 1]);
+            O[it][4 * q + 2] = fmaf(own, lo_bf16(z[1]), O[it][4 * q + 2]);
+            O[it][4 * q + 3] = fmaf(own, hi_bf16(z[1]), O[it][4 * q + 3]);
           }
         }
         if (R.out_f32) {

@@ -288,9 +288,17 @@ __global__ __launch_bounds__(64 * W) void la_walk_f32_kernel(LaParams P) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int m = 16 * mi + 4 * q4 + r;
-          const float w = (acc[0][r] + acc[1][r]) * (R.p_scale * exp2_diff(sG[m], Gn));
-          sp[m * PS + n] = after + (R.dots != nullptr) <= r ? w : 0.0f;
-          if (mi == ni && after == r) s_own[m] = w;
+          acc[0][r] = (acc[0][r] + acc[1][r]) * (R.p_scale * exp2_diff(sG[m], Gn));
+          sp[m * PS + n] = after <= r ? acc[0][r] : 0.0f;
+        }
+        if (R.dots) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (after == r) {
+              const int m = 16 * mi + 4 * q4 + r;
+              s_own[m] = acc[0][r];
+              sp[m * PS + n] = 0.0f;
+            }
         }
       }
       // The rows that the output is multiplied with, then the next chunk's: what is waited for
