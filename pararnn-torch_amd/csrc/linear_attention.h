@@ -73,7 +73,7 @@ struct LaRole {
   void* out;            // (batch, token, head, vd) by the strides below
   long long o_sb, o_st, o_sh;
   int out_f32;          // out holds floats (heads that are summed afterwards)
-  LaView dot;           // dots[token] = out . dot where dots is given
+  LaView dot;           // dots[token] = (out without the token's own pair) . dot, where given
   float* dots;          // [column tile][head][token of the whole batch]
   int kd, vd;           // columns of x, y and of z, out
   int sk, sv;           // strides of the state's kd and vd axes
@@ -285,9 +285,8 @@ inline int la_widest(const LaParams& p, int roles) {
 // states.  *_tile_cols: columns of z that a workgroup takes where the widest role has vd.
 int la_walk_f32(LaParams p, int roles, bool state_only, int dtype, hipStream_t stream);
 int la_f32_tile_cols(int vd);
-// bf16 storage with widths in multiples of 8, rows that admit 16-byte accesses (x, y, z, dot) or
-// 8-byte ones (out), and tokens at least a row apart, in ascending order.
-// dots: some role has dots.
+// bf16 storage with widths in multiples of 8, rows that admit 16-byte accesses (x, y, z, dot, out),
+// and tokens at least a row apart.  dots: some role has dots.
 int la_walk_bf16(LaParams p, int roles, bool state_only, bool dots, hipStream_t stream);
 int la_bf16_tile_cols(int vd);
 

@@ -139,8 +139,8 @@ __device__ __forceinline__ double flow_at(const DecayGradArgs& A, const LaPiece&
 }
 
 // A workgroup per part and head.  The dots are read twice (their sum first, to tie the end), the
-// second time from the L2; 8 x 2048 tokens of 16 heads take 7.0 us, a chain of reductions in fp64,
-// with two products of states a part (1001 tokens x 3, 6 heads of (48, 72)) 7.5.
+// second time from the L2; 8 x 2048 tokens of 16 heads take 8.1 us, a chain of reductions in fp64
+// behind two products of states a part, 1001 tokens x 3 of 6 heads of (48, 72) 8.7.
 __global__ __launch_bounds__(256) void la_decay_grad_kernel(DecayGradArgs A) {
   __shared__ double s_wave[4];
   constexpr int kEach = 4;
@@ -360,9 +360,9 @@ struct Scratch {
 };
 
 // Whether the walks run on the bf16 matrix instructions: bf16 storage whose widths and rows admit
-// 16-byte accesses.  What is odd takes the fp32 walk: 8 x 2048 tokens of 16 heads of (64, 64) 62 us
-// on bf16 instructions and 140 in fp32, a training step 245 and 472, 4 x 2048 of (128, 128) 77 and
-// 223, of (32, 32) 42 and 65.
+// 16-byte accesses.  What is odd takes the fp32 walk: 8 x 2048 tokens of 16 heads of (64, 64) 63 us
+// on bf16 instructions and 138 in fp32, a training step 235 and 464, 4 x 2048 of (128, 128) 80 and
+// 207, 8 x 2048 of (32, 32) 49 and 77.
 bool on_bf16(const Problem& a, const prnn_la_view* other) {
   if (a.dtype != PRNN_BF16 || a.Dk % 8 || a.Dv % 8) return false;
   return view(a.q, a, a.Dk).vec && view(a.k, a, a.Dk).vec && view(a.v, a, a.Dv).vec &&
@@ -392,13 +392,13 @@ struct Walks {
 // So pieces are as long as makes the first equal to what falls with their length, unless the
 // chip has workgroups enough with longer ones: about 8 waves a CU on bf16 instructions, 16 in
 // fp32, run at a time.  Lengths of 64, 256 and 1024 and this rule's, us, heads of (64, 64) in bf16:
-// 2 x 512 tokens of 4 heads 19, 33, 31 and 19; 2048 of 4 heads 23, 33, 92 and 23, their training
-// step 60, 81, 218 and 60; 16384 of 8 heads 86, 55, 97 and 53, their training step 285, 206, 288
-// and 198; 8 x 2048 of 16 heads 97, 65, 99 and 64; 32 x 300 of 4 heads 29, 36, 23 and 23 (whole).
+// 2 x 512 tokens of 4 heads 20, 35, 34 and 20; 2048 of 4 heads 24, 36, 99 and 24, their training
+// step 63, 87, 233 and 63; 16384 of 8 heads 88, 58, 104 and 56, their training step 263, 171, 265
+// and 161; 8 x 2048 of 16 heads 94, 63, 106 and 63; 32 x 300 of 4 heads 31, 39, 25 and 25 (whole).
 //
 // Pieces that are longer for that get their states from the contributions of shorter parts, of the
-// length above: a training step of 8 x 2048 tokens of 16 heads 214 us, with parts as long as the
-// pieces 228.  A piece that a walk ends with has no contribution formed.
+// length above: a training step of 8 x 2048 tokens of 16 heads 234 us, with parts as long as the
+// pieces 249.  A piece that a walk ends with has no contribution formed.
 LaSeqs pieces(const Problem& a, long long len, long long sub, long long span) {
   LaSeqs s{a.cu_seqlens, sequences(a), a.T, a.T + 1, sequences(a), a.T + 1, a.T + 1};
   if (len < a.T) {
@@ -414,7 +414,7 @@ LaSeqs cut(const Problem& a, const Walks& w, int widest, int roles, int states) 
   const double serial = w.bf16 ? 0.085 : 0.17, per_piece = 0.12, bytes_us = 5.3e6, launches = 8.0;
   const double tokens = 1.0 * a.B * a.T;
   // packed sequences of unknown lengths: one may be all there is (100 of 60 tokens, 8 heads of (64,
-  // 64): 11 us where that is known, 42 where not)
+  // 64): 12 us where that is known, 43 where not)
   const double longest = a.cu_seqlens && a.longest > 0 ? std::min(a.longest, a.T) : a.T;
   const double falls = per_piece * longest + 16.0 * states * a.Dk * a.Dv * a.H * tokens / bytes_us;
   const long long best = std::max(1ll, std::llround(std::sqrt(falls / serial) / 64)) * 64;

@@ -14,20 +14,23 @@
 //
 // Operands in bf16 parts: the pairs' weights and the state (S itself stays fp32) in two, 16 bits, so
 // that an output is as good as a sum in fp32 that is rounded once (one part each: outputs 2.35e-3 off
-// in the 2-norm, for 1.66e-3 of the rounding alone, and 85 us for 90 on 16384 tokens of 8 heads of
+// in the 2-norm, for 1.66e-3 of the rounding alone, and 86 us for 91 on 16384 tokens of 8 heads of
 // (128, 128)); what enters the state, w z, in three, 24 bits, where the state is an fp32 result, and
 // in two where it only goes on to be rounded.  DOTS: roles may have dots with their output (the
 // decays' gradient).
 //
+// An infinity counts as one that is not finite, no more: its parts and their products may be NaN where
+// the sum is infinite.
+//
 // Bound by the chain inside a chunk at the two or three waves a SIMD that the state leaves registers
-// for: between the products stand 770 (forward) to 910 (backward) vector instructions a wave and
-// chunk of 64 at (64, 64) against 44 to 50 matrix instructions (scaling, splitting, packing); in the backward
-// walk they take 29 % of a wave's cycles, waits for LDS, memory and barriers 43 %, and the matrix
-// units are busy for 14 % of the time.  16384 tokens of 8 heads of (128, 128): the
-// pieces' contributions 27 us (67 MB of k and v, 2.4 TB/s), the walk 42 (134 MB, 3.2 TB/s).  8 x
-// 2048 tokens of 16 heads of (64, 64): 21 and 34, backward with all gradients 21 and 112.  Chunks
-// of 32 (half the work on pairs, twice the scalings of the state, two buffers and one barrier) were
-// no faster: 34 forward, 134 backward, contributions on a packed batch 28 for 24.
+// for: between the products stand 930 (forward) to 970 (backward) vector instructions a wave and
+// chunk of 64 at (64, 64) against 58 and 50 matrix instructions (scaling, splitting, packing); in the
+// backward walk they take 28 % of a wave's cycles, waits for LDS, memory and barriers 45 %, and the
+// matrix units are busy for 13 % of the time.  16384 tokens of 8 heads of (128, 128): the pieces'
+// contributions 28 us (67 MB of k and v, 2.4 TB/s), the walk 47 (134 MB, 2.9 TB/s).  8 x 2048 tokens
+// of 16 heads of (64, 64): 22 and 37, backward with all gradients 22 and 120 (115 without the token's
+// own pair left out of the dots).  Chunks of 32 (half the work on pairs, twice the scalings of the
+// state, two buffers and one barrier) were no faster when these took 34 and 112: 34 and 134.
 #include "linear_attention.h"
 
 namespace prnn {
@@ -649,8 +652,8 @@ int launch_kd(const LaParams& p, int roles, bool state_only, bool dots, hipStrea
 
 // A wave per 32 columns, as many as the head has, up to four: a workgroup forms the pairs once for
 // all of them.  Tiles of 32, 64 and 128 columns, forward in us: 8 x 2048 tokens of 16 heads of
-// (64, 64) 90, 62, 87; 4 x 2048 of (96, 96) 106, 91, 67; of (128, 128) 141, 99, 78; 8 x 2048 of
-// (32, 32) 42, 43, 59.
+// (64, 64) 85, 63, 79; 4 x 2048 of (96, 96) 119, 97, 71; of (128, 128) 149, 104, 80; 8 x 2048 of
+// (32, 32) 49, 47, 66.
 int la_bf16_tile_cols(int vd) { return vd <= 32 ? 32 : vd <= 64 ? 64 : 128; }
 
 int la_walk_bf16(LaParams p, int roles, bool state_only, bool dots, hipStream_t stream) {

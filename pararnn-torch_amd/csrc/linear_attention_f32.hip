@@ -11,9 +11,9 @@
 // a 16-bit matrix product could pass 65504.
 //
 // Bound by the chain from chunk to chunk (LDS, products of 16 x 16 x 4, decays in fp64), which the
-// waves of a CU do not hide: 8 x 2048 tokens of 16 heads of (64, 64) in fp32 136 us with the
-// pieces' contributions, 63 TFLOP/s of the 154 of a large product.  Training on 3 x 1001 tokens of
-// 6 heads of (48, 72): contributions 13 us, walk 18; backward 13 and 43.
+// waves of a CU do not hide: 8 x 2048 tokens of 16 heads of (64, 64) in fp32 138 us with the
+// pieces' contributions, 62 TFLOP/s of the 154 of a large product.  Training on 3 x 1001 tokens of
+// 6 heads of (48, 72): contributions 13 us, walk 18; backward 13 and 45.
 #include "linear_attention.h"
 
 namespace prnn {
@@ -467,8 +467,9 @@ int launch_kt(const LaParams& p, int roles, bool state_only, hipStream_t stream)
 }  // namespace
 
 // Four waves, or two where four would leave half of them without columns.  Tiles of 32 and 64
-// columns, forward in us: 8 x 2048 tokens of 16 heads of (64, 64) 192 and 144, 4 x 2048 of (96, 96)
-// 184 and 188, of (128, 128) 296 and 231; a training step on widths (48, 72) 125 and 147.
+// columns, forward in us: 8 x 2048 tokens of 16 heads of (64, 64) 184 and 137, 4 x 2048 of (96, 96)
+// 185 and 174 (on the edge of the rule), of (128, 128) 297 and 209; a training step on widths (48, 72)
+// 113 and 140.
 int la_f32_tile_cols(int vd) { return (vd + 63) / 64 * 64 - vd >= 32 ? 32 : 64; }
 
 int la_walk_f32(LaParams p, int roles, bool state_only, int dtype, hipStream_t stream) {

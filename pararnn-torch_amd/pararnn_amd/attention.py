@@ -14,8 +14,10 @@ Layouts: ``q`` ``(B, T, Hq, Dk)``, ``k`` ``(B, T, Hk, Dk)``, ``v`` ``(B, T, Hv, 
 strides whose last one is 1 (views of one fused projection are read as they are).  ``H`` is the
 largest of the head counts and of the decay's; each count divides it, and consecutive heads share
 an array that has fewer.  Widths up to 256.  float32, bfloat16 and float16; arithmetic and states
-are float32 (bfloat16 products take bfloat16 operands, see the kernels), results are rounded
-once.  Results do not depend on the order in which workgroups run: no atomics.
+are float32 (bfloat16 products take operands of 16 bits or more in bfloat16 parts, see the
+kernels), results are rounded once.  What an infinity or NaN reaches is not finite, whether the sum
+would be infinite or not a number.  Results do not depend on the order in which workgroups run: no
+atomics.
 """
 
 from __future__ import annotations
