@@ -568,7 +568,10 @@ int forward(const Problem& a, const prnn_la_view& out, float* state_out, const i
 
 int backward(const Problem& a, const prnn_la_view& go, const float* gs, void* dq, void* dk,
              void* dv, void* dg, float* dh0, void* ws, hipStream_t st) {
-  const Walks w{on_bf16(a, &go), a.dtype};
+  // the bf16 walk writes 16 bytes at a time: dense rows of widths in eights, from such a boundary
+  const uintptr_t bases = reinterpret_cast<uintptr_t>(dq) | reinterpret_cast<uintptr_t>(dk) |
+                          reinterpret_cast<uintptr_t>(dv);
+  const Walks w{on_bf16(a, &go) && (bases & 15) == 0, a.dtype};
   const Scratch s = carve(ws, a, w, true, dg != nullptr);
   LaParams p = params(a, backward_cut(a, w));
   const LaView q = view(a.q, a, a.Dk), k = view(a.k, a, a.Dk), v = view(a.v, a, a.Dv),
