@@ -9,7 +9,8 @@
 //   small part of it (exp(-12) of it and less, which fp32 differences of the whole would lose).  The
 //   flow itself stays bounded while the sum's roundings add up, so the sum is tied at both ends of a
 //   sequence (<S_0, dL/dS_0> and <S_T, dL/dS_T>, zero without states) and of every piece, whose
-//   states are there; what it misses the end by is taken back along the way;
+//   states are there; what it misses the end by is taken back along the way, by the squares of its
+//   terms;
 // * la_head_sum_kernel: gradients of shared heads, summed in a fixed order.
 #include "linear_attention.h"
 
@@ -139,10 +140,10 @@ __device__ __forceinline__ double flow_at(const DecayGradArgs& A, const LaPiece&
 }
 
 // A workgroup per part and head.  The dots are read twice (their sum first, to tie the end), the
-// second time from the L2; 8 x 2048 tokens of 16 heads take 8.1 us, a chain of reductions in fp64
-// behind two products of states a part, 1001 tokens x 3 of 6 heads of (48, 72) 8.7.
+// second time from the L2; 8 x 2048 tokens of 16 heads take 9.1 us, a chain of reductions in fp64
+// behind two products of states a part, 1001 tokens x 3 of 6 heads of (48, 72) 9.3.
 __global__ __launch_bounds__(256) void la_decay_grad_kernel(DecayGradArgs A) {
-  __shared__ double s_wave[4];
+  __shared__ double s_wave[4], s_weight[4];
   constexpr int kEach = 4;
   const int h = blockIdx.y, p = blockIdx.x, tid = threadIdx.x;
   const int lane = tid & 63, wave = tid >> 6;
@@ -154,12 +155,13 @@ __global__ __launch_bounds__(256) void la_decay_grad_kernel(DecayGradArgs A) {
     return;
   }
   const size_t t0 = A.seqs.cu ? pc.begin : static_cast<size_t>(pc.seq) * A.seqs.T + pc.begin;
-  // what the flow gains behind tokens base + t, base + t + stride, ..: all loads before the first
-  // sum, zeros behind the part's end
-  auto steps = [&](double* x, int base, int t, int stride) {
+  // what the flow gains behind tokens base + t, base + t + stride, .., and the weight of its error:
+  // all loads before the first sum, zeros behind the part's end
+  auto steps = [&](double* x, double* w, int base, int t, int stride) {
     const uint32_t bytes = min(n - base, 256 * kEach) * 4u;
+    double in[kEach];
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) x[i] = 0.0;
+    for (int i = 0; i < kEach; ++i) x[i] = in[i] = 0.0;
     for (int k = 0; k < A.tiles; ++k) {
       const size_t at = (static_cast<size_t>(k) * A.H + h) * A.batch_tokens + t0 + base;
       const rsrc_t rk = make_rsrc(A.k_dots + at, bytes), rq = make_rsrc(A.q_dots + at, bytes);
@@ -170,7 +172,15 @@ __global__ __launch_bounds__(256) void la_decay_grad_kernel(DecayGradArgs A) {
         v[i] = ldb<float>(rq, (t + i * stride) * 4u, 0);
       }
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) x[i] += static_cast<double>(u[i]) - v[i];
+      for (int i = 0; i < kEach; ++i) {
+        x[i] += u[i];
+        in[i] += v[i];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      w[i] = x[i] * x[i] + in[i] * in[i];
+      x[i] -= in[i];
     }
   };
   const size_t row = static_cast<size_t>(A.H) * A.DD;
@@ -184,42 +194,61 @@ __global__ __launch_bounds__(256) void la_decay_grad_kernel(DecayGradArgs A) {
     end = flow_at(A, pc, pc.end, h, s_wave);
   else if (A.gs)
     end = block_dot(A.last + head, A.gs + head, A.DD, s_wave);
-  double all = 0.0;
+  double all = 0.0, weight = 0.0;
   for (int base = 0; base < n; base += 256 * kEach) {
-    double x[kEach];
-    steps(x, base, tid, 256);
+    double x[kEach], w[kEach];
+    steps(x, w, base, tid, 256);
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) all += x[i];
+    for (int i = 0; i < kEach; ++i) {
+      all += x[i];
+      weight += w[i];
+    }
   }
   all = block_sum(all, s_wave);
-  const double miss = (begin + all - end) / n;  // per token
-  double flow = begin, total = 0.0;
+  weight = block_sum(weight, s_weight) + begin * begin + end * end;
+  // What is missed at the end, a unit of weight: every term of the sum is off by a like part of itself,
+  // so the squares say how much of it came from where.  (The last token alone may hand more to the
+  // final state than ever flows through a strong decay: what that is off by is not the others'.)
+  const double miss = weight > 0.0 ? (begin + all - end) / weight : weight;
+  double flow = begin, known = begin * begin, total = 0.0;
   for (int base = 0; base < n; base += 256 * kEach) {
-    double x[kEach], d[kEach], sum = 0.0;
+    double x[kEach], w[kEach], d[kEach], c[kEach], sum = 0.0, squares = 0.0;
     uint32_t g[kEach];  // decays, loaded ahead too (the last token's behind the end)
 #pragma unroll
     for (int i = 0; i < kEach; ++i)
       g[i] = la_decay_bits(A.g, la_batch(A.seqs, pc), min(pc.begin + base + tid * kEach + i, pc.end - 1), h);
-    steps(x, base, tid * kEach, 1);
+    steps(x, w, base, tid * kEach, 1);
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       d[i] = sum;  // what came before within the thread's tokens
+      c[i] = squares;
       sum += x[i];
+      squares += w[i];
     }
-    double run = sum;
+    double run = sum, run_c = squares;
 #pragma unroll
     for (int k = 1; k < 64; k <<= 1) {
-      const double o = __shfl_up(run, k);
-      if (lane >= k) run += o;
+      const double o = __shfl_up(run, k), p = __shfl_up(run_c, k);
+      if (lane >= k) {
+        run += o;
+        run_c += p;
+      }
     }
     __syncthreads();
-    if (lane == 63) s_wave[wave] = run;
+    if (lane == 63) {
+      s_wave[wave] = run;
+      s_weight[wave] = run_c;
+    }
     __syncthreads();
-    double before = flow + run - sum;
+    double before = flow + run - sum, before_c = known + run_c - squares;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      if (w < wave) before += s_wave[w];
-      flow += s_wave[w];
+    for (int i = 0; i < 4; ++i) {
+      if (i < wave) {
+        before += s_wave[i];
+        before_c += s_weight[i];
+      }
+      flow += s_wave[i];
+      known += s_weight[i];
     }
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
@@ -227,7 +256,7 @@ __global__ __launch_bounds__(256) void la_decay_grad_kernel(DecayGradArgs A) {
       if (t >= n) continue;
       // nothing comes through a factor that is zero
       const float v = la_decay_value(A.g, g[i]) <= -104.0f ? 0.0f
-                          : static_cast<float>(before + d[i] - miss * t);
+                          : static_cast<float>(before + d[i] - miss * (before_c + c[i]));
       total += v;
       if (A.dg) {
         const size_t at = (t0 + t) * A.H + h;

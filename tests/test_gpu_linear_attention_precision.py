@@ -124,3 +124,24 @@ def test_gradients_through_resets(at, dtype):
         e = _rel(x, want[name]) if want[name].any() else float(x.double().norm())
         print(f"case resets {at[:3]} {dtype} {name}: {e:.1e}", flush=True)
         assert e <= tol, (name, e)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("T", [1, 2, 64, 300, 1500])
+@pytest.mark.parametrize("g", [-6.0, -10.0, -20.0])
+def test_decay_gradient_of_strong_decays_with_states(g, T, dtype):
+    """With gradients of the final state: what the last token hands to it is of the order of one, what
+    flows through the token's decay exp(g) of that.  The bounds of the test above (2.5e-5 for e of sums
+    of 64 in fp32, 8e-3 in bfloat16 operands)."""
+    from pararnn_amd import linear_attention
+
+    q, k, v, a, h0, go, gs = _inputs(2, T, (2, 1, 2), 64, 64, dtype, seed=T, g=g, g_dtype=F32)
+    exact = [t.double().requires_grad_(True) for t in (q, k, v, a, h0)]
+    o64, s64 = O.linear_attention(*exact)
+    want = torch.autograd.grad([o64, s64], exact[3], [go.double(), gs.double()])[0]
+    mine = [t.to(DEV).requires_grad_(True) for t in (q, k, v, a, h0)]
+    out, state = linear_attention(*mine[:4], h0=mine[4], return_state=True)
+    got = torch.autograd.grad([out, state], mine[3], [go.to(DEV), gs.to(DEV)])[0]
+    e = _rel(got, want)
+    print(f"case decay {g}, {T} tokens with states, {dtype}: {e:.1e}", flush=True)
+    assert e <= (8e-3 if dtype == BF16 else 2.5e-5)
