@@ -561,7 +561,9 @@ PRNN_API int prnn_linear_attention_step(const void* q, long long q_sb, long long
  * stats: (N, G, 2) floats (mean, rstd) that the forward call writes and the backward call reads;
  * not needed (may be NULL) where L = 1 and a group is at most 256 accesses of 16 bytes (4 or 2
  * bytes where alignment or an odd width allows no more).  The backward call's alignment of x,
- * gate, gy, dx and dgate may differ from the forward call's only if stats is given to both. */
+ * gate, gy, dx and dgate may differ from the forward call's only if stats is given to both.
+ * Workspace: backward 0 or 1; 2 more where all arrays lie on 16-byte boundaries (a group of 2048
+ * 16-bit channels per token then takes its sums per workgroup, not per token). */
 PRNN_API size_t prnn_group_norm_workspace_size(int N, int L, int C, int G, int dtype,
                                                int backward);
 PRNN_API int prnn_group_norm(const void* x, const void* w, const void* b, const void* gate,

@@ -985,9 +985,12 @@ using namespace prnn;
 extern "C" PRNN_API size_t prnn_group_norm_workspace_size(int N, int L, int C, int G, int dtype,
                                                           int backward) {
   if (N < 1 || L < 1 || C < 1 || G < 1 || C % G) return 0;
+  const bool aligned = backward & 2;
+  backward &= 1;
   // the largest over the alignments that a call may turn out to have
   size_t most = 0;
   for (uintptr_t bits : {uintptr_t{0}, uintptr_t{4}, uintptr_t{2}}) {
+    if (bits && aligned) break;
     const Plan p = plan(N, L, C / G, G, dtype, bits, backward != 0);
     Carver c(nullptr);
     if (p.token) {

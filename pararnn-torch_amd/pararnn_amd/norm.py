@@ -42,7 +42,8 @@ def _flat(t: Tensor | None) -> Tensor | None:
 
 @functools.lru_cache(maxsize=256)
 def _workspace_bytes(n: int, length: int, c: int, groups: int, code: int, backward: int) -> int:
-    return _lib.load().prnn_group_norm_workspace_size(n, length, c, groups, code, backward)
+    # 2: all arrays here lie on 16-byte boundaries
+    return _lib.load().prnn_group_norm_workspace_size(n, length, c, groups, code, backward | 2)
 
 
 def _codes(x, weight, bias, groups, eps, act, over) -> tuple:
