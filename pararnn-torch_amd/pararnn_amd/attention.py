@@ -36,6 +36,7 @@ from pararnn_amd.ragged import PackedSequences
 
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
+_increment_version = torch._C._increment_version  # of torch.autograd.graph, without its wrapper
 
 
 def _enqueue(fn, dev: torch.device, *args) -> int:
@@ -78,7 +79,7 @@ def _writes(what: str, *tensors: Tensor) -> None:
             if t.requires_grad:
                 raise RuntimeError(f"{what} writes in place and has no autograd; call it under "
                                    "torch.no_grad()")
-    torch.autograd.graph.increment_version(tensors)
+    _increment_version(tensors)
 
 
 def _rows(t: Tensor) -> Tensor:
@@ -405,7 +406,8 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
                                     or log_decay.requires_grad or state.requires_grad):
         raise RuntimeError(f"{what} has no autograd; call it under torch.no_grad()")
-    _no_tangents(what, q, k, v, log_decay, state)
+    if forward_ad._current_level >= 0:
+        _no_tangents(what, q, k, v, log_decay, state)
     timed = q.dim() == 4
     if timed:
         if q.shape[1] != 1 or k.dim() != 4 or k.shape[1] != 1 or v.dim() != 4 or v.shape[1] != 1:
@@ -453,8 +455,10 @@ def linear_attention_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, st
         if out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
             raise ValueError(f"{what}: out must be contiguous, of q's type and on its device")
         res = out
-        _writes(what, out)
-    _writes(what, state)
+    if out is None:
+        _writes(what, state)
+    else:
+        _writes(what, state, out)
     rc = _enqueue(
         _lib.load().prnn_linear_attention_step, dev,
         q.data_ptr(), q.stride(0), q.stride(1), hq, k.data_ptr(), k.stride(0), k.stride(1), hk,
