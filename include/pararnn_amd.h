@@ -554,6 +554,46 @@ PRNN_API int prnn_linear_attention_step(const void* q, long long q_sb, long long
                                         int B, int H, int Dk, int Dv, float scale, int dtype,
                                         void* stream);
 
+/* ---- Gated delta rule -------------------------------------------------------
+ * Per head, with a log decay g_t and a rate b_t (beta):
+ *   u_t = b_t (v_t - exp(g_t) S_{t-1}^T k_t),  S_t = exp(g_t) S_{t-1} + k_t u_t^T,
+ *   o_t = scale S_t^T q_t.
+ * The problem is the linear attention's (layouts, packed sequences, states, tables) with beta per
+ * token, float32 or of the storage type, by strides.  bfloat16 arrays whose widths are multiples of 8
+ * must have rows on 16-byte boundaries, at least a row apart.
+ * kept (prnn_delta_rule_kept_size bytes, 256-byte aligned; NULL: no backward pass follows): what the
+ * backward call of the same problem reads of the forward one. */
+typedef struct prnn_delta_rule_problem {
+  prnn_linear_attention_problem la;
+  const void* b;
+  long long b_sb, b_st, b_sh;
+  int b_dtype;
+} prnn_delta_rule_problem;
+
+PRNN_API size_t prnn_delta_rule_workspace_size(const prnn_delta_rule_problem* problem);
+PRNN_API size_t prnn_delta_rule_kept_size(const prnn_delta_rule_problem* problem);
+PRNN_API int prnn_delta_rule(const prnn_delta_rule_problem* problem, const prnn_la_view* out,
+                             float* state_out, const int* out_table, int out_rows, void* kept,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
+/* Gradients as prnn_linear_attention_backward's, and db (batch, token, H) in beta's type (NULL: not
+ * wanted). */
+PRNN_API size_t prnn_delta_rule_backward_workspace_size(const prnn_delta_rule_problem* problem,
+                                                        int decay_grad);
+PRNN_API int prnn_delta_rule_backward(const prnn_delta_rule_problem* problem, const prnn_la_view* go,
+                                      const float* gs, const void* kept, void* dq, void* dk, void* dv,
+                                      void* dg, void* db, float* dh0, void* workspace,
+                                      size_t workspace_bytes, void* stream);
+
+/* One token per row, as prnn_linear_attention_step; beta (B, H) by strides. */
+PRNN_API int prnn_delta_rule_step(const void* q, long long q_sb, long long q_sh, int q_heads,
+                                  const void* k, long long k_sb, long long k_sh, int k_heads,
+                                  const void* v, long long v_sb, long long v_sh, int v_heads,
+                                  const void* g, long long g_sb, long long g_sh, int g_dtype,
+                                  const void* b, long long b_sb, long long b_sh, int b_dtype,
+                                  float* state, const int* block_table, int rows, void* out, int B,
+                                  int H, int Dk, int Dv, float scale, int dtype, void* stream);
+
 /* ---- Group norm, channels last --------------------------------------------
  * x, gate, y (N, L, C), statistics over a sample's L tokens and a group's C / G channels (L = 1:
  * per token).  y = act(z) with z = w (x - mean) rstd + b, or z act(gate) where gate is given.

@@ -1,0 +1,34 @@
+"""The delta-rule block's operators from their definitions, on the CPU: the rule token by token, the
+residual norm from its sums, a beam step candidate by candidate.  Plain torch in the inputs' own type
+(float64 in the tests), the first two differentiable by autograd."""
+
+from __future__ import annotations
+
+import torch
+
+
+def delta_rule(q, k, v, log_decay, beta, h0=None, scale=None, cu=None):
+    """(out (B, T, H, Dv), final states (sequences, H, Dk, Dv)); ``cu``: offsets as a list."""
+    H = max(q.shape[2], k.shape[2], v.shape[2], log_decay.shape[-1])
+    q, k, v = (x.repeat_interleave(H // x.shape[2], dim=2) for x in (q, k, v))
+    B, T, _, Dk = q.shape
+    scale = Dk ** -0.5 if scale is None else scale
+    a = torch.exp(log_decay).expand(B, T, H)
+    S = B if cu is None else len(cu) - 1
+    if h0 is None:
+        h0 = q.new_zeros(S, H, Dk, v.shape[-1])
+
+    def walk(q, k, v, a, b, s):
+        out = []
+        for t in range(q.shape[1]):
+            s = a[:, t, :, None, None] * s
+            u = b[:, t, :, None] * (v[:, t] - (k[:, t, :, :, None] * s).sum(-2))
+            s = s + k[:, t, :, :, None] * u[:, :, None, :]
+            out.append(scale * (q[:, t, :, :, None] * s).sum(-2))
+        return (torch.stack(out, 1) if out else v[:, :0]), s
+
+    if cu is None:
+        return walk(q, k, v, a, beta, h0)
+    parts = [walk(*(x[:, cu[i]:cu[i + 1]] for x in (q, k, v, a, beta)), h0[i:i + 1])
+             for i in range(S)]
+    return torch.cat([o for o, _ in parts], 1), torch.cat([s for _, s in parts])

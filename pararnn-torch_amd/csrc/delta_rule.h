@@ -1,0 +1,190 @@
+// Gated delta rule: what its kernels and their host code share.
+//
+// One head holds a state S (Dk x Dv) in fp32; a token with log decay g_t and rate b_t writes what
+// the decayed state lacks of v_t at k_t:
+//
+//   e_t = v_t - exp(g_t) S_{t-1}^T k_t,   u_t = b_t e_t,
+//   S_t = exp(g_t) S_{t-1} + k_t u_t^T,   o_t = scale S_t^T q_t.
+//
+// Chunks of 64 tokens, G_i the running sum of g inside a chunk (its first token included), S the
+// state before it, and the strictly lower N_ij = exp(G_i - G_j) k_i . k_j:
+//
+//   (1 + N diag(b)) e = v - exp(G) K S             a unit triangular system
+//   o  = scale [ exp(G) Q S + P u ],               P_ij = exp(G_i - G_j) q_i . k_j  (j <= i)
+//   S' = exp(G_last) S + (exp(G_last - G) K)^T u.
+//
+// Its gradients, with R = dL/dS behind the chunk:
+//
+//   (1 + diag(b) N)^T du = scale P^T go + exp(G_last - G) K R,     dv = b du,   db = du . e
+//   R' = exp(G_last) R + (scale exp(G) Q)^T go - (exp(G) K)^T dv
+//   dq = scale [ exp(G) go S^T + (go u^T . lower) K ]
+//   dk = exp(G_last - G) u R^T + scale (go u^T . lower)^T Q - exp(G) dv S^T - (X + X^T) K,
+//   X_ij = exp(G_i - G_j) dv_i . u_j (j < i).
+//
+// The inverses of the systems, the pairs P and the decays' exponentials do not depend on the state:
+// a kernel of their own forms them for all chunks at once (delta_rule_systems.hip).  What is left
+// goes from chunk to chunk: three products forwards (delta_rule_walk.h), the same three backwards.
+// With the states before and the adjoints behind the chunks, all other gradients are formed for all
+// chunks at once (delta_rule_grad.hip).
+//
+// Two arithmetics: bf16 storage of widths in eights on bf16 matrix instructions, operands that are
+// not given in bf16 in two or three bf16 parts; everything else (fp32, fp16, odd widths) on fp32
+// ones.
+#pragma once
+
+#include "linear_attention.h"
+
+namespace prnn {
+
+constexpr int kDrC = 64;  // tokens of a chunk
+
+// ---- where chunks and pieces lie ---------------------------------------------------------
+//
+// Units of `len` tokens counted from every sequence's own start, so that a sequence's results do
+// not depend on what lies next to it.  Unit i of sequence s of a packed stream is number
+// s + floor(cu[s] / len) + i: numbers are distinct and below n_seq + ceil(T / len).
+struct DrUnit {
+  int seq, index, count;  // index of `count` in its sequence
+  int s0, s1;             // the sequence's tokens
+  int begin, end;         // the unit's
+  bool any;               // false: no unit has this number
+};
+
+__device__ __forceinline__ int dr_base(const LaSeqs& q, int len, int s, int s0) {
+  return q.cu ? s + s0 / len : s * (q.T > len ? (q.T + len - 1) / len : 1);
+}
+
+__device__ __forceinline__ DrUnit dr_unit(const LaSeqs& q, int len, int id) {
+  DrUnit r;
+  if (q.cu == nullptr) {
+    r.count = q.T > len ? (q.T + len - 1) / len : 1;
+    r.seq = id / r.count;
+    r.index = id - r.seq * r.count;
+    r.s0 = 0;
+    r.s1 = q.T;
+    r.any = r.seq < q.n_seq;
+  } else {
+    int lo = 0, hi = q.n_seq;  // the last s with s + cu[s] / len <= id
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (mid + la_offset(q, mid) / len <= id) lo = mid; else hi = mid;
+    }
+    r.seq = lo;
+    r.s0 = la_offset(q, lo);
+    r.s1 = la_offset(q, lo + 1);
+    if (r.s1 < r.s0) r.s1 = r.s0;
+    r.count = r.s1 - r.s0 > len ? (r.s1 - r.s0 + len - 1) / len : 1;
+    r.index = id - lo - r.s0 / len;
+    r.any = r.index >= 0 && r.index < r.count;
+  }
+  const long long b = r.s0 + static_cast<long long>(r.index) * len;
+  r.begin = b < r.s1 ? static_cast<int>(b) : r.s1;
+  r.end = r.s1 - r.begin > len ? r.begin + len : r.s1;
+  return r;
+}
+inline long long dr_units(const LaSeqs& q, long long len) {
+  if (q.cu) return q.n_seq + (q.T + len - 1) / len;
+  return static_cast<long long>(q.n_seq) * (q.T > len ? (q.T + len - 1) / len : 1);
+}
+
+// Token 0 of a unit among all tokens of the batch (rows of dense arrays).
+__device__ __forceinline__ size_t dr_token(const LaSeqs& q, const DrUnit& u, int t) {
+  return q.cu ? static_cast<size_t>(t) : static_cast<size_t>(u.seq) * q.T + t;
+}
+__device__ __forceinline__ int dr_batch(const LaSeqs& q, const DrUnit& u) { return q.cu ? 0 : u.seq; }
+
+// ---- a chunk's system --------------------------------------------------------------------
+//
+// Per chunk and head: the strictly lower part of the inverse, then the pairs, each as the tiles
+// (0, 0), (1, 0), (1, 1) of 32 x 32 (the transposed ones, for the walk backwards: (0, 0), (0, 1),
+// (1, 1)), rows of 32 elements whose units of four are exchanged by the row (dr_unit_of), bf16 in
+// two parts of 6 KB or fp32; then kDrW rows of 64 floats.
+constexpr int kDrTiles = 3 * 32 * 32 * 4;  // bytes of a matrix in either arithmetic
+enum { kWg, kWr, kWb, kWhi, kWlo, kWmeta, kDrW };  // exp(G), exp(G_last - G), b, G in two parts
+constexpr int kDrSys = 2 * kDrTiles + kDrW * 64 * 4;
+static_assert(kDrSys % 256 == 0, "blocks stay aligned");
+// kWmeta: [0] exp(G_last), [1] the first token that is not finite (64: none), as an integer
+
+template <typename E>
+__device__ __forceinline__ int dr_unit_of(int row, int unit) {
+  return unit ^ ((sizeof(E) == 2 ? row >> 2 : row >> 1) & 7);
+}
+
+// A token's rate.
+__device__ __forceinline__ float dr_rate(const LaDecay& b, int batch, int t, int h) {
+  const uint32_t bits = la_decay_bits(b, batch, t, h);
+  return b.dtype == PRNN_F32   ? __uint_as_float(bits)
+         : b.dtype == PRNN_F16 ? Narrow<f16>::val(bits)
+                               : Narrow<bf16>::val(bits);
+}
+
+struct DrSystems {
+  LaSeqs seqs;
+  LaView q, k;
+  LaDecay g, b;
+  char* sys;
+  int H, Dk, dtype, transposed;
+  float scale;
+};
+
+struct DrWalk {
+  LaSeqs seqs;               // len: tokens of a piece, a multiple of 64
+  LaView q, k, z;            // z: v, backwards go
+  const char* sys;
+  void* out;                 // forwards: o by the strides below, storage type
+  long long o_sb, o_st, o_sh;
+  void* e;                   // (token, H, Dv) of the arithmetic's type: written forwards, read backwards
+  void* keep;                // (chunk, H, Dk, Dv): states before the chunks, adjoints behind them
+  void* dv;                  // backwards, dense (token, H, Dv): of the arithmetic's type
+  float* dv32;               // or floats besides (heads that are summed afterwards)
+  float* db;                 // [wave's columns][token][H]
+  size_t tokens;             // of the whole batch
+  LaState init, last;
+  float *piece, *transfer;   // pieces' own states (piece, H, Dk, Dv) and transfers (piece, H, Dk, Dk)
+  int H, Dk, Dv, dtype;
+  int tiles, own_tiles;      // column tiles of a launch; of them of the state (the rest: transfers)
+  float scale;
+};
+
+struct DrGrad {
+  LaSeqs seqs;
+  LaView q, k, go;
+  LaDecay g, b;
+  const char* sys;           // the transposed systems: only their decays and rates are read
+  const void *e, *dv;        // (token, H, Dv) of the arithmetic's type
+  const void *before, *behind;  // (chunk, H, Dk, Dv)
+  const float* db;           // [wave's columns][token][H]
+  int db_tiles;
+  void *dq, *dk;             // (token, H, Dk): the arithmetic's type, or floats (q_f32, k_f32)
+  int q_f32, k_f32;
+  void *dg, *dbeta;          // (token, H); dg NULL: not wanted, or sums per chunk:
+  float* g_part;             // (chunk, H)
+  int H, Dk, Dv, dtype, g_dtype, b_dtype;
+  size_t tokens;
+  float scale;
+};
+
+enum DrKind { kDrForward, kDrState, kDrBackward, kDrAdjoint };  // kDrState, kDrAdjoint: pieces' own
+
+int dr_systems(const DrSystems& a, bool bf16, hipStream_t stream);
+int dr_walk_bf16(const DrWalk& a, DrKind kind, int cols, hipStream_t stream);
+int dr_walk_bf16_back(const DrWalk& a, DrKind kind, int cols, hipStream_t stream);
+int dr_walk_f32(const DrWalk& a, DrKind kind, hipStream_t stream);
+int dr_grad(const DrGrad& a, bool bf16, hipStream_t stream);
+
+// How a walk covers the Dv columns of the state: workgroups, and their waves in all, `cols` columns
+// each.
+struct DrCover {
+  int group, tiles, waves;
+};
+inline DrCover dr_walk_cols(int Dk, int Dv, int cols, bool bf16) {
+  int group = 4;  // waves of a workgroup
+  if (!bf16)
+    group = Dk <= 128 ? 4 : 2;
+  else if (Dk <= 128 && (cols == 32 ? Dv <= 64 : Dv <= 32))
+    group = 2;
+  const int tiles = (Dv + cols * group - 1) / (cols * group);
+  return DrCover{group, tiles, tiles * group};
+}
+
+}  // namespace prnn

@@ -1,0 +1,79 @@
+// Gated delta rule: rows of tokens from memory, to LDS or as operands.
+#pragma once
+
+#include <type_traits>
+
+#include "delta_rule.h"
+#include "tiles.h"
+
+namespace prnn {
+
+constexpr int dr_row_k(bool narrow, int cols) {
+  return narrow ? (cols >= 128 ? cols * 2 + 48 : cols * 2 + 16) : (cols + 4) * 4;
+}
+constexpr int dr_row_z(bool narrow, int cols) {
+  return narrow ? (cols == 32 ? 64 : cols == 64 ? 144 : cols * 2 + 48) : (cols + 4) * 4;
+}
+
+// Rows of 64 tokens of a head on their way from memory to LDS: 16-byte units in bf16, single
+// elements of any storage type to floats.
+template <class M, int COLS, int NT>
+struct Staged {
+  static constexpr bool kNarrow = sizeof(typename M::E) == 2;
+  static constexpr int U = kNarrow ? COLS / 8 : COLS;  // units of a row
+  static constexpr int N = kDrC * U / NT;
+  static_assert(kDrC * U % NT == 0, "whole units");
+  std::conditional_t<kNarrow, u4, uint32_t> r[N];
+
+  // `width` columns from c0; tokens [0, n) from `p` are there
+  __device__ __forceinline__ void fetch(const char* p, long long st, int n, int c0, int width, int dtype) {
+    const int tid = threadIdx.x;
+    const rsrc_t b = make_rsrc(p, 0x7fffffffu);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int e = tid + k * NT, row = e / U, c = e % U;
+      if constexpr (kNarrow) {
+        r[k] = __builtin_amdgcn_raw_buffer_load_b128(
+            b, la_in((row < n) & (c0 + c * 8 < width), row * static_cast<int>(st) * 2 + (c0 + c * 8) * 2), 0, 0);
+      } else if (dtype == PRNN_F32) {
+        r[k] = __builtin_amdgcn_raw_buffer_load_b32(
+            b, la_in((row < n) & (c0 + c < width), (row * static_cast<int>(st) + c0 + c) * 4), 0, 0);
+      } else {
+        r[k] = __builtin_amdgcn_raw_buffer_load_b16(
+            b, la_in((row < n) & (c0 + c < width), (row * static_cast<int>(st) + c0 + c) * 2), 0, 0);
+      }
+    }
+  }
+  template <int RB>
+  __device__ __forceinline__ void put(char* tile, int dtype) const {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int e = threadIdx.x + k * NT, row = e / U, c = e % U;
+      if constexpr (kNarrow) {
+        *reinterpret_cast<u4*>(tile + row * RB + c * 16) = r[k];
+      } else {
+        const float v = dtype == PRNN_F32   ? __uint_as_float(r[k])
+                        : dtype == PRNN_F16 ? Narrow<f16>::val(r[k])
+                                            : Narrow<bf16>::val(r[k]);
+        *reinterpret_cast<float*>(tile + row * RB + c * 4) = v;
+      }
+    }
+  }
+};
+
+// Eight elements of a row from column c0 as they are multiplied; zeros outside.
+template <class M, typename T>
+__device__ __forceinline__ Op<M, 1> global_op(rsrc_t r, bool in, uint32_t row, int c0, int width) {
+  Op<M, 1> o;
+  if constexpr (sizeof(typename M::E) == 2) {
+    o.p[0] = __builtin_bit_cast(
+        b8, __builtin_amdgcn_raw_buffer_load_b128(r, la_in(in & (c0 < width), row + c0 * 2), 0, 0));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      o.x[i] = ldb<T>(r, la_in(in & (c0 + i < width), row + (c0 + i) * static_cast<int>(sizeof(T))), 0);
+  }
+  return o;
+}
+
+}  // namespace prnn

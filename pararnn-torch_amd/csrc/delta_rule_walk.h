@@ -1,0 +1,529 @@
+// Gated delta rule, the walks from chunk to chunk, forwards and backwards.
+//
+// A wave keeps NC columns of the state (or of its adjoint) in the result layout of the matrix
+// instructions (tiles.h), lane = column, and goes through its piece's chunks.  The three products
+// of a chunk's chain, with rows of K read from LDS along and across,
+//
+//   forwards   x = K S,   e = (1 + T)(v - exp(G) x),          S' = exp(G_last) S + K^T (..u)
+//   backwards  x = K R,   du = (1 + T)(P^T go + .. x),        R' = exp(G_last) R + Q^T (..go) - K^T (..dv)
+//
+// take what the one before left in registers, so a wave's chain meets no other wave: the two
+// barriers of a chunk only hand K, Q and the system through LDS.  The output is formed transposed
+// from the same registers (state and u as first operands), so that a lane holds consecutive columns
+// of a token.
+#pragma once
+
+#include "delta_rule_loads.h"
+
+namespace prnn {
+
+// The same in one go, a few loads at a time: where the registers for a chunk ahead are not there.
+template <class M, int COLS, int NT, int RB>
+__device__ __forceinline__ void fill(char* tile, const char* p, long long st, int n, int width, int dtype) {
+  constexpr int kAt = 16;
+  const rsrc_t b = make_rsrc(p, 0x7fffffffu);
+  for (int e0 = threadIdx.x; e0 < kDrC * COLS; e0 += kAt * NT) {
+    float v[kAt];
+#pragma unroll
+    for (int k = 0; k < kAt; ++k) {
+      const int e = e0 + k * NT, row = e / COLS, c = e % COLS;
+      const uint32_t at = la_in((row < n) & (c < width), (row * static_cast<int>(st) + c) * (dtype == PRNN_F32 ? 4 : 2));
+      v[k] = dtype == PRNN_F32 ? ldb<float>(b, at, 0) : dtype == PRNN_F16 ? ldb<f16>(b, at, 0) : ldb<bf16>(b, at, 0);
+    }
+#pragma unroll
+    for (int k = 0; k < kAt; ++k) {
+      const int e = e0 + k * NT, row = e / COLS, c = e % COLS;
+      *reinterpret_cast<float*>(tile + row * RB + c * 4) = v[k];
+    }
+  }
+}
+struct NotStaged {};
+
+// Operand of a stored matrix (the system's inverse or the pairs): rows NC rt .. of the 64, step f of
+// the contraction over tokens.  UPPER: the transposed ones.
+template <class M, int NC, bool UPPER>
+struct Stored {
+  static constexpr int G = 64 / NC;
+  static constexpr int kTile = kDrTiles / 3 / M::kParts;
+  // whether there is anything in the 32 x 32 tile
+  static constexpr bool any(int rt, int f) {
+    const int a = NC * rt / 32, b = 8 * G * f / 32;
+    return UPPER ? b >= a : b <= a;
+  }
+  static __device__ __forceinline__ Op<M, M::kParts> get(const char* m, int rt, int f, int n, int g) {
+    using E = typename M::E;
+    const int a = NC * rt / 32, b = 8 * G * f / 32;
+    const int row = (NC * rt + n) & 31, c = (8 * G * f & 31) + 4 * g;
+    const char* t = m + (a + b) * kTile + row * 32 * static_cast<int>(sizeof(E));
+    const int u0 = dr_unit_of<E>(row, c / 4), u1 = dr_unit_of<E>(row, c / 4 + G);
+    Op<M, M::kParts> o;
+    if constexpr (sizeof(E) == 2) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        union {
+          u2 h[2];
+          b8 v;
+        } x;
+        x.h[0] = *reinterpret_cast<const u2*>(t + p * 3 * kTile + u0 * 8);
+        x.h[1] = *reinterpret_cast<const u2*>(t + p * 3 * kTile + u1 * 8);
+        o.p[p] = x.v;
+      }
+    } else {
+      const f4 x = *reinterpret_cast<const f4*>(t + u0 * 16), y = *reinterpret_cast<const f4*>(t + u1 * 16);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        o.x[i] = x[i];
+        o.x[4 + i] = y[i];
+      }
+    }
+    return o;
+  }
+};
+
+// Workgroups of one head's column tiles, which read the same rows and systems, are 8 apart: they
+// run on one XCD (workgroups go to the 8 XCDs in turn).
+__device__ __forceinline__ void dr_place(int tiles, int H, int& tile, int& h, int& piece) {
+  const int group = blockIdx.x / (8 * tiles), in = blockIdx.x - group * 8 * tiles;
+  tile = in >> 3;
+  const int item = group * 8 + (in & 7);
+  piece = item / H;
+  h = item - piece * H;
+}
+
+template <class M, int NC, int KD, int W, int KIND>
+__global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
+  using E = typename M::E;
+  constexpr bool kNarrow = sizeof(E) == 2;
+  constexpr bool kBack = KIND == kDrBackward || KIND == kDrAdjoint;
+  constexpr bool kOwn = KIND == kDrState || KIND == kDrAdjoint;  // pieces' own states only
+  constexpr int G = 64 / NC, NT = 64 * W, VT = NC * W;
+  constexpr int RT = NC * NC / 64;   // registers of a tile
+  constexpr int KT = KD / NC;        // the state's tiles
+  constexpr int KF = KD / (8 * G);   // steps of a contraction over its rows
+  constexpr int TT = kDrC / NC;      // token tiles
+  constexpr int TF = kDrC / (8 * G); // steps of a contraction over tokens
+  constexpr int RK = dr_row_k(kNarrow, KD), RZ = dr_row_z(kNarrow, VT);
+  constexpr bool kQ = KIND != kDrState;  // Q takes part
+  constexpr bool kP = KIND != kDrState;
+  constexpr int ES = static_cast<int>(sizeof(E));
+  using A_t = Acc<NC>;
+  using Mat = Stored<M, NC, kBack>;
+  // fp32 widths over 64 have no registers for the next chunk's K and Q, over 128 no LDS for the system
+  constexpr bool kAhead = kNarrow || KD <= 64, kSysLds = kNarrow || KD <= 128;
+  static_assert(kAhead || kDrC * KD % (16 * NT) == 0, "whole rounds of fill");
+  constexpr int kSysBytes = kP ? 2 * kDrTiles : kDrTiles;
+  constexpr int kSysUnits = kSysBytes / 16 / NT;
+  static_assert(kSysBytes % (16 * NT) == 0, "whole units");
+  __shared__ __align__(16) char sK[kDrC * RK];
+  __shared__ __align__(16) char sQ[kQ ? kDrC * RK : 16];
+  __shared__ __align__(16) char sZ[kDrC * RZ];
+  __shared__ __align__(16) char sE[KIND == kDrBackward ? kDrC * RZ : 16];
+  __shared__ __align__(16) char s_sys[kSysLds ? kSysBytes : 16];
+  __shared__ __align__(16) float sW[kDrW * 64];
+
+  int tile, h, piece;
+  dr_place(A.tiles, A.H, tile, h, piece);
+  const DrUnit pc = dr_unit(A.seqs, A.seqs.len, piece);
+  if (!pc.any || pc.seq >= A.seqs.n_seq) return;
+  // the last piece of the walk's direction hands its state to none
+  if (kOwn && pc.index == (kBack ? 0 : pc.count - 1)) return;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int nn = lane % NC, g = lane / NC;
+  const bool transfer = kOwn && tile >= A.own_tiles;
+  const int col0 = (transfer ? tile - A.own_tiles : tile) * VT;
+  const int width = transfer ? A.Dk : A.Dv;  // the state's columns
+  const int col = col0 + NC * wave + nn;
+  const int batch = dr_batch(A.seqs, pc);
+  const int row0 = dr_base(A.seqs, kDrC, pc.seq, pc.s0) + (pc.begin - pc.s0) / kDrC;
+  const int chunks = (pc.end - pc.begin + kDrC - 1) / kDrC;
+  const size_t state_floats = static_cast<size_t>(A.Dk) * A.Dv;
+  const size_t tok0 = dr_token(A.seqs, pc, 0);
+
+  // ---- the state that the piece begins with
+  A_t S[KT];
+#pragma unroll
+  for (int t = 0; t < KT; ++t)
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const int i = NC * t + 4 * G * (r >> 2) + 4 * g + (r & 3);
+      S[t][r] = transfer && i == col ? 1.0f : 0.0f;
+    }
+  if (!kOwn) {
+    const float* src = nullptr;
+    if (A.piece && pc.count > 1)
+      src = A.piece + (static_cast<size_t>(piece) * A.H + h) * state_floats;
+    else if (const float* row = la_row(A.init, pc.seq, A.H * state_floats))
+      src = row + h * state_floats;
+    if (src) {
+      const rsrc_t rs = make_rsrc(src, static_cast<uint32_t>(state_floats) * 4);
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          const int i = NC * t + 4 * G * (r >> 2) + 4 * g + (r & 3);
+          S[t][r] = ldb<float>(rs, la_in((i < A.Dk) & (col < A.Dv), (i * A.Dv + col) * 4), 0);
+        }
+    }
+  }
+
+  std::conditional_t<kAhead, Staged<M, KD, NT>, NotStaged> rk, rq;
+  Staged<M, VT, NT> rz, re;
+  u4 rs[kSysLds ? kSysUnits : 1], rw[(kDrW * 64 / 4 + NT - 1) / NT];
+  const int size = kNarrow || A.dtype != PRNN_F32 ? 2 : 4;
+  auto head = [&](const LaView& v, int t) {
+    return static_cast<const char*>(v.p) +
+           (batch * v.sb + (h / v.rep) * v.sh + static_cast<long long>(t) * v.st) * size;
+  };
+  auto fetch = [&](int c) {
+    const int t = pc.begin + c * kDrC, n = min(pc.end - t, kDrC);
+    const char* sys = A.sys + (static_cast<size_t>(row0 + c) * A.H + h) * kDrSys;
+#pragma unroll
+    for (int k = 0; k < (kSysLds ? kSysUnits : 0); ++k) rs[k] = *reinterpret_cast<const u4*>(sys + (tid + k * NT) * 16);
+    const char* w = sys + 2 * kDrTiles;
+#pragma unroll
+    for (int k = 0; k < (kDrW * 16 + NT - 1) / NT; ++k)
+      if (tid + k * NT < kDrW * 16) rw[k] = *reinterpret_cast<const u4*>(w + (tid + k * NT) * 16);
+    if constexpr (kAhead) rk.fetch(head(A.k, t), A.k.st, n, 0, A.Dk, A.dtype);
+    if constexpr (kAhead && kQ) rq.fetch(head(A.q, t), A.q.st, n, 0, A.Dk, A.dtype);
+    rz.fetch(head(A.z, t), A.z.st, transfer ? 0 : n, col0, A.Dv, A.dtype);
+    if constexpr (KIND == kDrBackward)
+      re.fetch(static_cast<const char*>(A.e) + ((tok0 + t) * A.H + h) * A.Dv * ES,
+               static_cast<long long>(A.H) * A.Dv, n, col0, A.Dv, kNarrow ? PRNN_BF16 : PRNN_F32);
+  };
+  if (chunks > 0) fetch(kBack ? chunks - 1 : 0);
+
+  for (int step = 0; step < chunks; ++step) {
+    const int c = kBack ? chunks - 1 - step : step;
+    const int t0 = pc.begin + c * kDrC, n = min(pc.end - t0, kDrC);
+    if constexpr (kAhead) {
+      rk.template put<RK>(sK, A.dtype);
+      if constexpr (kQ) rq.template put<RK>(sQ, A.dtype);
+    } else {
+      fill<M, KD, NT, RK>(sK, head(A.k, t0), A.k.st, n, A.Dk, A.dtype);
+      if constexpr (kQ) fill<M, KD, NT, RK>(sQ, head(A.q, t0), A.q.st, n, A.Dk, A.dtype);
+    }
+    rz.template put<RZ>(sZ, A.dtype);
+    if constexpr (KIND == kDrBackward) re.template put<RZ>(sE, kNarrow ? PRNN_BF16 : PRNN_F32);
+#pragma unroll
+    for (int k = 0; k < (kSysLds ? kSysUnits : 0); ++k) *reinterpret_cast<u4*>(s_sys + (tid + k * NT) * 16) = rs[k];
+#pragma unroll
+    for (int k = 0; k < (kDrW * 16 + NT - 1) / NT; ++k)
+      if (tid + k * NT < kDrW * 16) *reinterpret_cast<u4*>(reinterpret_cast<char*>(sW) + (tid + k * NT) * 16) = rw[k];
+    const char* sS = kSysLds ? s_sys : A.sys + (static_cast<size_t>(row0 + c) * A.H + h) * kDrSys;
+    __syncthreads();
+    if (step + 1 < chunks) fetch(kBack ? c - 1 : c + 1);
+
+    // what the gradients of this chunk need of the state
+    if (!kOwn && A.keep) {
+      const rsrc_t rs = make_rsrc(static_cast<E*>(A.keep) + (static_cast<size_t>(row0 + c) * A.H + h) * state_floats,
+                                  static_cast<uint32_t>(state_floats) * ES);
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          const int i = NC * t + 4 * G * (r >> 2) + 4 * g + (r & 3);
+          store_elem<M>(rs, la_in((i < A.Dk) & (col < A.Dv), (i * A.Dv + col) * ES), S[t][r]);
+        }
+    }
+
+    // ---- x = K S and the state's part of the output, S^T Q^T
+    A_t X[TT], O[TT];
+#pragma unroll
+    for (int t = 0; t < TT; ++t)
+#pragma unroll
+      for (int r = 0; r < RT; ++r) X[t][r] = O[t][r] = 0.0f;
+#pragma unroll
+    for (int f = 0; f < KF; ++f) {
+      float s[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] = S[(8 * f + e) / RT][(8 * f + e) % RT];
+      const auto sp = parts_of<M, 2>(s);
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        mul<NC>(X[t], row_op<M, G>(sK + (NC * t + nn) * RK, f, g), sp);
+        if constexpr (KIND == kDrForward) mul<NC>(O[t], sp, row_op<M, G>(sQ + (NC * t + nn) * RK, f, g));
+      }
+    }
+
+    const char* zat = sZ + NC * wave * ES + col_share<M, G, RZ>(lane);
+    float y[NC];  // the system's right side: token of element i at_token(i)
+    auto at_token = [&](int i) { return NC * (i / RT) + 4 * G * ((i % RT) >> 2) + 4 * g + (i & 3); };
+    auto weight = [&](int which, int i) {  // of elements i .. i + 3
+      return *reinterpret_cast<const f4*>(&sW[which * 64 + at_token(i)]);
+    };
+    A_t Y[TT];
+    Op<M, 1> zo[TF];
+#pragma unroll
+    for (int f = 0; f < TF; ++f) zo[f] = col_op<M, G, RZ>(zat, 8 * G * f, 0);
+    if constexpr (!kBack) {
+#pragma unroll
+      for (int f = 0; f < TF; ++f) {
+        float v[8];
+        values(zo[f], v);
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+          const f4 w = weight(kWg, 8 * f + e);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int i = 8 * f + e + r;
+            y[i] = fmaf(-w[r], X[i / RT][i % RT], v[e + r]);
+          }
+        }
+      }
+    } else {
+      // P^T go, then the adjoint behind the chunk
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r) Y[t][r] = 0.0f;
+#pragma unroll
+        for (int f = 0; f < TF; ++f)
+          if (Mat::any(t, f)) mul<NC>(Y[t], Mat::get(sS + kDrTiles, t, f, nn, g), zo[f]);
+      }
+#pragma unroll
+      for (int i = 0; i < NC; i += 4) {
+        const f4 w = weight(kWr, i);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          y[i + r] = fmaf(w[r], X[(i + r) / RT][(i + r) % RT], Y[(i + r) / RT][(i + r) % RT]);
+      }
+    }
+
+    // A token that is not finite, in this column or (the system's word) in all of them, must not
+    // reach earlier ones through products with zeros: from it on the column's tokens take no part,
+    // and get NaN afterwards.
+    int stop = kDrC;
+    bool poisoned = false;
+    if constexpr (!kBack) {
+      float zero = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NC; ++i) zero = fmaf(y[i], 0.0f, zero);
+      const int all = __float_as_int(sW[kWmeta * 64 + 1]);
+      poisoned = __any(!(zero == 0.0f) || all < kDrC);
+      if (poisoned) {
+        stop = all;
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+          if (!(y[i] * 0.0f == 0.0f)) stop = min(stop, at_token(i));
+#pragma unroll
+        for (int m = NC; m < 64; m <<= 1) stop = min(stop, __shfl_xor(stop, m));
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+          if (at_token(i) >= stop) y[i] = 0.0f;
+      }
+    }
+
+    // ---- (1 + T) y
+    Op<M, 2> yo[TF];
+#pragma unroll
+    for (int f = 0; f < TF; ++f) {
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = y[8 * f + e];
+      yo[f] = parts_of<M, 2>(v);
+    }
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+#pragma unroll
+      for (int r = 0; r < RT; ++r) Y[t][r] = y[RT * t + r];
+#pragma unroll
+      for (int f = 0; f < TF; ++f)
+        if (Mat::any(t, f)) mul<NC>(Y[t], Mat::get(sS, t, f, nn, g), yo[f]);
+    }
+
+    float u[NC];  // what is written: b e forwards, b du = dv backwards
+#pragma unroll
+    for (int i = 0; i < NC; i += 4) {
+      const f4 b = weight(kWb, i);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) u[i + r] = b[r] * Y[(i + r) / RT][(i + r) % RT];
+    }
+    if (!kBack && poisoned) {
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        if (at_token(i) >= stop) u[i] = 0.0f;
+    }
+
+    if constexpr (KIND == kDrForward) {
+      // ---- out
+      Op<M, 2> uo[TF];
+#pragma unroll
+      for (int f = 0; f < TF; ++f) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = u[8 * f + e];
+        uo[f] = parts_of<M, 2>(v);
+      }
+      const rsrc_t ro = make_rsrc(static_cast<char*>(A.out) + (batch * A.o_sb + h * A.o_sh +
+                                                               static_cast<long long>(t0) * A.o_st) * size,
+                                  0x7fffffffu);
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        const int tok = NC * t + nn;
+        const float w = sW[kWg * 64 + tok] * A.scale;
+#pragma unroll
+        for (int r = 0; r < RT; ++r) O[t][r] *= w;
+#pragma unroll
+        for (int f = 0; f < TF; ++f)
+          if (Mat::any(t, f)) mul<NC>(O[t], uo[f], Mat::get(sS + kDrTiles, t, f, nn, g));
+        if (poisoned) {
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+            const int s = __shfl(stop, 4 * G * (r >> 2) + 4 * g + (r & 3));
+            if (tok >= s) O[t][r] = __int_as_float(0x7fc00000);
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < RT / 4; ++q) {
+          const int cc = col0 + NC * wave + 4 * G * q + 4 * g;
+          const uint32_t at = (tok * static_cast<int>(A.o_st) + cc) * size;
+          if constexpr (kNarrow) {
+            __builtin_amdgcn_raw_buffer_store_b64(
+                u2{pack_bf16x2(O[t][4 * q], O[t][4 * q + 1]), pack_bf16x2(O[t][4 * q + 2], O[t][4 * q + 3])},
+                ro, la_in((tok < n) & (cc < A.Dv), at), 0, 0);
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const uint32_t to = la_in((tok < n) & (cc + r < A.Dv), at + r * size);
+              if (A.dtype == PRNN_F32)
+                stb<float>(ro, to, 0, O[t][4 * q + r]);
+              else if (A.dtype == PRNN_F16)
+                stb<f16>(ro, to, 0, O[t][4 * q + r]);
+              else
+                stb<bf16>(ro, to, 0, O[t][4 * q + r]);
+            }
+          }
+        }
+      }
+      if (A.e) {
+        const rsrc_t re = make_rsrc(static_cast<E*>(A.e) + ((tok0 + t0) * A.H + h) * A.Dv, 0x7fffffffu);
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          const int tok = at_token(i);
+          const float v = tok >= stop ? __int_as_float(0x7fc00000) : Y[i / RT][i % RT];
+          store_elem<M>(re, la_in((tok < n) & (col < A.Dv), (tok * A.H * A.Dv + col) * ES), v);
+        }
+      }
+    }
+    if constexpr (KIND == kDrBackward) {
+      // ---- db: du . e over the wave's columns; dv
+      float d[NC];
+      const char* eat = sE + NC * wave * ES + col_share<M, G, RZ>(lane);
+#pragma unroll
+      for (int f = 0; f < TF; ++f) {
+        float v[8];
+        values(col_op<M, G, RZ>(eat, 8 * G * f, 0), v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int i = 8 * f + e;
+          d[i] = col < A.Dv ? v[e] * Y[i / RT][i % RT] : 0.0f;
+        }
+      }
+      float sum;
+      int which;  // element whose sum this lane has
+      if constexpr (NC == 32) {
+        float h2[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(d[i]), __float_as_uint(d[16 + i]), false, false);
+          h2[i] = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+        }
+        sum = row_sums16(h2, lane);
+        which = lane & 31;
+      } else {
+        sum = row_sums16(d, lane);
+        which = lane & 15;
+      }
+      const int tok = at_token(which);
+      if (tok < n)
+        A.db[(static_cast<size_t>(tile * W + wave) * A.tokens + tok0 + t0 + tok) * A.H + h] = sum;
+      const rsrc_t rd = make_rsrc(static_cast<E*>(A.dv) + ((tok0 + t0) * A.H + h) * A.Dv, 0x7fffffffu);
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        const int tk = at_token(i);
+        store_elem<M>(rd, la_in((tk < n) & (col < A.Dv), (tk * A.H * A.Dv + col) * ES), u[i]);
+      }
+      if (A.dv32) {
+        const rsrc_t rf = make_rsrc(A.dv32 + ((tok0 + t0) * A.H + h) * A.Dv, 0x7fffffffu);
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          const int tk = at_token(i);
+          stb<float>(rf, la_in((tk < n) & (col < A.Dv), (tk * A.H * A.Dv + col) * 4), 0, u[i]);
+        }
+      }
+    }
+
+    // ---- the state behind (backwards: the adjoint before) the chunk
+    const float tot = sW[kWmeta * 64];
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int r = 0; r < RT; ++r) S[t][r] *= tot;
+    const char* kat = sK + col_share<M, G, RK>(lane);
+    const char* qat = sQ + col_share<M, G, RK>(lane);
+#pragma unroll
+    for (int f = 0; f < TF; ++f) {
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; e += 4) {
+        const f4 w = weight(kBack ? kWg : kWr, 8 * f + e);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[e + r] = (kBack ? -w[r] : w[r]) * u[8 * f + e + r];
+      }
+      const auto uo = parts_of<M, 3>(v);
+#pragma unroll
+      for (int t = 0; t < KT; ++t) mul<NC>(S[t], col_op<M, G, RK>(kat, 8 * G * f, NC * t), uo);
+      if constexpr (kBack) {
+        float z[8];
+        values(zo[f], z);
+#pragma unroll
+        for (int e = 0; e < 8; e += 4) {
+          const f4 w = weight(kWg, 8 * f + e);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) z[e + r] *= w[r] * A.scale;
+        }
+        const auto go = parts_of<M, 3>(z);
+#pragma unroll
+        for (int t = 0; t < KT; ++t) mul<NC>(S[t], col_op<M, G, RK>(qat, 8 * G * f, NC * t), go);
+      }
+    }
+    if (!kBack && poisoned && stop < kDrC) {
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) S[t][r] = __int_as_float(0x7fc00000);
+    }
+    __syncthreads();
+  }
+
+  // ---- the state behind the piece
+  float* dst = nullptr;
+  if (kOwn) {
+    dst = transfer ? A.transfer + (static_cast<size_t>(piece) * A.H + h) * A.Dk * A.Dk
+                   : A.piece + (static_cast<size_t>(piece) * A.H + h) * state_floats;
+  } else if (pc.index == (kBack ? 0 : pc.count - 1)) {
+    if (float* row = la_row(A.last, pc.seq, A.H * state_floats)) dst = row + h * state_floats;
+  }
+  if (dst) {
+    const rsrc_t rs = make_rsrc(dst, static_cast<uint32_t>(A.Dk * width) * 4);
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        const int i = NC * t + 4 * G * (r >> 2) + 4 * g + (r & 3);
+        stb<float>(rs, la_in((i < A.Dk) & (col < width), (i * width + col) * 4), 0, S[t][r]);
+      }
+  }
+}
+
+template <class M, int NC, int KD, int W, int KIND>
+int dr_launch_walk(const DrWalk& a, hipStream_t stream) {
+  const long long items = dr_units(a.seqs, a.seqs.len) * a.H;
+  const long long groups = (items + 7) / 8 * 8 * a.tiles;
+  if (int rc = check_grid("delta_rule", groups, 64 * W)) return rc;
+  dr_walk_kernel<M, NC, KD, W, KIND><<<static_cast<unsigned>(groups), 64 * W, 0, stream>>>(a);
+  PRNN_HIP(hipGetLastError());
+  return PRNN_OK;
+}
+
+}  // namespace prnn

@@ -1,0 +1,36 @@
+// Gated delta rule, the walks forwards on bf16 matrix instructions.
+#include "delta_rule_walk.h"
+
+namespace prnn {
+namespace {
+
+template <int KIND, int KD>
+int launch_cols(const DrWalk& a, int cols, hipStream_t stream) {
+  const int group = dr_walk_cols(a.Dk, a.Dv, cols, true).group;
+  if (cols == 16 && group == 4) return dr_launch_walk<InBf16, 16, KD, 4, KIND>(a, stream);
+  if constexpr (KD <= 128) {
+    if (cols == 16) return dr_launch_walk<InBf16, 16, KD, 2, KIND>(a, stream);
+    if (group == 4) return dr_launch_walk<InBf16, 32, KD, 4, KIND>(a, stream);
+    if constexpr (KD <= 64) return dr_launch_walk<InBf16, 32, KD, 2, KIND>(a, stream);
+  }
+  return fail(PRNN_ERR_RUNTIME, "no walk of %d columns a wave for keys of %d", cols, a.Dk);
+}
+template <int KIND>
+int launch_kd(const DrWalk& a, int cols, hipStream_t stream) {
+  if (a.Dk <= 32) return launch_cols<KIND, 32>(a, cols, stream);
+  if (a.Dk <= 64) return launch_cols<KIND, 64>(a, cols, stream);
+  if (a.Dk <= 128) return launch_cols<KIND, 128>(a, cols, stream);
+  return launch_cols<KIND, 256>(a, cols, stream);
+}
+
+}  // namespace
+
+int dr_walk_bf16(const DrWalk& a, DrKind kind, int cols, hipStream_t stream) {
+  switch (kind) {
+    case kDrForward: return launch_kd<kDrForward>(a, cols, stream);
+    case kDrState: return launch_kd<kDrState>(a, cols, stream);
+    default: return dr_walk_bf16_back(a, kind, cols, stream);
+  }
+}
+
+}  // namespace prnn

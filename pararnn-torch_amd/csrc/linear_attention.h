@@ -290,4 +290,21 @@ int la_f32_tile_cols(int vd);
 int la_walk_bf16(LaParams p, int roles, bool state_only, bool dots, hipStream_t stream);
 int la_bf16_tile_cols(int vd);
 
+// What the entry points check of a problem, and an array of it as the kernels read it (D: its width).
+int la_check(const prnn_linear_attention_problem* a);
+LaView la_view(const prnn_la_view& v, const prnn_linear_attention_problem& a, int D);
+
+// Gradients of shared heads: dst (token, H / rep, D) of the storage type, the sums of src (token, H,
+// D) over heads that share an array, in their order.  src NULL: nothing to do.
+struct LaHeadSums {
+  const float* src[3];
+  void* dst[3];
+  int rep[3], D[3];
+  int H;
+  size_t tokens;
+};
+int la_head_sums(const LaHeadSums& a, int dtype, hipStream_t stream);
+// dg (H) = the sums of per_part (parts, H), in a fixed order.
+int la_decay_sums(const float* per_part, void* dg, int g_dtype, int parts, int H, hipStream_t stream);
+
 }  // namespace prnn

@@ -295,17 +295,9 @@ __global__ __launch_bounds__(64) void la_decay_sum_kernel(const float* __restric
 
 // ---- gradients of shared heads ---------------------------------------------------------
 
-struct HeadSumArgs {
-  const float* src[3];  // (token, H, D)
-  void* dst[3];         // (token, H / rep, D)
-  int rep[3], D[3];
-  int H;
-  size_t tokens;
-};
-
 // Bound by memory: 3003 tokens, 6 heads to 3 in fp32, (48, 72): 6.6 us.
 template <typename T>
-__global__ __launch_bounds__(256) void la_head_sum_kernel(HeadSumArgs A) {
+__global__ __launch_bounds__(256) void la_head_sum_kernel(LaHeadSums A) {
   const int k = blockIdx.y;
   if (A.src[k] == nullptr) return;
   const int D = A.D[k], rep = A.rep[k], heads = A.H / rep;
@@ -643,7 +635,7 @@ int backward(const Problem& a, const prnn_la_view& go, const float* gs, void* dq
   p.role[2] = role(k, q, o, a.Dk, a.Dv, false, 1);
   void* outs[3] = {dq, dk, dv};
   const int D[3] = {a.Dk, a.Dk, a.Dv}, heads[3] = {a.q.heads, a.k.heads, a.v.heads};
-  HeadSumArgs hs{};
+  LaHeadSums hs{};
   bool sums = false;
   for (int i = 0; i < 3; ++i) {
     LaRole& r = p.role[i];
@@ -669,17 +661,10 @@ int backward(const Problem& a, const prnn_la_view& go, const float* gs, void* dq
   }
   if (int rc = w.run(p, 3, false, dg != nullptr, st)) return rc;
   const size_t tokens = static_cast<size_t>(a.B) * a.T;
-  if (sums && tokens) {
+  if (sums) {
     hs.H = a.H;
     hs.tokens = tokens;
-    const size_t most = tokens * a.H * std::max(a.Dk, a.Dv);
-    const unsigned blocks = static_cast<unsigned>(std::min<size_t>((most + 1023) / 1024, 4096));
-    if (int rc = with_storage(a.dtype, [&](auto z) {
-          la_head_sum_kernel<decltype(z)><<<dim3(blocks, 3), 256, 0, st>>>(hs);
-          PRNN_HIP(hipGetLastError());
-          return static_cast<int>(PRNN_OK);
-        }))
-      return rc;
+    if (int rc = la_head_sums(hs, a.dtype, st)) return rc;
   }
   if (dg) {
     DecayGradArgs d{};
@@ -707,14 +692,36 @@ int backward(const Problem& a, const prnn_la_view& go, const float* gs, void* dq
     la_decay_grad_kernel<<<grid, 256, 0, st>>>(d);
     PRNN_HIP(hipGetLastError());
     if (per_head) {
-      la_decay_sum_kernel<<<a.H, 64, 0, st>>>(s.per_part, dg, a.g_dtype, d.seqs.pieces, a.H);
-      PRNN_HIP(hipGetLastError());
+      if (int rc = la_decay_sums(s.per_part, dg, a.g_dtype, d.seqs.pieces, a.H, st)) return rc;
     }
   }
   return PRNN_OK;
 }
 
 }  // namespace
+
+int la_check(const prnn_linear_attention_problem* a) { return check(a); }
+LaView la_view(const prnn_la_view& v, const prnn_linear_attention_problem& a, int D) {
+  return view(v, a, D);
+}
+
+int la_head_sums(const LaHeadSums& a, int dtype, hipStream_t stream) {
+  if (a.tokens == 0) return PRNN_OK;
+  const size_t most = a.tokens * a.H * std::max({a.D[0], a.D[1], a.D[2]});
+  const unsigned blocks = static_cast<unsigned>(std::min<size_t>((most + 1023) / 1024, 4096));
+  return with_storage(dtype, [&](auto z) {
+    la_head_sum_kernel<decltype(z)><<<dim3(blocks, 3), 256, 0, stream>>>(a);
+    PRNN_HIP(hipGetLastError());
+    return static_cast<int>(PRNN_OK);
+  });
+}
+
+int la_decay_sums(const float* per_part, void* dg, int g_dtype, int parts, int H, hipStream_t stream) {
+  la_decay_sum_kernel<<<H, 64, 0, stream>>>(per_part, dg, g_dtype, parts, H);
+  PRNN_HIP(hipGetLastError());
+  return PRNN_OK;
+}
+
 }  // namespace prnn
 
 using namespace prnn;

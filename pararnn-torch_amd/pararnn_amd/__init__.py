@@ -18,6 +18,7 @@ from pararnn_amd.config import (
     NewtonStats,
     compile_safe_config,
 )
+from pararnn_amd.delta import delta_rule, delta_rule_step
 from pararnn_amd.newton import (
     auto_newton_iters,
     fused_newton,
@@ -65,6 +66,8 @@ __all__ = [
     "compile_safe_config",
     "copy_pages",
     "default_agreement_atol",
+    "delta_rule",
+    "delta_rule_step",
     "fork_pages",
     "free_pages",
     "fused_newton",

@@ -48,6 +48,13 @@ class LaProblem(ctypes.Structure):
                 ("scale", ctypes.c_float), ("longest", ctypes.c_int)]
 
 
+class DeltaProblem(ctypes.Structure):
+    """``prnn_delta_rule_problem``."""
+
+    _fields_ = [("la", LaProblem), ("b", ctypes.c_void_p), ("b_sb", ctypes.c_longlong),
+                ("b_st", ctypes.c_longlong), ("b_sh", ctypes.c_longlong), ("b_dtype", ctypes.c_int)]
+
+
 class Pool(ctypes.Structure):
     """``prnn_pool``."""
 
@@ -62,6 +69,7 @@ _S = ctypes.c_size_t
 _L = ctypes.c_longlong
 _LAP = ctypes.POINTER(LaProblem)
 _LAV = ctypes.POINTER(LaView)
+_DRP = ctypes.POINTER(DeltaProblem)
 _PP = ctypes.POINTER(Pool)
 SIGNATURES: dict[str, tuple] = {
     "prnn_abi_version": (_I, []),
@@ -155,6 +163,15 @@ SIGNATURES: dict[str, tuple] = {
     "prnn_linear_attention_step": (
         _I, [_P, _L, _L, _I, _P, _L, _L, _I, _P, _L, _L, _I, _P, _L, _L, _I, _P, _P, _I, _P,
              _I, _I, _I, _I, _F, _I, _P]),
+    "prnn_delta_rule_workspace_size": (_S, [_DRP]),
+    "prnn_delta_rule_kept_size": (_S, [_DRP]),
+    "prnn_delta_rule": (_I, [_DRP, _LAV, _P, _P, _I, _P, _P, _S, _P]),
+    "prnn_delta_rule_backward_workspace_size": (_S, [_DRP, _I]),
+    "prnn_delta_rule_backward": (
+        _I, [_DRP, _LAV, _P, _P, _P, _P, _P, _P, _P, _P, _P, _S, _P]),
+    "prnn_delta_rule_step": (
+        _I, [_P, _L, _L, _I, _P, _L, _L, _I, _P, _L, _L, _I, _P, _L, _L, _I, _P, _L, _L, _I, _P, _P,
+             _I, _P, _I, _I, _I, _I, _F, _I, _P]),
     "prnn_group_norm_workspace_size": (_S, [_I, _I, _I, _I, _I, _I]),
     "prnn_group_norm": (
         _I, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _F, _I, _I, _I, _P, _S, _P]),

@@ -176,9 +176,11 @@ def _at(t: Tensor | None) -> int | None:
 class _Problem:
     """A checked call: the C problem and the tensors that it points to."""
 
+    what = "linear_attention"
+
     def __init__(self, q: Tensor, k: Tensor, v: Tensor, g: Tensor, h0: Tensor | None,
                  table: Tensor | None, packed: PackedSequences | None, scale: float | None):
-        what = "linear_attention"
+        what = self.what
         code = _DTYPES.get(q.dtype)
         # the quick look first: calls of small sizes are bound by the host
         if not (code is not None and q.is_cuda and k.dtype is q.dtype and v.dtype is q.dtype
@@ -246,7 +248,9 @@ class _Problem:
 
     def again(self, q: Tensor, k: Tensor, v: Tensor, g: Tensor, h0: Tensor | None) -> _Problem:
         """The same checked call on tensors like those it was made of (backward)."""
-        p = object.__new__(_Problem)
+        return self._onto(object.__new__(_Problem), q, k, v, g, h0)
+
+    def _onto(self, p, q: Tensor, k: Tensor, v: Tensor, g: Tensor, h0: Tensor | None):
         p.q, p.k, p.v, p.g = _tiles(q), _tiles(k), _tiles(v), g
         p.h0 = None if h0 is None else h0.contiguous()
         p.dims, p.codes, p.scale = self.dims, self.codes, self.scale
@@ -254,6 +258,30 @@ class _Problem:
         p.longest = self.longest
         p._fill()
         return p
+
+    def destination(self, block_table: Tensor | None, state_out: Tensor | None,
+                    state_table: Tensor | None, return_state: bool):
+        """(where the final states go, the table of their rows) of a call without gradients."""
+        _, _, heads, dk, dv = self.dims
+        q, what = self.q, self.what
+        if state_out is None:
+            if not return_state:
+                return None, None
+            return q.new_empty(self.sequences, heads, dk, dv, dtype=torch.float32), None
+        if return_state:
+            raise ValueError(f"{what}: state_out and return_state exclude each other")
+        table = None
+        if state_table is not None:
+            table = _check_table(what, "state_table", state_table, self.sequences, q.device)
+        elif block_table is not None:
+            table = self.table if self.table is not None else _check_table(
+                what, "block_table", block_table, self.sequences, q.device)
+        _check_state(what, "state_out", state_out, q, (heads, dk, dv),
+                     self.sequences if table is None else None)
+        if not state_out.is_contiguous():
+            raise ValueError(f"{what}: state_out must be contiguous")
+        _writes(what, state_out)
+        return state_out, table
 
     def forget(self) -> _Problem:
         """Keeps what was checked, not the tensors."""
@@ -367,24 +395,7 @@ def linear_attention(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, *,
         raise RuntimeError("linear_attention: block_table and state_out are inference-only; call "
                            "it under torch.no_grad()")
     p = _Problem(q, k, v, log_decay, h0, None if h0 is None else block_table, packed, scale)
-    _, _, heads, dk, dv = p.dims
-    dest, table = None, None
-    if state_out is not None:
-        if return_state:
-            raise ValueError("linear_attention: state_out and return_state exclude each other")
-        if state_table is not None:
-            table = _check_table("linear_attention", "state_table", state_table, p.sequences, q.device)
-        elif block_table is not None:
-            table = p.table if p.table is not None else _check_table(
-                "linear_attention", "block_table", block_table, p.sequences, q.device)
-        _check_state("linear_attention", "state_out", state_out, q, (heads, dk, dv),
-                     p.sequences if table is None else None)
-        if not state_out.is_contiguous():
-            raise ValueError("linear_attention: state_out must be contiguous")
-        _writes("linear_attention", state_out)
-        dest = state_out
-    elif return_state:
-        dest = q.new_empty(p.sequences, heads, dk, dv, dtype=torch.float32)
+    dest, table = p.destination(block_table, state_out, state_table, return_state)
     out = _forward(p, dest, table)
     return (out, dest) if return_state else out
 
