@@ -616,6 +616,26 @@ PRNN_API int prnn_group_norm_backward(const void* gy, const void* x, const void*
                                       int act, int w_dtype, int dtype, void* workspace,
                                       size_t workspace_bytes, void* stream);
 
+/* ---- Residual norm -----------------------------------------------------------
+ * The norms behind and before a block with its gate and residual scale, rows (N, C), C <= 16384:
+ *   f = norm(y) pw (post) or y;  h = x + scale act(gate) f;  z = norm(h) w + b.
+ * norm: (t - mean) rstd, or without the mean (layer = 0).  y NULL: z = norm(x) w + b alone.  act of
+ * the gate: 0 itself, 1 silu, 2 sigmoid; gate NULL: 1.  w, b, pw, scale (C; NULL: 1, 0, 1,
+ * scale_number) float32 or of x's type.  Backward: gh and gz (one may be NULL: zero); any gradient
+ * may be NULL; workspace only for dw, db, dpw, dscale. */
+PRNN_API int prnn_residual_norm(const void* x, const void* y, const void* w, const void* b,
+                                const void* pw, const void* gate, const void* scale,
+                                float scale_number, void* h, void* z, int N, int C, float eps,
+                                int layer, int post, int act, int w_dtype, int dtype, void* stream);
+PRNN_API size_t prnn_residual_norm_backward_workspace_size(int N, int C);
+PRNN_API int prnn_residual_norm_backward(const void* gh, const void* gz, const void* x,
+                                         const void* y, const void* w, const void* pw,
+                                         const void* gate, const void* scale, float scale_number,
+                                         void* dx, void* dy, void* dw, void* db, void* dpw,
+                                         void* dgate, void* dscale, int N, int C, float eps,
+                                         int layer, int post, int act, int w_dtype, int dtype,
+                                         void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- Pages of a state cache ------------------------------------------------
  * A cache is one or several pools whose rows 0 .. slots - 1 belong together (a slot), and used
  * (slots) int32: 0 = free.  Lists are int32 on the device; entries outside 0 .. slots - 1 are

@@ -32,3 +32,25 @@ def delta_rule(q, k, v, log_decay, beta, h0=None, scale=None, cu=None):
     parts = [walk(*(x[:, cu[i]:cu[i + 1]] for x in (q, k, v, a, beta)), h0[i:i + 1])
              for i in range(S)]
     return torch.cat([o for o, _ in parts], 1), torch.cat([s for _, s in parts])
+
+
+def residual_norm(x, y, weight=None, bias=None, post_norm=False, post_weight=None, gate=None,
+                  activation=None, scale=1.0, norm="rms", eps=1e-6):
+    """(h, z) of one token after another's channels."""
+
+    def normed(t):
+        if norm == "layer":
+            t = t - t.mean(-1, keepdim=True)
+        return t / torch.sqrt((t * t).mean(-1, keepdim=True) + eps)
+
+    h = x
+    if y is not None:
+        f = normed(y) if post_norm else y
+        f = f if post_weight is None else f * post_weight
+        if gate is not None:
+            f = f * {None: lambda t: t, "sigmoid": torch.sigmoid,
+                     "silu": lambda t: t * torch.sigmoid(t)}[activation](gate)
+        h = x + scale * f
+    z = normed(h)
+    z = z if weight is None else z * weight
+    return h, z if bias is None else z + bias

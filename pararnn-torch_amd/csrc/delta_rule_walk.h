@@ -190,6 +190,85 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
       re.fetch(static_cast<const char*>(A.e) + ((tok0 + t) * A.H + h) * A.Dv * ES,
                static_cast<long long>(A.H) * A.Dv, n, col0, A.Dv, kNarrow ? PRNN_BF16 : PRNN_F32);
   };
+  // What a chunk leaves is stored after the next one's rows have come: loads and stores come back in
+  // order, and a wait for rows behind stores would wait for those too (155 us for .. without).
+  constexpr int kHeld = kNarrow ? NC / 2 : NC;
+  uint32_t held_o[KIND == kDrForward ? kHeld : 1], held_u[kOwn ? 1 : kHeld];  // out; e or dv
+  float held32[KIND == kDrBackward && kNarrow ? NC : 1], held_db = 0.0f;
+  int held_n = 0, held_c = 0;
+  auto at_token = [&](int i) { return NC * (i / RT) + 4 * G * ((i % RT) >> 2) + 4 * g + (i & 3); };
+  auto hold = [&](uint32_t* to, const float* v) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      if constexpr (kNarrow)
+        to[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+      else
+        to[i] = __float_as_uint(v[i]);
+    }
+  };
+  auto flush = [&]() {
+    const int t0 = pc.begin + held_c * kDrC, n = held_n;  // nothing held: 0 tokens
+    if constexpr (KIND == kDrForward) {
+      const rsrc_t ro = make_rsrc(static_cast<char*>(A.out) + (batch * A.o_sb + h * A.o_sh +
+                                                               static_cast<long long>(t0) * A.o_st) * size,
+                                  0x7fffffffu);
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        const int tok = NC * t + nn;
+#pragma unroll
+        for (int q = 0; q < RT / 4; ++q) {
+          const int cc = col0 + NC * wave + 4 * G * q + 4 * g;
+          const uint32_t at = (tok * static_cast<int>(A.o_st) + cc) * size;
+          if constexpr (kNarrow) {
+            const int i = (RT * t + 4 * q) / 2;
+            __builtin_amdgcn_raw_buffer_store_b64(u2{held_o[i], held_o[i + 1]}, ro,
+                                                  la_in((tok < n) & (cc < A.Dv), at), 0, 0);
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const uint32_t to = la_in((tok < n) & (cc + r < A.Dv), at + r * size);
+              const float v = __uint_as_float(held_o[RT * t + 4 * q + r]);
+              if (A.dtype == PRNN_F32)
+                stb<float>(ro, to, 0, v);
+              else if (A.dtype == PRNN_F16)
+                stb<f16>(ro, to, 0, v);
+              else
+                stb<bf16>(ro, to, 0, v);
+            }
+          }
+        }
+      }
+    }
+    if constexpr (!kOwn) {
+      void* p = kBack ? A.dv : A.e;
+      if (p) {
+        const rsrc_t r = make_rsrc(static_cast<E*>(p) + ((tok0 + t0) * A.H + h) * A.Dv, 0x7fffffffu);
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          const int tok = at_token(i);
+          const uint32_t to = la_in((tok < n) & (col < A.Dv), (tok * A.H * A.Dv + col) * ES);
+          if constexpr (kNarrow)
+            __builtin_amdgcn_raw_buffer_store_b16(i & 1 ? held_u[i / 2] >> 16 : held_u[i / 2], r, to, 0, 0);
+          else
+            __builtin_amdgcn_raw_buffer_store_b32(held_u[i], r, to, 0, 0);
+        }
+      }
+    }
+    if constexpr (KIND == kDrBackward) {
+      const int tok = at_token(lane % NC);
+      if (tok < n) A.db[(static_cast<size_t>(tile * W + wave) * A.tokens + tok0 + t0 + tok) * A.H + h] = held_db;
+      if constexpr (kNarrow) {
+        if (A.dv32) {
+          const rsrc_t rf = make_rsrc(A.dv32 + ((tok0 + t0) * A.H + h) * A.Dv, 0x7fffffffu);
+#pragma unroll
+          for (int i = 0; i < NC; ++i) {
+            const int tk = at_token(i);
+            stb<float>(rf, la_in((tk < n) & (col < A.Dv), (tk * A.H * A.Dv + col) * 4), 0, held32[i]);
+          }
+        }
+      }
+    }
+  };
   if (chunks > 0) fetch(kBack ? chunks - 1 : 0);
 
   for (int step = 0; step < chunks; ++step) {
@@ -209,10 +288,7 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
 #pragma unroll
     for (int k = 0; k < (kDrW * 16 + NT - 1) / NT; ++k)
       if (tid + k * NT < kDrW * 16) *reinterpret_cast<u4*>(reinterpret_cast<char*>(sW) + (tid + k * NT) * 16) = rw[k];
-    const char* sS = kSysLds ? s_sys : A.sys + (static_cast<size_t>(row0 + c) * A.H + h) * kDrSys;
-    __syncthreads();
-    if (step + 1 < chunks) fetch(kBack ? c - 1 : c + 1);
-
+    if (!kOwn) flush();
     // what the gradients of this chunk need of the state
     if (!kOwn && A.keep) {
       const rsrc_t rs = make_rsrc(static_cast<E*>(A.keep) + (static_cast<size_t>(row0 + c) * A.H + h) * state_floats,
@@ -225,6 +301,9 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
           store_elem<M>(rs, la_in((i < A.Dk) & (col < A.Dv), (i * A.Dv + col) * ES), S[t][r]);
         }
     }
+    const char* sS = kSysLds ? s_sys : A.sys + (static_cast<size_t>(row0 + c) * A.H + h) * kDrSys;
+    __syncthreads();
+    if (step + 1 < chunks) fetch(kBack ? c - 1 : c + 1);
 
     // ---- x = K S and the state's part of the output, S^T Q^T
     A_t X[TT], O[TT];
@@ -247,7 +326,6 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
 
     const char* zat = sZ + NC * wave * ES + col_share<M, G, RZ>(lane);
     float y[NC];  // the system's right side: token of element i at_token(i)
-    auto at_token = [&](int i) { return NC * (i / RT) + 4 * G * ((i % RT) >> 2) + 4 * g + (i & 3); };
     auto weight = [&](int which, int i) {  // of elements i .. i + 3
       return *reinterpret_cast<const f4*>(&sW[which * 64 + at_token(i)]);
     };
@@ -354,9 +432,6 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
         for (int e = 0; e < 8; ++e) v[e] = u[8 * f + e];
         uo[f] = parts_of<M, 2>(v);
       }
-      const rsrc_t ro = make_rsrc(static_cast<char*>(A.out) + (batch * A.o_sb + h * A.o_sh +
-                                                               static_cast<long long>(t0) * A.o_st) * size,
-                                  0x7fffffffu);
 #pragma unroll
       for (int t = 0; t < TT; ++t) {
         const int tok = NC * t + nn;
@@ -373,36 +448,16 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
             if (tok >= s) O[t][r] = __int_as_float(0x7fc00000);
           }
         }
-#pragma unroll
-        for (int q = 0; q < RT / 4; ++q) {
-          const int cc = col0 + NC * wave + 4 * G * q + 4 * g;
-          const uint32_t at = (tok * static_cast<int>(A.o_st) + cc) * size;
-          if constexpr (kNarrow) {
-            __builtin_amdgcn_raw_buffer_store_b64(
-                u2{pack_bf16x2(O[t][4 * q], O[t][4 * q + 1]), pack_bf16x2(O[t][4 * q + 2], O[t][4 * q + 3])},
-                ro, la_in((tok < n) & (cc < A.Dv), at), 0, 0);
-          } else {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const uint32_t to = la_in((tok < n) & (cc + r < A.Dv), at + r * size);
-              if (A.dtype == PRNN_F32)
-                stb<float>(ro, to, 0, O[t][4 * q + r]);
-              else if (A.dtype == PRNN_F16)
-                stb<f16>(ro, to, 0, O[t][4 * q + r]);
-              else
-                stb<bf16>(ro, to, 0, O[t][4 * q + r]);
-            }
-          }
-        }
       }
-      if (A.e) {
-        const rsrc_t re = make_rsrc(static_cast<E*>(A.e) + ((tok0 + t0) * A.H + h) * A.Dv, 0x7fffffffu);
+      float v[NC];
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-          const int tok = at_token(i);
-          const float v = tok >= stop ? __int_as_float(0x7fc00000) : Y[i / RT][i % RT];
-          store_elem<M>(re, la_in((tok < n) & (col < A.Dv), (tok * A.H * A.Dv + col) * ES), v);
-        }
+      for (int i = 0; i < NC; ++i) v[i] = O[i / RT][i % RT];
+      hold(held_o, v);
+      if (A.e) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i)
+          v[i] = at_token(i) >= stop ? __int_as_float(0x7fc00000) : Y[i / RT][i % RT];
+        hold(held_u, v);
       }
     }
     if constexpr (KIND == kDrBackward) {
@@ -419,8 +474,6 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
           d[i] = col < A.Dv ? v[e] * Y[i / RT][i % RT] : 0.0f;
         }
       }
-      float sum;
-      int which;  // element whose sum this lane has
       if constexpr (NC == 32) {
         float h2[16];
 #pragma unroll
@@ -428,30 +481,18 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
           const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(d[i]), __float_as_uint(d[16 + i]), false, false);
           h2[i] = __uint_as_float(s[0]) + __uint_as_float(s[1]);
         }
-        sum = row_sums16(h2, lane);
-        which = lane & 31;
+        held_db = row_sums16(h2, lane);
       } else {
-        sum = row_sums16(d, lane);
-        which = lane & 15;
+        held_db = row_sums16(d, lane);
       }
-      const int tok = at_token(which);
-      if (tok < n)
-        A.db[(static_cast<size_t>(tile * W + wave) * A.tokens + tok0 + t0 + tok) * A.H + h] = sum;
-      const rsrc_t rd = make_rsrc(static_cast<E*>(A.dv) + ((tok0 + t0) * A.H + h) * A.Dv, 0x7fffffffu);
+      hold(held_u, u);
+      if constexpr (kNarrow) {
 #pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        const int tk = at_token(i);
-        store_elem<M>(rd, la_in((tk < n) & (col < A.Dv), (tk * A.H * A.Dv + col) * ES), u[i]);
-      }
-      if (A.dv32) {
-        const rsrc_t rf = make_rsrc(A.dv32 + ((tok0 + t0) * A.H + h) * A.Dv, 0x7fffffffu);
-#pragma unroll
-        for (int i = 0; i < NC; ++i) {
-          const int tk = at_token(i);
-          stb<float>(rf, la_in((tk < n) & (col < A.Dv), (tk * A.H * A.Dv + col) * 4), 0, u[i]);
-        }
+        for (int i = 0; i < NC; ++i) held32[i] = u[i];
       }
     }
+    held_n = n;
+    held_c = c;
 
     // ---- the state behind (backwards: the adjoint before) the chunk
     const float tot = sW[kWmeta * 64];
@@ -495,6 +536,8 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
     }
     __syncthreads();
   }
+
+  if (!kOwn) flush();
 
   // ---- the state behind the piece
   float* dst = nullptr;

@@ -1,0 +1,184 @@
+// Residual norm: the norms behind and before a block with its gate and residual scale.
+//
+//   f = norm(y) p  or  y        a = act(gate)  or  1        h = x + s a f
+//   z = norm(h) w + b           norm(t) = (t - mean) rstd, or without the mean (rms)
+//
+// backwards, with n2 = norm(h), n1 = norm(y), r their rstd, m(.) the mean over a row:
+//
+//   dn2 = gz w,   dh = gh + r2 (dn2 - [m(dn2)] - n2 m(dn2 n2)),   dx = dh,   df = dh s a,
+//   dy = r1 (df p - [m(df p)] - n1 m(df p n1))  or  df,   dgate = dh s f act'(gate),
+//   and sums over rows: dw = gz n2, db = gz, dp = df n1, ds = dh a f.
+//
+// A row lies in the registers of NT threads, E elements each: every array is read once and written
+// once, the statistics are two-pass and the backward pass forms them again from x, y and the gate.
+#pragma once
+
+#include "prnn_host.h"
+
+namespace prnn {
+
+constexpr int kRnMax = 16384;  // channels: 1024 threads of 16
+
+struct RnArgs {
+  const void *x, *y, *w, *b, *pw, *gate, *scale;  // scale NULL: `number`
+  void *h, *z;
+  const void *gh, *gz;
+  void *dx, *dy, *dgate;
+  float* parts;   // (workgroup, 4, C): sums of dw, db, dp, ds over its rows
+  int N, C;
+  int layer, post, act, w_dtype;
+  int want;       // which of the sums (bits 0 .. 3)
+  float number, eps;
+};
+
+int rn_forward(const RnArgs& a, int dtype, bool vec, hipStream_t stream);
+int rn_backward(const RnArgs& a, int dtype, bool vec, int groups, hipStream_t stream);
+
+// Threads of a row: 8 elements each up to 512 threads, then 16 (1024 threads have 128 registers each,
+// where what lies in them spills: only for what does not fit otherwise).
+inline int rn_threads(int C) {
+  int nt = 64;
+  while (nt < 512 && nt * 8 < C) nt *= 2;
+  return C <= 8192 ? nt : 1024;
+}
+// Workgroups of the backward pass: one's sums over its rows are written and read once more, so not
+// more than keep the chip busy.
+inline int rn_groups(int N, int C) {
+  const int rows = rn_threads(C) >= 256 ? 1 : 256 / rn_threads(C);
+  const int groups = (N + rows - 1) / rows;
+  const int most = rn_threads(C) > 256 ? 256 * 1024 / rn_threads(C) : 1024;
+  return groups < most ? groups : most;
+}
+
+template <typename T, int V, int E, int NT>
+struct RnRow {
+  static constexpr int K = E / V;
+  int C, lane;
+  __device__ __forceinline__ int col(int i) const { return ((i / V) * NT + lane) * V + i % V; }
+  // Rows through buffers of their own bytes: columns behind the width are read as zero, not written.
+  __device__ __forceinline__ void load(float* v, const void* p, long long row) const {
+    if (p == nullptr) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) v[i] = 0.0f;
+      return;
+    }
+    const T* at = static_cast<const T*>(p) + row * C;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * NT + lane) * V;
+      if constexpr (V == 1) {
+        v[k] = c < C ? to_f32(at[c]) : 0.0f;
+      } else {
+        typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+        u4 w{0, 0, 0, 0};
+        if (c < C) w = *reinterpret_cast<const u4*>(at + c);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          if constexpr (sizeof(T) == 4)
+            v[k * V + i] = __uint_as_float(w[i]);
+          else
+            v[k * V + i] = i & 1 ? Narrow<T>::hi(w[i / 2]) : Narrow<T>::lo(w[i / 2]);
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void store(void* p, long long row, const float* v) const {
+    if (p == nullptr) return;
+    T* at = static_cast<T*>(p) + row * C;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * NT + lane) * V;
+      if constexpr (V == 1) {
+        if (c < C) at[c] = from_f32<T>(v[k]);
+      } else {
+        typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+        u4 w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (sizeof(T) == 4)
+            w[i] = __float_as_uint(v[k * V + i]);
+          else
+            w[i] = Narrow<T>::pack(v[k * V + 2 * i], v[k * V + 2 * i + 1]);
+        }
+        if (c < C) *reinterpret_cast<u4*>(at + c) = w;
+      }
+    }
+  }
+  // a parameter per channel, `none` where there is none
+  __device__ __forceinline__ void param(float* v, const void* p, int dtype, float none) const {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int c = col(i);
+      v[i] = none;
+      if (p != nullptr && c < C)
+        v[i] = dtype == PRNN_F32 ? static_cast<const float*>(p)[c] : to_f32(static_cast<const T*>(p)[c]);
+    }
+  }
+};
+
+// Sums of two values over the NT threads of a row, in all of them; `turn` alternates the LDS places,
+// so one barrier a sum is enough.
+template <int NT>
+__device__ __forceinline__ void rn_sum(float& a, float& b, float* lds, int& turn) {
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    a += __shfl_xor(a, m);
+    b += __shfl_xor(b, m);
+  }
+  if constexpr (NT > 64) {
+    constexpr int W = NT / 64;
+    const int wave = threadIdx.x >> 6, first = wave / W * W;
+    float* at = lds + turn * 32;
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0) {
+      at[wave * 2] = a;
+      at[wave * 2 + 1] = b;
+    }
+    __syncthreads();
+    a = b = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      a += at[(first + w) * 2];
+      b += at[(first + w) * 2 + 1];
+    }
+  }
+}
+
+// t -> (t - mean) rstd in place; returns rstd.
+template <typename R, int E, int NT>
+__device__ __forceinline__ float rn_norm(const R& row, float* t, int layer, float eps, float* lds, int& turn) {
+  const float inv = 1.0f / static_cast<float>(row.C);
+  if (layer) {
+    float s = 0.0f, none = 0.0f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) s += t[i];  // zeros behind the width
+    rn_sum<NT>(s, none, lds, turn);
+    s *= inv;
+#pragma unroll
+    for (int i = 0; i < E; ++i) t[i] = row.col(i) < row.C ? t[i] - s : 0.0f;
+  }
+  float q = 0.0f, none = 0.0f;
+#pragma unroll
+  for (int i = 0; i < E; ++i) q = fmaf(t[i], t[i], q);
+  rn_sum<NT>(q, none, lds, turn);
+  // not v_rsq_f32: the statistics keep all bits
+  const float r = 1.0f / sqrtf(fmaf(q, inv, eps));
+#pragma unroll
+  for (int i = 0; i < E; ++i) t[i] *= r;
+  return r;
+}
+
+// act(g) in a, its derivative in d.
+__device__ __forceinline__ void rn_act(float g, int act, float& a, float& d) {
+  if (act == 0) {
+    a = g;
+    d = 1.0f;
+    return;
+  }
+  const float e = fexp(-fabsf(g)), s = 1.0f / (1.0f + e);  // of |g|: e is at most 1
+  const float sig = g >= 0.0f ? s : e * s, com = g >= 0.0f ? e * s : s;
+  a = act == 1 ? g * sig : sig;
+  d = act == 1 ? sig * fmaf(g, com, 1.0f) : sig * com;
+}
+
+}  // namespace prnn

@@ -27,7 +27,7 @@ from pararnn_amd.newton import (
     slstm_picard_next,
 )
 from pararnn_amd.layers import ParaRNN
-from pararnn_amd.norm import group_norm
+from pararnn_amd.norm import group_norm, residual_norm
 from pararnn_amd.ops import newton_gru_head_fused, newton_slstm_fused, slstm_init_fused
 from pararnn_amd.pages import (
     compact_pages,
@@ -77,6 +77,7 @@ __all__ = [
     "newton_apply",
     "newton_gru_head_fused",
     "newton_slstm_fused",
+    "residual_norm",
     "sequential_apply",
     "slstm_auto_picard",
     "slstm_init_fused",
