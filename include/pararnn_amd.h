@@ -636,6 +636,18 @@ PRNN_API int prnn_residual_norm_backward(const void* gh, const void* gz, const v
                                          int layer, int post, int act, int w_dtype, int dtype,
                                          void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- Beam search's selection ---------------------------------------------------
+ * The M <= 128 largest of scores[b, k] + log_softmax(logits[b, k])[t] of every search b, the largest
+ * first, ties to the lowest k V + t: their totals, k and t; -infinity, -1 and -1 where there are fewer
+ * (a total of -infinity is never chosen, nor one of a beam whose logits hold an infinity or NaN).
+ * ended (B, K bytes; NULL: none): a beam that goes on with token `pad` alone, at its own score.
+ * logits (B, K, V) by strides of searches and beams. */
+PRNN_API size_t prnn_beam_select_workspace_size(int B, int K, int V, int M);
+PRNN_API int prnn_beam_select(const void* logits, long long l_sb, long long l_sk,
+                              const float* scores, const void* ended, int pad, float* out_scores,
+                              int* out_parents, int* out_tokens, int B, int K, int V, int M,
+                              int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- Pages of a state cache ------------------------------------------------
  * A cache is one or several pools whose rows 0 .. slots - 1 belong together (a slot), and used
  * (slots) int32: 0 = free.  Lists are int32 on the device; entries outside 0 .. slots - 1 are
@@ -657,6 +669,13 @@ PRNN_API int prnn_pages_free(int* used, int slots, const int* list, int n, void*
 /* Slot dst[i] of every pool gets slot src[i]; no dst may be another entry's src or dst. */
 PRNN_API int prnn_pages_copy(int slots, const prnn_pool* pools, int n_pools, const int* src,
                              const int* dst, int n, void* stream);
+/* Beams (B, K) of searches and their children: table (B, K) names the beams' slots, parents (B, K)
+ * each child's beam of its search (outside 0 .. K - 1: none).  A beam's first child keeps its slot, the
+ * other children, in order, take the slots of the beams without children, in order, with a copy of
+ * their parent's slot in every pool; table is rewritten.  K <= 1024; scratch: 2 B K ints.  No two
+ * entries of table name one slot. */
+PRNN_API int prnn_pages_reorder(int slots, const prnn_pool* pools, int n_pools, int* table,
+                                const int* parents, int B, int K, int* scratch, void* stream);
 /* The live slots move into the lowest ones: the i-th lowest free slot below their number gets the
  * i-th lowest live one above it.  tables[k] (lens[k] entries, in place, none overlapping another):
  * live slots become their new places, free ones -1.  live: their number (one int).  scratch: 2 slots + 1 ints. */

@@ -54,3 +54,40 @@ def residual_norm(x, y, weight=None, bias=None, post_norm=False, post_weight=Non
     z = normed(h)
     z = z if weight is None else z * weight
     return h, z if bias is None else z + bias
+
+
+def beam_select(logits, scores, beams, ended=None, pad=0):
+    """Lists (score, parent, token) per search, candidate by candidate in float64."""
+    B, K, V = logits.shape
+    found = []
+    for b in range(B):
+        rows = []
+        for k in range(K):
+            s = float(scores[b, k])
+            if ended is not None and ended[b, k]:
+                rows.append((-s, k, pad))
+                continue
+            x = logits[b, k].double()
+            if bool(torch.isnan(x).any() | (x == float("inf")).any()):
+                continue
+            p = s + torch.log_softmax(x, -1) if bool((x > float("-inf")).any()) else x
+            rows += [(-float(p[t]), k, t) for t in torch.nonzero(p > float("-inf"))[:, 0].tolist()]
+        rows = sorted(r for r in rows if r[0] < float("inf"))[:beams]
+        found.append([(-s, k, t) for s, k, t in rows])
+    return found
+
+
+def reorder_pages(table, parents):
+    """(the new table, {slot: the slot whose rows it takes}) of one search; lists."""
+    K, kept, copies, new = len(table), set(), {}, [None] * len(table)
+    for i, p in enumerate(parents):
+        if 0 <= p < K and p not in kept:
+            kept.add(p)
+            new[i] = table[p]
+    spare = [table[k] for k in range(K) if k not in kept]
+    for i, p in enumerate(parents):
+        if new[i] is None:
+            new[i] = spare.pop(0)
+            if 0 <= p < K:
+                copies[new[i]] = table[p]
+    return new, copies

@@ -1,0 +1,356 @@
+// Beam search: the best continuations over beams and vocabulary.
+//
+//   total(k, t) = score_k + logits_kt - logsumexp_t(logits_kt),  the M largest of a search's K V,
+//   ties to the lowest k V + t.
+//
+// Two launches.  The first reads the logits once: a workgroup per beam and slice of 8192 tokens, 32
+// values a thread in registers, gives the slice's largest value, its sum of exponentials and its M
+// best.  The second, a workgroup per search, joins the slices' sums in fp64 and chooses among the
+// slices' best: candidates of two beams may lie next to each other, and which one goes on must not
+// hang on a sum's rounding.
+//
+// The M best of some thousand values: the M-th largest of the threads' own largest is a bound that at
+// least M values reach, and only values of those M threads can; what reaches it (a few more than M of
+// ordinary logits) is ranked by counting, so the order of arrival does not matter.
+#include <algorithm>
+
+#include "prnn_host.h"
+
+namespace prnn {
+namespace {
+
+constexpr int kMost = 128;     // candidates that are wanted
+constexpr int kEach = 32;      // tokens of a thread
+constexpr int kSlice = 256 * kEach;
+constexpr int kRound = 16;     // candidates of a thread and round of the second launch
+
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+// Order of floats as of unsigned numbers; -infinity and NaN are 0: never chosen.
+__device__ __forceinline__ uint32_t order(float v) {
+  const uint32_t b = __float_as_uint(v);
+  if (!(v > -INFINITY)) return 0u;
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t order(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  if (!(v > -static_cast<double>(INFINITY))) return 0ull;
+  return b >> 63 ? ~b : b | 1ull << 63;
+}
+__device__ __forceinline__ double value(uint64_t o) {
+  return __builtin_bit_cast(double, o >> 63 ? o & ~(1ull << 63) : ~o);
+}
+
+struct Slice {
+  double sum;  // of exp(logit - most)
+  float most;  // NaN: the beam has no finite probabilities
+  int count;
+};
+
+struct BeamArgs {
+  const void* logits;
+  long long sb, sk;
+  const float* scores;
+  const uint8_t* ended;
+  Slice* slices;          // (B K, S)
+  uint2* best;            // (B K, S, M): order and token
+  float* out_scores;
+  int *out_parents, *out_tokens;
+  int B, K, V, M, S, pad;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs A) {
+  constexpr int V = 16 / sizeof(T);
+  __shared__ __align__(16) uint64_t s_top[256];
+  __shared__ uint64_t s_list[kMost * kEach];
+  __shared__ double s_sum[4];
+  __shared__ float s_most[4];
+  __shared__ uint64_t s_bound;
+  __shared__ int s_count;
+  const int tid = threadIdx.x, slice = blockIdx.x % A.S, row = blockIdx.x / A.S;
+  const int b = row / A.K, k = row - b * A.K;
+  if (A.ended && A.ended[row]) return;
+  const T* p = static_cast<const T*>(A.logits) + b * A.sb + k * A.sk;
+  // units of 16 bytes as memory has them; the row starts `skip` values into the first
+  const int skip = static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
+  float v[kEach];
+  bool broken = false;
+#pragma unroll
+  for (int u = 0; u < kEach / V; ++u) {
+    const int t0 = slice * kSlice + (u * 256 + tid) * V - skip;
+    if (t0 >= 0 && t0 + V <= A.V) {
+      const u4 w = *reinterpret_cast<const u4*>(p + t0);
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if constexpr (sizeof(T) == 4)
+          v[u * V + i] = __uint_as_float(w[i]);
+        else
+          v[u * V + i] = i & 1 ? Narrow<T>::hi(w[i / 2]) : Narrow<T>::lo(w[i / 2]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        v[u * V + i] = t0 + i >= 0 && t0 + i < A.V ? to_f32(p[t0 + i]) : -INFINITY;
+    }
+  }
+  float most = -INFINITY;
+  uint64_t top = 0;
+  auto key = [&](int i) {
+    const int t = slice * kSlice + ((i / V) * 256 + tid) * V - skip + i % V;
+    const uint32_t o = order(v[i]);
+    return o ? static_cast<uint64_t>(o) << 32 | static_cast<uint32_t>(~t) : 0ull;
+  };
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    broken |= !(v[i] < INFINITY);  // NaN or infinity
+    most = fmaxf(most, v[i]);
+    const uint64_t o = key(i);
+    top = o > top ? o : top;
+  }
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) most = fmaxf(most, __shfl_xor(most, m));
+  if (__any(broken)) most = INFINITY;
+  s_top[tid] = top;
+  if ((tid & 63) == 0) s_most[tid >> 6] = most;
+  if (tid == 0) {
+    s_bound = 1;
+    s_count = 0;
+  }
+  __syncthreads();
+  most = fmaxf(fmaxf(s_most[0], s_most[1]), fmaxf(s_most[2], s_most[3]));
+  const bool none = most == -INFINITY, bad = most == INFINITY;
+  float part = 0.0f;
+  if (!none && !bad) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) part += fexp(v[i] - most);
+  }
+  double sum = part;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m);
+  if ((tid & 63) == 0) s_sum[tid >> 6] = sum;
+  // this thread's place among the threads' largest
+  int above = 0;
+  if (top) {
+#pragma unroll 8
+    for (int i = 0; i < 256; i += 2) {
+      const ulong2 o = *reinterpret_cast<const ulong2*>(&s_top[i]);
+      above += (o.x > top) + (o.y > top);
+    }
+    if (above == A.M - 1) s_bound = top;
+  }
+  __syncthreads();
+  const uint64_t bound = s_bound;
+  if (top >= bound) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const uint64_t o = key(i);
+      if (o >= bound) s_list[atomicAdd(&s_count, 1)] = o;
+    }
+  }
+  __syncthreads();
+  const int n = s_count;
+  const size_t at = static_cast<size_t>(row) * A.S + slice;
+  for (int i = tid; i < n; i += 256) {
+    const uint64_t o = s_list[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += s_list[j] > o;
+    if (rank < A.M)
+      A.best[at * A.M + rank] = make_uint2(static_cast<uint32_t>(o >> 32), ~static_cast<uint32_t>(o));
+  }
+  if (tid == 0)
+    A.slices[at] = Slice{(s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]), bad ? NAN : most, min(n, A.M)};
+}
+
+__device__ __forceinline__ bool before(uint64_t a, uint32_t ta, uint64_t b, uint32_t tb) {
+  return a > b || (a == b && ta < tb);
+}
+
+__global__ __launch_bounds__(256) void beam_choose_kernel(BeamArgs A) {
+  __shared__ uint64_t s_top[256], s_list[kMost * kRound + kMost];
+  __shared__ uint32_t s_topt[256], s_listt[kMost * kRound + kMost];
+  __shared__ uint64_t s_carry[kMost];
+  __shared__ uint32_t s_carryt[kMost];
+  __shared__ uint64_t s_bound;
+  __shared__ uint32_t s_boundt;
+  __shared__ int s_count, s_held;
+  __shared__ double s_off[kMost], s_most[kMost];  // a total is (logit - most) + off
+  const int tid = threadIdx.x, b = blockIdx.x;
+  const int per = A.S * A.M;  // candidates of a beam
+  if (tid == 0) s_held = 0;
+  // score - log(sum), beams in blocks of kMost; the largest logit stays apart (masks of the type's lowest
+  // value would swallow the logarithm)
+  for (int k0 = 0; k0 < A.K; k0 += kMost) {
+    __syncthreads();
+    for (int k = k0 + tid; k < min(A.K, k0 + kMost); k += 256) {
+      const int row = b * A.K + k;
+      const double score = A.scores[row];
+      double off = score, most = -static_cast<double>(INFINITY);
+      if (!(A.ended && A.ended[row])) {
+        double sum = 0.0;
+        bool bad = false;
+        for (int s = 0; s < A.S; ++s) {
+          const float m = A.slices[static_cast<size_t>(row) * A.S + s].most;
+          bad |= m != m;
+          most = fmax(most, static_cast<double>(m));
+        }
+        for (int s = 0; s < A.S; ++s) {
+          const Slice x = A.slices[static_cast<size_t>(row) * A.S + s];
+          if (x.sum > 0.0) sum += x.sum * exp(static_cast<double>(x.most) - most);
+        }
+        off = bad ? -static_cast<double>(INFINITY) : score - log(sum);
+      }
+      s_off[k - k0] = off;
+      s_most[k - k0] = most;
+    }
+    __syncthreads();
+    const long long end = static_cast<long long>(min(A.K, k0 + kMost)) * per;
+    for (long long base = static_cast<long long>(k0) * per; base < end; base += 256 * kRound) {
+      uint64_t o[kRound], top = 0;
+      uint32_t t[kRound], topt = ~0u;
+#pragma unroll
+      for (int i = 0; i < kRound; ++i) {
+        const long long c = base + i * 256 + tid;
+        o[i] = 0;
+        t[i] = ~0u;
+        if (c >= end) continue;
+        const int k = static_cast<int>(c / per), in = static_cast<int>(c - static_cast<long long>(k) * per);
+        const int row = b * A.K + k;
+        if (A.ended && A.ended[row]) {  // goes on as it is, with one token
+          if (in == 0) {
+            o[i] = order(s_off[k - k0]);
+            t[i] = static_cast<uint32_t>(k) * A.V + A.pad;
+          }
+        } else {
+          const int s = in / A.M, r = in - s * A.M;
+          const size_t at = static_cast<size_t>(row) * A.S + s;
+          if (r < A.slices[at].count) {
+            const uint2 c2 = A.best[at * A.M + r];
+            const float logit = __uint_as_float(c2.x & 0x80000000u ? c2.x & 0x7fffffffu : ~c2.x);
+            o[i] = order((static_cast<double>(logit) - s_most[k - k0]) + s_off[k - k0]);
+            t[i] = static_cast<uint32_t>(k) * A.V + c2.y;
+          }
+        }
+        if (o[i] && before(o[i], t[i], top, topt)) {
+          top = o[i];
+          topt = t[i];
+        }
+      }
+      s_top[tid] = top;
+      s_topt[tid] = topt;
+      if (tid == 0) {
+        s_bound = 1;
+        s_boundt = ~0u;
+      }
+      const int held = s_held;
+      for (int i = tid; i < held; i += 256) {
+        s_list[i] = s_carry[i];
+        s_listt[i] = s_carryt[i];
+      }
+      if (tid == 0) s_count = held;
+      __syncthreads();
+      if (top) {
+        int above = 0;
+        for (int i = 0; i < 256; ++i) above += before(s_top[i], s_topt[i], top, topt);
+        if (above == A.M - 1) {
+          s_bound = top;
+          s_boundt = topt;
+        }
+      }
+      __syncthreads();
+      const uint64_t bound = s_bound;
+      const uint32_t boundt = s_boundt;
+#pragma unroll
+      for (int i = 0; i < kRound; ++i)
+        if (o[i] && !before(bound, boundt, o[i], t[i])) {
+          const int to = atomicAdd(&s_count, 1);
+          s_list[to] = o[i];
+          s_listt[to] = t[i];
+        }
+      __syncthreads();
+      const int n = s_count;
+      for (int i = tid; i < n; i += 256) {
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += before(s_list[j], s_listt[j], s_list[i], s_listt[i]);
+        if (rank < A.M) {
+          s_carry[rank] = s_list[i];
+          s_carryt[rank] = s_listt[i];
+        }
+      }
+      if (tid == 0) s_held = min(n, A.M);
+      __syncthreads();
+    }
+  }
+  __syncthreads();
+  const int held = s_held;
+  for (int i = tid; i < A.M; i += 256) {
+    const bool any = i < held;
+    const size_t at = static_cast<size_t>(b) * A.M + i;
+    A.out_scores[at] = any ? static_cast<float>(value(s_carry[i])) : -INFINITY;
+    A.out_parents[at] = any ? static_cast<int>(s_carryt[i] / A.V) : -1;
+    A.out_tokens[at] = any ? static_cast<int>(s_carryt[i] % A.V) : -1;
+  }
+}
+
+// One slice more than the tokens need: a row may start inside a 16-byte unit.
+int slices_of(int V) { return (V + 15 + kSlice - 1) / kSlice; }
+
+struct Scratch {
+  Slice* slices;
+  uint2* best;
+  size_t bytes;
+};
+Scratch carve(void* ws, int B, int K, int V, int M) {
+  Carver c(ws);
+  Scratch s{};
+  const size_t n = static_cast<size_t>(B) * K * slices_of(V);
+  s.slices = static_cast<Slice*>(c.take(n * sizeof(Slice)));
+  s.best = static_cast<uint2*>(c.take(n * M * sizeof(uint2)));
+  s.bytes = c.used;
+  return s;
+}
+
+int check(int B, int K, int V, int M) {
+  if (B < 0 || K < 1 || V < 1 || M < 1 || M > kMost)
+    return fail(PRNN_ERR_VALUE, "B=%d, K=%d, V=%d, M=%d: M must be in 1 .. %d", B, K, V, M, kMost);
+  if (static_cast<long long>(K) * V >= 1ll << 31 || static_cast<long long>(B) * K >= 1ll << 31)
+    return fail(PRNN_ERR_VALUE, "K=%d beams of V=%d tokens are more than 2^31 - 1", K, V);
+  return PRNN_OK;
+}
+
+}  // namespace
+}  // namespace prnn
+
+using namespace prnn;
+
+extern "C" PRNN_API size_t prnn_beam_select_workspace_size(int B, int K, int V, int M) {
+  return check(B, K, V, M) ? 0 : carve(nullptr, B, K, V, M).bytes;
+}
+
+extern "C" PRNN_API int prnn_beam_select(const void* logits, long long l_sb, long long l_sk,
+                                         const float* scores, const void* ended, int pad,
+                                         float* out_scores, int* out_parents, int* out_tokens, int B,
+                                         int K, int V, int M, int dtype, void* workspace, size_t bytes,
+                                         void* stream) {
+  if (int rc = check_dtype(dtype)) return rc;
+  if (int rc = check(B, K, V, M)) return rc;
+  if (ended && (pad < 0 || pad >= V)) return fail(PRNN_ERR_VALUE, "pad=%d is no token of %d", pad, V);
+  if (B == 0) return PRNN_OK;
+  if (!logits || !scores || !out_scores || !out_parents || !out_tokens)
+    return fail(PRNN_ERR_VALUE, "logits, scores and the outputs must be non-null");
+  const Scratch s = carve(workspace, B, K, V, M);
+  if (workspace == nullptr || bytes < s.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255))
+    return fail(PRNN_ERR_VALUE, "the workspace must hold %zu bytes, 256-byte aligned (got %zu)", s.bytes, bytes);
+  const BeamArgs a{logits, l_sb, l_sk, scores, static_cast<const uint8_t*>(ended), s.slices, s.best,
+                   out_scores, out_parents, out_tokens, B, K, V, M, slices_of(V), pad};
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const long long groups = static_cast<long long>(B) * K * a.S;
+  if (int rc = check_grid("beam_select", groups, 256)) return rc;
+  return with_storage(dtype, [&](auto z) {
+    beam_slice_kernel<decltype(z)><<<static_cast<unsigned>(groups), 256, 0, st>>>(a);
+    PRNN_HIP(hipGetLastError());
+    beam_choose_kernel<<<B, 256, 0, st>>>(a);
+    PRNN_HIP(hipGetLastError());
+    return static_cast<int>(PRNN_OK);
+  });
+}

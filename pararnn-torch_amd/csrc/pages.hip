@@ -157,6 +157,39 @@ __global__ __launch_bounds__(256) void pages_copy_kernel(Pools P, int slots,
   copy_entry(P, s, d, blockIdx.x - i * per);
 }
 
+// A beam's first child keeps its slot; the other children, in order, take the slots of the beams
+// without children, in order, and get a copy.  A workgroup per search; src, dst: the copies, -1 where
+// there is none.  No copy's source is another's destination: one has a child, the other none.
+constexpr int kBeams = kPlan;
+__global__ __launch_bounds__(kPlan) void pages_reorder_kernel(int* table, const int* __restrict__ parents,
+                                                              int K, int slots, int* src, int* dst) {
+  __shared__ int lds[kPlan / 64], first[kBeams], old[kBeams], spare[kBeams];
+  const int i = threadIdx.x;
+  const size_t at = static_cast<size_t>(blockIdx.x) * K + i;
+  const bool in = i < K;
+  int p = in ? parents[at] : -1;
+  if (p >= K) p = -1;
+  if (in) {
+    first[i] = kBeams;
+    old[i] = table[at];
+  }
+  __syncthreads();
+  if (p >= 0) atomicMin(&first[p], i);
+  __syncthreads();
+  const bool barren = in && first[i] == kBeams, other = in && (p < 0 || first[p] != i);
+  int total;
+  const int free = block_rank(barren, lds, total);
+  if (barren) spare[free] = old[i];
+  const int rank = block_rank(other, lds, total);
+  __syncthreads();
+  if (!in) return;
+  const int from = p >= 0 ? old[p] : -1, to = other ? spare[rank] : from;
+  table[at] = to;
+  const bool copy = other && from >= 0 && from < slots && to >= 0 && to < slots;
+  src[at] = copy ? from : -1;
+  dst[at] = copy ? to : -1;
+}
+
 // scratch: [0] moves, [1 .. slots] new place of every slot, then the movers (slots / 2 at most)
 // and the holes below them, as many.
 __global__ __launch_bounds__(kPlan) void pages_plan_kernel(int* used, int slots, int* live,
@@ -318,6 +351,23 @@ extern "C" PRNN_API int prnn_pages_copy(int slots, const prnn_pool* pools, int n
     return fail(PRNN_ERR_VALUE, "pages_copy: n=%d, src and dst must be non-null", n);
   if (n == 0 || slots == 0) return PRNN_OK;
   return copy(pools, n_pools, slots, src, dst, n, static_cast<hipStream_t>(stream));
+}
+
+extern "C" PRNN_API int prnn_pages_reorder(int slots, const prnn_pool* pools, int n_pools, int* table,
+                                           const int* parents, int B, int K, int* scratch,
+                                           void* stream) {
+  int none = 0;
+  if (int rc = check_cache("pages_reorder", &none, slots, pools, n_pools)) return rc;
+  if (B < 0 || K < 1 || K > kBeams || static_cast<long long>(B) * K > 1ll << 30)
+    return fail(PRNN_ERR_VALUE, "pages_reorder: B=%d, K=%d: K must be in 1 .. %d", B, K, kBeams);
+  if (B == 0) return PRNN_OK;
+  if (!table || !parents || !scratch)
+    return fail(PRNN_ERR_VALUE, "pages_reorder: table, parents and scratch must be non-null");
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  const int n = B * K;
+  pages_reorder_kernel<<<B, kPlan, 0, st>>>(table, parents, K, slots, scratch, scratch + n);
+  PRNN_HIP(hipGetLastError());
+  return slots == 0 ? PRNN_OK : copy(pools, n_pools, slots, scratch, scratch + n, n, st);
 }
 
 extern "C" PRNN_API int prnn_pages_compact(int* used, int slots, const prnn_pool* pools,

@@ -9,6 +9,7 @@ names (``pararnn::newton_slstm_fused``, ``pararnn::newton_gru_head_fused``).
 """
 
 from pararnn_amd.attention import linear_attention, linear_attention_step
+from pararnn_amd.beams import beam_select
 from pararnn_amd.cells import ParaGRU, ParaSLSTM
 from pararnn_amd.decode import can_decode_step, decode_step, decode_wx
 from pararnn_amd.config import (
@@ -34,6 +35,7 @@ from pararnn_amd.pages import (
     copy_pages,
     fork_pages,
     free_pages,
+    reorder_pages,
     take_pages,
 )
 from pararnn_amd.ragged import PackedSequences
@@ -59,6 +61,7 @@ __all__ = [
     "ParaRNN",
     "ParaSLSTM",
     "auto_newton_iters",
+    "beam_select",
     "can_decode_step",
     "decode_step",
     "decode_wx",
@@ -77,6 +80,7 @@ __all__ = [
     "newton_apply",
     "newton_gru_head_fused",
     "newton_slstm_fused",
+    "reorder_pages",
     "residual_norm",
     "sequential_apply",
     "slstm_auto_picard",

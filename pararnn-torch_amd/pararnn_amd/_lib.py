@@ -183,6 +183,10 @@ SIGNATURES: dict[str, tuple] = {
     "prnn_residual_norm_backward": (
         _I, [_P, _P, _P, _P, _P, _P, _P, _P, _F, _P, _P, _P, _P, _P, _P, _P, _I, _I, _F, _I, _I, _I,
              _I, _I, _P, _S, _P]),
+    "prnn_beam_select_workspace_size": (_S, [_I, _I, _I, _I]),
+    "prnn_beam_select": (
+        _I, [_P, _L, _L, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _P, _S, _P]),
+    "prnn_pages_reorder": (_I, [_I, _PP, _I, _P, _P, _I, _I, _P, _P]),
     "prnn_pages_take": (_I, [_P, _I, _P, _I, _P]),
     "prnn_pages_fork": (_I, [_P, _I, _PP, _I, _P, _P, _I, _P, _P]),
     "prnn_pages_free": (_I, [_P, _I, _P, _I, _P]),

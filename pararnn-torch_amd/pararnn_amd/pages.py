@@ -1,4 +1,4 @@
-"""Slots of a state cache: taking, forking, freeing and compacting them on the GPU.
+"""Slots of a state cache: taking, forking, freeing, reordering and compacting them on the GPU.
 
 A serving program keeps its sessions' recurrent states in pools ``(slots, ...)``: a linear
 attention's ``(slots, H, Dk, Dv)``, a cell's ``(slots, 4, d)`` or ``(slots, d)``, one per layer;
@@ -112,6 +112,44 @@ def copy_pages(pools: Sequence[Tensor] | Tensor, src: Tensor, dst: Tensor) -> No
     rc = _enqueue(_lib.load().prnn_pages_copy, dev, slots, rows, len(pools), src.data_ptr(),
                   dst.data_ptr(), src.shape[0])
     _lib.check(rc, "copy_pages")
+
+
+def reorder_pages(pools: Sequence[Tensor] | Tensor, table: Tensor, parents: Tensor) -> Tensor:
+    """Lets the beams' states follow a selection: ``table`` ``(B, K)`` (or ``(K,)``) int32 names the
+    slots of the beams of ``B`` searches, ``parents`` of the same shape each child's beam of its own
+    search (:func:`beam_select`'s); ``table``, rewritten in place and returned, then names a slot for
+    every child that holds its parent's rows in every pool.
+
+    A beam's first child keeps its slot; the other children, in order, take the slots of the beams
+    without children, in order, so a search keeps its slots and only what they hold is copied, once
+    for every beam without a child.  A child without a parent (an entry outside ``0 .. K - 1``, -1) or
+    of a beam whose slot is outside the pool gets a slot that is not written.  ``K`` at most 1024; no
+    two entries of ``table`` may name one slot."""
+    what = "reorder_pages"
+    pools, rows, slots, dev = _pools(what, pools, None, None)
+    if dev is None:
+        raise ValueError(f"{what} needs a pool")
+    if table.device != dev or parents.device != dev:
+        raise RuntimeError(f"{what}: tensors on different devices ({table.device}, "
+                           f"{parents.device} vs {dev})")
+    if table.dtype != torch.int32:
+        raise TypeError(f"{what}: table must be int32, got {table.dtype}")
+    if table.dim() not in (1, 2) or not table.is_contiguous():
+        raise ValueError(f"{what}: table must be (B, K) or (K,) and contiguous (it is changed in "
+                         f"place), got {tuple(table.shape)}")
+    if parents.shape != table.shape:
+        raise ValueError(f"{what}: parents {tuple(parents.shape)} != table {tuple(table.shape)}")
+    beams = table.shape[-1]
+    if not 1 <= beams <= 1024 or table.numel() > 1 << 30:
+        raise ValueError(f"{what}: K={beams} beams are not in 1 .. 1024")
+    parents = _slots(what, "parents", parents.reshape(-1), dev)
+    _writes(what, table, *pools)
+    searches = table.numel() // beams
+    scratch = torch.empty(2 * table.numel(), dtype=torch.int32, device=dev)
+    rc = _enqueue(_lib.load().prnn_pages_reorder, dev, slots, rows, len(pools), table.data_ptr(),
+                  parents.data_ptr(), searches, beams, scratch.data_ptr())
+    _lib.check(rc, what)
+    return table
 
 
 def compact_pages(used: Tensor, pools: Sequence[Tensor] | Tensor,
