@@ -127,20 +127,28 @@ struct DrSystems {
   float scale;
 };
 
+// Matrices that are only read as operands lie in memory as such: tiles of 32 rows, steps of 16 columns,
+// lane by lane the 8 places that it has of a row (tiles.h); what is behind the matrix holds zeros.
+inline __host__ __device__ size_t dr_operand_elems(int rows, int cols) {
+  return static_cast<size_t>((rows + 31) / 32) * ((cols + 15) / 16) * 512;
+}
+__device__ __forceinline__ uint32_t dr_operand_at(int cols, int i, int j) {
+  const int lane = (i & 31) + 32 * ((j >> 2) & 1), e = (j & 3) + 4 * ((j >> 3) & 1);
+  return (((i >> 5) * ((cols + 15) / 16) + (j >> 4)) * 64 + lane) * 8 + e;
+}
+
 struct DrWalk {
   LaSeqs seqs;               // len: tokens of a piece, a multiple of 64
   LaView q, k, z;            // z: v, backwards go
   const char* sys;
   void* out;                 // forwards: o by the strides below, storage type
   long long o_sb, o_st, o_sh;
-  void* e;                   // (token, H, Dv) of the arithmetic's type: written forwards, read backwards
-  void* keep;                // (chunk, H, Dk, Dv): states before the chunks, adjoints behind them
+  void* e;                   // forwards: (chunk, H), 64 x Dv as operands, of the arithmetic's type
+  void* keep;                // (chunk, H), Dk x Dv likewise: states before the chunks, adjoints behind them
   void* dv;                  // backwards, dense (token, H, Dv): of the arithmetic's type
   float* dv32;               // or floats besides (heads that are summed afterwards)
-  float* db;                 // [wave's columns][token][H]
-  size_t tokens;             // of the whole batch
   LaState init, last;
-  float *piece, *transfer;   // pieces' own states (piece, H, Dk, Dv) and transfers (piece, H, Dk, Dk)
+  float *piece, *transfer;   // (piece, H, Dk, Dv), (piece, H) as operands: the pieces' own states, their transfers
   int H, Dk, Dv, dtype;
   int tiles, own_tiles;      // column tiles of a launch; of them of the state (the rest: transfers)
   float scale;
@@ -151,16 +159,13 @@ struct DrGrad {
   LaView q, k, go;
   LaDecay g, b;
   const char* sys;           // the transposed systems: only their decays and rates are read
-  const void *e, *dv;        // (token, H, Dv) of the arithmetic's type
-  const void *before, *behind;  // (chunk, H, Dk, Dv)
-  const float* db;           // [wave's columns][token][H]
-  int db_tiles;
+  const void *e, *before, *behind;  // as operands: (chunk, H), 64 x Dv and Dk x Dv
+  const void* dv;            // (token, H, Dv) of the arithmetic's type
   void *dq, *dk;             // (token, H, Dk): the arithmetic's type, or floats (q_f32, k_f32)
   int q_f32, k_f32;
   void *dg, *dbeta;          // (token, H); dg NULL: not wanted, or sums per chunk:
   float* g_part;             // (chunk, H)
   int H, Dk, Dv, dtype, g_dtype, b_dtype;
-  size_t tokens;
   float scale;
 };
 
@@ -170,12 +175,13 @@ int dr_systems(const DrSystems& a, bool bf16, hipStream_t stream);
 int dr_walk_bf16(const DrWalk& a, DrKind kind, int cols, hipStream_t stream);
 int dr_walk_bf16_back(const DrWalk& a, DrKind kind, int cols, hipStream_t stream);
 int dr_walk_f32(const DrWalk& a, DrKind kind, hipStream_t stream);
+// The pieces' own states and transfers to the states that the pieces begin with.
+int dr_join(const DrWalk& a, bool back, hipStream_t stream);
 int dr_grad(const DrGrad& a, bool bf16, hipStream_t stream);
 
-// How a walk covers the Dv columns of the state: workgroups, and their waves in all, `cols` columns
-// each.
+// How a walk covers columns of the state: workgroups of `group` waves of `cols` columns each.
 struct DrCover {
-  int group, tiles, waves;
+  int group, tiles;
 };
 inline DrCover dr_walk_cols(int Dk, int Dv, int cols, bool bf16) {
   int group = 4;  // waves of a workgroup
@@ -184,7 +190,7 @@ inline DrCover dr_walk_cols(int Dk, int Dv, int cols, bool bf16) {
   else if (Dk <= 128 && (cols == 32 ? Dv <= 64 : Dv <= 32))
     group = 2;
   const int tiles = (Dv + cols * group - 1) / (cols * group);
-  return DrCover{group, tiles, tiles * group};
+  return DrCover{group, tiles};
 }
 
 }  // namespace prnn

@@ -47,8 +47,7 @@ LaSeqs sequences_of(const Problem& a) {
   return q;
 }
 
-// What the backward pass reads of the forward one: e (token, H, Dv), then the states before the
-// chunks (chunk, H, Dk, Dv), both of the arithmetic's type.
+// What the backward pass reads of the forward one, as operands: e, then the states before the chunks.
 struct Kept {
   void *e, *before;
   size_t bytes;
@@ -57,8 +56,9 @@ Kept kept_of(void* p, const Problem& a) {
   Carver c(p);
   const size_t size = on_bf16(a) ? 2 : 4, heads = a.la.H;
   Kept k{};
-  k.e = c.take(tokens_of(a) * heads * a.la.Dv * size);
-  k.before = c.take(dr_units(sequences_of(a), kDrC) * heads * a.la.Dk * a.la.Dv * size);
+  const size_t units = dr_units(sequences_of(a), kDrC);
+  k.e = c.take(units * heads * dr_operand_elems(kDrC, a.la.Dv) * size);
+  k.before = c.take(units * heads * dr_operand_elems(a.la.Dk, a.la.Dv) * size);
   k.bytes = c.used;
   return k;
 }
@@ -66,8 +66,16 @@ Kept kept_of(void* p, const Problem& a) {
 struct Scratch {
   char* sys;
   void *behind, *dv;
-  float *db, *dq32, *dk32, *dv32, *g_part;
+  float *piece, *transfer;
+  float *dq32, *dk32, *dv32, *g_part;
   size_t bytes;
+};
+
+// How a walk is laid out: columns of a wave, tokens of a piece (more than T: whole sequences).
+struct Plan {
+  int cols;
+  LaSeqs seqs;
+  bool cut;
 };
 
 // Columns of a wave: 32, or 16 where there are not enough waves of 32 for the chip's 1024 SIMDs (and
@@ -78,20 +86,59 @@ int wave_cols(const Problem& a, const LaSeqs& q) {
   return dr_units(q, q.len) * a.la.H * ((a.la.Dv + 31) / 32) >= 1024 ? 32 : 16;
 }
 
-Scratch carve(void* ws, const Problem& a, bool backward, bool decay_grad) {
+// A sequence's chunks come one after another.  Cut into n pieces they go side by side, but every piece
+// but the last walks a second time, without outputs and over Dv + Dk columns, and the join takes the
+// pieces one after another.  In units of a chunk of the full walk (4.2 us): 0.6 for one of the state
+// alone, 0.4 for a piece's step of the join, 4 for the two launches more.  A CU's second workgroup
+// makes both slower by half, further ones wait.
+Plan plan(const Problem& a) {
+  Plan p{16, sequences_of(a), false};
+  const long long longest = a.la.cu_seqlens && a.la.longest > 0 ? std::min(a.la.longest, a.la.T) : a.la.T;
+  const long long chunks = (longest + kDrC - 1) / kDrC, tokens = 1ll * a.la.B * a.la.T;
+  const double seqs = std::max(1.0, static_cast<double>(tokens) / std::max(1ll, longest));  // as if all were as long
+  const int group_cols = dr_walk_cols(a.la.Dk, a.la.Dv, 16, on_bf16(a)).group * 16;
+  const double tiles = (a.la.Dv + group_cols - 1) / group_cols;
+  const double own = tiles + (a.la.Dk + group_cols - 1) / group_cols;
+  auto slower = [](double groups) {
+    const double x = groups / 256.0;
+    return x <= 1.0 ? 1.0 : std::max(0.5 + 0.5 * x, 0.75 * x);
+  };
+  double best = 0.0;
+  long long pieces = 1;
+  for (long long n = 1; n <= 64 && n <= chunks; ++n) {
+    const double each = static_cast<double>((chunks + n - 1) / n), heads = seqs * a.la.H * n;
+    double t = each * slower(heads * tiles);
+    if (n > 1) t += 0.6 * each * slower(heads * own) + 0.4 * n + 4.0;
+    if (n == 1 || t < best) {
+      best = t;
+      pieces = n;
+    }
+  }
+  if (pieces > 1) {
+    p.seqs.len = static_cast<int>((chunks + pieces - 1) / pieces * kDrC);
+    p.cut = p.seqs.len < longest;
+    if (!p.cut) p.seqs.len = 1 << 30;
+  }
+  p.cols = wave_cols(a, p.seqs);
+  return p;
+}
+
+Scratch carve(void* ws, const Problem& a, const Plan& plan, bool backward, bool decay_grad) {
   Carver c(ws);
   Scratch s{};
-  const LaSeqs q = sequences_of(a);
   const size_t heads = a.la.H, tokens = tokens_of(a), size = on_bf16(a) ? 2 : 4;
-  const size_t units = dr_units(q, kDrC);
+  const size_t units = dr_units(plan.seqs, kDrC);
   s.sys = static_cast<char*>(c.take(units * heads * kDrSys));
+  if (plan.cut) {
+    const size_t pieces = dr_units(plan.seqs, plan.seqs.len) * heads;
+    s.piece = static_cast<float*>(c.take(4 * pieces * a.la.Dk * a.la.Dv));
+    s.transfer = static_cast<float*>(c.take(4 * pieces * dr_operand_elems(a.la.Dk, a.la.Dk)));
+  }
   if (backward) {
-    s.behind = c.take(units * heads * a.la.Dk * a.la.Dv * size);
-    const size_t waves = dr_walk_cols(a.la.Dk, a.la.Dv, wave_cols(a, q), on_bf16(a)).waves;
-    s.db = static_cast<float*>(c.take(4 * waves * tokens * heads));
+    s.behind = c.take(units * heads * dr_operand_elems(a.la.Dk, a.la.Dv) * size);
     // dv is written where it is wanted, unless its heads are summed or it is stored in another type
     const bool sums = a.la.v.heads != a.la.H;
-    if (sums || (on_bf16(a) ? false : a.la.dtype != PRNN_F32)) s.dv = c.take(tokens * heads * a.la.Dv * size);
+    if (sums || (!on_bf16(a) && a.la.dtype != PRNN_F32)) s.dv = c.take(tokens * heads * a.la.Dv * size);
     if (sums && on_bf16(a)) s.dv32 = static_cast<float*>(c.take(4 * tokens * heads * a.la.Dv));
     if (a.la.q.heads != a.la.H) s.dq32 = static_cast<float*>(c.take(4 * tokens * heads * a.la.Dk));
     if (a.la.k.heads != a.la.H) s.dk32 = static_cast<float*>(c.take(4 * tokens * heads * a.la.Dk));
@@ -99,6 +146,9 @@ Scratch carve(void* ws, const Problem& a, bool backward, bool decay_grad) {
   }
   s.bytes = c.used;
   return s;
+}
+size_t need(const Problem& a, bool backward, bool decay_grad) {
+  return carve(nullptr, a, plan(a), backward, decay_grad).bytes;
 }
 
 int check_ws(const char* what, size_t need, const void* ws, size_t bytes) {
@@ -128,30 +178,48 @@ int systems(const Problem& a, const Scratch& s, bool transposed, hipStream_t st)
   return dr_systems(y, on_bf16(a), st);
 }
 
-DrWalk walk_of(const Problem& a, const Scratch& s) {
+DrWalk walk_of(const Problem& a, const Plan& plan, const Scratch& s) {
   DrWalk w{};
-  w.seqs = sequences_of(a);
+  w.seqs = plan.seqs;
   w.q = la_view(a.la.q, a.la, a.la.Dk);
   w.k = la_view(a.la.k, a.la, a.la.Dk);
   w.sys = s.sys;
-  w.tokens = tokens_of(a);
+  w.piece = s.piece;
+  w.transfer = s.transfer;
   w.H = a.la.H;
   w.Dk = a.la.Dk;
   w.Dv = a.la.Dv;
   w.dtype = a.la.dtype;
-  w.tiles = w.own_tiles = dr_walk_cols(a.la.Dk, a.la.Dv, wave_cols(a, w.seqs), on_bf16(a)).tiles;
   w.scale = a.la.scale;
   return w;
 }
-int run(const DrWalk& w, DrKind kind, const Problem& a, hipStream_t st) {
-  return on_bf16(a) ? dr_walk_bf16(w, kind, wave_cols(a, w.seqs), st) : dr_walk_f32(w, kind, st);
+int run(DrWalk w, DrKind kind, const Problem& a, const Plan& plan, hipStream_t st) {
+  const bool own = kind == kDrState || kind == kDrAdjoint;
+  w.own_tiles = dr_walk_cols(a.la.Dk, a.la.Dv, plan.cols, on_bf16(a)).tiles;
+  w.tiles = w.own_tiles;
+  if (own) {
+    const int cols = dr_walk_cols(a.la.Dk, a.la.Dv, plan.cols, on_bf16(a)).group * plan.cols;
+    w.tiles += (a.la.Dk + cols - 1) / cols;
+  }
+  return on_bf16(a) ? dr_walk_bf16(w, kind, plan.cols, st) : dr_walk_f32(w, kind, st);
+}
+// The walk of a direction; of a cut sequence the pieces' own states and the join before it.
+int walk(const DrWalk& w, bool back, const Problem& a, const Plan& plan, hipStream_t st) {
+  if (plan.cut) {
+    DrWalk own = w;
+    own.keep = nullptr;
+    if (int rc = run(own, back ? kDrAdjoint : kDrState, a, plan, st)) return rc;
+    if (int rc = dr_join(w, back, st)) return rc;
+  }
+  return run(w, back ? kDrBackward : kDrForward, a, plan, st);
 }
 
 int forward(const Problem& a, const prnn_la_view& out, float* state_out, const int* out_table, int out_rows,
             void* kept, void* ws, hipStream_t st) {
-  const Scratch s = carve(ws, a, false, false);
+  const Plan p = plan(a);
+  const Scratch s = carve(ws, a, p, false, false);
   if (int rc = systems(a, s, false, st)) return rc;
-  DrWalk w = walk_of(a, s);
+  DrWalk w = walk_of(a, p, s);
   w.z = la_view(a.la.v, a.la, a.la.Dv);
   w.out = const_cast<void*>(out.p);
   w.o_sb = out.sb;
@@ -164,25 +232,24 @@ int forward(const Problem& a, const prnn_la_view& out, float* state_out, const i
   }
   w.init = LaState{const_cast<float*>(a.la.h0), a.la.h0_table, a.la.h0_rows};
   w.last = LaState{state_out, out_table, out_rows};
-  return run(w, kDrForward, a, st);
+  return walk(w, false, a, p, st);
 }
 
 int backward(const Problem& a, const prnn_la_view& go, const float* gs, const void* kept, void* dq, void* dk,
              void* dv, void* dg, void* db, float* dh0, void* ws, hipStream_t st) {
   const bool per_head = a.la.g_sb == 0 && a.la.g_st == 0;
-  const Scratch s = carve(ws, a, true, dg != nullptr);
+  const Plan p = plan(a);
+  const Scratch s = carve(ws, a, p, true, dg != nullptr);
   const Kept k = kept_of(const_cast<void*>(kept), a);
   if (int rc = systems(a, s, true, st)) return rc;
-  DrWalk w = walk_of(a, s);
+  DrWalk w = walk_of(a, p, s);
   w.z = la_view(go, a.la, a.la.Dv);
-  w.e = k.e;
   w.keep = s.behind;
   w.dv = s.dv ? s.dv : dv;
   w.dv32 = s.dv32;
-  w.db = s.db;
   w.init = LaState{const_cast<float*>(gs), nullptr, sequences(a)};
   w.last = LaState{dh0, nullptr, sequences(a)};
-  if (int rc = run(w, kDrBackward, a, st)) return rc;
+  if (int rc = walk(w, true, a, p, st)) return rc;
   DrGrad g{};
   g.seqs = w.seqs;
   g.q = w.q;
@@ -195,8 +262,6 @@ int backward(const Problem& a, const prnn_la_view& go, const float* gs, const vo
   g.dv = w.dv;
   g.before = k.before;
   g.behind = s.behind;
-  g.db = s.db;
-  g.db_tiles = dr_walk_cols(a.la.Dk, a.la.Dv, wave_cols(a, w.seqs), on_bf16(a)).waves;
   g.q_f32 = s.dq32 != nullptr;
   g.k_f32 = s.dk32 != nullptr;
   g.dq = g.q_f32 ? s.dq32 : dq;
@@ -210,7 +275,6 @@ int backward(const Problem& a, const prnn_la_view& go, const float* gs, const vo
   g.dtype = a.la.dtype;
   g.g_dtype = a.la.g_dtype;
   g.b_dtype = a.b_dtype;
-  g.tokens = tokens_of(a);
   g.scale = a.la.scale;
   if (int rc = dr_grad(g, on_bf16(a), st)) return rc;
   LaHeadSums hs{};
@@ -243,7 +307,7 @@ using namespace prnn;
 
 extern "C" PRNN_API size_t prnn_delta_rule_workspace_size(const prnn_delta_rule_problem* a) {
   if (check(a)) return 0;
-  return carve(nullptr, *a, false, false).bytes;
+  return need(*a, false, false);
 }
 
 extern "C" PRNN_API size_t prnn_delta_rule_kept_size(const prnn_delta_rule_problem* a) {
@@ -262,14 +326,14 @@ extern "C" PRNN_API int prnn_delta_rule(const prnn_delta_rule_problem* a, const 
   if (sequences(*a) == 0) return PRNN_OK;
   if (kept && (reinterpret_cast<uintptr_t>(kept) & 255))
     return fail(PRNN_ERR_VALUE, "what is kept must lie on a 256-byte boundary");
-  if (int rc = check_ws("workspace", carve(nullptr, *a, false, false).bytes, workspace, bytes)) return rc;
+  if (int rc = check_ws("workspace", need(*a, false, false), workspace, bytes)) return rc;
   return forward(*a, *out, state_out, out_table, out_rows, kept, workspace, static_cast<hipStream_t>(stream));
 }
 
 extern "C" PRNN_API size_t prnn_delta_rule_backward_workspace_size(const prnn_delta_rule_problem* a,
                                                                    int decay_grad) {
   if (check(a)) return 0;
-  return carve(nullptr, *a, true, decay_grad != 0).bytes;
+  return need(*a, true, decay_grad != 0);
 }
 
 extern "C" PRNN_API int prnn_delta_rule_backward(const prnn_delta_rule_problem* a, const prnn_la_view* go,
@@ -289,6 +353,6 @@ extern "C" PRNN_API int prnn_delta_rule_backward(const prnn_delta_rule_problem* 
   if (a->la.h0 && a->la.h0_rows < sequences(*a))
     return fail(PRNN_ERR_VALUE, "h0 has %d rows for %d sequences", a->la.h0_rows, sequences(*a));
   if (sequences(*a) == 0) return PRNN_OK;
-  if (int rc = check_ws("workspace", carve(nullptr, *a, true, dg != nullptr).bytes, workspace, bytes)) return rc;
+  if (int rc = check_ws("workspace", need(*a, true, dg != nullptr), workspace, bytes)) return rc;
   return backward(*a, *go, gs, kept, dq, dk, dv, dg, db, dh0, workspace, static_cast<hipStream_t>(stream));
 }

@@ -1,34 +1,38 @@
 // Gated delta rule: the gradients of q, k, the log decays and the rates, a workgroup per chunk and
 // head, all chunks at once (the walks leave the states before the chunks and the adjoints behind).
 //
-// 1. Pairs of tokens, a tile of 32 x 32 of the lower triangle per wave, rows straight from memory:
-//    go u^T, dv u^T, q k^T, k k^T; with the decays' weights the first two go to LDS as operands.
-// 2. dq and dk in tiles of 32 columns and 32 tokens, formed transposed (lane: token).
+// 1. Pairs of tokens, a tile of 32 x 32 of the lower triangle per wave: go e^T, dv e^T, q k^T, k k^T;
+//    and the products with the states, tiles of 32 columns and 32 tokens, formed transposed (lane:
+//    token).  Tokens' rows come through LDS in slabs of 64 columns, states and e as operands.
+// 2. The pairs, weighted, as operands in LDS, over the slabs of go and dv: the rest of dq and dk.
 // 3. dL/dg_t is the flow through the decay of token t,
 //      F_t = sum over sources j < t and uses l >= t of what l reads of j,
 //    where a source may also be the state before the chunk and a use the adjoint behind it.  It is
 //    summed as that double sum and not as a running difference of gains and losses: behind a strong
-//    decay the flow is a tiny part of either.
+//    decay the flow is a tiny part of either.  The rates' gradient is what all read of a unit of what
+//    the token writes: the same sums by rows, and the token's own.
 #include "delta_rule_loads.h"
 
 namespace prnn {
 namespace {
 
-constexpr int kSlab = 64;  // columns of k and q in LDS at a time
-constexpr int kLf = 65;    // floats of a row of the flow's matrix
+constexpr int kLf = 65;  // floats of a row of the flow's matrix
 
-template <class M, typename T>
-__global__ __launch_bounds__(256) void dr_grad_kernel(DrGrad A) {
+// KS slabs of 64 columns of dq and dk at a time; WIDE: keys of more than KS, in several passes (the
+// pairs then need a place of their own).
+template <class M, int KS, bool WIDE>
+__global__ __launch_bounds__(256, sizeof(typename M::E) == 2 && KS == 1 ? 2 : 1) void dr_grad_kernel(DrGrad A) {
   using E = typename M::E;
-  using D = std::conditional_t<sizeof(E) == 2, bf16, float>;  // dense arrays
   constexpr bool kNarrow = sizeof(E) == 2;
   constexpr int ES = static_cast<int>(sizeof(E));
-  constexpr int RW = dr_row_z(kNarrow, 64), RK = dr_row_k(kNarrow, kSlab), P = M::kParts;
-  __shared__ __align__(16) char sW1[P][kDrC * RW], sX[P][kDrC * RW];
-  __shared__ __align__(16) char sK[kDrC * RK], sQ[kDrC * RK];
+  constexpr int kAt = kNarrow ? 4 : 2 / KS;  // steps whose operands are under way
+  constexpr int RB = dr_row_k(kNarrow, 64), P = M::kParts, kSlab = kDrC * RB;
+  __shared__ __align__(16) char lds[(WIDE ? 4 + P : 4) * kSlab], s_x[P][kSlab];
   __shared__ float sF[kDrC * kLf], s_in[8][kDrC], s_out[8][kDrC];
   __shared__ __align__(16) float sw[kDrW * 64];
-  __shared__ float s_through;
+  __shared__ float s_through, s_own[kDrC], s_into[kDrC], s_waves[4];
+  char *const sK = lds, *const sQ = lds + kSlab, *const sG = lds + 2 * kSlab, *const sD = lds + 3 * kSlab;
+  char* const sP = WIDE ? lds + 4 * kSlab : sG;  // the pairs go u^T, by parts
   const int h = blockIdx.x % A.H, id = blockIdx.x / A.H;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l32 = lane & 31, half = lane >> 5;
   const DrUnit u = dr_unit(A.seqs, kDrC, id);
@@ -39,159 +43,222 @@ __global__ __launch_bounds__(256) void dr_grad_kernel(DrGrad A) {
   const int n = u.end - u.begin, batch = dr_batch(A.seqs, u);
   const size_t tok0 = dr_token(A.seqs, u, u.begin);
   const size_t unit = static_cast<size_t>(id) * A.H + h;
+  const int TS = A.dtype == PRNN_F32 ? 4 : 2, kCode = kNarrow ? PRNN_BF16 : PRNN_F32;
+  auto rows = [&](const LaView& v) {
+    return static_cast<const char*>(v.p) + (batch * v.sb + (h / v.rep) * v.sh +
+                                            static_cast<long long>(u.begin) * v.st) * TS;
+  };
+  const char *pq = rows(A.q), *pk = rows(A.k), *pg = rows(A.go);
+  const char* pd = static_cast<const char*>(A.dv) + (tok0 * A.H + h) * A.Dv * ES;
+  auto operands = [&](const void* p, int r, int c) {
+    const size_t elems = dr_operand_elems(r, c);
+    return make_rsrc(static_cast<const E*>(p) + unit * elems, static_cast<uint32_t>(elems) * ES);
+  };
+  const rsrc_t re = operands(A.e, kDrC, A.Dv), rS = operands(A.before, A.Dk, A.Dv),
+               rR = operands(A.behind, A.Dk, A.Dv);
+  const int vs = (A.Dv + 15) / 16, last_k = (A.Dk - 1) / 64 * 64;
+  Staged<M, 64, 256> ga, gb, ka, kb;
+  ga.fetch(pg, A.go.st, n, 0, A.Dv, A.dtype);
+  gb.fetch(pd, static_cast<long long>(A.H) * A.Dv, n, 0, A.Dv, kCode);
+  ka.fetch(pk, A.k.st, n, last_k, A.Dk, A.dtype);
+  kb.fetch(pq, A.q.st, n, last_k, A.Dk, A.dtype);
   const float* weights = reinterpret_cast<const float*>(A.sys + unit * kDrSys + 2 * kDrTiles);
   for (int i = tid; i < kDrW * 64; i += 256) sw[i] = weights[i];
+  ga.template put<RB>(sG, A.dtype);
+  gb.template put<RB>(sD, kCode);
+  ka.template put<RB>(sK, A.dtype);
+  kb.template put<RB>(sQ, A.dtype);
 
-  auto rows = [&](const LaView& v) {
-    return make_rsrc(static_cast<const T*>(v.p) + (batch * v.sb + (h / v.rep) * v.sh +
-                                                   static_cast<long long>(u.begin) * v.st), 0x7fffffffu);
-  };
-  auto dense = [&](const void* p, int width) {
-    return make_rsrc(static_cast<const D*>(p) + (tok0 * A.H + h) * width, 0x7fffffffu);
-  };
-  auto state = [&](const void* p) {
-    return make_rsrc(static_cast<const D*>(p) + unit * A.Dk * A.Dv, static_cast<uint32_t>(A.Dk * A.Dv) * ES);
-  };
-  const rsrc_t rq = rows(A.q), rk = rows(A.k), rg = rows(A.go);
-  const rsrc_t re = dense(A.e, A.Dv), rd = dense(A.dv, A.Dv);
-  const rsrc_t rS = state(A.before), rR = state(A.behind);
-  const int TS = static_cast<int>(sizeof(T)), row_e = A.H * A.Dv * ES;
-  const bool flow = A.dg || A.g_part;
-  __syncthreads();
-
-  // ---- 1
-  if (wave < 3) {
-    const int it = wave > 0, jt = wave > 1, i = 32 * it + l32, j = 32 * jt + l32;
-    f16v GU, DU, QK, KK;
+  // pairs of the wave's tile; state products of its tile of every slab
+  const int pi = wave > 0, pj = wave > 1, i = 32 * pi + l32;
+  const int kt = wave & 1, it = wave >> 1, t = 32 * it + l32;
+  f16v GU, DU, QK, KK;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) GU[r] = DU[r] = QK[r] = KK[r] = 0.0f;
-    for (int c = 8 * half; c < A.Dv + 8 * half; c += 16) {
-      const auto ej = global_op<M, D>(re, j < n, j * row_e, c, A.Dv);
-      mul<32>(GU, ej, global_op<M, T>(rg, i < n, i * static_cast<int>(A.go.st) * TS, c, A.Dv));
-      mul<32>(DU, ej, global_op<M, D>(rd, i < n, i * row_e, c, A.Dv));
+  for (int r = 0; r < 16; ++r) GU[r] = DU[r] = QK[r] = KK[r] = 0.0f;
+
+  auto keys = [&]() {
+#pragma unroll
+    for (int f = 0; f < 4; ++f) {
+      const auto kj = row_op<M, 2>(sK + (32 * pj + l32) * RB, f, half);
+      mul<32>(QK, kj, row_op<M, 2>(sQ + i * RB, f, half));
+      mul<32>(KK, kj, row_op<M, 2>(sK + i * RB, f, half));
     }
-    if (flow)
-      for (int c = 8 * half; c < A.Dk + 8 * half; c += 16) {
-        const auto kj = global_op<M, T>(rk, j < n, j * static_cast<int>(A.k.st) * TS, c, A.Dk);
-        mul<32>(QK, kj, global_op<M, T>(rq, i < n, i * static_cast<int>(A.q.st) * TS, c, A.Dk));
-        mul<32>(KK, kj, global_op<M, T>(rk, i < n, i * static_cast<int>(A.k.st) * TS, c, A.Dk));
-      }
-    const float Hi = sw[kWhi * 64 + i], Lo = sw[kWlo * 64 + i];
+  };
+
+  for (int p0 = 0; p0 < A.Dk; p0 += 64 * KS) {
+    f16v dq[KS], du[KS], ds[KS];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      float w1[4], x[4];
-      const int j0 = 32 * jt + 8 * q + 4 * half;
+    for (int s = 0; s < KS; ++s)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int jj = j0 + r, e = 4 * q + r;
-        const float w = fexp((Hi - sw[kWhi * 64 + jj]) + (Lo - sw[kWlo * 64 + jj])) * sw[kWb * 64 + jj];
-        w1[r] = jj <= i ? w * A.scale * GU[e] : 0.0f;
-        x[r] = jj < i ? w * DU[e] : 0.0f;
-        sF[jj * kLf + i] = jj < i ? QK[e] * w1[r] - KK[e] * x[r] : 0.0f;
+      for (int r = 0; r < 16; ++r) dq[s][r] = du[s][r] = ds[s][r] = 0.0f;
+    // ---- 1
+    for (int v0 = 0; v0 < A.Dv; v0 += 64) {
+      if (p0 > 0 || v0 > 0) {
+        ga.fetch(pg, A.go.st, n, v0, A.Dv, A.dtype);
+        gb.fetch(pd, static_cast<long long>(A.H) * A.Dv, n, v0, A.Dv, kCode);
+        __syncthreads();
+        ga.template put<RB>(sG, A.dtype);
+        gb.template put<RB>(sD, kCode);
       }
-      if constexpr (kNarrow) {
-        const u2 a{pack_bf16x2(w1[0], w1[1]), pack_bf16x2(w1[2], w1[3])};
-        const u2 b{pack_bf16x2(w1[0] - lo_bf16(a[0]), w1[1] - hi_bf16(a[0])),
-                   pack_bf16x2(w1[2] - lo_bf16(a[1]), w1[3] - hi_bf16(a[1]))};
-        *reinterpret_cast<u2*>(sW1[0] + i * RW + j0 * 2) = a;
-        *reinterpret_cast<u2*>(sW1[P - 1] + i * RW + j0 * 2) = b;
-      } else {
-        *reinterpret_cast<f4*>(sW1[0] + i * RW + j0 * 4) = f4{w1[0], w1[1], w1[2], w1[3]};
-      }
-      // -(X + X^T): either triangle from the one value
+      Op<M, 1> ei[kAt], S[KS][kAt], R[KS][kAt];
+      auto fetch = [&](int f0) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int jj = j0 + r;
-        if (jj > i) continue;
-        if constexpr (kNarrow) {
-          const bf16 a = from_f32<bf16>(-x[r]), b = from_f32<bf16>(-x[r] - to_f32(a));
-          *reinterpret_cast<bf16*>(sX[0] + i * RW + jj * 2) = a;
-          *reinterpret_cast<bf16*>(sX[0] + jj * RW + i * 2) = a;
-          *reinterpret_cast<bf16*>(sX[P - 1] + i * RW + jj * 2) = b;
-          *reinterpret_cast<bf16*>(sX[P - 1] + jj * RW + i * 2) = b;
-        } else {
-          *reinterpret_cast<float*>(sX[0] + i * RW + jj * 4) = -x[r];
-          *reinterpret_cast<float*>(sX[0] + jj * RW + i * 4) = -x[r];
+        for (int f = 0; f < kAt; ++f) {
+          const int step = v0 / 16 + f0 + f;
+          ei[f] = global_op<M>(re, step < vs, it * vs + step);
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            const int tile = p0 / 32 + 2 * s + kt;
+            S[s][f] = global_op<M>(rS, (step < vs) & (32 * tile < A.Dk), tile * vs + step);
+            R[s][f] = global_op<M>(rR, (step < vs) & (32 * tile < A.Dk), tile * vs + step);
+          }
+        }
+      };
+      fetch(0);
+      __syncthreads();
+      // under the operands' way: pairs of what is in LDS
+      if (p0 == 0 && v0 == 0 && wave < 3) keys();
+      for (int f0 = 0; f0 < 4; f0 += kAt) {
+        if (f0 > 0) fetch(f0);
+#pragma unroll
+        for (int f = 0; f < kAt; ++f) {
+          const auto gi = row_op<M, 2>(sG + t * RB, f0 + f, half), di = row_op<M, 2>(sD + t * RB, f0 + f, half);
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            mul<32>(dq[s], S[s][f], gi);
+            mul<32>(du[s], R[s][f], ei[f]);
+            mul<32>(ds[s], S[s][f], di);
+          }
+        }
+      }
+      if (p0 == 0 && wave < 3) {
+        for (int f0 = 0; f0 < 4; f0 += kAt) {
+          Op<M, 1> ej[kAt];
+#pragma unroll
+          for (int f = 0; f < kAt; ++f) {
+            const int step = v0 / 16 + f0 + f;
+            ej[f] = global_op<M>(re, step < vs, pj * vs + step);
+          }
+#pragma unroll
+          for (int f = 0; f < kAt; ++f) {
+            mul<32>(GU, ej[f], row_op<M, 2>(sG + i * RB, f0 + f, half));
+            mul<32>(DU, ej[f], row_op<M, 2>(sD + i * RB, f0 + f, half));
+          }
         }
       }
     }
-  } else {
-    // the rates' gradient: the walk's columns in their order
-    if (A.dbeta && lane < n) {
-      float d = 0.0f;
-      for (int t = 0; t < A.db_tiles; ++t) d += A.db[(static_cast<size_t>(t) * A.tokens + tok0 + lane) * A.H + h];
-      const size_t at = (tok0 + lane) * A.H + h;
-      if (A.b_dtype == PRNN_F32)
-        static_cast<float*>(A.dbeta)[at] = d;
-      else if (A.b_dtype == PRNN_F16)
-        static_cast<f16*>(A.dbeta)[at] = from_f32<f16>(d);
-      else
-        static_cast<bf16*>(A.dbeta)[at] = from_f32<bf16>(d);
-    }
-    if (flow) {  // from the state before to the adjoint behind
-      float d = 0.0f;
-      for (int e = lane * 8; e < A.Dk * A.Dv; e += 512) {
-        float a[8], b[8];
-        values(global_op<M, D>(rS, true, 0, e, A.Dk * A.Dv), a);
-        values(global_op<M, D>(rR, true, 0, e, A.Dk * A.Dv), b);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) d = fmaf(a[i], b[i], d);
+    if (p0 == 0) {
+      for (int c0 = last_k - 64; c0 >= 0; c0 -= 64) {
+        ka.fetch(pk, A.k.st, n, c0, A.Dk, A.dtype);
+        kb.fetch(pq, A.q.st, n, c0, A.Dk, A.dtype);
+        __syncthreads();
+        ka.template put<RB>(sK, A.dtype);
+        kb.template put<RB>(sQ, A.dtype);
+        __syncthreads();
+        if (wave < 3) keys();
       }
+      __syncthreads();  // go and dv have been read: the pairs take their place
+      if (wave < 3) {
+        const float Hi = sw[kWhi * 64 + i], Lo = sw[kWlo * 64 + i];
 #pragma unroll
-      for (int m = 1; m < 64; m <<= 1) d += __shfl_xor(d, m);
-      if (lane == 0) s_through = d * sw[kWmeta * 64];
+        for (int q = 0; q < 4; ++q) {
+          float w1[4], x[4];
+          const int j0 = 32 * pj + 8 * q + 4 * half;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int jj = j0 + r, e = 4 * q + r;
+            const float w = fexp((Hi - sw[kWhi * 64 + jj]) + (Lo - sw[kWlo * 64 + jj]));
+            w1[r] = jj <= i ? w * A.scale * GU[e] : 0.0f;
+            x[r] = jj < i ? w * DU[e] : 0.0f;
+            // what token i reads of a unit of what j writes (its rate is still to come)
+            sF[jj * kLf + i] = jj < i ? QK[e] * w1[r] - KK[e] * x[r] : 0.0f;
+            if (jj == i) s_own[i] = QK[e] * w1[r];
+            w1[r] *= sw[kWb * 64 + jj];
+            x[r] *= sw[kWb * 64 + jj];
+          }
+          if constexpr (kNarrow) {
+            const u2 a{pack_bf16x2(w1[0], w1[1]), pack_bf16x2(w1[2], w1[3])};
+            const u2 b{pack_bf16x2(w1[0] - lo_bf16(a[0]), w1[1] - hi_bf16(a[0])),
+                       pack_bf16x2(w1[2] - lo_bf16(a[1]), w1[3] - hi_bf16(a[1]))};
+            *reinterpret_cast<u2*>(sP + i * RB + j0 * 2) = a;
+            *reinterpret_cast<u2*>(sP + kSlab + i * RB + j0 * 2) = b;
+          } else {
+            *reinterpret_cast<f4*>(sP + i * RB + j0 * 4) = f4{w1[0], w1[1], w1[2], w1[3]};
+          }
+          // -(X + X^T): either triangle from the one value
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int jj = j0 + r;
+            if (jj > i) continue;
+            if constexpr (kNarrow) {
+              const bf16 a = from_f32<bf16>(-x[r]), b = from_f32<bf16>(-x[r] - to_f32(a));
+              *reinterpret_cast<bf16*>(s_x[0] + i * RB + jj * 2) = a;
+              *reinterpret_cast<bf16*>(s_x[0] + jj * RB + i * 2) = a;
+              *reinterpret_cast<bf16*>(s_x[P - 1] + i * RB + jj * 2) = b;
+              *reinterpret_cast<bf16*>(s_x[P - 1] + jj * RB + i * 2) = b;
+            } else {
+              *reinterpret_cast<float*>(s_x[0] + i * RB + jj * 4) = -x[r];
+              *reinterpret_cast<float*>(s_x[0] + jj * RB + i * 4) = -x[r];
+            }
+          }
+        }
+      } else {  // from the state before to the adjoint behind
+        float d = 0.0f;
+        const int ops = static_cast<int>(dr_operand_elems(A.Dk, A.Dv) / 512);
+        for (int o = 0; o < ops; o += 2 * kAt) {
+          Op<M, 1> a[2 * kAt], b[2 * kAt];
+#pragma unroll
+          for (int k = 0; k < 2 * kAt; ++k) {
+            a[k] = global_op<M>(rS, o + k < ops, o + k);
+            b[k] = global_op<M>(rR, o + k < ops, o + k);
+          }
+#pragma unroll
+          for (int k = 0; k < 2 * kAt; ++k) {
+            float x[8], y[8];
+            values(a[k], x);
+            values(b[k], y);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) d = fmaf(x[e], y[e], d);
+          }
+        }
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) d += __shfl_xor(d, m);
+        if (lane == 0) s_through = d * sw[kWmeta * 64];
+      }
+      __syncthreads();
     }
-  }
 
-  // ---- 2
-  const int kt = wave & 1, it = wave >> 1, i = 32 * it + l32;
-  const float wg = sw[kWg * 64 + i], wr = sw[kWr * 64 + i] * sw[kWb * 64 + i];
-  for (int c0 = 0; c0 < A.Dk; c0 += kSlab) {
-    {
-      Staged<M, kSlab, 256> k, q;
-      constexpr int kCode = kNarrow ? PRNN_BF16 : std::is_same_v<T, float> ? PRNN_F32
-                            : std::is_same_v<T, f16>                       ? PRNN_F16
-                                                                           : PRNN_BF16;
-      auto at = [&](const LaView& v) {
-        return reinterpret_cast<const char*>(static_cast<const T*>(v.p) + (batch * v.sb + (h / v.rep) * v.sh +
-                                                                           static_cast<long long>(u.begin) * v.st));
-      };
-      k.fetch(at(A.k), A.k.st, n, c0, A.Dk, kCode);
-      q.fetch(at(A.q), A.q.st, n, c0, A.Dk, kCode);
-      __syncthreads();  // the pairs are there; the last slab has been read
-      k.template put<RK>(sK, kCode);
-      q.template put<RK>(sQ, kCode);
-    }
-    __syncthreads();
-    const int row = c0 + 32 * kt + l32;
-    f16v dq, du, ds;
+    // ---- 2
+    const float wg = sw[kWg * 64 + t], wr = sw[kWr * 64 + t], rate = sw[kWb * 64 + t];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) dq[r] = du[r] = ds[r] = 0.0f;
-    if (c0 + 32 * kt < A.Dk) {
-      const bool in = row < A.Dk;
-      const uint32_t at = row * A.Dv * ES;
-      for (int c = 8 * half; c < A.Dv + 8 * half; c += 16) {
-        const auto s = global_op<M, D>(rS, in, at, c, A.Dv), r = global_op<M, D>(rR, in, at, c, A.Dv);
-        mul<32>(dq, s, global_op<M, T>(rg, i < n, i * static_cast<int>(A.go.st) * TS, c, A.Dv));
-        mul<32>(du, r, global_op<M, D>(re, i < n, i * row_e, c, A.Dv));
-        mul<32>(ds, s, global_op<M, D>(rd, i < n, i * row_e, c, A.Dv));
+    for (int s = 0; s < KS; ++s) {
+      const int c0 = p0 + 64 * s;
+      if (c0 >= A.Dk) continue;
+      if (c0 > 0) {
+        ka.fetch(pk, A.k.st, n, c0, A.Dk, A.dtype);
+        kb.fetch(pq, A.q.st, n, c0, A.Dk, A.dtype);
+        __syncthreads();
+        ka.template put<RB>(sK, A.dtype);
+        kb.template put<RB>(sQ, A.dtype);
+        __syncthreads();
       }
+      if (c0 + 32 * kt >= A.Dk) continue;
       float in_sum = 0.0f, out_sum = 0.0f;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int col = 32 * kt + 8 * q + 4 * half;
         float qv[4], kv[4];
         if constexpr (kNarrow) {
-          const u2 a = *reinterpret_cast<const u2*>(sQ + i * RK + col * 2);
-          const u2 b = *reinterpret_cast<const u2*>(sK + i * RK + col * 2);
+          const u2 a = *reinterpret_cast<const u2*>(sQ + t * RB + col * 2);
+          const u2 b = *reinterpret_cast<const u2*>(sK + t * RB + col * 2);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             qv[r] = r & 1 ? hi_bf16(a[r >> 1]) : lo_bf16(a[r >> 1]);
             kv[r] = r & 1 ? hi_bf16(b[r >> 1]) : lo_bf16(b[r >> 1]);
           }
         } else {
-          const f4 a = *reinterpret_cast<const f4*>(sQ + i * RK + col * 4);
-          const f4 b = *reinterpret_cast<const f4*>(sK + i * RK + col * 4);
+          const f4 a = *reinterpret_cast<const f4*>(sQ + t * RB + col * 4);
+          const f4 b = *reinterpret_cast<const f4*>(sK + t * RB + col * 4);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             qv[r] = a[r];
@@ -201,26 +268,26 @@ __global__ __launch_bounds__(256) void dr_grad_kernel(DrGrad A) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int e = 4 * q + r;
-          dq[e] *= wg * A.scale;
-          ds[e] *= wg;
-          du[e] *= wr;
-          in_sum = fmaf(qv[r], dq[e], fmaf(-kv[r], ds[e], in_sum));
-          out_sum = fmaf(kv[r], du[e], out_sum);
-          du[e] -= ds[e];
+          dq[s][e] *= wg * A.scale;
+          ds[s][e] *= wg;
+          du[s][e] *= wr;
+          in_sum = fmaf(qv[r], dq[s][e], fmaf(-kv[r], ds[s][e], in_sum));
+          out_sum = fmaf(kv[r], du[s][e], out_sum);
+          du[s][e] = fmaf(rate, du[s][e], -ds[s][e]);
         }
       }
       in_sum += __shfl_xor(in_sum, 32);
       out_sum += __shfl_xor(out_sum, 32);
       if (half == 0) {
-        s_in[c0 / 32 + kt][i] = in_sum;
-        s_out[c0 / 32 + kt][i] = out_sum;
+        s_in[c0 / 32 + kt][t] = in_sum;
+        s_out[c0 / 32 + kt][t] = out_sum;
       }
-      const char* kat = sK + 32 * kt * ES + col_share<M, 2, RK>(lane);
-      const char* qat = sQ + 32 * kt * ES + col_share<M, 2, RK>(lane);
+      const char* kat = sK + 32 * kt * ES + col_share<M, 2, RB>(lane);
+      const char* qat = sQ + 32 * kt * ES + col_share<M, 2, RB>(lane);
 #pragma unroll
       for (int f = 0; f < 4; ++f) {
         const int jt = f >> 1;
-        const auto kc = col_op<M, 2, RK>(kat, 16 * f, 0);
+        const auto kc = col_op<M, 2, RB>(kat, 16 * f, 0);
         Op<M, P> x;
         auto both = [&](auto&& get) {
 #pragma unroll
@@ -232,15 +299,15 @@ __global__ __launch_bounds__(256) void dr_grad_kernel(DrGrad A) {
               x = one;
           }
         };
-        both([&](int p) { return row_op<M, 2>(sX[p] + i * RW, f, half); });
-        mul<32>(du, kc, x);
+        both([&](int p) { return row_op<M, 2>(s_x[p] + t * RB, f, half); });
+        mul<32>(du[s], kc, x);
         if (jt <= it) {
-          both([&](int p) { return row_op<M, 2>(sW1[p] + i * RW, f, half); });
-          mul<32>(dq, kc, x);
+          both([&](int p) { return row_op<M, 2>(sP + p * kSlab + t * RB, f, half); });
+          mul<32>(dq[s], kc, x);
         }
         if (jt >= it) {
-          both([&](int p) { return col_op<M, 2, RW>(sW1[p] + col_share<M, 2, RW>(lane), 16 * f, 32 * it); });
-          mul<32>(du, col_op<M, 2, RK>(qat, 16 * f, 0), x);
+          both([&](int p) { return col_op<M, 2, RB>(sP + p * kSlab + col_share<M, 2, RB>(lane), 16 * f, 32 * it); });
+          mul<32>(du[s], col_op<M, 2, RB>(qat, 16 * f, 0), x);
         }
       }
       auto out = [&](void* p, int f32, const f16v& v) {
@@ -249,60 +316,90 @@ __global__ __launch_bounds__(256) void dr_grad_kernel(DrGrad A) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const int col = c0 + 32 * kt + 8 * q + 4 * half;
-          const uint32_t to = (i * A.H * A.Dk + col) * size;
+          const uint32_t to = (t * A.H * A.Dk + col) * size;
           if (kNarrow && !f32) {
             __builtin_amdgcn_raw_buffer_store_b64(
                 u2{pack_bf16x2(v[4 * q], v[4 * q + 1]), pack_bf16x2(v[4 * q + 2], v[4 * q + 3])}, r,
-                la_in((i < n) & (col < A.Dk), to), 0, 0);
+                la_in((t < n) & (col < A.Dk), to), 0, 0);
           } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const uint32_t one = la_in((i < n) & (col + e < A.Dk), to + e * size);
-              if (f32)
+              const uint32_t one = la_in((t < n) & (col + e < A.Dk), to + e * size);
+              if (f32 || A.dtype == PRNN_F32)
                 stb<float>(r, one, 0, v[4 * q + e]);
+              else if (A.dtype == PRNN_F16)
+                stb<f16>(r, one, 0, v[4 * q + e]);
               else
-                stb<T>(r, one, 0, v[4 * q + e]);
+                stb<bf16>(r, one, 0, v[4 * q + e]);
             }
           }
         }
       };
-      out(A.dq, A.q_f32, dq);
-      out(A.dk, A.k_f32, du);
+      out(A.dq, A.q_f32, dq[s]);
+      out(A.dk, A.k_f32, du[s]);
     }
   }
-  if (!flow) return;
+  if (!A.dg && !A.g_part && !A.dbeta) return;
   __syncthreads();
 
-  // ---- 3
-  if (wave != 0) return;
-  const int tiles = (A.Dk + 31) / 32;
-  float into = 0.0f, from = 0.0f;
-  for (int t = 0; t < tiles; ++t) {
-    into += s_in[t][lane];
-    from += s_out[t][lane];
-  }
-  // row j: sums of its uses from l on
-#pragma unroll 8
-  for (int l = 63; l > 0; --l) {
-    if (l > lane) {
-      from += sF[lane * kLf + l];
-      sF[lane * kLf + l] = from;
+  // ---- 3: four lanes per token, a quarter of the others' each
+  const int tok = tid >> 2, part = tid & 3, tiles = (A.Dk + 31) / 32;
+  {
+    // row tok: sums of its uses from l on, what the adjoint behind reads among them
+    float m[16], sum = 0.0f, out = 0.0f;
+#pragma unroll
+    for (int x = 15; x >= 0; --x) {
+      const int l = 16 * part + x;
+      sum += l > tok ? sF[tok * kLf + l] : 0.0f;
+      m[x] = sum;
+    }
+    for (int k = 0; k < tiles; ++k) out += s_out[k][tok];
+    const float s1 = __shfl_down(sum, 1), s2 = __shfl_down(sum, 2), s3 = __shfl_down(sum, 3);
+    const float after = out + ((part < 1 ? s3 : 0.0f) + (part < 2 ? s2 : 0.0f)) + (part < 3 ? s1 : 0.0f);
+    const float rate = sw[kWb * 64 + tok];
+#pragma unroll
+    for (int x = 0; x < 16; ++x) {
+      const int l = 16 * part + x;
+      if (l > tok) sF[tok * kLf + l] = rate * (after + m[x]);
+    }
+    if (wave == 3) {  // what the tokens from one on read of the state before
+      float into = 0.0f;
+      for (int k = 0; k < tiles; ++k) into += s_in[k][lane];
+#pragma unroll
+      for (int m = 1; m < 64; m <<= 1) {
+        const float o = __shfl_down(into, m);
+        if (lane + m < 64) into += o;
+      }
+      s_into[lane] = into + s_through;
+    }
+    if (A.dbeta && part == 0 && tok < n) {
+      const float d = after + m[0] + s_own[tok];
+      const size_t at = (tok0 + tok) * A.H + h;
+      if (A.b_dtype == PRNN_F32)
+        static_cast<float*>(A.dbeta)[at] = d;
+      else if (A.b_dtype == PRNN_F16)
+        static_cast<f16*>(A.dbeta)[at] = from_f32<f16>(d);
+      else
+        static_cast<bf16*>(A.dbeta)[at] = from_f32<bf16>(d);
     }
   }
-  // the state's uses from token i on
+  if (!A.dg && !A.g_part) return;
+  __syncthreads();
+  // column tok: the sources before it
+  float F = 0.0f;
 #pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const float o = __shfl_down(into, m);
-    if (lane + m < 64) into += o;
+  for (int x = 0; x < 16; ++x) {
+    const int j = 16 * part + x;
+    F += j < tok ? sF[j * kLf + tok] : 0.0f;
   }
-  float F = s_through + into;
-#pragma unroll 8
-  for (int j = 0; j < 63; ++j)
-    if (j < lane) F += sF[j * kLf + lane];
-  const bool there = lane < n;
-  if (!there || la_decay(A.g, batch, u.begin + (there ? lane : 0), h) <= -104.0f) F = 0.0f;
-  if (A.dg && there) {
-    const size_t at = (tok0 + lane) * A.H + h;
+  F += __shfl_xor(F, 1);
+  F += __shfl_xor(F, 2);
+  F += s_into[tok];
+  const bool there = tok < n;
+  // nothing comes through a factor that is zero
+  if (!there || la_decay(A.g, batch, u.begin + (there ? tok : 0), h) <= -104.0f) F = 0.0f;
+  if (A.dg && there && part == 0) {
+    const size_t at = (tok0 + tok) * A.H + h;
     if (A.g_dtype == PRNN_F32)
       static_cast<float*>(A.dg)[at] = F;
     else if (A.g_dtype == PRNN_F16)
@@ -311,26 +408,34 @@ __global__ __launch_bounds__(256) void dr_grad_kernel(DrGrad A) {
       static_cast<bf16*>(A.dg)[at] = from_f32<bf16>(F);
   }
   if (A.g_part) {
+    F = part == 0 ? F : 0.0f;
 #pragma unroll
-    for (int m = 1; m < 64; m <<= 1) F += __shfl_xor(F, m);
-    if (lane == 0) A.g_part[unit] = F;
+    for (int m = 4; m < 64; m <<= 1) F += __shfl_xor(F, m);
+    if (lane == 0) s_waves[wave] = F;
+    __syncthreads();
+    if (tid == 0) A.g_part[unit] = (s_waves[0] + s_waves[1]) + (s_waves[2] + s_waves[3]);
   }
 }
 
-template <class M, typename T>
+template <class M, int KS, bool WIDE>
 int launch(const DrGrad& a, hipStream_t stream) {
   const long long groups = dr_units(a.seqs, kDrC) * a.H;
   if (int rc = check_grid("delta_rule backward", groups, 256)) return rc;
-  dr_grad_kernel<M, T><<<static_cast<unsigned>(groups), 256, 0, stream>>>(a);
+  dr_grad_kernel<M, KS, WIDE><<<static_cast<unsigned>(groups), 256, 0, stream>>>(a);
   PRNN_HIP(hipGetLastError());
   return PRNN_OK;
+}
+template <class M>
+int launch_width(const DrGrad& a, hipStream_t stream) {
+  if (a.Dk <= 64) return launch<M, 1, false>(a, stream);
+  if constexpr (sizeof(typename M::E) == 4) return launch<M, 1, true>(a, stream);  // registers
+  else return a.Dk <= 128 ? launch<M, 2, false>(a, stream) : launch<M, 2, true>(a, stream);
 }
 
 }  // namespace
 
 int dr_grad(const DrGrad& a, bool bf16_walk, hipStream_t stream) {
-  if (bf16_walk) return launch<InBf16, bf16>(a, stream);
-  return with_storage(a.dtype, [&](auto z) { return launch<InF32, decltype(z)>(a, stream); });
+  return bf16_walk ? launch_width<InBf16>(a, stream) : launch_width<InF32>(a, stream);
 }
 
 }  // namespace prnn

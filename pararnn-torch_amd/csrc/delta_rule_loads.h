@@ -61,17 +61,22 @@ struct Staged {
   }
 };
 
-// Eight elements of a row from column c0 as they are multiplied; zeros outside.
-template <class M, typename T>
-__device__ __forceinline__ Op<M, 1> global_op(rsrc_t r, bool in, uint32_t row, int c0, int width) {
+// Operand `which` of an array of them (dr_operand_at).
+template <class M>
+__device__ __forceinline__ Op<M, 1> global_op(rsrc_t r, bool in, int which) {
+  constexpr int ES = static_cast<int>(sizeof(typename M::E));
+  const int lane = threadIdx.x & 63;
   Op<M, 1> o;
-  if constexpr (sizeof(typename M::E) == 2) {
+  if constexpr (ES == 2) {
     o.p[0] = __builtin_bit_cast(
-        b8, __builtin_amdgcn_raw_buffer_load_b128(r, la_in(in & (c0 < width), row + c0 * 2), 0, 0));
+        b8, __builtin_amdgcn_raw_buffer_load_b128(r, la_in(in, (which * 64 + lane) * 16), 0, 0));
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      o.x[i] = ldb<T>(r, la_in(in & (c0 + i < width), row + (c0 + i) * static_cast<int>(sizeof(T))), 0);
+    for (int k = 0; k < 2; ++k) {
+      const u4 w = __builtin_amdgcn_raw_buffer_load_b128(r, la_in(in, (which * 64 + lane) * 32 + 16 * k), 0, 0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o.x[4 * k + i] = __uint_as_float(w[i]);
+    }
   }
   return o;
 }

@@ -1,8 +1,8 @@
 // Gated delta rule: every chunk's triangular system and pairs, a workgroup per chunk and head.
 //
-// Three waves, one per tile of 32 x 32 of the lower triangle: k k^T and q k^T by rows straight from
-// memory (no LDS: 16 bytes a lane are an operand), weighted by the exponentials of the decays'
-// differences.  The unit triangular 1 + M is inverted in fp32: the four diagonal blocks of 16 by
+// Three waves, one per tile of 32 x 32 of the lower triangle: k k^T and q k^T, weighted by the
+// exponentials of the decays' differences, which a fourth wave sums up.  Rows come through LDS: a load
+// of operands straight from memory touches a line for every 32 bytes (12400 of 30000 cycles a system).  The unit triangular 1 + M is inverted in fp32: the four diagonal blocks of 16 by
 // substitution, a column per lane of one wave; below them T_ij = -T_ii sum_m M_im T_mj in block
 // columns, one per wave, on v_mfma_f32_16x16x4_f32 with the results as the next products' operands.
 // (A product of powers (1 - M)(1 + M^2)(1 + M^4) .. has fewer steps, but the powers of keys that lie
@@ -18,51 +18,48 @@ __device__ __forceinline__ bool not_finite(float v) {
   return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u;
 }
 
-template <class M, typename T>
-__global__ __launch_bounds__(192) void dr_systems_kernel(DrSystems A) {
+template <class M>
+__global__ __launch_bounds__(256) void dr_systems_kernel(DrSystems A) {
   using E = typename M::E;
-  __shared__ __align__(16) float sM[kDrC * kLd], sT[kDrC * kLd];
-  __shared__ float s_hi[kDrC], s_lo[kDrC], s_b[kDrC];
+  constexpr bool kNarrow = sizeof(E) == 2;
+  constexpr int RB = dr_row_k(kNarrow, 64);
+  __shared__ __align__(16) float lds[2 * kDrC * kLd];  // slabs of k and q, then the system and its inverse
+  static_assert(2 * kDrC * RB <= static_cast<int>(sizeof(lds)), "slabs fit");
+  __shared__ __align__(16) float s_hi[kDrC], s_lo[kDrC], s_b[kDrC];
+  __shared__ float s_whole;
   __shared__ int s_stop;
+  __shared__ bool s_bad[kDrC];
+  float *const sM = lds, *const sT = lds + kDrC * kLd;
+  char *const sK = reinterpret_cast<char*>(lds), *const sQ = sK + kDrC * RB;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l32 = lane & 31, half = lane >> 5;
+  const int it = wave > 0, jt = wave > 1;  // (the fourth wave's are not used)
+  const int ti = 32 * it + l32, tj = 32 * jt + l32;
+
   const int h = blockIdx.x % A.H, id = blockIdx.x / A.H;
   const DrUnit u = dr_unit(A.seqs, kDrC, id);
   if (!u.any || u.begin >= u.end) return;
   const int n = u.end - u.begin, batch = dr_batch(A.seqs, u);
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l32 = lane & 31, half = lane >> 5;
+  auto rows = [&](const LaView& v) {
+    return static_cast<const char*>(v.p) +
+           (batch * v.sb + (h / v.rep) * v.sh + static_cast<long long>(u.begin) * v.st) * (A.dtype == PRNN_F32 ? 4 : 2);
+  };
+  const char *pk = rows(A.k), *pq = rows(A.q);
+  Staged<M, 64, 256> rk, rq;
+  rk.fetch(pk, A.k.st, n, 0, A.Dk, A.dtype);
+  rq.fetch(pq, A.q.st, n, 0, A.Dk, A.dtype);
+  float g = 0.0f, rate = 0.0f;
+  if (wave == 3 && lane < n) {
+    g = la_decay(A.g, batch, u.begin + lane, h);
+    rate = dr_rate(A.b, batch, u.begin + lane, h);
+  }
   char* sys = A.sys + (static_cast<size_t>(id) * A.H + h) * kDrSys;
   float* weights = reinterpret_cast<float*>(sys + 2 * kDrTiles);
-
   // ---- products: registers earlier tokens j, lanes later ones i (transposed pairs the other way)
-  const int it = wave > 0, jt = wave > 1;
-  auto rows = [&](const LaView& v) {
-    return make_rsrc(static_cast<const T*>(v.p) + (batch * v.sb + (h / v.rep) * v.sh +
-                                                   static_cast<long long>(u.begin) * v.st), 0x7fffffffu);
-  };
-  const rsrc_t rk = rows(A.k), rq = rows(A.q);
-  const int ti = 32 * it + l32, tj = 32 * jt + l32;
-  const uint32_t ki = ti * static_cast<int>(A.k.st) * sizeof(T), kj = tj * static_cast<int>(A.k.st) * sizeof(T),
-                 qi = ti * static_cast<int>(A.q.st) * sizeof(T);
   if (tid == 0) s_stop = kDrC;
   f16v N, P;
 #pragma unroll
   for (int r = 0; r < 16; ++r) N[r] = P[r] = 0.0f;
-  bool bad = false;
-  for (int c = 8 * half; c < A.Dk + 8 * half; c += 16) {
-    const auto k1 = global_op<M, T>(rk, ti < n, ki, c, A.Dk), q1 = global_op<M, T>(rq, ti < n, qi, c, A.Dk);
-    const auto k0 = global_op<M, T>(rk, tj < n, kj, c, A.Dk);
-    mul<32>(N, k0, k1);
-    if (A.transposed)
-      mul<32>(P, q1, k0);
-    else
-      mul<32>(P, k0, q1);
-    float x[8];
-    values(k1, x);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) bad |= not_finite(x[i]);
-  }
-  float hi = 0.0f, lo = 0.0f, rate = 0.0f, back = 0.0f, whole = 0.0f;
-  if (wave == 0) {
-    const float g = lane < n ? la_decay(A.g, batch, u.begin + lane, h) : 0.0f;
+  if (wave == 3) {
     double G = g;
 #pragma unroll
     for (int k = 1; k < 64; k <<= 1) {
@@ -70,60 +67,114 @@ __global__ __launch_bounds__(192) void dr_systems_kernel(DrSystems A) {
       if (lane >= k) G += o;
     }
     const double last = __shfl(G, 63);
-    hi = static_cast<float>(G);
-    lo = static_cast<float>(G - hi);
-    back = static_cast<float>(last - G);
-    whole = static_cast<float>(last);
-    if (lane < n) rate = dr_rate(A.b, batch, u.begin + lane, h);
+    const float hi = static_cast<float>(G), lo = static_cast<float>(G - hi);
     s_hi[lane] = hi;
     s_lo[lane] = lo;
     s_b[lane] = rate;
-    if (not_finite(g) | not_finite(rate)) atomicMin(&s_stop, lane);
-  }
-  __syncthreads();
-  if (bad && it == jt) atomicMin(&s_stop, ti);
-  if (wave == 0) {
     weights[kWg * 64 + lane] = fexp(hi);
-    weights[kWr * 64 + lane] = fexp(back);
+    weights[kWr * 64 + lane] = fexp(static_cast<float>(last - G));
     weights[kWb * 64 + lane] = rate;
     weights[kWhi * 64 + lane] = hi;
     weights[kWlo * 64 + lane] = lo;
+    s_bad[lane] = not_finite(g) | not_finite(rate);
+    if (lane == 0) s_whole = fexp(static_cast<float>(last));
   }
-  __syncthreads();
-  const int stop = s_stop;
-  if (wave == 0)
-    weights[kWmeta * 64 + lane] = lane == 0 ? fexp(whole) : lane == 1 ? __int_as_float(stop) : 0.0f;
-
-  // ---- weights; the system's matrix without what is not finite
-  char* pairs = sys + kDrTiles + wave * (kDrTiles / 3 / M::kParts);
-  const float Hi = s_hi[ti], Lo = s_lo[ti], Bi = s_b[ti];
-  const float Hj = s_hi[tj], Lj = s_lo[tj];
+  bool bad = false;
+  for (int c0 = 0; c0 < A.Dk; c0 += 64) {
+    if (c0 > 0) __syncthreads();
+    rk.template put<RB>(sK, A.dtype);
+    rq.template put<RB>(sQ, A.dtype);
+    __syncthreads();
+    if (c0 + 64 < A.Dk) {
+      rk.fetch(pk, A.k.st, n, c0 + 64, A.Dk, A.dtype);
+      rq.fetch(pq, A.q.st, n, c0 + 64, A.Dk, A.dtype);
+    }
+    if (wave < 3) {
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int j = 32 * jt + 8 * q + 4 * half, i = 32 * it + 8 * q + 4 * half;
-    f4 m, p;
+      for (int f = 0; f < 4; ++f) {
+        const auto k0 = row_op<M, 2>(sK + tj * RB, f, half), k1 = row_op<M, 2>(sK + ti * RB, f, half);
+        const auto q1 = row_op<M, 2>(sQ + ti * RB, f, half);
+        mul<32>(N, k0, k1);
+        if (A.transposed)
+          mul<32>(P, q1, k0);
+        else
+          mul<32>(P, k0, q1);
+        float x[8];
+        values(k1, x);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const float w = fexp((Hi - s_hi[j + r]) + (Lo - s_lo[j + r]));
-      const float b = A.transposed ? Bi : s_b[j + r];
-      m[r] = ((j + r < ti) & (ti < stop)) ? N[4 * q + r] * w * b : 0.0f;
-      if (A.transposed) {  // lane: token j, registers: tokens i
-        const float v = fexp((s_hi[i + r] - Hj) + (s_lo[i + r] - Lj));
-        p[r] = tj <= i + r ? P[4 * q + r] * v * A.scale : 0.0f;
-      } else {
-        p[r] = j + r <= ti ? P[4 * q + r] * w * A.scale : 0.0f;
+        for (int i = 0; i < 8; ++i) bad |= not_finite(x[i]);
       }
     }
-    *reinterpret_cast<f4*>(&sM[ti * kLd + j]) = m;
-    const int unit = dr_unit_of<E>(l32, 2 * q + half);
+  }
+  if (bad && it == jt && wave < 3) atomicMin(&s_stop, ti);
+  if (wave == 3 && s_bad[lane]) atomicMin(&s_stop, lane);
+  __syncthreads();
+  const int stop = s_stop;
+  if (wave == 3)
+    weights[kWmeta * 64 + lane] = lane == 0 ? s_whole : lane == 1 ? __int_as_float(stop) : 0.0f;
+
+  // ---- weights; the system's matrix without what is not finite
+  if (wave < 3) {
+    char* pairs = sys + kDrTiles + wave * (kDrTiles / 3 / M::kParts);
+    const float Hi = s_hi[ti], Lo = s_lo[ti], Bi = s_b[ti];
+    const float Hj = s_hi[tj], Lj = s_lo[tj];
+    float pair[16];
+    auto four = [](const float* v) { return *reinterpret_cast<const f4*>(v); };
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int j = 32 * jt + 8 * q + 4 * half, i = 32 * it + 8 * q + 4 * half;
+      const f4 hj = four(s_hi + j), lj = four(s_lo + j), bj = four(s_b + j);
+      f4 m, p;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float w = fexp((Hi - hj[r]) + (Lo - lj[r]));
+        m[r] = ((j + r < ti) & (ti < stop)) ? N[4 * q + r] * w * (A.transposed ? Bi : bj[r]) : 0.0f;
+        p[r] = j + r <= ti ? P[4 * q + r] * w * A.scale : 0.0f;
+      }
+      if (A.transposed) {  // lane: token j, registers: tokens i
+        const f4 hi = four(s_hi + i), li = four(s_lo + i);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          p[r] = tj <= i + r ? P[4 * q + r] * fexp((hi[r] - Hj) + (li[r] - Lj)) * A.scale : 0.0f;
+      }
+      *reinterpret_cast<f4*>(&sM[ti * kLd + j]) = m;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) pair[4 * q + r] = p[r];
+    }
     if constexpr (sizeof(E) == 2) {
-      const u2 a{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3])};
-      const u2 b{pack_bf16x2(p[0] - lo_bf16(a[0]), p[1] - hi_bf16(a[0])),
-                 pack_bf16x2(p[2] - lo_bf16(a[1]), p[3] - hi_bf16(a[1]))};
-      *reinterpret_cast<u2*>(pairs + l32 * 64 + unit * 8) = a;
-      *reinterpret_cast<u2*>(pairs + kDrTiles / 2 + l32 * 64 + unit * 8) = b;
+      // this lane holds units 2 q + half of its row; halves of the wave exchange them, so that either has
+      // two units side by side (in one order or the other: the exchange by rows keeps such pairs)
+      const bool odd = dr_unit_of<E>(l32, 0) & 1;
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        u2 hi[2], lo[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float* p = pair + 8 * m + 4 * k;
+          hi[k] = u2{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3])};
+          lo[k] = u2{pack_bf16x2(p[0] - lo_bf16(hi[k][0]), p[1] - hi_bf16(hi[k][0])),
+                     pack_bf16x2(p[2] - lo_bf16(hi[k][1]), p[3] - hi_bf16(hi[k][1]))};
+        }
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          uint32_t a = hi[0][w], b = hi[1][w], c = lo[0][w], d = lo[1][w];
+          swap_halves(a, b);
+          swap_halves(c, d);
+          hi[0][w] = a;
+          hi[1][w] = b;
+          lo[0][w] = c;
+          lo[1][w] = d;
+        }
+        const int at = l32 * 64 + (dr_unit_of<E>(l32, 4 * m + 2 * half) & ~1) * 8;
+        const u2 h0 = odd ? hi[1] : hi[0], h1 = odd ? hi[0] : hi[1], l0 = odd ? lo[1] : lo[0], l1 = odd ? lo[0] : lo[1];
+        *reinterpret_cast<u4*>(pairs + at) = u4{h0[0], h0[1], h1[0], h1[1]};
+        *reinterpret_cast<u4*>(pairs + kDrTiles / 2 + at) = u4{l0[0], l0[1], l1[0], l1[1]};
+      }
     } else {
-      *reinterpret_cast<f4*>(pairs + l32 * 128 + unit * 16) = p;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *reinterpret_cast<f4*>(pairs + l32 * 128 + dr_unit_of<E>(l32, 2 * q + half) * 16) =
+            f4{pair[4 * q], pair[4 * q + 1], pair[4 * q + 2], pair[4 * q + 3]};
     }
   }
   __syncthreads();
@@ -177,35 +228,57 @@ __global__ __launch_bounds__(192) void dr_systems_kernel(DrSystems A) {
   __syncthreads();
 
   // ---- the strictly triangular part of the inverse
+  if (wave < 3) {
   char* tiles = sys + wave * (kDrTiles / 3 / M::kParts);
   const int row = (A.transposed ? 32 * jt : 32 * it) + l32, col0 = A.transposed ? 32 * it : 32 * jt;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int unit = 4 * half + k, col = col0 + 4 * unit;
-    f4 t;
+  for (int m = 0; m < 2; ++m) {
+    f4 t[2];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const float v = A.transposed ? sT[(col + r) * kLd + row] : sT[row * kLd + col + r];
-      t[r] = (A.transposed ? col + r > row : col + r < row) ? v : 0.0f;
+    for (int k = 0; k < 2; ++k) {
+      const int col = col0 + 4 * (4 * half + 2 * m + k);
+      f4 w;
+      if (A.transposed) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) w[r] = sT[(col + r) * kLd + row];
+      } else {
+        w = *reinterpret_cast<const f4*>(&sT[row * kLd + col]);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float v = w[r];
+        t[k][r] = (A.transposed ? col + r > row : col + r < row) ? v : 0.0f;
+      }
     }
-    const int to = dr_unit_of<E>(l32, unit);
+    const int to = dr_unit_of<E>(l32, 4 * half + 2 * m);
     if constexpr (sizeof(E) == 2) {
-      const u2 a{pack_bf16x2(t[0], t[1]), pack_bf16x2(t[2], t[3])};
-      const u2 b{pack_bf16x2(t[0] - lo_bf16(a[0]), t[1] - hi_bf16(a[0])),
-                 pack_bf16x2(t[2] - lo_bf16(a[1]), t[3] - hi_bf16(a[1]))};
-      *reinterpret_cast<u2*>(tiles + l32 * 64 + to * 8) = a;
-      *reinterpret_cast<u2*>(tiles + kDrTiles / 2 + l32 * 64 + to * 8) = b;
+      if (to & 1) {
+        const f4 x = t[0];
+        t[0] = t[1];
+        t[1] = x;
+      }
+      u4 hi, lo;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float a = t[k >> 1][2 * (k & 1)], b = t[k >> 1][2 * (k & 1) + 1];
+        hi[k] = pack_bf16x2(a, b);
+        lo[k] = pack_bf16x2(a - lo_bf16(hi[k]), b - hi_bf16(hi[k]));
+      }
+      *reinterpret_cast<u4*>(tiles + l32 * 64 + (to & ~1) * 8) = hi;
+      *reinterpret_cast<u4*>(tiles + kDrTiles / 2 + l32 * 64 + (to & ~1) * 8) = lo;
     } else {
-      *reinterpret_cast<f4*>(tiles + l32 * 128 + to * 16) = t;
+      *reinterpret_cast<f4*>(tiles + l32 * 128 + to * 16) = t[0];
+      *reinterpret_cast<f4*>(tiles + l32 * 128 + dr_unit_of<E>(l32, 4 * half + 2 * m + 1) * 16) = t[1];
     }
+  }
   }
 }
 
-template <class M, typename T>
+template <class M>
 int launch(const DrSystems& a, hipStream_t stream) {
   const long long groups = dr_units(a.seqs, kDrC) * a.H;
-  if (int rc = check_grid("delta_rule", groups, 192)) return rc;
-  dr_systems_kernel<M, T><<<static_cast<unsigned>(groups), 192, 0, stream>>>(a);
+  if (int rc = check_grid("delta_rule", groups, 256)) return rc;
+  dr_systems_kernel<M><<<static_cast<unsigned>(groups), 256, 0, stream>>>(a);
   PRNN_HIP(hipGetLastError());
   return PRNN_OK;
 }
@@ -213,8 +286,7 @@ int launch(const DrSystems& a, hipStream_t stream) {
 }  // namespace
 
 int dr_systems(const DrSystems& a, bool bf16_walk, hipStream_t stream) {
-  if (bf16_walk) return launch<InBf16, bf16>(a, stream);
-  return with_storage(a.dtype, [&](auto z) { return launch<InF32, decltype(z)>(a, stream); });
+  return bf16_walk ? launch<InBf16>(a, stream) : launch<InF32>(a, stream);
 }
 
 }  // namespace prnn

@@ -117,7 +117,6 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
   __shared__ __align__(16) char sK[kDrC * RK];
   __shared__ __align__(16) char sQ[kQ ? kDrC * RK : 16];
   __shared__ __align__(16) char sZ[kDrC * RZ];
-  __shared__ __align__(16) char sE[KIND == kDrBackward ? kDrC * RZ : 16];
   __shared__ __align__(16) char s_sys[kSysLds ? kSysBytes : 16];
   __shared__ __align__(16) float sW[kDrW * 64];
 
@@ -131,7 +130,6 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
   const int nn = lane % NC, g = lane / NC;
   const bool transfer = kOwn && tile >= A.own_tiles;
   const int col0 = (transfer ? tile - A.own_tiles : tile) * VT;
-  const int width = transfer ? A.Dk : A.Dv;  // the state's columns
   const int col = col0 + NC * wave + nn;
   const int batch = dr_batch(A.seqs, pc);
   const int row0 = dr_base(A.seqs, kDrC, pc.seq, pc.s0) + (pc.begin - pc.s0) / kDrC;
@@ -146,7 +144,7 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       const int i = NC * t + 4 * G * (r >> 2) + 4 * g + (r & 3);
-      S[t][r] = transfer && i == col ? 1.0f : 0.0f;
+      S[t][r] = transfer && i == col && i < A.Dk ? 1.0f : 0.0f;
     }
   if (!kOwn) {
     const float* src = nullptr;
@@ -167,7 +165,7 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
   }
 
   std::conditional_t<kAhead, Staged<M, KD, NT>, NotStaged> rk, rq;
-  Staged<M, VT, NT> rz, re;
+  Staged<M, VT, NT> rz;
   u4 rs[kSysLds ? kSysUnits : 1], rw[(kDrW * 64 / 4 + NT - 1) / NT];
   const int size = kNarrow || A.dtype != PRNN_F32 ? 2 : 4;
   auto head = [&](const LaView& v, int t) {
@@ -186,15 +184,12 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
     if constexpr (kAhead) rk.fetch(head(A.k, t), A.k.st, n, 0, A.Dk, A.dtype);
     if constexpr (kAhead && kQ) rq.fetch(head(A.q, t), A.q.st, n, 0, A.Dk, A.dtype);
     rz.fetch(head(A.z, t), A.z.st, transfer ? 0 : n, col0, A.Dv, A.dtype);
-    if constexpr (KIND == kDrBackward)
-      re.fetch(static_cast<const char*>(A.e) + ((tok0 + t) * A.H + h) * A.Dv * ES,
-               static_cast<long long>(A.H) * A.Dv, n, col0, A.Dv, kNarrow ? PRNN_BF16 : PRNN_F32);
   };
   // What a chunk leaves is stored after the next one's rows have come: loads and stores come back in
   // order, and a wait for rows behind stores would wait for those too (155 us for .. without).
   constexpr int kHeld = kNarrow ? NC / 2 : NC;
   uint32_t held_o[KIND == kDrForward ? kHeld : 1], held_u[kOwn ? 1 : kHeld];  // out; e or dv
-  float held32[KIND == kDrBackward && kNarrow ? NC : 1], held_db = 0.0f;
+  float held32[KIND == kDrBackward && kNarrow ? NC : 1];
   int held_n = 0, held_c = 0;
   auto at_token = [&](int i) { return NC * (i / RT) + 4 * G * ((i % RT) >> 2) + 4 * g + (i & 3); };
   auto hold = [&](uint32_t* to, const float* v) {
@@ -241,12 +236,17 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
     }
     if constexpr (!kOwn) {
       void* p = kBack ? A.dv : A.e;
-      if (p) {
-        const rsrc_t r = make_rsrc(static_cast<E*>(p) + ((tok0 + t0) * A.H + h) * A.Dv, 0x7fffffffu);
+      if (p && n > 0) {
+        // backwards dense rows of the tokens that are there, forwards operands (zeros behind the sequence)
+        const size_t unit = static_cast<size_t>(row0 + held_c) * A.H + h;
+        const rsrc_t r = make_rsrc(static_cast<E*>(p) + (kBack ? ((tok0 + t0) * A.H + h) * A.Dv
+                                                               : unit * dr_operand_elems(kDrC, A.Dv)),
+                                   0x7fffffffu);
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
           const int tok = at_token(i);
-          const uint32_t to = la_in((tok < n) & (col < A.Dv), (tok * A.H * A.Dv + col) * ES);
+          const uint32_t to = kBack ? la_in((tok < n) & (col < A.Dv), (tok * A.H * A.Dv + col) * ES)
+                                    : la_in(col < (A.Dv + 15) / 16 * 16, dr_operand_at(A.Dv, tok, col) * ES);
           if constexpr (kNarrow)
             __builtin_amdgcn_raw_buffer_store_b16(i & 1 ? held_u[i / 2] >> 16 : held_u[i / 2], r, to, 0, 0);
           else
@@ -255,8 +255,6 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
       }
     }
     if constexpr (KIND == kDrBackward) {
-      const int tok = at_token(lane % NC);
-      if (tok < n) A.db[(static_cast<size_t>(tile * W + wave) * A.tokens + tok0 + t0 + tok) * A.H + h] = held_db;
       if constexpr (kNarrow) {
         if (A.dv32) {
           const rsrc_t rf = make_rsrc(A.dv32 + ((tok0 + t0) * A.H + h) * A.Dv, 0x7fffffffu);
@@ -282,7 +280,6 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
       if constexpr (kQ) fill<M, KD, NT, RK>(sQ, head(A.q, t0), A.q.st, n, A.Dk, A.dtype);
     }
     rz.template put<RZ>(sZ, A.dtype);
-    if constexpr (KIND == kDrBackward) re.template put<RZ>(sE, kNarrow ? PRNN_BF16 : PRNN_F32);
 #pragma unroll
     for (int k = 0; k < (kSysLds ? kSysUnits : 0); ++k) *reinterpret_cast<u4*>(s_sys + (tid + k * NT) * 16) = rs[k];
 #pragma unroll
@@ -291,14 +288,16 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
     if (!kOwn) flush();
     // what the gradients of this chunk need of the state
     if (!kOwn && A.keep) {
-      const rsrc_t rs = make_rsrc(static_cast<E*>(A.keep) + (static_cast<size_t>(row0 + c) * A.H + h) * state_floats,
-                                  static_cast<uint32_t>(state_floats) * ES);
+      const size_t elems = dr_operand_elems(A.Dk, A.Dv);
+      const rsrc_t rs = make_rsrc(static_cast<E*>(A.keep) + (static_cast<size_t>(row0 + c) * A.H + h) * elems,
+                                  static_cast<uint32_t>(elems) * ES);
 #pragma unroll
       for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
           const int i = NC * t + 4 * G * (r >> 2) + 4 * g + (r & 3);
-          store_elem<M>(rs, la_in((i < A.Dk) & (col < A.Dv), (i * A.Dv + col) * ES), S[t][r]);
+          store_elem<M>(rs, la_in((i < (A.Dk + 31) / 32 * 32) & (col < (A.Dv + 15) / 16 * 16),
+                                  dr_operand_at(A.Dv, i, col) * ES), S[t][r]);
         }
     }
     const char* sS = kSysLds ? s_sys : A.sys + (static_cast<size_t>(row0 + c) * A.H + h) * kDrSys;
@@ -461,30 +460,6 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
       }
     }
     if constexpr (KIND == kDrBackward) {
-      // ---- db: du . e over the wave's columns; dv
-      float d[NC];
-      const char* eat = sE + NC * wave * ES + col_share<M, G, RZ>(lane);
-#pragma unroll
-      for (int f = 0; f < TF; ++f) {
-        float v[8];
-        values(col_op<M, G, RZ>(eat, 8 * G * f, 0), v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int i = 8 * f + e;
-          d[i] = col < A.Dv ? v[e] * Y[i / RT][i % RT] : 0.0f;
-        }
-      }
-      if constexpr (NC == 32) {
-        float h2[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(d[i]), __float_as_uint(d[16 + i]), false, false);
-          h2[i] = __uint_as_float(s[0]) + __uint_as_float(s[1]);
-        }
-        held_db = row_sums16(h2, lane);
-      } else {
-        held_db = row_sums16(d, lane);
-      }
       hold(held_u, u);
       if constexpr (kNarrow) {
 #pragma unroll
@@ -542,19 +517,22 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
   // ---- the state behind the piece
   float* dst = nullptr;
   if (kOwn) {
-    dst = transfer ? A.transfer + (static_cast<size_t>(piece) * A.H + h) * A.Dk * A.Dk
+    dst = transfer ? A.transfer + (static_cast<size_t>(piece) * A.H + h) * dr_operand_elems(A.Dk, A.Dk)
                    : A.piece + (static_cast<size_t>(piece) * A.H + h) * state_floats;
   } else if (pc.index == (kBack ? 0 : pc.count - 1)) {
     if (float* row = la_row(A.last, pc.seq, A.H * state_floats)) dst = row + h * state_floats;
   }
   if (dst) {
-    const rsrc_t rs = make_rsrc(dst, static_cast<uint32_t>(A.Dk * width) * 4);
+    const rsrc_t rs = make_rsrc(
+        dst, static_cast<uint32_t>(transfer ? dr_operand_elems(A.Dk, A.Dk) : state_floats) * 4);
+    const int rows = transfer ? (A.Dk + 31) / 32 * 32 : A.Dk, cols = transfer ? (A.Dk + 15) / 16 * 16 : A.Dv;
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
         const int i = NC * t + 4 * G * (r >> 2) + 4 * g + (r & 3);
-        stb<float>(rs, la_in((i < A.Dk) & (col < width), (i * width + col) * 4), 0, S[t][r]);
+        const uint32_t at = transfer ? dr_operand_at(A.Dk, i, col) : static_cast<uint32_t>(i * A.Dv + col);
+        stb<float>(rs, la_in((i < rows) & (col < cols), at * 4), 0, S[t][r]);
       }
   }
 }

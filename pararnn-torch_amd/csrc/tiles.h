@@ -210,24 +210,11 @@ __device__ __forceinline__ void store_elem(rsrc_t r, uint32_t at, float v) {
     stb<float>(r, at, 0, v);
 }
 
-// Sums of v[0 .. 15] over the 16 lanes of a row: lane i of it gets that of v[i].
-template <int CTRL>
-__device__ __forceinline__ float dpp_of(float v) {
-  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
-}
-__device__ __forceinline__ float row_sums16(const float* v, int lane) {
-  const bool b3 = lane & 8, b2 = lane & 4, b1 = lane & 2, b0 = lane & 1;
-  float a[8], c[4], d[2];
-#pragma unroll
-  for (int i = 0; i < 8; ++i)  // i and 15 - i
-    a[i] = (b3 ? v[8 + i] : v[i]) + dpp_of<0x140>(b3 ? v[i] : v[8 + i]);
-#pragma unroll
-  for (int i = 0; i < 4; ++i)  // i and 7 - i
-    c[i] = (b2 ? a[4 + i] : a[i]) + dpp_of<0x141>(b2 ? a[i] : a[4 + i]);
-#pragma unroll
-  for (int i = 0; i < 2; ++i)  // i and i ^ 2
-    d[i] = (b1 ? c[2 + i] : c[i]) + dpp_of<0x4e>(b1 ? c[i] : c[2 + i]);
-  return (b0 ? d[1] : d[0]) + dpp_of<0xb1>(b0 ? d[0] : d[1]);
+// Upper half of a's lanes for the lower half of b's.
+__device__ __forceinline__ void swap_halves(uint32_t& a, uint32_t& b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  a = r[0];
+  b = r[1];
 }
 
 }  // namespace prnn
