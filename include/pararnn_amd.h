@@ -562,7 +562,8 @@ PRNN_API int prnn_linear_attention_step(const void* q, long long q_sb, long long
  * token, float32 or of the storage type, by strides.  bfloat16 arrays whose widths are multiples of 8
  * must have rows on 16-byte boundaries, at least a row apart.
  * kept (prnn_delta_rule_kept_size bytes, 256-byte aligned; NULL: no backward pass follows): what the
- * backward call of the same problem reads of the forward one. */
+ * backward call of the same problem reads of the forward one; the forward call's workspace is smaller
+ * with it (workspace_size's kept: whether it is given). */
 typedef struct prnn_delta_rule_problem {
   prnn_linear_attention_problem la;
   const void* b;
@@ -570,7 +571,7 @@ typedef struct prnn_delta_rule_problem {
   int b_dtype;
 } prnn_delta_rule_problem;
 
-PRNN_API size_t prnn_delta_rule_workspace_size(const prnn_delta_rule_problem* problem);
+PRNN_API size_t prnn_delta_rule_workspace_size(const prnn_delta_rule_problem* problem, int kept);
 PRNN_API size_t prnn_delta_rule_kept_size(const prnn_delta_rule_problem* problem);
 PRNN_API int prnn_delta_rule(const prnn_delta_rule_problem* problem, const prnn_la_view* out,
                              float* state_out, const int* out_table, int out_rows, void* kept,

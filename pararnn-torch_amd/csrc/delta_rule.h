@@ -15,7 +15,7 @@
 //
 // Its gradients, with R = dL/dS behind the chunk:
 //
-//   (1 + diag(b) N)^T du = scale P^T go + exp(G_last - G) K R,     dv = b du,   db = du . e
+//   (1 + N diag(b))^T dv = diag(b) [ scale P^T go + exp(G_last - G) K R ]     the same system
 //   R' = exp(G_last) R + (scale exp(G) Q)^T go - (exp(G) K)^T dv
 //   dq = scale [ exp(G) go S^T + (go u^T . lower) K ]
 //   dk = exp(G_last - G) u R^T + scale (go u^T . lower)^T Q - exp(G) dv S^T - (X + X^T) K,
@@ -96,8 +96,7 @@ __device__ __forceinline__ int dr_batch(const LaSeqs& q, const DrUnit& u) { retu
 // ---- a chunk's system --------------------------------------------------------------------
 //
 // Per chunk and head: the strictly lower part of the inverse, then the pairs, each as the tiles
-// (0, 0), (1, 0), (1, 1) of 32 x 32 (the transposed ones, for the walk backwards: (0, 0), (0, 1),
-// (1, 1)), rows of 32 elements whose units of four are exchanged by the row (dr_unit_of), bf16 in
+// (0, 0), (1, 0), (1, 1) of 32 x 32, rows of 32 elements whose units of four are exchanged by the row (dr_unit_of), bf16 in
 // two parts of 6 KB or fp32; then kDrW rows of 64 floats.
 constexpr int kDrTiles = 3 * 32 * 32 * 4;  // bytes of a matrix in either arithmetic
 enum { kWg, kWr, kWb, kWhi, kWlo, kWmeta, kDrW };  // exp(G), exp(G_last - G), b, G in two parts
@@ -123,7 +122,7 @@ struct DrSystems {
   LaView q, k;
   LaDecay g, b;
   char* sys;
-  int H, Dk, dtype, transposed;
+  int H, Dk, dtype;
   float scale;
 };
 
@@ -158,7 +157,7 @@ struct DrGrad {
   LaSeqs seqs;
   LaView q, k, go;
   LaDecay g, b;
-  const char* sys;           // the transposed systems: only their decays and rates are read
+  const char* sys;           // only its decays and rates are read
   const void *e, *before, *behind;  // as operands: (chunk, H), 64 x Dv and Dk x Dv
   const void* dv;            // (token, H, Dv) of the arithmetic's type
   void *dq, *dk;             // (token, H, Dk): the arithmetic's type, or floats (q_f32, k_f32)

@@ -47,9 +47,11 @@ LaSeqs sequences_of(const Problem& a) {
   return q;
 }
 
-// What the backward pass reads of the forward one, as operands: e, then the states before the chunks.
+// What the backward pass reads of the forward one: as operands e and the states before the chunks, and
+// the chunks' systems.
 struct Kept {
   void *e, *before;
+  char* sys;
   size_t bytes;
 };
 Kept kept_of(void* p, const Problem& a) {
@@ -59,6 +61,7 @@ Kept kept_of(void* p, const Problem& a) {
   const size_t units = dr_units(sequences_of(a), kDrC);
   k.e = c.take(units * heads * dr_operand_elems(kDrC, a.la.Dv) * size);
   k.before = c.take(units * heads * dr_operand_elems(a.la.Dk, a.la.Dv) * size);
+  k.sys = static_cast<char*>(c.take(units * heads * kDrSys));
   k.bytes = c.used;
   return k;
 }
@@ -123,12 +126,12 @@ Plan plan(const Problem& a) {
   return p;
 }
 
-Scratch carve(void* ws, const Problem& a, const Plan& plan, bool backward, bool decay_grad) {
+Scratch carve(void* ws, const Problem& a, const Plan& plan, bool systems, bool backward, bool decay_grad) {
   Carver c(ws);
   Scratch s{};
   const size_t heads = a.la.H, tokens = tokens_of(a), size = on_bf16(a) ? 2 : 4;
   const size_t units = dr_units(plan.seqs, kDrC);
-  s.sys = static_cast<char*>(c.take(units * heads * kDrSys));
+  if (systems) s.sys = static_cast<char*>(c.take(units * heads * kDrSys));
   if (plan.cut) {
     const size_t pieces = dr_units(plan.seqs, plan.seqs.len) * heads;
     s.piece = static_cast<float*>(c.take(4 * pieces * a.la.Dk * a.la.Dv));
@@ -147,8 +150,8 @@ Scratch carve(void* ws, const Problem& a, const Plan& plan, bool backward, bool 
   s.bytes = c.used;
   return s;
 }
-size_t need(const Problem& a, bool backward, bool decay_grad) {
-  return carve(nullptr, a, plan(a), backward, decay_grad).bytes;
+size_t need(const Problem& a, bool systems, bool backward, bool decay_grad) {
+  return carve(nullptr, a, plan(a), systems, backward, decay_grad).bytes;
 }
 
 int check_ws(const char* what, size_t need, const void* ws, size_t bytes) {
@@ -162,28 +165,27 @@ LaDecay decay_of(const Problem& a) {
 }
 LaDecay rate_of(const Problem& a) { return LaDecay{a.b, a.b_sb, a.b_st, a.b_sh, a.b_dtype}; }
 
-int systems(const Problem& a, const Scratch& s, bool transposed, hipStream_t st) {
+int systems(const Problem& a, char* sys, hipStream_t st) {
   DrSystems y{};
   y.seqs = sequences_of(a);
   y.q = la_view(a.la.q, a.la, a.la.Dk);
   y.k = la_view(a.la.k, a.la, a.la.Dk);
   y.g = decay_of(a);
   y.b = rate_of(a);
-  y.sys = s.sys;
+  y.sys = sys;
   y.H = a.la.H;
   y.Dk = a.la.Dk;
   y.dtype = a.la.dtype;
-  y.transposed = transposed;
   y.scale = a.la.scale;
   return dr_systems(y, on_bf16(a), st);
 }
 
-DrWalk walk_of(const Problem& a, const Plan& plan, const Scratch& s) {
+DrWalk walk_of(const Problem& a, const Plan& plan, const Scratch& s, const char* sys) {
   DrWalk w{};
   w.seqs = plan.seqs;
   w.q = la_view(a.la.q, a.la, a.la.Dk);
   w.k = la_view(a.la.k, a.la, a.la.Dk);
-  w.sys = s.sys;
+  w.sys = sys;
   w.piece = s.piece;
   w.transfer = s.transfer;
   w.H = a.la.H;
@@ -217,16 +219,17 @@ int walk(const DrWalk& w, bool back, const Problem& a, const Plan& plan, hipStre
 int forward(const Problem& a, const prnn_la_view& out, float* state_out, const int* out_table, int out_rows,
             void* kept, void* ws, hipStream_t st) {
   const Plan p = plan(a);
-  const Scratch s = carve(ws, a, p, false, false);
-  if (int rc = systems(a, s, false, st)) return rc;
-  DrWalk w = walk_of(a, p, s);
+  const Scratch s = carve(ws, a, p, kept == nullptr, false, false);
+  const Kept k = kept_of(kept, a);
+  char* sys = kept ? k.sys : s.sys;
+  if (int rc = systems(a, sys, st)) return rc;
+  DrWalk w = walk_of(a, p, s, sys);
   w.z = la_view(a.la.v, a.la, a.la.Dv);
   w.out = const_cast<void*>(out.p);
   w.o_sb = out.sb;
   w.o_st = a.la.T > 1 ? out.st : a.la.Dv;
   w.o_sh = out.sh;
   if (kept) {
-    const Kept k = kept_of(kept, a);
     w.e = k.e;
     w.keep = k.before;
   }
@@ -239,10 +242,9 @@ int backward(const Problem& a, const prnn_la_view& go, const float* gs, const vo
              void* dv, void* dg, void* db, float* dh0, void* ws, hipStream_t st) {
   const bool per_head = a.la.g_sb == 0 && a.la.g_st == 0;
   const Plan p = plan(a);
-  const Scratch s = carve(ws, a, p, true, dg != nullptr);
+  const Scratch s = carve(ws, a, p, false, true, dg != nullptr);
   const Kept k = kept_of(const_cast<void*>(kept), a);
-  if (int rc = systems(a, s, true, st)) return rc;
-  DrWalk w = walk_of(a, p, s);
+  DrWalk w = walk_of(a, p, s, k.sys);
   w.z = la_view(go, a.la, a.la.Dv);
   w.keep = s.behind;
   w.dv = s.dv ? s.dv : dv;
@@ -257,7 +259,7 @@ int backward(const Problem& a, const prnn_la_view& go, const float* gs, const vo
   g.go = w.z;
   g.g = decay_of(a);
   g.b = rate_of(a);
-  g.sys = s.sys;
+  g.sys = k.sys;
   g.e = k.e;
   g.dv = w.dv;
   g.before = k.before;
@@ -305,9 +307,9 @@ int backward(const Problem& a, const prnn_la_view& go, const float* gs, const vo
 
 using namespace prnn;
 
-extern "C" PRNN_API size_t prnn_delta_rule_workspace_size(const prnn_delta_rule_problem* a) {
+extern "C" PRNN_API size_t prnn_delta_rule_workspace_size(const prnn_delta_rule_problem* a, int kept) {
   if (check(a)) return 0;
-  return need(*a, false, false);
+  return need(*a, kept == 0, false, false);
 }
 
 extern "C" PRNN_API size_t prnn_delta_rule_kept_size(const prnn_delta_rule_problem* a) {
@@ -326,14 +328,14 @@ extern "C" PRNN_API int prnn_delta_rule(const prnn_delta_rule_problem* a, const 
   if (sequences(*a) == 0) return PRNN_OK;
   if (kept && (reinterpret_cast<uintptr_t>(kept) & 255))
     return fail(PRNN_ERR_VALUE, "what is kept must lie on a 256-byte boundary");
-  if (int rc = check_ws("workspace", need(*a, false, false), workspace, bytes)) return rc;
+  if (int rc = check_ws("workspace", need(*a, kept == nullptr, false, false), workspace, bytes)) return rc;
   return forward(*a, *out, state_out, out_table, out_rows, kept, workspace, static_cast<hipStream_t>(stream));
 }
 
 extern "C" PRNN_API size_t prnn_delta_rule_backward_workspace_size(const prnn_delta_rule_problem* a,
                                                                    int decay_grad) {
   if (check(a)) return 0;
-  return need(*a, true, decay_grad != 0);
+  return need(*a, false, true, decay_grad != 0);
 }
 
 extern "C" PRNN_API int prnn_delta_rule_backward(const prnn_delta_rule_problem* a, const prnn_la_view* go,
@@ -353,6 +355,6 @@ extern "C" PRNN_API int prnn_delta_rule_backward(const prnn_delta_rule_problem* 
   if (a->la.h0 && a->la.h0_rows < sequences(*a))
     return fail(PRNN_ERR_VALUE, "h0 has %d rows for %d sequences", a->la.h0_rows, sequences(*a));
   if (sequences(*a) == 0) return PRNN_OK;
-  if (int rc = check_ws("workspace", need(*a, true, dg != nullptr), workspace, bytes)) return rc;
+  if (int rc = check_ws("workspace", need(*a, false, true, dg != nullptr), workspace, bytes)) return rc;
   return backward(*a, *go, gs, kept, dq, dk, dv, dg, db, dh0, workspace, static_cast<hipStream_t>(stream));
 }

@@ -54,7 +54,7 @@ __global__ __launch_bounds__(256) void dr_systems_kernel(DrSystems A) {
   }
   char* sys = A.sys + (static_cast<size_t>(id) * A.H + h) * kDrSys;
   float* weights = reinterpret_cast<float*>(sys + 2 * kDrTiles);
-  // ---- products: registers earlier tokens j, lanes later ones i (transposed pairs the other way)
+  // ---- products: registers earlier tokens j, lanes later ones i
   if (tid == 0) s_stop = kDrC;
   f16v N, P;
 #pragma unroll
@@ -95,10 +95,7 @@ __global__ __launch_bounds__(256) void dr_systems_kernel(DrSystems A) {
         const auto k0 = row_op<M, 2>(sK + tj * RB, f, half), k1 = row_op<M, 2>(sK + ti * RB, f, half);
         const auto q1 = row_op<M, 2>(sQ + ti * RB, f, half);
         mul<32>(N, k0, k1);
-        if (A.transposed)
-          mul<32>(P, q1, k0);
-        else
-          mul<32>(P, k0, q1);
+        mul<32>(P, k0, q1);
         float x[8];
         values(k1, x);
 #pragma unroll
@@ -116,26 +113,19 @@ __global__ __launch_bounds__(256) void dr_systems_kernel(DrSystems A) {
   // ---- weights; the system's matrix without what is not finite
   if (wave < 3) {
     char* pairs = sys + kDrTiles + wave * (kDrTiles / 3 / M::kParts);
-    const float Hi = s_hi[ti], Lo = s_lo[ti], Bi = s_b[ti];
-    const float Hj = s_hi[tj], Lj = s_lo[tj];
+    const float Hi = s_hi[ti], Lo = s_lo[ti];
     float pair[16];
     auto four = [](const float* v) { return *reinterpret_cast<const f4*>(v); };
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const int j = 32 * jt + 8 * q + 4 * half, i = 32 * it + 8 * q + 4 * half;
+      const int j = 32 * jt + 8 * q + 4 * half;
       const f4 hj = four(s_hi + j), lj = four(s_lo + j), bj = four(s_b + j);
       f4 m, p;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const float w = fexp((Hi - hj[r]) + (Lo - lj[r]));
-        m[r] = ((j + r < ti) & (ti < stop)) ? N[4 * q + r] * w * (A.transposed ? Bi : bj[r]) : 0.0f;
+        m[r] = ((j + r < ti) & (ti < stop)) ? N[4 * q + r] * w * bj[r] : 0.0f;
         p[r] = j + r <= ti ? P[4 * q + r] * w * A.scale : 0.0f;
-      }
-      if (A.transposed) {  // lane: token j, registers: tokens i
-        const f4 hi = four(s_hi + i), li = four(s_lo + i);
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          p[r] = tj <= i + r ? P[4 * q + r] * fexp((hi[r] - Hj) + (li[r] - Lj)) * A.scale : 0.0f;
       }
       *reinterpret_cast<f4*>(&sM[ti * kLd + j]) = m;
 #pragma unroll
@@ -230,25 +220,16 @@ __global__ __launch_bounds__(256) void dr_systems_kernel(DrSystems A) {
   // ---- the strictly triangular part of the inverse
   if (wave < 3) {
   char* tiles = sys + wave * (kDrTiles / 3 / M::kParts);
-  const int row = (A.transposed ? 32 * jt : 32 * it) + l32, col0 = A.transposed ? 32 * it : 32 * jt;
+  const int row = 32 * it + l32, col0 = 32 * jt;
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
     f4 t[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const int col = col0 + 4 * (4 * half + 2 * m + k);
-      f4 w;
-      if (A.transposed) {
+      const f4 w = *reinterpret_cast<const f4*>(&sT[row * kLd + col]);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) w[r] = sT[(col + r) * kLd + row];
-      } else {
-        w = *reinterpret_cast<const f4*>(&sT[row * kLd + col]);
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float v = w[r];
-        t[k][r] = (A.transposed ? col + r > row : col + r < row) ? v : 0.0f;
-      }
+      for (int r = 0; r < 4; ++r) t[k][r] = col + r < row ? w[r] : 0.0f;
     }
     const int to = dr_unit_of<E>(l32, 4 * half + 2 * m);
     if constexpr (sizeof(E) == 2) {

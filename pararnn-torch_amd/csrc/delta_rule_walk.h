@@ -5,7 +5,7 @@
 // of a chunk's chain, with rows of K read from LDS along and across,
 //
 //   forwards   x = K S,   e = (1 + T)(v - exp(G) x),          S' = exp(G_last) S + K^T (..u)
-//   backwards  x = K R,   du = (1 + T)(P^T go + .. x),        R' = exp(G_last) R + Q^T (..go) - K^T (..dv)
+//   backwards  x = K R,   dv = (1 + T)^T b (P^T go + .. x),     R' = exp(G_last) R + Q^T (..go) - K^T (..dv)
 //
 // take what the one before left in registers, so a wave's chain meets no other wave: the two
 // barriers of a chunk only hand K, Q and the system through LDS.  The output is formed transposed
@@ -39,37 +39,61 @@ __device__ __forceinline__ void fill(char* tile, const char* p, long long st, in
 }
 struct NotStaged {};
 
-// Operand of a stored matrix (the system's inverse or the pairs): rows NC rt .. of the 64, step f of
-// the contraction over tokens.  UPPER: the transposed ones.
-template <class M, int NC, bool UPPER>
+// Operands of a stored matrix (the system's inverse or the pairs): rows NC rt .. of the 64, step f of
+// the contraction over tokens; BACK: of the transposed matrix, read down the stored rows.
+template <class M, int NC, bool BACK>
 struct Stored {
+  using E = typename M::E;
   static constexpr int G = 64 / NC;
+  static constexpr int ES = static_cast<int>(sizeof(E)), kRow = 32 * ES, kUnit = 4 * ES;
   static constexpr int kTile = kDrTiles / 3 / M::kParts;
   // whether there is anything in the 32 x 32 tile
   static constexpr bool any(int rt, int f) {
     const int a = NC * rt / 32, b = 8 * G * f / 32;
-    return UPPER ? b >= a : b <= a;
+    return BACK ? b >= a : b <= a;
+  }
+  static __device__ __forceinline__ const char* at(const char* tile, int row, int col) {
+    return tile + row * kRow + dr_unit_of<E>(row, col >> 2) * kUnit + (col & 3) * ES;
   }
   static __device__ __forceinline__ Op<M, M::kParts> get(const char* m, int rt, int f, int n, int g) {
-    using E = typename M::E;
-    const int a = NC * rt / 32, b = 8 * G * f / 32;
-    const int row = (NC * rt + n) & 31, c = (8 * G * f & 31) + 4 * g;
-    const char* t = m + (a + b) * kTile + row * 32 * static_cast<int>(sizeof(E));
-    const int u0 = dr_unit_of<E>(row, c / 4), u1 = dr_unit_of<E>(row, c / 4 + G);
+    const char* t = m + (NC * rt / 32 + 8 * G * f / 32) * kTile;
+    const int own = (NC * rt) & 31, other = (8 * G * f) & 31;
     Op<M, M::kParts> o;
-    if constexpr (sizeof(E) == 2) {
+    if constexpr (ES == 2) {
+      const char *x, *y;
+      if constexpr (BACK) {
+        const int lane = threadIdx.x & 63, i = lane & 15, gg = lane >> 4;
+        const int row = other + (G == 2 ? 4 * (gg >> 1) : 4 * gg) + (i >> 2);
+        const int col = own + (G == 2 ? 16 * (gg & 1) : 0) + 4 * (i & 3);
+        x = at(t, row, col);
+        y = at(t, row + 4 * G, col);
+      } else {
+        x = at(t, own + n, other + 4 * g);
+        y = at(t, own + n, other + 4 * G + 4 * g);
+      }
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         union {
           u2 h[2];
+          s4 s[2];
           b8 v;
-        } x;
-        x.h[0] = *reinterpret_cast<const u2*>(t + p * 3 * kTile + u0 * 8);
-        x.h[1] = *reinterpret_cast<const u2*>(t + p * 3 * kTile + u1 * 8);
-        o.p[p] = x.v;
+        } r;
+        if constexpr (BACK) {
+          r.s[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(x + p * 3 * kTile));
+          r.s[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(y + p * 3 * kTile));
+        } else {
+          r.h[0] = *reinterpret_cast<const u2*>(x + p * 3 * kTile);
+          r.h[1] = *reinterpret_cast<const u2*>(y + p * 3 * kTile);
+        }
+        o.p[p] = r.v;
       }
+    } else if constexpr (BACK) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        o.x[i] = *reinterpret_cast<const float*>(at(t, other + 4 * G * (i >> 2) + 4 * g + (i & 3), own + n));
     } else {
-      const f4 x = *reinterpret_cast<const f4*>(t + u0 * 16), y = *reinterpret_cast<const f4*>(t + u1 * 16);
+      const f4 x = *reinterpret_cast<const f4*>(at(t, own + n, other + 4 * g));
+      const f4 y = *reinterpret_cast<const f4*>(at(t, own + n, other + 4 * G + 4 * g));
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         o.x[i] = x[i];
@@ -300,7 +324,7 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
                                   dr_operand_at(A.Dv, i, col) * ES), S[t][r]);
         }
     }
-    const char* sS = kSysLds ? s_sys : A.sys + (static_cast<size_t>(row0 + c) * A.H + h) * kDrSys;
+    const char* const sS = kSysLds ? s_sys : A.sys + (static_cast<size_t>(row0 + c) * A.H + h) * kDrSys;
     __syncthreads();
     if (step + 1 < chunks) fetch(kBack ? c - 1 : c + 1);
 
@@ -359,10 +383,10 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
       }
 #pragma unroll
       for (int i = 0; i < NC; i += 4) {
-        const f4 w = weight(kWr, i);
+        const f4 w = weight(kWr, i), b = weight(kWb, i);
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          y[i + r] = fmaf(w[r], X[(i + r) / RT][(i + r) % RT], Y[(i + r) / RT][(i + r) % RT]);
+          y[i + r] = b[r] * fmaf(w[r], X[(i + r) / RT][(i + r) % RT], Y[(i + r) / RT][(i + r) % RT]);
       }
     }
 
@@ -408,10 +432,10 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
         if (Mat::any(t, f)) mul<NC>(Y[t], Mat::get(sS, t, f, nn, g), yo[f]);
     }
 
-    float u[NC];  // what is written: b e forwards, b du = dv backwards
+    float u[NC];  // what is written: b e forwards, dv backwards
 #pragma unroll
     for (int i = 0; i < NC; i += 4) {
-      const f4 b = weight(kWb, i);
+      const f4 b = kBack ? f4{1.0f, 1.0f, 1.0f, 1.0f} : weight(kWb, i);
 #pragma unroll
       for (int r = 0; r < 4; ++r) u[i + r] = b[r] * Y[(i + r) / RT][(i + r) % RT];
     }

@@ -163,7 +163,7 @@ SIGNATURES: dict[str, tuple] = {
     "prnn_linear_attention_step": (
         _I, [_P, _L, _L, _I, _P, _L, _L, _I, _P, _L, _L, _I, _P, _L, _L, _I, _P, _P, _I, _P,
              _I, _I, _I, _I, _F, _I, _P]),
-    "prnn_delta_rule_workspace_size": (_S, [_DRP]),
+    "prnn_delta_rule_workspace_size": (_S, [_DRP, _I]),
     "prnn_delta_rule_kept_size": (_S, [_DRP]),
     "prnn_delta_rule": (_I, [_DRP, _LAV, _P, _P, _I, _P, _P, _S, _P]),
     "prnn_delta_rule_backward_workspace_size": (_S, [_DRP, _I]),

@@ -89,7 +89,7 @@ def _forward(p: _DeltaProblem, state_out: Tensor | None, table: Tensor | None,
     lib, dev, c = _lib.load(), p.q.device, ctypes.byref(p.c)
     out = p.q.new_empty(batch, time, heads, dv)
     keep = _workspace(lib.prnn_delta_rule_kept_size(c), dev) if kept else None
-    need = lib.prnn_delta_rule_workspace_size(c)
+    need = lib.prnn_delta_rule_workspace_size(c, int(kept))
     ws = _workspace(need, dev) if need else None
     rc = _enqueue(lib.prnn_delta_rule, dev, c, ctypes.byref(_view(out)), _at(state_out), _at(table),
                   0 if state_out is None else state_out.shape[0], _at(keep), _at(ws), need)
