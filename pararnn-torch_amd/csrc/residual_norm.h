@@ -13,6 +13,8 @@
 // once, the statistics are two-pass and the backward pass forms them again from x, y and the gate.
 #pragma once
 
+#include <algorithm>
+
 #include "prnn_host.h"
 
 namespace prnn {
@@ -41,13 +43,14 @@ inline int rn_threads(int C) {
   while (nt < 512 && nt * 8 < C) nt *= 2;
   return C <= 8192 ? nt : 1024;
 }
-// Workgroups of the backward pass: one's sums over its rows are written and read once more, so not
-// more than keep the chip busy.
-inline int rn_groups(int N, int C) {
+// Workgroups of the backward pass: as many as run at a time, 12 waves a CU of 16-byte accesses, 8 of
+// single elements (16384 x 1024 in bf16: 61 us, with 8 waves 69; a workgroup's sums over its rows are
+// written and read once more).
+inline int rn_groups(int N, int C, bool vec) {
   const int rows = rn_threads(C) >= 256 ? 1 : 256 / rn_threads(C);
-  const int groups = (N + rows - 1) / rows;
-  const int most = rn_threads(C) > 256 ? 256 * 1024 / rn_threads(C) : 1024;
-  return groups < most ? groups : most;
+  const long long groups = (static_cast<long long>(N) + rows - 1) / rows;
+  const int most = (vec ? 768 : 512) * 256 / std::max(256, rn_threads(C));
+  return static_cast<int>(std::min<long long>(groups, most));
 }
 
 template <typename T, int V, int E, int NT>
@@ -55,31 +58,38 @@ struct RnRow {
   static constexpr int K = E / V;
   int C, lane;
   __device__ __forceinline__ int col(int i) const { return ((i / V) * NT + lane) * V + i % V; }
-  // Rows through buffers of their own bytes: columns behind the width are read as zero, not written.
-  __device__ __forceinline__ void load(float* v, const void* p, long long row) const {
-    if (p == nullptr) {
+  // A row on its way: 16-byte units, or elements one by one.  Zeros behind the width and where there is
+  // no array.
+  static constexpr int U = V == 1 ? E : E * static_cast<int>(sizeof(T)) / 4;
+  struct Raw {
+    uint32_t w[U];
+  };
+  __device__ __forceinline__ Raw fetch(const void* p, long long row) const {
+    Raw r;
+    const rsrc_t b = make_rsrc(p ? static_cast<const T*>(p) + row * C : nullptr, p ? C * static_cast<uint32_t>(sizeof(T)) : 0u);
+    if constexpr (V == 1) {
 #pragma unroll
-      for (int i = 0; i < E; ++i) v[i] = 0.0f;
-      return;
-    }
-    const T* at = static_cast<const T*>(p) + row * C;
+      for (int k = 0; k < K; ++k) r.w[k] = ldb_bits(static_cast<T*>(nullptr), b, (k * NT + lane) * sizeof(T), 0);
+    } else {
+      typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int c = (k * NT + lane) * V;
-      if constexpr (V == 1) {
-        v[k] = c < C ? to_f32(at[c]) : 0.0f;
-      } else {
-        typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-        u4 w{0, 0, 0, 0};
-        if (c < C) w = *reinterpret_cast<const u4*>(at + c);
+      for (int k = 0; k < K; ++k) {
+        const u4 w = __builtin_amdgcn_raw_buffer_load_b128(b, (k * NT + lane) * 16, 0, 0);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          if constexpr (sizeof(T) == 4)
-            v[k * V + i] = __uint_as_float(w[i]);
-          else
-            v[k * V + i] = i & 1 ? Narrow<T>::hi(w[i / 2]) : Narrow<T>::lo(w[i / 2]);
-        }
+        for (int i = 0; i < 4; ++i) r.w[4 * k + i] = w[i];
       }
+    }
+    return r;
+  }
+  __device__ __forceinline__ void values(const Raw& r, float* v) const {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      if constexpr (V == 1)
+        v[i] = bits_to_f32(static_cast<T*>(nullptr), r.w[i]);
+      else if constexpr (sizeof(T) == 4)
+        v[i] = __uint_as_float(r.w[i]);
+      else
+        v[i] = i & 1 ? Narrow<T>::hi(r.w[i / 2]) : Narrow<T>::lo(r.w[i / 2]);
     }
   }
   __device__ __forceinline__ void store(void* p, long long row, const float* v) const {
@@ -116,15 +126,27 @@ struct RnRow {
   }
 };
 
+// Sum over the wave, in all lanes: rows of 16 by shifts, the rows' last lanes handed on.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float rn_add(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ float rn_wave_sum(float v) {
+  v = rn_add<0x111, 0xf>(v);
+  v = rn_add<0x112, 0xf>(v);
+  v = rn_add<0x114, 0xf>(v);
+  v = rn_add<0x118, 0xf>(v);
+  v = rn_add<0x142, 0xa>(v);
+  v = rn_add<0x143, 0xc>(v);
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
+}
+
 // Sums of two values over the NT threads of a row, in all of them; `turn` alternates the LDS places,
 // so one barrier a sum is enough.
 template <int NT>
 __device__ __forceinline__ void rn_sum(float& a, float& b, float* lds, int& turn) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    a += __shfl_xor(a, m);
-    b += __shfl_xor(b, m);
-  }
+  a = rn_wave_sum(a);
+  b = rn_wave_sum(b);
   if constexpr (NT > 64) {
     constexpr int W = NT / 64;
     const int wave = threadIdx.x >> 6, first = wave / W * W;

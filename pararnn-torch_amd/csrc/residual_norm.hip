@@ -21,15 +21,26 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rn_forward_kernel(RnArgs 
   row.param(p, A.pw, A.w_dtype, 1.0f);
   row.param(s, A.scale, A.w_dtype, A.number);
   const int step = static_cast<int>(gridDim.x) * R;
-  for (int base = blockIdx.x * R; base < A.N; base += step) {
-    const int mine = base + static_cast<int>(threadIdx.x) / NT;
-    const bool there = mine < A.N;
-    const long long at = there ? mine : A.N - 1;  // the last row again: the sums meet in barriers
+  constexpr bool kAhead = E == 8;  // registers for the row behind this one
+  auto place = [&](long long base) { return min(base + static_cast<int>(threadIdx.x) / NT, A.N - 1ll); };
+  typename Row::Raw rx, ry, rg;  // the next row's are under way
+  auto fetch = [&](long long base) {
+    const long long at = place(base);  // behind the last row that one again: the sums meet in barriers
+    rx = row.fetch(A.x, at);
+    ry = row.fetch(A.y, at);
+    rg = row.fetch(A.gate, at);
+  };
+  if (kAhead) fetch(blockIdx.x * R);
+  for (long long base = blockIdx.x * R; base < A.N; base += step) {
+    if (!kAhead) fetch(base);
+    const long long at = place(base);
+    const bool there = base + static_cast<int>(threadIdx.x) / NT < A.N;
     float h[E], f[E], g[E];
-    row.load(h, A.x, at);
+    row.values(rx, h);
+    row.values(ry, f);
+    row.values(rg, g);
+    if (kAhead) fetch(base + step);
     if (A.y) {
-      row.load(f, A.y, at);
-      if (A.gate) row.load(g, A.gate, at);
       if (A.post) {
         rn_norm<Row, E, NT>(row, f, A.layer, A.eps, lds, turn);
 #pragma unroll
@@ -87,7 +98,7 @@ __global__ __launch_bounds__(1024) void rn_sum_kernel(RnSums A) {
 template <typename T, int V, int E, int NT>
 int launch(const RnArgs& a, hipStream_t stream) {
   constexpr int R = NT < 256 ? 256 / NT : 1, block = NT < 256 ? 256 : NT;
-  const int groups = std::min((a.N + R - 1) / R, 256 * (2048 / block));
+  const int groups = static_cast<int>(std::min((a.N + R - 1ll) / R, 256ll * (2048 / block)));
   rn_forward_kernel<T, V, E, NT><<<groups, block, 0, stream>>>(a);
   PRNN_HIP(hipGetLastError());
   return PRNN_OK;
@@ -103,7 +114,7 @@ int launch_row(const RnArgs& a, hipStream_t stream) {
   return launch<T, V, 16, 1024>(a, stream);
 }
 
-size_t parts_bytes(int N, int C) { return sizeof(float) * 4 * static_cast<size_t>(rn_groups(N, C)) * C; }
+size_t parts_bytes(int N, int C) { return sizeof(float) * 4 * static_cast<size_t>(rn_groups(N, C, true)) * C; }
 
 int check(int N, int C, float eps, int act, int w_dtype, int dtype) {
   if (int rc = check_dtype(dtype)) return rc;
@@ -203,10 +214,10 @@ extern "C" PRNN_API int prnn_residual_norm_backward(
   a.number = scale_number;
   a.eps = eps;
   a.want = (dw ? 1 : 0) | (db ? 2 : 0) | (dpw ? 4 : 0) | (dscale ? 8 : 0);
-  const int groups = rn_groups(N, C);
+  const bool vec = vectors(C, dtype, {gh, gz, x, y, gate, dx, dy, dgate});
+  const int groups = rn_groups(N, C, vec);
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  if (int rc = rn_backward(a, dtype, vectors(C, dtype, {gh, gz, x, y, gate, dx, dy, dgate}), groups, st))
-    return rc;
+  if (int rc = rn_backward(a, dtype, vec, groups, st)) return rc;
   if (!sums) return PRNN_OK;
   return with_storage(dtype, [&](auto t) {
     const RnSums s{a.parts, {dw, db, dpw, dscale}, groups, C, w_dtype, dtype};

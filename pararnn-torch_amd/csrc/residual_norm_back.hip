@@ -9,7 +9,7 @@ namespace prnn {
 namespace {
 
 template <typename T, int V, int E, int NT>
-__global__ __launch_bounds__(NT < 256 ? 256 : NT) void rn_backward_kernel(RnArgs A) {
+__global__ __launch_bounds__(NT < 256 ? 256 : NT, E == 8 && V > 1 && NT <= 256 ? 3 : 1) void rn_backward_kernel(RnArgs A) {
   constexpr int R = NT < 256 ? 256 / NT : 1, block = NT < 256 ? 256 : NT;
   __shared__ float lds[64];
   __shared__ float s_sum[R > 1 ? E * block : 1];
@@ -26,23 +26,36 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rn_backward_kernel(RnArgs
 #pragma unroll
     for (int i = 0; i < E; ++i) sums[k][i] = 0.0f;
   const int step = static_cast<int>(gridDim.x) * R;
-  for (int base = blockIdx.x * R; base < A.N; base += step) {
-    const int mine = base + static_cast<int>(threadIdx.x) / NT;
-    const bool there = mine < A.N;
-    const long long at = there ? mine : A.N - 1;
+  constexpr bool kAhead = E == 8;  // registers for the row behind this one
+  auto place = [&](long long base) { return min(base + static_cast<int>(threadIdx.x) / NT, A.N - 1ll); };
+  typename Row::Raw rx, ry, rg, rz, rh;  // the next row's are under way
+  auto fetch = [&](long long base) {
+    const long long at = place(base);
+    rx = row.fetch(A.x, at);
+    rz = row.fetch(A.gz, at);
+    rh = row.fetch(A.gh, at);
+    ry = row.fetch(A.y, at);
+    rg = row.fetch(A.gate, at);
+  };
+  if (kAhead) fetch(blockIdx.x * R);
+  for (long long base = blockIdx.x * R; base < A.N; base += step) {
+    if (!kAhead) fetch(base);
+    const long long at = place(base);
+    const bool there = base + static_cast<int>(threadIdx.x) / NT < A.N;
     float h[E], n1[E], a[E], d[E], gz[E], dh[E];
-    row.load(h, A.x, at);
-    row.load(gz, A.gz, at);
-    row.load(dh, A.gh, at);
+    row.values(rx, h);
+    row.values(rz, gz);
+    row.values(rh, dh);
+    row.values(ry, n1);
+    row.values(rg, d);
+    if (kAhead) fetch(base + step);
     if (!there) {  // another one's row: nothing to the sums
 #pragma unroll
       for (int i = 0; i < E; ++i) gz[i] = dh[i] = 0.0f;
     }
     float r1 = 1.0f;
     if (A.y) {
-      row.load(n1, A.y, at);
       if (A.gate) {
-        row.load(d, A.gate, at);
 #pragma unroll
         for (int i = 0; i < E; ++i) rn_act(d[i], A.act, a[i], d[i]);
       } else {
