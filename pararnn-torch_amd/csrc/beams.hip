@@ -11,7 +11,8 @@
 //
 // The M best of some thousand values: the M-th largest of the threads' own largest is a bound that at
 // least M values reach, and only values of those M threads can; what reaches it (a few more than M of
-// ordinary logits) is ranked by counting, so the order of arrival does not matter.
+// ordinary logits) is ranked by counting, so the order of arrival does not matter.  Up to 32 best the
+// bound is the largest of the four waves' own, found by a quarter of the comparisons.
 #include <algorithm>
 
 #include "prnn_host.h"
@@ -22,7 +23,8 @@ namespace {
 constexpr int kMost = 128;     // candidates that are wanted
 constexpr int kEach = 32;      // tokens of a thread
 constexpr int kSlice = 256 * kEach;
-constexpr int kRound = 16;     // candidates of a thread and round of the second launch
+constexpr int kFew = 32;       // up to which a bound is a wave's
+constexpr int kRound = 4;     // candidates of a thread and round of the second launch
 
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
@@ -59,14 +61,15 @@ struct BeamArgs {
   int B, K, V, M, S, pad;
 };
 
-template <typename T>
+// MOST: candidates that are wanted at most.
+template <typename T, int MOST>
 __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs A) {
   constexpr int V = 16 / sizeof(T);
   __shared__ __align__(16) uint64_t s_top[256];
-  __shared__ uint64_t s_list[kMost * kEach];
+  __shared__ uint64_t s_list[(MOST <= kFew ? 4 : 1) * MOST * kEach];
   __shared__ double s_sum[4];
   __shared__ float s_most[4];
-  __shared__ uint64_t s_bound;
+  __shared__ uint64_t s_bound[4];
   __shared__ int s_count;
   const int tid = threadIdx.x, slice = blockIdx.x % A.S, row = blockIdx.x / A.S;
   const int b = row / A.K, k = row - b * A.K;
@@ -95,28 +98,25 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs A) {
     }
   }
   float most = -INFINITY;
-  uint64_t top = 0;
-  auto key = [&](int i) {
-    const int t = slice * kSlice + ((i / V) * 256 + tid) * V - skip + i % V;
-    const uint32_t o = order(v[i]);
-    return o ? static_cast<uint64_t>(o) << 32 | static_cast<uint32_t>(~t) : 0ull;
-  };
+  auto token = [&](int i) { return slice * kSlice + ((i / V) * 256 + tid) * V - skip + i % V; };
+  uint32_t first = 0;  // order and place of this thread's largest, the lowest token of equals
+  int place = 0;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     broken |= !(v[i] < INFINITY);  // NaN or infinity
     most = fmaxf(most, v[i]);
-    const uint64_t o = key(i);
-    top = o > top ? o : top;
+    const uint32_t o = order(v[i]);
+    place = o > first ? token(i) : place;
+    first = o > first ? o : first;
   }
+  const uint64_t top = first ? static_cast<uint64_t>(first) << 32 | static_cast<uint32_t>(~place) : 0ull;
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) most = fmaxf(most, __shfl_xor(most, m));
   if (__any(broken)) most = INFINITY;
   s_top[tid] = top;
   if ((tid & 63) == 0) s_most[tid >> 6] = most;
-  if (tid == 0) {
-    s_bound = 1;
-    s_count = 0;
-  }
+  if (tid < 4) s_bound[tid] = 1;
+  if (tid == 0) s_count = 0;
   __syncthreads();
   most = fmaxf(fmaxf(s_most[0], s_most[1]), fmaxf(s_most[2], s_most[3]));
   const bool none = most == -INFINITY, bad = most == INFINITY;
@@ -132,20 +132,26 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs A) {
   // this thread's place among the threads' largest
   int above = 0;
   if (top) {
+    constexpr int kAmong = MOST <= kFew ? 64 : 256;
+    const int first = MOST <= kFew ? tid & ~63 : 0;
 #pragma unroll 8
-    for (int i = 0; i < 256; i += 2) {
-      const ulong2 o = *reinterpret_cast<const ulong2*>(&s_top[i]);
+    for (int i = 0; i < kAmong; i += 2) {
+      const ulong2 o = *reinterpret_cast<const ulong2*>(&s_top[first + i]);
       above += (o.x > top) + (o.y > top);
     }
-    if (above == A.M - 1) s_bound = top;
+    if (above == A.M - 1) s_bound[first >> 6] = top;
   }
   __syncthreads();
-  const uint64_t bound = s_bound;
+  uint64_t bound = s_bound[0];
+#pragma unroll
+  for (int w = 1; w < 4; ++w) bound = s_bound[w] > bound ? s_bound[w] : bound;
   if (top >= bound) {
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const uint64_t o = key(i);
-      if (o >= bound) s_list[atomicAdd(&s_count, 1)] = o;
+      const uint32_t o = order(v[i]);
+      if (o < static_cast<uint32_t>(bound >> 32) || o == 0) continue;
+      const uint64_t key = static_cast<uint64_t>(o) << 32 | static_cast<uint32_t>(~token(i));
+      if (key >= bound) s_list[atomicAdd(&s_count, 1)] = key;
     }
   }
   __syncthreads();
@@ -162,120 +168,106 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs A) {
     A.slices[at] = Slice{(s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]), bad ? NAN : most, min(n, A.M)};
 }
 
-__device__ __forceinline__ bool before(uint64_t a, uint32_t ta, uint64_t b, uint32_t tb) {
-  return a > b || (a == b && ta < tb);
+// A candidate of the second launch: the order of its total, its place k V + t.
+struct __align__(16) Total {
+  uint64_t o;
+  uint32_t t, none;
+};
+__device__ __forceinline__ bool before(const Total& a, const Total& b) {
+  return a.o > b.o || (a.o == b.o && a.t < b.t);
 }
 
 __global__ __launch_bounds__(256) void beam_choose_kernel(BeamArgs A) {
-  __shared__ uint64_t s_top[256], s_list[kMost * kRound + kMost];
-  __shared__ uint32_t s_topt[256], s_listt[kMost * kRound + kMost];
-  __shared__ uint64_t s_carry[kMost];
-  __shared__ uint32_t s_carryt[kMost];
-  __shared__ uint64_t s_bound;
-  __shared__ uint32_t s_boundt;
+  __shared__ Total s_top[256], s_list[kMost * kRound + kMost], s_carry[kMost], s_bound[4];
   __shared__ int s_count, s_held;
   __shared__ double s_off[kMost], s_most[kMost];  // a total is (logit - most) + off
-  const int tid = threadIdx.x, b = blockIdx.x;
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, b = blockIdx.x;
   const int per = A.S * A.M;  // candidates of a beam
+  const bool few = A.M <= kFew;
   if (tid == 0) s_held = 0;
-  // score - log(sum), beams in blocks of kMost; the largest logit stays apart (masks of the type's lowest
-  // value would swallow the logarithm)
+  // score - log(sum), beams in blocks of kMost, a beam a wave; the largest logit stays apart (masks of
+  // the type's lowest value would swallow the logarithm)
   for (int k0 = 0; k0 < A.K; k0 += kMost) {
     __syncthreads();
-    for (int k = k0 + tid; k < min(A.K, k0 + kMost); k += 256) {
+    for (int k = k0 + wave; k < min(A.K, k0 + kMost); k += 4) {
       const int row = b * A.K + k;
-      const double score = A.scores[row];
-      double off = score, most = -static_cast<double>(INFINITY);
+      double off = A.scores[row], most = -static_cast<double>(INFINITY);
       if (!(A.ended && A.ended[row])) {
-        double sum = 0.0;
+        const Slice* x = A.slices + static_cast<size_t>(row) * A.S;
+        float top = -INFINITY;
         bool bad = false;
-        for (int s = 0; s < A.S; ++s) {
-          const float m = A.slices[static_cast<size_t>(row) * A.S + s].most;
-          bad |= m != m;
-          most = fmax(most, static_cast<double>(m));
+        double sum = 0.0;
+        for (int s = lane; s < A.S; s += 64) {
+          bad |= x[s].most != x[s].most;
+          top = fmaxf(top, x[s].most);
         }
-        for (int s = 0; s < A.S; ++s) {
-          const Slice x = A.slices[static_cast<size_t>(row) * A.S + s];
-          if (x.sum > 0.0) sum += x.sum * exp(static_cast<double>(x.most) - most);
-        }
-        off = bad ? -static_cast<double>(INFINITY) : score - log(sum);
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
+        for (int s = lane; s < A.S; s += 64)
+          if (x[s].sum > 0.0) sum += x[s].sum * exp(static_cast<double>(x[s].most) - top);
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m);
+        most = top;
+        off = __any(bad) ? -static_cast<double>(INFINITY) : off - log(sum);
       }
-      s_off[k - k0] = off;
-      s_most[k - k0] = most;
+      if (lane == 0) {
+        s_off[k - k0] = off;
+        s_most[k - k0] = most;
+      }
     }
     __syncthreads();
     const long long end = static_cast<long long>(min(A.K, k0 + kMost)) * per;
     for (long long base = static_cast<long long>(k0) * per; base < end; base += 256 * kRound) {
-      uint64_t o[kRound], top = 0;
-      uint32_t t[kRound], topt = ~0u;
+      Total c[kRound], top{0, ~0u, 0};
 #pragma unroll
       for (int i = 0; i < kRound; ++i) {
-        const long long c = base + i * 256 + tid;
-        o[i] = 0;
-        t[i] = ~0u;
-        if (c >= end) continue;
-        const int k = static_cast<int>(c / per), in = static_cast<int>(c - static_cast<long long>(k) * per);
+        const long long at = base + i * 256 + tid;
+        c[i] = Total{0, ~0u, 0};
+        if (at >= end) continue;
+        const int k = static_cast<int>(at / per), in = static_cast<int>(at - static_cast<long long>(k) * per);
         const int row = b * A.K + k;
         if (A.ended && A.ended[row]) {  // goes on as it is, with one token
-          if (in == 0) {
-            o[i] = order(s_off[k - k0]);
-            t[i] = static_cast<uint32_t>(k) * A.V + A.pad;
-          }
+          if (in == 0) c[i] = Total{order(s_off[k - k0]), static_cast<uint32_t>(k) * A.V + A.pad, 0};
         } else {
           const int s = in / A.M, r = in - s * A.M;
-          const size_t at = static_cast<size_t>(row) * A.S + s;
-          if (r < A.slices[at].count) {
-            const uint2 c2 = A.best[at * A.M + r];
-            const float logit = __uint_as_float(c2.x & 0x80000000u ? c2.x & 0x7fffffffu : ~c2.x);
-            o[i] = order((static_cast<double>(logit) - s_most[k - k0]) + s_off[k - k0]);
-            t[i] = static_cast<uint32_t>(k) * A.V + c2.y;
-          }
+          const size_t slice = static_cast<size_t>(row) * A.S + s;
+          const uint2 best = A.best[slice * A.M + r];
+          const float logit = __uint_as_float(best.x & 0x80000000u ? best.x & 0x7fffffffu : ~best.x);
+          if (r < A.slices[slice].count)
+            c[i] = Total{order((static_cast<double>(logit) - s_most[k - k0]) + s_off[k - k0]),
+                         static_cast<uint32_t>(k) * A.V + best.y, 0};
         }
-        if (o[i] && before(o[i], t[i], top, topt)) {
-          top = o[i];
-          topt = t[i];
-        }
+        if (c[i].o && before(c[i], top)) top = c[i];
       }
       s_top[tid] = top;
-      s_topt[tid] = topt;
-      if (tid == 0) {
-        s_bound = 1;
-        s_boundt = ~0u;
-      }
+      if (tid < 4) s_bound[tid] = Total{1, ~0u, 0};
       const int held = s_held;
-      for (int i = tid; i < held; i += 256) {
-        s_list[i] = s_carry[i];
-        s_listt[i] = s_carryt[i];
-      }
+      for (int i = tid; i < held; i += 256) s_list[i] = s_carry[i];
       if (tid == 0) s_count = held;
       __syncthreads();
-      if (top) {
+      // where candidates are few, all are ranked
+      if (end - base > 128 && top.o) {
+        const int first = few ? tid & ~63 : 0, among = few ? 64 : 256;
         int above = 0;
-        for (int i = 0; i < 256; ++i) above += before(s_top[i], s_topt[i], top, topt);
-        if (above == A.M - 1) {
-          s_bound = top;
-          s_boundt = topt;
-        }
+#pragma unroll 8
+        for (int i = 0; i < among; ++i) above += before(s_top[first + i], top);
+        if (above == A.M - 1) s_bound[first >> 6] = top;
       }
       __syncthreads();
-      const uint64_t bound = s_bound;
-      const uint32_t boundt = s_boundt;
+      Total bound = s_bound[0];
+#pragma unroll
+      for (int w = 1; w < 4; ++w) bound = before(s_bound[w], bound) ? s_bound[w] : bound;
 #pragma unroll
       for (int i = 0; i < kRound; ++i)
-        if (o[i] && !before(bound, boundt, o[i], t[i])) {
-          const int to = atomicAdd(&s_count, 1);
-          s_list[to] = o[i];
-          s_listt[to] = t[i];
-        }
+        if (c[i].o && !before(bound, c[i])) s_list[atomicAdd(&s_count, 1)] = c[i];
       __syncthreads();
       const int n = s_count;
       for (int i = tid; i < n; i += 256) {
+        const Total own = s_list[i];
         int rank = 0;
-        for (int j = 0; j < n; ++j) rank += before(s_list[j], s_listt[j], s_list[i], s_listt[i]);
-        if (rank < A.M) {
-          s_carry[rank] = s_list[i];
-          s_carryt[rank] = s_listt[i];
-        }
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) rank += before(s_list[j], own);
+        if (rank < A.M) s_carry[rank] = own;
       }
       if (tid == 0) s_held = min(n, A.M);
       __syncthreads();
@@ -286,9 +278,9 @@ __global__ __launch_bounds__(256) void beam_choose_kernel(BeamArgs A) {
   for (int i = tid; i < A.M; i += 256) {
     const bool any = i < held;
     const size_t at = static_cast<size_t>(b) * A.M + i;
-    A.out_scores[at] = any ? static_cast<float>(value(s_carry[i])) : -INFINITY;
-    A.out_parents[at] = any ? static_cast<int>(s_carryt[i] / A.V) : -1;
-    A.out_tokens[at] = any ? static_cast<int>(s_carryt[i] % A.V) : -1;
+    A.out_scores[at] = any ? static_cast<float>(value(s_carry[i].o)) : -INFINITY;
+    A.out_parents[at] = any ? static_cast<int>(s_carry[i].t / A.V) : -1;
+    A.out_tokens[at] = any ? static_cast<int>(s_carry[i].t % A.V) : -1;
   }
 }
 
@@ -347,7 +339,13 @@ extern "C" PRNN_API int prnn_beam_select(const void* logits, long long l_sb, lon
   const long long groups = static_cast<long long>(B) * K * a.S;
   if (int rc = check_grid("beam_select", groups, 256)) return rc;
   return with_storage(dtype, [&](auto z) {
-    beam_slice_kernel<decltype(z)><<<static_cast<unsigned>(groups), 256, 0, st>>>(a);
+    using T = decltype(z);
+    if (M <= 16)
+      beam_slice_kernel<T, 16><<<static_cast<unsigned>(groups), 256, 0, st>>>(a);
+    else if (M <= kFew)
+      beam_slice_kernel<T, kFew><<<static_cast<unsigned>(groups), 256, 0, st>>>(a);
+    else
+      beam_slice_kernel<T, kMost><<<static_cast<unsigned>(groups), 256, 0, st>>>(a);
     PRNN_HIP(hipGetLastError());
     beam_choose_kernel<<<B, 256, 0, st>>>(a);
     PRNN_HIP(hipGetLastError());

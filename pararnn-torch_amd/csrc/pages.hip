@@ -120,18 +120,17 @@ __device__ __forceinline__ void copy_part(const prnn_pool& pool, int src, int ds
   const char* s = static_cast<const char*>(pool.p) + src * pool.row_bytes + at;
   char* d = static_cast<char*>(pool.p) + dst * pool.row_bytes + at;
   if (((reinterpret_cast<uintptr_t>(pool.p) | pool.row_bytes) & 15) == 0) {
+    // buffers of what is left: behind it nothing is read or written, without a branch
+    typedef uint32_t u4 __attribute__((ext_vector_type(4)));
     constexpr int kEach = kPart / 16 / 256;
-    uint4 v[kEach];
+    const rsrc_t rs = make_rsrc(s, static_cast<uint32_t>(left)), rd = make_rsrc(d, static_cast<uint32_t>(left));
+    u4 v[kEach];
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int o = (i * 256 + threadIdx.x) * 16;
-      if (o < left) v[i] = *reinterpret_cast<const uint4*>(s + o);
-    }
+    for (int i = 0; i < kEach; ++i)
+      v[i] = __builtin_amdgcn_raw_buffer_load_b128(rs, (i * 256 + threadIdx.x) * 16, 0, 0);
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int o = (i * 256 + threadIdx.x) * 16;
-      if (o < left) *reinterpret_cast<uint4*>(d + o) = v[i];
-    }
+    for (int i = 0; i < kEach; ++i)
+      __builtin_amdgcn_raw_buffer_store_b128(v[i], rd, (i * 256 + threadIdx.x) * 16, 0, 0);
   } else if (((reinterpret_cast<uintptr_t>(pool.p) | pool.row_bytes) & 3) == 0) {
     for (int o = threadIdx.x * 4; o < left; o += 1024)
       *reinterpret_cast<uint32_t*>(d + o) = *reinterpret_cast<const uint32_t*>(s + o);
