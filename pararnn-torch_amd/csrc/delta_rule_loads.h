@@ -2,6 +2,7 @@
 #pragma once
 
 #include <type_traits>
+#include <utility>
 
 #include "delta_rule.h"
 #include "tiles.h"
@@ -25,22 +26,29 @@ struct Staged {
   static_assert(kDrC * U % NT == 0, "whole units");
   std::conditional_t<kNarrow, u4, uint32_t> r[N];
 
-  // `width` columns from c0; tokens [0, n) from `p` are there
+  // `width` columns from c0; tokens [0, n) from `p` are there: the others lie behind the buffer's end (a
+  // row is at most a stride wide, or they are told by a comparison).
   __device__ __forceinline__ void fetch(const char* p, long long st, int n, int c0, int width, int dtype) {
     const int tid = threadIdx.x;
-    const rsrc_t b = make_rsrc(p, 0x7fffffffu);
+    if constexpr (kNarrow) {
+      constexpr int D = NT / U;  // rows between a thread's loads
+      static_assert(NT % U == 0, "whole rows");
+      const int step = static_cast<int>(st) * 2, c = c0 + tid % U * 8;
+      const rsrc_t b = make_rsrc(p, n > 0 ? (n - 1) * step + width * 2 : 0);
+      const uint32_t at = la_in(c < width, tid / U * step + c * 2);
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const int e = tid + k * NT, row = e / U, c = e % U;
-      if constexpr (kNarrow) {
-        r[k] = __builtin_amdgcn_raw_buffer_load_b128(
-            b, la_in((row < n) & (c0 + c * 8 < width), row * static_cast<int>(st) * 2 + (c0 + c * 8) * 2), 0, 0);
-      } else if (dtype == PRNN_F32) {
-        r[k] = __builtin_amdgcn_raw_buffer_load_b32(
-            b, la_in((row < n) & (c0 + c < width), (row * static_cast<int>(st) + c0 + c) * 4), 0, 0);
-      } else {
-        r[k] = __builtin_amdgcn_raw_buffer_load_b16(
-            b, la_in((row < n) & (c0 + c < width), (row * static_cast<int>(st) + c0 + c) * 2), 0, 0);
+      for (int k = 0; k < N; ++k) r[k] = __builtin_amdgcn_raw_buffer_load_b128(b, at + k * D * step, 0, 0);
+    } else {
+      const rsrc_t b = make_rsrc(p, 0x7fffffffu);
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const int e = tid + k * NT, row = e / U, c = e % U;
+        if (dtype == PRNN_F32)
+          r[k] = __builtin_amdgcn_raw_buffer_load_b32(
+              b, la_in((row < n) & (c0 + c < width), (row * static_cast<int>(st) + c0 + c) * 4), 0, 0);
+        else
+          r[k] = __builtin_amdgcn_raw_buffer_load_b16(
+              b, la_in((row < n) & (c0 + c < width), (row * static_cast<int>(st) + c0 + c) * 2), 0, 0);
       }
     }
   }

@@ -216,6 +216,15 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
   float held32[KIND == kDrBackward && kNarrow ? NC : 1];
   int held_n = 0, held_c = 0;
   auto at_token = [&](int i) { return NC * (i / RT) + 4 * G * ((i % RT) >> 2) + 4 * g + (i & 3); };
+  // Element (row, col) of a matrix of operands (dr_operand_at) with row = NC t + 4 G q + 4 g + r: this
+  // lane's share of the address, and the rest, the same for all lanes.
+  const int v_steps = (A.Dv + 15) / 16;
+  const uint32_t operand_lane = la_in(
+      col < v_steps * 16, (((col >> 4) * 64 + 4 * g + 32 * ((col >> 2) & 1)) * 8 + (col & 3) + 4 * ((col >> 3) & 1)) * ES);
+  auto operand_rest = [&](int t, int reg) {
+    const int q = reg >> 2, r = reg & 3, row = NC == 32 ? 8 * q + r : 16 * (t & 1) + r;
+    return std::pair<int, int>{(NC == 32 ? t : t >> 1) * v_steps * 512 * ES, row * 8 * ES};
+  };
   auto hold = [&](uint32_t* to, const float* v) {
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
@@ -228,24 +237,24 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
   auto flush = [&]() {
     const int t0 = pc.begin + held_c * kDrC, n = held_n;  // nothing held: 0 tokens
     if constexpr (KIND == kDrForward) {
+      const int step = static_cast<int>(A.o_st) * size, c0 = col0 + NC * wave + 4 * g;
       const rsrc_t ro = make_rsrc(static_cast<char*>(A.out) + (batch * A.o_sb + h * A.o_sh +
                                                                static_cast<long long>(t0) * A.o_st) * size,
-                                  0x7fffffffu);
+                                  !kNarrow ? 0x7fffffffu : n > 0 ? (n - 1) * step + A.Dv * size : 0);
 #pragma unroll
       for (int t = 0; t < TT; ++t) {
         const int tok = NC * t + nn;
 #pragma unroll
         for (int q = 0; q < RT / 4; ++q) {
-          const int cc = col0 + NC * wave + 4 * G * q + 4 * g;
-          const uint32_t at = (tok * static_cast<int>(A.o_st) + cc) * size;
+          const int cc = c0 + 4 * G * q;
           if constexpr (kNarrow) {
             const int i = (RT * t + 4 * q) / 2;
             __builtin_amdgcn_raw_buffer_store_b64(u2{held_o[i], held_o[i + 1]}, ro,
-                                                  la_in((tok < n) & (cc < A.Dv), at), 0, 0);
+                                                  la_in(cc < A.Dv, tok * step + cc * 2), 0, 0);
           } else {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const uint32_t to = la_in((tok < n) & (cc + r < A.Dv), at + r * size);
+              const uint32_t to = la_in((tok < n) & (cc + r < A.Dv), tok * step + (cc + r) * size);
               const float v = __uint_as_float(held_o[RT * t + 4 * q + r]);
               if (A.dtype == PRNN_F32)
                 stb<float>(ro, to, 0, v);
@@ -261,20 +270,22 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
     if constexpr (!kOwn) {
       void* p = kBack ? A.dv : A.e;
       if (p && n > 0) {
-        // backwards dense rows of the tokens that are there, forwards operands (zeros behind the sequence)
-        const size_t unit = static_cast<size_t>(row0 + held_c) * A.H + h;
-        const rsrc_t r = make_rsrc(static_cast<E*>(p) + (kBack ? ((tok0 + t0) * A.H + h) * A.Dv
-                                                               : unit * dr_operand_elems(kDrC, A.Dv)),
-                                   0x7fffffffu);
+        // backwards dense rows of the tokens that are there (the others lie behind the buffer), forwards
+        // operands (zeros behind the sequence)
+        const int step = A.H * A.Dv * ES;
+        const size_t elems = dr_operand_elems(kDrC, A.Dv);
+        const rsrc_t r = kBack ? make_rsrc(static_cast<E*>(p) + ((tok0 + t0) * A.H + h) * A.Dv, (n - 1) * step + A.Dv * ES)
+                               : make_rsrc(static_cast<E*>(p) + (static_cast<size_t>(row0 + held_c) * A.H + h) * elems,
+                                           static_cast<uint32_t>(elems) * ES);
+        const uint32_t lane_at = kBack ? la_in(col < A.Dv, 4 * g * step + col * ES) : operand_lane;
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
-          const int tok = at_token(i);
-          const uint32_t to = kBack ? la_in((tok < n) & (col < A.Dv), (tok * A.H * A.Dv + col) * ES)
-                                    : la_in(col < (A.Dv + 15) / 16 * 16, dr_operand_at(A.Dv, tok, col) * ES);
+          const auto rest = kBack ? std::pair<int, int>{0, (at_token(i) - 4 * g) * step} : operand_rest(i / RT, i % RT);
           if constexpr (kNarrow)
-            __builtin_amdgcn_raw_buffer_store_b16(i & 1 ? held_u[i / 2] >> 16 : held_u[i / 2], r, to, 0, 0);
+            __builtin_amdgcn_raw_buffer_store_b16(i & 1 ? held_u[i / 2] >> 16 : held_u[i / 2], r,
+                                                  lane_at + rest.second, rest.first, 0);
           else
-            __builtin_amdgcn_raw_buffer_store_b32(held_u[i], r, to, 0, 0);
+            __builtin_amdgcn_raw_buffer_store_b32(held_u[i], r, lane_at + rest.second, rest.first, 0);
         }
       }
     }
@@ -319,9 +330,9 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
       for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-          const int i = NC * t + 4 * G * (r >> 2) + 4 * g + (r & 3);
-          store_elem<M>(rs, la_in((i < (A.Dk + 31) / 32 * 32) & (col < (A.Dv + 15) / 16 * 16),
-                                  dr_operand_at(A.Dv, i, col) * ES), S[t][r]);
+          const auto rest = operand_rest(t, r);
+          if (NC * t < (A.Dk + 31) / 32 * 32)  // rows behind the matrix: zeros up to the end of its tile
+            store_elem<M>(rs, operand_lane + rest.second, rest.first, S[t][r]);
         }
     }
     const char* const sS = kSysLds ? s_sys : A.sys + (static_cast<size_t>(row0 + c) * A.H + h) * kDrSys;

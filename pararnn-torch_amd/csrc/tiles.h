@@ -203,11 +203,11 @@ __device__ __forceinline__ Op<M, 1> col_op(const char* at, int t0, int c0) {
 
 // One element rounded to the arithmetic's type.
 template <class M>
-__device__ __forceinline__ void store_elem(rsrc_t r, uint32_t at, float v) {
+__device__ __forceinline__ void store_elem(rsrc_t r, uint32_t at, uint32_t base, float v) {
   if constexpr (sizeof(typename M::E) == 2)
-    stb<bf16>(r, at, 0, v);
+    stb<bf16>(r, at, base, v);
   else
-    stb<float>(r, at, 0, v);
+    stb<float>(r, at, base, v);
 }
 
 // Upper half of a's lanes for the lower half of b's.
