@@ -351,11 +351,19 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) s[e] = S[(8 * f + e) / RT][(8 * f + e) % RT];
       const auto sp = parts_of<M, 2>(s);
+      Op<M, 1> ko[TT], qo[TT];
 #pragma unroll
       for (int t = 0; t < TT; ++t) {
-        mul<NC>(X[t], row_op<M, G>(sK + (NC * t + nn) * RK, f, g), sp);
-        if constexpr (KIND == kDrForward) mul<NC>(O[t], sp, row_op<M, G>(sQ + (NC * t + nn) * RK, f, g));
+        ko[t] = row_op<M, G>(sK + (NC * t + nn) * RK, f, g);
+        if constexpr (KIND == kDrForward) qo[t] = row_op<M, G>(sQ + (NC * t + nn) * RK, f, g);
       }
+#pragma unroll
+      for (int k = 0; k < kPairs<1, 2>; ++k)
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+          mul_one<NC>(X[t], ko[t], sp, k);
+          if constexpr (KIND == kDrForward) mul_one<NC>(O[t], sp, qo[t], k);
+        }
     }
 
     const char* zat = sZ + NC * wave * ES + col_share<M, G, RZ>(lane);
@@ -385,12 +393,20 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
     } else {
       // P^T go, then the adjoint behind the chunk
 #pragma unroll
-      for (int t = 0; t < TT; ++t) {
+      for (int t = 0; t < TT; ++t)
 #pragma unroll
         for (int r = 0; r < RT; ++r) Y[t][r] = 0.0f;
 #pragma unroll
-        for (int f = 0; f < TF; ++f)
-          if (Mat::any(t, f)) mul<NC>(Y[t], Mat::get(sS + kDrTiles, t, f, nn, g), zo[f]);
+      for (int f = 0; f < TF; ++f) {
+        Op<M, M::kParts> m[TT];
+#pragma unroll
+        for (int t = 0; t < TT; ++t)
+          if (Mat::any(t, f)) m[t] = Mat::get(sS + kDrTiles, t, f, nn, g);
+#pragma unroll
+        for (int k = 0; k < kPairs<M::kParts, 1>; ++k)
+#pragma unroll
+          for (int t = 0; t < TT; ++t)
+            if (Mat::any(t, f)) mul_one<NC>(Y[t], m[t], zo[f], k);
       }
 #pragma unroll
       for (int i = 0; i < NC; i += 4) {
@@ -435,12 +451,20 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
       yo[f] = parts_of<M, 2>(v);
     }
 #pragma unroll
-    for (int t = 0; t < TT; ++t) {
+    for (int t = 0; t < TT; ++t)
 #pragma unroll
       for (int r = 0; r < RT; ++r) Y[t][r] = y[RT * t + r];
 #pragma unroll
-      for (int f = 0; f < TF; ++f)
-        if (Mat::any(t, f)) mul<NC>(Y[t], Mat::get(sS, t, f, nn, g), yo[f]);
+    for (int f = 0; f < TF; ++f) {
+      Op<M, M::kParts> m[TT];
+#pragma unroll
+      for (int t = 0; t < TT; ++t)
+        if (Mat::any(t, f)) m[t] = Mat::get(sS, t, f, nn, g);
+#pragma unroll
+      for (int k = 0; k < kPairs<M::kParts, 2>; ++k)
+#pragma unroll
+        for (int t = 0; t < TT; ++t)
+          if (Mat::any(t, f)) mul_one<NC>(Y[t], m[t], yo[f], k);
     }
 
     float u[NC];  // what is written: b e forwards, dv backwards
@@ -468,20 +492,28 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
       }
 #pragma unroll
       for (int t = 0; t < TT; ++t) {
-        const int tok = NC * t + nn;
-        const float w = sW[kWg * 64 + tok] * A.scale;
+        const float w = sW[kWg * 64 + NC * t + nn] * A.scale;
 #pragma unroll
         for (int r = 0; r < RT; ++r) O[t][r] *= w;
+      }
 #pragma unroll
-        for (int f = 0; f < TF; ++f)
-          if (Mat::any(t, f)) mul<NC>(O[t], uo[f], Mat::get(sS + kDrTiles, t, f, nn, g));
-        if (poisoned) {
+      for (int f = 0; f < TF; ++f) {
+        Op<M, M::kParts> m[TT];
 #pragma unroll
-          for (int r = 0; r < RT; ++r) {
-            const int s = __shfl(stop, 4 * G * (r >> 2) + 4 * g + (r & 3));
-            if (tok >= s) O[t][r] = __int_as_float(0x7fc00000);
-          }
-        }
+        for (int t = 0; t < TT; ++t)
+          if (Mat::any(t, f)) m[t] = Mat::get(sS + kDrTiles, t, f, nn, g);
+#pragma unroll
+        for (int k = 0; k < kPairs<2, M::kParts>; ++k)
+#pragma unroll
+          for (int t = 0; t < TT; ++t)
+            if (Mat::any(t, f)) mul_one<NC>(O[t], uo[f], m[t], k);
+      }
+      if (poisoned) {
+#pragma unroll
+        for (int t = 0; t < TT; ++t)
+#pragma unroll
+          for (int r = 0; r < RT; ++r)
+            if (NC * t + nn >= __shfl(stop, 4 * G * (r >> 2) + 4 * g + (r & 3))) O[t][r] = __int_as_float(0x7fc00000);
       }
       float v[NC];
 #pragma unroll
@@ -522,8 +554,16 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
         for (int r = 0; r < 4; ++r) v[e + r] = (kBack ? -w[r] : w[r]) * u[8 * f + e + r];
       }
       const auto uo = parts_of<M, 3>(v);
+      auto into = [&](const char* rows, const Op<M, 3>& o) {
+        Op<M, 1> c[KT];
 #pragma unroll
-      for (int t = 0; t < KT; ++t) mul<NC>(S[t], col_op<M, G, RK>(kat, 8 * G * f, NC * t), uo);
+        for (int t = 0; t < KT; ++t) c[t] = col_op<M, G, RK>(rows, 8 * G * f, NC * t);
+#pragma unroll
+        for (int k = 0; k < kPairs<1, 3>; ++k)
+#pragma unroll
+          for (int t = 0; t < KT; ++t) mul_one<NC>(S[t], c[t], o, k);
+      };
+      into(kat, uo);
       if constexpr (kBack) {
         float z[8];
         values(zo[f], z);
@@ -534,8 +574,7 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
           for (int r = 0; r < 4; ++r) z[e + r] *= w[r] * A.scale;
         }
         const auto go = parts_of<M, 3>(z);
-#pragma unroll
-        for (int t = 0; t < KT; ++t) mul<NC>(S[t], col_op<M, G, RK>(qat, 8 * G * f, NC * t), go);
+        into(qat, go);
       }
     }
     if (!kBack && poisoned && stop < kDrC) {

@@ -85,6 +85,21 @@ __device__ __forceinline__ void mul(Acc<NC>& c, const Op<InF32, P>& a, const Op<
   for (int i = 0; i < 8; ++i) c = mfma_f32<NC>(a.x[i], b.x[i], c);
 }
 
+// The same product by product, so that several sums can take turns (a matrix instruction waits for the
+// last one of its own sum): products kPairs<P, R> of operands of P and R parts, number k of them.
+template <int P, int R>
+constexpr int kPairs = P == 1 || R == 1 ? P * R : 3;  // (two parts each: the small ones' product is left out)
+template <int NC, int P, int R>
+__device__ __forceinline__ void mul_one(Acc<NC>& c, const Op<InBf16, P>& a, const Op<InBf16, R>& b, int k) {
+  static_assert(P == 1 || R == 1 || (P == 2 && R == 2), "products are listed for these");
+  const int i = P == 1 ? 0 : R == 1 ? k : k == 2, j = P == 1 ? k : R == 1 ? 0 : k == 1;
+  c = mfma_bf16<NC>(a.p[i], b.p[j], c);
+}
+template <int NC, int P, int R>
+__device__ __forceinline__ void mul_one(Acc<NC>& c, const Op<InF32, P>& a, const Op<InF32, R>& b, int k) {
+  if (k == 0) mul<NC>(c, a, b);
+}
+
 __device__ __forceinline__ b8 pack8(const float* x) {
   union {
     uint32_t w[4];
