@@ -81,12 +81,12 @@ struct Plan {
   bool cut;
 };
 
-// Columns of a wave: 32, or 16 where there are not enough waves of 32 for the chip's 1024 SIMDs (and
+// Columns of a wave: 32, or 16 where there are not enough waves of 32 for two of the chip's 1024 SIMDs (and
 // where 32 columns of wide keys do not fit the registers).
 int wave_cols(const Problem& a, const LaSeqs& q) {
   if (!on_bf16(a)) return 16;
   if (a.la.Dk > 128 || (a.la.Dk > 64 && a.la.Dv <= 64)) return 16;
-  return dr_units(q, q.len) * a.la.H * ((a.la.Dv + 31) / 32) >= 1024 ? 32 : 16;
+  return dr_units(q, q.len) * a.la.H * ((a.la.Dv + 31) / 32) >= 2048 ? 32 : 16;
 }
 
 // A sequence's chunks come one after another.  Cut into n pieces they go side by side, but every piece
@@ -98,20 +98,21 @@ Plan plan(const Problem& a) {
   Plan p{16, sequences_of(a), false};
   const long long longest = a.la.cu_seqlens && a.la.longest > 0 ? std::min(a.la.longest, a.la.T) : a.la.T;
   const long long chunks = (longest + kDrC - 1) / kDrC, tokens = 1ll * a.la.B * a.la.T;
-  const double seqs = std::max(1.0, static_cast<double>(tokens) / std::max(1ll, longest));  // as if all were as long
   const int group_cols = dr_walk_cols(a.la.Dk, a.la.Dv, 16, on_bf16(a)).group * 16;
   const double tiles = (a.la.Dv + group_cols - 1) / group_cols;
-  const double own = tiles + (a.la.Dk + group_cols - 1) / group_cols;
-  auto slower = [](double groups) {
-    const double x = groups / 256.0;
-    return x <= 1.0 ? 1.0 : std::max(0.5 + 0.5 * x, 0.75 * x);
+  // of a packed batch half the tokens are taken to be in sequences that are cut
+  const double own = (tiles + (a.la.Dk + group_cols - 1) / group_cols) * (a.la.cu_seqlens ? 0.5 : 1.0);
+  const double work = static_cast<double>(tokens) / kDrC * a.la.H / 256.0;  // chunks a CU and column tile
+  auto time = [&](double each, double tiles) {
+    const double x = work * tiles / each;
+    return each * (x <= 1.0 ? 1.0 : std::max(0.5 + 0.5 * x, 0.75 * x));
   };
   double best = 0.0;
   long long pieces = 1;
   for (long long n = 1; n <= 64 && n <= chunks; ++n) {
-    const double each = static_cast<double>((chunks + n - 1) / n), heads = seqs * a.la.H * n;
-    double t = each * slower(heads * tiles);
-    if (n > 1) t += 0.6 * each * slower(heads * own) + 0.4 * n + 4.0;
+    const double each = static_cast<double>((chunks + n - 1) / n);
+    double t = time(each, tiles);
+    if (n > 1) t += 0.6 * time(each, own) + 0.4 * n + 4.0;
     if (n == 1 || t < best) {
       best = t;
       pieces = n;
