@@ -28,8 +28,8 @@ struct Staged {
 
   // `width` columns from c0; tokens [0, n) from `p` are there: the others lie behind the buffer's end (a
   // row is at most a stride wide, or they are told by a comparison).
-  __device__ __forceinline__ void fetch(const char* p, long long st, int n, int c0, int width, int dtype) {
-    const int tid = threadIdx.x;
+  __device__ __forceinline__ void fetch(const char* p, long long st, int n, int c0, int width, int dtype,
+                                        int tid = threadIdx.x) {
     if constexpr (kNarrow) {
       constexpr int D = NT / U;  // rows between a thread's loads
       static_assert(NT % U == 0, "whole rows");
@@ -53,10 +53,10 @@ struct Staged {
     }
   }
   template <int RB>
-  __device__ __forceinline__ void put(char* tile, int dtype) const {
+  __device__ __forceinline__ void put(char* tile, int dtype, int tid = threadIdx.x) const {
 #pragma unroll
     for (int k = 0; k < N; ++k) {
-      const int e = threadIdx.x + k * NT, row = e / U, c = e % U;
+      const int e = tid + k * NT, row = e / U, c = e % U;
       if constexpr (kNarrow) {
         *reinterpret_cast<u4*>(tile + row * RB + c * 16) = r[k];
       } else {

@@ -7,8 +7,8 @@
 //   forwards   x = K S,   e = (1 + T)(v - exp(G) x),          S' = exp(G_last) S + K^T (..u)
 //   backwards  x = K R,   dv = (1 + T)^T b (P^T go + .. x),     R' = exp(G_last) R + Q^T (..go) - K^T (..dv)
 //
-// take what the one before left in registers, so a wave's chain meets no other wave: the two
-// barriers of a chunk only hand K, Q and the system through LDS.  The output is formed transposed
+// take what the one before left in registers, so a wave's chain meets no other wave: a chunk's
+// barriers only hand K, Q and the system through LDS.  The output is formed transposed
 // from the same registers (state and u as first operands), so that a lane holds consecutive columns
 // of a token.
 #pragma once
@@ -114,13 +114,16 @@ __device__ __forceinline__ void dr_place(int tiles, int H, int& tile, int& h, in
   h = item - piece * H;
 }
 
-template <class M, int NC, int KD, int W, int KIND>
-__global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
+// W waves of NC columns each.  L: waves besides that do nothing but bring the next chunk to LDS, into
+// one of two buffers, while the others work on this one (bringing it took 4500 of a chunk's 9700 cycles
+// of a wave that does both); 0: the same waves do it, and the chunk's LDS is there once.
+template <class M, int NC, int KD, int W, int L, int KIND>
+__global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
   using E = typename M::E;
   constexpr bool kNarrow = sizeof(E) == 2;
   constexpr bool kBack = KIND == kDrBackward || KIND == kDrAdjoint;
   constexpr bool kOwn = KIND == kDrState || KIND == kDrAdjoint;  // pieces' own states only
-  constexpr int G = 64 / NC, NT = 64 * W, VT = NC * W;
+  constexpr int G = 64 / NC, NT = 64 * (L ? L : W), VT = NC * W;  // NT: threads that bring rows
   constexpr int RT = NC * NC / 64;   // registers of a tile
   constexpr int KT = KD / NC;        // the state's tiles
   constexpr int KF = KD / (8 * G);   // steps of a contraction over its rows
@@ -138,11 +141,11 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
   constexpr int kSysBytes = kP ? 2 * kDrTiles : kDrTiles;
   constexpr int kSysUnits = kSysBytes / 16 / NT;
   static_assert(kSysBytes % (16 * NT) == 0, "whole units");
-  __shared__ __align__(16) char sK[kDrC * RK];
-  __shared__ __align__(16) char sQ[kQ ? kDrC * RK : 16];
-  __shared__ __align__(16) char sZ[kDrC * RZ];
-  __shared__ __align__(16) char s_sys[kSysLds ? kSysBytes : 16];
-  __shared__ __align__(16) float sW[kDrW * 64];
+  static_assert(L == 0 || (kAhead && kSysLds), "waves that only load hold a chunk");
+  // a chunk in LDS: K, Q, z, the system and the pairs, the weights
+  constexpr int oQ = kDrC * RK, oZ = oQ + (kQ ? kDrC * RK : 0), oS = oZ + kDrC * RZ,
+                oW = oS + (kSysLds ? kSysBytes : 0), kChunk = oW + kDrW * 64 * 4;
+  __shared__ __align__(16) char lds[(L ? 2 : 1) * kChunk];
 
   int tile, h, piece;
   dr_place(A.tiles, A.H, tile, h, piece);
@@ -150,7 +153,8 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
   if (!pc.any || pc.seq >= A.seqs.n_seq) return;
   // the last piece of the walk's direction hands its state to none
   if (kOwn && pc.index == (kBack ? 0 : pc.count - 1)) return;
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int tid = L ? static_cast<int>(threadIdx.x) - 64 * W : static_cast<int>(threadIdx.x);  // of those that bring rows
   const int nn = lane % NC, g = lane / NC;
   const bool transfer = kOwn && tile >= A.own_tiles;
   const int col0 = (transfer ? tile - A.own_tiles : tile) * VT;
@@ -160,6 +164,61 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
   const int chunks = (pc.end - pc.begin + kDrC - 1) / kDrC;
   const size_t state_floats = static_cast<size_t>(A.Dk) * A.Dv;
   const size_t tok0 = dr_token(A.seqs, pc, 0);
+
+  std::conditional_t<kAhead, Staged<M, KD, NT>, NotStaged> rk, rq;
+  Staged<M, VT, NT> rz;
+  u4 rs[kSysLds ? kSysUnits : 1], rw[(kDrW * 64 / 4 + NT - 1) / NT];
+  const int size = kNarrow || A.dtype != PRNN_F32 ? 2 : 4;
+  auto head = [&](const LaView& v, int t) {
+    return static_cast<const char*>(v.p) +
+           (batch * v.sb + (h / v.rep) * v.sh + static_cast<long long>(t) * v.st) * size;
+  };
+  auto fetch = [&](int c) {
+    const int t = pc.begin + c * kDrC, n = min(pc.end - t, kDrC);
+    const char* sys = A.sys + (static_cast<size_t>(row0 + c) * A.H + h) * kDrSys;
+#pragma unroll
+    for (int k = 0; k < (kSysLds ? kSysUnits : 0); ++k) rs[k] = *reinterpret_cast<const u4*>(sys + (tid + k * NT) * 16);
+    const char* w = sys + 2 * kDrTiles;
+#pragma unroll
+    for (int k = 0; k < (kDrW * 16 + NT - 1) / NT; ++k)
+      if (tid + k * NT < kDrW * 16) rw[k] = *reinterpret_cast<const u4*>(w + (tid + k * NT) * 16);
+    if constexpr (kAhead) rk.fetch(head(A.k, t), A.k.st, n, 0, A.Dk, A.dtype, tid);
+    if constexpr (kAhead && kQ) rq.fetch(head(A.q, t), A.q.st, n, 0, A.Dk, A.dtype, tid);
+    rz.fetch(head(A.z, t), A.z.st, transfer ? 0 : n, col0, A.Dv, A.dtype, tid);
+  };
+  auto chunk_of = [&](int step) { return kBack ? chunks - 1 - step : step; };
+  auto put = [&](char* to, int c) {
+    if constexpr (kAhead) {
+      rk.template put<RK>(to, A.dtype, tid);
+      if constexpr (kQ) rq.template put<RK>(to + oQ, A.dtype, tid);
+    } else {
+      const int t = pc.begin + c * kDrC, n = min(pc.end - t, kDrC);
+      fill<M, KD, NT, RK>(to, head(A.k, t), A.k.st, n, A.Dk, A.dtype);
+      if constexpr (kQ) fill<M, KD, NT, RK>(to + oQ, head(A.q, t), A.q.st, n, A.Dk, A.dtype);
+    }
+    rz.template put<RZ>(to + oZ, A.dtype, tid);
+#pragma unroll
+    for (int k = 0; k < (kSysLds ? kSysUnits : 0); ++k) *reinterpret_cast<u4*>(to + oS + (tid + k * NT) * 16) = rs[k];
+#pragma unroll
+    for (int k = 0; k < (kDrW * 16 + NT - 1) / NT; ++k)
+      if (tid + k * NT < kDrW * 16) *reinterpret_cast<u4*>(to + oW + (tid + k * NT) * 16) = rw[k];
+  };
+  if constexpr (L > 0) {
+    if (wave >= W) {  // one barrier a chunk, as the others' below
+      if (chunks > 0) {
+        fetch(chunk_of(0));
+        put(lds, 0);
+      }
+      if (chunks > 1) fetch(chunk_of(1));
+      __syncthreads();
+      for (int step = 0; step < chunks; ++step) {
+        if (step + 1 < chunks) put(lds + (~step & 1) * kChunk, 0);
+        if (step + 2 < chunks) fetch(chunk_of(step + 2));
+        __syncthreads();
+      }
+      return;
+    }
+  }
 
   // ---- the state that the piece begins with
   A_t S[KT];
@@ -188,27 +247,6 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
     }
   }
 
-  std::conditional_t<kAhead, Staged<M, KD, NT>, NotStaged> rk, rq;
-  Staged<M, VT, NT> rz;
-  u4 rs[kSysLds ? kSysUnits : 1], rw[(kDrW * 64 / 4 + NT - 1) / NT];
-  const int size = kNarrow || A.dtype != PRNN_F32 ? 2 : 4;
-  auto head = [&](const LaView& v, int t) {
-    return static_cast<const char*>(v.p) +
-           (batch * v.sb + (h / v.rep) * v.sh + static_cast<long long>(t) * v.st) * size;
-  };
-  auto fetch = [&](int c) {
-    const int t = pc.begin + c * kDrC, n = min(pc.end - t, kDrC);
-    const char* sys = A.sys + (static_cast<size_t>(row0 + c) * A.H + h) * kDrSys;
-#pragma unroll
-    for (int k = 0; k < (kSysLds ? kSysUnits : 0); ++k) rs[k] = *reinterpret_cast<const u4*>(sys + (tid + k * NT) * 16);
-    const char* w = sys + 2 * kDrTiles;
-#pragma unroll
-    for (int k = 0; k < (kDrW * 16 + NT - 1) / NT; ++k)
-      if (tid + k * NT < kDrW * 16) rw[k] = *reinterpret_cast<const u4*>(w + (tid + k * NT) * 16);
-    if constexpr (kAhead) rk.fetch(head(A.k, t), A.k.st, n, 0, A.Dk, A.dtype);
-    if constexpr (kAhead && kQ) rq.fetch(head(A.q, t), A.q.st, n, 0, A.Dk, A.dtype);
-    rz.fetch(head(A.z, t), A.z.st, transfer ? 0 : n, col0, A.Dv, A.dtype);
-  };
   // What a chunk leaves is stored after the next one's rows have come: loads and stores come back in
   // order, and a wait for rows behind stores would wait for those too (155 us for .. without).
   constexpr int kHeld = kNarrow ? NC / 2 : NC;
@@ -302,24 +340,18 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
       }
     }
   };
-  if (chunks > 0) fetch(kBack ? chunks - 1 : 0);
+  if constexpr (L > 0) {
+    __syncthreads();
+  } else {
+    if (chunks > 0) fetch(chunk_of(0));
+  }
 
   for (int step = 0; step < chunks; ++step) {
-    const int c = kBack ? chunks - 1 - step : step;
-    const int t0 = pc.begin + c * kDrC, n = min(pc.end - t0, kDrC);
-    if constexpr (kAhead) {
-      rk.template put<RK>(sK, A.dtype);
-      if constexpr (kQ) rq.template put<RK>(sQ, A.dtype);
-    } else {
-      fill<M, KD, NT, RK>(sK, head(A.k, t0), A.k.st, n, A.Dk, A.dtype);
-      if constexpr (kQ) fill<M, KD, NT, RK>(sQ, head(A.q, t0), A.q.st, n, A.Dk, A.dtype);
-    }
-    rz.template put<RZ>(sZ, A.dtype);
-#pragma unroll
-    for (int k = 0; k < (kSysLds ? kSysUnits : 0); ++k) *reinterpret_cast<u4*>(s_sys + (tid + k * NT) * 16) = rs[k];
-#pragma unroll
-    for (int k = 0; k < (kDrW * 16 + NT - 1) / NT; ++k)
-      if (tid + k * NT < kDrW * 16) *reinterpret_cast<u4*>(reinterpret_cast<char*>(sW) + (tid + k * NT) * 16) = rw[k];
+    const int c = chunk_of(step), t0 = pc.begin + c * kDrC, n = min(pc.end - t0, kDrC);
+    char* const at = lds + (L ? (step & 1) * kChunk : 0);
+    const char *const sK = at, *const sQ = at + oQ, *const sZ = at + oZ;
+    const float* const sW = reinterpret_cast<const float*>(at + oW);
+    if constexpr (L == 0) put(at, c);
     if (!kOwn) flush();
     // what the gradients of this chunk need of the state
     if (!kOwn && A.keep) {
@@ -335,9 +367,11 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
             store_elem<M>(rs, operand_lane + rest.second, rest.first, S[t][r]);
         }
     }
-    const char* const sS = kSysLds ? s_sys : A.sys + (static_cast<size_t>(row0 + c) * A.H + h) * kDrSys;
-    __syncthreads();
-    if (step + 1 < chunks) fetch(kBack ? c - 1 : c + 1);
+    const char* const sS = kSysLds ? at + oS : A.sys + (static_cast<size_t>(row0 + c) * A.H + h) * kDrSys;
+    if constexpr (L == 0) {
+      __syncthreads();
+      if (step + 1 < chunks) fetch(chunk_of(step + 1));
+    }
 
     // ---- x = K S and the state's part of the output, S^T Q^T
     A_t X[TT], O[TT];
@@ -611,12 +645,12 @@ __global__ __launch_bounds__(64 * W, 1) void dr_walk_kernel(DrWalk A) {
   }
 }
 
-template <class M, int NC, int KD, int W, int KIND>
+template <class M, int NC, int KD, int W, int L, int KIND>
 int dr_launch_walk(const DrWalk& a, hipStream_t stream) {
   const long long items = dr_units(a.seqs, a.seqs.len) * a.H;
   const long long groups = (items + 7) / 8 * 8 * a.tiles;
-  if (int rc = check_grid("delta_rule", groups, 64 * W)) return rc;
-  dr_walk_kernel<M, NC, KD, W, KIND><<<static_cast<unsigned>(groups), 64 * W, 0, stream>>>(a);
+  if (int rc = check_grid("delta_rule", groups, 64 * (W + L))) return rc;
+  dr_walk_kernel<M, NC, KD, W, L, KIND><<<static_cast<unsigned>(groups), 64 * (W + L), 0, stream>>>(a);
   PRNN_HIP(hipGetLastError());
   return PRNN_OK;
 }
