@@ -263,6 +263,36 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
     const int q = reg >> 2, r = reg & 3, row = NC == 32 ? 8 * q + r : 16 * (t & 1) + r;
     return std::pair<int, int>{(NC == 32 ? t : t >> 1) * v_steps * 512 * ES, row * 8 * ES};
   };
+  // bf16: what is stored is turned by a product with the unit matrix (exact), so that a lane has four
+  // columns of a row and not a row's place in four of them: 8 bytes a store and not 2.
+  Op<M, 1> unit[2];
+  if constexpr (kNarrow && !kOwn) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int place = NC == 32 ? nn - 16 * j : nn + 16 * j;  // of the contraction that is this lane's column
+      float one[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) one[e] = place == 4 * G * (e >> 2) + 4 * g + (e & 3) ? 1.0f : 0.0f;
+      unit[j] = parts_of<M, 1>(one);
+    }
+  }
+  auto turned = [&](const Op<M, 1>* o, int t) {  // tile t of the operands: lane its row, registers columns
+    A_t d;
+#pragma unroll
+    for (int r = 0; r < RT; ++r) d[r] = 0.0f;
+    if constexpr (NC == 32) {
+      mul<NC>(d, o[2 * t], unit[0]);
+      mul<NC>(d, o[2 * t + 1], unit[1]);
+    } else {
+      mul<NC>(d, o[t >> 1], unit[t & 1]);
+    }
+    return d;
+  };
+  auto operand8 = [&](int row, int q) {  // place of columns 4 G q + 4 g .. + 3 of the wave's at `row`
+    const int cc = col0 + NC * wave + 4 * G * q + 4 * g;
+    return la_in(cc < v_steps * 16, (((row >> 5) * v_steps + (cc >> 4)) * 64 + (row & 31) + 32 * ((cc >> 2) & 1)) * 16 +
+                                        ((cc >> 3) & 1) * 8);
+  };
   auto hold = [&](uint32_t* to, const float* v) {
 #pragma unroll
     for (int i = 0; i < kHeld; ++i) {
@@ -270,6 +300,23 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
         to[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
       else
         to[i] = __float_as_uint(v[i]);
+    }
+  };
+  auto hold_rows = [&](uint32_t* to, float* v) {
+    if constexpr (kNarrow) {
+      Op<M, 1> o[TF];
+#pragma unroll
+      for (int f = 0; f < TF; ++f) o[f] = parts_of<M, 1>(v + 8 * f);
+      float d[NC];
+#pragma unroll
+      for (int t = 0; t < TT; ++t) {
+        const A_t x = turned(o, t);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) d[RT * t + r] = x[r];
+      }
+      hold(to, d);
+    } else {
+      hold(to, v);
     }
   };
   auto flush = [&]() {
@@ -316,14 +363,21 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
                                : make_rsrc(static_cast<E*>(p) + (static_cast<size_t>(row0 + held_c) * A.H + h) * elems,
                                            static_cast<uint32_t>(elems) * ES);
         const uint32_t lane_at = kBack ? la_in(col < A.Dv, 4 * g * step + col * ES) : operand_lane;
+        if constexpr (kNarrow) {
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
+          for (int t = 0; t < TT; ++t)
+#pragma unroll
+            for (int q = 0; q < RT / 4; ++q) {
+              const int i = (RT * t + 4 * q) / 2, tok = NC * t + nn, cc = col0 + NC * wave + 4 * G * q + 4 * g;
+              __builtin_amdgcn_raw_buffer_store_b64(
+                  u2{held_u[i], held_u[i + 1]}, r,
+                  kBack ? la_in(cc < A.Dv, tok * step + cc * 2) : operand8(tok, q), 0, 0);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < (kNarrow ? 0 : NC); ++i) {
           const auto rest = kBack ? std::pair<int, int>{0, (at_token(i) - 4 * g) * step} : operand_rest(i / RT, i % RT);
-          if constexpr (kNarrow)
-            __builtin_amdgcn_raw_buffer_store_b16(i & 1 ? held_u[i / 2] >> 16 : held_u[i / 2], r,
-                                                  lane_at + rest.second, rest.first, 0);
-          else
-            __builtin_amdgcn_raw_buffer_store_b32(held_u[i], r, lane_at + rest.second, rest.first, 0);
+          __builtin_amdgcn_raw_buffer_store_b32(held_u[i], r, lane_at + rest.second, rest.first, 0);
         }
       }
     }
@@ -354,7 +408,7 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
     if constexpr (L == 0) put(at, c);
     if (!kOwn) flush();
     // what the gradients of this chunk need of the state
-    if (!kOwn && A.keep) {
+    if (!kOwn && !kNarrow && A.keep) {
       const size_t elems = dr_operand_elems(A.Dk, A.Dv);
       const rsrc_t rs = make_rsrc(static_cast<E*>(A.keep) + (static_cast<size_t>(row0 + c) * A.H + h) * elems,
                                   static_cast<uint32_t>(elems) * ES);
@@ -379,12 +433,14 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
     for (int t = 0; t < TT; ++t)
 #pragma unroll
       for (int r = 0; r < RT; ++r) X[t][r] = O[t][r] = 0.0f;
+    Op<M, 1> rounded[kNarrow && !kOwn ? KF : 1];
 #pragma unroll
     for (int f = 0; f < KF; ++f) {
       float s[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) s[e] = S[(8 * f + e) / RT][(8 * f + e) % RT];
       const auto sp = parts_of<M, 2>(s);
+      if constexpr (kNarrow && !kOwn) rounded[f].p[0] = sp.p[0];
       Op<M, 1> ko[TT], qo[TT];
 #pragma unroll
       for (int t = 0; t < TT; ++t) {
@@ -398,6 +454,24 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
           mul_one<NC>(X[t], ko[t], sp, k);
           if constexpr (KIND == kDrForward) mul_one<NC>(O[t], sp, qo[t], k);
         }
+    }
+
+    if constexpr (kNarrow && !kOwn) {
+      if (A.keep) {
+        const size_t elems = dr_operand_elems(A.Dk, A.Dv);
+        const rsrc_t rs = make_rsrc(static_cast<E*>(A.keep) + (static_cast<size_t>(row0 + c) * A.H + h) * elems,
+                                    static_cast<uint32_t>(elems) * ES);
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+          if (NC * t >= (A.Dk + 31) / 32 * 32) continue;  // rows behind the matrix: zeros up to the end of its tile
+          const A_t d = turned(rounded, t);
+#pragma unroll
+          for (int q = 0; q < RT / 4; ++q)
+            __builtin_amdgcn_raw_buffer_store_b64(
+                u2{pack_bf16x2(d[4 * q], d[4 * q + 1]), pack_bf16x2(d[4 * q + 2], d[4 * q + 3])}, rs,
+                operand8(NC * t + nn, q), 0, 0);
+        }
+      }
     }
 
     const char* zat = sZ + NC * wave * ES + col_share<M, G, RZ>(lane);
@@ -557,11 +631,14 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
 #pragma unroll
         for (int i = 0; i < NC; ++i)
           v[i] = at_token(i) >= stop ? __int_as_float(0x7fc00000) : Y[i / RT][i % RT];
-        hold(held_u, v);
+        hold_rows(held_u, v);
       }
     }
     if constexpr (KIND == kDrBackward) {
-      hold(held_u, u);
+      float dv[NC];
+#pragma unroll
+      for (int i = 0; i < NC; ++i) dv[i] = u[i];
+      hold_rows(held_u, dv);
       if constexpr (kNarrow) {
 #pragma unroll
         for (int i = 0; i < NC; ++i) held32[i] = u[i];

@@ -6,8 +6,10 @@ namespace {
 
 template <int KIND>
 int launch_kd(const DrWalk& a, hipStream_t stream) {
-  if (a.Dk <= 32) return dr_launch_walk<InF32, 16, 32, 4, 4, KIND>(a, stream);
-  if (a.Dk <= 64) return dr_launch_walk<InF32, 16, 64, 4, 4, KIND>(a, stream);
+  // waves that only load as on bf16 instructions (two chunks in LDS up to widths of 64)
+  constexpr int kLoad = KIND != kDrState && KIND != kDrAdjoint ? 4 : 0;
+  if (a.Dk <= 32) return dr_launch_walk<InF32, 16, 32, 4, kLoad, KIND>(a, stream);
+  if (a.Dk <= 64) return dr_launch_walk<InF32, 16, 64, 4, kLoad, KIND>(a, stream);
   if (a.Dk <= 128) return dr_launch_walk<InF32, 16, 128, 4, 0, KIND>(a, stream);
   return dr_launch_walk<InF32, 16, 256, 2, 0, KIND>(a, stream);
 }
