@@ -104,10 +104,8 @@ constexpr int kDrSys = 2 * kDrTiles + kDrW * 64 * 4;
 static_assert(kDrSys % 256 == 0, "blocks stay aligned");
 // kWmeta: [0] exp(G_last), [1] the first token that is not finite (64: none), as an integer
 
-template <typename E>
-__device__ __forceinline__ int dr_unit_of(int row, int unit) {
-  return unit ^ ((sizeof(E) == 2 ? row >> 2 : row >> 1) & 7);
-}
+// (so that 16 or 32 rows of a step fall into all banks, two words each)
+__device__ __forceinline__ int dr_unit_of(int row, int unit) { return unit ^ ((row >> 1) & 7); }
 
 // A token's rate.
 __device__ __forceinline__ float dr_rate(const LaDecay& b, int batch, int t, int h) {

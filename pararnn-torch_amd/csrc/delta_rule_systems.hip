@@ -134,7 +134,7 @@ __global__ __launch_bounds__(256) void dr_systems_kernel(DrSystems A) {
     if constexpr (sizeof(E) == 2) {
       // this lane holds units 2 q + half of its row; halves of the wave exchange them, so that either has
       // two units side by side (in one order or the other: the exchange by rows keeps such pairs)
-      const bool odd = dr_unit_of<E>(l32, 0) & 1;
+      const bool odd = dr_unit_of(l32, 0) & 1;
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
         u2 hi[2], lo[2];
@@ -155,7 +155,7 @@ __global__ __launch_bounds__(256) void dr_systems_kernel(DrSystems A) {
           lo[0][w] = c;
           lo[1][w] = d;
         }
-        const int at = l32 * 64 + (dr_unit_of<E>(l32, 4 * m + 2 * half) & ~1) * 8;
+        const int at = l32 * 64 + (dr_unit_of(l32, 4 * m + 2 * half) & ~1) * 8;
         const u2 h0 = odd ? hi[1] : hi[0], h1 = odd ? hi[0] : hi[1], l0 = odd ? lo[1] : lo[0], l1 = odd ? lo[0] : lo[1];
         *reinterpret_cast<u4*>(pairs + at) = u4{h0[0], h0[1], h1[0], h1[1]};
         *reinterpret_cast<u4*>(pairs + kDrTiles / 2 + at) = u4{l0[0], l0[1], l1[0], l1[1]};
@@ -163,7 +163,7 @@ __global__ __launch_bounds__(256) void dr_systems_kernel(DrSystems A) {
     } else {
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<f4*>(pairs + l32 * 128 + dr_unit_of<E>(l32, 2 * q + half) * 16) =
+        *reinterpret_cast<f4*>(pairs + l32 * 128 + dr_unit_of(l32, 2 * q + half) * 16) =
             f4{pair[4 * q], pair[4 * q + 1], pair[4 * q + 2], pair[4 * q + 3]};
     }
   }
@@ -231,7 +231,7 @@ __global__ __launch_bounds__(256) void dr_systems_kernel(DrSystems A) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) t[k][r] = col + r < row ? w[r] : 0.0f;
     }
-    const int to = dr_unit_of<E>(l32, 4 * half + 2 * m);
+    const int to = dr_unit_of(l32, 4 * half + 2 * m);
     if constexpr (sizeof(E) == 2) {
       if (to & 1) {
         const f4 x = t[0];
@@ -249,7 +249,7 @@ __global__ __launch_bounds__(256) void dr_systems_kernel(DrSystems A) {
       *reinterpret_cast<u4*>(tiles + kDrTiles / 2 + l32 * 64 + (to & ~1) * 8) = lo;
     } else {
       *reinterpret_cast<f4*>(tiles + l32 * 128 + to * 16) = t[0];
-      *reinterpret_cast<f4*>(tiles + l32 * 128 + dr_unit_of<E>(l32, 4 * half + 2 * m + 1) * 16) = t[1];
+      *reinterpret_cast<f4*>(tiles + l32 * 128 + dr_unit_of(l32, 4 * half + 2 * m + 1) * 16) = t[1];
     }
   }
   }

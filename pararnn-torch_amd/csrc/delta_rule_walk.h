@@ -53,7 +53,7 @@ struct Stored {
     return BACK ? b >= a : b <= a;
   }
   static __device__ __forceinline__ const char* at(const char* tile, int row, int col) {
-    return tile + row * kRow + dr_unit_of<E>(row, col >> 2) * kUnit + (col & 3) * ES;
+    return tile + row * kRow + dr_unit_of(row, col >> 2) * kUnit + (col & 3) * ES;
   }
   static __device__ __forceinline__ Op<M, M::kParts> get(const char* m, int rt, int f, int n, int g) {
     const char* t = m + (NC * rt / 32 + 8 * G * f / 32) * kTile;
