@@ -185,21 +185,14 @@ __global__ __launch_bounds__(256, sizeof(typename M::E) == 2 && KS == 1 ? 2 : 1)
           } else {
             *reinterpret_cast<f4*>(sP + i * RB + j0 * 4) = f4{w1[0], w1[1], w1[2], w1[3]};
           }
-          // -(X + X^T): either triangle from the one value
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int jj = j0 + r;
-            if (jj > i) continue;
-            if constexpr (kNarrow) {
-              const bf16 a = from_f32<bf16>(-x[r]), b = from_f32<bf16>(-x[r] - to_f32(a));
-              *reinterpret_cast<bf16*>(s_x[0] + i * RB + jj * 2) = a;
-              *reinterpret_cast<bf16*>(s_x[0] + jj * RB + i * 2) = a;
-              *reinterpret_cast<bf16*>(s_x[P - 1] + i * RB + jj * 2) = b;
-              *reinterpret_cast<bf16*>(s_x[P - 1] + jj * RB + i * 2) = b;
-            } else {
-              *reinterpret_cast<float*>(s_x[0] + i * RB + jj * 4) = -x[r];
-              *reinterpret_cast<float*>(s_x[0] + jj * RB + i * 4) = -x[r];
-            }
+          if constexpr (kNarrow) {
+            const u2 a{pack_bf16x2(-x[0], -x[1]), pack_bf16x2(-x[2], -x[3])};
+            const u2 b{pack_bf16x2(-x[0] - lo_bf16(a[0]), -x[1] - hi_bf16(a[0])),
+                       pack_bf16x2(-x[2] - lo_bf16(a[1]), -x[3] - hi_bf16(a[1]))};
+            *reinterpret_cast<u2*>(s_x[0] + i * RB + j0 * 2) = a;
+            *reinterpret_cast<u2*>(s_x[P - 1] + i * RB + j0 * 2) = b;
+          } else {
+            *reinterpret_cast<f4*>(s_x[0] + i * RB + j0 * 4) = f4{-x[0], -x[1], -x[2], -x[3]};
           }
         }
       } else {  // from the state before to the adjoint behind
@@ -299,8 +292,15 @@ __global__ __launch_bounds__(256, sizeof(typename M::E) == 2 && KS == 1 ? 2 : 1)
               x = one;
           }
         };
-        both([&](int p) { return row_op<M, 2>(s_x[p] + t * RB, f, half); });
-        mul<32>(du[s], kc, x);
+        // -(X + X^T), rows of X before the token and columns behind it
+        if (jt <= it) {
+          both([&](int p) { return row_op<M, 2>(s_x[p] + t * RB, f, half); });
+          mul<32>(du[s], kc, x);
+        }
+        if (jt >= it) {
+          both([&](int p) { return col_op<M, 2, RB>(s_x[p] + col_share<M, 2, RB>(lane), 16 * f, 32 * it); });
+          mul<32>(du[s], kc, x);
+        }
         if (jt <= it) {
           both([&](int p) { return row_op<M, 2>(sP + p * kSlab + t * RB, f, half); });
           mul<32>(dq[s], kc, x);

@@ -46,66 +46,81 @@ __global__ __launch_bounds__(256) void dr_join_kernel(JoinArgs A) {
   for (int r = 0; r < R; ++r)
 #pragma unroll
     for (int e = 0; e < 16; ++e) S[r][e] = ldb<float>(ri, at(r, e), 0);
-  for (int k = 0; k < u.count; ++k) {
-    const int p = first + (A.back ? u.count - 1 - k : k);
-    const size_t unit = static_cast<size_t>(p) * A.H + h;
-    const rsrc_t rp = make_rsrc(A.piece + unit * state_floats, static_cast<uint32_t>(state_floats) * 4);
-    const bool more = k + 1 < u.count;  // the last one hands on to none
-    // the transfer's operands are under way while the state is handed round
-    const float* M = A.transfer + unit * transfer_floats;
-    const rsrc_t rm = make_rsrc(M, more ? static_cast<uint32_t>(transfer_floats) * 4 : 0u);
+  // a piece's own state and the operands of its transfer (for one row tile a wave all of them, a piece
+  // ahead; the last piece hands on to none)
+  constexpr int kHeld = R == 1 ? 2 : 1;
+  struct Piece {
     u4 m[8][2];
-    auto fetch = [&](int r, int f0) {
+    f16v own[R];
+  };
+  Piece held[kHeld];
+  auto unit_of = [&](int k) { return static_cast<size_t>(first + (A.back ? u.count - 1 - k : k)) * A.H + h; };
+  auto operands = [&](Piece& x, int k, int r, int f0) {
+    const rsrc_t rm = make_rsrc(A.transfer + unit_of(k) * transfer_floats,
+                                k + 1 < u.count ? static_cast<uint32_t>(transfer_floats) * 4 : 0u);
 #pragma unroll
-      for (int f = 0; f < 8; ++f)
+    for (int f = 0; f < 8; ++f)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          m[f][e] = __builtin_amdgcn_raw_buffer_load_b128(
-              rm, la_in(f0 + f < steps, (((4 * r + wave) * steps + f0 + f) * 64 + lane) * 32 + e * 16), 0, 0);
-    };
-    fetch(0, 0);
-    f16v U[R];
+      for (int e = 0; e < 2; ++e)
+        x.m[f][e] = __builtin_amdgcn_raw_buffer_load_b128(
+            rm, la_in(f0 + f < steps, (((4 * r + wave) * steps + f0 + f) * 64 + lane) * 32 + e * 16), 0, 0);
+  };
+  auto fetch = [&](Piece& x, int k) {
+    k = min(k, u.count - 1);
+    operands(x, k, 0, 0);
+    const rsrc_t rp = make_rsrc(A.piece + unit_of(k) * state_floats,
+                                k + 1 < u.count ? static_cast<uint32_t>(state_floats) * 4 : 0u);
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) U[r][e] = more ? ldb<float>(rp, at(r, e), 0) : 0.0f;
+      for (int e = 0; e < 16; ++e) x.own[r][e] = ldb<float>(rp, at(r, e), 0);
+  };
+  auto step = [&](Piece& x, Piece& other, int k) {
+    const rsrc_t rp = make_rsrc(A.piece + unit_of(k) * state_floats, static_cast<uint32_t>(state_floats) * 4);
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int e = 0; e < 16; ++e) stb<float>(rp, at(r, e), 0, S[r][e]);
-    if (!more) break;
     __syncthreads();  // the last step's operands have been read
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int f = 0; f < 2; ++f) {
-        float x[8];
+        float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = S[r][8 * f + e];
-        const auto o = parts_of<InBf16, 3>(x);
+        for (int e = 0; e < 8; ++e) v[e] = S[r][8 * f + e];
+        const auto o = parts_of<InBf16, 3>(v);
 #pragma unroll
         for (int j = 0; j < 3; ++j)
           *reinterpret_cast<b8*>(&lds[2 * (4 * r + wave) + f][j][lane * 16]) = o.p[j];
       }
+    if (kHeld == 2) fetch(other, k + 1);
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int r = 0; r < R; ++r) {
+      f16v sum = x.own[r];
 #pragma unroll
       for (int f0 = 0; f0 < F; f0 += 8) {
-        if (r > 0 || f0 > 0) fetch(r, f0);
+        if (r > 0 || f0 > 0) operands(x, k, r, f0);
 #pragma unroll
         for (int f = 0; f < 8; ++f) {
           Op<InBf16, 3> s;
 #pragma unroll
           for (int j = 0; j < 3; ++j) s.p[j] = *reinterpret_cast<const b8*>(&lds[f0 + f][j][lane * 16]);
-          float x[8];
+          float v[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(m[f][e >> 2][e & 3]);
-          mul<32>(U[r], parts_of<InBf16, 3>(x), s);
+          for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(x.m[f][e >> 2][e & 3]);
+          mul<32>(sum, parts_of<InBf16, 3>(v), s);
         }
       }
-#pragma unroll
-    for (int r = 0; r < R; ++r) S[r] = U[r];
+      S[r] = sum;
+    }
+    if (kHeld == 1) fetch(x, k + 1);
+  };
+  fetch(held[0], 0);
+  for (int k = 0; k < u.count; k += kHeld) {
+    step(held[0], held[kHeld - 1], k);
+    if (kHeld == 2 && k + 1 < u.count) step(held[1], held[0], k + 1);
   }
 }
 
