@@ -145,7 +145,8 @@ struct DrWalk {
   void* dv;                  // backwards, dense (token, H, Dv): of the arithmetic's type
   float* dv32;               // or floats besides (heads that are summed afterwards)
   LaState init, last;
-  float *piece, *transfer;   // (piece, H, Dk, Dv), (piece, H) as operands: the pieces' own states, their transfers
+  float* piece;              // (piece, H, Dk, Dv): the pieces' own states
+  uint16_t* transfer;        // (piece, H): their transfers, as operands in three bf16 parts
   int H, Dk, Dv, dtype;
   int tiles, own_tiles;      // column tiles of a launch; of them of the state (the rest: transfers)
   float scale;

@@ -69,7 +69,8 @@ Kept kept_of(void* p, const Problem& a) {
 struct Scratch {
   char* sys;
   void *behind, *dv;
-  float *piece, *transfer;
+  float* piece;
+  uint16_t* transfer;
   float *dq32, *dk32, *dv32, *g_part;
   size_t bytes;
 };
@@ -136,7 +137,7 @@ Scratch carve(void* ws, const Problem& a, const Plan& plan, bool systems, bool b
   if (plan.cut) {
     const size_t pieces = dr_units(plan.seqs, plan.seqs.len) * heads;
     s.piece = static_cast<float*>(c.take(4 * pieces * a.la.Dk * a.la.Dv));
-    s.transfer = static_cast<float*>(c.take(4 * pieces * dr_operand_elems(a.la.Dk, a.la.Dk)));
+    s.transfer = static_cast<uint16_t*>(c.take(6 * pieces * dr_operand_elems(a.la.Dk, a.la.Dk)));
   }
   if (backward) {
     s.behind = c.take(units * heads * dr_operand_elems(a.la.Dk, a.la.Dv) * size);

@@ -15,7 +15,7 @@ namespace {
 struct JoinArgs {
   LaSeqs seqs;
   float* piece;           // in: U_p, out: S_p  (piece, H, Dk, Dv)
-  const float* transfer;  // (piece, H): operands
+  const uint16_t* transfer;  // (piece, H): operands in three parts
   LaState init;
   int H, Dk, Dv, tiles, back;
 };
@@ -33,7 +33,7 @@ __global__ __launch_bounds__(256) void dr_join_kernel(JoinArgs A) {
   if (!u.any || u.seq != seq || u.count < 2) return;
   const int col = 32 * tile + l32;
   const size_t state_floats = static_cast<size_t>(A.Dk) * A.Dv;
-  const size_t transfer_floats = dr_operand_elems(A.Dk, A.Dk);
+  const size_t elems = dr_operand_elems(A.Dk, A.Dk);
   const int steps = (A.Dk + 15) / 16;
   auto at = [&](int r, int e) {  // element of register e of row tile r of this wave
     const int i = 32 * (4 * r + wave) + 8 * (e >> 2) + 4 * half + (e & 3);
@@ -46,41 +46,54 @@ __global__ __launch_bounds__(256) void dr_join_kernel(JoinArgs A) {
   for (int r = 0; r < R; ++r)
 #pragma unroll
     for (int e = 0; e < 16; ++e) S[r][e] = ldb<float>(ri, at(r, e), 0);
-  // a piece's own state and the operands of its transfer (for one row tile a wave all of them, a piece
-  // ahead; the last piece hands on to none)
-  constexpr int kHeld = R == 1 ? 2 : 1;
-  struct Piece {
-    u4 m[8][2];
-    f16v own[R];
-  };
-  Piece held[kHeld];
-  auto unit_of = [&](int k) { return static_cast<size_t>(first + (A.back ? u.count - 1 - k : k)) * A.H + h; };
-  auto operands = [&](Piece& x, int k, int r, int f0) {
-    const rsrc_t rm = make_rsrc(A.transfer + unit_of(k) * transfer_floats,
-                                k + 1 < u.count ? static_cast<uint32_t>(transfer_floats) * 4 : 0u);
-#pragma unroll
-    for (int f = 0; f < 8; ++f)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        x.m[f][e] = __builtin_amdgcn_raw_buffer_load_b128(
-            rm, la_in(f0 + f < steps, (((4 * r + wave) * steps + f0 + f) * 64 + lane) * 32 + e * 16), 0, 0);
-  };
-  auto fetch = [&](Piece& x, int k) {
+  // A piece's own state and the operands of its transfer.  Where a wave has one tile of rows they are all
+  // in registers, each loaded for the next piece as soon as it has been used for this one.
+  constexpr bool kAhead = R == 1;
+  Op<InBf16, 3> m[8];
+  f16v own[R];
+  auto unit_of = [&](int k) {
     k = min(k, u.count - 1);
-    operands(x, k, 0, 0);
+    return static_cast<size_t>(first + (A.back ? u.count - 1 - k : k)) * A.H + h;
+  };
+  auto transfer_of = [&](int k) {  // (the last piece hands on to none)
+    return make_rsrc(A.transfer + unit_of(k) * 3 * elems, k + 1 < u.count ? static_cast<uint32_t>(elems) * 6 : 0u);
+  };
+  auto operand = [&](rsrc_t rm, int r, int f) {
+    Op<InBf16, 3> o;
+#pragma unroll
+    for (int j = 0; j < 3; ++j)
+      o.p[j] = __builtin_bit_cast(
+          b8, __builtin_amdgcn_raw_buffer_load_b128(
+                  rm, la_in(f < steps, j * static_cast<uint32_t>(elems) * 2 + (((4 * r + wave) * steps + f) * 64 + lane) * 16),
+                  0, 0));
+    return o;
+  };
+  auto state = [&](int k) {
     const rsrc_t rp = make_rsrc(A.piece + unit_of(k) * state_floats,
                                 k + 1 < u.count ? static_cast<uint32_t>(state_floats) * 4 : 0u);
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x.own[r][e] = ldb<float>(rp, at(r, e), 0);
+      for (int e = 0; e < 16; ++e) own[r][e] = ldb<float>(rp, at(r, e), 0);
   };
-  auto step = [&](Piece& x, Piece& other, int k) {
+  state(0);
+  if (kAhead) {
+    const rsrc_t rm = transfer_of(0);
+#pragma unroll
+    for (int f = 0; f < 8; ++f) m[f] = operand(rm, 0, f);
+  }
+  for (int k = 0; k < u.count; ++k) {
     const rsrc_t rp = make_rsrc(A.piece + unit_of(k) * state_floats, static_cast<uint32_t>(state_floats) * 4);
+    f16v sum[R][2];  // a matrix instruction waits for its own sum's last one
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int r = 0; r < R; ++r) {
+      sum[r][0] = own[r];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) stb<float>(rp, at(r, e), 0, S[r][e]);
+      for (int e = 0; e < 16; ++e) {
+        sum[r][1][e] = 0.0f;
+        stb<float>(rp, at(r, e), 0, S[r][e]);
+      }
+    }
     __syncthreads();  // the last step's operands have been read
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -94,33 +107,27 @@ __global__ __launch_bounds__(256) void dr_join_kernel(JoinArgs A) {
         for (int j = 0; j < 3; ++j)
           *reinterpret_cast<b8*>(&lds[2 * (4 * r + wave) + f][j][lane * 16]) = o.p[j];
       }
-    if (kHeld == 2) fetch(other, k + 1);
+    state(k + 1);
     __syncthreads();
+    const rsrc_t now = transfer_of(k), next = transfer_of(k + 1);
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      f16v sum = x.own[r];
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int f0 = 0; f0 < F; f0 += 8) {
-        if (r > 0 || f0 > 0) operands(x, k, r, f0);
+      for (int f = 0; f < F; ++f) {
+        Op<InBf16, 3> s;
 #pragma unroll
-        for (int f = 0; f < 8; ++f) {
-          Op<InBf16, 3> s;
-#pragma unroll
-          for (int j = 0; j < 3; ++j) s.p[j] = *reinterpret_cast<const b8*>(&lds[f0 + f][j][lane * 16]);
-          float v[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(x.m[f][e >> 2][e & 3]);
-          mul<32>(sum, parts_of<InBf16, 3>(v), s);
+        for (int j = 0; j < 3; ++j) s.p[j] = *reinterpret_cast<const b8*>(&lds[f][j][lane * 16]);
+        if constexpr (kAhead) {
+          mul<32>(sum[r][f & 1], m[f], s);
+          m[f] = operand(next, 0, f);
+        } else {
+          mul<32>(sum[r][f & 1], operand(now, r, f), s);
         }
       }
-      S[r] = sum;
-    }
-    if (kHeld == 1) fetch(x, k + 1);
-  };
-  fetch(held[0], 0);
-  for (int k = 0; k < u.count; k += kHeld) {
-    step(held[0], held[kHeld - 1], k);
-    if (kHeld == 2 && k + 1 < u.count) step(held[1], held[0], k + 1);
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) S[r][e] = sum[r][0][e] + sum[r][1][e];
   }
 }
 

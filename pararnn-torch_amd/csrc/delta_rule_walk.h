@@ -700,24 +700,40 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
   if (!kOwn) flush();
 
   // ---- the state behind the piece
-  float* dst = nullptr;
-  if (kOwn) {
-    dst = transfer ? A.transfer + (static_cast<size_t>(piece) * A.H + h) * dr_operand_elems(A.Dk, A.Dk)
-                   : A.piece + (static_cast<size_t>(piece) * A.H + h) * state_floats;
-  } else if (pc.index == (kBack ? 0 : pc.count - 1)) {
-    if (float* row = la_row(A.last, pc.seq, A.H * state_floats)) dst = row + h * state_floats;
-  }
-  if (dst) {
-    const rsrc_t rs = make_rsrc(
-        dst, static_cast<uint32_t>(transfer ? dr_operand_elems(A.Dk, A.Dk) : state_floats) * 4);
-    const int rows = transfer ? (A.Dk + 31) / 32 * 32 : A.Dk, cols = transfer ? (A.Dk + 15) / 16 * 16 : A.Dv;
+  if (transfer) {
+    const size_t elems = dr_operand_elems(A.Dk, A.Dk);
+    const rsrc_t rs = make_rsrc(A.transfer + (static_cast<size_t>(piece) * A.H + h) * 3 * elems,
+                                static_cast<uint32_t>(elems) * 6);
 #pragma unroll
     for (int t = 0; t < KT; ++t)
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
         const int i = NC * t + 4 * G * (r >> 2) + 4 * g + (r & 3);
-        const uint32_t at = transfer ? dr_operand_at(A.Dk, i, col) : static_cast<uint32_t>(i * A.Dv + col);
-        stb<float>(rs, la_in((i < rows) & (col < cols), at * 4), 0, S[t][r]);
+        const uint32_t at = la_in((i < (A.Dk + 31) / 32 * 32) & (col < (A.Dk + 15) / 16 * 16),
+                                  dr_operand_at(A.Dk, i, col) * 2);
+        float v = S[t][r];
+#pragma unroll
+        for (int j = 0; j < 3; ++j) {
+          stb<bf16>(rs, at, j * static_cast<uint32_t>(elems) * 2, v);
+          v -= round_to<bf16>(v);
+        }
+      }
+    return;
+  }
+  float* dst = nullptr;
+  if (kOwn) {
+    dst = A.piece + (static_cast<size_t>(piece) * A.H + h) * state_floats;
+  } else if (pc.index == (kBack ? 0 : pc.count - 1)) {
+    if (float* row = la_row(A.last, pc.seq, A.H * state_floats)) dst = row + h * state_floats;
+  }
+  if (dst) {
+    const rsrc_t rs = make_rsrc(dst, static_cast<uint32_t>(state_floats) * 4);
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        const int i = NC * t + 4 * G * (r >> 2) + 4 * g + (r & 3);
+        stb<float>(rs, la_in((i < A.Dk) & (col < A.Dv), (i * A.Dv + col) * 4), 0, S[t][r]);
       }
   }
 }
