@@ -57,7 +57,8 @@ def residual_norm(x, y, weight=None, bias=None, post_norm=False, post_weight=Non
 
 
 def beam_select(logits, scores, beams, ended=None, pad=0):
-    """Lists (score, parent, token) per search, candidate by candidate in float64."""
+    """Lists (score, parent, token) per search, candidate by candidate in float64; equal totals go to the
+    lowest beam, the larger logit, the lowest token."""
     B, K, V = logits.shape
     found = []
     for b in range(B):
@@ -65,15 +66,16 @@ def beam_select(logits, scores, beams, ended=None, pad=0):
         for k in range(K):
             s = float(scores[b, k])
             if ended is not None and ended[b, k]:
-                rows.append((-s, k, pad))
+                rows.append((-s, k, 0.0, pad))
                 continue
             x = logits[b, k].double()
             if bool(torch.isnan(x).any() | (x == float("inf")).any()):
                 continue
             p = s + torch.log_softmax(x, -1) if bool((x > float("-inf")).any()) else x
-            rows += [(-float(p[t]), k, t) for t in torch.nonzero(p > float("-inf"))[:, 0].tolist()]
+            rows += [(-float(p[t]), k, -float(x[t]), t)
+                     for t in torch.nonzero(p > float("-inf"))[:, 0].tolist()]
         rows = sorted(r for r in rows if r[0] < float("inf"))[:beams]
-        found.append([(-s, k, t) for s, k, t in rows])
+        found.append([(-s, k, t) for s, k, _, t in rows])
     return found
 
 

@@ -1,7 +1,8 @@
 // Beam search: the best continuations over beams and vocabulary.
 //
 //   total(k, t) = score_k + logits_kt - logsumexp_t(logits_kt),  the M largest of a search's K V,
-//   ties to the lowest k V + t.
+//   ties to the lowest beam, in a beam to the larger logit (a score far from zero makes totals of
+//   different logits equal), then to the lowest token.
 //
 // Two launches.  The first reads the logits once: a workgroup per beam and slice of 8192 tokens, 32
 // values a thread in registers, gives the slice's largest value, its sum of exponentials and its M
@@ -28,14 +29,15 @@ constexpr int kRound = 4;     // candidates of a thread and round of the second 
 
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
-// Order of floats as of unsigned numbers; -infinity and NaN are 0: never chosen.
+// Order of floats as of unsigned numbers, zeros of either sign alike; -infinity and NaN are 0: never
+// chosen.
 __device__ __forceinline__ uint32_t order(float v) {
-  const uint32_t b = __float_as_uint(v);
+  const uint32_t b = v == 0.0f ? 0u : __float_as_uint(v);
   if (!(v > -INFINITY)) return 0u;
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ uint64_t order(double v) {
-  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint64_t b = v == 0.0 ? 0ull : __builtin_bit_cast(uint64_t, v);
   if (!(v > -static_cast<double>(INFINITY))) return 0ull;
   return b >> 63 ? ~b : b | 1ull << 63;
 }
@@ -168,14 +170,17 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs A) {
     A.slices[at] = Slice{(s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]), bad ? NAN : most, min(n, A.M)};
 }
 
-// A candidate of the second launch: the order of its total, its place k V + t.
-struct __align__(16) Total {
+// A candidate of the second launch: the orders of its total and, turned, of its logit, its beam and
+// token.
+struct Total {
   uint64_t o;
-  uint32_t t, none;
+  uint32_t k, low, t;
 };
 __device__ __forceinline__ bool before(const Total& a, const Total& b) {
-  return a.o > b.o || (a.o == b.o && a.t < b.t);
+  const uint64_t x = static_cast<uint64_t>(a.k) << 32 | a.low, y = static_cast<uint64_t>(b.k) << 32 | b.low;
+  return a.o > b.o || (a.o == b.o && (x < y || (x == y && a.t < b.t)));
 }
+constexpr Total kNoTotal{0, ~0u, ~0u, ~0u};
 
 __global__ __launch_bounds__(256) void beam_choose_kernel(BeamArgs A) {
   __shared__ Total s_top[256], s_list[kMost * kRound + kMost], s_carry[kMost], s_bound[4];
@@ -218,16 +223,16 @@ __global__ __launch_bounds__(256) void beam_choose_kernel(BeamArgs A) {
     __syncthreads();
     const long long end = static_cast<long long>(min(A.K, k0 + kMost)) * per;
     for (long long base = static_cast<long long>(k0) * per; base < end; base += 256 * kRound) {
-      Total c[kRound], top{0, ~0u, 0};
+      Total c[kRound], top = kNoTotal;
 #pragma unroll
       for (int i = 0; i < kRound; ++i) {
         const long long at = base + i * 256 + tid;
-        c[i] = Total{0, ~0u, 0};
+        c[i] = kNoTotal;
         if (at >= end) continue;
         const int k = static_cast<int>(at / per), in = static_cast<int>(at - static_cast<long long>(k) * per);
         const int row = b * A.K + k;
         if (A.ended && A.ended[row]) {  // goes on as it is, with one token
-          if (in == 0) c[i] = Total{order(s_off[k - k0]), static_cast<uint32_t>(k) * A.V + A.pad, 0};
+          if (in == 0) c[i] = Total{order(s_off[k - k0]), static_cast<uint32_t>(k), 0, static_cast<uint32_t>(A.pad)};
         } else {
           const int s = in / A.M, r = in - s * A.M;
           const size_t slice = static_cast<size_t>(row) * A.S + s;
@@ -235,12 +240,12 @@ __global__ __launch_bounds__(256) void beam_choose_kernel(BeamArgs A) {
           const float logit = __uint_as_float(best.x & 0x80000000u ? best.x & 0x7fffffffu : ~best.x);
           if (r < A.slices[slice].count)
             c[i] = Total{order((static_cast<double>(logit) - s_most[k - k0]) + s_off[k - k0]),
-                         static_cast<uint32_t>(k) * A.V + best.y, 0};
+                         static_cast<uint32_t>(k), ~best.x, best.y};
         }
         if (c[i].o && before(c[i], top)) top = c[i];
       }
       s_top[tid] = top;
-      if (tid < 4) s_bound[tid] = Total{1, ~0u, 0};
+      if (tid < 4) s_bound[tid] = Total{1, ~0u, ~0u, ~0u};
       const int held = s_held;
       for (int i = tid; i < held; i += 256) s_list[i] = s_carry[i];
       if (tid == 0) s_count = held;
@@ -279,8 +284,8 @@ __global__ __launch_bounds__(256) void beam_choose_kernel(BeamArgs A) {
     const bool any = i < held;
     const size_t at = static_cast<size_t>(b) * A.M + i;
     A.out_scores[at] = any ? static_cast<float>(value(s_carry[i].o)) : -INFINITY;
-    A.out_parents[at] = any ? static_cast<int>(s_carry[i].t / A.V) : -1;
-    A.out_tokens[at] = any ? static_cast<int>(s_carry[i].t % A.V) : -1;
+    A.out_parents[at] = any ? static_cast<int>(s_carry[i].k) : -1;
+    A.out_tokens[at] = any ? static_cast<int>(s_carry[i].t) : -1;
   }
 }
 

@@ -22,8 +22,8 @@ def beam_select(logits: Tensor, scores: Tensor, *, beams: int | None = None,
     ``logits`` ``(B, K, V)`` float32, bfloat16 or float16, ``scores`` ``(B, K)`` float32, the beams'
     totals so far (``-inf``: a beam that is not there, as all but the first at a search's start).
     Returns ``(scores, parents, tokens)``, each ``(B, beams)`` (``K`` of them by default, at most 128),
-    the largest total first, float32, int32 and int32.  Ties go to the lowest beam, then the lowest
-    token; totals are formed and compared in float64.  Where fewer candidates are left, the rest are
+    the largest total first, float32, int32 and int32.  Totals are formed and compared in float64;
+    ties go to the lowest beam, in a beam to the larger logit, then to the lowest token.  Where fewer candidates are left, the rest are
     ``-inf``, -1 and -1.  A logit of ``-inf`` is masked; a beam whose logits hold NaN or ``+inf``
     proposes nothing.
 
