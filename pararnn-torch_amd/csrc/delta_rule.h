@@ -148,6 +148,7 @@ struct DrWalk {
   float* piece;              // (piece, H, Dk, Dv): the pieces' own states
   uint16_t* transfer;        // (piece, H): their transfers, as operands in three bf16 parts
   int H, Dk, Dv, dtype;
+  int group;                 // waves of a workgroup (dr_walk_group)
   int tiles, own_tiles;      // column tiles of a launch; of them of the state (the rest: transfers)
   float scale;
 };
@@ -177,18 +178,14 @@ int dr_walk_f32(const DrWalk& a, DrKind kind, hipStream_t stream);
 int dr_join(const DrWalk& a, bool back, hipStream_t stream);
 int dr_grad(const DrGrad& a, bool bf16, hipStream_t stream);
 
-// How a walk covers columns of the state: workgroups of `group` waves of `cols` columns each.
-struct DrCover {
-  int group, tiles;
-};
-inline DrCover dr_walk_cols(int Dk, int Dv, int cols, bool bf16) {
-  int group = 4;  // waves of a workgroup
-  if (!bf16)
-    group = Dk <= 128 ? 4 : 2;
-  else if (Dk <= 128 && (cols == 32 ? Dv <= 64 : Dv <= 32))
-    group = 2;
-  const int tiles = (Dv + cols * group - 1) / (cols * group);
-  return DrCover{group, tiles};
+// Waves of a walk's workgroup, `cols` columns each.  items: (piece, head) pairs.  Narrow values have two
+// column tiles' waves at most; and where there is a CU for each half of a workgroup, halves (D = 64, 128
+// sequences' heads: 99 us forwards, 112 whole; 350 pieces: 155 us, 117 whole).
+inline int dr_walk_group(int Dk, int Dv, int cols, bool bf16, long long items) {
+  if (!bf16) return Dk <= 128 ? 4 : 2;
+  if (Dk > 128) return 4;
+  if (cols == 32) return Dv <= 64 ? 2 : 4;
+  return Dv <= 32 || (Dk <= 64 && items * ((Dv + 31) / 32) <= 256) ? 2 : 4;
 }
 
 }  // namespace prnn

@@ -99,7 +99,7 @@ Plan plan(const Problem& a) {
   Plan p{16, sequences_of(a), false};
   const long long longest = a.la.cu_seqlens && a.la.longest > 0 ? std::min(a.la.longest, a.la.T) : a.la.T;
   const long long chunks = (longest + kDrC - 1) / kDrC, tokens = 1ll * a.la.B * a.la.T;
-  const int group_cols = dr_walk_cols(a.la.Dk, a.la.Dv, 16, on_bf16(a)).group * 16;
+  const int group_cols = dr_walk_group(a.la.Dk, a.la.Dv, 16, on_bf16(a), 1 << 20) * 16;
   const double tiles = (a.la.Dv + group_cols - 1) / group_cols;
   // of a packed batch half the tokens are taken to be in sequences that are cut
   const double own = (tiles + (a.la.Dk + group_cols - 1) / group_cols) * (a.la.cu_seqlens ? 0.5 : 1.0);
@@ -199,12 +199,12 @@ DrWalk walk_of(const Problem& a, const Plan& plan, const Scratch& s, const char*
 }
 int run(DrWalk w, DrKind kind, const Problem& a, const Plan& plan, hipStream_t st) {
   const bool own = kind == kDrState || kind == kDrAdjoint;
-  w.own_tiles = dr_walk_cols(a.la.Dk, a.la.Dv, plan.cols, on_bf16(a)).tiles;
-  w.tiles = w.own_tiles;
-  if (own) {
-    const int cols = dr_walk_cols(a.la.Dk, a.la.Dv, plan.cols, on_bf16(a)).group * plan.cols;
-    w.tiles += (a.la.Dk + cols - 1) / cols;
-  }
+  // (pieces' own states have the transfers' columns besides)
+  const long long items = dr_units(plan.seqs, plan.seqs.len) * a.la.H * (own ? 2 : 1);
+  w.group = dr_walk_group(a.la.Dk, a.la.Dv, plan.cols, on_bf16(a), items);
+  const int cols = w.group * plan.cols;
+  w.own_tiles = (a.la.Dv + cols - 1) / cols;
+  w.tiles = w.own_tiles + (own ? (a.la.Dk + cols - 1) / cols : 0);
   return on_bf16(a) ? dr_walk_bf16(w, kind, plan.cols, st) : dr_walk_f32(w, kind, st);
 }
 // The walk of a direction; of a cut sequence the pieces' own states and the join before it.

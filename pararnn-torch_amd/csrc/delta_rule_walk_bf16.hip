@@ -6,14 +6,13 @@ namespace {
 
 template <int KIND, int KD>
 int launch_cols(const DrWalk& a, int cols, hipStream_t stream) {
-  const int group = dr_walk_cols(a.Dk, a.Dv, cols, true).group;
   // Waves that only load: not for pieces' own states, of which two workgroups a CU run without (D = 128,
   // 512 of them: 74 us, 87 with), nor where two chunks do not fit LDS.
   constexpr int kLoad = KD <= 128 && KIND != kDrState && KIND != kDrAdjoint ? 4 : 0;
-  if (cols == 16 && group == 4) return dr_launch_walk<InBf16, 16, KD, 4, kLoad, KIND>(a, stream);
+  if (cols == 16 && a.group == 4) return dr_launch_walk<InBf16, 16, KD, 4, kLoad, KIND>(a, stream);
   if constexpr (KD <= 128) {
     if (cols == 16) return dr_launch_walk<InBf16, 16, KD, 2, kLoad, KIND>(a, stream);
-    if (group == 4) return dr_launch_walk<InBf16, 32, KD, 4, 0, KIND>(a, stream);
+    if (a.group == 4) return dr_launch_walk<InBf16, 32, KD, 4, 0, KIND>(a, stream);
     if constexpr (KD <= 64) return dr_launch_walk<InBf16, 32, KD, 2, 0, KIND>(a, stream);
   }
   return fail(PRNN_ERR_RUNTIME, "no walk of %d columns a wave for keys of %d", cols, a.Dk);
