@@ -30,7 +30,7 @@ __global__ __launch_bounds__(256, sizeof(typename M::E) == 2 && KS == 1 ? 2 : 1)
   __shared__ __align__(16) char lds[(WIDE ? 4 + P : 4) * kSlab], s_x[P][kSlab];
   __shared__ float sF[kDrC * kLf], s_in[8][kDrC], s_out[8][kDrC];
   __shared__ __align__(16) float sw[kDrW * 64];
-  __shared__ float s_through, s_own[kDrC], s_into[kDrC], s_waves[4];
+  __shared__ float s_through[4], s_own[kDrC], s_into[kDrC], s_waves[4];
   char *const sK = lds, *const sQ = lds + kSlab, *const sG = lds + 2 * kSlab, *const sD = lds + 3 * kSlab;
   char* const sP = WIDE ? lds + 4 * kSlab : sG;  // the pairs go u^T, by parts
   const int h = blockIdx.x % A.H, id = blockIdx.x / A.H;
@@ -63,6 +63,23 @@ __global__ __launch_bounds__(256, sizeof(typename M::E) == 2 && KS == 1 ? 2 : 1)
   ka.fetch(pk, A.k.st, n, last_k, A.Dk, A.dtype);
   kb.fetch(pq, A.q.st, n, last_k, A.Dk, A.dtype);
   const float* weights = reinterpret_cast<const float*>(A.sys + unit * kDrSys + 2 * kDrTiles);
+  // operands of a wave's tiles of the states and of its tokens' e; the pairs' earlier tokens are the same
+  // (waves 0 and 1: the first 32, wave 2: the others)
+  const int kt = wave & 1, it = wave >> 1, t = 32 * it + l32;
+  Op<M, 1> ei[kAt], S[KS][kAt], R[KS][kAt];
+  auto fetch = [&](int p0, int v0, int f0) {
+#pragma unroll
+    for (int f = 0; f < kAt; ++f) {
+      const int step = v0 / 16 + f0 + f;
+      ei[f] = global_op<M>(re, step < vs, it * vs + step);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const int tile = p0 / 32 + 2 * s + kt;
+        S[s][f] = global_op<M>(rS, (step < vs) & (32 * tile < A.Dk), tile * vs + step);
+        R[s][f] = global_op<M>(rR, (step < vs) & (32 * tile < A.Dk), tile * vs + step);
+      }
+    }
+  };
   for (int i = tid; i < kDrW * 64; i += 256) sw[i] = weights[i];
   ga.template put<RB>(sG, A.dtype);
   gb.template put<RB>(sD, kCode);
@@ -71,8 +88,8 @@ __global__ __launch_bounds__(256, sizeof(typename M::E) == 2 && KS == 1 ? 2 : 1)
 
   // pairs of the wave's tile; state products of its tile of every slab
   const int pi = wave > 0, pj = wave > 1, i = 32 * pi + l32;
-  const int kt = wave & 1, it = wave >> 1, t = 32 * it + l32;
   f16v GU, DU, QK, KK;
+  float through = 0.0f;
 #pragma unroll
   for (int r = 0; r < 16; ++r) GU[r] = DU[r] = QK[r] = KK[r] = 0.0f;
 
@@ -100,26 +117,12 @@ __global__ __launch_bounds__(256, sizeof(typename M::E) == 2 && KS == 1 ? 2 : 1)
         ga.template put<RB>(sG, A.dtype);
         gb.template put<RB>(sD, kCode);
       }
-      Op<M, 1> ei[kAt], S[KS][kAt], R[KS][kAt];
-      auto fetch = [&](int f0) {
-#pragma unroll
-        for (int f = 0; f < kAt; ++f) {
-          const int step = v0 / 16 + f0 + f;
-          ei[f] = global_op<M>(re, step < vs, it * vs + step);
-#pragma unroll
-          for (int s = 0; s < KS; ++s) {
-            const int tile = p0 / 32 + 2 * s + kt;
-            S[s][f] = global_op<M>(rS, (step < vs) & (32 * tile < A.Dk), tile * vs + step);
-            R[s][f] = global_op<M>(rR, (step < vs) & (32 * tile < A.Dk), tile * vs + step);
-          }
-        }
-      };
-      fetch(0);
+      fetch(p0, v0, 0);
       __syncthreads();
       // under the operands' way: pairs of what is in LDS
       if (p0 == 0 && v0 == 0 && wave < 3) keys();
       for (int f0 = 0; f0 < 4; f0 += kAt) {
-        if (f0 > 0) fetch(f0);
+        if (f0 > 0) fetch(p0, v0, f0);
 #pragma unroll
         for (int f = 0; f < kAt; ++f) {
           const auto gi = row_op<M, 2>(sG + t * RB, f0 + f, half), di = row_op<M, 2>(sD + t * RB, f0 + f, half);
@@ -130,19 +133,24 @@ __global__ __launch_bounds__(256, sizeof(typename M::E) == 2 && KS == 1 ? 2 : 1)
             mul<32>(ds[s], S[s][f], di);
           }
         }
-      }
-      if (p0 == 0 && wave < 3) {
-        for (int f0 = 0; f0 < 4; f0 += kAt) {
-          Op<M, 1> ej[kAt];
+        // from the state before to the adjoint behind: two waves have the same operands, a step each
 #pragma unroll
-          for (int f = 0; f < kAt; ++f) {
-            const int step = v0 / 16 + f0 + f;
-            ej[f] = global_op<M>(re, step < vs, pj * vs + step);
+        for (int f = 0; f < kAt; ++f) {
+          if (((f0 + f) & 1) != it) continue;
+#pragma unroll
+          for (int s = 0; s < KS; ++s) {
+            float x[8], y[8];
+            values(S[s][f], x);
+            values(R[s][f], y);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) through = fmaf(x[e], y[e], through);
           }
+        }
+        if (p0 == 0 && wave < 3) {
 #pragma unroll
           for (int f = 0; f < kAt; ++f) {
-            mul<32>(GU, ej[f], row_op<M, 2>(sG + i * RB, f0 + f, half));
-            mul<32>(DU, ej[f], row_op<M, 2>(sD + i * RB, f0 + f, half));
+            mul<32>(GU, ei[f], row_op<M, 2>(sG + i * RB, f0 + f, half));
+            mul<32>(DU, ei[f], row_op<M, 2>(sD + i * RB, f0 + f, half));
           }
         }
       }
@@ -195,28 +203,6 @@ __global__ __launch_bounds__(256, sizeof(typename M::E) == 2 && KS == 1 ? 2 : 1)
             *reinterpret_cast<f4*>(s_x[0] + i * RB + j0 * 4) = f4{-x[0], -x[1], -x[2], -x[3]};
           }
         }
-      } else {  // from the state before to the adjoint behind
-        float d = 0.0f;
-        const int ops = static_cast<int>(dr_operand_elems(A.Dk, A.Dv) / 512);
-        for (int o = 0; o < ops; o += 2 * kAt) {
-          Op<M, 1> a[2 * kAt], b[2 * kAt];
-#pragma unroll
-          for (int k = 0; k < 2 * kAt; ++k) {
-            a[k] = global_op<M>(rS, o + k < ops, o + k);
-            b[k] = global_op<M>(rR, o + k < ops, o + k);
-          }
-#pragma unroll
-          for (int k = 0; k < 2 * kAt; ++k) {
-            float x[8], y[8];
-            values(a[k], x);
-            values(b[k], y);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) d = fmaf(x[e], y[e], d);
-          }
-        }
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) d += __shfl_xor(d, m);
-        if (lane == 0) s_through = d * sw[kWmeta * 64];
       }
       __syncthreads();
     }
@@ -235,7 +221,8 @@ __global__ __launch_bounds__(256, sizeof(typename M::E) == 2 && KS == 1 ? 2 : 1)
         kb.template put<RB>(sQ, A.dtype);
         __syncthreads();
       }
-      if (c0 + 32 * kt >= A.Dk) continue;
+      const bool any = c0 + 32 * kt < A.Dk;
+      if (any) {
       float in_sum = 0.0f, out_sum = 0.0f;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
@@ -310,6 +297,7 @@ __global__ __launch_bounds__(256, sizeof(typename M::E) == 2 && KS == 1 ? 2 : 1)
           mul<32>(du[s], col_op<M, 2, RB>(qat, 16 * f, 0), x);
         }
       }
+      }
       auto out = [&](void* p, int f32, const f16v& v) {
         const int size = f32 ? 4 : TS;
         const rsrc_t r = make_rsrc(static_cast<char*>(p) + (tok0 * A.H + h) * A.Dk * size, 0x7fffffffu);
@@ -317,11 +305,6 @@ __global__ __launch_bounds__(256, sizeof(typename M::E) == 2 && KS == 1 ? 2 : 1)
         for (int q = 0; q < 4; ++q) {
           const int col = c0 + 32 * kt + 8 * q + 4 * half;
           const uint32_t to = (t * A.H * A.Dk + col) * size;
-          if (kNarrow && !f32) {
-            __builtin_amdgcn_raw_buffer_store_b64(
-                u2{pack_bf16x2(v[4 * q], v[4 * q + 1]), pack_bf16x2(v[4 * q + 2], v[4 * q + 3])}, r,
-                la_in((t < n) & (col < A.Dk), to), 0, 0);
-          } else {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const uint32_t one = la_in((t < n) & (col + e < A.Dk), to + e * size);
@@ -332,14 +315,44 @@ __global__ __launch_bounds__(256, sizeof(typename M::E) == 2 && KS == 1 ? 2 : 1)
               else
                 stb<bf16>(r, one, 0, v[4 * q + e]);
             }
-          }
         }
       };
-      out(A.dq, A.q_f32, dq[s]);
-      out(A.dk, A.k_f32, du[s]);
+      if constexpr (kNarrow) {
+        // bf16 rows leave by way of LDS, 16 bytes a lane side by side: 8 bytes of 64 tokens an instruction
+        // took 2900 cycles of a workgroup's 28800
+        auto put = [&](char* to, const f16v& v) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<u2*>(to + t * RB + (32 * kt + 8 * q + 4 * half) * 2) =
+                u2{pack_bf16x2(v[4 * q], v[4 * q + 1]), pack_bf16x2(v[4 * q + 2], v[4 * q + 3])};
+        };
+        __syncthreads();  // k and q have been read
+        if (any && !A.q_f32) put(sQ, dq[s]);
+        if (any && !A.k_f32) put(sK, du[s]);
+        __syncthreads();
+        auto rows_out = [&](void* p, const char* from) {
+          const rsrc_t r = make_rsrc(static_cast<char*>(p) + (tok0 * A.H + h) * A.Dk * 2, 0x7fffffffu);
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const int row = (tid + 256 * k) >> 3, unit = tid & 7, col = c0 + 8 * unit;
+            __builtin_amdgcn_raw_buffer_store_b128(*reinterpret_cast<const u4*>(from + row * RB + unit * 16), r,
+                                                   la_in((row < n) & (col < A.Dk), (row * A.H * A.Dk + col) * 2), 0, 0);
+          }
+        };
+        if (!A.q_f32) rows_out(A.dq, sQ);
+        if (!A.k_f32) rows_out(A.dk, sK);
+        if (any && A.q_f32) out(A.dq, 1, dq[s]);
+        if (any && A.k_f32) out(A.dk, 1, du[s]);
+      } else if (any) {
+        out(A.dq, A.q_f32, dq[s]);
+        out(A.dk, A.k_f32, du[s]);
+      }
     }
   }
   if (!A.dg && !A.g_part && !A.dbeta) return;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) through += __shfl_xor(through, m);
+  if (lane == 0) s_through[wave] = through;
   __syncthreads();
 
   // ---- 3: four lanes per token, a quarter of the others' each
@@ -350,7 +363,8 @@ __global__ __launch_bounds__(256, sizeof(typename M::E) == 2 && KS == 1 ? 2 : 1)
 #pragma unroll
     for (int x = 15; x >= 0; --x) {
       const int l = 16 * part + x;
-      sum += l > tok ? sF[tok * kLf + l] : 0.0f;
+      const float flow = sF[tok * kLf + l];
+      sum += l > tok ? flow : 0.0f;
       m[x] = sum;
     }
     for (int k = 0; k < tiles; ++k) out += s_out[k][tok];
@@ -360,7 +374,7 @@ __global__ __launch_bounds__(256, sizeof(typename M::E) == 2 && KS == 1 ? 2 : 1)
 #pragma unroll
     for (int x = 0; x < 16; ++x) {
       const int l = 16 * part + x;
-      if (l > tok) sF[tok * kLf + l] = rate * (after + m[x]);
+      sF[tok * kLf + l] = rate * (after + m[x]);  // (up to l = tok: not read)
     }
     if (wave == 3) {  // what the tokens from one on read of the state before
       float into = 0.0f;
@@ -370,7 +384,7 @@ __global__ __launch_bounds__(256, sizeof(typename M::E) == 2 && KS == 1 ? 2 : 1)
         const float o = __shfl_down(into, m);
         if (lane + m < 64) into += o;
       }
-      s_into[lane] = into + s_through;
+      s_into[lane] = into + ((s_through[0] + s_through[1]) + (s_through[2] + s_through[3])) * sw[kWmeta * 64];
     }
     if (A.dbeta && part == 0 && tok < n) {
       const float d = after + m[0] + s_own[tok];
@@ -390,7 +404,8 @@ __global__ __launch_bounds__(256, sizeof(typename M::E) == 2 && KS == 1 ? 2 : 1)
 #pragma unroll
   for (int x = 0; x < 16; ++x) {
     const int j = 16 * part + x;
-    F += j < tok ? sF[j * kLf + tok] : 0.0f;
+    const float flow = sF[j * kLf + tok];
+    F += j < tok ? flow : 0.0f;
   }
   F += __shfl_xor(F, 1);
   F += __shfl_xor(F, 2);
