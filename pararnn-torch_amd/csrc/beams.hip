@@ -25,7 +25,7 @@ constexpr int kMost = 128;     // candidates that are wanted
 constexpr int kEach = 32;      // tokens of a thread
 constexpr int kSlice = 256 * kEach;
 constexpr int kFew = 32;       // up to which a bound is a wave's
-constexpr int kRound = 4;     // candidates of a thread and round of the second launch
+constexpr int kRound = 2;     // candidates of a thread and round of the second launch
 
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
@@ -77,55 +77,57 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs A) {
   const int b = row / A.K, k = row - b * A.K;
   if (A.ended && A.ended[row]) return;
   const T* p = static_cast<const T*>(A.logits) + b * A.sb + k * A.sk;
-  // units of 16 bytes as memory has them; the row starts `skip` values into the first
+  // units of 16 bytes as memory has them; the row starts `skip` values into the first.  All loads go out
+  // together (in branches they came one after another): units behind the row lie behind the buffer, and
+  // what else is in its first and last one is taken out afterwards.
   const int skip = static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
+  const int first_token = slice * kSlice - skip;
+  const long long bytes = (static_cast<long long>(A.V) - first_token) * static_cast<long long>(sizeof(T));
+  const rsrc_t row_part =
+      make_rsrc(p + first_token, static_cast<uint32_t>(min(max(bytes, 0ll), static_cast<long long>(kSlice * sizeof(T))) + 15) & ~15u);
+  u4 raw[kEach / V];
+#pragma unroll
+  for (int u = 0; u < kEach / V; ++u)
+    raw[u] = __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(row_part, (u * 256 + tid) * 16, 0, 0));
   float v[kEach];
-  bool broken = false;
 #pragma unroll
-  for (int u = 0; u < kEach / V; ++u) {
-    const int t0 = slice * kSlice + (u * 256 + tid) * V - skip;
-    if (t0 >= 0 && t0 + V <= A.V) {
-      const u4 w = *reinterpret_cast<const u4*>(p + t0);
+  for (int u = 0; u < kEach / V; ++u)
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        if constexpr (sizeof(T) == 4)
-          v[u * V + i] = __uint_as_float(w[i]);
-        else
-          v[u * V + i] = i & 1 ? Narrow<T>::hi(w[i / 2]) : Narrow<T>::lo(w[i / 2]);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        v[u * V + i] = t0 + i >= 0 && t0 + i < A.V ? to_f32(p[t0 + i]) : -INFINITY;
+    for (int i = 0; i < V; ++i) {
+      if constexpr (sizeof(T) == 4)
+        v[u * V + i] = __uint_as_float(raw[u][i]);
+      else
+        v[u * V + i] = i & 1 ? Narrow<T>::hi(raw[u][i / 2]) : Narrow<T>::lo(raw[u][i / 2]);
     }
+  auto token = [&](int i) { return first_token + ((i / V) * 256 + tid) * V + i % V; };
+  if (first_token < 0 || first_token + kSlice > A.V) {
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      if (token(i) < 0 || token(i) >= A.V) v[i] = -INFINITY;
   }
-  float most = -INFINITY;
-  auto token = [&](int i) { return slice * kSlice + ((i / V) * 256 + tid) * V - skip + i % V; };
-  uint32_t first = 0;  // order and place of this thread's largest, the lowest token of equals
+  // this thread's largest, the lowest token of equals; NaN is found by the sum of exponentials
+  float most = v[0];
+#pragma unroll
+  for (int i = 1; i < kEach; ++i) most = fmaxf(most, v[i]);
   int place = 0;
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) {
-    broken |= !(v[i] < INFINITY);  // NaN or infinity
-    most = fmaxf(most, v[i]);
-    const uint32_t o = order(v[i]);
-    place = o > first ? token(i) : place;
-    first = o > first ? o : first;
-  }
-  const uint64_t top = first ? static_cast<uint64_t>(first) << 32 | static_cast<uint32_t>(~place) : 0ull;
+  for (int i = kEach - 1; i >= 0; --i) place = v[i] == most ? i : place;
+  const uint32_t first = order(most);
+  const uint64_t top = first ? static_cast<uint64_t>(first) << 32 | static_cast<uint32_t>(~(first_token + ((place / V) * 256 + tid) * V + place % V)) : 0ull;
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) most = fmaxf(most, __shfl_xor(most, m));
-  if (__any(broken)) most = INFINITY;
   s_top[tid] = top;
   if ((tid & 63) == 0) s_most[tid >> 6] = most;
   if (tid < 4) s_bound[tid] = 1;
   if (tid == 0) s_count = 0;
   __syncthreads();
   most = fmaxf(fmaxf(s_most[0], s_most[1]), fmaxf(s_most[2], s_most[3]));
-  const bool none = most == -INFINITY, bad = most == INFINITY;
+  const bool none = !(most > -INFINITY);
   float part = 0.0f;
-  if (!none && !bad) {
+  {
+    const float from = none ? 0.0f : most;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) part += fexp(v[i] - most);
+    for (int i = 0; i < kEach; ++i) part += fexp(v[i] - from);  // NaN of an infinity too
   }
   double sum = part;
 #pragma unroll
@@ -147,11 +149,14 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs A) {
   uint64_t bound = s_bound[0];
 #pragma unroll
   for (int w = 1; w < 4; ++w) bound = s_bound[w] > bound ? s_bound[w] : bound;
+  const uint32_t lowest = static_cast<uint32_t>(bound >> 32);
+  const float least = lowest == 0 ? -INFINITY : __uint_as_float(lowest & 0x80000000u ? lowest & 0x7fffffffu : ~lowest);
   if (top >= bound) {
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
+      if (!(v[i] >= least)) continue;
       const uint32_t o = order(v[i]);
-      if (o < static_cast<uint32_t>(bound >> 32) || o == 0) continue;
+      if (o == 0) continue;
       const uint64_t key = static_cast<uint64_t>(o) << 32 | static_cast<uint32_t>(~token(i));
       if (key >= bound) s_list[atomicAdd(&s_count, 1)] = key;
     }
@@ -166,86 +171,115 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs A) {
     if (rank < A.M)
       A.best[at * A.M + rank] = make_uint2(static_cast<uint32_t>(o >> 32), ~static_cast<uint32_t>(o));
   }
-  if (tid == 0)
-    A.slices[at] = Slice{(s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]), bad ? NAN : most, min(n, A.M)};
+  if (tid == 0) {
+    const double all = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+    A.slices[at] = Slice{all, all - all == 0.0 ? most : NAN, min(n, A.M)};
+  }
 }
 
-// A candidate of the second launch: the orders of its total and, turned, of its logit, its beam and
-// token.
+// A candidate of the second launch: the order of its total; its beam and, turned, its logit's order; its
+// token.  Compared without branches (with them 32 choices among 448 took 21 us, 11 without).
 struct Total {
-  uint64_t o;
-  uint32_t k, low, t;
+  uint64_t o, place;
+  uint32_t t;
 };
-__device__ __forceinline__ bool before(const Total& a, const Total& b) {
-  const uint64_t x = static_cast<uint64_t>(a.k) << 32 | a.low, y = static_cast<uint64_t>(b.k) << 32 | b.low;
-  return a.o > b.o || (a.o == b.o && (x < y || (x == y && a.t < b.t)));
+__device__ __forceinline__ Total total(double v, int k, uint32_t low, uint32_t t) {
+  return Total{order(v), static_cast<uint64_t>(static_cast<uint32_t>(k)) << 32 | low, t};
 }
-constexpr Total kNoTotal{0, ~0u, ~0u, ~0u};
+__device__ __forceinline__ bool before(const Total& a, const Total& b) {
+  return (a.o > b.o) | ((a.o == b.o) & ((a.place < b.place) | ((a.place == b.place) & (a.t < b.t))));
+}
+constexpr Total kNoTotal{0, ~0ull, ~0u};
 
 __global__ __launch_bounds__(256) void beam_choose_kernel(BeamArgs A) {
   __shared__ Total s_top[256], s_list[kMost * kRound + kMost], s_carry[kMost], s_bound[4];
   __shared__ int s_count, s_held;
   __shared__ double s_off[kMost], s_most[kMost];  // a total is (logit - most) + off
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, b = blockIdx.x;
-  const int per = A.S * A.M;  // candidates of a beam
+  const int per = A.S * A.M;  // candidates of a beam; all of kMost beams' are below 2^26
   const bool few = A.M <= kFew;
   if (tid == 0) s_held = 0;
   // score - log(sum), beams in blocks of kMost, a beam a wave; the largest logit stays apart (masks of
   // the type's lowest value would swallow the logarithm)
   for (int k0 = 0; k0 < A.K; k0 += kMost) {
     __syncthreads();
-    for (int k = k0 + wave; k < min(A.K, k0 + kMost); k += 4) {
-      const int row = b * A.K + k;
-      double off = A.scores[row], most = -static_cast<double>(INFINITY);
-      if (!(A.ended && A.ended[row])) {
-        const Slice* x = A.slices + static_cast<size_t>(row) * A.S;
-        float top = -INFINITY;
-        bool bad = false;
-        double sum = 0.0;
-        for (int s = lane; s < A.S; s += 64) {
-          bad |= x[s].most != x[s].most;
-          top = fmaxf(top, x[s].most);
+    const int end = min(A.K - k0, kMost) * per;
+    // a round's candidates, the first ones under way while the totals' shares are formed
+    uint2 best[kRound];
+    int beam[kRound];  // -1: none
+    bool over[kRound]; // goes on as it is, with one token
+    auto load = [&](int base) {
+      int count[kRound], rank[kRound];
+#pragma unroll
+      for (int i = 0; i < kRound; ++i) {
+        const int at = min(base + i * 256 + tid, end - 1);
+        const int k = at / per, in = at - k * per, s = in / A.M;
+        const int row = b * A.K + k0 + k;
+        const size_t slice = static_cast<size_t>(row) * A.S + s;
+        rank[i] = in - s * A.M;
+        over[i] = A.ended && A.ended[row];
+        best[i] = A.best[slice * A.M + rank[i]];
+        count[i] = A.slices[slice].count;
+        if (over[i]) {
+          rank[i] = in;
+          count[i] = 1;
         }
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
-        for (int s = lane; s < A.S; s += 64)
-          if (x[s].sum > 0.0) sum += x[s].sum * exp(static_cast<double>(x[s].most) - top);
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m);
-        most = top;
-        off = __any(bad) ? -static_cast<double>(INFINITY) : off - log(sum);
+        beam[i] = k;
       }
-      if (lane == 0) {
-        s_off[k - k0] = off;
-        s_most[k - k0] = most;
+#pragma unroll
+      for (int i = 0; i < kRound; ++i)
+        if (base + i * 256 + tid >= end || rank[i] >= count[i]) beam[i] = -1;
+    };
+    for (int base = 0; base < end; base += 256 * kRound) {
+      load(base);
+      if (base == 0) {
+        for (int k = k0 + wave; k < min(A.K, k0 + kMost); k += 4) {
+          const int row = b * A.K + k;
+          double off = A.scores[row], most = -static_cast<double>(INFINITY);
+          if (!(A.ended && A.ended[row])) {
+            const Slice* x = A.slices + static_cast<size_t>(row) * A.S;
+            Slice own = lane < A.S ? x[lane] : Slice{0.0, -INFINITY, 0};
+            float top = own.most;
+            bool bad = top != top;
+            double sum = 0.0;
+            for (int s = lane + 64; s < A.S; s += 64) {
+              bad |= x[s].most != x[s].most;
+              top = fmaxf(top, x[s].most);
+            }
+#pragma unroll
+            for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
+            for (int s = lane;; own = x[s]) {
+              if (own.sum > 0.0) sum += own.sum * exp(static_cast<double>(own.most) - top);
+              if ((s += 64) >= A.S) break;
+            }
+#pragma unroll
+            for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m);
+            most = top;
+            off = __any(bad) ? -static_cast<double>(INFINITY) : off - log(sum);
+          }
+          if (lane == 0) {
+            s_off[k - k0] = off;
+            s_most[k - k0] = most;
+          }
+        }
+        __syncthreads();
       }
-    }
-    __syncthreads();
-    const long long end = static_cast<long long>(min(A.K, k0 + kMost)) * per;
-    for (long long base = static_cast<long long>(k0) * per; base < end; base += 256 * kRound) {
       Total c[kRound], top = kNoTotal;
 #pragma unroll
       for (int i = 0; i < kRound; ++i) {
-        const long long at = base + i * 256 + tid;
         c[i] = kNoTotal;
-        if (at >= end) continue;
-        const int k = static_cast<int>(at / per), in = static_cast<int>(at - static_cast<long long>(k) * per);
-        const int row = b * A.K + k;
-        if (A.ended && A.ended[row]) {  // goes on as it is, with one token
-          if (in == 0) c[i] = Total{order(s_off[k - k0]), static_cast<uint32_t>(k), 0, static_cast<uint32_t>(A.pad)};
+        const int k = beam[i];
+        if (k < 0) continue;
+        if (over[i]) {
+          c[i] = total(s_off[k], k0 + k, 0, A.pad);
         } else {
-          const int s = in / A.M, r = in - s * A.M;
-          const size_t slice = static_cast<size_t>(row) * A.S + s;
-          const uint2 best = A.best[slice * A.M + r];
-          const float logit = __uint_as_float(best.x & 0x80000000u ? best.x & 0x7fffffffu : ~best.x);
-          if (r < A.slices[slice].count)
-            c[i] = Total{order((static_cast<double>(logit) - s_most[k - k0]) + s_off[k - k0]),
-                         static_cast<uint32_t>(k), ~best.x, best.y};
+          const float logit = __uint_as_float(best[i].x & 0x80000000u ? best[i].x & 0x7fffffffu : ~best[i].x);
+          c[i] = total((static_cast<double>(logit) - s_most[k]) + s_off[k], k0 + k, ~best[i].x, best[i].y);
         }
         if (c[i].o && before(c[i], top)) top = c[i];
       }
       s_top[tid] = top;
-      if (tid < 4) s_bound[tid] = Total{1, ~0u, ~0u, ~0u};
+      if (tid < 4) s_bound[tid] = Total{1, ~0ull, ~0u};
       const int held = s_held;
       for (int i = tid; i < held; i += 256) s_list[i] = s_carry[i];
       if (tid == 0) s_count = held;
@@ -284,7 +318,7 @@ __global__ __launch_bounds__(256) void beam_choose_kernel(BeamArgs A) {
     const bool any = i < held;
     const size_t at = static_cast<size_t>(b) * A.M + i;
     A.out_scores[at] = any ? static_cast<float>(value(s_carry[i].o)) : -INFINITY;
-    A.out_parents[at] = any ? static_cast<int>(s_carry[i].k) : -1;
+    A.out_parents[at] = any ? static_cast<int>(s_carry[i].place >> 32) : -1;
     A.out_tokens[at] = any ? static_cast<int>(s_carry[i].t) : -1;
   }
 }
