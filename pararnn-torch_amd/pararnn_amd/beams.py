@@ -7,12 +7,20 @@ nothing and can be captured in a HIP graph.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from pararnn_amd import _lib
 from pararnn_amd.attention import _at, _enqueue, _no_tangents
-from pararnn_amd.ops import _validate, _workspace
+from pararnn_amd.ops import _DTYPES, _validate, _workspace
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(*sizes: int) -> int:
+    return _lib.load().prnn_beam_select_workspace_size(*sizes)
 
 
 def beam_select(logits: Tensor, scores: Tensor, *, beams: int | None = None,
@@ -31,13 +39,16 @@ def beam_select(logits: Tensor, scores: Tensor, *, beams: int | None = None,
     propose the token ``pad`` alone, whatever their logits.  No autograd.
     """
     what = "beam_select"
-    code = _validate(what, logits)
+    code = _DTYPES.get(logits.dtype) if logits.is_cuda else None
+    if code is None:
+        _validate(what, logits)
     if logits.dim() != 3:
         raise ValueError(f"{what}: logits must be (B, K, V), got {tuple(logits.shape)}")
     searches, given, vocab = logits.shape
     if torch.is_grad_enabled() and (logits.requires_grad or scores.requires_grad):
         raise RuntimeError(f"{what} has no autograd; call it under torch.no_grad()")
-    _no_tangents(what, logits, scores)
+    if forward_ad._current_level >= 0:
+        _no_tangents(what, logits, scores)
     if scores.device != logits.device or (ended is not None and ended.device != logits.device):
         raise RuntimeError(f"{what}: tensors on different devices")
     if scores.dtype != torch.float32:
@@ -62,14 +73,14 @@ def beam_select(logits: Tensor, scores: Tensor, *, beams: int | None = None,
     if logits.stride(-1) != 1 and vocab > 1:
         logits = logits.contiguous()
     scores = scores.contiguous()
-    dev, lib = logits.device, _lib.load()
+    dev = logits.device
     best = torch.empty(searches, wanted, dtype=torch.float32, device=dev)
     both = torch.empty(2, searches, wanted, dtype=torch.int32, device=dev)
-    need = lib.prnn_beam_select_workspace_size(searches, given, vocab, wanted)
+    need = _workspace_bytes(searches, given, vocab, wanted)
     ws = _workspace(need, dev)
-    rc = _enqueue(lib.prnn_beam_select, dev, logits.data_ptr(), logits.stride(0), logits.stride(1),
+    rc = _enqueue(_lib.load().prnn_beam_select, dev, logits.data_ptr(), logits.stride(0), logits.stride(1),
                   scores.data_ptr(), _at(ended), int(pad), best.data_ptr(), both.data_ptr(),
                   both.data_ptr() + 4 * searches * wanted, searches, given, vocab, wanted, code,
                   ws.data_ptr(), need)
     _lib.check(rc, what)
-    return best, both[0], both[1]
+    return best, *both.unbind()

@@ -211,7 +211,11 @@ def delta_rule_step(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, beta: Te
             log_decay = log_decay[:, 0]
         if beta.dim() == 3 and beta.shape[1] == 1:
             beta = beta[:, 0]
-    code = _validate(what, q, k, v)
+    code = _DTYPES.get(q.dtype)
+    # the quick look first: calls of small sizes are bound by the host
+    if not (code is not None and q.is_cuda and k.dtype is q.dtype and v.dtype is q.dtype
+            and k.device == q.device and v.device == q.device):
+        code = _validate(what, q, k, v)
     if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
         raise ValueError(f"{what}: q, k and v must be (B, heads, width), got {tuple(q.shape)}, "
                          f"{tuple(k.shape)}, {tuple(v.shape)}")

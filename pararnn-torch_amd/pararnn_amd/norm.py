@@ -23,6 +23,7 @@ import functools
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from pararnn_amd import _lib
 from pararnn_amd.attention import _at, _enqueue, _no_tangents, _once
@@ -164,6 +165,11 @@ def group_norm(x: Tensor, num_groups: int, weight: Tensor | None = None,
     return _forward(x, weight, bias, gate, codes)[0]
 
 
+@functools.lru_cache(maxsize=256)
+def _sums_bytes(rows: int, width: int) -> int:
+    return _lib.load().prnn_residual_norm_backward_workspace_size(rows, width)
+
+
 class _ResidualNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, y, weight, bias, post_weight, gate, scale, number, codes):
@@ -194,7 +200,7 @@ class _ResidualNorm(torch.autograd.Function):
         db = sums(width, dtype=bias_type, device=dev) if need[3] and bias_type else None
         lib, ws, size = _lib.load(), None, 0
         if dw is not None or db is not None or dp is not None or ds is not None:
-            size = lib.prnn_residual_norm_backward_workspace_size(rows, width)
+            size = _sums_bytes(rows, width)
             ws = _workspace(size, dev)
         rc = _enqueue(lib.prnn_residual_norm_backward, dev, _at(gh), _at(gz), x.data_ptr(), _at(y),
                       _at(weight), _at(post_weight), _at(gate), _at(scale), number, _at(dx), _at(dy),
@@ -231,7 +237,9 @@ def residual_norm(x: Tensor, y: Tensor | None, weight: Tensor | None = None,
     + bias)``.  Differentiable in all tensors.
     """
     what = "residual_norm"
-    _validate(what, x, y, gate)
+    if not (x.is_cuda and x.dtype in _DTYPES and (y is None or y.dtype is x.dtype and y.device == x.device)
+            and (gate is None or gate.dtype is x.dtype and gate.device == x.device)):
+        _validate(what, x, y, gate)
     if x.dim() < 1 or not 1 <= x.shape[-1] <= 16384:
         raise ValueError(f"{what}: x must be (..., C) with C in 1 .. 16384, got {tuple(x.shape)}")
     c = x.shape[-1]
@@ -270,7 +278,8 @@ def residual_norm(x: Tensor, y: Tensor | None, weight: Tensor | None = None,
     rows = x.numel() // c
     if rows >= 1 << 31:
         raise ValueError(f"{what}: x has {rows} tokens, more than 2^31 - 1")
-    _no_tangents(what, x, y, gate, *(t for _, t in params))
+    if forward_ad._current_level >= 0:
+        _no_tangents(what, x, y, gate, weight, bias, post_weight, vector)
     grads = torch.is_grad_enabled() and any(
         t is not None and t.requires_grad for t in (x, y, weight, bias, post_weight, gate, vector))
     given = x
