@@ -21,20 +21,22 @@ constexpr int kLf = 65;  // floats of a row of the flow's matrix
 // KS slabs of 64 columns of dq and dk at a time; WIDE: keys of more than KS, in several passes (the
 // pairs then need a place of their own).
 template <class M, int KS, bool WIDE>
-__global__ __launch_bounds__(256, sizeof(typename M::E) == 2 && KS == 1 ? 2 : 1) void dr_grad_kernel(DrGrad A) {
+__global__ __launch_bounds__(512, sizeof(typename M::E) == 2 && KS == 1 ? 4 : 2) void dr_grad_kernel(DrGrad A) {
   using E = typename M::E;
   constexpr bool kNarrow = sizeof(E) == 2;
   constexpr int ES = static_cast<int>(sizeof(E));
-  constexpr int kAt = kNarrow ? 4 : 2 / KS;  // steps whose operands are under way
+  constexpr int kAt = 2;  // steps whose operands are under way
   constexpr int RB = dr_row_k(kNarrow, 64), P = M::kParts, kSlab = kDrC * RB;
   __shared__ __align__(16) char lds[(WIDE ? 4 + P : 4) * kSlab], s_x[P][kSlab];
-  __shared__ float sF[kDrC * kLf], s_in[8][kDrC], s_out[8][kDrC];
+  __shared__ float sF[kDrC * kLf], s_in[2][8][kDrC], s_out[8][kDrC];
   __shared__ __align__(16) float sw[kDrW * 64];
-  __shared__ float s_through[4], s_own[kDrC], s_into[kDrC], s_waves[4];
+  __shared__ float s_through[4], s_own[kDrC], s_into[kDrC], s_waves[8];
   char *const sK = lds, *const sQ = lds + kSlab, *const sG = lds + 2 * kSlab, *const sD = lds + 3 * kSlab;
   char* const sP = WIDE ? lds + 4 * kSlab : sG;  // the pairs go u^T, by parts
   const int h = blockIdx.x % A.H, id = blockIdx.x / A.H;
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l32 = lane & 31, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, half = lane >> 5;
+  const int wave = (tid >> 6) & 3;
+  const bool lead = __builtin_amdgcn_readfirstlane(tid >> 8) == 0;  // pairs and dq; the other waves dk
   const DrUnit u = dr_unit(A.seqs, kDrC, id);
   if (!u.any || u.begin >= u.end) {
     if (A.g_part && tid == 0) A.g_part[static_cast<size_t>(id) * A.H + h] = 0.0f;
@@ -57,7 +59,7 @@ __global__ __launch_bounds__(256, sizeof(typename M::E) == 2 && KS == 1 ? 2 : 1)
   const rsrc_t re = operands(A.e, kDrC, A.Dv), rS = operands(A.before, A.Dk, A.Dv),
                rR = operands(A.behind, A.Dk, A.Dv);
   const int vs = (A.Dv + 15) / 16, last_k = (A.Dk - 1) / 64 * 64;
-  Staged<M, 64, 256> ga, gb, ka, kb;
+  Staged<M, 64, 512> ga, gb, ka, kb;
   ga.fetch(pg, A.go.st, n, 0, A.Dv, A.dtype);
   gb.fetch(pd, static_cast<long long>(A.H) * A.Dv, n, 0, A.Dv, kCode);
   ka.fetch(pk, A.k.st, n, last_k, A.Dk, A.dtype);
@@ -66,6 +68,19 @@ __global__ __launch_bounds__(256, sizeof(typename M::E) == 2 && KS == 1 ? 2 : 1)
   // operands of a wave's tiles of the states and of its tokens' e; the pairs' earlier tokens are the same
   // (waves 0 and 1: the first 32, wave 2: the others)
   const int kt = wave & 1, it = wave >> 1, t = 32 * it + l32;
+  for (int i = tid; i < kDrW * 64; i += 512) sw[i] = weights[i];
+  ga.template put<RB>(sG, A.dtype);
+  gb.template put<RB>(sD, kCode);
+  ka.template put<RB>(sK, A.dtype);
+  kb.template put<RB>(sQ, A.dtype);
+
+  // The first four waves: the pairs go e^T, dv e^T, q k^T, k k^T of their tile and a tile of dq in every
+  // slab, the others: e R^T and dv S^T of their tile of dk.  Either way its own code, with the same
+  // barriers: in common branches the registers of both were taken.
+  const int pi = wave > 0, pj = wave > 1, i = 32 * pi + l32;
+  float through = 0.0f;
+  auto run = [&](auto role) {
+  constexpr bool kLead = decltype(role)::value;
   Op<M, 1> ei[kAt], S[KS][kAt], R[KS][kAt];
   auto fetch = [&](int p0, int v0, int f0) {
 #pragma unroll
@@ -76,38 +91,21 @@ __global__ __launch_bounds__(256, sizeof(typename M::E) == 2 && KS == 1 ? 2 : 1)
       for (int s = 0; s < KS; ++s) {
         const int tile = p0 / 32 + 2 * s + kt;
         S[s][f] = global_op<M>(rS, (step < vs) & (32 * tile < A.Dk), tile * vs + step);
-        R[s][f] = global_op<M>(rR, (step < vs) & (32 * tile < A.Dk), tile * vs + step);
+        if constexpr (!kLead) R[s][f] = global_op<M>(rR, (step < vs) & (32 * tile < A.Dk), tile * vs + step);
       }
     }
   };
-  for (int i = tid; i < kDrW * 64; i += 256) sw[i] = weights[i];
-  ga.template put<RB>(sG, A.dtype);
-  gb.template put<RB>(sD, kCode);
-  ka.template put<RB>(sK, A.dtype);
-  kb.template put<RB>(sQ, A.dtype);
+  const bool pairs = kLead && wave < 3;
 
-  // pairs of the wave's tile; state products of its tile of every slab
-  const int pi = wave > 0, pj = wave > 1, i = 32 * pi + l32;
-  f16v GU, DU, QK, KK;
-  float through = 0.0f;
+  for (int p0 = 0; p0 < (WIDE ? A.Dk : 1); p0 += 64 * KS) {
+    f16v GU, DU;
 #pragma unroll
-  for (int r = 0; r < 16; ++r) GU[r] = DU[r] = QK[r] = KK[r] = 0.0f;
-
-  auto keys = [&]() {
-#pragma unroll
-    for (int f = 0; f < 4; ++f) {
-      const auto kj = row_op<M, 2>(sK + (32 * pj + l32) * RB, f, half);
-      mul<32>(QK, kj, row_op<M, 2>(sQ + i * RB, f, half));
-      mul<32>(KK, kj, row_op<M, 2>(sK + i * RB, f, half));
-    }
-  };
-
-  for (int p0 = 0; p0 < A.Dk; p0 += 64 * KS) {
-    f16v dq[KS], du[KS], ds[KS];
+    for (int r = 0; r < 16; ++r) GU[r] = DU[r] = 0.0f;
+    f16v main[KS], ds[KS];  // dq, or dk and dv S^T
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) dq[s][r] = du[s][r] = ds[s][r] = 0.0f;
+      for (int r = 0; r < 16; ++r) main[s][r] = ds[s][r] = 0.0f;
     // ---- 1
     for (int v0 = 0; v0 < A.Dv; v0 += 64) {
       if (p0 > 0 || v0 > 0) {
@@ -119,43 +117,54 @@ __global__ __launch_bounds__(256, sizeof(typename M::E) == 2 && KS == 1 ? 2 : 1)
       }
       fetch(p0, v0, 0);
       __syncthreads();
-      // under the operands' way: pairs of what is in LDS
-      if (p0 == 0 && v0 == 0 && wave < 3) keys();
+#pragma unroll
       for (int f0 = 0; f0 < 4; f0 += kAt) {
         if (f0 > 0) fetch(p0, v0, f0);
-#pragma unroll
-        for (int f = 0; f < kAt; ++f) {
-          const auto gi = row_op<M, 2>(sG + t * RB, f0 + f, half), di = row_op<M, 2>(sD + t * RB, f0 + f, half);
-#pragma unroll
-          for (int s = 0; s < KS; ++s) {
-            mul<32>(dq[s], S[s][f], gi);
-            mul<32>(du[s], R[s][f], ei[f]);
-            mul<32>(ds[s], S[s][f], di);
-          }
-        }
-        // from the state before to the adjoint behind: two waves have the same operands, a step each
-#pragma unroll
-        for (int f = 0; f < kAt; ++f) {
-          if (((f0 + f) & 1) != it) continue;
-#pragma unroll
-          for (int s = 0; s < KS; ++s) {
-            float x[8], y[8];
-            values(S[s][f], x);
-            values(R[s][f], y);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) through = fmaf(x[e], y[e], through);
-          }
-        }
-        if (p0 == 0 && wave < 3) {
+        if constexpr (kLead) {
 #pragma unroll
           for (int f = 0; f < kAt; ++f) {
-            mul<32>(GU, ei[f], row_op<M, 2>(sG + i * RB, f0 + f, half));
-            mul<32>(DU, ei[f], row_op<M, 2>(sD + i * RB, f0 + f, half));
+            const auto gi = row_op<M, 2>(sG + t * RB, f0 + f, half);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) mul<32>(main[s], S[s][f], gi);
+            if (p0 == 0 && pairs) {
+              mul<32>(GU, ei[f], row_op<M, 2>(sG + i * RB, f0 + f, half));
+              mul<32>(DU, ei[f], row_op<M, 2>(sD + i * RB, f0 + f, half));
+            }
+          }
+        } else {
+#pragma unroll
+          for (int f = 0; f < kAt; ++f) {
+            const auto di = row_op<M, 2>(sD + t * RB, f0 + f, half);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+              mul<32>(main[s], R[s][f], ei[f]);
+              mul<32>(ds[s], S[s][f], di);
+              // from the state before to the adjoint behind: two waves have the same operands, a step each
+              if (((f0 + f) & 1) == it) {
+                float x[8], y[8];
+                values(S[s][f], x);
+                values(R[s][f], y);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) through = fmaf(x[e], y[e], through);
+              }
+            }
           }
         }
       }
     }
     if (p0 == 0) {
+      f16v QK, KK;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) QK[r] = KK[r] = 0.0f;
+      auto keys = [&]() {
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+          const auto kj = row_op<M, 2>(sK + (32 * pj + l32) * RB, f, half);
+          mul<32>(QK, kj, row_op<M, 2>(sQ + i * RB, f, half));
+          mul<32>(KK, kj, row_op<M, 2>(sK + i * RB, f, half));
+        }
+      };
+      if (pairs) keys();
       for (int c0 = last_k - 64; c0 >= 0; c0 -= 64) {
         ka.fetch(pk, A.k.st, n, c0, A.Dk, A.dtype);
         kb.fetch(pq, A.q.st, n, c0, A.Dk, A.dtype);
@@ -163,10 +172,10 @@ __global__ __launch_bounds__(256, sizeof(typename M::E) == 2 && KS == 1 ? 2 : 1)
         ka.template put<RB>(sK, A.dtype);
         kb.template put<RB>(sQ, A.dtype);
         __syncthreads();
-        if (wave < 3) keys();
+        if (pairs) keys();
       }
       __syncthreads();  // go and dv have been read: the pairs take their place
-      if (wave < 3) {
+      if (pairs) {
         const float Hi = sw[kWhi * 64 + i], Lo = sw[kWlo * 64 + i];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -182,25 +191,21 @@ __global__ __launch_bounds__(256, sizeof(typename M::E) == 2 && KS == 1 ? 2 : 1)
             sF[jj * kLf + i] = jj < i ? QK[e] * w1[r] - KK[e] * x[r] : 0.0f;
             if (jj == i) s_own[i] = QK[e] * w1[r];
             w1[r] *= sw[kWb * 64 + jj];
-            x[r] *= sw[kWb * 64 + jj];
+            x[r] *= -sw[kWb * 64 + jj];
           }
           if constexpr (kNarrow) {
-            const u2 a{pack_bf16x2(w1[0], w1[1]), pack_bf16x2(w1[2], w1[3])};
-            const u2 b{pack_bf16x2(w1[0] - lo_bf16(a[0]), w1[1] - hi_bf16(a[0])),
-                       pack_bf16x2(w1[2] - lo_bf16(a[1]), w1[3] - hi_bf16(a[1]))};
-            *reinterpret_cast<u2*>(sP + i * RB + j0 * 2) = a;
-            *reinterpret_cast<u2*>(sP + kSlab + i * RB + j0 * 2) = b;
+            auto both = [&](char* hi, char* lo, const float* v) {
+              const u2 a{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+              const u2 b{pack_bf16x2(v[0] - lo_bf16(a[0]), v[1] - hi_bf16(a[0])),
+                         pack_bf16x2(v[2] - lo_bf16(a[1]), v[3] - hi_bf16(a[1]))};
+              *reinterpret_cast<u2*>(hi + i * RB + j0 * 2) = a;
+              *reinterpret_cast<u2*>(lo + i * RB + j0 * 2) = b;
+            };
+            both(sP, sP + kSlab, w1);
+            both(s_x[0], s_x[P - 1], x);
           } else {
             *reinterpret_cast<f4*>(sP + i * RB + j0 * 4) = f4{w1[0], w1[1], w1[2], w1[3]};
-          }
-          if constexpr (kNarrow) {
-            const u2 a{pack_bf16x2(-x[0], -x[1]), pack_bf16x2(-x[2], -x[3])};
-            const u2 b{pack_bf16x2(-x[0] - lo_bf16(a[0]), -x[1] - hi_bf16(a[0])),
-                       pack_bf16x2(-x[2] - lo_bf16(a[1]), -x[3] - hi_bf16(a[1]))};
-            *reinterpret_cast<u2*>(s_x[0] + i * RB + j0 * 2) = a;
-            *reinterpret_cast<u2*>(s_x[P - 1] + i * RB + j0 * 2) = b;
-          } else {
-            *reinterpret_cast<f4*>(s_x[0] + i * RB + j0 * 4) = f4{-x[0], -x[1], -x[2], -x[3]};
+            *reinterpret_cast<f4*>(s_x[0] + i * RB + j0 * 4) = f4{x[0], x[1], x[2], x[3]};
           }
         }
       }
@@ -208,7 +213,31 @@ __global__ __launch_bounds__(256, sizeof(typename M::E) == 2 && KS == 1 ? 2 : 1)
     }
 
     // ---- 2
-    const float wg = sw[kWg * 64 + t], wr = sw[kWr * 64 + t], rate = sw[kWb * 64 + t];
+    auto four = [&](const char* row, int col, float* v) {
+      if constexpr (kNarrow) {
+        const u2 a = *reinterpret_cast<const u2*>(row + col * 2);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = r & 1 ? hi_bf16(a[r >> 1]) : lo_bf16(a[r >> 1]);
+      } else {
+        const f4 a = *reinterpret_cast<const f4*>(row + col * 4);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = a[r];
+      }
+    };
+    // the parts of a pair's operand
+    auto parts = [&](auto&& get) {
+      Op<M, P> x;
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        const auto one = get(p);
+        if constexpr (kNarrow)
+          x.p[p] = one.p[0];
+        else
+          x = one;
+      }
+      return x;
+    };
+    const int col_at = col_share<M, 2, RB>(lane);
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const int c0 = p0 + 64 * s;
@@ -222,81 +251,66 @@ __global__ __launch_bounds__(256, sizeof(typename M::E) == 2 && KS == 1 ? 2 : 1)
         __syncthreads();
       }
       const bool any = c0 + 32 * kt < A.Dk;
-      if (any) {
-      float in_sum = 0.0f, out_sum = 0.0f;
+      const char* const kat = sK + 32 * kt * ES + col_at;
+      if constexpr (kLead) if (any) {
+        f16v& dq = main[s];
+        const float w = sw[kWg * 64 + t] * A.scale;
+        float in_sum = 0.0f;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int col = 32 * kt + 8 * q + 4 * half;
-        float qv[4], kv[4];
-        if constexpr (kNarrow) {
-          const u2 a = *reinterpret_cast<const u2*>(sQ + t * RB + col * 2);
-          const u2 b = *reinterpret_cast<const u2*>(sK + t * RB + col * 2);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            qv[r] = r & 1 ? hi_bf16(a[r >> 1]) : lo_bf16(a[r >> 1]);
-            kv[r] = r & 1 ? hi_bf16(b[r >> 1]) : lo_bf16(b[r >> 1]);
-          }
-        } else {
-          const f4 a = *reinterpret_cast<const f4*>(sQ + t * RB + col * 4);
-          const f4 b = *reinterpret_cast<const f4*>(sK + t * RB + col * 4);
+        for (int q = 0; q < 4; ++q) {
+          float v[4];
+          four(sQ + t * RB, 32 * kt + 8 * q + 4 * half, v);
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            qv[r] = a[r];
-            kv[r] = b[r];
+            dq[4 * q + r] *= w;
+            in_sum = fmaf(v[r], dq[4 * q + r], in_sum);
           }
         }
+        in_sum += __shfl_xor(in_sum, 32);
+        if (half == 0) s_in[0][c0 / 32 + kt][t] = in_sum;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int e = 4 * q + r;
-          dq[s][e] *= wg * A.scale;
-          ds[s][e] *= wg;
-          du[s][e] *= wr;
-          in_sum = fmaf(qv[r], dq[s][e], fmaf(-kv[r], ds[s][e], in_sum));
-          out_sum = fmaf(kv[r], du[s][e], out_sum);
-          du[s][e] = fmaf(rate, du[s][e], -ds[s][e]);
-        }
+        for (int f = 0; f < 4; ++f)
+          if ((f >> 1) <= it)
+            mul<32>(dq, col_op<M, 2, RB>(kat, 16 * f, 0),
+                    parts([&](int p) { return row_op<M, 2>(sP + p * kSlab + t * RB, f, half); }));
       }
-      in_sum += __shfl_xor(in_sum, 32);
-      out_sum += __shfl_xor(out_sum, 32);
-      if (half == 0) {
-        s_in[c0 / 32 + kt][t] = in_sum;
-        s_out[c0 / 32 + kt][t] = out_sum;
-      }
-      const char* kat = sK + 32 * kt * ES + col_share<M, 2, RB>(lane);
-      const char* qat = sQ + 32 * kt * ES + col_share<M, 2, RB>(lane);
+      if constexpr (!kLead) if (any) {
+        f16v &du = main[s], &dS = ds[s];
+        const float wg = sw[kWg * 64 + t], wr = sw[kWr * 64 + t], rate = sw[kWb * 64 + t];
+        float in_sum = 0.0f, out_sum = 0.0f;
 #pragma unroll
-      for (int f = 0; f < 4; ++f) {
-        const int jt = f >> 1;
-        const auto kc = col_op<M, 2, RB>(kat, 16 * f, 0);
-        Op<M, P> x;
-        auto both = [&](auto&& get) {
+        for (int q = 0; q < 4; ++q) {
+          float v[4];
+          four(sK + t * RB, 32 * kt + 8 * q + 4 * half, v);
 #pragma unroll
-          for (int p = 0; p < P; ++p) {
-            const auto one = get(p);
-            if constexpr (kNarrow)
-              x.p[p] = one.p[0];
-            else
-              x = one;
+          for (int r = 0; r < 4; ++r) {
+            const int e = 4 * q + r;
+            dS[e] *= wg;
+            du[e] *= wr;
+            in_sum = fmaf(-v[r], dS[e], in_sum);
+            out_sum = fmaf(v[r], du[e], out_sum);
+            du[e] = fmaf(rate, du[e], -dS[e]);
           }
-        };
-        // -(X + X^T), rows of X before the token and columns behind it
-        if (jt <= it) {
-          both([&](int p) { return row_op<M, 2>(s_x[p] + t * RB, f, half); });
-          mul<32>(du[s], kc, x);
         }
-        if (jt >= it) {
-          both([&](int p) { return col_op<M, 2, RB>(s_x[p] + col_share<M, 2, RB>(lane), 16 * f, 32 * it); });
-          mul<32>(du[s], kc, x);
+        in_sum += __shfl_xor(in_sum, 32);
+        out_sum += __shfl_xor(out_sum, 32);
+        if (half == 0) {
+          s_in[1][c0 / 32 + kt][t] = in_sum;
+          s_out[c0 / 32 + kt][t] = out_sum;
         }
-        if (jt <= it) {
-          both([&](int p) { return row_op<M, 2>(sP + p * kSlab + t * RB, f, half); });
-          mul<32>(dq[s], kc, x);
+        const char* const qat = sQ + 32 * kt * ES + col_at;
+#pragma unroll
+        for (int f = 0; f < 4; ++f) {
+          const int jt = f >> 1;
+          const auto kc = col_op<M, 2, RB>(kat, 16 * f, 0);
+          // -(X + X^T), rows of X before the token and columns behind it
+          if (jt <= it) mul<32>(du, kc, parts([&](int p) { return row_op<M, 2>(s_x[p] + t * RB, f, half); }));
+          if (jt >= it) {
+            mul<32>(du, kc, parts([&](int p) { return col_op<M, 2, RB>(s_x[p] + col_at, 16 * f, 32 * it); }));
+            mul<32>(du, col_op<M, 2, RB>(qat, 16 * f, 0),
+                    parts([&](int p) { return col_op<M, 2, RB>(sP + p * kSlab + col_at, 16 * f, 32 * it); }));
+          }
         }
-        if (jt >= it) {
-          both([&](int p) { return col_op<M, 2, RB>(sP + p * kSlab + col_share<M, 2, RB>(lane), 16 * f, 32 * it); });
-          mul<32>(du[s], col_op<M, 2, RB>(qat, 16 * f, 0), x);
-        }
-      }
       }
       auto out = [&](void* p, int f32, const f16v& v) {
         const int size = f32 ? 4 : TS;
@@ -306,79 +320,80 @@ __global__ __launch_bounds__(256, sizeof(typename M::E) == 2 && KS == 1 ? 2 : 1)
           const int col = c0 + 32 * kt + 8 * q + 4 * half;
           const uint32_t to = (t * A.H * A.Dk + col) * size;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t one = la_in((t < n) & (col + e < A.Dk), to + e * size);
-              if (f32 || A.dtype == PRNN_F32)
-                stb<float>(r, one, 0, v[4 * q + e]);
-              else if (A.dtype == PRNN_F16)
-                stb<f16>(r, one, 0, v[4 * q + e]);
-              else
-                stb<bf16>(r, one, 0, v[4 * q + e]);
-            }
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t one = la_in((t < n) & (col + e < A.Dk), to + e * size);
+            if (f32 || A.dtype == PRNN_F32)
+              stb<float>(r, one, 0, v[4 * q + e]);
+            else if (A.dtype == PRNN_F16)
+              stb<f16>(r, one, 0, v[4 * q + e]);
+            else
+              stb<bf16>(r, one, 0, v[4 * q + e]);
+          }
         }
       };
       if constexpr (kNarrow) {
-        // bf16 rows leave by way of LDS, 16 bytes a lane side by side: 8 bytes of 64 tokens an instruction
-        // took 2900 cycles of a workgroup's 28800
+        // bf16 rows leave by way of LDS, 16 bytes a lane side by side
         auto put = [&](char* to, const f16v& v) {
 #pragma unroll
           for (int q = 0; q < 4; ++q)
             *reinterpret_cast<u2*>(to + t * RB + (32 * kt + 8 * q + 4 * half) * 2) =
                 u2{pack_bf16x2(v[4 * q], v[4 * q + 1]), pack_bf16x2(v[4 * q + 2], v[4 * q + 3])};
         };
-        __syncthreads();  // k and q have been read
-        if (any && !A.q_f32) put(sQ, dq[s]);
-        if (any && !A.k_f32) put(sK, du[s]);
-        __syncthreads();
         auto rows_out = [&](void* p, const char* from) {
           const rsrc_t r = make_rsrc(static_cast<char*>(p) + (tok0 * A.H + h) * A.Dk * 2, 0x7fffffffu);
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int row = (tid + 256 * k) >> 3, unit = tid & 7, col = c0 + 8 * unit;
-            __builtin_amdgcn_raw_buffer_store_b128(*reinterpret_cast<const u4*>(from + row * RB + unit * 16), r,
-                                                   la_in((row < n) & (col < A.Dk), (row * A.H * A.Dk + col) * 2), 0, 0);
-          }
+          const int row = tid >> 3, unit = tid & 7, col = c0 + 8 * unit;
+          __builtin_amdgcn_raw_buffer_store_b128(*reinterpret_cast<const u4*>(from + row * RB + unit * 16), r,
+                                                 la_in((row < n) & (col < A.Dk), (row * A.H * A.Dk + col) * 2), 0, 0);
         };
+        __syncthreads();  // k and q have been read
+        const bool f32 = kLead ? A.q_f32 : A.k_f32;
+        if (any && !f32) put(kLead ? sQ : sK, main[s]);
+        __syncthreads();
         if (!A.q_f32) rows_out(A.dq, sQ);
         if (!A.k_f32) rows_out(A.dk, sK);
-        if (any && A.q_f32) out(A.dq, 1, dq[s]);
-        if (any && A.k_f32) out(A.dk, 1, du[s]);
+        if (any && f32) out(kLead ? A.dq : A.dk, 1, main[s]);
       } else if (any) {
-        out(A.dq, A.q_f32, dq[s]);
-        out(A.dk, A.k_f32, du[s]);
+        out(kLead ? A.dq : A.dk, kLead ? A.q_f32 : A.k_f32, main[s]);
       }
     }
   }
+  };
+  if (lead)
+    run(std::true_type{});
+  else
+    run(std::false_type{});
   if (!A.dg && !A.g_part && !A.dbeta) return;
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) through += __shfl_xor(through, m);
-  if (lane == 0) s_through[wave] = through;
+  if (lane == 0 && !lead) s_through[wave] = through;
   __syncthreads();
 
-  // ---- 3: four lanes per token, a quarter of the others' each
-  const int tok = tid >> 2, part = tid & 3, tiles = (A.Dk + 31) / 32;
+  // ---- 3: eight lanes per token, an eighth of the others' each
+  const int tok = tid >> 3, part = tid & 7, tiles = (A.Dk + 31) / 32;
   {
     // row tok: sums of its uses from l on, what the adjoint behind reads among them
-    float m[16], sum = 0.0f, out = 0.0f;
+    float m[8], sum = 0.0f, after = 0.0f;
 #pragma unroll
-    for (int x = 15; x >= 0; --x) {
-      const int l = 16 * part + x;
+    for (int x = 7; x >= 0; --x) {
+      const int l = 8 * part + x;
       const float flow = sF[tok * kLf + l];
       sum += l > tok ? flow : 0.0f;
       m[x] = sum;
     }
-    for (int k = 0; k < tiles; ++k) out += s_out[k][tok];
-    const float s1 = __shfl_down(sum, 1), s2 = __shfl_down(sum, 2), s3 = __shfl_down(sum, 3);
-    const float after = out + ((part < 1 ? s3 : 0.0f) + (part < 2 ? s2 : 0.0f)) + (part < 3 ? s1 : 0.0f);
+#pragma unroll
+    for (int k = 1; k < 8; k <<= 1) {
+      const float o = __shfl_down(sum, k);
+      if (part + k < 8) sum += o;
+    }
+    const float later = __shfl_down(sum, 1);
+    for (int k = 0; k < tiles; ++k) after += s_out[k][tok];
+    after += part < 7 ? later : 0.0f;
     const float rate = sw[kWb * 64 + tok];
 #pragma unroll
-    for (int x = 0; x < 16; ++x) {
-      const int l = 16 * part + x;
-      sF[tok * kLf + l] = rate * (after + m[x]);  // (up to l = tok: not read)
-    }
-    if (wave == 3) {  // what the tokens from one on read of the state before
+    for (int x = 0; x < 8; ++x) sF[tok * kLf + 8 * part + x] = rate * (after + m[x]);  // (up to l = tok: not read)
+    if (!lead && wave == 3) {  // what the tokens from one on read of the state before
       float into = 0.0f;
-      for (int k = 0; k < tiles; ++k) into += s_in[k][lane];
+      for (int k = 0; k < tiles; ++k) into += s_in[0][k][lane] + s_in[1][k][lane];
 #pragma unroll
       for (int m = 1; m < 64; m <<= 1) {
         const float o = __shfl_down(into, m);
@@ -402,13 +417,13 @@ __global__ __launch_bounds__(256, sizeof(typename M::E) == 2 && KS == 1 ? 2 : 1)
   // column tok: the sources before it
   float F = 0.0f;
 #pragma unroll
-  for (int x = 0; x < 16; ++x) {
-    const int j = 16 * part + x;
+  for (int x = 0; x < 8; ++x) {
+    const int j = 8 * part + x;
     const float flow = sF[j * kLf + tok];
     F += j < tok ? flow : 0.0f;
   }
-  F += __shfl_xor(F, 1);
-  F += __shfl_xor(F, 2);
+#pragma unroll
+  for (int m = 1; m < 8; m <<= 1) F += __shfl_xor(F, m);
   F += s_into[tok];
   const bool there = tok < n;
   // nothing comes through a factor that is zero
@@ -425,18 +440,20 @@ __global__ __launch_bounds__(256, sizeof(typename M::E) == 2 && KS == 1 ? 2 : 1)
   if (A.g_part) {
     F = part == 0 ? F : 0.0f;
 #pragma unroll
-    for (int m = 4; m < 64; m <<= 1) F += __shfl_xor(F, m);
-    if (lane == 0) s_waves[wave] = F;
+    for (int m = 8; m < 64; m <<= 1) F += __shfl_xor(F, m);
+    if (lane == 0) s_waves[tid >> 6] = F;
     __syncthreads();
-    if (tid == 0) A.g_part[unit] = (s_waves[0] + s_waves[1]) + (s_waves[2] + s_waves[3]);
+    if (tid == 0)
+      A.g_part[unit] = ((s_waves[0] + s_waves[1]) + (s_waves[2] + s_waves[3])) +
+                       ((s_waves[4] + s_waves[5]) + (s_waves[6] + s_waves[7]));
   }
 }
 
 template <class M, int KS, bool WIDE>
 int launch(const DrGrad& a, hipStream_t stream) {
   const long long groups = dr_units(a.seqs, kDrC) * a.H;
-  if (int rc = check_grid("delta_rule backward", groups, 256)) return rc;
-  dr_grad_kernel<M, KS, WIDE><<<static_cast<unsigned>(groups), 256, 0, stream>>>(a);
+  if (int rc = check_grid("delta_rule backward", groups, 512)) return rc;
+  dr_grad_kernel<M, KS, WIDE><<<static_cast<unsigned>(groups), 512, 0, stream>>>(a);
   PRNN_HIP(hipGetLastError());
   return PRNN_OK;
 }
