@@ -25,7 +25,7 @@ __global__ __launch_bounds__(512, sizeof(typename M::E) == 2 && KS == 1 ? 4 : 2)
   using E = typename M::E;
   constexpr bool kNarrow = sizeof(E) == 2;
   constexpr int ES = static_cast<int>(sizeof(E));
-  constexpr int kAt = 2;  // steps whose operands are under way
+  constexpr int kAt = kNarrow ? 4 : 2;  // steps whose operands are under way
   constexpr int RB = dr_row_k(kNarrow, 64), P = M::kParts, kSlab = kDrC * RB;
   __shared__ __align__(16) char lds[(WIDE ? 4 + P : 4) * kSlab], s_x[P][kSlab];
   __shared__ float sF[kDrC * kLf], s_in[2][8][kDrC], s_out[8][kDrC];
