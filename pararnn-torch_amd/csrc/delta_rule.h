@@ -96,8 +96,8 @@ __device__ __forceinline__ int dr_batch(const LaSeqs& q, const DrUnit& u) { retu
 // ---- a chunk's system --------------------------------------------------------------------
 //
 // Per chunk and head: the strictly lower part of the inverse, then the pairs, each as the tiles
-// (0, 0), (1, 0), (1, 1) of 32 x 32, rows of 32 elements whose units of four are exchanged by the row (dr_unit_of), bf16 in
-// two parts of 6 KB or fp32; then kDrW rows of 64 floats.
+// (0, 0), (1, 0), (1, 1) of 32 x 32, rows of 32 elements whose units of four are exchanged by the row
+// (dr_unit_of), bf16 in two parts of 6 KB or fp32; then kDrW rows of 64 floats.
 constexpr int kDrTiles = 3 * 32 * 32 * 4;  // bytes of a matrix in either arithmetic
 enum { kWg, kWr, kWb, kWhi, kWlo, kWmeta, kDrW };  // exp(G), exp(G_last - G), b, G in two parts
 constexpr int kDrSys = 2 * kDrTiles + kDrW * 64 * 4;

@@ -11,6 +11,11 @@
 //    summed as that double sum and not as a running difference of gains and losses: behind a strong
 //    decay the flow is a tiny part of either.  The rates' gradient is what all read of a unit of what
 //    the token writes: the same sums by rows, and the token's own.
+//
+// Eight waves: four for the pairs and dq, four for dk, each with its own code and the same barriers, so
+// that two workgroups a CU (what LDS holds) are four waves a SIMD.  4096 chunks of bf16, D = 64: 98 us for
+// 300 MB (3.1 TB/s; four waves that did all took 121); the phases' latencies bound it, no unit is busy
+// for half of the time.
 #include "delta_rule_loads.h"
 
 namespace prnn {
@@ -65,8 +70,6 @@ __global__ __launch_bounds__(512, sizeof(typename M::E) == 2 && KS == 1 ? 4 : 2)
   ka.fetch(pk, A.k.st, n, last_k, A.Dk, A.dtype);
   kb.fetch(pq, A.q.st, n, last_k, A.Dk, A.dtype);
   const float* weights = reinterpret_cast<const float*>(A.sys + unit * kDrSys + 2 * kDrTiles);
-  // operands of a wave's tiles of the states and of its tokens' e; the pairs' earlier tokens are the same
-  // (waves 0 and 1: the first 32, wave 2: the others)
   const int kt = wave & 1, it = wave >> 1, t = 32 * it + l32;
   for (int i = tid; i < kDrW * 64; i += 512) sw[i] = weights[i];
   ga.template put<RB>(sG, A.dtype);
@@ -80,283 +83,285 @@ __global__ __launch_bounds__(512, sizeof(typename M::E) == 2 && KS == 1 ? 4 : 2)
   const int pi = wave > 0, pj = wave > 1, i = 32 * pi + l32;
   float through = 0.0f;
   auto run = [&](auto role) {
-  constexpr bool kLead = decltype(role)::value;
-  Op<M, 1> ei[kAt], S[KS][kAt], R[KS][kAt];
-  auto fetch = [&](int p0, int v0, int f0) {
+    constexpr bool kLead = decltype(role)::value;
+    // operands of a wave's tiles of the states and of its tokens' e; the pairs' earlier tokens are the
+    // same ones (waves 0 and 1: the first 32, wave 2: the others)
+    Op<M, 1> ei[kAt], S[KS][kAt], R[KS][kAt];
+    auto fetch = [&](int p0, int v0, int f0) {
 #pragma unroll
-    for (int f = 0; f < kAt; ++f) {
-      const int step = v0 / 16 + f0 + f;
-      ei[f] = global_op<M>(re, step < vs, it * vs + step);
+      for (int f = 0; f < kAt; ++f) {
+        const int step = v0 / 16 + f0 + f;
+        ei[f] = global_op<M>(re, step < vs, it * vs + step);
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const int tile = p0 / 32 + 2 * s + kt;
-        S[s][f] = global_op<M>(rS, (step < vs) & (32 * tile < A.Dk), tile * vs + step);
-        if constexpr (!kLead) R[s][f] = global_op<M>(rR, (step < vs) & (32 * tile < A.Dk), tile * vs + step);
+        for (int s = 0; s < KS; ++s) {
+          const int tile = p0 / 32 + 2 * s + kt;
+          S[s][f] = global_op<M>(rS, (step < vs) & (32 * tile < A.Dk), tile * vs + step);
+          if constexpr (!kLead) R[s][f] = global_op<M>(rR, (step < vs) & (32 * tile < A.Dk), tile * vs + step);
+        }
       }
-    }
-  };
-  const bool pairs = kLead && wave < 3;
+    };
+    const bool pairs = kLead && wave < 3;
 
-  for (int p0 = 0; p0 < (WIDE ? A.Dk : 1); p0 += 64 * KS) {
-    f16v GU, DU;
+    for (int p0 = 0; p0 < (WIDE ? A.Dk : 1); p0 += 64 * KS) {
+      f16v GU, DU;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) GU[r] = DU[r] = 0.0f;
-    f16v main[KS], ds[KS];  // dq, or dk and dv S^T
+      for (int r = 0; r < 16; ++r) GU[r] = DU[r] = 0.0f;
+      f16v main[KS], ds[KS];  // dq, or dk and dv S^T
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
+      for (int s = 0; s < KS; ++s)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) main[s][r] = ds[s][r] = 0.0f;
-    // ---- 1
-    for (int v0 = 0; v0 < A.Dv; v0 += 64) {
-      if (p0 > 0 || v0 > 0) {
-        ga.fetch(pg, A.go.st, n, v0, A.Dv, A.dtype);
-        gb.fetch(pd, static_cast<long long>(A.H) * A.Dv, n, v0, A.Dv, kCode);
+        for (int r = 0; r < 16; ++r) main[s][r] = ds[s][r] = 0.0f;
+      // ---- 1
+      for (int v0 = 0; v0 < A.Dv; v0 += 64) {
+        if (p0 > 0 || v0 > 0) {
+          ga.fetch(pg, A.go.st, n, v0, A.Dv, A.dtype);
+          gb.fetch(pd, static_cast<long long>(A.H) * A.Dv, n, v0, A.Dv, kCode);
+          __syncthreads();
+          ga.template put<RB>(sG, A.dtype);
+          gb.template put<RB>(sD, kCode);
+        }
+        fetch(p0, v0, 0);
         __syncthreads();
-        ga.template put<RB>(sG, A.dtype);
-        gb.template put<RB>(sD, kCode);
-      }
-      fetch(p0, v0, 0);
-      __syncthreads();
 #pragma unroll
-      for (int f0 = 0; f0 < 4; f0 += kAt) {
-        if (f0 > 0) fetch(p0, v0, f0);
-        if constexpr (kLead) {
+        for (int f0 = 0; f0 < 4; f0 += kAt) {
+          if (f0 > 0) fetch(p0, v0, f0);
+          if constexpr (kLead) {
 #pragma unroll
-          for (int f = 0; f < kAt; ++f) {
-            const auto gi = row_op<M, 2>(sG + t * RB, f0 + f, half);
+            for (int f = 0; f < kAt; ++f) {
+              const auto gi = row_op<M, 2>(sG + t * RB, f0 + f, half);
 #pragma unroll
-            for (int s = 0; s < KS; ++s) mul<32>(main[s], S[s][f], gi);
-            if (p0 == 0 && pairs) {
-              mul<32>(GU, ei[f], row_op<M, 2>(sG + i * RB, f0 + f, half));
-              mul<32>(DU, ei[f], row_op<M, 2>(sD + i * RB, f0 + f, half));
+              for (int s = 0; s < KS; ++s) mul<32>(main[s], S[s][f], gi);
+              if (p0 == 0 && pairs) {
+                mul<32>(GU, ei[f], row_op<M, 2>(sG + i * RB, f0 + f, half));
+                mul<32>(DU, ei[f], row_op<M, 2>(sD + i * RB, f0 + f, half));
+              }
             }
-          }
-        } else {
+          } else {
 #pragma unroll
-          for (int f = 0; f < kAt; ++f) {
-            const auto di = row_op<M, 2>(sD + t * RB, f0 + f, half);
+            for (int f = 0; f < kAt; ++f) {
+              const auto di = row_op<M, 2>(sD + t * RB, f0 + f, half);
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-              mul<32>(main[s], R[s][f], ei[f]);
-              mul<32>(ds[s], S[s][f], di);
-              // from the state before to the adjoint behind: two waves have the same operands, a step each
-              if (((f0 + f) & 1) == it) {
-                float x[8], y[8];
-                values(S[s][f], x);
-                values(R[s][f], y);
+              for (int s = 0; s < KS; ++s) {
+                mul<32>(main[s], R[s][f], ei[f]);
+                mul<32>(ds[s], S[s][f], di);
+                // from the state before to the adjoint behind: two waves have the same operands, a step each
+                if (((f0 + f) & 1) == it) {
+                  float x[8], y[8];
+                  values(S[s][f], x);
+                  values(R[s][f], y);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) through = fmaf(x[e], y[e], through);
+                  for (int e = 0; e < 8; ++e) through = fmaf(x[e], y[e], through);
+                }
               }
             }
           }
         }
       }
-    }
-    if (p0 == 0) {
-      f16v QK, KK;
+      if (p0 == 0) {
+        f16v QK, KK;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) QK[r] = KK[r] = 0.0f;
-      auto keys = [&]() {
+        for (int r = 0; r < 16; ++r) QK[r] = KK[r] = 0.0f;
+        auto keys = [&]() {
 #pragma unroll
-        for (int f = 0; f < 4; ++f) {
-          const auto kj = row_op<M, 2>(sK + (32 * pj + l32) * RB, f, half);
-          mul<32>(QK, kj, row_op<M, 2>(sQ + i * RB, f, half));
-          mul<32>(KK, kj, row_op<M, 2>(sK + i * RB, f, half));
-        }
-      };
-      if (pairs) keys();
-      for (int c0 = last_k - 64; c0 >= 0; c0 -= 64) {
-        ka.fetch(pk, A.k.st, n, c0, A.Dk, A.dtype);
-        kb.fetch(pq, A.q.st, n, c0, A.Dk, A.dtype);
-        __syncthreads();
-        ka.template put<RB>(sK, A.dtype);
-        kb.template put<RB>(sQ, A.dtype);
-        __syncthreads();
+          for (int f = 0; f < 4; ++f) {
+            const auto kj = row_op<M, 2>(sK + (32 * pj + l32) * RB, f, half);
+            mul<32>(QK, kj, row_op<M, 2>(sQ + i * RB, f, half));
+            mul<32>(KK, kj, row_op<M, 2>(sK + i * RB, f, half));
+          }
+        };
         if (pairs) keys();
-      }
-      __syncthreads();  // go and dv have been read: the pairs take their place
-      if (pairs) {
-        const float Hi = sw[kWhi * 64 + i], Lo = sw[kWlo * 64 + i];
+        for (int c0 = last_k - 64; c0 >= 0; c0 -= 64) {
+          ka.fetch(pk, A.k.st, n, c0, A.Dk, A.dtype);
+          kb.fetch(pq, A.q.st, n, c0, A.Dk, A.dtype);
+          __syncthreads();
+          ka.template put<RB>(sK, A.dtype);
+          kb.template put<RB>(sQ, A.dtype);
+          __syncthreads();
+          if (pairs) keys();
+        }
+        __syncthreads();  // go and dv have been read: the pairs take their place
+        if (pairs) {
+          const float Hi = sw[kWhi * 64 + i], Lo = sw[kWlo * 64 + i];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float w1[4], x[4];
-          const int j0 = 32 * pj + 8 * q + 4 * half;
+          for (int q = 0; q < 4; ++q) {
+            float w1[4], x[4];
+            const int j0 = 32 * pj + 8 * q + 4 * half;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int jj = j0 + r, e = 4 * q + r;
-            const float w = fexp((Hi - sw[kWhi * 64 + jj]) + (Lo - sw[kWlo * 64 + jj]));
-            w1[r] = jj <= i ? w * A.scale * GU[e] : 0.0f;
-            x[r] = jj < i ? w * DU[e] : 0.0f;
-            // what token i reads of a unit of what j writes (its rate is still to come)
-            sF[jj * kLf + i] = jj < i ? QK[e] * w1[r] - KK[e] * x[r] : 0.0f;
-            if (jj == i) s_own[i] = QK[e] * w1[r];
-            w1[r] *= sw[kWb * 64 + jj];
-            x[r] *= -sw[kWb * 64 + jj];
-          }
-          if constexpr (kNarrow) {
-            auto both = [&](char* hi, char* lo, const float* v) {
-              const u2 a{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-              const u2 b{pack_bf16x2(v[0] - lo_bf16(a[0]), v[1] - hi_bf16(a[0])),
-                         pack_bf16x2(v[2] - lo_bf16(a[1]), v[3] - hi_bf16(a[1]))};
-              *reinterpret_cast<u2*>(hi + i * RB + j0 * 2) = a;
-              *reinterpret_cast<u2*>(lo + i * RB + j0 * 2) = b;
-            };
-            both(sP, sP + kSlab, w1);
-            both(s_x[0], s_x[P - 1], x);
-          } else {
-            *reinterpret_cast<f4*>(sP + i * RB + j0 * 4) = f4{w1[0], w1[1], w1[2], w1[3]};
-            *reinterpret_cast<f4*>(s_x[0] + i * RB + j0 * 4) = f4{x[0], x[1], x[2], x[3]};
+            for (int r = 0; r < 4; ++r) {
+              const int jj = j0 + r, e = 4 * q + r;
+              const float w = fexp((Hi - sw[kWhi * 64 + jj]) + (Lo - sw[kWlo * 64 + jj]));
+              w1[r] = jj <= i ? w * A.scale * GU[e] : 0.0f;
+              x[r] = jj < i ? w * DU[e] : 0.0f;
+              // what token i reads of a unit of what j writes (its rate is still to come)
+              sF[jj * kLf + i] = jj < i ? QK[e] * w1[r] - KK[e] * x[r] : 0.0f;
+              if (jj == i) s_own[i] = QK[e] * w1[r];
+              w1[r] *= sw[kWb * 64 + jj];
+              x[r] *= -sw[kWb * 64 + jj];
+            }
+            if constexpr (kNarrow) {
+              auto both = [&](char* hi, char* lo, const float* v) {
+                const u2 a{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+                const u2 b{pack_bf16x2(v[0] - lo_bf16(a[0]), v[1] - hi_bf16(a[0])),
+                           pack_bf16x2(v[2] - lo_bf16(a[1]), v[3] - hi_bf16(a[1]))};
+                *reinterpret_cast<u2*>(hi + i * RB + j0 * 2) = a;
+                *reinterpret_cast<u2*>(lo + i * RB + j0 * 2) = b;
+              };
+              both(sP, sP + kSlab, w1);
+              both(s_x[0], s_x[P - 1], x);
+            } else {
+              *reinterpret_cast<f4*>(sP + i * RB + j0 * 4) = f4{w1[0], w1[1], w1[2], w1[3]};
+              *reinterpret_cast<f4*>(s_x[0] + i * RB + j0 * 4) = f4{x[0], x[1], x[2], x[3]};
+            }
           }
         }
+        __syncthreads();
       }
-      __syncthreads();
-    }
 
-    // ---- 2
-    auto four = [&](const char* row, int col, float* v) {
-      if constexpr (kNarrow) {
-        const u2 a = *reinterpret_cast<const u2*>(row + col * 2);
+      // ---- 2
+      auto four = [&](const char* row, int col, float* v) {
+        if constexpr (kNarrow) {
+          const u2 a = *reinterpret_cast<const u2*>(row + col * 2);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = r & 1 ? hi_bf16(a[r >> 1]) : lo_bf16(a[r >> 1]);
-      } else {
-        const f4 a = *reinterpret_cast<const f4*>(row + col * 4);
+          for (int r = 0; r < 4; ++r) v[r] = r & 1 ? hi_bf16(a[r >> 1]) : lo_bf16(a[r >> 1]);
+        } else {
+          const f4 a = *reinterpret_cast<const f4*>(row + col * 4);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = a[r];
-      }
-    };
-    // the parts of a pair's operand
-    auto parts = [&](auto&& get) {
-      Op<M, P> x;
-#pragma unroll
-      for (int p = 0; p < P; ++p) {
-        const auto one = get(p);
-        if constexpr (kNarrow)
-          x.p[p] = one.p[0];
-        else
-          x = one;
-      }
-      return x;
-    };
-    const int col_at = col_share<M, 2, RB>(lane);
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int c0 = p0 + 64 * s;
-      if (c0 >= A.Dk) continue;
-      if (c0 > 0) {
-        ka.fetch(pk, A.k.st, n, c0, A.Dk, A.dtype);
-        kb.fetch(pq, A.q.st, n, c0, A.Dk, A.dtype);
-        __syncthreads();
-        ka.template put<RB>(sK, A.dtype);
-        kb.template put<RB>(sQ, A.dtype);
-        __syncthreads();
-      }
-      const bool any = c0 + 32 * kt < A.Dk;
-      const char* const kat = sK + 32 * kt * ES + col_at;
-      if constexpr (kLead) if (any) {
-        f16v& dq = main[s];
-        const float w = sw[kWg * 64 + t] * A.scale;
-        float in_sum = 0.0f;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float v[4];
-          four(sQ + t * RB, 32 * kt + 8 * q + 4 * half, v);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            dq[4 * q + r] *= w;
-            in_sum = fmaf(v[r], dq[4 * q + r], in_sum);
-          }
-        }
-        in_sum += __shfl_xor(in_sum, 32);
-        if (half == 0) s_in[0][c0 / 32 + kt][t] = in_sum;
-#pragma unroll
-        for (int f = 0; f < 4; ++f)
-          if ((f >> 1) <= it)
-            mul<32>(dq, col_op<M, 2, RB>(kat, 16 * f, 0),
-                    parts([&](int p) { return row_op<M, 2>(sP + p * kSlab + t * RB, f, half); }));
-      }
-      if constexpr (!kLead) if (any) {
-        f16v &du = main[s], &dS = ds[s];
-        const float wg = sw[kWg * 64 + t], wr = sw[kWr * 64 + t], rate = sw[kWb * 64 + t];
-        float in_sum = 0.0f, out_sum = 0.0f;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float v[4];
-          four(sK + t * RB, 32 * kt + 8 * q + 4 * half, v);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int e = 4 * q + r;
-            dS[e] *= wg;
-            du[e] *= wr;
-            in_sum = fmaf(-v[r], dS[e], in_sum);
-            out_sum = fmaf(v[r], du[e], out_sum);
-            du[e] = fmaf(rate, du[e], -dS[e]);
-          }
-        }
-        in_sum += __shfl_xor(in_sum, 32);
-        out_sum += __shfl_xor(out_sum, 32);
-        if (half == 0) {
-          s_in[1][c0 / 32 + kt][t] = in_sum;
-          s_out[c0 / 32 + kt][t] = out_sum;
-        }
-        const char* const qat = sQ + 32 * kt * ES + col_at;
-#pragma unroll
-        for (int f = 0; f < 4; ++f) {
-          const int jt = f >> 1;
-          const auto kc = col_op<M, 2, RB>(kat, 16 * f, 0);
-          // -(X + X^T), rows of X before the token and columns behind it
-          if (jt <= it) mul<32>(du, kc, parts([&](int p) { return row_op<M, 2>(s_x[p] + t * RB, f, half); }));
-          if (jt >= it) {
-            mul<32>(du, kc, parts([&](int p) { return col_op<M, 2, RB>(s_x[p] + col_at, 16 * f, 32 * it); }));
-            mul<32>(du, col_op<M, 2, RB>(qat, 16 * f, 0),
-                    parts([&](int p) { return col_op<M, 2, RB>(sP + p * kSlab + col_at, 16 * f, 32 * it); }));
-          }
-        }
-      }
-      auto out = [&](void* p, int f32, const f16v& v) {
-        const int size = f32 ? 4 : TS;
-        const rsrc_t r = make_rsrc(static_cast<char*>(p) + (tok0 * A.H + h) * A.Dk * size, 0x7fffffffu);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int col = c0 + 32 * kt + 8 * q + 4 * half;
-          const uint32_t to = (t * A.H * A.Dk + col) * size;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t one = la_in((t < n) & (col + e < A.Dk), to + e * size);
-            if (f32 || A.dtype == PRNN_F32)
-              stb<float>(r, one, 0, v[4 * q + e]);
-            else if (A.dtype == PRNN_F16)
-              stb<f16>(r, one, 0, v[4 * q + e]);
-            else
-              stb<bf16>(r, one, 0, v[4 * q + e]);
-          }
+          for (int r = 0; r < 4; ++r) v[r] = a[r];
         }
       };
-      if constexpr (kNarrow) {
-        // bf16 rows leave by way of LDS, 16 bytes a lane side by side
-        auto put = [&](char* to, const f16v& v) {
+      // the parts of a pair's operand
+      auto parts = [&](auto&& get) {
+        Op<M, P> x;
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            *reinterpret_cast<u2*>(to + t * RB + (32 * kt + 8 * q + 4 * half) * 2) =
-                u2{pack_bf16x2(v[4 * q], v[4 * q + 1]), pack_bf16x2(v[4 * q + 2], v[4 * q + 3])};
+        for (int p = 0; p < P; ++p) {
+          const auto one = get(p);
+          if constexpr (kNarrow)
+            x.p[p] = one.p[0];
+          else
+            x = one;
+        }
+        return x;
+      };
+      const int col_at = col_share<M, 2, RB>(lane);
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const int c0 = p0 + 64 * s;
+        if (c0 >= A.Dk) continue;
+        if (c0 > 0) {
+          ka.fetch(pk, A.k.st, n, c0, A.Dk, A.dtype);
+          kb.fetch(pq, A.q.st, n, c0, A.Dk, A.dtype);
+          __syncthreads();
+          ka.template put<RB>(sK, A.dtype);
+          kb.template put<RB>(sQ, A.dtype);
+          __syncthreads();
+        }
+        const bool any = c0 + 32 * kt < A.Dk;
+        const char* const kat = sK + 32 * kt * ES + col_at;
+        if constexpr (kLead) if (any) {
+          f16v& dq = main[s];
+          const float w = sw[kWg * 64 + t] * A.scale;
+          float in_sum = 0.0f;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float v[4];
+            four(sQ + t * RB, 32 * kt + 8 * q + 4 * half, v);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              dq[4 * q + r] *= w;
+              in_sum = fmaf(v[r], dq[4 * q + r], in_sum);
+            }
+          }
+          in_sum += __shfl_xor(in_sum, 32);
+          if (half == 0) s_in[0][c0 / 32 + kt][t] = in_sum;
+#pragma unroll
+          for (int f = 0; f < 4; ++f)
+            if ((f >> 1) <= it)
+              mul<32>(dq, col_op<M, 2, RB>(kat, 16 * f, 0),
+                      parts([&](int p) { return row_op<M, 2>(sP + p * kSlab + t * RB, f, half); }));
+        }
+        if constexpr (!kLead) if (any) {
+          f16v &du = main[s], &dS = ds[s];
+          const float wg = sw[kWg * 64 + t], wr = sw[kWr * 64 + t], rate = sw[kWb * 64 + t];
+          float in_sum = 0.0f, out_sum = 0.0f;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float v[4];
+            four(sK + t * RB, 32 * kt + 8 * q + 4 * half, v);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int e = 4 * q + r;
+              dS[e] *= wg;
+              du[e] *= wr;
+              in_sum = fmaf(-v[r], dS[e], in_sum);
+              out_sum = fmaf(v[r], du[e], out_sum);
+              du[e] = fmaf(rate, du[e], -dS[e]);
+            }
+          }
+          in_sum += __shfl_xor(in_sum, 32);
+          out_sum += __shfl_xor(out_sum, 32);
+          if (half == 0) {
+            s_in[1][c0 / 32 + kt][t] = in_sum;
+            s_out[c0 / 32 + kt][t] = out_sum;
+          }
+          const char* const qat = sQ + 32 * kt * ES + col_at;
+#pragma unroll
+          for (int f = 0; f < 4; ++f) {
+            const int jt = f >> 1;
+            const auto kc = col_op<M, 2, RB>(kat, 16 * f, 0);
+            // -(X + X^T), rows of X before the token and columns behind it
+            if (jt <= it) mul<32>(du, kc, parts([&](int p) { return row_op<M, 2>(s_x[p] + t * RB, f, half); }));
+            if (jt >= it) {
+              mul<32>(du, kc, parts([&](int p) { return col_op<M, 2, RB>(s_x[p] + col_at, 16 * f, 32 * it); }));
+              mul<32>(du, col_op<M, 2, RB>(qat, 16 * f, 0),
+                      parts([&](int p) { return col_op<M, 2, RB>(sP + p * kSlab + col_at, 16 * f, 32 * it); }));
+            }
+          }
+        }
+        auto out = [&](void* p, int f32, const f16v& v) {
+          const int size = f32 ? 4 : TS;
+          const rsrc_t r = make_rsrc(static_cast<char*>(p) + (tok0 * A.H + h) * A.Dk * size, 0x7fffffffu);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int col = c0 + 32 * kt + 8 * q + 4 * half;
+            const uint32_t to = (t * A.H * A.Dk + col) * size;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t one = la_in((t < n) & (col + e < A.Dk), to + e * size);
+              if (f32 || A.dtype == PRNN_F32)
+                stb<float>(r, one, 0, v[4 * q + e]);
+              else if (A.dtype == PRNN_F16)
+                stb<f16>(r, one, 0, v[4 * q + e]);
+              else
+                stb<bf16>(r, one, 0, v[4 * q + e]);
+            }
+          }
         };
-        auto rows_out = [&](void* p, const char* from) {
-          const rsrc_t r = make_rsrc(static_cast<char*>(p) + (tok0 * A.H + h) * A.Dk * 2, 0x7fffffffu);
-          const int row = tid >> 3, unit = tid & 7, col = c0 + 8 * unit;
-          __builtin_amdgcn_raw_buffer_store_b128(*reinterpret_cast<const u4*>(from + row * RB + unit * 16), r,
-                                                 la_in((row < n) & (col < A.Dk), (row * A.H * A.Dk + col) * 2), 0, 0);
-        };
-        __syncthreads();  // k and q have been read
-        const bool f32 = kLead ? A.q_f32 : A.k_f32;
-        if (any && !f32) put(kLead ? sQ : sK, main[s]);
-        __syncthreads();
-        if (!A.q_f32) rows_out(A.dq, sQ);
-        if (!A.k_f32) rows_out(A.dk, sK);
-        if (any && f32) out(kLead ? A.dq : A.dk, 1, main[s]);
-      } else if (any) {
-        out(kLead ? A.dq : A.dk, kLead ? A.q_f32 : A.k_f32, main[s]);
+        if constexpr (kNarrow) {
+          // bf16 rows leave by way of LDS, 16 bytes a lane side by side
+          auto put = [&](char* to, const f16v& v) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              *reinterpret_cast<u2*>(to + t * RB + (32 * kt + 8 * q + 4 * half) * 2) =
+                  u2{pack_bf16x2(v[4 * q], v[4 * q + 1]), pack_bf16x2(v[4 * q + 2], v[4 * q + 3])};
+          };
+          auto rows_out = [&](void* p, const char* from) {
+            const rsrc_t r = make_rsrc(static_cast<char*>(p) + (tok0 * A.H + h) * A.Dk * 2, 0x7fffffffu);
+            const int row = tid >> 3, unit = tid & 7, col = c0 + 8 * unit;
+            __builtin_amdgcn_raw_buffer_store_b128(*reinterpret_cast<const u4*>(from + row * RB + unit * 16), r,
+                                                   la_in((row < n) & (col < A.Dk), (row * A.H * A.Dk + col) * 2), 0, 0);
+          };
+          __syncthreads();  // k and q have been read
+          const bool f32 = kLead ? A.q_f32 : A.k_f32;
+          if (any && !f32) put(kLead ? sQ : sK, main[s]);
+          __syncthreads();
+          if (!A.q_f32) rows_out(A.dq, sQ);
+          if (!A.k_f32) rows_out(A.dk, sK);
+          if (any && f32) out(kLead ? A.dq : A.dk, 1, main[s]);
+        } else if (any) {
+          out(kLead ? A.dq : A.dk, kLead ? A.q_f32 : A.k_f32, main[s]);
+        }
       }
     }
-  }
   };
   if (lead)
     run(std::true_type{});

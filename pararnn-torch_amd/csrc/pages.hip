@@ -159,6 +159,7 @@ __global__ __launch_bounds__(256) void pages_copy_kernel(Pools P, int slots,
 // A beam's first child keeps its slot; the other children, in order, take the slots of the beams
 // without children, in order, and get a copy.  A workgroup per search; src, dst: the copies, -1 where
 // there is none.  No copy's source is another's destination: one has a child, the other none.
+// Latency: 32 searches of 8 beams 3.8 us, the copies (of 128 KB a slot) 7.5.
 constexpr int kBeams = kPlan;
 __global__ __launch_bounds__(kPlan) void pages_reorder_kernel(int* table, const int* __restrict__ parents,
                                                               int K, int slots, int* src, int* dst) {

@@ -1,6 +1,4 @@
 // Residual norm (residual_norm.h): the forward pass, the sums over rows and the C entry points.
-//
-// Bound by memory where rows are many, by a launch's latency where they are few.
 #include "residual_norm.h"
 
 #include <algorithm>

@@ -20,7 +20,7 @@ PRNN_OK = 0
 PRNN_ERR_VALUE = 1
 PRNN_ERR_TYPE = 2
 PRNN_ERR_RUNTIME = 3
-ABI_VERSION = 15
+ABI_VERSION = 16
 
 class BlockMove(ctypes.Structure):
     """``prnn_block_move``."""

@@ -153,7 +153,8 @@ def delta_rule(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, beta: Tensor,
     ``cu_seqlens``, ``block_table``, ``state_out``, ``state_table`` and ``return_state`` are
     :func:`linear_attention`'s.  Gradients of the output and of the returned states flow to ``q``,
     ``k``, ``v``, ``log_decay``, ``beta`` and ``h0``; between the passes a call keeps what its tokens
-    wrote (as large as the output, or twice that) and the states before its chunks of 64 tokens.
+    wrote (as large as the output, or twice that), the states before its chunks of 64 tokens (likewise
+    for widths of 64) and 26 KB of a chunk's system per head.
     """
     what = "delta_rule"
     _no_tangents(what, q, k, v, log_decay, beta, h0)
