@@ -140,9 +140,9 @@ struct DrWalk {
   const char* sys;
   void* out;                 // forwards: o by the strides below, storage type
   long long o_sb, o_st, o_sh;
-  void* e;                   // forwards: (chunk, H), 64 x Dv as operands, of the arithmetic's type
+  void* e;                   // forwards: (chunk, H), 64 x Dv as operands, bf16 in two parts or fp32
   void* keep;                // (chunk, H), Dk x Dv likewise: states before the chunks, adjoints behind them
-  void* dv;                  // backwards, dense (token, H, Dv): of the arithmetic's type
+  void *dv, *dv_lo;          // backwards, dense (token, H, Dv): of the arithmetic's type, bf16: and what that leaves
   float* dv32;               // or floats besides (heads that are summed afterwards)
   LaState init, last;
   float* piece;              // (piece, H, Dk, Dv): the pieces' own states
@@ -159,7 +159,7 @@ struct DrGrad {
   LaDecay g, b;
   const char* sys;           // only its decays and rates are read
   const void *e, *before, *behind;  // as operands: (chunk, H), 64 x Dv and Dk x Dv
-  const void* dv;            // (token, H, Dv) of the arithmetic's type
+  const void *dv, *dv_lo;    // (token, H, Dv) of the arithmetic's type
   void *dq, *dk;             // (token, H, Dk): the arithmetic's type, or floats (q_f32, k_f32)
   int q_f32, k_f32;
   void *dg, *dbeta;          // (token, H); dg NULL: not wanted, or sums per chunk:

@@ -56,7 +56,7 @@ struct Kept {
 };
 Kept kept_of(void* p, const Problem& a) {
   Carver c(p);
-  const size_t size = on_bf16(a) ? 2 : 4, heads = a.la.H;
+  const size_t size = 4, heads = a.la.H;  // bytes of an element, in two bf16 parts or fp32
   Kept k{};
   const size_t units = dr_units(sequences_of(a), kDrC);
   k.e = c.take(units * heads * dr_operand_elems(kDrC, a.la.Dv) * size);
@@ -68,7 +68,7 @@ Kept kept_of(void* p, const Problem& a) {
 
 struct Scratch {
   char* sys;
-  void *behind, *dv;
+  void *behind, *dv, *dv_lo;
   float* piece;
   uint16_t* transfer;
   float *dq32, *dk32, *dv32, *g_part;
@@ -140,7 +140,8 @@ Scratch carve(void* ws, const Problem& a, const Plan& plan, bool systems, bool b
     s.transfer = static_cast<uint16_t*>(c.take(6 * pieces * dr_operand_elems(a.la.Dk, a.la.Dk)));
   }
   if (backward) {
-    s.behind = c.take(units * heads * dr_operand_elems(a.la.Dk, a.la.Dv) * size);
+    s.behind = c.take(units * heads * dr_operand_elems(a.la.Dk, a.la.Dv) * 4);
+    if (on_bf16(a)) s.dv_lo = c.take(tokens * heads * a.la.Dv * 2);
     // dv is written where it is wanted, unless its heads are summed or it is stored in another type
     const bool sums = a.la.v.heads != a.la.H;
     if (sums || (!on_bf16(a) && a.la.dtype != PRNN_F32)) s.dv = c.take(tokens * heads * a.la.Dv * size);
@@ -250,6 +251,7 @@ int backward(const Problem& a, const prnn_la_view& go, const float* gs, const vo
   w.z = la_view(go, a.la, a.la.Dv);
   w.keep = s.behind;
   w.dv = s.dv ? s.dv : dv;
+  w.dv_lo = s.dv_lo;
   w.dv32 = s.dv32;
   w.init = LaState{const_cast<float*>(gs), nullptr, sequences(a)};
   w.last = LaState{dh0, nullptr, sequences(a)};
@@ -264,6 +266,7 @@ int backward(const Problem& a, const prnn_la_view& go, const float* gs, const vo
   g.sys = k.sys;
   g.e = k.e;
   g.dv = w.dv;
+  g.dv_lo = s.dv_lo;
   g.before = k.before;
   g.behind = s.behind;
   g.q_f32 = s.dq32 != nullptr;

@@ -30,14 +30,18 @@ __global__ __launch_bounds__(512, sizeof(typename M::E) == 2 && KS == 1 ? 4 : 2)
   using E = typename M::E;
   constexpr bool kNarrow = sizeof(E) == 2;
   constexpr int ES = static_cast<int>(sizeof(E));
-  constexpr int kAt = kNarrow ? 4 : 2;  // steps whose operands are under way
+  constexpr int kAt = 2;  // steps whose operands are under way
   constexpr int RB = dr_row_k(kNarrow, 64), P = M::kParts, kSlab = kDrC * RB;
-  __shared__ __align__(16) char lds[(WIDE ? 4 + P : 4) * kSlab], s_x[P][kSlab];
+  // k, q, go, dv (bf16: and what that leaves); the pairs go u^T and X by parts, in the place of go and dv
+  // where those are read once
+  constexpr int kRows = 3 + P, kSlabs = kRows + (WIDE ? 2 * P : 1);
+  __shared__ __align__(16) char lds[kSlabs * kSlab];
   __shared__ float sF[kDrC * kLf], s_in[2][8][kDrC], s_out[8][kDrC];
   __shared__ __align__(16) float sw[kDrW * 64];
   __shared__ float s_through[4], s_own[kDrC], s_into[kDrC], s_waves[8];
   char *const sK = lds, *const sQ = lds + kSlab, *const sG = lds + 2 * kSlab, *const sD = lds + 3 * kSlab;
-  char* const sP = WIDE ? lds + 4 * kSlab : sG;  // the pairs go u^T, by parts
+  char *const sL = lds + 4 * kSlab, *const sP = WIDE ? lds + kRows * kSlab : sG;
+  char* const s_x = WIDE ? lds + (kRows + P) * kSlab : lds + 4 * kSlab;
   const int h = blockIdx.x % A.H, id = blockIdx.x / A.H;
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, half = lane >> 5;
   const int wave = (tid >> 6) & 3;
@@ -57,16 +61,20 @@ __global__ __launch_bounds__(512, sizeof(typename M::E) == 2 && KS == 1 ? 4 : 2)
   };
   const char *pq = rows(A.q), *pk = rows(A.k), *pg = rows(A.go);
   const char* pd = static_cast<const char*>(A.dv) + (tok0 * A.H + h) * A.Dv * ES;
+  const char* pl = kNarrow ? static_cast<const char*>(A.dv_lo) + (tok0 * A.H + h) * A.Dv * ES : nullptr;
   auto operands = [&](const void* p, int r, int c) {
     const size_t elems = dr_operand_elems(r, c);
-    return make_rsrc(static_cast<const E*>(p) + unit * elems, static_cast<uint32_t>(elems) * ES);
+    return make_rsrc(static_cast<const E*>(p) + unit * P * elems, static_cast<uint32_t>(elems) * P * ES);
   };
   const rsrc_t re = operands(A.e, kDrC, A.Dv), rS = operands(A.before, A.Dk, A.Dv),
                rR = operands(A.behind, A.Dk, A.Dv);
+  const int part_e = static_cast<int>(dr_operand_elems(kDrC, A.Dv)) * ES,
+            part_s = static_cast<int>(dr_operand_elems(A.Dk, A.Dv)) * ES;
   const int vs = (A.Dv + 15) / 16, last_k = (A.Dk - 1) / 64 * 64;
-  Staged<M, 64, 512> ga, gb, ka, kb;
+  Staged<M, 64, 512> ga, gb, gl, ka, kb;
   ga.fetch(pg, A.go.st, n, 0, A.Dv, A.dtype);
   gb.fetch(pd, static_cast<long long>(A.H) * A.Dv, n, 0, A.Dv, kCode);
+  if constexpr (kNarrow) gl.fetch(pl, static_cast<long long>(A.H) * A.Dv, n, 0, A.Dv, kCode);
   ka.fetch(pk, A.k.st, n, last_k, A.Dk, A.dtype);
   kb.fetch(pq, A.q.st, n, last_k, A.Dk, A.dtype);
   const float* weights = reinterpret_cast<const float*>(A.sys + unit * kDrSys + 2 * kDrTiles);
@@ -74,6 +82,7 @@ __global__ __launch_bounds__(512, sizeof(typename M::E) == 2 && KS == 1 ? 4 : 2)
   for (int i = tid; i < kDrW * 64; i += 512) sw[i] = weights[i];
   ga.template put<RB>(sG, A.dtype);
   gb.template put<RB>(sD, kCode);
+  if constexpr (kNarrow) gl.template put<RB>(sL, kCode);
   ka.template put<RB>(sK, A.dtype);
   kb.template put<RB>(sQ, A.dtype);
 
@@ -86,19 +95,29 @@ __global__ __launch_bounds__(512, sizeof(typename M::E) == 2 && KS == 1 ? 4 : 2)
     constexpr bool kLead = decltype(role)::value;
     // operands of a wave's tiles of the states and of its tokens' e; the pairs' earlier tokens are the
     // same ones (waves 0 and 1: the first 32, wave 2: the others)
-    Op<M, 1> ei[kAt], S[KS][kAt], R[KS][kAt];
+    Op<M, P> ei[kAt], S[KS][kAt], R[KS][kAt];
     auto fetch = [&](int p0, int v0, int f0) {
 #pragma unroll
       for (int f = 0; f < kAt; ++f) {
         const int step = v0 / 16 + f0 + f;
-        ei[f] = global_op<M>(re, step < vs, it * vs + step);
+        ei[f] = global_op<M>(re, step < vs, it * vs + step, part_e);
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
           const int tile = p0 / 32 + 2 * s + kt;
-          S[s][f] = global_op<M>(rS, (step < vs) & (32 * tile < A.Dk), tile * vs + step);
-          if constexpr (!kLead) R[s][f] = global_op<M>(rR, (step < vs) & (32 * tile < A.Dk), tile * vs + step);
+          S[s][f] = global_op<M>(rS, (step < vs) & (32 * tile < A.Dk), tile * vs + step, part_s);
+          if constexpr (!kLead) R[s][f] = global_op<M>(rR, (step < vs) & (32 * tile < A.Dk), tile * vs + step, part_s);
         }
       }
+    };
+    auto dv_op = [&](int token, int f) {
+      Op<M, P> o;
+      if constexpr (kNarrow) {
+        o.p[0] = row_op<M, 2>(sD + token * RB, f, half).p[0];
+        o.p[1] = row_op<M, 2>(sL + token * RB, f, half).p[0];
+      } else {
+        o = row_op<M, 2>(sD + token * RB, f, half);
+      }
+      return o;
     };
     const bool pairs = kLead && wave < 3;
 
@@ -116,9 +135,11 @@ __global__ __launch_bounds__(512, sizeof(typename M::E) == 2 && KS == 1 ? 4 : 2)
         if (p0 > 0 || v0 > 0) {
           ga.fetch(pg, A.go.st, n, v0, A.Dv, A.dtype);
           gb.fetch(pd, static_cast<long long>(A.H) * A.Dv, n, v0, A.Dv, kCode);
+          if constexpr (kNarrow) gl.fetch(pl, static_cast<long long>(A.H) * A.Dv, n, v0, A.Dv, kCode);
           __syncthreads();
           ga.template put<RB>(sG, A.dtype);
           gb.template put<RB>(sD, kCode);
+          if constexpr (kNarrow) gl.template put<RB>(sL, kCode);
         }
         fetch(p0, v0, 0);
         __syncthreads();
@@ -133,13 +154,13 @@ __global__ __launch_bounds__(512, sizeof(typename M::E) == 2 && KS == 1 ? 4 : 2)
               for (int s = 0; s < KS; ++s) mul<32>(main[s], S[s][f], gi);
               if (p0 == 0 && pairs) {
                 mul<32>(GU, ei[f], row_op<M, 2>(sG + i * RB, f0 + f, half));
-                mul<32>(DU, ei[f], row_op<M, 2>(sD + i * RB, f0 + f, half));
+                mul<32>(DU, ei[f], dv_op(i, f0 + f));
               }
             }
           } else {
 #pragma unroll
             for (int f = 0; f < kAt; ++f) {
-              const auto di = row_op<M, 2>(sD + t * RB, f0 + f, half);
+              const auto di = dv_op(t, f0 + f);
 #pragma unroll
               for (int s = 0; s < KS; ++s) {
                 mul<32>(main[s], R[s][f], ei[f]);
@@ -207,10 +228,10 @@ __global__ __launch_bounds__(512, sizeof(typename M::E) == 2 && KS == 1 ? 4 : 2)
                 *reinterpret_cast<u2*>(lo + i * RB + j0 * 2) = b;
               };
               both(sP, sP + kSlab, w1);
-              both(s_x[0], s_x[P - 1], x);
+              both(s_x, s_x + kSlab, x);
             } else {
               *reinterpret_cast<f4*>(sP + i * RB + j0 * 4) = f4{w1[0], w1[1], w1[2], w1[3]};
-              *reinterpret_cast<f4*>(s_x[0] + i * RB + j0 * 4) = f4{x[0], x[1], x[2], x[3]};
+              *reinterpret_cast<f4*>(s_x + i * RB + j0 * 4) = f4{x[0], x[1], x[2], x[3]};
             }
           }
         }
@@ -309,9 +330,9 @@ __global__ __launch_bounds__(512, sizeof(typename M::E) == 2 && KS == 1 ? 4 : 2)
             const int jt = f >> 1;
             const auto kc = col_op<M, 2, RB>(kat, 16 * f, 0);
             // -(X + X^T), rows of X before the token and columns behind it
-            if (jt <= it) mul<32>(du, kc, parts([&](int p) { return row_op<M, 2>(s_x[p] + t * RB, f, half); }));
+            if (jt <= it) mul<32>(du, kc, parts([&](int p) { return row_op<M, 2>(s_x + p * kSlab + t * RB, f, half); }));
             if (jt >= it) {
-              mul<32>(du, kc, parts([&](int p) { return col_op<M, 2, RB>(s_x[p] + col_at, 16 * f, 32 * it); }));
+              mul<32>(du, kc, parts([&](int p) { return col_op<M, 2, RB>(s_x + p * kSlab + col_at, 16 * f, 32 * it); }));
               mul<32>(du, col_op<M, 2, RB>(qat, 16 * f, 0),
                       parts([&](int p) { return col_op<M, 2, RB>(sP + p * kSlab + col_at, 16 * f, 32 * it); }));
             }

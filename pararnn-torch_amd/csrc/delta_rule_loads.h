@@ -69,15 +69,17 @@ struct Staged {
   }
 };
 
-// Operand `which` of an array of them (dr_operand_at).
+// Operand `which` of an array of them (dr_operand_at), its parts `part` bytes apart.
 template <class M>
-__device__ __forceinline__ Op<M, 1> global_op(rsrc_t r, bool in, int which) {
+__device__ __forceinline__ Op<M, M::kParts> global_op(rsrc_t r, bool in, int which, int part) {
   constexpr int ES = static_cast<int>(sizeof(typename M::E));
   const int lane = threadIdx.x & 63;
-  Op<M, 1> o;
+  Op<M, M::kParts> o;
   if constexpr (ES == 2) {
-    o.p[0] = __builtin_bit_cast(
-        b8, __builtin_amdgcn_raw_buffer_load_b128(r, la_in(in, (which * 64 + lane) * 16), 0, 0));
+#pragma unroll
+    for (int k = 0; k < M::kParts; ++k)
+      o.p[k] = __builtin_bit_cast(
+          b8, __builtin_amdgcn_raw_buffer_load_b128(r, la_in(in, (which * 64 + lane) * 16 + k * part), 0, 0));
   } else {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {

@@ -254,7 +254,8 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
   // What a chunk leaves is stored after the next one's rows have come: loads and stores come back in
   // order, and a wait for rows behind stores would wait for those too.
   constexpr int kHeld = kNarrow ? NC / 2 : NC;
-  uint32_t held_o[KIND == kDrForward ? kHeld : 1], held_u[kOwn ? 1 : kHeld];  // out; e or dv
+  // out; e or dv, and what bf16 leaves of them
+  uint32_t held_o[KIND == kDrForward ? kHeld : 1], held_u[kOwn ? 1 : kHeld], held_l[kOwn || !kNarrow ? 1 : kHeld];
   float held32[KIND == kDrBackward && kNarrow ? NC : 1];
   int held_n = 0, held_c = 0;
   auto at_token = [&](int i) { return NC * (i / RT) + 4 * G * ((i % RT) >> 2) + 4 * g + (i & 3); };
@@ -306,21 +307,28 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
         to[i] = __float_as_uint(v[i]);
     }
   };
-  auto hold_rows = [&](uint32_t* to, float* v) {
+  auto hold_rows = [&](float* v) {
     if constexpr (kNarrow) {
-      Op<M, 1> o[TF];
+      Op<M, 1> o[2][TF];
 #pragma unroll
-      for (int f = 0; f < TF; ++f) o[f] = parts_of<M, 1>(v + 8 * f);
-      float d[NC];
-#pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        const A_t x = turned(o, t);
-#pragma unroll
-        for (int r = 0; r < RT; ++r) d[RT * t + r] = x[r];
+      for (int f = 0; f < TF; ++f) {
+        const auto both = parts_of<M, 2>(v + 8 * f);
+        o[0][f].p[0] = both.p[0];
+        o[1][f].p[0] = both.p[1];
       }
-      hold(to, d);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        float d[NC];
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+          const A_t x = turned(o[p], t);
+#pragma unroll
+          for (int r = 0; r < RT; ++r) d[RT * t + r] = x[r];
+        }
+        hold(p ? held_l : held_u, d);
+      }
     } else {
-      hold(to, v);
+      hold(held_u, v);
     }
   };
   auto flush = [&]() {
@@ -364,18 +372,20 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
         const int step = A.H * A.Dv * ES;
         const size_t elems = dr_operand_elems(kDrC, A.Dv);
         const rsrc_t r = kBack ? make_rsrc(static_cast<E*>(p) + ((tok0 + t0) * A.H + h) * A.Dv, (n - 1) * step + A.Dv * ES)
-                               : make_rsrc(static_cast<E*>(p) + (static_cast<size_t>(row0 + held_c) * A.H + h) * elems,
-                                           static_cast<uint32_t>(elems) * ES);
+                               : make_rsrc(static_cast<E*>(p) + (static_cast<size_t>(row0 + held_c) * A.H + h) * M::kParts * elems,
+                                           static_cast<uint32_t>(elems) * M::kParts * ES);
         const uint32_t lane_at = kBack ? la_in(col < A.Dv, 4 * g * step + col * ES) : operand_lane;
         if constexpr (kNarrow) {
+          const rsrc_t rl = kBack ? make_rsrc(static_cast<E*>(A.dv_lo) + ((tok0 + t0) * A.H + h) * A.Dv, (n - 1) * step + A.Dv * ES) : r;
 #pragma unroll
           for (int t = 0; t < TT; ++t)
 #pragma unroll
             for (int q = 0; q < RT / 4; ++q) {
               const int i = (RT * t + 4 * q) / 2, tok = NC * t + nn, cc = col0 + NC * wave + 4 * G * q + 4 * g;
-              __builtin_amdgcn_raw_buffer_store_b64(
-                  u2{held_u[i], held_u[i + 1]}, r,
-                  kBack ? la_in(cc < A.Dv, tok * step + cc * 2) : operand8(tok, q), 0, 0);
+              const uint32_t to = kBack ? la_in(cc < A.Dv, tok * step + cc * 2) : operand8(tok, q);
+              __builtin_amdgcn_raw_buffer_store_b64(u2{held_u[i], held_u[i + 1]}, r, to, 0, 0);
+              __builtin_amdgcn_raw_buffer_store_b64(u2{held_l[i], held_l[i + 1]}, rl,
+                                                    kBack ? to : to + static_cast<uint32_t>(elems) * 2, 0, 0);
             }
         }
 #pragma unroll
@@ -437,14 +447,27 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
     for (int t = 0; t < TT; ++t)
 #pragma unroll
       for (int r = 0; r < RT; ++r) X[t][r] = O[t][r] = 0.0f;
-    Op<M, 1> rounded[kNarrow && !kOwn ? KF : 1];
+    Op<M, 1> rounded[2][kNarrow && !kOwn ? KF : 1];  // by parts
 #pragma unroll
     for (int f = 0; f < KF; ++f) {
       float s[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) s[e] = S[(8 * f + e) / RT][(8 * f + e) % RT];
-      const auto sp = parts_of<M, 2>(s);
-      if constexpr (kNarrow && !kOwn) rounded[f].p[0] = sp.p[0];
+      // three parts in the chain (16 bits of a state would be 1e-6 of it after some hundred tokens), two
+      // where an output is rounded
+      const auto sp = parts_of<M, 3>(s);
+      Op<M, 2> so;
+      if constexpr (kNarrow) {
+        so.p[0] = sp.p[0];
+        so.p[1] = sp.p[1];
+        if constexpr (!kOwn) {
+          rounded[0][f].p[0] = sp.p[0];
+          rounded[1][f].p[0] = sp.p[1];
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) so.x[e] = sp.x[e];
+      }
       Op<M, 1> ko[TT], qo[TT];
 #pragma unroll
       for (int t = 0; t < TT; ++t) {
@@ -452,28 +475,32 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
         if constexpr (KIND == kDrForward) qo[t] = row_op<M, G>(sQ + (NC * t + nn) * RK, f, g);
       }
 #pragma unroll
-      for (int k = 0; k < kPairs<1, 2>; ++k)
+      for (int k = 0; k < kPairs<1, 3>; ++k)
 #pragma unroll
         for (int t = 0; t < TT; ++t) {
           mul_one<NC>(X[t], ko[t], sp, k);
-          if constexpr (KIND == kDrForward) mul_one<NC>(O[t], sp, qo[t], k);
+          if constexpr (KIND == kDrForward)
+            if (k < kPairs<1, 2>) mul_one<NC>(O[t], so, qo[t], k);
         }
     }
 
     if constexpr (kNarrow && !kOwn) {
       if (A.keep) {
         const size_t elems = dr_operand_elems(A.Dk, A.Dv);
-        const rsrc_t rs = make_rsrc(static_cast<E*>(A.keep) + (static_cast<size_t>(row0 + c) * A.H + h) * elems,
-                                    static_cast<uint32_t>(elems) * ES);
+        const rsrc_t rs = make_rsrc(static_cast<E*>(A.keep) + (static_cast<size_t>(row0 + c) * A.H + h) * 2 * elems,
+                                    static_cast<uint32_t>(elems) * 2 * ES);
 #pragma unroll
         for (int t = 0; t < KT; ++t) {
           if (NC * t >= (A.Dk + 31) / 32 * 32) continue;  // rows behind the matrix: zeros up to the end of its tile
-          const A_t d = turned(rounded, t);
 #pragma unroll
-          for (int q = 0; q < RT / 4; ++q)
-            __builtin_amdgcn_raw_buffer_store_b64(
-                u2{pack_bf16x2(d[4 * q], d[4 * q + 1]), pack_bf16x2(d[4 * q + 2], d[4 * q + 3])}, rs,
-                operand8(NC * t + nn, q), 0, 0);
+          for (int p = 0; p < 2; ++p) {
+            const A_t d = turned(rounded[p], t);
+#pragma unroll
+            for (int q = 0; q < RT / 4; ++q)
+              __builtin_amdgcn_raw_buffer_store_b64(
+                  u2{pack_bf16x2(d[4 * q], d[4 * q + 1]), pack_bf16x2(d[4 * q + 2], d[4 * q + 3])}, rs,
+                  operand8(NC * t + nn, q) + p * static_cast<uint32_t>(elems) * 2, 0, 0);
+          }
         }
       }
     }
@@ -554,13 +581,13 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
     }
 
     // ---- (1 + T) y
-    Op<M, 2> yo[TF];
+    Op<M, 3> yo[TF];
 #pragma unroll
     for (int f = 0; f < TF; ++f) {
       float v[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = y[8 * f + e];
-      yo[f] = parts_of<M, 2>(v);
+      yo[f] = parts_of<M, 3>(v);
     }
 #pragma unroll
     for (int t = 0; t < TT; ++t)
@@ -573,7 +600,7 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
       for (int t = 0; t < TT; ++t)
         if (Mat::any(t, f)) m[t] = Mat::get(sS, t, f, nn, g);
 #pragma unroll
-      for (int k = 0; k < kPairs<M::kParts, 2>; ++k)
+      for (int k = 0; k < kPairs<M::kParts, 3>; ++k)
 #pragma unroll
         for (int t = 0; t < TT; ++t)
           if (Mat::any(t, f)) mul_one<NC>(Y[t], m[t], yo[f], k);
@@ -635,14 +662,14 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
 #pragma unroll
         for (int i = 0; i < NC; ++i)
           v[i] = at_token(i) >= stop ? __int_as_float(0x7fc00000) : Y[i / RT][i % RT];
-        hold_rows(held_u, v);
+        hold_rows(v);
       }
     }
     if constexpr (KIND == kDrBackward) {
       float dv[NC];
 #pragma unroll
       for (int i = 0; i < NC; ++i) dv[i] = u[i];
-      hold_rows(held_u, dv);
+      hold_rows(dv);
       if constexpr (kNarrow) {
 #pragma unroll
         for (int i = 0; i < NC; ++i) held32[i] = u[i];

@@ -88,11 +88,12 @@ __device__ __forceinline__ void mul(Acc<NC>& c, const Op<InF32, P>& a, const Op<
 // The same product by product, so that several sums can take turns (a matrix instruction waits for the
 // last one of its own sum): products kPairs<P, R> of operands of P and R parts, number k of them.
 template <int P, int R>
-constexpr int kPairs = P == 1 || R == 1 ? P * R : 3;  // (two parts each: the small ones' product is left out)
+constexpr int kPairs = P == 1 || R == 1 ? P * R : R == 2 ? 3 : 5;  // (of two parts and two or three the largest)
 template <int NC, int P, int R>
 __device__ __forceinline__ void mul_one(Acc<NC>& c, const Op<InBf16, P>& a, const Op<InBf16, R>& b, int k) {
-  static_assert(P == 1 || R == 1 || (P == 2 && R == 2), "products are listed for these");
-  const int i = P == 1 ? 0 : R == 1 ? k : k == 2, j = P == 1 ? k : R == 1 ? 0 : k == 1;
+  static_assert(P == 1 || R == 1 || (P == 2 && (R == 2 || R == 3)), "products are listed for these");
+  const int i = P == 1 ? 0 : R == 1 ? k : k == 2 || k == 4;
+  const int j = P == 1 ? k : R == 1 ? 0 : k == 3 ? 2 : k == 1 || k == 4;
   c = mfma_bf16<NC>(a.p[i], b.p[j], c);
 }
 template <int NC, int P, int R>
@@ -155,6 +156,14 @@ __device__ __forceinline__ void values(const Op<InBf16, 1>& o, float* x) {
 __device__ __forceinline__ void values(const Op<InF32, 1>& o, float* x) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] = o.x[i];
+}
+
+__device__ __forceinline__ void values(const Op<InBf16, 2>& o, float* x) {
+  float y[8];
+  values(Op<InBf16, 1>{{o.p[0]}}, x);
+  values(Op<InBf16, 1>{{o.p[1]}}, y);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] += y[i];
 }
 
 // Step f of a contraction along a row in memory, `g` the lane's group.
