@@ -212,11 +212,10 @@ int run(DrWalk w, DrKind kind, const Problem& a, const Plan& plan, hipStream_t s
 int walk(const DrWalk& w, bool back, const Problem& a, const Plan& plan, hipStream_t st) {
   if (plan.cut) {
     DrWalk own = w;
-    own.keep = nullptr;
     if (int rc = run(own, back ? kDrAdjoint : kDrState, a, plan, st)) return rc;
     if (int rc = dr_join(w, back, st)) return rc;
   }
-  return run(w, back ? kDrBackward : kDrForward, a, plan, st);
+  return run(w, back ? kDrBackward : w.keep ? kDrKept : kDrForward, a, plan, st);
 }
 
 int forward(const Problem& a, const prnn_la_view& out, float* state_out, const int* out_table, int out_rows,

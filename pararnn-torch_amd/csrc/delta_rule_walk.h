@@ -127,6 +127,7 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
   constexpr bool kNarrow = sizeof(E) == 2;
   constexpr bool kBack = KIND == kDrBackward || KIND == kDrAdjoint;
   constexpr bool kOwn = KIND == kDrState || KIND == kDrAdjoint;  // pieces' own states only
+  constexpr bool kOut = KIND == kDrForward || KIND == kDrKept, kKeeps = KIND == kDrKept || KIND == kDrBackward;
   constexpr int G = 64 / NC, NT = 64 * (L ? L : W), VT = NC * W;  // NT: threads that bring rows
   constexpr int RT = NC * NC / 64;   // registers of a tile
   constexpr int KT = KD / NC;        // the state's tiles
@@ -255,7 +256,7 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
   // order, and a wait for rows behind stores would wait for those too.
   constexpr int kHeld = kNarrow ? NC / 2 : NC;
   // out; e or dv, and what bf16 leaves of them
-  uint32_t held_o[KIND == kDrForward ? kHeld : 1], held_u[kOwn ? 1 : kHeld], held_l[kOwn || !kNarrow ? 1 : kHeld];
+  uint32_t held_o[kOut ? kHeld : 1], held_u[kKeeps ? kHeld : 1], held_l[kKeeps && kNarrow ? kHeld : 1];
   float held32[KIND == kDrBackward && kNarrow ? NC : 1];
   int held_n = 0, held_c = 0;
   auto at_token = [&](int i) { return NC * (i / RT) + 4 * G * ((i % RT) >> 2) + 4 * g + (i & 3); };
@@ -271,7 +272,7 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
   // bf16: what is stored is turned by a product with the unit matrix (exact), so that a lane has four
   // columns of a row and not a row's place in four of them: 8 bytes a store and not 2.
   Op<M, 1> unit[2];
-  if constexpr (kNarrow && !kOwn) {
+  if constexpr (kNarrow && kKeeps) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int place = NC == 32 ? nn - 16 * j : nn + 16 * j;  // of the contraction that is this lane's column
@@ -293,10 +294,19 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
     }
     return d;
   };
-  auto operand8 = [&](int row, int q) {  // place of columns 4 G q + 4 g .. + 3 of the wave's at `row`
-    const int cc = col0 + NC * wave + 4 * G * q + 4 * g;
-    return la_in(cc < v_steps * 16, (((row >> 5) * v_steps + (cc >> 4)) * 64 + (row & 31) + 32 * ((cc >> 2) & 1)) * 16 +
-                                        ((cc >> 3) & 1) * 8);
+  // Of such rows, for memory as operands: four words are a lane's 8 places of a step.  NC = 32: as they
+  // come, words 4 j .. of tile j / 2 and step j % 2; 16: of tiles 2 j and 2 j + 1, halves of the wave exchange theirs.
+  auto paired = [&](uint32_t* w) {
+    if constexpr (NC == 16) {
+      swap_halves(w[0], w[2]);
+      swap_halves(w[1], w[3]);
+    }
+    return u4{w[0], w[1], w[2], w[3]};
+  };
+  auto operand16 = [&](int j) {  // their place
+    const int row = NC == 32 ? 32 * (j >> 1) + nn : 16 * (2 * j + (lane >> 5)) + nn;
+    const int step = (col0 + NC * wave + (NC == 32 ? 16 * (j & 1) : 0)) >> 4;
+    return la_in(step < v_steps, (((row >> 5) * v_steps + step) * 64 + (row & 31) + 32 * (g & 1)) * 16);
   };
   auto hold = [&](uint32_t* to, const float* v) {
 #pragma unroll
@@ -333,7 +343,7 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
   };
   auto flush = [&]() {
     const int t0 = pc.begin + held_c * kDrC, n = held_n;  // nothing held: 0 tokens
-    if constexpr (KIND == kDrForward) {
+    if constexpr (kOut) {
       const int step = static_cast<int>(A.o_st) * size, c0 = col0 + NC * wave + 4 * g;
       const rsrc_t ro = make_rsrc(static_cast<char*>(A.out) + (batch * A.o_sb + h * A.o_sh +
                                                                static_cast<long long>(t0) * A.o_st) * size,
@@ -364,9 +374,9 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
         }
       }
     }
-    if constexpr (!kOwn) {
-      void* p = kBack ? A.dv : A.e;
-      if (p && n > 0) {
+    if constexpr (kKeeps) {
+      void* const p = kBack ? A.dv : A.e;
+      if (n > 0) {
         // backwards dense rows of the tokens that are there (the others lie behind the buffer), forwards
         // operands (zeros behind the sequence)
         const int step = A.H * A.Dv * ES;
@@ -376,16 +386,23 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
                                            static_cast<uint32_t>(elems) * M::kParts * ES);
         const uint32_t lane_at = kBack ? la_in(col < A.Dv, 4 * g * step + col * ES) : operand_lane;
         if constexpr (kNarrow) {
+          if constexpr (!kBack) {
+#pragma unroll
+            for (int j = 0; j < kHeld / 4; ++j) {
+              const uint32_t to = operand16(j);
+              __builtin_amdgcn_raw_buffer_store_b128(paired(held_u + 4 * j), r, to, 0, 0);
+              __builtin_amdgcn_raw_buffer_store_b128(paired(held_l + 4 * j), r, to + static_cast<uint32_t>(elems) * 2, 0, 0);
+            }
+          }
           const rsrc_t rl = kBack ? make_rsrc(static_cast<E*>(A.dv_lo) + ((tok0 + t0) * A.H + h) * A.Dv, (n - 1) * step + A.Dv * ES) : r;
 #pragma unroll
-          for (int t = 0; t < TT; ++t)
+          for (int t = 0; t < (kBack ? TT : 0); ++t)
 #pragma unroll
             for (int q = 0; q < RT / 4; ++q) {
               const int i = (RT * t + 4 * q) / 2, tok = NC * t + nn, cc = col0 + NC * wave + 4 * G * q + 4 * g;
-              const uint32_t to = kBack ? la_in(cc < A.Dv, tok * step + cc * 2) : operand8(tok, q);
+              const uint32_t to = la_in(cc < A.Dv, tok * step + cc * 2);
               __builtin_amdgcn_raw_buffer_store_b64(u2{held_u[i], held_u[i + 1]}, r, to, 0, 0);
-              __builtin_amdgcn_raw_buffer_store_b64(u2{held_l[i], held_l[i + 1]}, rl,
-                                                    kBack ? to : to + static_cast<uint32_t>(elems) * 2, 0, 0);
+              __builtin_amdgcn_raw_buffer_store_b64(u2{held_l[i], held_l[i + 1]}, rl, to, 0, 0);
             }
         }
 #pragma unroll
@@ -422,7 +439,7 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
     if constexpr (L == 0) put(at, c);
     if (!kOwn) flush();
     // what the gradients of this chunk need of the state
-    if (!kOwn && !kNarrow && A.keep) {
+    if constexpr (kKeeps && !kNarrow) {
       const size_t elems = dr_operand_elems(A.Dk, A.Dv);
       const rsrc_t rs = make_rsrc(static_cast<E*>(A.keep) + (static_cast<size_t>(row0 + c) * A.H + h) * elems,
                                   static_cast<uint32_t>(elems) * ES);
@@ -447,7 +464,7 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
     for (int t = 0; t < TT; ++t)
 #pragma unroll
       for (int r = 0; r < RT; ++r) X[t][r] = O[t][r] = 0.0f;
-    Op<M, 1> rounded[2][kNarrow && !kOwn ? KF : 1];  // by parts
+    Op<M, 1> rounded[2][kNarrow && kKeeps ? KF : 1];  // by parts
 #pragma unroll
     for (int f = 0; f < KF; ++f) {
       float s[8];
@@ -460,7 +477,7 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
       if constexpr (kNarrow) {
         so.p[0] = sp.p[0];
         so.p[1] = sp.p[1];
-        if constexpr (!kOwn) {
+        if constexpr (kKeeps) {
           rounded[0][f].p[0] = sp.p[0];
           rounded[1][f].p[0] = sp.p[1];
         }
@@ -472,35 +489,38 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
 #pragma unroll
       for (int t = 0; t < TT; ++t) {
         ko[t] = row_op<M, G>(sK + (NC * t + nn) * RK, f, g);
-        if constexpr (KIND == kDrForward) qo[t] = row_op<M, G>(sQ + (NC * t + nn) * RK, f, g);
+        if constexpr (kOut) qo[t] = row_op<M, G>(sQ + (NC * t + nn) * RK, f, g);
       }
 #pragma unroll
       for (int k = 0; k < kPairs<1, 3>; ++k)
 #pragma unroll
         for (int t = 0; t < TT; ++t) {
           mul_one<NC>(X[t], ko[t], sp, k);
-          if constexpr (KIND == kDrForward)
+          if constexpr (kOut)
             if (k < kPairs<1, 2>) mul_one<NC>(O[t], so, qo[t], k);
         }
     }
 
-    if constexpr (kNarrow && !kOwn) {
-      if (A.keep) {
-        const size_t elems = dr_operand_elems(A.Dk, A.Dv);
-        const rsrc_t rs = make_rsrc(static_cast<E*>(A.keep) + (static_cast<size_t>(row0 + c) * A.H + h) * 2 * elems,
-                                    static_cast<uint32_t>(elems) * 2 * ES);
+    if constexpr (kNarrow && kKeeps) {
+      const size_t elems = dr_operand_elems(A.Dk, A.Dv);
+      const rsrc_t rs = make_rsrc(static_cast<E*>(A.keep) + (static_cast<size_t>(row0 + c) * A.H + h) * 2 * elems,
+                                  static_cast<uint32_t>(elems) * 2 * ES);
 #pragma unroll
-        for (int t = 0; t < KT; ++t) {
-          if (NC * t >= (A.Dk + 31) / 32 * 32) continue;  // rows behind the matrix: zeros up to the end of its tile
+      for (int t = 0; t < KT; t += 32 / NC) {
+        if (NC * t >= A.Dk) continue;  // (rows behind the matrix: zeros up to the end of its tile of 32)
 #pragma unroll
-          for (int p = 0; p < 2; ++p) {
-            const A_t d = turned(rounded[p], t);
+        for (int p = 0; p < 2; ++p) {
+          uint32_t w[8];
 #pragma unroll
-            for (int q = 0; q < RT / 4; ++q)
-              __builtin_amdgcn_raw_buffer_store_b64(
-                  u2{pack_bf16x2(d[4 * q], d[4 * q + 1]), pack_bf16x2(d[4 * q + 2], d[4 * q + 3])}, rs,
-                  operand8(NC * t + nn, q) + p * static_cast<uint32_t>(elems) * 2, 0, 0);
+          for (int k = 0; k < 32 / NC; ++k) {
+            const A_t d = turned(rounded[p], t + k);
+#pragma unroll
+            for (int r = 0; r < RT; r += 2) w[(RT * k + r) / 2] = pack_bf16x2(d[r], d[r + 1]);
           }
+#pragma unroll
+          for (int j = 0; j < NC / 16; ++j)
+            __builtin_amdgcn_raw_buffer_store_b128(
+                paired(w + 4 * j), rs, operand16(NC * t / 32 * (NC / 16) + j) + p * static_cast<uint32_t>(elems) * 2, 0, 0);
         }
       }
     }
@@ -619,7 +639,7 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
         if (at_token(i) >= stop) u[i] = 0.0f;
     }
 
-    if constexpr (KIND == kDrForward) {
+    if constexpr (kOut) {
       // ---- out
       Op<M, 2> uo[TF];
 #pragma unroll
@@ -658,7 +678,7 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
 #pragma unroll
       for (int i = 0; i < NC; ++i) v[i] = O[i / RT][i % RT];
       hold(held_o, v);
-      if (A.e) {
+      if constexpr (KIND == kDrKept) {
 #pragma unroll
         for (int i = 0; i < NC; ++i)
           v[i] = at_token(i) >= stop ? __int_as_float(0x7fc00000) : Y[i / RT][i % RT];
@@ -777,6 +797,28 @@ int dr_launch_walk(const DrWalk& a, hipStream_t stream) {
   dr_walk_kernel<M, NC, KD, W, L, KIND><<<static_cast<unsigned>(groups), 64 * (W + L), 0, stream>>>(a);
   PRNN_HIP(hipGetLastError());
   return PRNN_OK;
+}
+
+// On bf16 matrix instructions.
+template <int KIND, int KD>
+int dr_launch_cols(const DrWalk& a, int cols, hipStream_t stream) {
+  // Waves that only load: not for pieces' own states, of which two workgroups a CU run without (D = 128,
+  // 512 of them: 74 us, 87 with), nor where two chunks do not fit LDS.
+  constexpr int kLoad = KD <= 128 && KIND != kDrState && KIND != kDrAdjoint ? 4 : 0;
+  if (cols == 16 && a.group == 4) return dr_launch_walk<InBf16, 16, KD, 4, kLoad, KIND>(a, stream);
+  if constexpr (KD <= 128) {
+    if (cols == 16) return dr_launch_walk<InBf16, 16, KD, 2, kLoad, KIND>(a, stream);
+    if (a.group == 4) return dr_launch_walk<InBf16, 32, KD, 4, 0, KIND>(a, stream);
+    if constexpr (KD <= 64) return dr_launch_walk<InBf16, 32, KD, 2, 0, KIND>(a, stream);
+  }
+  return fail(PRNN_ERR_RUNTIME, "no walk of %d columns a wave for keys of %d", cols, a.Dk);
+}
+template <int KIND>
+int dr_launch_bf16(const DrWalk& a, int cols, hipStream_t stream) {
+  if (a.Dk <= 32) return dr_launch_cols<KIND, 32>(a, cols, stream);
+  if (a.Dk <= 64) return dr_launch_cols<KIND, 64>(a, cols, stream);
+  if (a.Dk <= 128) return dr_launch_cols<KIND, 128>(a, cols, stream);
+  return dr_launch_cols<KIND, 256>(a, cols, stream);
 }
 
 }  // namespace prnn

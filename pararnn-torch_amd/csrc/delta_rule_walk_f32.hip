@@ -19,6 +19,7 @@ int launch_kd(const DrWalk& a, hipStream_t stream) {
 int dr_walk_f32(const DrWalk& a, DrKind kind, hipStream_t stream) {
   switch (kind) {
     case kDrForward: return launch_kd<kDrForward>(a, stream);
+    case kDrKept: return launch_kd<kDrKept>(a, stream);
     case kDrState: return launch_kd<kDrState>(a, stream);
     case kDrBackward: return launch_kd<kDrBackward>(a, stream);
     default: return launch_kd<kDrAdjoint>(a, stream);
