@@ -61,7 +61,7 @@ Kept kept_of(void* p, const Problem& a) {
   const size_t units = dr_units(sequences_of(a), kDrC);
   k.e = c.take(units * heads * dr_operand_elems(kDrC, a.la.Dv) * size);
   k.before = c.take(units * heads * dr_operand_elems(a.la.Dk, a.la.Dv) * size);
-  k.sys = static_cast<char*>(c.take(units * heads * kDrSys));
+  k.sys = static_cast<char*>(c.take(units * heads * dr_sys_bytes(on_bf16(a))));
   k.bytes = c.used;
   return k;
 }
@@ -133,7 +133,7 @@ Scratch carve(void* ws, const Problem& a, const Plan& plan, bool systems, bool b
   Scratch s{};
   const size_t heads = a.la.H, tokens = tokens_of(a), size = on_bf16(a) ? 2 : 4;
   const size_t units = dr_units(plan.seqs, kDrC);
-  if (systems) s.sys = static_cast<char*>(c.take(units * heads * kDrSys));
+  if (systems) s.sys = static_cast<char*>(c.take(units * heads * dr_sys_bytes(on_bf16(a))));
   if (plan.cut) {
     const size_t pieces = dr_units(plan.seqs, plan.seqs.len) * heads;
     s.piece = static_cast<float*>(c.take(4 * pieces * a.la.Dk * a.la.Dv));
@@ -168,7 +168,7 @@ LaDecay decay_of(const Problem& a) {
 }
 LaDecay rate_of(const Problem& a) { return LaDecay{a.b, a.b_sb, a.b_st, a.b_sh, a.b_dtype}; }
 
-int systems(const Problem& a, char* sys, hipStream_t st) {
+int systems(const Problem& a, char* sys, bool kept, hipStream_t st) {
   DrSystems y{};
   y.seqs = sequences_of(a);
   y.q = la_view(a.la.q, a.la, a.la.Dk);
@@ -179,6 +179,7 @@ int systems(const Problem& a, char* sys, hipStream_t st) {
   y.H = a.la.H;
   y.Dk = a.la.Dk;
   y.dtype = a.la.dtype;
+  y.third = kept && a.la.Dk <= 64;
   y.scale = a.la.scale;
   return dr_systems(y, on_bf16(a), st);
 }
@@ -224,7 +225,7 @@ int forward(const Problem& a, const prnn_la_view& out, float* state_out, const i
   const Scratch s = carve(ws, a, p, kept == nullptr, false, false);
   const Kept k = kept_of(kept, a);
   char* sys = kept ? k.sys : s.sys;
-  if (int rc = systems(a, sys, st)) return rc;
+  if (int rc = systems(a, sys, kept != nullptr, st)) return rc;
   DrWalk w = walk_of(a, p, s, sys);
   w.z = la_view(a.la.v, a.la, a.la.Dv);
   w.out = const_cast<void*>(out.p);

@@ -58,8 +58,8 @@ __global__ __launch_bounds__(256) void dr_systems_kernel(DrSystems A) {
     g = la_decay(A.g, batch, u.begin + lane, h);
     rate = dr_rate(A.b, batch, u.begin + lane, h);
   }
-  char* sys = A.sys + (static_cast<size_t>(id) * A.H + h) * kDrSys;
-  float* weights = reinterpret_cast<float*>(sys + 2 * kDrTiles);
+  char* sys = A.sys + (static_cast<size_t>(id) * A.H + h) * dr_sys_bytes(kNarrow);
+  float* weights = reinterpret_cast<float*>(sys + 2 * dr_matrix(kNarrow));
   // ---- products: registers earlier tokens j, lanes later ones i
   if (tid == 0) s_stop = kDrC;
   f16v N, P;
@@ -118,7 +118,7 @@ __global__ __launch_bounds__(256) void dr_systems_kernel(DrSystems A) {
 
   // ---- weights; the system's matrix without what is not finite
   if (wave < 3) {
-    char* pairs = sys + kDrTiles + wave * (kDrTiles / 3 / M::kParts);
+    char* pairs = sys + dr_matrix(kNarrow) + wave * (kDrTiles / 3 / M::kParts);
     const float Hi = s_hi[ti], Lo = s_lo[ti];
     float pair[16];
     auto four = [](const float* v) { return *reinterpret_cast<const f4*>(v); };
@@ -143,28 +143,34 @@ __global__ __launch_bounds__(256) void dr_systems_kernel(DrSystems A) {
       const bool odd = dr_unit_of(l32, 0) & 1;
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        u2 hi[2], lo[2];
+        uint32_t part[3][2][2];
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const float* p = pair + 8 * m + 4 * k;
-          hi[k] = u2{pack_bf16x2(p[0], p[1]), pack_bf16x2(p[2], p[3])};
-          lo[k] = u2{pack_bf16x2(p[0] - lo_bf16(hi[k][0]), p[1] - hi_bf16(hi[k][0])),
-                     pack_bf16x2(p[2] - lo_bf16(hi[k][1]), p[3] - hi_bf16(hi[k][1]))};
-        }
+        for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          uint32_t a = hi[0][w], b = hi[1][w], c = lo[0][w], d = lo[1][w];
-          swap_halves(a, b);
-          swap_halves(c, d);
-          hi[0][w] = a;
-          hi[1][w] = b;
-          lo[0][w] = c;
-          lo[1][w] = d;
-        }
+          for (int w = 0; w < 2; ++w) {
+            float x = pair[8 * m + 4 * k + 2 * w], y = pair[8 * m + 4 * k + 2 * w + 1];
+#pragma unroll
+            for (int p = 0; p < 3; ++p) {
+              const uint32_t v = part[p][k][w] = pack_bf16x2(x, y);
+              x -= lo_bf16(v);
+              y -= hi_bf16(v);
+            }
+          }
         const int at = l32 * 64 + (dr_unit_of(l32, 4 * m + 2 * half) & ~1) * 8;
-        const u2 h0 = odd ? hi[1] : hi[0], h1 = odd ? hi[0] : hi[1], l0 = odd ? lo[1] : lo[0], l1 = odd ? lo[0] : lo[1];
-        *reinterpret_cast<u4*>(pairs + at) = u4{h0[0], h0[1], h1[0], h1[1]};
-        *reinterpret_cast<u4*>(pairs + kDrTiles / 2 + at) = u4{l0[0], l0[1], l1[0], l1[1]};
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+          if (p == 2 && !A.third) break;
+          u2 a, b;
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            uint32_t c = part[p][0][w], d = part[p][1][w];
+            swap_halves(c, d);
+            a[w] = c;
+            b[w] = d;
+          }
+          const u2 first = odd ? b : a, second = odd ? a : b;
+          *reinterpret_cast<u4*>(pairs + p * (kDrTiles / 2) + at) = u4{first[0], first[1], second[0], second[1]};
+        }
       }
     } else {
 #pragma unroll
@@ -244,15 +250,21 @@ __global__ __launch_bounds__(256) void dr_systems_kernel(DrSystems A) {
         t[0] = t[1];
         t[1] = x;
       }
-      u4 hi, lo;
+      u4 part[3];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const float a = t[k >> 1][2 * (k & 1)], b = t[k >> 1][2 * (k & 1) + 1];
-        hi[k] = pack_bf16x2(a, b);
-        lo[k] = pack_bf16x2(a - lo_bf16(hi[k]), b - hi_bf16(hi[k]));
+        float a = t[k >> 1][2 * (k & 1)], b = t[k >> 1][2 * (k & 1) + 1];
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+          const uint32_t v = pack_bf16x2(a, b);
+          part[p][k] = v;
+          a -= lo_bf16(v);
+          b -= hi_bf16(v);
+        }
       }
-      *reinterpret_cast<u4*>(tiles + l32 * 64 + (to & ~1) * 8) = hi;
-      *reinterpret_cast<u4*>(tiles + kDrTiles / 2 + l32 * 64 + (to & ~1) * 8) = lo;
+#pragma unroll
+      for (int p = 0; p < 3; ++p)
+        *reinterpret_cast<u4*>(tiles + p * (kDrTiles / 2) + l32 * 64 + (to & ~1) * 8) = part[p];
     } else {
       *reinterpret_cast<f4*>(tiles + l32 * 128 + to * 16) = t[0];
       *reinterpret_cast<f4*>(tiles + l32 * 128 + dr_unit_of(l32, 4 * half + 2 * m + 1) * 16) = t[1];

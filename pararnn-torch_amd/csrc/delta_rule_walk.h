@@ -50,7 +50,7 @@ struct Stored {
   using E = typename M::E;
   static constexpr int G = 64 / NC;
   static constexpr int ES = static_cast<int>(sizeof(E)), kRow = 32 * ES, kUnit = 4 * ES;
-  static constexpr int kTile = kDrTiles / 3 / M::kParts;
+  static constexpr int kTile = kDrTiles / 3 / (ES == 2 ? 2 : 1);
   // whether there is anything in the 32 x 32 tile
   static constexpr bool any(int rt, int f) {
     const int a = NC * rt / 32, b = 8 * G * f / 32;
@@ -59,10 +59,11 @@ struct Stored {
   static __device__ __forceinline__ const char* at(const char* tile, int row, int col) {
     return tile + row * kRow + dr_unit_of(row, col >> 2) * kUnit + (col & 3) * ES;
   }
-  static __device__ __forceinline__ Op<M, M::kParts> get(const char* m, int rt, int f, int n, int g) {
+  template <int P>
+  static __device__ __forceinline__ Op<M, P> get(const char* m, int rt, int f, int n, int g) {
     const char* t = m + (NC * rt / 32 + 8 * G * f / 32) * kTile;
     const int own = (NC * rt) & 31, other = (8 * G * f) & 31;
-    Op<M, M::kParts> o;
+    Op<M, P> o;
     if constexpr (ES == 2) {
       const char *x, *y;
       if constexpr (BACK) {
@@ -76,7 +77,7 @@ struct Stored {
         y = at(t, own + n, other + 4 * G + 4 * g);
       }
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
+      for (int p = 0; p < P; ++p) {
         union {
           u2 h[2];
           s4 s[2];
@@ -118,11 +119,17 @@ __device__ __forceinline__ void dr_place(int tiles, int H, int& tile, int& h, in
   h = item - piece * H;
 }
 
+// Pieces' own states run two workgroups a CU (D = 128: 82 us for 512 of them, 111 at one, a few registers
+// over that limit).
+template <class M, int NC, int KD, int W, int KIND>
+constexpr int dr_pair_waves =
+    (KIND == kDrState || KIND == kDrAdjoint) && sizeof(typename M::E) == 2 && NC == 16 && KD <= 128 && W == 4 ? 2 : 1;
+
 // W waves of NC columns each.  L: waves besides that do nothing but bring the next chunk to LDS, into
 // one of two buffers, while the others work on this one (bringing it took 4500 of a chunk's 9700 cycles
 // of a wave that does both); 0: the same waves do it, and the chunk's LDS is there once.
 template <class M, int NC, int KD, int W, int L, int KIND>
-__global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
+__global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) void dr_walk_kernel(DrWalk A) {
   using E = typename M::E;
   constexpr bool kNarrow = sizeof(E) == 2;
   constexpr bool kBack = KIND == kDrBackward || KIND == kDrAdjoint;
@@ -143,9 +150,10 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
   // fp32 widths over 64 have no registers for the next chunk's K and Q, over 128 no LDS for the system
   constexpr bool kAhead = kNarrow || KD <= 64, kSysLds = kNarrow || KD <= 128;
   static_assert(kAhead || kDrC * KD % (16 * NT) == 0, "whole rounds of fill");
-  constexpr int kSysBytes = kP ? 2 * kDrTiles : kDrTiles;
-  constexpr int kSysUnits = kSysBytes / 16 / NT;
-  static_assert(kSysBytes % (16 * NT) == 0, "whole units");
+  // parts of the pairs that take part, and what is read of the system: all but the pairs' parts behind them
+  constexpr int kPParts = !kNarrow ? 1 : kBack && KD <= 64 ? 3 : 2;
+  constexpr int kPairsAt = dr_matrix(kNarrow), kSysBytes = kPairsAt + (kP ? kDrTiles / (kNarrow ? 2 : 1) * kPParts : 0);
+  constexpr int kSysUnits = (kSysBytes / 16 + NT - 1) / NT;
   static_assert(L == 0 || (kAhead && kSysLds), "waves that only load hold a chunk");
   // a chunk in LDS: K, Q, z, the system and the pairs, the weights
   constexpr int oQ = kDrC * RK, oZ = oQ + (kQ ? kDrC * RK : 0), oS = oZ + kDrC * RZ,
@@ -180,10 +188,11 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
   };
   auto fetch = [&](int c) {
     const int t = pc.begin + c * kDrC, n = min(pc.end - t, kDrC);
-    const char* sys = A.sys + (static_cast<size_t>(row0 + c) * A.H + h) * kDrSys;
+    const char* sys = A.sys + (static_cast<size_t>(row0 + c) * A.H + h) * dr_sys_bytes(kNarrow);
 #pragma unroll
-    for (int k = 0; k < (kSysLds ? kSysUnits : 0); ++k) rs[k] = *reinterpret_cast<const u4*>(sys + (tid + k * NT) * 16);
-    const char* w = sys + 2 * kDrTiles;
+    for (int k = 0; k < (kSysLds ? kSysUnits : 0); ++k)
+      if (tid + k * NT < kSysBytes / 16) rs[k] = *reinterpret_cast<const u4*>(sys + (tid + k * NT) * 16);
+    const char* w = sys + 2 * dr_matrix(kNarrow);
 #pragma unroll
     for (int k = 0; k < (kDrW * 16 + NT - 1) / NT; ++k)
       if (tid + k * NT < kDrW * 16) rw[k] = *reinterpret_cast<const u4*>(w + (tid + k * NT) * 16);
@@ -203,7 +212,8 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
     }
     rz.template put<RZ>(to + oZ, A.dtype, tid);
 #pragma unroll
-    for (int k = 0; k < (kSysLds ? kSysUnits : 0); ++k) *reinterpret_cast<u4*>(to + oS + (tid + k * NT) * 16) = rs[k];
+    for (int k = 0; k < (kSysLds ? kSysUnits : 0); ++k)
+      if (tid + k * NT < kSysBytes / 16) *reinterpret_cast<u4*>(to + oS + (tid + k * NT) * 16) = rs[k];
 #pragma unroll
     for (int k = 0; k < (kDrW * 16 + NT - 1) / NT; ++k)
       if (tid + k * NT < kDrW * 16) *reinterpret_cast<u4*>(to + oW + (tid + k * NT) * 16) = rw[k];
@@ -452,7 +462,7 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
             store_elem<M>(rs, operand_lane + rest.second, rest.first, S[t][r]);
         }
     }
-    const char* const sS = kSysLds ? at + oS : A.sys + (static_cast<size_t>(row0 + c) * A.H + h) * kDrSys;
+    const char* const sS = kSysLds ? at + oS : A.sys + (static_cast<size_t>(row0 + c) * A.H + h) * dr_sys_bytes(kNarrow);
     if constexpr (L == 0) {
       __syncthreads();
       if (step + 1 < chunks) fetch(chunk_of(step + 1));
@@ -557,12 +567,12 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
         for (int r = 0; r < RT; ++r) Y[t][r] = 0.0f;
 #pragma unroll
       for (int f = 0; f < TF; ++f) {
-        Op<M, M::kParts> m[TT];
+        Op<M, kPParts> m[TT];
 #pragma unroll
         for (int t = 0; t < TT; ++t)
-          if (Mat::any(t, f)) m[t] = Mat::get(sS + kDrTiles, t, f, nn, g);
+          if (Mat::any(t, f)) m[t] = Mat::template get<kPParts>(sS + kPairsAt, t, f, nn, g);
 #pragma unroll
-        for (int k = 0; k < kPairs<M::kParts, 1>; ++k)
+        for (int k = 0; k < kPairs<kPParts, 1>; ++k)
 #pragma unroll
           for (int t = 0; t < TT; ++t)
             if (Mat::any(t, f)) mul_one<NC>(Y[t], m[t], zo[f], k);
@@ -615,12 +625,12 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
       for (int r = 0; r < RT; ++r) Y[t][r] = y[RT * t + r];
 #pragma unroll
     for (int f = 0; f < TF; ++f) {
-      Op<M, M::kParts> m[TT];
+      Op<M, 3> m[TT];
 #pragma unroll
       for (int t = 0; t < TT; ++t)
-        if (Mat::any(t, f)) m[t] = Mat::get(sS, t, f, nn, g);
+        if (Mat::any(t, f)) m[t] = Mat::template get<3>(sS, t, f, nn, g);
 #pragma unroll
-      for (int k = 0; k < kPairs<M::kParts, 3>; ++k)
+      for (int k = 0; k < kPairs<3, 3>; ++k)
 #pragma unroll
         for (int t = 0; t < TT; ++t)
           if (Mat::any(t, f)) mul_one<NC>(Y[t], m[t], yo[f], k);
@@ -657,12 +667,12 @@ __global__ __launch_bounds__(64 * (W + L), 1) void dr_walk_kernel(DrWalk A) {
       }
 #pragma unroll
       for (int f = 0; f < TF; ++f) {
-        Op<M, M::kParts> m[TT];
+        Op<M, 2> m[TT];
 #pragma unroll
         for (int t = 0; t < TT; ++t)
-          if (Mat::any(t, f)) m[t] = Mat::get(sS + kDrTiles, t, f, nn, g);
+          if (Mat::any(t, f)) m[t] = Mat::template get<2>(sS + kPairsAt, t, f, nn, g);
 #pragma unroll
-        for (int k = 0; k < kPairs<2, M::kParts>; ++k)
+        for (int k = 0; k < kPairs<2, 2>; ++k)
 #pragma unroll
           for (int t = 0; t < TT; ++t)
             if (Mat::any(t, f)) mul_one<NC>(O[t], uo[f], m[t], k);

@@ -88,11 +88,11 @@ __device__ __forceinline__ void mul(Acc<NC>& c, const Op<InF32, P>& a, const Op<
 // The same product by product, so that several sums can take turns (a matrix instruction waits for the
 // last one of its own sum): products kPairs<P, R> of operands of P and R parts, number k of them.
 template <int P, int R>
-constexpr int kPairs = P == 1 || R == 1 ? P * R : R == 2 ? 3 : 5;  // (of two parts and two or three the largest)
+constexpr int kPairs = P == 1 || R == 1 ? P * R : P == 3 ? 6 : 3;  // (of two or three parts each the largest)
 template <int NC, int P, int R>
 __device__ __forceinline__ void mul_one(Acc<NC>& c, const Op<InBf16, P>& a, const Op<InBf16, R>& b, int k) {
-  static_assert(P == 1 || R == 1 || (P == 2 && (R == 2 || R == 3)), "products are listed for these");
-  const int i = P == 1 ? 0 : R == 1 ? k : k == 2 || k == 4;
+  static_assert(P == 1 || R == 1 || (P == R && P < 4), "products are listed for these");
+  const int i = P == 1 ? 0 : R == 1 ? k : k == 5 ? 2 : k == 2 || k == 4;
   const int j = P == 1 ? k : R == 1 ? 0 : k == 3 ? 2 : k == 1 || k == 4;
   c = mfma_bf16<NC>(a.p[i], b.p[j], c);
 }
