@@ -28,8 +28,8 @@
 // chunks at once (delta_rule_grad.hip).
 //
 // Two arithmetics: bf16 storage of widths in eights on bf16 matrix instructions, operands that are
-// not given in bf16 in two or three bf16 parts; everything else (fp32, fp16, odd widths) on fp32
-// ones.
+// not given in bf16 in two or three bf16 parts (delta_rule_walk.h); everything else (fp32, fp16, odd
+// widths) on fp32 ones.
 #pragma once
 
 #include "linear_attention.h"
@@ -185,7 +185,7 @@ int dr_grad(const DrGrad& a, bool bf16, hipStream_t stream);
 
 // Waves of a walk's workgroup, `cols` columns each.  items: (piece, head) pairs.  Narrow values have two
 // column tiles' waves at most; and where there is a CU for each half of a workgroup, halves (D = 64, 128
-// sequences' heads: 99 us forwards, 112 whole; 350 pieces: 155 us, 117 whole).
+// sequences' heads: 99 us forwards, 112 whole; 350 pieces: 155 us, 117 whole; both in two parts).
 inline int dr_walk_group(int Dk, int Dv, int cols, bool bf16, long long items) {
   if (!bf16) return Dk <= 128 ? 4 : 2;
   if (Dk > 128) return 4;

@@ -13,9 +13,9 @@
 //    the token writes: the same sums by rows, and the token's own.
 //
 // Eight waves: four for the pairs and dq, four for dk, each with its own code and the same barriers, so
-// that two workgroups a CU (what LDS holds) are four waves a SIMD.  4096 chunks of bf16, D = 64: 98 us for
-// 300 MB (3.1 TB/s; four waves that did all took 121); the phases' latencies bound it, no unit is busy
-// for half of the time.
+// that two workgroups a CU (what LDS holds) are four waves a SIMD (four waves that did all took 1.24
+// times as long).  4096 chunks of bf16, D = 64: 128 us for 435 MB, of which 260 reach memory (3.4 TB/s of
+// all); the phases' latencies bound it, no unit is busy for half of the time.
 #include "delta_rule_loads.h"
 
 namespace prnn {

@@ -4,7 +4,7 @@
 // Bound by the state's traffic (read once, written once).  A workgroup takes 4 L columns of a head's
 // state and keeps them: L lanes of four columns side by side, the rows spread over 256 / L groups of
 // lanes, U rows a thread in registers.  One pass forms S^T k and S^T q; their sums over the groups
-// give u and o, then the rows go back.  256 sessions of 16 heads, D = 128: 537 MB in 88 us on a pool that
+// give u and o, then the rows go back.  256 sessions of 16 heads, D = 128: 537 MB in 87 us on a pool that
 // the last call has touched (half of it is still in the last-level cache), 117 otherwise (4.6 TB/s); one
 // session of 8 heads 4.8 us, a launch's own time.
 #include "linear_attention.h"

@@ -10,9 +10,10 @@
 // before they vanish.)
 //
 // Bound by what it moves and by its chain of phases, of which four workgroups a CU hide a part: 4096
-// systems of bf16 keys of 64 in 46 us, 37 MB in and 107 MB out (3.1 TB/s; of a workgroup's 16000 cycles
-// 7000 are a wait for rows).  Workgroups that go on to further chunks were slower: they hold the next
-// rows in registers.
+// systems of bf16 keys of 64 in 55 us, 37 MB in and 154 MB out (3.5 TB/s; of a workgroup's 17000 cycles
+// 7000 are a wait for rows).  The third part of the inverse and of the pairs is 9 us of it: with 16 bits
+// of them fp32 states were up to 1.8e-6 off where keys overlap and decays are slow, 5e-7 with 24.
+// Workgroups that go on to further chunks were slower: they hold the next rows in registers.
 #include "delta_rule_loads.h"
 
 namespace prnn {

@@ -11,10 +11,15 @@
 // barriers only hand K, Q and the system through LDS.  The output is formed transposed from the same
 // registers (state and u as first operands), so that a lane holds consecutive columns of a token.
 //
-// Bound by this chain: one wave a SIMD goes through 7900 cycles a chunk forwards and 7000 backwards (bf16,
-// D = 64; matrix instructions 1600 of them, the rest splits of results into bf16 parts, LDS reads and
-// waits), so 2048 tokens of 128 heads take 97 and 86 us and 16384 tokens of 8 heads, D = 128, in 16
-// pieces, 67 us.
+// Bound by this chain: one wave a SIMD goes through some 8000 cycles a chunk (bf16, D = 64; matrix
+// instructions 2200 of them, the rest splits of results into bf16 parts, LDS reads and waits), so 2048
+// tokens of 128 heads take 125 us forwards with what is kept and 110 backwards, and 16384 tokens of 8
+// heads, D = 128, in 16 pieces, 73 us.
+//
+// bf16 operands: K, Q and z as they are given; the state, the system and its right side in three parts
+// (24 bits) where they form the chain, in two where an output is rounded to 8 bits afterwards; what the
+// gradients read (e, dv, states, adjoints) in two: their own sums are rounded to 8 bits too, and with one
+// part they came out at 1.5 to 3 times that rounding.
 #pragma once
 
 #include "delta_rule_loads.h"
@@ -119,7 +124,7 @@ __device__ __forceinline__ void dr_place(int tiles, int H, int& tile, int& h, in
   h = item - piece * H;
 }
 
-// Pieces' own states run two workgroups a CU (D = 128: 82 us for 512 of them, 111 at one, a few registers
+// Pieces' own states run two workgroups a CU (D = 128: 87 us for 512 of them, 111 at one, a few registers
 // over that limit).
 template <class M, int NC, int KD, int W, int KIND>
 constexpr int dr_pair_waves =
@@ -480,8 +485,7 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
       float s[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) s[e] = S[(8 * f + e) / RT][(8 * f + e) % RT];
-      // three parts in the chain (16 bits of a state would be 1e-6 of it after some hundred tokens), two
-      // where an output is rounded
+      // three parts in the chain, two where an output is rounded
       const auto sp = parts_of<M, 3>(s);
       Op<M, 2> so;
       if constexpr (kNarrow) {
@@ -813,7 +817,7 @@ int dr_launch_walk(const DrWalk& a, hipStream_t stream) {
 template <int KIND, int KD>
 int dr_launch_cols(const DrWalk& a, int cols, hipStream_t stream) {
   // Waves that only load: not for pieces' own states, of which two workgroups a CU run without (D = 128,
-  // 512 of them: 74 us, 87 with), nor where two chunks do not fit LDS.
+  // 512 of them: 74 us, 87 with, in two parts throughout), nor where two chunks do not fit LDS.
   constexpr int kLoad = KD <= 128 && KIND != kDrState && KIND != kDrAdjoint ? 4 : 0;
   if (cols == 16 && a.group == 4) return dr_launch_walk<InBf16, 16, KD, 4, kLoad, KIND>(a, stream);
   if constexpr (KD <= 128) {

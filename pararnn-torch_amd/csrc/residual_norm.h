@@ -11,8 +11,8 @@
 //
 // A row lies in the registers of NT threads, E elements each: every array is read once and written
 // once, the statistics are two-pass and the backward pass forms them again from x, y and the gate.
-// Bound by memory where rows are many: 16384 rows of 1024 in bf16 with gate and both norms take 42 us
-// forwards (168 MB, 4.0 TB/s) and 62 backwards (268 MB, 4.3 TB/s); a launch's latency where they are few
+// Bound by memory where rows are many: 16384 rows of 1024 in bf16 with gate and both norms take 41 us
+// forwards (168 MB, 4.1 TB/s) and 61 backwards (268 MB, 4.4 TB/s); a launch's latency where they are few
 // (32 rows 6.4 us).
 #pragma once
 

@@ -13,10 +13,9 @@ pool of states, in place.  Layouts, packed sequences, shared heads, states and p
 
 The rule is stable where ``beta_t |k_t|^2`` lies in 0 .. 2: keys of unit length and rates in (0, 1),
 or up to 2 where a state may also be reflected.  float32, bfloat16 and float16; arithmetic and
-states are float32 (bfloat16 of widths in eights on bfloat16 matrix products: operands of 16 bits or
-more where they reach an output or a state; the backward pass keeps the states before its chunks
-and what the tokens wrote in bfloat16 too), results are rounded once.  No atomics: equal calls give
-equal bits.
+states are float32 (bfloat16 of widths in eights on bfloat16 matrix products: operands of 24 bits
+where they reach a state, of 16 where they only reach a result of bfloat16, and in what the backward
+pass keeps), results are rounded once.  No atomics: equal calls give equal bits.
 """
 
 from __future__ import annotations
@@ -153,8 +152,8 @@ def delta_rule(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, beta: Tensor,
     ``cu_seqlens``, ``block_table``, ``state_out``, ``state_table`` and ``return_state`` are
     :func:`linear_attention`'s.  Gradients of the output and of the returned states flow to ``q``,
     ``k``, ``v``, ``log_decay``, ``beta`` and ``h0``; between the passes a call keeps what its tokens
-    wrote (as large as the output, or twice that), the states before its chunks of 64 tokens (likewise
-    for widths of 64) and 26 KB of a chunk's system per head.
+    wrote and the states before its chunks of 64 tokens, 4 bytes an element, and 38 KB (bfloat16 of
+    widths in eights) or 26 KB of a chunk's system per head.
     """
     what = "delta_rule"
     _no_tangents(what, q, k, v, log_decay, beta, h0)
