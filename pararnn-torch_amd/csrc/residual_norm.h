@@ -39,20 +39,23 @@ struct RnArgs {
 int rn_forward(const RnArgs& a, int dtype, bool vec, hipStream_t stream);
 int rn_backward(const RnArgs& a, int dtype, bool vec, int groups, hipStream_t stream);
 
-// Threads of a row: 8 elements each up to 512 threads, then 16 (1024 threads have 128 registers each,
-// where what lies in them spills: only for what does not fit otherwise).
+// Threads of a row: 8 elements each, of rows over 8192 16.
 inline int rn_threads(int C) {
   int nt = 64;
-  while (nt < 512 && nt * 8 < C) nt *= 2;
-  return C <= 8192 ? nt : 1024;
+  while (nt < 1024 && nt * 8 < C) nt *= 2;
+  return nt;
 }
+// The backward pass holds more of a row, and 1024 threads have 128 registers each: rows of 4097 .. 8192
+// elements of 16 bits take 512 threads of 16 (4096 x 8192 with all options: 232 us, 309 with 1024 of 8;
+// fp32 564 and 418).  Over 8192 registers spill (1 TB/s of such rows).
+inline int rn_back_threads(int C, bool narrow) { return narrow && C > 4096 && C <= 8192 ? 512 : rn_threads(C); }
 // Workgroups of the backward pass: as many as run at a time, 12 waves a CU of 16-byte accesses, 8 of
 // single elements (16384 x 1024 in bf16: 61 us, with 8 waves 69; a workgroup's sums over its rows are
 // written and read once more).
-inline int rn_groups(int N, int C, bool vec) {
-  const int rows = rn_threads(C) >= 256 ? 1 : 256 / rn_threads(C);
+inline int rn_groups(int N, int C, bool vec, bool narrow) {
+  const int nt = rn_back_threads(C, narrow), rows = nt >= 256 ? 1 : 256 / nt;
   const long long groups = (static_cast<long long>(N) + rows - 1) / rows;
-  const int most = (vec ? 768 : 512) * 256 / std::max(256, rn_threads(C));
+  const int most = (vec ? 768 : 512) * 256 / std::max(256, nt);
   return static_cast<int>(std::min<long long>(groups, most));
 }
 

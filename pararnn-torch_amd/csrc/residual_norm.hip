@@ -107,12 +107,13 @@ int launch_row(const RnArgs& a, hipStream_t stream) {
     case 64: return launch<T, V, 8, 64>(a, stream);
     case 128: return launch<T, V, 8, 128>(a, stream);
     case 256: return launch<T, V, 8, 256>(a, stream);
-    case 512: return a.C <= 4096 ? launch<T, V, 8, 512>(a, stream) : launch<T, V, 16, 512>(a, stream);
+    case 512: return launch<T, V, 8, 512>(a, stream);
   }
-  return launch<T, V, 16, 1024>(a, stream);
+  return a.C <= 8192 ? launch<T, V, 8, 1024>(a, stream) : launch<T, V, 16, 1024>(a, stream);
 }
 
-size_t parts_bytes(int N, int C) { return sizeof(float) * 4 * static_cast<size_t>(rn_groups(N, C, true)) * C; }
+// (for any type: 16 bits and whole units have the most workgroups)
+size_t parts_bytes(int N, int C) { return sizeof(float) * 4 * static_cast<size_t>(rn_groups(N, C, true, true)) * C; }
 
 int check(int N, int C, float eps, int act, int w_dtype, int dtype) {
   if (int rc = check_dtype(dtype)) return rc;
@@ -213,7 +214,7 @@ extern "C" PRNN_API int prnn_residual_norm_backward(
   a.eps = eps;
   a.want = (dw ? 1 : 0) | (db ? 2 : 0) | (dpw ? 4 : 0) | (dscale ? 8 : 0);
   const bool vec = vectors(C, dtype, {gh, gz, x, y, gate, dx, dy, dgate});
-  const int groups = rn_groups(N, C, vec);
+  const int groups = rn_groups(N, C, vec, dtype != PRNN_F32);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   if (int rc = rn_backward(a, dtype, vec, groups, st)) return rc;
   if (!sums) return PRNN_OK;

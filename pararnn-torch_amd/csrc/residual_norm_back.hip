@@ -26,7 +26,7 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT, E == 8 && V > 1 && NT <= 256 ?
 #pragma unroll
     for (int i = 0; i < E; ++i) sums[k][i] = 0.0f;
   const int step = static_cast<int>(gridDim.x) * R;
-  constexpr bool kAhead = E == 8;  // registers for the row behind this one
+  constexpr bool kAhead = E == 8 && NT < 1024;  // registers for the row behind this one
   auto place = [&](long long base) { return min(base + static_cast<int>(threadIdx.x) / NT, A.N - 1ll); };
   typename Row::Raw rx, ry, rg, rz, rh;  // the next row's are under way
   auto fetch = [&](long long base) {
@@ -144,12 +144,17 @@ int launch(const RnArgs& a, int groups, hipStream_t stream) {
 }
 template <typename T, int V>
 int launch_row(const RnArgs& a, int groups, hipStream_t stream) {
-  switch (rn_threads(a.C)) {
+  switch (rn_back_threads(a.C, sizeof(T) == 2)) {
     case 64: return launch<T, V, 8, 64>(a, groups, stream);
     case 128: return launch<T, V, 8, 128>(a, groups, stream);
     case 256: return launch<T, V, 8, 256>(a, groups, stream);
-    case 512: return a.C <= 4096 ? launch<T, V, 8, 512>(a, groups, stream) : launch<T, V, 16, 512>(a, groups, stream);
+    case 512:
+      if constexpr (sizeof(T) == 2)
+        if (a.C > 4096) return launch<T, V, 16, 512>(a, groups, stream);
+      return launch<T, V, 8, 512>(a, groups, stream);
   }
+  if constexpr (sizeof(T) == 4)
+    if (a.C <= 8192) return launch<T, V, 8, 1024>(a, groups, stream);
   return launch<T, V, 16, 1024>(a, groups, stream);
 }
 
