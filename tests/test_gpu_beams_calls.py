@@ -45,6 +45,26 @@ def test_zeros_of_either_sign_and_scores_that_swallow_logits():
     _check(logits, torch.tensor([[-INF, -1e30, -1e30]]), 100)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("V", [8177, 8192, 16384, 16381])
+def test_slices_end_where_the_vocabulary_does(V, dtype):
+    """Rows off a 16-byte boundary and slices with nothing or little of them; what lies next to a row (an
+    infinity here) is not read as its own."""
+    r = torch.Generator().manual_seed(V)
+    wide = torch.full((2, 3, V + 3), INF).to(dtype)
+    for shift in (0, 1, 2, 3):
+        logits = wide.clone()[..., shift:shift + V]
+        logits.copy_((torch.randn(2, 3, V, generator=r) * 2).to(dtype))
+        want = O.beam_select(logits, torch.zeros(2, 3), 5)
+        there = wide.to(DEV)[..., shift:shift + V]
+        there.copy_(logits)
+        from pararnn_amd import beam_select
+
+        _, p, t = beam_select(there, _t(2, 3), beams=5)
+        for b in range(2):
+            assert list(zip(p[b].tolist(), t[b].tolist())) == [(k, i) for _, k, i in want[b]]
+
+
 def test_captured_search():
     """Selection and pages in one graph, replayed on other logits: as eager calls."""
     from pararnn_amd import beam_select, reorder_pages

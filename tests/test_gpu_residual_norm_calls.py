@@ -110,6 +110,24 @@ def test_rows_keep_to_themselves(bad, dtype):
                 assert not torch.isfinite(got[1][3]).any(), name
 
 
+@pytest.mark.parametrize("width", [40, 1000, 4104, 8192, 9000])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_some_gradients_only(dtype, width):
+    """A leaf alone has the gradient that it has among all."""
+    from pararnn_amd import residual_norm
+
+    case = ((9, width), "layer", True, True, "silu", True, "vector", True, True, False)
+    given, fixed, seeds = _on(case, dtype)
+    want = dict(zip(given, _run(given, fixed, seeds)[2:]))
+    for name in given:
+        leaves = dict(given)
+        leaves[name] = leaves[name].detach().requires_grad_(True)
+        h, z = residual_norm(**leaves, **fixed)
+        out = [t for t in (h, z) if t.requires_grad]
+        got, = torch.autograd.grad(out, [leaves[name]], seeds[-len(out):])
+        assert torch.equal(got, want[name]), name
+
+
 def test_rows_of_zeros_and_large_values():
     """A row of zeros under eps = 1e-6 and zero variance; values whose squares pass float32's range are
     the caller's, those of 1e15 are not."""
