@@ -176,7 +176,7 @@ enum DrKind { kDrForward, kDrKept, kDrState, kDrBackward, kDrAdjoint };
 
 int dr_systems(const DrSystems& a, bool bf16, hipStream_t stream);
 int dr_walk_bf16(const DrWalk& a, DrKind kind, int cols, hipStream_t stream);
-int dr_walk_bf16_kept(const DrWalk& a, int cols, hipStream_t stream);
+int dr_walk_bf16_out(const DrWalk& a, bool kept, int cols, hipStream_t stream);
 int dr_walk_bf16_back(const DrWalk& a, DrKind kind, int cols, hipStream_t stream);
 int dr_walk_f32(const DrWalk& a, DrKind kind, hipStream_t stream);
 // The pieces' own states and transfers to the states that the pieces begin with.

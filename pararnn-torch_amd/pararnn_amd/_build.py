@@ -58,6 +58,10 @@ def _flags() -> list[str]:
 #    trackers: the fused Newton launch 1.87 -> 1.80 ms at config 3, the
 #    packed-stream line ~1.5% faster.
 _FILE_FLAGS = {
+    # the delta rule's walks: 131 -> 126 us (packed prompts), 126 -> 123 (training), fp32 59 -> 57; pieces'
+    # own states are slower with either (86 -> 96)
+    "delta_rule_walk_bf16_out.hip": ["-mllvm", "-amdgpu-sched-strategy=max-ilp"],
+    "delta_rule_walk_f32.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
     "gru_wide.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
     "gru_wide_rev.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
     "slstm_diag.hip": ["-mllvm", "-amdgpu-use-amdgpu-trackers=1"],
