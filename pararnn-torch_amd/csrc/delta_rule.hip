@@ -52,8 +52,10 @@ LaSeqs sequences_of(const Problem& a) {
 struct Kept {
   void *e, *before;
   char* sys;
+  int* order;  // of a packed batch's pieces
   size_t bytes;
 };
+int pieces_of(const Problem& a);  // (of a plan; 0: not packed)
 Kept kept_of(void* p, const Problem& a) {
   Carver c(p);
   const size_t size = 4, heads = a.la.H;  // bytes of an element, in two bf16 parts or fp32
@@ -62,12 +64,14 @@ Kept kept_of(void* p, const Problem& a) {
   k.e = c.take(units * heads * dr_operand_elems(kDrC, a.la.Dv) * size);
   k.before = c.take(units * heads * dr_operand_elems(a.la.Dk, a.la.Dv) * size);
   k.sys = static_cast<char*>(c.take(units * heads * dr_sys_bytes(on_bf16(a))));
+  k.order = static_cast<int*>(c.take(4 * static_cast<size_t>(pieces_of(a))));
   k.bytes = c.used;
   return k;
 }
 
 struct Scratch {
   char* sys;
+  int* order;
   void *behind, *dv, *dv_lo;
   float* piece;
   uint16_t* transfer;
@@ -128,12 +132,20 @@ Plan plan(const Problem& a) {
   return p;
 }
 
+int pieces_of(const Problem& a) {
+  const Plan p = plan(a);
+  return a.la.cu_seqlens ? static_cast<int>(std::min<long long>(dr_units(p.seqs, p.seqs.len), 1 << 30)) : 0;
+}
+
 Scratch carve(void* ws, const Problem& a, const Plan& plan, bool systems, bool backward, bool decay_grad) {
   Carver c(ws);
   Scratch s{};
   const size_t heads = a.la.H, tokens = tokens_of(a), size = on_bf16(a) ? 2 : 4;
   const size_t units = dr_units(plan.seqs, kDrC);
-  if (systems) s.sys = static_cast<char*>(c.take(units * heads * dr_sys_bytes(on_bf16(a))));
+  if (systems) {
+    s.sys = static_cast<char*>(c.take(units * heads * dr_sys_bytes(on_bf16(a))));
+    s.order = static_cast<int*>(c.take(4 * static_cast<size_t>(pieces_of(a))));
+  }
   if (plan.cut) {
     const size_t pieces = dr_units(plan.seqs, plan.seqs.len) * heads;
     s.piece = static_cast<float*>(c.take(4 * pieces * a.la.Dk * a.la.Dv));
@@ -168,7 +180,7 @@ LaDecay decay_of(const Problem& a) {
 }
 LaDecay rate_of(const Problem& a) { return LaDecay{a.b, a.b_sb, a.b_st, a.b_sh, a.b_dtype}; }
 
-int systems(const Problem& a, char* sys, bool kept, hipStream_t st) {
+int systems(const Problem& a, const Plan& plan, char* sys, int* order, bool kept, hipStream_t st) {
   DrSystems y{};
   y.seqs = sequences_of(a);
   y.q = la_view(a.la.q, a.la, a.la.Dk);
@@ -180,16 +192,21 @@ int systems(const Problem& a, char* sys, bool kept, hipStream_t st) {
   y.Dk = a.la.Dk;
   y.dtype = a.la.dtype;
   y.third = kept && a.la.Dk <= 64;
+  y.pieces = plan.seqs;
+  y.n_pieces = pieces_of(a);
+  y.order = y.n_pieces ? order : nullptr;
   y.scale = a.la.scale;
   return dr_systems(y, on_bf16(a), st);
 }
 
-DrWalk walk_of(const Problem& a, const Plan& plan, const Scratch& s, const char* sys) {
+DrWalk walk_of(const Problem& a, const Plan& plan, const Scratch& s, const char* sys, const int* order) {
   DrWalk w{};
   w.seqs = plan.seqs;
   w.q = la_view(a.la.q, a.la, a.la.Dk);
   w.k = la_view(a.la.k, a.la, a.la.Dk);
   w.sys = sys;
+  w.n_pieces = pieces_of(a);
+  w.order = w.n_pieces ? order : nullptr;
   w.piece = s.piece;
   w.transfer = s.transfer;
   w.H = a.la.H;
@@ -225,8 +242,9 @@ int forward(const Problem& a, const prnn_la_view& out, float* state_out, const i
   const Scratch s = carve(ws, a, p, kept == nullptr, false, false);
   const Kept k = kept_of(kept, a);
   char* sys = kept ? k.sys : s.sys;
-  if (int rc = systems(a, sys, kept != nullptr, st)) return rc;
-  DrWalk w = walk_of(a, p, s, sys);
+  int* order = kept ? k.order : s.order;
+  if (int rc = systems(a, p, sys, order, kept != nullptr, st)) return rc;
+  DrWalk w = walk_of(a, p, s, sys, order);
   w.z = la_view(a.la.v, a.la, a.la.Dv);
   w.out = const_cast<void*>(out.p);
   w.o_sb = out.sb;
@@ -247,7 +265,7 @@ int backward(const Problem& a, const prnn_la_view& go, const float* gs, const vo
   const Plan p = plan(a);
   const Scratch s = carve(ws, a, p, false, true, dg != nullptr);
   const Kept k = kept_of(const_cast<void*>(kept), a);
-  DrWalk w = walk_of(a, p, s, k.sys);
+  DrWalk w = walk_of(a, p, s, k.sys, k.order);
   w.z = la_view(go, a.la, a.la.Dv);
   w.keep = s.behind;
   w.dv = s.dv ? s.dv : dv;

@@ -25,6 +25,44 @@ __device__ __forceinline__ bool not_finite(float v) {
   return (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u;
 }
 
+constexpr int kLengths = 1024;  // that are told apart, in chunks
+// Places of the pieces by their lengths, longest first, by counting.  Pieces of one length come in any
+// order: it decides when they run, not what they give.
+__device__ __forceinline__ void pieces_in_order(const DrSystems& A, int* count) {
+  const int tid = threadIdx.x;
+  auto place = [&](int i) {
+    const DrUnit u = dr_unit(A.pieces, A.pieces.len, i);
+    const int chunks = u.any ? (u.end - u.begin + kDrC - 1) / kDrC + 1 : 0;
+    return kLengths - 1 - min(chunks, kLengths - 1);
+  };
+  for (int i = tid; i < kLengths; i += 256) count[i] = 0;
+  __syncthreads();
+  for (int i = tid; i < A.n_pieces; i += 256) atomicAdd(&count[place(i)], 1);
+  __syncthreads();
+  int own[kLengths / 256], sum = 0;
+#pragma unroll
+  for (int k = 0; k < kLengths / 256; ++k) {
+    own[k] = sum;
+    sum += count[tid * (kLengths / 256) + k];
+  }
+  // sums of the threads before: over the wave, then over the waves
+  int before = sum;
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) {
+    const int o = __shfl_up(before, m);
+    if ((tid & 63) >= m) before += o;
+  }
+  int* const waves = count + kLengths;
+  if ((tid & 63) == 63) waves[tid >> 6] = before;
+  __syncthreads();
+  before -= sum;
+  for (int w = 0; w < tid >> 6; ++w) before += waves[w];
+#pragma unroll
+  for (int k = 0; k < kLengths / 256; ++k) count[tid * (kLengths / 256) + k] = before + own[k];
+  __syncthreads();
+  for (int i = tid; i < A.n_pieces; i += 256) A.order[atomicAdd(&count[place(i)], 1)] = i;
+}
+
 template <class M>
 __global__ __launch_bounds__(256) void dr_systems_kernel(DrSystems A) {
   using E = typename M::E;
@@ -42,7 +80,12 @@ __global__ __launch_bounds__(256) void dr_systems_kernel(DrSystems A) {
   const int it = wave > 0, jt = wave > 1;  // (the fourth wave's are not used)
   const int ti = 32 * it + l32, tj = 32 * jt + l32;
 
-  const int h = blockIdx.x % A.H, id = blockIdx.x / A.H;
+  static_assert((kLengths + 4) * 4 <= static_cast<int>(sizeof(lds)), "counts fit");
+  if (A.order && blockIdx.x == 0) {  // a workgroup more, before the others
+    pieces_in_order(A, reinterpret_cast<int*>(lds));
+    return;
+  }
+  const int item = blockIdx.x - (A.order ? 1 : 0), h = item % A.H, id = item / A.H;
   const DrUnit u = dr_unit(A.seqs, kDrC, id);
   if (!u.any || u.begin >= u.end) return;
   const int n = u.end - u.begin, batch = dr_batch(A.seqs, u);
@@ -276,7 +319,7 @@ __global__ __launch_bounds__(256) void dr_systems_kernel(DrSystems A) {
 
 template <class M>
 int launch(const DrSystems& a, hipStream_t stream) {
-  const long long groups = dr_units(a.seqs, kDrC) * a.H;
+  const long long groups = dr_units(a.seqs, kDrC) * a.H + (a.order ? 1 : 0);
   if (int rc = check_grid("delta_rule", groups, 256)) return rc;
   dr_systems_kernel<M><<<static_cast<unsigned>(groups), 256, 0, stream>>>(a);
   PRNN_HIP(hipGetLastError());

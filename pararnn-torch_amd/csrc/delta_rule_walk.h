@@ -167,6 +167,7 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
 
   int tile, h, piece;
   dr_place(A.tiles, A.H, tile, h, piece);
+  if (A.order && piece < A.n_pieces) piece = A.order[piece];
   const DrUnit pc = dr_unit(A.seqs, A.seqs.len, piece);
   if (!pc.any || pc.seq >= A.seqs.n_seq) return;
   // the last piece of the walk's direction hands its state to none
