@@ -133,8 +133,9 @@ Plan plan(const Problem& a) {
 }
 
 int pieces_of(const Problem& a) {
+  if (a.la.cu_seqlens == nullptr) return 0;
   const Plan p = plan(a);
-  return a.la.cu_seqlens ? static_cast<int>(std::min<long long>(dr_units(p.seqs, p.seqs.len), 1 << 30)) : 0;
+  return static_cast<int>(std::min<long long>(dr_units(p.seqs, p.seqs.len), 1 << 30));
 }
 
 Scratch carve(void* ws, const Problem& a, const Plan& plan, bool systems, bool backward, bool decay_grad) {

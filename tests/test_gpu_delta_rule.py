@@ -8,10 +8,9 @@ random walk: sqrt(2000) 2^-24 = 2.7e-6 at these sizes; gradients pass two such c
 decays', a double sum over a chunk, among them).  States of bfloat16 inputs: operands of 16 bits (two
 parts: 2^-17 of a value at most, 0.4 of that in the mean square) in three products of a chain (key
 times state, the system, the state), 2^-17 0.4 sqrt(3) = 5.3e-6; three parts in the last one: 1e-5
-bounds both chains.  Outputs of 16 bits: one rounding, at most 2^-8 of a value and 0.4 of that in the
-mean square; gradients of 16 bits besides take what the tokens wrote, the states and the adjoints in
-bfloat16, four independent roundings: 0.4 sqrt(5) 2^-8 = 3.5e-3, and the decays' and rates', sums of
-such products over a few dozen terms of either sign, twice that."""
+bounds both chains.  Results of 16 bits: one rounding, at most 2^-8 = 3.9e-3 of a value, of sums whose
+operands have 16 bits at least (the decays' and rates' gradients are small differences of such sums
+where keys are few: twice that)."""
 
 import pytest
 import torch
