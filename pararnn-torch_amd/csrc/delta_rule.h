@@ -97,13 +97,11 @@ __device__ __forceinline__ int dr_batch(const LaSeqs& q, const DrUnit& u) { retu
 //
 // Per chunk and head: the strictly lower part of the inverse, then the pairs, each as the tiles
 // (0, 0), (1, 0), (1, 1) of 32 x 32, rows of 32 elements whose units of four are exchanged by the row
-// (dr_unit_of): fp32, or three bf16 parts of 6 KB; then kDrW rows of 64 floats.  The third part of the
-// pairs is there only for a backward pass over keys of up to 64 (wider ones' LDS has no room for it).
-constexpr int kDrTiles = 3 * 32 * 32 * 4;  // bytes of a matrix in fp32, of two parts of it
-constexpr int dr_matrix(bool narrow) { return narrow ? kDrTiles / 2 * 3 : kDrTiles; }
+// (dr_unit_of), fp32; then kDrW rows of 64 floats.
+constexpr int kDrTiles = 3 * 32 * 32 * 4;  // bytes of a matrix
 enum { kWg, kWr, kWb, kWhi, kWlo, kWmeta, kDrW };  // exp(G), exp(G_last - G), b, G in two parts
-constexpr int dr_sys_bytes(bool narrow) { return 2 * dr_matrix(narrow) + kDrW * 64 * 4; }
-static_assert(dr_sys_bytes(true) % 256 == 0 && dr_sys_bytes(false) % 256 == 0, "blocks stay aligned");
+constexpr int kDrSys = 2 * kDrTiles + kDrW * 64 * 4;
+static_assert(kDrSys % 256 == 0, "blocks stay aligned");
 // kWmeta: [0] exp(G_last), [1] the first token that is not finite (64: none), as an integer
 
 // (so that 16 or 32 rows of a step fall into all banks, two words each)
@@ -123,9 +121,8 @@ struct DrSystems {
   LaDecay g, b;
   char* sys;
   int H, Dk, dtype;
-  int third;  // whether the pairs' third part is wanted
   // Of a packed batch also the order in which a walk takes its pieces, longest first (37 sequences of 130
-  // to 1500 tokens, 16 heads: 126 us in the order given, 82 so).
+  // to 1500 tokens, 16 heads: the walk 126 us in the order given, 82 so).
   LaSeqs pieces;
   int* order;  // NULL: none
   int n_pieces;

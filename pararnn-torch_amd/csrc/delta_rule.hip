@@ -63,7 +63,7 @@ Kept kept_of(void* p, const Problem& a) {
   const size_t units = dr_units(sequences_of(a), kDrC);
   k.e = c.take(units * heads * dr_operand_elems(kDrC, a.la.Dv) * size);
   k.before = c.take(units * heads * dr_operand_elems(a.la.Dk, a.la.Dv) * size);
-  k.sys = static_cast<char*>(c.take(units * heads * dr_sys_bytes(on_bf16(a))));
+  k.sys = static_cast<char*>(c.take(units * heads * kDrSys));
   k.order = static_cast<int*>(c.take(4 * static_cast<size_t>(pieces_of(a))));
   k.bytes = c.used;
   return k;
@@ -144,7 +144,7 @@ Scratch carve(void* ws, const Problem& a, const Plan& plan, bool systems, bool b
   const size_t heads = a.la.H, tokens = tokens_of(a), size = on_bf16(a) ? 2 : 4;
   const size_t units = dr_units(plan.seqs, kDrC);
   if (systems) {
-    s.sys = static_cast<char*>(c.take(units * heads * dr_sys_bytes(on_bf16(a))));
+    s.sys = static_cast<char*>(c.take(units * heads * kDrSys));
     s.order = static_cast<int*>(c.take(4 * static_cast<size_t>(pieces_of(a))));
   }
   if (plan.cut) {
@@ -181,7 +181,7 @@ LaDecay decay_of(const Problem& a) {
 }
 LaDecay rate_of(const Problem& a) { return LaDecay{a.b, a.b_sb, a.b_st, a.b_sh, a.b_dtype}; }
 
-int systems(const Problem& a, const Plan& plan, char* sys, int* order, bool kept, hipStream_t st) {
+int systems(const Problem& a, const Plan& plan, char* sys, int* order, hipStream_t st) {
   DrSystems y{};
   y.seqs = sequences_of(a);
   y.q = la_view(a.la.q, a.la, a.la.Dk);
@@ -192,7 +192,6 @@ int systems(const Problem& a, const Plan& plan, char* sys, int* order, bool kept
   y.H = a.la.H;
   y.Dk = a.la.Dk;
   y.dtype = a.la.dtype;
-  y.third = kept && a.la.Dk <= 64;
   y.pieces = plan.seqs;
   y.n_pieces = pieces_of(a);
   y.order = y.n_pieces ? order : nullptr;
@@ -244,7 +243,7 @@ int forward(const Problem& a, const prnn_la_view& out, float* state_out, const i
   const Kept k = kept_of(kept, a);
   char* sys = kept ? k.sys : s.sys;
   int* order = kept ? k.order : s.order;
-  if (int rc = systems(a, p, sys, order, kept != nullptr, st)) return rc;
+  if (int rc = systems(a, p, sys, order, st)) return rc;
   DrWalk w = walk_of(a, p, s, sys, order);
   w.z = la_view(a.la.v, a.la, a.la.Dv);
   w.out = const_cast<void*>(out.p);

@@ -77,7 +77,7 @@ __global__ __launch_bounds__(512, sizeof(typename M::E) == 2 && KS == 1 ? 4 : 2)
   if constexpr (kNarrow) gl.fetch(pl, static_cast<long long>(A.H) * A.Dv, n, 0, A.Dv, kCode);
   ka.fetch(pk, A.k.st, n, last_k, A.Dk, A.dtype);
   kb.fetch(pq, A.q.st, n, last_k, A.Dk, A.dtype);
-  const float* weights = reinterpret_cast<const float*>(A.sys + unit * dr_sys_bytes(kNarrow) + 2 * dr_matrix(kNarrow));
+  const float* weights = reinterpret_cast<const float*>(A.sys + unit * kDrSys + 2 * kDrTiles);
   const int kt = wave & 1, it = wave >> 1, t = 32 * it + l32;
   for (int i = tid; i < kDrW * 64; i += 512) sw[i] = weights[i];
   ga.template put<RB>(sG, A.dtype);

@@ -10,9 +10,8 @@
 // before they vanish.)
 //
 // Bound by what it moves and by its chain of phases, of which four workgroups a CU hide a part: 4096
-// systems of bf16 keys of 64 in 55 us, 37 MB in and 154 MB out (3.5 TB/s; of a workgroup's 17000 cycles
-// 7000 are a wait for rows).  The third part of the inverse and of the pairs is 9 us of it: with 16 bits
-// of them fp32 states were up to 1.8e-6 off where keys overlap and decays are slow, 5e-7 with 24.
+// systems of bf16 keys of 64 in 54 us, 37 MB in and 104 MB out (of a workgroup's 16000 cycles 7000 are a
+// wait for rows).  They are left in fp32, the walks' loading waves take them apart for bf16 products.
 // Workgroups that go on to further chunks were slower: they hold the next rows in registers.
 #include "delta_rule_loads.h"
 
@@ -102,8 +101,8 @@ __global__ __launch_bounds__(256) void dr_systems_kernel(DrSystems A) {
     g = la_decay(A.g, batch, u.begin + lane, h);
     rate = dr_rate(A.b, batch, u.begin + lane, h);
   }
-  char* sys = A.sys + (static_cast<size_t>(id) * A.H + h) * dr_sys_bytes(kNarrow);
-  float* weights = reinterpret_cast<float*>(sys + 2 * dr_matrix(kNarrow));
+  char* sys = A.sys + (static_cast<size_t>(id) * A.H + h) * kDrSys;
+  float* weights = reinterpret_cast<float*>(sys + 2 * kDrTiles);
   // ---- products: registers earlier tokens j, lanes later ones i
   if (tid == 0) s_stop = kDrC;
   f16v N, P;
@@ -162,9 +161,8 @@ __global__ __launch_bounds__(256) void dr_systems_kernel(DrSystems A) {
 
   // ---- weights; the system's matrix without what is not finite
   if (wave < 3) {
-    char* pairs = sys + dr_matrix(kNarrow) + wave * (kDrTiles / 3 / M::kParts);
+    char* pairs = sys + kDrTiles + wave * (kDrTiles / 3);
     const float Hi = s_hi[ti], Lo = s_lo[ti];
-    float pair[16];
     auto four = [](const float* v) { return *reinterpret_cast<const f4*>(v); };
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -178,49 +176,7 @@ __global__ __launch_bounds__(256) void dr_systems_kernel(DrSystems A) {
         p[r] = j + r <= ti ? P[4 * q + r] * w * A.scale : 0.0f;
       }
       *reinterpret_cast<f4*>(&sM[ti * kLd + j]) = m;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) pair[4 * q + r] = p[r];
-    }
-    if constexpr (sizeof(E) == 2) {
-      // this lane holds units 2 q + half of its row; halves of the wave exchange them, so that either has
-      // two units side by side (in one order or the other: the exchange by rows keeps such pairs)
-      const bool odd = dr_unit_of(l32, 0) & 1;
-#pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        uint32_t part[3][2][2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            float x = pair[8 * m + 4 * k + 2 * w], y = pair[8 * m + 4 * k + 2 * w + 1];
-#pragma unroll
-            for (int p = 0; p < 3; ++p) {
-              const uint32_t v = part[p][k][w] = pack_bf16x2(x, y);
-              x -= lo_bf16(v);
-              y -= hi_bf16(v);
-            }
-          }
-        const int at = l32 * 64 + (dr_unit_of(l32, 4 * m + 2 * half) & ~1) * 8;
-#pragma unroll
-        for (int p = 0; p < 3; ++p) {
-          if (p == 2 && !A.third) break;
-          u2 a, b;
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            uint32_t c = part[p][0][w], d = part[p][1][w];
-            swap_halves(c, d);
-            a[w] = c;
-            b[w] = d;
-          }
-          const u2 first = odd ? b : a, second = odd ? a : b;
-          *reinterpret_cast<u4*>(pairs + p * (kDrTiles / 2) + at) = u4{first[0], first[1], second[0], second[1]};
-        }
-      }
-    } else {
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        *reinterpret_cast<f4*>(pairs + l32 * 128 + dr_unit_of(l32, 2 * q + half) * 16) =
-            f4{pair[4 * q], pair[4 * q + 1], pair[4 * q + 2], pair[4 * q + 3]};
+      *reinterpret_cast<f4*>(pairs + l32 * 128 + dr_unit_of(l32, 2 * q + half) * 16) = p;
     }
   }
   __syncthreads();
@@ -275,45 +231,17 @@ __global__ __launch_bounds__(256) void dr_systems_kernel(DrSystems A) {
 
   // ---- the strictly triangular part of the inverse
   if (wave < 3) {
-  char* tiles = sys + wave * (kDrTiles / 3 / M::kParts);
-  const int row = 32 * it + l32, col0 = 32 * jt;
+    char* tiles = sys + wave * (kDrTiles / 3);
+    const int row = 32 * it + l32;
 #pragma unroll
-  for (int m = 0; m < 2; ++m) {
-    f4 t[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const int col = col0 + 4 * (4 * half + 2 * m + k);
+    for (int k = 0; k < 4; ++k) {
+      const int unit = 4 * half + k, col = 32 * jt + 4 * unit;
       const f4 w = *reinterpret_cast<const f4*>(&sT[row * kLd + col]);
+      f4 t;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) t[k][r] = col + r < row ? w[r] : 0.0f;
+      for (int r = 0; r < 4; ++r) t[r] = col + r < row ? w[r] : 0.0f;
+      *reinterpret_cast<f4*>(tiles + l32 * 128 + dr_unit_of(l32, unit) * 16) = t;
     }
-    const int to = dr_unit_of(l32, 4 * half + 2 * m);
-    if constexpr (sizeof(E) == 2) {
-      if (to & 1) {
-        const f4 x = t[0];
-        t[0] = t[1];
-        t[1] = x;
-      }
-      u4 part[3];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        float a = t[k >> 1][2 * (k & 1)], b = t[k >> 1][2 * (k & 1) + 1];
-#pragma unroll
-        for (int p = 0; p < 3; ++p) {
-          const uint32_t v = pack_bf16x2(a, b);
-          part[p][k] = v;
-          a -= lo_bf16(v);
-          b -= hi_bf16(v);
-        }
-      }
-#pragma unroll
-      for (int p = 0; p < 3; ++p)
-        *reinterpret_cast<u4*>(tiles + p * (kDrTiles / 2) + l32 * 64 + (to & ~1) * 8) = part[p];
-    } else {
-      *reinterpret_cast<f4*>(tiles + l32 * 128 + to * 16) = t[0];
-      *reinterpret_cast<f4*>(tiles + l32 * 128 + dr_unit_of(l32, 4 * half + 2 * m + 1) * 16) = t[1];
-    }
-  }
   }
 }
 

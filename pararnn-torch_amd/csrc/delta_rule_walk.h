@@ -13,8 +13,8 @@
 //
 // Bound by this chain: one wave a SIMD goes through some 8000 cycles a chunk (bf16, D = 64; matrix
 // instructions 2200 of them, the rest splits of results into bf16 parts, LDS reads and waits), so 2048
-// tokens of 128 heads take 125 us forwards with what is kept and 110 backwards, and 16384 tokens of 8
-// heads, D = 128, in 16 pieces, 73 us.
+// tokens of 128 heads take 128 us forwards with what is kept and 102 backwards, and 16384 tokens of 8
+// heads, D = 128, in 16 pieces, 67 us.
 //
 // bf16 operands: K, Q and z as they are given; the state, the system and its right side in three parts
 // (24 bits) where they form the chain, in two where an output is rounded to 8 bits afterwards; what the
@@ -155,10 +155,13 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
   // fp32 widths over 64 have no registers for the next chunk's K and Q, over 128 no LDS for the system
   constexpr bool kAhead = kNarrow || KD <= 64, kSysLds = kNarrow || KD <= 128;
   static_assert(kAhead || kDrC * KD % (16 * NT) == 0, "whole rounds of fill");
-  // parts of the pairs that take part, and what is read of the system: all but the pairs' parts behind them
-  constexpr int kPParts = !kNarrow ? 1 : kBack && KD <= 64 ? 3 : 2;
-  constexpr int kPairsAt = dr_matrix(kNarrow), kSysBytes = kPairsAt + (kP ? kDrTiles / (kNarrow ? 2 : 1) * kPParts : 0);
-  constexpr int kSysUnits = (kSysBytes / 16 + NT - 1) / NT;
+  // The system comes in fp32 and lies in LDS in bf16 parts: three of the inverse, two of the pairs, of which
+  // a backward pass takes a third where there is room for it.
+  constexpr int kTParts = kNarrow ? 3 : 1, kPParts = !kNarrow ? 1 : kBack && KD <= 64 ? 3 : 2;
+  constexpr int kPart = kDrTiles / (kNarrow ? 2 : 1);
+  constexpr int kPairsAt = kPart * kTParts, kSysBytes = kPairsAt + (kP ? kPart * kPParts : 0);
+  constexpr int kSysUnits = (kP ? 2 : 1) * kDrTiles / 16 / NT;
+  static_assert(kDrTiles % (16 * NT) == 0, "whole units");
   static_assert(L == 0 || (kAhead && kSysLds), "waves that only load hold a chunk");
   // a chunk in LDS: K, Q, z, the system and the pairs, the weights
   constexpr int oQ = kDrC * RK, oZ = oQ + (kQ ? kDrC * RK : 0), oS = oZ + kDrC * RZ,
@@ -194,11 +197,10 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
   };
   auto fetch = [&](int c) {
     const int t = pc.begin + c * kDrC, n = min(pc.end - t, kDrC);
-    const char* sys = A.sys + (static_cast<size_t>(row0 + c) * A.H + h) * dr_sys_bytes(kNarrow);
+    const char* sys = A.sys + (static_cast<size_t>(row0 + c) * A.H + h) * kDrSys;
 #pragma unroll
-    for (int k = 0; k < (kSysLds ? kSysUnits : 0); ++k)
-      if (tid + k * NT < kSysBytes / 16) rs[k] = *reinterpret_cast<const u4*>(sys + (tid + k * NT) * 16);
-    const char* w = sys + 2 * dr_matrix(kNarrow);
+    for (int k = 0; k < (kSysLds ? kSysUnits : 0); ++k) rs[k] = *reinterpret_cast<const u4*>(sys + (tid + k * NT) * 16);
+    const char* w = sys + 2 * kDrTiles;
 #pragma unroll
     for (int k = 0; k < (kDrW * 16 + NT - 1) / NT; ++k)
       if (tid + k * NT < kDrW * 16) rw[k] = *reinterpret_cast<const u4*>(w + (tid + k * NT) * 16);
@@ -218,8 +220,25 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
     }
     rz.template put<RZ>(to + oZ, A.dtype, tid);
 #pragma unroll
-    for (int k = 0; k < (kSysLds ? kSysUnits : 0); ++k)
-      if (tid + k * NT < kSysBytes / 16) *reinterpret_cast<u4*>(to + oS + (tid + k * NT) * 16) = rs[k];
+    for (int k = 0; k < (kSysLds ? kSysUnits : 0); ++k) {
+      if constexpr (kNarrow) {
+        constexpr int kUnits = kDrTiles / 16 / NT;  // of a matrix
+        const bool pairs = k >= kUnits;
+        char* const at = to + oS + (pairs ? kPairsAt : 0) + (tid + (pairs ? k - kUnits : k) * NT) * 8;
+        float x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(rs[k][e]);
+#pragma unroll
+        for (int p = 0; p < (pairs ? kPParts : kTParts); ++p) {
+          const u2 v{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
+          *reinterpret_cast<u2*>(at + p * kPart) = v;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] -= e & 1 ? hi_bf16(v[e >> 1]) : lo_bf16(v[e >> 1]);
+        }
+      } else {
+        *reinterpret_cast<u4*>(to + oS + (tid + k * NT) * 16) = rs[k];
+      }
+    }
 #pragma unroll
     for (int k = 0; k < (kDrW * 16 + NT - 1) / NT; ++k)
       if (tid + k * NT < kDrW * 16) *reinterpret_cast<u4*>(to + oW + (tid + k * NT) * 16) = rw[k];
@@ -468,7 +487,7 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
             store_elem<M>(rs, operand_lane + rest.second, rest.first, S[t][r]);
         }
     }
-    const char* const sS = kSysLds ? at + oS : A.sys + (static_cast<size_t>(row0 + c) * A.H + h) * dr_sys_bytes(kNarrow);
+    const char* const sS = kSysLds ? at + oS : A.sys + (static_cast<size_t>(row0 + c) * A.H + h) * kDrSys;
     if constexpr (L == 0) {
       __syncthreads();
       if (step + 1 < chunks) fetch(chunk_of(step + 1));

@@ -152,8 +152,8 @@ def delta_rule(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, beta: Tensor,
     ``cu_seqlens``, ``block_table``, ``state_out``, ``state_table`` and ``return_state`` are
     :func:`linear_attention`'s.  Gradients of the output and of the returned states flow to ``q``,
     ``k``, ``v``, ``log_decay``, ``beta`` and ``h0``; between the passes a call keeps what its tokens
-    wrote and the states before its chunks of 64 tokens, 4 bytes an element, and 38 KB (bfloat16 of
-    widths in eights) or 26 KB of a chunk's system per head.
+    wrote and the states before its chunks of 64 tokens, 4 bytes an element, and 26 KB of a chunk's
+    system per head.
     """
     what = "delta_rule"
     _no_tangents(what, q, k, v, log_decay, beta, h0)
