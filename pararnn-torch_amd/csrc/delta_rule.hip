@@ -35,13 +35,6 @@ int check_strides(const Problem& a, const prnn_la_view& other) {
   return PRNN_OK;
 }
 
-// Gradients of q and k are formed densely per head: a chunk of them is addressed in 31 bits.
-int check_gradients(const Problem& a) {
-  if (a.la.T > 1 && 1ll * a.la.H * a.la.Dk > 1ll << 23)
-    return fail(PRNN_ERR_VALUE, "gradients of H=%d heads of %d key channels are more than 2^23 a token", a.la.H, a.la.Dk);
-  return PRNN_OK;
-}
-
 int sequences(const Problem& a) { return a.la.cu_seqlens ? a.la.n_seq : a.la.B; }
 size_t tokens_of(const Problem& a) { return static_cast<size_t>(a.la.B) * a.la.T; }
 
@@ -358,8 +351,6 @@ extern "C" PRNN_API int prnn_delta_rule(const prnn_delta_rule_problem* a, const 
   if (sequences(*a) == 0) return PRNN_OK;
   if (kept && (reinterpret_cast<uintptr_t>(kept) & 255))
     return fail(PRNN_ERR_VALUE, "what is kept must lie on a 256-byte boundary");
-  if (kept)
-    if (int rc = check_gradients(*a)) return rc;
   if (int rc = check_ws("workspace", need(*a, kept == nullptr, false, false), workspace, bytes)) return rc;
   return forward(*a, *out, state_out, out_table, out_rows, kept, workspace, static_cast<hipStream_t>(stream));
 }
@@ -383,7 +374,6 @@ extern "C" PRNN_API int prnn_delta_rule_backward(const prnn_delta_rule_problem* 
   if (on_bf16(*a) && ((reinterpret_cast<uintptr_t>(dq) | reinterpret_cast<uintptr_t>(dk) |
                        reinterpret_cast<uintptr_t>(dv)) & 15))
     return fail(PRNN_ERR_VALUE, "dq, dk and dv must start on 16-byte boundaries");
-  if (int rc = check_gradients(*a)) return rc;
   if (a->la.h0_table) return fail(PRNN_ERR_VALUE, "a block table has no gradient");
   if (a->la.h0 && a->la.h0_rows < sequences(*a))
     return fail(PRNN_ERR_VALUE, "h0 has %d rows for %d sequences", a->la.h0_rows, sequences(*a));
