@@ -42,7 +42,8 @@ __global__ __launch_bounds__(256) void dr_join_kernel(JoinArgs A) {
   };
   f16v S[R];
   const float* init = la_row(A.init, seq, A.H * state_floats);
-  const rsrc_t ri = make_rsrc(init ? init + h * state_floats : A.piece, init ? static_cast<uint32_t>(state_floats) * 4 : 0);
+  const rsrc_t ri =
+      make_rsrc(init ? init + h * state_floats : A.piece, init ? static_cast<uint32_t>(state_floats) * 4 : 0);
 #pragma unroll
   for (int r = 0; r < R; ++r)
 #pragma unroll

@@ -176,7 +176,7 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
   // the last piece of the walk's direction hands its state to none
   if (kOwn && pc.index == (kBack ? 0 : pc.count - 1)) return;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int tid = L ? static_cast<int>(threadIdx.x) - 64 * W : static_cast<int>(threadIdx.x);  // of those that bring rows
+  const int tid = static_cast<int>(threadIdx.x) - (L ? 64 * W : 0);  // of those that bring rows
   const int nn = lane % NC, g = lane / NC;
   const bool transfer = kOwn && tile >= A.own_tiles;
   const int col0 = (transfer ? tile - A.own_tiles : tile) * VT;
@@ -416,8 +416,9 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
         // operands (zeros behind the sequence)
         const int step = A.H * A.Dv * ES;
         const size_t elems = dr_operand_elems(kDrC, A.Dv);
-        const rsrc_t r = kBack ? make_rsrc(static_cast<E*>(p) + ((tok0 + t0) * A.H + h) * A.Dv, (n - 1) * step + A.Dv * ES)
-                               : make_rsrc(static_cast<E*>(p) + (static_cast<size_t>(row0 + held_c) * A.H + h) * M::kParts * elems,
+        const size_t row = ((tok0 + t0) * A.H + h) * A.Dv, unit = static_cast<size_t>(row0 + held_c) * A.H + h;
+        const rsrc_t r = kBack ? make_rsrc(static_cast<E*>(p) + row, (n - 1) * step + A.Dv * ES)
+                               : make_rsrc(static_cast<E*>(p) + unit * M::kParts * elems,
                                            static_cast<uint32_t>(elems) * M::kParts * ES);
         const uint32_t lane_at = kBack ? la_in(col < A.Dv, 4 * g * step + col * ES) : operand_lane;
         if constexpr (kNarrow) {
@@ -426,10 +427,11 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
             for (int j = 0; j < kHeld / 4; ++j) {
               const uint32_t to = operand16(j);
               __builtin_amdgcn_raw_buffer_store_b128(paired(held_u + 4 * j), r, to, 0, 0);
-              __builtin_amdgcn_raw_buffer_store_b128(paired(held_l + 4 * j), r, to + static_cast<uint32_t>(elems) * 2, 0, 0);
+              __builtin_amdgcn_raw_buffer_store_b128(paired(held_l + 4 * j), r,
+                                                     to + static_cast<uint32_t>(elems) * 2, 0, 0);
             }
           }
-          const rsrc_t rl = kBack ? make_rsrc(static_cast<E*>(A.dv_lo) + ((tok0 + t0) * A.H + h) * A.Dv, (n - 1) * step + A.Dv * ES) : r;
+          const rsrc_t rl = kBack ? make_rsrc(static_cast<E*>(A.dv_lo) + row, (n - 1) * step + A.Dv * ES) : r;
 #pragma unroll
           for (int t = 0; t < (kBack ? TT : 0); ++t)
 #pragma unroll
@@ -554,7 +556,8 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
 #pragma unroll
           for (int j = 0; j < NC / 16; ++j)
             __builtin_amdgcn_raw_buffer_store_b128(
-                paired(w + 4 * j), rs, operand16(NC * t / 32 * (NC / 16) + j) + p * static_cast<uint32_t>(elems) * 2, 0, 0);
+                paired(w + 4 * j), rs,
+                operand16(NC * t / 32 * (NC / 16) + j) + p * static_cast<uint32_t>(elems) * 2, 0, 0);
         }
       }
     }
