@@ -639,8 +639,10 @@ PRNN_API int prnn_residual_norm_backward(const void* gh, const void* gz, const v
 
 /* ---- Beam search's selection ---------------------------------------------------
  * The M <= 128 largest of scores[b, k] + log_softmax(logits[b, k])[t] of every search b, the largest
- * first, ties to the lowest k, then the larger logit, then the lowest t: their totals, k and t; -infinity, -1 and -1 where there are fewer
- * (a total of -infinity is never chosen, nor one of a beam whose logits hold an infinity or NaN).
+ * first, ties to the lowest k, then the larger logit, then the lowest t: their totals, k and t;
+ * -infinity, -1 and -1 where there are fewer.  Totals are formed and compared in fp64 (an exponential to
+ * 2^-51 of its row's largest), the same wherever a row lies.  A total of -infinity is never chosen, nor
+ * one of a beam whose logits hold NaN or +infinity.
  * ended (B, K bytes; NULL: none): a beam that goes on with token `pad` alone, at its own score.
  * logits (B, K, V) by strides of searches and beams. */
 PRNN_API size_t prnn_beam_select_workspace_size(int B, int K, int V, int M);

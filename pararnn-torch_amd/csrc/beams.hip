@@ -4,20 +4,25 @@
 //   ties to the lowest beam, in a beam to the larger logit (a score far from zero makes totals of
 //   different logits equal), then to the lowest token.
 //
-// Two launches.  The first reads the logits once: a workgroup per beam and slice of 8192 tokens, 32
+// Two launches.  The first reads the logits once: a workgroup per beam and slice of 8176 tokens, 32
 // values a thread in registers, gives the slice's largest value, its sum of exponentials and its M
 // best.  The second, a workgroup per search, joins the slices' sums in fp64 and chooses among the
-// slices' best: candidates of two beams may lie next to each other, and which one goes on must not
-// hang on a sum's rounding.
+// slices' best.
+//
+// Candidates of two beams may lie next to each other, and equal beams tie: which one goes on must not
+// hang on where a row lies in memory.  So slices are of fixed tokens, the exponentials are formed in fp64
+// and added as whole multiples of 2^-50 of the slice's largest: the sum is the same in any order (which
+// thread holds a token goes by the row's address), and off by 2^-51 a token at most.
 //
 // The M best of some thousand values: the M-th largest of the threads' own largest is a bound that at
 // least M values reach, and only values of those M threads can; what reaches it (a few more than M of
 // ordinary logits) is ranked by counting, so the order of arrival does not matter.  Up to 32 best the
 // bound is the largest of the four waves' own, found by a quarter of the comparisons.
 //
-// 32 searches of 8 beams over 50257 bf16 logits: 15 us (26 MB; the exponentials' and comparisons'
-// instructions and the phases' latency bound it) and 11 us (latency: a wave per beam's sum, then three
-// rounds through LDS); one search of 4 beams over 32000: 7.4 and 8.8 us, latency.
+// 32 searches of 8 beams over 50257 bf16 logits: 26 us (26 MB; the exponentials' instructions, some twenty
+// of fp64 each, bound it: 15 us with exponentials and sums of fp32, which told equal beams apart) and 11
+// us (latency: a wave per beam's sum, then three rounds through LDS); one search of 4 beams over 32000:
+// 8.2 and 8.8 us, latency.
 #include <algorithm>
 
 #include "prnn_host.h"
@@ -28,6 +33,9 @@ namespace {
 constexpr int kMost = 128;     // candidates that are wanted
 constexpr int kEach = 32;      // tokens of a thread
 constexpr int kSlice = 256 * kEach;
+// Tokens of a slice: its values' places but those that a row's start inside a 16-byte unit may take.
+// Whole units, so that all slices of a row start at the same place in one.
+constexpr int kTokens = kSlice - 16;
 constexpr int kFew = 32;       // up to which a bound is a wave's
 constexpr int kRound = 2;     // candidates of a thread and round of the second launch
 
@@ -47,6 +55,27 @@ __device__ __forceinline__ uint64_t order(double v) {
 }
 __device__ __forceinline__ double value(uint64_t o) {
   return __builtin_bit_cast(double, o >> 63 ? o & ~(1ull << 63) : ~o);
+}
+
+// exp(x) for x <= 0 as a whole number of 2^-50: 2^n 2^f with |f| <= 1/2, 2^f = sum (f ln 2)^i / i! to i = 12.
+// Off by half of one, and by 2^-51 relative (what the sum leaves out, and the reduction).
+constexpr int kUnit = 50;
+struct Taylor {
+  double c[13] = {1.0};
+  constexpr Taylor() {
+    for (int i = 1; i < 13; ++i) c[i] = c[i - 1] * 0.69314718055994530942 / i;
+  }
+};
+__device__ __forceinline__ uint64_t exp_units(double x) {
+  // below -48 it is nothing of a unit, and a -infinity would leave NaN
+  const double t = fmax(x, -48.0) * 1.4426950408889634074, n = rint(t), f = t - n;
+  constexpr Taylor y;
+  double p = y.c[12];
+#pragma unroll
+  for (int i = 11; i >= 0; --i) p = fma(p, f, y.c[i]);
+  // p 2^n in units, rounded at the last place of a number in 2^52 .. 2^53
+  const double scale = __builtin_bit_cast(double, static_cast<uint64_t>(1023 + kUnit + static_cast<int>(n)) << 52);
+  return __builtin_bit_cast(uint64_t, fma(p, scale, 0x1p52)) & ((1ull << 52) - 1);
 }
 
 struct Slice {
@@ -73,8 +102,9 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs A) {
   constexpr int V = 16 / sizeof(T);
   __shared__ __align__(16) uint64_t s_top[256];
   __shared__ uint64_t s_list[(MOST <= kFew ? 4 : 1) * MOST * kEach];
-  __shared__ double s_sum[4];
+  __shared__ uint64_t s_sum[4];
   __shared__ float s_most[4];
+  __shared__ bool s_bad[4];
   __shared__ uint64_t s_bound[4];
   __shared__ int s_count;
   const int tid = threadIdx.x, slice = blockIdx.x % A.S, row = blockIdx.x / A.S;
@@ -85,11 +115,9 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs A) {
   // together (in branches they came one after another): units behind the row lie behind the buffer, and
   // what else is in its first and last one is taken out afterwards.
   const int skip = static_cast<int>((reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T));
-  const int first_token = slice * kSlice - skip;
-  const long long bytes = (static_cast<long long>(A.V) - first_token) * static_cast<long long>(sizeof(T));
-  const rsrc_t row_part = make_rsrc(
-      p + first_token,
-      static_cast<uint32_t>(min(max(bytes, 0ll), static_cast<long long>(kSlice * sizeof(T))) + 15) & ~15u);
+  const int first_token = slice * kTokens, there = min(A.V - first_token, kTokens);
+  const rsrc_t row_part =
+      make_rsrc(p + first_token - skip, ((there + skip) * static_cast<uint32_t>(sizeof(T)) + 15) & ~15u);
   u4 raw[kEach / V];
 #pragma unroll
   for (int u = 0; u < kEach / V; ++u)
@@ -104,13 +132,15 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs A) {
       else
         v[u * V + i] = i & 1 ? Narrow<T>::hi(raw[u][i / 2]) : Narrow<T>::lo(raw[u][i / 2]);
     }
-  auto token = [&](int i) { return first_token + ((i / V) * 256 + tid) * V + i % V; };
-  if (first_token < 0 || first_token + kSlice > A.V) {
+  auto place_of = [&](int i) { return ((i / V) * 256 + tid) * V + i % V - skip; };  // in the slice
+  auto token = [&](int i) { return first_token + place_of(i); };
+  // (of a whole slice the first wave's first unit and the last wave's last ones)
+  if (there < kTokens || (tid < 64 && skip) || tid >= 192) {
 #pragma unroll
     for (int i = 0; i < kEach; ++i)
-      if (token(i) < 0 || token(i) >= A.V) v[i] = -INFINITY;
+      if (place_of(i) < 0 || place_of(i) >= there) v[i] = -INFINITY;
   }
-  // this thread's largest, the lowest token of equals; NaN is found by the sum of exponentials
+  // this thread's largest, the lowest token of equals
   float most = v[0];
 #pragma unroll
   for (int i = 1; i < kEach; ++i) most = fmaxf(most, v[i]);
@@ -128,16 +158,23 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs A) {
   __syncthreads();
   most = fmaxf(fmaxf(s_most[0], s_most[1]), fmaxf(s_most[2], s_most[3]));
   const bool none = !(most > -INFINITY);
-  float part = 0.0f;
+  uint64_t sum = 0;
+  bool bad = false;  // NaN or an infinity: no finite probabilities
   {
-    const float from = none ? 0.0f : most;
+    const double from = none ? 0.0 : most;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) part += fexp(v[i] - from);  // NaN of an infinity too
+    for (int i = 0; i < kEach; ++i) {
+      sum += exp_units(v[i] - from);
+      bad |= !(v[i] < INFINITY);
+    }
   }
-  double sum = part;
 #pragma unroll
   for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m);
-  if ((tid & 63) == 0) s_sum[tid >> 6] = sum;
+  bad = __any(bad);
+  if ((tid & 63) == 0) {
+    s_sum[tid >> 6] = sum;
+    s_bad[tid >> 6] = bad;
+  }
   // this thread's place among the threads' largest
   int above = 0;
   if (top) {
@@ -177,8 +214,9 @@ __global__ __launch_bounds__(256) void beam_slice_kernel(BeamArgs A) {
       A.best[at * A.M + rank] = make_uint2(static_cast<uint32_t>(o >> 32), ~static_cast<uint32_t>(o));
   }
   if (tid == 0) {
-    const double all = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
-    A.slices[at] = Slice{all, all - all == 0.0 ? most : NAN, min(n, A.M)};
+    const uint64_t all = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+    const bool any_bad = s_bad[0] | s_bad[1] | s_bad[2] | s_bad[3];
+    A.slices[at] = Slice{static_cast<double>(all) * 0x1p-50, any_bad ? NAN : most, min(n, A.M)};
   }
 }
 
@@ -328,8 +366,7 @@ __global__ __launch_bounds__(256) void beam_choose_kernel(BeamArgs A) {
   }
 }
 
-// One slice more than the tokens need: a row may start inside a 16-byte unit.
-int slices_of(int V) { return (V + 15 + kSlice - 1) / kSlice; }
+int slices_of(int V) { return (V - 1) / kTokens + 1; }
 
 struct Scratch {
   Slice* slices;

@@ -30,10 +30,11 @@ def beam_select(logits: Tensor, scores: Tensor, *, beams: int | None = None,
     ``logits`` ``(B, K, V)`` float32, bfloat16 or float16, ``scores`` ``(B, K)`` float32, the beams'
     totals so far (``-inf``: a beam that is not there, as all but the first at a search's start).
     Returns ``(scores, parents, tokens)``, each ``(B, beams)`` (``K`` of them by default, at most 128),
-    the largest total first, float32, int32 and int32.  Totals are formed and compared in float64;
-    ties go to the lowest beam, in a beam to the larger logit, then to the lowest token.  Where fewer candidates are left, the rest are
-    ``-inf``, -1 and -1.  A logit of ``-inf`` is masked; a beam whose logits hold NaN or ``+inf``
-    proposes nothing.
+    the largest total first, float32, int32 and int32.  Totals are formed and compared in float64, an
+    exponential to 2^-51 of its row's largest, and do not depend on where a row lies in memory; ties go to
+    the lowest beam, in a beam to the larger logit, then to the lowest token.  Where fewer candidates are
+    left, the rest are ``-inf``, -1 and -1.  A logit of ``-inf`` is masked; a beam whose logits hold NaN or
+    ``+inf`` proposes nothing.
 
     ``ended`` ``(B, K)`` bool: beams that are finished and compete with their score as it is; they
     propose the token ``pad`` alone, whatever their logits.  No autograd.
