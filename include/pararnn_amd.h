@@ -675,7 +675,7 @@ PRNN_API int prnn_pages_copy(int slots, const prnn_pool* pools, int n_pools, con
 /* Beams (B, K) of searches and their children: table (B, K) names the beams' slots, parents (B, K)
  * each child's beam of its search (outside 0 .. K - 1: none).  A beam's first child keeps its slot, the
  * other children, in order, take the slots of the beams without children, in order, with a copy of
- * their parent's slot in every pool; table is rewritten.  K <= 1024; scratch: 2 B K ints.  No two
+ * their parent's slot in every pool; table is rewritten.  K <= 1024, B < 2^22; scratch: 2 B K ints.  No two
  * entries of table name one slot. */
 PRNN_API int prnn_pages_reorder(int slots, const prnn_pool* pools, int n_pools, int* table,
                                 const int* parents, int B, int K, int* scratch, void* stream);

@@ -360,6 +360,7 @@ extern "C" PRNN_API int prnn_pages_reorder(int slots, const prnn_pool* pools, in
   if (int rc = check_cache("pages_reorder", &none, slots, pools, n_pools)) return rc;
   if (B < 0 || K < 1 || K > kBeams || static_cast<long long>(B) * K > 1ll << 30)
     return fail(PRNN_ERR_VALUE, "pages_reorder: B=%d, K=%d: K must be in 1 .. %d", B, K, kBeams);
+  if (int rc = check_grid("pages_reorder", B, kPlan)) return rc;
   if (B == 0) return PRNN_OK;
   if (!table || !parents || !scratch)
     return fail(PRNN_ERR_VALUE, "pages_reorder: table, parents and scratch must be non-null");

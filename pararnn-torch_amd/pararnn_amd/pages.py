@@ -123,8 +123,8 @@ def reorder_pages(pools: Sequence[Tensor] | Tensor, table: Tensor, parents: Tens
     A beam's first child keeps its slot; the other children, in order, take the slots of the beams
     without children, in order, so a search keeps its slots and only what they hold is copied, once
     for every beam without a child.  A child without a parent (an entry outside ``0 .. K - 1``, -1) or
-    of a beam whose slot is outside the pool gets a slot that is not written.  ``K`` at most 1024; no
-    two entries of ``table`` may name one slot."""
+    of a beam whose slot is outside the pool gets a slot that is not written.  ``K`` at most 1024,
+    ``B`` below 2^22; no two entries of ``table`` may name one slot."""
     what = "reorder_pages"
     pools, rows, slots, dev = _pools(what, pools, None, None)
     if dev is None:
