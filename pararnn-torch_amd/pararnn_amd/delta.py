@@ -58,12 +58,13 @@ class _DeltaProblem(_Problem):
     what = "delta_rule"
 
     def __init__(self, q, k, v, g, beta, h0, table, packed, scale):
-        self.b = beta
-        self.b_code = _rate_code(self.what, beta, q)
+        self.b, self.b_code = beta, None
         super().__init__(q, k, v, g, h0, table, packed, scale)
 
     def _fill(self) -> None:
         super()._fill()
+        if self.b_code is None:  # (q, whose type it may be, has been checked by now)
+            self.b_code = _rate_code(self.what, self.b, self.q)
         batch, time, heads, _, _ = self.dims
         if tuple(self.b.shape) != (batch, time, heads):
             raise ValueError(f"{self.what}: beta must be {(batch, time, heads)}, got "
