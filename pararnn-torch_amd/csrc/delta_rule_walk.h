@@ -352,7 +352,10 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
         to[i] = __float_as_uint(v[i]);
     }
   };
-  auto hold_rows = [&](float* v) {
+  // Rows of tokens, those that `stop` tells (behind the walk's direction of it) as NaN: in bf16 only after
+  // they are turned, whose sums with zeros run over tokens.
+  auto hold_rows = [&](float* v, bool poisoned, int stop) {
+    constexpr float kNan = __builtin_nanf("");
     if constexpr (kNarrow) {
       Op<M, 1> o[2][TF];
 #pragma unroll
@@ -370,9 +373,19 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
 #pragma unroll
           for (int r = 0; r < RT; ++r) d[RT * t + r] = x[r];
         }
+        if (poisoned) {
+#pragma unroll
+          for (int i = 0; i < NC; ++i) {
+            const int r = i % RT, token = NC * (i / RT) + nn, from = __shfl(stop, 4 * G * (r >> 2) + 4 * g + (r & 3));
+            if (kBack ? token <= from : token >= from) d[i] = kNan;
+          }
+        }
         hold(p ? held_l : held_u, d);
       }
     } else {
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        if (kBack ? at_token(i) <= stop : at_token(i) >= stop) v[i] = kNan;
       hold(held_u, v);
     }
   };
@@ -571,6 +584,49 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
     Op<M, 1> zo[TF];
 #pragma unroll
     for (int f = 0; f < TF; ++f) zo[f] = col_op<M, G, RZ>(zat, 8 * G * f, 0);
+
+    // A token that is not finite, in this column or (the system's word) in all of them, must not reach
+    // earlier ones, and backwards later ones, through products with zeros: from it on (backwards: up to
+    // it) the column's tokens take no part, and get NaN afterwards.
+    constexpr int kNone = kBack ? -1 : kDrC;
+    int stop = kNone;
+    bool poisoned = false;
+    auto reached = [&](int token) { return kBack ? token <= stop : token >= stop; };
+    auto widen = [&](const float* x, int from) {  // by what is not finite of elements from .. from + 7
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (!(x[i] * 0.0f == 0.0f)) stop = kBack ? max(stop, at_token(from + i)) : min(stop, at_token(from + i));
+    };
+    auto agree = [&]() {  // the lanes of a column
+#pragma unroll
+      for (int m = NC; m < 64; m <<= 1) stop = kBack ? max(stop, __shfl_xor(stop, m)) : min(stop, __shfl_xor(stop, m));
+    };
+    if constexpr (kBack) {
+      float zero = 0.0f;
+#pragma unroll
+      for (int f = 0; f < TF; ++f) {
+        float v[8];
+        values(zo[f], v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) zero = fmaf(v[e], 0.0f, zero);
+      }
+      if (__any(!(zero == 0.0f))) {
+        float v[8];
+#pragma unroll
+        for (int f = 0; f < TF; ++f) {
+          values(zo[f], v);
+          widen(v, 8 * f);
+        }
+        agree();
+#pragma unroll
+        for (int f = 0; f < TF; ++f) {
+          values(zo[f], v);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = reached(at_token(8 * f + e)) ? 0.0f : v[e];
+          zo[f] = parts_of<M, 1>(v);
+        }
+      }
+    }
     if constexpr (!kBack) {
 #pragma unroll
       for (int f = 0; f < TF; ++f) {
@@ -613,27 +669,21 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
       }
     }
 
-    // A token that is not finite, in this column or (the system's word) in all of them, must not
-    // reach earlier ones through products with zeros: from it on the column's tokens take no part,
-    // and get NaN afterwards.
-    int stop = kDrC;
-    bool poisoned = false;
-    if constexpr (!kBack) {
+    {
       float zero = 0.0f;
 #pragma unroll
       for (int i = 0; i < NC; ++i) zero = fmaf(y[i], 0.0f, zero);
       const int all = __float_as_int(sW[kWmeta * 64 + 1]);
-      poisoned = __any(!(zero == 0.0f) || all < kDrC);
+      poisoned = __any(!(zero == 0.0f) || all < kDrC || stop != kNone);
       if (poisoned) {
-        stop = all;
+        // (backwards what such a token's keys do to the system, which is without them, is not known)
+        if (all < kDrC) stop = kBack ? kDrC - 1 : all;
+#pragma unroll
+        for (int f = 0; f < TF; ++f) widen(y + 8 * f, 8 * f);
+        agree();
 #pragma unroll
         for (int i = 0; i < NC; ++i)
-          if (!(y[i] * 0.0f == 0.0f)) stop = min(stop, at_token(i));
-#pragma unroll
-        for (int m = NC; m < 64; m <<= 1) stop = min(stop, __shfl_xor(stop, m));
-#pragma unroll
-        for (int i = 0; i < NC; ++i)
-          if (at_token(i) >= stop) y[i] = 0.0f;
+          if (reached(at_token(i))) y[i] = 0.0f;
       }
     }
 
@@ -670,10 +720,10 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
 #pragma unroll
       for (int r = 0; r < 4; ++r) u[i + r] = b[r] * Y[(i + r) / RT][(i + r) % RT];
     }
-    if (!kBack && poisoned) {
+    if (poisoned) {
 #pragma unroll
       for (int i = 0; i < NC; ++i)
-        if (at_token(i) >= stop) u[i] = 0.0f;
+        if (reached(at_token(i))) u[i] = 0.0f;
     }
 
     if constexpr (kOut) {
@@ -717,20 +767,19 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
       hold(held_o, v);
       if constexpr (KIND == kDrKept) {
 #pragma unroll
-        for (int i = 0; i < NC; ++i)
-          v[i] = at_token(i) >= stop ? __int_as_float(0x7fc00000) : Y[i / RT][i % RT];
-        hold_rows(v);
+        for (int i = 0; i < NC; ++i) v[i] = Y[i / RT][i % RT];
+        hold_rows(v, poisoned, stop);
       }
     }
     if constexpr (KIND == kDrBackward) {
       float dv[NC];
 #pragma unroll
       for (int i = 0; i < NC; ++i) dv[i] = u[i];
-      hold_rows(dv);
       if constexpr (kNarrow) {
 #pragma unroll
-        for (int i = 0; i < NC; ++i) held32[i] = u[i];
+        for (int i = 0; i < NC; ++i) held32[i] = reached(at_token(i)) ? __int_as_float(0x7fc00000) : u[i];
       }
+      hold_rows(dv, poisoned, stop);
     }
     held_n = n;
     held_c = c;
@@ -776,7 +825,7 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
         into(qat, go);
       }
     }
-    if (!kBack && poisoned && stop < kDrC) {
+    if (poisoned && stop != kNone) {
 #pragma unroll
       for (int t = 0; t < KT; ++t)
 #pragma unroll

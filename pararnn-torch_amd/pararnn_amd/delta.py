@@ -155,6 +155,10 @@ def delta_rule(q: Tensor, k: Tensor, v: Tensor, log_decay: Tensor, beta: Tensor,
     ``k``, ``v``, ``log_decay``, ``beta`` and ``h0``; between the passes a call keeps what its tokens
     wrote and the states before its chunks of 64 tokens, 4 bytes an element, and 26 KB of a chunk's
     system per head.
+
+    What is not finite in a token's inputs reaches no earlier token's output, and in its output's gradient
+    no later token's gradients; a ``q``, key, decay or rate that is not finite may leave NaN in the
+    gradients of all tokens of its chunk.
     """
     what = "delta_rule"
     _no_tangents(what, q, k, v, log_decay, beta, h0)
