@@ -28,8 +28,8 @@
 // chunks at once (delta_rule_grad.hip).
 //
 // Two arithmetics: bf16 storage of widths in eights on bf16 matrix instructions, operands that are
-// not given in bf16 in two or three bf16 parts (delta_rule_walk.h); everything else (fp32, fp16, odd
-// widths) on fp32 ones.
+// not given in bf16 in three bf16 parts, all of an fp32 value's 24 bits; everything else (fp32, fp16, odd
+// widths) on fp32 ones.  Whatever goes through memory (systems, kept errors, states and adjoints) is fp32.
 #pragma once
 
 #include "linear_attention.h"
@@ -129,7 +129,7 @@ struct DrSystems {
   float scale;
 };
 
-// Matrices that are only read as operands lie in memory as such: tiles of 32 rows, steps of 16 columns,
+// Matrices that are only read as operands lie in memory as such, in fp32: tiles of 32 rows, steps of 16 columns,
 // lane by lane the 8 places that it has of a row (tiles.h); what is behind the matrix holds zeros.
 inline __host__ __device__ size_t dr_operand_elems(int rows, int cols) {
   return static_cast<size_t>((rows + 31) / 32) * ((cols + 15) / 16) * 512;
@@ -145,10 +145,9 @@ struct DrWalk {
   const char* sys;
   void* out;                 // forwards: o by the strides below, storage type
   long long o_sb, o_st, o_sh;
-  void* e;                   // forwards: (chunk, H), 64 x Dv as operands, bf16 in two parts or fp32
-  void* keep;                // (chunk, H), Dk x Dv likewise: states before the chunks, adjoints behind them
-  void *dv, *dv_lo;          // backwards, dense (token, H, Dv): of the arithmetic's type, bf16: and what that leaves
-  float* dv32;               // or floats besides (heads that are summed afterwards)
+  float* e;                  // forwards: (chunk, H), 64 x Dv as operands
+  float* keep;               // (chunk, H), Dk x Dv likewise: states before the chunks, adjoints behind them
+  float* dv;                 // backwards, dense (token, H, Dv)
   LaState init, last;
   float* piece;              // (piece, H, Dk, Dv): the pieces' own states
   uint16_t* transfer;        // (piece, H): their transfers, as operands in three bf16 parts
@@ -163,11 +162,12 @@ struct DrWalk {
 struct DrGrad {
   LaSeqs seqs;
   LaView q, k, go;
-  LaDecay g, b;
+  LaDecay g;
   const char* sys;           // only its decays and rates are read
-  const void *e, *before, *behind;  // as operands: (chunk, H), 64 x Dv and Dk x Dv
-  const void *dv, *dv_lo;    // (token, H, Dv) of the arithmetic's type
-  void *dq, *dk;             // (token, H, Dk): the arithmetic's type, or floats (q_f32, k_f32)
+  const float *e, *before, *behind;  // as operands: (chunk, H), 64 x Dv and Dk x Dv
+  const float* dv;           // (token, H, Dv)
+  void* dv16;                // on bf16 instructions: where it goes as the result (NULL: heads are summed)
+  void *dq, *dk;             // (token, H, Dk): the storage type, or floats (q_f32, k_f32)
   int q_f32, k_f32;
   void *dg, *dbeta;          // (token, H); dg NULL: not wanted, or sums per chunk:
   float* g_part;             // (chunk, H)
@@ -189,7 +189,7 @@ int dr_grad(const DrGrad& a, bool bf16, hipStream_t stream);
 
 // Waves of a walk's workgroup, `cols` columns each.  items: (piece, head) pairs.  Narrow values have two
 // column tiles' waves at most; and where there is a CU for each half of a workgroup, halves (D = 64, 128
-// sequences' heads: 99 us forwards, 112 whole; 350 pieces: 155 us, 117 whole; both in two parts).
+// sequences' heads: 99 us forwards, 112 whole; 350 pieces: 155 us, 117 whole; with operands of two parts).
 inline int dr_walk_group(int Dk, int Dv, int cols, bool bf16, long long items) {
   if (!bf16) return Dk <= 128 ? 4 : 2;
   if (Dk > 128) return 4;

@@ -50,7 +50,7 @@ LaSeqs sequences_of(const Problem& a) {
 // What the backward pass reads of the forward one: as operands e and the states before the chunks, and
 // the chunks' systems.
 struct Kept {
-  void *e, *before;
+  float *e, *before;
   char* sys;
   int* order;  // of a packed batch's pieces
   size_t bytes;
@@ -58,11 +58,11 @@ struct Kept {
 int pieces_of(const Problem& a);  // (of a plan; 0: not packed)
 Kept kept_of(void* p, const Problem& a) {
   Carver c(p);
-  const size_t size = 4, heads = a.la.H;  // bytes of an element, in two bf16 parts or fp32
+  const size_t heads = a.la.H;
   Kept k{};
   const size_t units = dr_units(sequences_of(a), kDrC);
-  k.e = c.take(units * heads * dr_operand_elems(kDrC, a.la.Dv) * size);
-  k.before = c.take(units * heads * dr_operand_elems(a.la.Dk, a.la.Dv) * size);
+  k.e = static_cast<float*>(c.take(4 * units * heads * dr_operand_elems(kDrC, a.la.Dv)));
+  k.before = static_cast<float*>(c.take(4 * units * heads * dr_operand_elems(a.la.Dk, a.la.Dv)));
   k.sys = static_cast<char*>(c.take(units * heads * kDrSys));
   k.order = static_cast<int*>(c.take(4 * static_cast<size_t>(pieces_of(a))));
   k.bytes = c.used;
@@ -72,10 +72,10 @@ Kept kept_of(void* p, const Problem& a) {
 struct Scratch {
   char* sys;
   int* order;
-  void *behind, *dv, *dv_lo;
+  float *behind, *dv;
   float* piece;
   uint16_t* transfer;
-  float *dq32, *dk32, *dv32, *g_part;
+  float *dq32, *dk32, *g_part;
   size_t bytes;
 };
 
@@ -141,7 +141,7 @@ int pieces_of(const Problem& a) {
 Scratch carve(void* ws, const Problem& a, const Plan& plan, bool systems, bool backward, bool decay_grad) {
   Carver c(ws);
   Scratch s{};
-  const size_t heads = a.la.H, tokens = tokens_of(a), size = on_bf16(a) ? 2 : 4;
+  const size_t heads = a.la.H, tokens = tokens_of(a);
   const size_t units = dr_units(plan.seqs, kDrC);
   if (systems) {
     s.sys = static_cast<char*>(c.take(units * heads * kDrSys));
@@ -153,12 +153,10 @@ Scratch carve(void* ws, const Problem& a, const Plan& plan, bool systems, bool b
     s.transfer = static_cast<uint16_t*>(c.take(6 * pieces * dr_operand_elems(a.la.Dk, a.la.Dk)));
   }
   if (backward) {
-    s.behind = c.take(units * heads * dr_operand_elems(a.la.Dk, a.la.Dv) * 4);
-    if (on_bf16(a)) s.dv_lo = c.take(tokens * heads * a.la.Dv * 2);
-    // dv is written where it is wanted, unless its heads are summed or it is stored in another type
-    const bool sums = a.la.v.heads != a.la.H;
-    if (sums || (!on_bf16(a) && a.la.dtype != PRNN_F32)) s.dv = c.take(tokens * heads * a.la.Dv * size);
-    if (sums && on_bf16(a)) s.dv32 = static_cast<float*>(c.take(4 * tokens * heads * a.la.Dv));
+    s.behind = static_cast<float*>(c.take(4 * units * heads * dr_operand_elems(a.la.Dk, a.la.Dv)));
+    // fp32 dv is written where it is wanted, unless its heads are summed or it is stored in another type
+    if (a.la.v.heads != a.la.H || a.la.dtype != PRNN_F32)
+      s.dv = static_cast<float*>(c.take(4 * tokens * heads * a.la.Dv));
     if (a.la.q.heads != a.la.H) s.dq32 = static_cast<float*>(c.take(4 * tokens * heads * a.la.Dk));
     if (a.la.k.heads != a.la.H) s.dk32 = static_cast<float*>(c.take(4 * tokens * heads * a.la.Dk));
     if (decay_grad) s.g_part = static_cast<float*>(c.take(4 * units * heads));
@@ -268,9 +266,7 @@ int backward(const Problem& a, const prnn_la_view& go, const float* gs, const vo
   DrWalk w = walk_of(a, p, s, k.sys, k.order);
   w.z = la_view(go, a.la, a.la.Dv);
   w.keep = s.behind;
-  w.dv = s.dv ? s.dv : dv;
-  w.dv_lo = s.dv_lo;
-  w.dv32 = s.dv32;
+  w.dv = s.dv ? s.dv : static_cast<float*>(dv);
   w.init = LaState{const_cast<float*>(gs), nullptr, sequences(a)};
   w.last = LaState{dh0, nullptr, sequences(a)};
   if (int rc = walk(w, true, a, p, st)) return rc;
@@ -280,11 +276,10 @@ int backward(const Problem& a, const prnn_la_view& go, const float* gs, const vo
   g.k = w.k;
   g.go = w.z;
   g.g = decay_of(a);
-  g.b = rate_of(a);
   g.sys = k.sys;
   g.e = k.e;
   g.dv = w.dv;
-  g.dv_lo = s.dv_lo;
+  g.dv16 = on_bf16(a) && a.la.v.heads == a.la.H ? dv : nullptr;
   g.before = k.before;
   g.behind = s.behind;
   g.q_f32 = s.dq32 != nullptr;
@@ -303,7 +298,7 @@ int backward(const Problem& a, const prnn_la_view& go, const float* gs, const vo
   g.scale = a.la.scale;
   if (int rc = dr_grad(g, on_bf16(a), st)) return rc;
   LaHeadSums hs{};
-  const float* from[3] = {s.dq32, s.dk32, s.dv32 ? s.dv32 : static_cast<const float*>(s.dv)};
+  const float* from[3] = {s.dq32, s.dk32, g.dv16 ? nullptr : s.dv};
   void* to[3] = {dq, dk, dv};
   const int D[3] = {a.la.Dk, a.la.Dk, a.la.Dv}, heads[3] = {a.la.q.heads, a.la.k.heads, a.la.v.heads};
   bool sums = false;

@@ -4,7 +4,7 @@
 // 1. Pairs of tokens, a tile of 32 x 32 of the lower triangle per wave: go e^T, dv e^T, q k^T, k k^T;
 //    and the products with the states, tiles of 32 columns and 32 tokens, formed transposed (lane:
 //    token).  Tokens' rows come through LDS in slabs of 64 columns, states and e as operands.
-// 2. The pairs, weighted, as operands in LDS, over the slabs of go and dv: the rest of dq and dk.
+// 2. The pairs, weighted, in fp32 in LDS, over the slabs of go and dv: the rest of dq and dk.
 // 3. dL/dg_t is the flow through the decay of token t,
 //      F_t = sum over sources j < t and uses l >= t of what l reads of j,
 //    where a source may also be the state before the chunk and a use the adjoint behind it.  It is
@@ -14,8 +14,9 @@
 //
 // Eight waves: four for the pairs and dq, four for dk, each with its own code and the same barriers, so
 // that two workgroups a CU (what LDS holds) are four waves a SIMD (four waves that did all took 1.24
-// times as long).  4096 chunks of bf16, D = 64: 128 us for 435 MB, of which 260 reach memory (3.4 TB/s of
-// all); the phases' latencies bound it, no unit is busy for half of the time.
+// times as long).  4096 chunks of bf16, D = 64: 158 us for 470 MB, of which 317 reach memory (3 TB/s of all).
+// Vector instructions take half of the time, most of them the splits of fp32 operands into three bf16 parts
+// (125 us with two parts, whose 16 bits showed in the results' last place), the phases' latencies the rest.
 #include "delta_rule_loads.h"
 
 namespace prnn {
@@ -31,17 +32,16 @@ __global__ __launch_bounds__(512, sizeof(typename M::E) == 2 && KS == 1 ? 4 : 2)
   constexpr bool kNarrow = sizeof(E) == 2;
   constexpr int ES = static_cast<int>(sizeof(E));
   constexpr int kAt = 2;  // steps whose operands are under way
-  constexpr int RB = dr_row_k(kNarrow, 64), P = M::kParts, kSlab = kDrC * RB;
-  // k, q, go, dv (bf16: and what that leaves); the pairs go u^T and X by parts, in the place of go and dv
-  // where those are read once
-  constexpr int kRows = 3 + P, kSlabs = kRows + (WIDE ? 2 * P : 1);
-  __shared__ __align__(16) char lds[kSlabs * kSlab];
+  constexpr int RB = dr_row_k(kNarrow, 64), kSlab = kDrC * RB;
+  constexpr int RF = dr_row_k(false, 64), kFloats = kDrC * RF;  // a slab of floats
+  // k, q, go, dv; the pairs go u^T and X, in the place of go and dv where those are read once
+  constexpr int kPairsAt = WIDE ? 3 * kSlab + kFloats : 2 * kSlab;
+  __shared__ __align__(16) char lds[kPairsAt + 2 * kFloats];
   __shared__ float sF[kDrC * kLf], s_in[2][8][kDrC], s_out[8][kDrC];
   __shared__ __align__(16) float sw[kDrW * 64];
   __shared__ float s_through[4], s_own[kDrC], s_into[kDrC], s_waves[8];
   char *const sK = lds, *const sQ = lds + kSlab, *const sG = lds + 2 * kSlab, *const sD = lds + 3 * kSlab;
-  char *const sL = lds + 4 * kSlab, *const sP = WIDE ? lds + kRows * kSlab : sG;
-  char* const s_x = WIDE ? lds + (kRows + P) * kSlab : lds + 4 * kSlab;
+  char *const sP = lds + kPairsAt, *const s_x = sP + kFloats;
   const int h = blockIdx.x % A.H, id = blockIdx.x / A.H;
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, half = lane >> 5;
   const int wave = (tid >> 6) & 3;
@@ -54,35 +54,46 @@ __global__ __launch_bounds__(512, sizeof(typename M::E) == 2 && KS == 1 ? 4 : 2)
   const int n = u.end - u.begin, batch = dr_batch(A.seqs, u);
   const size_t tok0 = dr_token(A.seqs, u, u.begin);
   const size_t unit = static_cast<size_t>(id) * A.H + h;
-  const int TS = A.dtype == PRNN_F32 ? 4 : 2, kCode = kNarrow ? PRNN_BF16 : PRNN_F32;
+  const int TS = A.dtype == PRNN_F32 ? 4 : 2;
   auto rows = [&](const LaView& v) {
     return static_cast<const char*>(v.p) + (batch * v.sb + (h / v.rep) * v.sh +
                                             static_cast<long long>(u.begin) * v.st) * TS;
   };
   const char *pq = rows(A.q), *pk = rows(A.k), *pg = rows(A.go);
-  const char* pd = static_cast<const char*>(A.dv) + (tok0 * A.H + h) * A.Dv * ES;
-  const char* pl = kNarrow ? static_cast<const char*>(A.dv_lo) + (tok0 * A.H + h) * A.Dv * ES : nullptr;
-  auto operands = [&](const void* p, int r, int c) {
+  const float* pd = A.dv + (tok0 * A.H + h) * A.Dv;
+  const int d_step = A.H * A.Dv;
+  auto operands = [&](const float* p, int r, int c) {
     const size_t elems = dr_operand_elems(r, c);
-    return make_rsrc(static_cast<const E*>(p) + unit * P * elems, static_cast<uint32_t>(elems) * P * ES);
+    return make_rsrc(p + unit * elems, static_cast<uint32_t>(elems) * 4);
   };
   const rsrc_t re = operands(A.e, kDrC, A.Dv), rS = operands(A.before, A.Dk, A.Dv),
                rR = operands(A.behind, A.Dk, A.Dv);
-  const int part_e = static_cast<int>(dr_operand_elems(kDrC, A.Dv)) * ES,
-            part_s = static_cast<int>(dr_operand_elems(A.Dk, A.Dv)) * ES;
   const int vs = (A.Dv + 15) / 16, last_k = (A.Dk - 1) / 64 * 64;
-  Staged<M, 64, 512> ga, gb, gl, ka, kb;
+  Staged<M, 64, 512> ga, ka, kb;
+  std::conditional_t<kNarrow, StagedFloats<64, 512>, Staged<M, 64, 512>> gd;
+  auto fetch_dv = [&](int v0) {
+    if constexpr (kNarrow)
+      gd.fetch(pd, d_step, n, v0, A.Dv);
+    else
+      gd.fetch(reinterpret_cast<const char*>(pd), d_step, n, v0, A.Dv, PRNN_F32);
+  };
+  auto put_dv = [&](int v0, bool result) {
+    if constexpr (kNarrow) {
+      gd.template put<RF>(sD);
+      if (result && A.dv16) gd.as_bf16(static_cast<uint16_t*>(A.dv16) + (tok0 * A.H + h) * A.Dv, d_step, n, v0, A.Dv);
+    } else {
+      gd.template put<RF>(sD, PRNN_F32);
+    }
+  };
   ga.fetch(pg, A.go.st, n, 0, A.Dv, A.dtype);
-  gb.fetch(pd, static_cast<long long>(A.H) * A.Dv, n, 0, A.Dv, kCode);
-  if constexpr (kNarrow) gl.fetch(pl, static_cast<long long>(A.H) * A.Dv, n, 0, A.Dv, kCode);
+  fetch_dv(0);
   ka.fetch(pk, A.k.st, n, last_k, A.Dk, A.dtype);
   kb.fetch(pq, A.q.st, n, last_k, A.Dk, A.dtype);
   const float* weights = reinterpret_cast<const float*>(A.sys + unit * kDrSys + 2 * kDrTiles);
   const int kt = wave & 1, it = wave >> 1, t = 32 * it + l32;
   for (int i = tid; i < kDrW * 64; i += 512) sw[i] = weights[i];
   ga.template put<RB>(sG, A.dtype);
-  gb.template put<RB>(sD, kCode);
-  if constexpr (kNarrow) gl.template put<RB>(sL, kCode);
+  put_dv(0, true);
   ka.template put<RB>(sK, A.dtype);
   kb.template put<RB>(sQ, A.dtype);
 
@@ -95,29 +106,29 @@ __global__ __launch_bounds__(512, sizeof(typename M::E) == 2 && KS == 1 ? 4 : 2)
     constexpr bool kLead = decltype(role)::value;
     // operands of a wave's tiles of the states and of its tokens' e; the pairs' earlier tokens are the
     // same ones (waves 0 and 1: the first 32, wave 2: the others)
-    Op<M, P> ei[kAt], S[KS][kAt], R[KS][kAt];
+    Eight ei[kAt], S[KS][kAt], R[KS][kAt];
     auto fetch = [&](int p0, int v0, int f0) {
 #pragma unroll
       for (int f = 0; f < kAt; ++f) {
         const int step = v0 / 16 + f0 + f;
-        ei[f] = global_op<M>(re, step < vs, it * vs + step, part_e);
+        ei[f] = global_op(re, step < vs, it * vs + step);
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
           const int tile = p0 / 32 + 2 * s + kt;
-          S[s][f] = global_op<M>(rS, (step < vs) & (32 * tile < A.Dk), tile * vs + step, part_s);
-          if constexpr (!kLead) R[s][f] = global_op<M>(rR, (step < vs) & (32 * tile < A.Dk), tile * vs + step, part_s);
+          S[s][f] = global_op(rS, (step < vs) & (32 * tile < A.Dk), tile * vs + step);
+          if constexpr (!kLead) R[s][f] = global_op(rR, (step < vs) & (32 * tile < A.Dk), tile * vs + step);
         }
       }
     };
-    auto dv_op = [&](int token, int f) {
-      Op<M, P> o;
-      if constexpr (kNarrow) {
-        o.p[0] = row_op<M, 2>(sD + token * RB, f, half).p[0];
-        o.p[1] = row_op<M, 2>(sL + token * RB, f, half).p[0];
-      } else {
-        o = row_op<M, 2>(sD + token * RB, f, half);
-      }
-      return o;
+    // what lies in LDS as floats, as operands of 24 bits: a token's dv, a pair's row and column
+    auto float_row = [&](const char* rows, int token, int f) {
+      auto o = row_op<InF32, 2>(rows + token * RF, f, half);
+      return parts_of<M, 3>(o.x);
+    };
+    const int column_at = col_share<InF32, 2, RF>(lane);
+    auto float_col = [&](const char* rows, int t0, int c0) {
+      auto o = col_op<InF32, 2, RF>(rows + column_at, t0, c0);
+      return parts_of<M, 3>(o.x);
     };
     const bool pairs = kLead && wave < 3;
 
@@ -134,12 +145,10 @@ __global__ __launch_bounds__(512, sizeof(typename M::E) == 2 && KS == 1 ? 4 : 2)
       for (int v0 = 0; v0 < A.Dv; v0 += 64) {
         if (p0 > 0 || v0 > 0) {
           ga.fetch(pg, A.go.st, n, v0, A.Dv, A.dtype);
-          gb.fetch(pd, static_cast<long long>(A.H) * A.Dv, n, v0, A.Dv, kCode);
-          if constexpr (kNarrow) gl.fetch(pl, static_cast<long long>(A.H) * A.Dv, n, v0, A.Dv, kCode);
+          fetch_dv(v0);
           __syncthreads();
           ga.template put<RB>(sG, A.dtype);
-          gb.template put<RB>(sD, kCode);
-          if constexpr (kNarrow) gl.template put<RB>(sL, kCode);
+          put_dv(v0, p0 == 0);
         }
         fetch(p0, v0, 0);
         __syncthreads();
@@ -151,28 +160,26 @@ __global__ __launch_bounds__(512, sizeof(typename M::E) == 2 && KS == 1 ? 4 : 2)
             for (int f = 0; f < kAt; ++f) {
               const auto gi = row_op<M, 2>(sG + t * RB, f0 + f, half);
 #pragma unroll
-              for (int s = 0; s < KS; ++s) mul<32>(main[s], S[s][f], gi);
+              for (int s = 0; s < KS; ++s) mul<32>(main[s], whole<M>(S[s][f]), gi);
               if (p0 == 0 && pairs) {
-                mul<32>(GU, ei[f], row_op<M, 2>(sG + i * RB, f0 + f, half));
-                mul<32>(DU, ei[f], dv_op(i, f0 + f));
+                const auto e = whole<M>(ei[f]);
+                mul<32>(GU, e, row_op<M, 2>(sG + i * RB, f0 + f, half));
+                mul<32>(DU, e, float_row(sD, i, f0 + f));
               }
             }
           } else {
 #pragma unroll
             for (int f = 0; f < kAt; ++f) {
-              const auto di = dv_op(t, f0 + f);
+              const auto di = float_row(sD, t, f0 + f), e = whole<M>(ei[f]);
 #pragma unroll
               for (int s = 0; s < KS; ++s) {
-                mul<32>(main[s], R[s][f], ei[f]);
-                mul<32>(ds[s], S[s][f], di);
                 // from the state before to the adjoint behind: two waves have the same operands, a step each
                 if (((f0 + f) & 1) == it) {
-                  float x[8], y[8];
-                  values(S[s][f], x);
-                  values(R[s][f], y);
 #pragma unroll
-                  for (int e = 0; e < 8; ++e) through = fmaf(x[e], y[e], through);
+                  for (int x = 0; x < 8; ++x) through = fmaf(S[s][f].x[x], R[s][f].x[x], through);
                 }
+                mul<32>(main[s], whole<M>(R[s][f]), e);
+                mul<32>(ds[s], whole<M>(S[s][f]), di);
               }
             }
           }
@@ -219,20 +226,8 @@ __global__ __launch_bounds__(512, sizeof(typename M::E) == 2 && KS == 1 ? 4 : 2)
               w1[r] *= sw[kWb * 64 + jj];
               x[r] *= -sw[kWb * 64 + jj];
             }
-            if constexpr (kNarrow) {
-              auto both = [&](char* hi, char* lo, const float* v) {
-                const u2 a{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-                const u2 b{pack_bf16x2(v[0] - lo_bf16(a[0]), v[1] - hi_bf16(a[0])),
-                           pack_bf16x2(v[2] - lo_bf16(a[1]), v[3] - hi_bf16(a[1]))};
-                *reinterpret_cast<u2*>(hi + i * RB + j0 * 2) = a;
-                *reinterpret_cast<u2*>(lo + i * RB + j0 * 2) = b;
-              };
-              both(sP, sP + kSlab, w1);
-              both(s_x, s_x + kSlab, x);
-            } else {
-              *reinterpret_cast<f4*>(sP + i * RB + j0 * 4) = f4{w1[0], w1[1], w1[2], w1[3]};
-              *reinterpret_cast<f4*>(s_x + i * RB + j0 * 4) = f4{x[0], x[1], x[2], x[3]};
-            }
+            *reinterpret_cast<f4*>(sP + i * RF + j0 * 4) = f4{w1[0], w1[1], w1[2], w1[3]};
+            *reinterpret_cast<f4*>(s_x + i * RF + j0 * 4) = f4{x[0], x[1], x[2], x[3]};
           }
         }
         __syncthreads();
@@ -249,19 +244,6 @@ __global__ __launch_bounds__(512, sizeof(typename M::E) == 2 && KS == 1 ? 4 : 2)
 #pragma unroll
           for (int r = 0; r < 4; ++r) v[r] = a[r];
         }
-      };
-      // the parts of a pair's operand
-      auto parts = [&](auto&& get) {
-        Op<M, P> x;
-#pragma unroll
-        for (int p = 0; p < P; ++p) {
-          const auto one = get(p);
-          if constexpr (kNarrow)
-            x.p[p] = one.p[0];
-          else
-            x = one;
-        }
-        return x;
       };
       const int col_at = col_share<M, 2, RB>(lane);
 #pragma unroll
@@ -297,8 +279,7 @@ __global__ __launch_bounds__(512, sizeof(typename M::E) == 2 && KS == 1 ? 4 : 2)
 #pragma unroll
           for (int f = 0; f < 4; ++f)
             if ((f >> 1) <= it)
-              mul<32>(dq, col_op<M, 2, RB>(kat, 16 * f, 0),
-                      parts([&](int p) { return row_op<M, 2>(sP + p * kSlab + t * RB, f, half); }));
+              mul<32>(dq, col_op<M, 2, RB>(kat, 16 * f, 0), float_row(sP, t, f));
         }
         if constexpr (!kLead) if (any) {
           f16v &du = main[s], &dS = ds[s];
@@ -330,11 +311,10 @@ __global__ __launch_bounds__(512, sizeof(typename M::E) == 2 && KS == 1 ? 4 : 2)
             const int jt = f >> 1;
             const auto kc = col_op<M, 2, RB>(kat, 16 * f, 0);
             // -(X + X^T), rows of X before the token and columns behind it
-            if (jt <= it) mul<32>(du, kc, parts([&](int p) { return row_op<M, 2>(s_x + p * kSlab + t * RB, f, half); }));
+            if (jt <= it) mul<32>(du, kc, float_row(s_x, t, f));
             if (jt >= it) {
-              mul<32>(du, kc, parts([&](int p) { return col_op<M, 2, RB>(s_x + p * kSlab + col_at, 16 * f, 32 * it); }));
-              mul<32>(du, col_op<M, 2, RB>(qat, 16 * f, 0),
-                      parts([&](int p) { return col_op<M, 2, RB>(sP + p * kSlab + col_at, 16 * f, 32 * it); }));
+              mul<32>(du, kc, float_col(s_x, 16 * f, 32 * it));
+              mul<32>(du, col_op<M, 2, RB>(qat, 16 * f, 0), float_col(sP, 16 * f, 32 * it));
             }
           }
         }

@@ -9,11 +9,12 @@
 
 namespace prnn {
 
+// Bytes of a row in LDS.  (Keys of 128 and values of 64 leave no room for more: two chunks of them fill it.)
 constexpr int dr_row_k(bool narrow, int cols) {
-  return narrow ? (cols >= 128 ? cols * 2 + 48 : cols * 2 + 16) : (cols + 4) * 4;
+  return narrow ? (cols > 128 ? cols * 2 + 48 : cols * 2 + 16) : (cols + 4) * 4;
 }
-constexpr int dr_row_z(bool narrow, int cols) {
-  return narrow ? (cols == 32 ? 64 : cols == 64 ? 144 : cols * 2 + 48) : (cols + 4) * 4;
+constexpr int dr_row_z(bool narrow, int cols, int keys) {
+  return !narrow ? (cols + 4) * 4 : cols == 32 || (cols == 64 && keys == 128) ? cols * 2 : cols == 64 ? 144 : cols * 2 + 48;
 }
 
 // Rows of 64 tokens of a head on their way from memory to LDS: 16-byte units in bf16, single
@@ -69,26 +70,56 @@ struct Staged {
   }
 };
 
-// Operand `which` of an array of them (dr_operand_at), its parts `part` bytes apart.
-template <class M>
-__device__ __forceinline__ Op<M, M::kParts> global_op(rsrc_t r, bool in, int which, int part) {
-  constexpr int ES = static_cast<int>(sizeof(typename M::E));
-  const int lane = threadIdx.x & 63;
-  Op<M, M::kParts> o;
-  if constexpr (ES == 2) {
+// Dense rows of floats, widths in fours, on their way from memory to LDS rows of RB bytes.
+template <int COLS, int NT>
+struct StagedFloats {
+  static constexpr int U = COLS / 4, N = kDrC * U / NT;
+  static_assert(NT % U == 0 && kDrC * U % NT == 0, "whole rows and units");
+  u4 r[N];
+  __device__ __forceinline__ void fetch(const float* p, int st, int n, int c0, int width) {
+    const int c = c0 + threadIdx.x % U * 4;
+    const rsrc_t b = make_rsrc(p, n > 0 ? ((n - 1) * st + width) * 4 : 0);
+    const uint32_t at = la_in(c < width, (threadIdx.x / U * st + c) * 4);
 #pragma unroll
-    for (int k = 0; k < M::kParts; ++k)
-      o.p[k] = __builtin_bit_cast(
-          b8, __builtin_amdgcn_raw_buffer_load_b128(r, la_in(in, (which * 64 + lane) * 16 + k * part), 0, 0));
-  } else {
+    for (int k = 0; k < N; ++k) r[k] = __builtin_amdgcn_raw_buffer_load_b128(b, at + k * (NT / U) * st * 4, 0, 0);
+  }
+  template <int RB>
+  __device__ __forceinline__ void put(char* tile) const {
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      const u4 w = __builtin_amdgcn_raw_buffer_load_b128(r, la_in(in, (which * 64 + lane) * 32 + 16 * k), 0, 0);
+    for (int k = 0; k < N; ++k)
+      *reinterpret_cast<u4*>(tile + (threadIdx.x / U + k * (NT / U)) * RB + threadIdx.x % U * 16) = r[k];
+  }
+  // The rows to memory, rounded to bf16.
+  __device__ __forceinline__ void as_bf16(uint16_t* p, int st, int n, int c0, int width) const {
+    const int c = c0 + threadIdx.x % U * 4;
+    const rsrc_t b = make_rsrc(p, n > 0 ? ((n - 1) * st + width) * 2 : 0);
+    const uint32_t at = la_in(c < width, (threadIdx.x / U * st + c) * 2);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o.x[4 * k + i] = __uint_as_float(w[i]);
-    }
+    for (int k = 0; k < N; ++k)
+      __builtin_amdgcn_raw_buffer_store_b64(u2{pack_bf16x2(__uint_as_float(r[k][0]), __uint_as_float(r[k][1])),
+                                               pack_bf16x2(__uint_as_float(r[k][2]), __uint_as_float(r[k][3]))},
+                                            b, at + k * (NT / U) * st * 2, 0, 0);
+  }
+};
+
+// The eight floats that a lane has of operand `which` of an array of them (dr_operand_at).
+struct Eight {
+  float x[8];
+};
+__device__ __forceinline__ Eight global_op(rsrc_t r, bool in, int which) {
+  Eight o;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const u4 w = __builtin_amdgcn_raw_buffer_load_b128(r, la_in(in, (which * 64 + (threadIdx.x & 63)) * 32 + 16 * k), 0, 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o.x[4 * k + i] = __uint_as_float(w[i]);
   }
   return o;
+}
+// As an operand of 24 bits.
+template <class M>
+__device__ __forceinline__ Op<M, 3> whole(Eight o) {
+  return parts_of<M, 3>(o.x);
 }
 
 }  // namespace prnn

@@ -11,15 +11,14 @@
 // barriers only hand K, Q and the system through LDS.  The output is formed transposed from the same
 // registers (state and u as first operands), so that a lane holds consecutive columns of a token.
 //
-// Bound by this chain: one wave a SIMD goes through some 8000 cycles a chunk (bf16, D = 64; matrix
-// instructions 2200 of them, the rest splits of results into bf16 parts, LDS reads and waits), so 2048
-// tokens of 128 heads take 128 us forwards with what is kept and 102 backwards, and 16384 tokens of 8
-// heads, D = 128, in 16 pieces, 67 us.
+// Bound by this chain: one wave a SIMD goes through some 9500 cycles a chunk (bf16, D = 64; matrix
+// instructions 2700 of them, the rest splits of results into bf16 parts, LDS reads and waits), so 2048
+// tokens of 128 heads take 129 us forwards with what is kept and 116 backwards, and 16384 tokens of 8
+// heads, D = 128, in 16 pieces, 74 us.
 //
-// bf16 operands: K, Q and z as they are given; the state, the system and its right side in three parts
-// (24 bits) where they form the chain, in two where an output is rounded to 8 bits afterwards; what the
-// gradients read (e, dv, states, adjoints) in two: their own sums are rounded to 8 bits too, and with one
-// part they came out at 1.5 to 3 times that rounding.
+// bf16 operands: K, Q and z as they are given; the state, what the tokens write, the system and its right
+// side in three parts (all 24 bits of an fp32 value).  What the gradients read (e, dv, states, adjoints)
+// leaves in fp32.
 #pragma once
 
 #include "delta_rule_loads.h"
@@ -49,13 +48,14 @@ __device__ __forceinline__ void fill(char* tile, const char* p, long long st, in
 struct NotStaged {};
 
 // Operands of a stored matrix (the system's inverse or the pairs): rows NC rt .. of the 64, step f of
-// the contraction over tokens; BACK: of the transposed matrix, read down the stored rows.
+// the contraction over tokens; BACK: of the transposed matrix, read down the stored rows.  On bf16
+// instructions it lies in LDS in three parts, one after another.
 template <class M, int NC, bool BACK>
 struct Stored {
-  using E = typename M::E;
+  static constexpr bool kSplit = sizeof(typename M::E) == 2;
   static constexpr int G = 64 / NC;
-  static constexpr int ES = static_cast<int>(sizeof(E)), kRow = 32 * ES, kUnit = 4 * ES;
-  static constexpr int kTile = kDrTiles / 3 / (ES == 2 ? 2 : 1);
+  static constexpr int ES = kSplit ? 2 : 4, kRow = 32 * ES, kUnit = 4 * ES;
+  static constexpr int kTile = kDrTiles / 3 / (kSplit ? 2 : 1);
   // whether there is anything in the 32 x 32 tile
   static constexpr bool any(int rt, int f) {
     const int a = NC * rt / 32, b = 8 * G * f / 32;
@@ -64,12 +64,11 @@ struct Stored {
   static __device__ __forceinline__ const char* at(const char* tile, int row, int col) {
     return tile + row * kRow + dr_unit_of(row, col >> 2) * kUnit + (col & 3) * ES;
   }
-  template <int P>
-  static __device__ __forceinline__ Op<M, P> get(const char* m, int rt, int f, int n, int g) {
+  static __device__ __forceinline__ Op<M, 3> get(const char* m, int rt, int f, int n, int g) {
     const char* t = m + (NC * rt / 32 + 8 * G * f / 32) * kTile;
     const int own = (NC * rt) & 31, other = (8 * G * f) & 31;
-    Op<M, P> o;
-    if constexpr (ES == 2) {
+    if constexpr (kSplit) {
+      Op<M, 3> o;
       const char *x, *y;
       if constexpr (BACK) {
         const int lane = threadIdx.x & 63, i = lane & 15, gg = lane >> 4;
@@ -82,7 +81,7 @@ struct Stored {
         y = at(t, own + n, other + 4 * G + 4 * g);
       }
 #pragma unroll
-      for (int p = 0; p < P; ++p) {
+      for (int p = 0; p < 3; ++p) {
         union {
           u2 h[2];
           s4 s[2];
@@ -97,20 +96,24 @@ struct Stored {
         }
         o.p[p] = r.v;
       }
-    } else if constexpr (BACK) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        o.x[i] = *reinterpret_cast<const float*>(at(t, other + 4 * G * (i >> 2) + 4 * g + (i & 3), own + n));
+      return o;
     } else {
-      const f4 x = *reinterpret_cast<const f4*>(at(t, own + n, other + 4 * g));
-      const f4 y = *reinterpret_cast<const f4*>(at(t, own + n, other + 4 * G + 4 * g));
+      float v[8];
+      if constexpr (BACK) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        o.x[i] = x[i];
-        o.x[4 + i] = y[i];
+        for (int i = 0; i < 8; ++i)
+          v[i] = *reinterpret_cast<const float*>(at(t, other + 4 * G * (i >> 2) + 4 * g + (i & 3), own + n));
+      } else {
+        const f4 x = *reinterpret_cast<const f4*>(at(t, own + n, other + 4 * g));
+        const f4 y = *reinterpret_cast<const f4*>(at(t, own + n, other + 4 * G + 4 * g));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[i] = x[i];
+          v[4 + i] = y[i];
+        }
       }
+      return parts_of<M, 3>(v);
     }
-    return o;
   }
 };
 
@@ -146,7 +149,7 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
   constexpr int KF = KD / (8 * G);   // steps of a contraction over its rows
   constexpr int TT = kDrC / NC;      // token tiles
   constexpr int TF = kDrC / (8 * G); // steps of a contraction over tokens
-  constexpr int RK = dr_row_k(kNarrow, KD), RZ = dr_row_z(kNarrow, VT);
+  constexpr int RK = dr_row_k(kNarrow, KD), RZ = dr_row_z(kNarrow, VT, KD);
   constexpr bool kQ = KIND != kDrState;  // Q takes part
   constexpr bool kP = KIND != kDrState;
   constexpr int ES = static_cast<int>(sizeof(E));
@@ -155,11 +158,9 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
   // fp32 widths over 64 have no registers for the next chunk's K and Q, over 128 no LDS for the system
   constexpr bool kAhead = kNarrow || KD <= 64, kSysLds = kNarrow || KD <= 128;
   static_assert(kAhead || kDrC * KD % (16 * NT) == 0, "whole rounds of fill");
-  // The system comes in fp32 and lies in LDS in bf16 parts: three of the inverse, two of the pairs, of which
-  // a backward pass takes a third where there is room for it.
-  constexpr int kTParts = kNarrow ? 3 : 1, kPParts = !kNarrow ? 1 : kBack && KD <= 64 ? 3 : 2;
-  constexpr int kPart = kDrTiles / (kNarrow ? 2 : 1);
-  constexpr int kPairsAt = kPart * kTParts, kSysBytes = kPairsAt + (kP ? kPart * kPParts : 0);
+  // (the system comes in fp32)
+  constexpr int kPart = kDrTiles / (kNarrow ? 2 : 1), kPairsAt = (kNarrow ? 3 : 1) * kPart;
+  constexpr int kSysBytes = kPairsAt * (kP ? 2 : 1);
   constexpr int kSysUnits = (kP ? 2 : 1) * kDrTiles / 16 / NT;
   static_assert(kDrTiles % (16 * NT) == 0, "whole units");
   static_assert(L == 0 || (kAhead && kSysLds), "waves that only load hold a chunk");
@@ -229,7 +230,7 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(rs[k][e]);
 #pragma unroll
-        for (int p = 0; p < (pairs ? kPParts : kTParts); ++p) {
+        for (int p = 0; p < 3; ++p) {
           const u2 v{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3])};
           *reinterpret_cast<u2*>(at + p * kPart) = v;
 #pragma unroll
@@ -290,22 +291,23 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
   // What a chunk leaves is stored after the next one's rows have come: loads and stores come back in
   // order, and a wait for rows behind stores would wait for those too.
   constexpr int kHeld = kNarrow ? NC / 2 : NC;
-  // out; e or dv, and what bf16 leaves of them
-  uint32_t held_o[kOut ? kHeld : 1], held_u[kKeeps ? kHeld : 1], held_l[kKeeps && kNarrow ? kHeld : 1];
-  float held32[KIND == kDrBackward && kNarrow ? NC : 1];
+  uint32_t held_o[kOut ? kHeld : 1];
+  float held_k[kKeeps ? NC : 1];  // e or dv
   int held_n = 0, held_c = 0;
   auto at_token = [&](int i) { return NC * (i / RT) + 4 * G * ((i % RT) >> 2) + 4 * g + (i & 3); };
   // Element (row, col) of a matrix of operands (dr_operand_at) with row = NC t + 4 G q + 4 g + r: this
   // lane's share of the address, and the rest, the same for all lanes.
   const int v_steps = (A.Dv + 15) / 16;
   const uint32_t operand_lane = la_in(
-      col < v_steps * 16, (((col >> 4) * 64 + 4 * g + 32 * ((col >> 2) & 1)) * 8 + (col & 3) + 4 * ((col >> 3) & 1)) * ES);
+      col < v_steps * 16, (((col >> 4) * 64 + 4 * g + 32 * ((col >> 2) & 1)) * 8 + (col & 3) + 4 * ((col >> 3) & 1)) * 4);
   auto operand_rest = [&](int t, int reg) {
     const int q = reg >> 2, r = reg & 3, row = NC == 32 ? 8 * q + r : 16 * (t & 1) + r;
-    return std::pair<int, int>{(NC == 32 ? t : t >> 1) * v_steps * 512 * ES, row * 8 * ES};
+    return std::pair<int, int>{(NC == 32 ? t : t >> 1) * v_steps * 2048, row * 32};
   };
-  // bf16: what is stored is turned by a product with the unit matrix (exact), so that a lane has four
-  // columns of a row and not a row's place in four of them: 8 bytes a store and not 2.
+  // bf16: e and the states are turned by products of its three parts with the unit matrix (their sum is the
+  // value, exactly), so that a lane has four columns of a row and not a row's place in four of them: 16
+  // bytes a store and not 4.
+  constexpr bool kTurned = KIND == kDrKept && kNarrow;  // held_k
   Op<M, 1> unit[2];
   if constexpr (kNarrow && kKeeps) {
 #pragma unroll
@@ -317,31 +319,23 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
       unit[j] = parts_of<M, 1>(one);
     }
   }
-  auto turned = [&](const Op<M, 1>* o, int t) {  // tile t of the operands: lane its row, registers columns
-    A_t d;
+  // Step f of a contraction into its tile (NC = 32: of two steps, `d` the sum; 16: of half a step, j which):
+  // lane its row, registers columns.
+  auto turn = [&](A_t& d, const Op<M, 3>& o, int j) {
+    if (NC == 16 || j == 0) {
 #pragma unroll
-    for (int r = 0; r < RT; ++r) d[r] = 0.0f;
-    if constexpr (NC == 32) {
-      mul<NC>(d, o[2 * t], unit[0]);
-      mul<NC>(d, o[2 * t + 1], unit[1]);
-    } else {
-      mul<NC>(d, o[t >> 1], unit[t & 1]);
+      for (int r = 0; r < RT; ++r) d[r] = 0.0f;
     }
-    return d;
+    mul<NC>(d, o, unit[j]);
   };
-  // Of such rows, for memory as operands: four words are a lane's 8 places of a step.  NC = 32: as they
-  // come, words 4 j .. of tile j / 2 and step j % 2; 16: of tiles 2 j and 2 j + 1, halves of the wave exchange theirs.
-  auto paired = [&](uint32_t* w) {
-    if constexpr (NC == 16) {
-      swap_halves(w[0], w[2]);
-      swap_halves(w[1], w[3]);
-    }
-    return u4{w[0], w[1], w[2], w[3]};
+  // The place of registers 4 q .. of such a tile among operands in memory.
+  auto turned_at = [&](int t, int q) {
+    const int row = NC * t + nn, step = (col0 + NC * wave + (NC == 32 ? 16 * (q >> 1) : 0)) >> 4;
+    return la_in(step < v_steps, (((row >> 5) * v_steps + step) * 64 + (row & 31) + 32 * (g & 1)) * 32 +
+                                     16 * (NC == 32 ? q & 1 : g >> 1));
   };
-  auto operand16 = [&](int j) {  // their place
-    const int row = NC == 32 ? 32 * (j >> 1) + nn : 16 * (2 * j + (lane >> 5)) + nn;
-    const int step = (col0 + NC * wave + (NC == 32 ? 16 * (j & 1) : 0)) >> 4;
-    return la_in(step < v_steps, (((row >> 5) * v_steps + step) * 64 + (row & 31) + 32 * (g & 1)) * 16);
+  auto four = [](const float* v) {
+    return u4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
   };
   auto hold = [&](uint32_t* to, const float* v) {
 #pragma unroll
@@ -352,41 +346,34 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
         to[i] = __float_as_uint(v[i]);
     }
   };
-  // Rows of tokens, those that `stop` tells (behind the walk's direction of it) as NaN: in bf16 only after
-  // they are turned, whose sums with zeros run over tokens.
+  // A chunk's e, or dv; NaN for the tokens that `stop` tells (behind the walk's direction of it).
   auto hold_rows = [&](float* v, bool poisoned, int stop) {
     constexpr float kNan = __builtin_nanf("");
-    if constexpr (kNarrow) {
-      Op<M, 1> o[2][TF];
+    if constexpr (kTurned) {
+      A_t d[TT];
 #pragma unroll
       for (int f = 0; f < TF; ++f) {
-        const auto both = parts_of<M, 2>(v + 8 * f);
-        o[0][f].p[0] = both.p[0];
-        o[1][f].p[0] = both.p[1];
+        const auto o = parts_of<M, 3>(v + 8 * f);
+        if constexpr (NC == 32) {
+          turn(d[f >> 1], o, f & 1);
+        } else {
+          turn(d[2 * f], o, 0);
+          turn(d[2 * f + 1], o, 1);
+        }
       }
+      // (only now: the products' sums with zeros run over tokens)
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        float d[NC];
-#pragma unroll
-        for (int t = 0; t < TT; ++t) {
-          const A_t x = turned(o[p], t);
-#pragma unroll
-          for (int r = 0; r < RT; ++r) d[RT * t + r] = x[r];
-        }
+      for (int i = 0; i < NC; ++i) {
+        held_k[i] = d[i / RT][i % RT];
         if (poisoned) {
-#pragma unroll
-          for (int i = 0; i < NC; ++i) {
-            const int r = i % RT, token = NC * (i / RT) + nn, from = __shfl(stop, 4 * G * (r >> 2) + 4 * g + (r & 3));
-            if (kBack ? token <= from : token >= from) d[i] = kNan;
-          }
+          const int r = i % RT, token = NC * (i / RT) + nn, from = __shfl(stop, 4 * G * (r >> 2) + 4 * g + (r & 3));
+          if (token >= from) held_k[i] = kNan;
         }
-        hold(p ? held_l : held_u, d);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < NC; ++i)
-        if (kBack ? at_token(i) <= stop : at_token(i) >= stop) v[i] = kNan;
-      hold(held_u, v);
+        held_k[i] = (kBack ? at_token(i) <= stop : at_token(i) >= stop) ? kNan : v[i];
     }
   };
   auto flush = [&]() {
@@ -423,53 +410,26 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
       }
     }
     if constexpr (kKeeps) {
-      void* const p = kBack ? A.dv : A.e;
       if (n > 0) {
         // backwards dense rows of the tokens that are there (the others lie behind the buffer), forwards
         // operands (zeros behind the sequence)
-        const int step = A.H * A.Dv * ES;
+        const int step = A.H * A.Dv * 4;
         const size_t elems = dr_operand_elems(kDrC, A.Dv);
         const size_t row = ((tok0 + t0) * A.H + h) * A.Dv, unit = static_cast<size_t>(row0 + held_c) * A.H + h;
-        const rsrc_t r = kBack ? make_rsrc(static_cast<E*>(p) + row, (n - 1) * step + A.Dv * ES)
-                               : make_rsrc(static_cast<E*>(p) + unit * M::kParts * elems,
-                                           static_cast<uint32_t>(elems) * M::kParts * ES);
-        const uint32_t lane_at = kBack ? la_in(col < A.Dv, 4 * g * step + col * ES) : operand_lane;
-        if constexpr (kNarrow) {
-          if constexpr (!kBack) {
+        const rsrc_t r = kBack ? make_rsrc(A.dv + row, (n - 1) * step + A.Dv * 4)
+                               : make_rsrc(A.e + unit * elems, static_cast<uint32_t>(elems) * 4);
+        if constexpr (kTurned) {
 #pragma unroll
-            for (int j = 0; j < kHeld / 4; ++j) {
-              const uint32_t to = operand16(j);
-              __builtin_amdgcn_raw_buffer_store_b128(paired(held_u + 4 * j), r, to, 0, 0);
-              __builtin_amdgcn_raw_buffer_store_b128(paired(held_l + 4 * j), r,
-                                                     to + static_cast<uint32_t>(elems) * 2, 0, 0);
-            }
-          }
-          const rsrc_t rl = kBack ? make_rsrc(static_cast<E*>(A.dv_lo) + row, (n - 1) * step + A.Dv * ES) : r;
+          for (int t = 0; t < TT; ++t)
 #pragma unroll
-          for (int t = 0; t < (kBack ? TT : 0); ++t)
-#pragma unroll
-            for (int q = 0; q < RT / 4; ++q) {
-              const int i = (RT * t + 4 * q) / 2, tok = NC * t + nn, cc = col0 + NC * wave + 4 * G * q + 4 * g;
-              const uint32_t to = la_in(cc < A.Dv, tok * step + cc * 2);
-              __builtin_amdgcn_raw_buffer_store_b64(u2{held_u[i], held_u[i + 1]}, r, to, 0, 0);
-              __builtin_amdgcn_raw_buffer_store_b64(u2{held_l[i], held_l[i + 1]}, rl, to, 0, 0);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < (kNarrow ? 0 : NC); ++i) {
-          const auto rest = kBack ? std::pair<int, int>{0, (at_token(i) - 4 * g) * step} : operand_rest(i / RT, i % RT);
-          __builtin_amdgcn_raw_buffer_store_b32(held_u[i], r, lane_at + rest.second, rest.first, 0);
-        }
-      }
-    }
-    if constexpr (KIND == kDrBackward) {
-      if constexpr (kNarrow) {
-        if (A.dv32) {
-          const rsrc_t rf = make_rsrc(A.dv32 + ((tok0 + t0) * A.H + h) * A.Dv, 0x7fffffffu);
+            for (int q = 0; q < RT / 4; ++q)
+              __builtin_amdgcn_raw_buffer_store_b128(four(held_k + RT * t + 4 * q), r, turned_at(t, q), 0, 0);
+        } else {
+          const uint32_t lane_at = kBack ? la_in(col < A.Dv, 4 * g * step + col * 4) : operand_lane;
 #pragma unroll
           for (int i = 0; i < NC; ++i) {
-            const int tk = at_token(i);
-            stb<float>(rf, la_in((tk < n) & (col < A.Dv), (tk * A.H * A.Dv + col) * 4), 0, held32[i]);
+            const auto rest = kBack ? std::pair<int, int>{0, (at_token(i) - 4 * g) * step} : operand_rest(i / RT, i % RT);
+            stb<float>(r, lane_at + rest.second, rest.first, held_k[i]);
           }
         }
       }
@@ -491,15 +451,14 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
     // what the gradients of this chunk need of the state
     if constexpr (kKeeps && !kNarrow) {
       const size_t elems = dr_operand_elems(A.Dk, A.Dv);
-      const rsrc_t rs = make_rsrc(static_cast<E*>(A.keep) + (static_cast<size_t>(row0 + c) * A.H + h) * elems,
-                                  static_cast<uint32_t>(elems) * ES);
+      const rsrc_t rs = make_rsrc(A.keep + (static_cast<size_t>(row0 + c) * A.H + h) * elems, static_cast<uint32_t>(elems) * 4);
 #pragma unroll
       for (int t = 0; t < KT; ++t)
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
           const auto rest = operand_rest(t, r);
           if (NC * t < (A.Dk + 31) / 32 * 32)  // rows behind the matrix: zeros up to the end of its tile
-            store_elem<M>(rs, operand_lane + rest.second, rest.first, S[t][r]);
+            stb<float>(rs, operand_lane + rest.second, rest.first, S[t][r]);
         }
     }
     const char* const sS = kSysLds ? at + oS : A.sys + (static_cast<size_t>(row0 + c) * A.H + h) * kDrSys;
@@ -514,25 +473,31 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
     for (int t = 0; t < TT; ++t)
 #pragma unroll
       for (int r = 0; r < RT; ++r) X[t][r] = O[t][r] = 0.0f;
-    Op<M, 1> rounded[2][kNarrow && kKeeps ? KF : 1];  // by parts
+    const size_t keep_elems = dr_operand_elems(A.Dk, A.Dv);
+    const rsrc_t keep = make_rsrc(A.keep + (static_cast<size_t>(row0 + c) * A.H + h) * keep_elems,
+                                  kNarrow && kKeeps ? static_cast<uint32_t>(keep_elems) * 4 : 0);
+    A_t kept;
 #pragma unroll
     for (int f = 0; f < KF; ++f) {
       float s[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) s[e] = S[(8 * f + e) / RT][(8 * f + e) % RT];
-      // three parts in the chain, two where an output is rounded
       const auto sp = parts_of<M, 3>(s);
-      Op<M, 2> so;
-      if constexpr (kNarrow) {
-        so.p[0] = sp.p[0];
-        so.p[1] = sp.p[1];
-        if constexpr (kKeeps) {
-          rounded[0][f].p[0] = sp.p[0];
-          rounded[1][f].p[0] = sp.p[1];
-        }
-      } else {
+      if constexpr (kNarrow && kKeeps) {
+        // the state before the chunk (backwards the adjoint behind it): zeros up to the end of its tile of 32
+        // rows
 #pragma unroll
-        for (int e = 0; e < 8; ++e) so.x[e] = sp.x[e];
+        for (int j = 0; j < 2; ++j) {
+          const int t = NC == 32 ? f >> 1 : 2 * f + j;
+          if (NC == 32 && j != (f & 1)) continue;
+          turn(kept, sp, j);
+          if ((NC == 32 && j == 0) || NC * t / 32 * 32 >= A.Dk) continue;
+#pragma unroll
+          for (int q = 0; q < RT / 4; ++q) {
+            const float v[4] = {kept[4 * q], kept[4 * q + 1], kept[4 * q + 2], kept[4 * q + 3]};
+            __builtin_amdgcn_raw_buffer_store_b128(four(v), keep, turned_at(t, q), 0, 0);
+          }
+        }
       }
       Op<M, 1> ko[TT], qo[TT];
 #pragma unroll
@@ -545,34 +510,8 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
 #pragma unroll
         for (int t = 0; t < TT; ++t) {
           mul_one<NC>(X[t], ko[t], sp, k);
-          if constexpr (kOut)
-            if (k < kPairs<1, 2>) mul_one<NC>(O[t], so, qo[t], k);
+          if constexpr (kOut) mul_one<NC>(O[t], sp, qo[t], k);
         }
-    }
-
-    if constexpr (kNarrow && kKeeps) {
-      const size_t elems = dr_operand_elems(A.Dk, A.Dv);
-      const rsrc_t rs = make_rsrc(static_cast<E*>(A.keep) + (static_cast<size_t>(row0 + c) * A.H + h) * 2 * elems,
-                                  static_cast<uint32_t>(elems) * 2 * ES);
-#pragma unroll
-      for (int t = 0; t < KT; t += 32 / NC) {
-        if (NC * t >= A.Dk) continue;  // (rows behind the matrix: zeros up to the end of its tile of 32)
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          uint32_t w[8];
-#pragma unroll
-          for (int k = 0; k < 32 / NC; ++k) {
-            const A_t d = turned(rounded[p], t + k);
-#pragma unroll
-            for (int r = 0; r < RT; r += 2) w[(RT * k + r) / 2] = pack_bf16x2(d[r], d[r + 1]);
-          }
-#pragma unroll
-          for (int j = 0; j < NC / 16; ++j)
-            __builtin_amdgcn_raw_buffer_store_b128(
-                paired(w + 4 * j), rs,
-                operand16(NC * t / 32 * (NC / 16) + j) + p * static_cast<uint32_t>(elems) * 2, 0, 0);
-        }
-      }
     }
 
     const char* zat = sZ + NC * wave * ES + col_share<M, G, RZ>(lane);
@@ -650,12 +589,12 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
         for (int r = 0; r < RT; ++r) Y[t][r] = 0.0f;
 #pragma unroll
       for (int f = 0; f < TF; ++f) {
-        Op<M, kPParts> m[TT];
+        Op<M, 3> m[TT];
 #pragma unroll
         for (int t = 0; t < TT; ++t)
-          if (Mat::any(t, f)) m[t] = Mat::template get<kPParts>(sS + kPairsAt, t, f, nn, g);
+          if (Mat::any(t, f)) m[t] = Mat::get(sS + kPairsAt, t, f, nn, g);
 #pragma unroll
-        for (int k = 0; k < kPairs<kPParts, 1>; ++k)
+        for (int k = 0; k < kPairs<3, 1>; ++k)
 #pragma unroll
           for (int t = 0; t < TT; ++t)
             if (Mat::any(t, f)) mul_one<NC>(Y[t], m[t], zo[f], k);
@@ -705,7 +644,7 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
       Op<M, 3> m[TT];
 #pragma unroll
       for (int t = 0; t < TT; ++t)
-        if (Mat::any(t, f)) m[t] = Mat::template get<3>(sS, t, f, nn, g);
+        if (Mat::any(t, f)) m[t] = Mat::get(sS, t, f, nn, g);
 #pragma unroll
       for (int k = 0; k < kPairs<3, 3>; ++k)
 #pragma unroll
@@ -728,13 +667,13 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
 
     if constexpr (kOut) {
       // ---- out
-      Op<M, 2> uo[TF];
+      Op<M, 3> uo[TF];
 #pragma unroll
       for (int f = 0; f < TF; ++f) {
         float v[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = u[8 * f + e];
-        uo[f] = parts_of<M, 2>(v);
+        uo[f] = parts_of<M, 3>(v);
       }
 #pragma unroll
       for (int t = 0; t < TT; ++t) {
@@ -744,12 +683,12 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
       }
 #pragma unroll
       for (int f = 0; f < TF; ++f) {
-        Op<M, 2> m[TT];
+        Op<M, 3> m[TT];
 #pragma unroll
         for (int t = 0; t < TT; ++t)
-          if (Mat::any(t, f)) m[t] = Mat::template get<2>(sS + kPairsAt, t, f, nn, g);
+          if (Mat::any(t, f)) m[t] = Mat::get(sS + kPairsAt, t, f, nn, g);
 #pragma unroll
-        for (int k = 0; k < kPairs<2, 2>; ++k)
+        for (int k = 0; k < kPairs<3, 3>; ++k)
 #pragma unroll
           for (int t = 0; t < TT; ++t)
             if (Mat::any(t, f)) mul_one<NC>(O[t], uo[f], m[t], k);
@@ -775,10 +714,6 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
       float dv[NC];
 #pragma unroll
       for (int i = 0; i < NC; ++i) dv[i] = u[i];
-      if constexpr (kNarrow) {
-#pragma unroll
-        for (int i = 0; i < NC; ++i) held32[i] = reached(at_token(i)) ? __int_as_float(0x7fc00000) : u[i];
-      }
       hold_rows(dv, poisoned, stop);
     }
     held_n = n;

@@ -35,11 +35,9 @@ using Acc = typename Shape<NC>::Acc;
 
 struct InBf16 {
   using E = uint16_t;
-  static constexpr int kParts = 2;  // of a matrix that is kept as an operand
 };
 struct InF32 {
   using E = float;
-  static constexpr int kParts = 1;
 };
 
 // Operands: of P parts that add up to the value (fp32: one, whatever P).
@@ -158,14 +156,6 @@ __device__ __forceinline__ void values(const Op<InF32, 1>& o, float* x) {
   for (int i = 0; i < 8; ++i) x[i] = o.x[i];
 }
 
-__device__ __forceinline__ void values(const Op<InBf16, 2>& o, float* x) {
-  float y[8];
-  values(Op<InBf16, 1>{{o.p[0]}}, x);
-  values(Op<InBf16, 1>{{o.p[1]}}, y);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] += y[i];
-}
-
 // Step f of a contraction along a row in memory, `g` the lane's group.
 template <class M, int G>
 __device__ __forceinline__ Op<M, 1> row_op(const char* row, int f, int g) {
@@ -223,22 +213,6 @@ __device__ __forceinline__ Op<M, 1> col_op(const char* at, int t0, int c0) {
       r.x[i] = *reinterpret_cast<const float*>(at + (t0 + (i >> 2) * 4 * G + (i & 3)) * RB + c0 * 4);
   }
   return r;
-}
-
-// One element rounded to the arithmetic's type.
-template <class M>
-__device__ __forceinline__ void store_elem(rsrc_t r, uint32_t at, uint32_t base, float v) {
-  if constexpr (sizeof(typename M::E) == 2)
-    stb<bf16>(r, at, base, v);
-  else
-    stb<float>(r, at, base, v);
-}
-
-// Upper half of a's lanes for the lower half of b's.
-__device__ __forceinline__ void swap_halves(uint32_t& a, uint32_t& b) {
-  const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
-  a = r[0];
-  b = r[1];
 }
 
 }  // namespace prnn

@@ -13,9 +13,9 @@ pool of states, in place.  Layouts, packed sequences, shared heads, states and p
 
 The rule is stable where ``beta_t |k_t|^2`` lies in 0 .. 2: keys of unit length and rates in (0, 1),
 or up to 2 where a state may also be reflected.  float32, bfloat16 and float16; arithmetic and
-states are float32 (bfloat16 of widths in eights on bfloat16 matrix products: operands of 24 bits
-where they reach a state, of 16 where they only reach a result of bfloat16, and in what the backward
-pass keeps), results are rounded once.  No atomics: equal calls give equal bits.
+states are float32 (bfloat16 of widths in eights on bfloat16 matrix products, whose operands are all 24
+bits of a float32 value in three parts), results are rounded once.  Sums run in a fixed order: equal calls
+give equal bits.
 """
 
 from __future__ import annotations
