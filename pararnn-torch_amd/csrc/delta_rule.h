@@ -40,8 +40,8 @@ constexpr int kDrC = 64;  // tokens of a chunk
 
 // ---- where chunks and pieces lie ---------------------------------------------------------
 //
-// Units of `len` tokens counted from every sequence's own start, so that a sequence's results do
-// not depend on what lies next to it.  Unit i of sequence s of a packed stream is number
+// Units of `len` tokens counted from every sequence's own start.  (How long pieces are goes by the whole
+// batch, and with it the last bits of a result.)  Unit i of sequence s of a packed stream is number
 // s + floor(cu[s] / len) + i: numbers are distinct and below n_seq + ceil(T / len).
 struct DrUnit {
   int seq, index, count;  // index of `count` in its sequence
@@ -86,6 +86,14 @@ inline long long dr_units(const LaSeqs& q, long long len) {
   if (q.cu) return q.n_seq + (q.T + len - 1) / len;
   return static_cast<long long>(q.n_seq) * (q.T > len ? (q.T + len - 1) / len : 1);
 }
+
+// Between a cut sequence's pieces i and i + 1 lies slot i of its own, for a state and a transfer.  Of a
+// packed stream it is number floor(cu[s] / len) + i: the last of a sequence's, with n = ceil(L / len) pieces,
+// is below floor((cu[s] + L) / len), where the next one's begin, and all are below T / len.
+__device__ __forceinline__ size_t dr_slot(const LaSeqs& q, const DrUnit& piece, int i) {
+  return static_cast<size_t>(q.cu ? piece.s0 / q.len : piece.seq * (piece.count - 1)) + i;
+}
+inline long long dr_slots(const LaSeqs& q) { return q.cu ? q.T / q.len : dr_units(q, q.len) - q.n_seq; }
 
 // Token 0 of a unit among all tokens of the batch (rows of dense arrays).
 __device__ __forceinline__ size_t dr_token(const LaSeqs& q, const DrUnit& u, int t) {
@@ -149,8 +157,8 @@ struct DrWalk {
   float* keep;               // (chunk, H), Dk x Dv likewise: states before the chunks, adjoints behind them
   float* dv;                 // backwards, dense (token, H, Dv)
   LaState init, last;
-  float* piece;              // (piece, H, Dk, Dv): the pieces' own states
-  uint16_t* transfer;        // (piece, H): their transfers, as operands in three bf16 parts
+  float* piece;              // (slot, H, Dk, Dv): the pieces' own states, then those that they begin with
+  uint16_t* transfer;        // (slot, H): their transfers, as operands in three bf16 parts
   int H, Dk, Dv, dtype;
   const int* order;          // of the pieces (DrSystems), NULL: as they are
   int n_pieces;

@@ -148,9 +148,9 @@ Scratch carve(void* ws, const Problem& a, const Plan& plan, bool systems, bool b
     s.order = static_cast<int*>(c.take(4 * static_cast<size_t>(pieces_of(a))));
   }
   if (plan.cut) {
-    const size_t pieces = dr_units(plan.seqs, plan.seqs.len) * heads;
-    s.piece = static_cast<float*>(c.take(4 * pieces * a.la.Dk * a.la.Dv));
-    s.transfer = static_cast<uint16_t*>(c.take(6 * pieces * dr_operand_elems(a.la.Dk, a.la.Dk)));
+    const size_t slots = dr_slots(plan.seqs) * heads;
+    s.piece = static_cast<float*>(c.take(4 * slots * a.la.Dk * a.la.Dv));
+    s.transfer = static_cast<uint16_t*>(c.take(6 * slots * dr_operand_elems(a.la.Dk, a.la.Dk)));
   }
   if (backward) {
     s.behind = static_cast<float*>(c.take(4 * units * heads * dr_operand_elems(a.la.Dk, a.la.Dv)));

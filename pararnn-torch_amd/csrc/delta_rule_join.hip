@@ -15,8 +15,8 @@ namespace {
 
 struct JoinArgs {
   LaSeqs seqs;
-  float* piece;           // in: U_p, out: S_p  (piece, H, Dk, Dv)
-  const uint16_t* transfer;  // (piece, H): operands in three parts
+  float* piece;           // in: U_p, out: S_{p+1}  (slot, H, Dk, Dv)
+  const uint16_t* transfer;  // (slot, H): operands in three parts
   LaState init;
   int H, Dk, Dv, tiles, back;
 };
@@ -54,8 +54,8 @@ __global__ __launch_bounds__(256) void dr_join_kernel(JoinArgs A) {
   Op<InBf16, 3> m[8];
   f16v own[R];
   auto unit_of = [&](int k) {
-    k = min(k, u.count - 1);
-    return static_cast<size_t>(first + (A.back ? u.count - 1 - k : k)) * A.H + h;
+    k = min(k, u.count - 2);
+    return dr_slot(A.seqs, u, A.back ? u.count - 2 - k : k) * A.H + h;
   };
   auto transfer_of = [&](int k) {  // (the last piece hands on to none)
     return make_rsrc(A.transfer + unit_of(k) * 3 * elems, k + 1 < u.count ? static_cast<uint32_t>(elems) * 6 : 0u);
@@ -84,17 +84,14 @@ __global__ __launch_bounds__(256) void dr_join_kernel(JoinArgs A) {
 #pragma unroll
     for (int f = 0; f < 8; ++f) m[f] = operand(rm, 0, f);
   }
-  for (int k = 0; k < u.count; ++k) {
+  for (int k = 0; k + 1 < u.count; ++k) {
     const rsrc_t rp = make_rsrc(A.piece + unit_of(k) * state_floats, static_cast<uint32_t>(state_floats) * 4);
     f16v sum[R][2];  // a matrix instruction waits for its own sum's last one
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       sum[r][0] = own[r];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        sum[r][1][e] = 0.0f;
-        stb<float>(rp, at(r, e), 0, S[r][e]);
-      }
+      for (int e = 0; e < 16; ++e) sum[r][1][e] = 0.0f;
     }
     __syncthreads();  // the last step's operands have been read
 #pragma unroll
@@ -129,7 +126,10 @@ __global__ __launch_bounds__(256) void dr_join_kernel(JoinArgs A) {
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) S[r][e] = sum[r][0][e] + sum[r][1][e];
+      for (int e = 0; e < 16; ++e) {
+        S[r][e] = sum[r][0][e] + sum[r][1][e];
+        stb<float>(rp, at(r, e), 0, S[r][e]);  // in the place of the piece's own
+      }
   }
 }
 

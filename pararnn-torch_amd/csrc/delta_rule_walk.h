@@ -272,8 +272,8 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
     }
   if (!kOwn) {
     const float* src = nullptr;
-    if (A.piece && pc.count > 1)
-      src = A.piece + (static_cast<size_t>(piece) * A.H + h) * state_floats;
+    if (A.piece && pc.index != (kBack ? pc.count - 1 : 0))
+      src = A.piece + (dr_slot(A.seqs, pc, kBack ? pc.index : pc.index - 1) * A.H + h) * state_floats;
     else if (const float* row = la_row(A.init, pc.seq, A.H * state_floats))
       src = row + h * state_floats;
     if (src) {
@@ -772,9 +772,10 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
   if (!kOwn) flush();
 
   // ---- the state behind the piece
+  const size_t slot = kOwn ? dr_slot(A.seqs, pc, kBack ? pc.index - 1 : pc.index) : 0;
   if (transfer) {
     const size_t elems = dr_operand_elems(A.Dk, A.Dk);
-    const rsrc_t rs = make_rsrc(A.transfer + (static_cast<size_t>(piece) * A.H + h) * 3 * elems,
+    const rsrc_t rs = make_rsrc(A.transfer + (slot * A.H + h) * 3 * elems,
                                 static_cast<uint32_t>(elems) * 6);
 #pragma unroll
     for (int t = 0; t < KT; ++t)
@@ -794,7 +795,7 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
   }
   float* dst = nullptr;
   if (kOwn) {
-    dst = A.piece + (static_cast<size_t>(piece) * A.H + h) * state_floats;
+    dst = A.piece + (slot * A.H + h) * state_floats;
   } else if (pc.index == (kBack ? 0 : pc.count - 1)) {
     if (float* row = la_row(A.last, pc.seq, A.H * state_floats)) dst = row + h * state_floats;
   }
