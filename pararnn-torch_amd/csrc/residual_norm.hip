@@ -63,12 +63,12 @@ __global__ __launch_bounds__(NT < 256 ? 256 : NT) void rn_forward_kernel(RnArgs 
   }
 }
 
-// dst[c] = the workgroups' sums in their order: 64 columns a workgroup, its 4 waves a quarter of the
+// dst[c] = the workgroups' sums in their order: 64 columns a workgroup, its 16 waves a sixteenth of the
 // parts each.
 struct RnSums {
   const float* parts;
   void* dst[4];
-  int groups, C, w_dtype, dtype;
+  int groups, C, w_dtype;
 };
 template <typename T>
 __global__ __launch_bounds__(1024) void rn_sum_kernel(RnSums A) {
@@ -219,7 +219,7 @@ extern "C" PRNN_API int prnn_residual_norm_backward(
   if (int rc = rn_backward(a, dtype, vec, groups, st)) return rc;
   if (!sums) return PRNN_OK;
   return with_storage(dtype, [&](auto t) {
-    const RnSums s{a.parts, {dw, db, dpw, dscale}, groups, C, w_dtype, dtype};
+    const RnSums s{a.parts, {dw, db, dpw, dscale}, groups, C, w_dtype};
     rn_sum_kernel<decltype(t)><<<dim3((C + 63) / 64, 4), 1024, 0, st>>>(s);
     PRNN_HIP(hipGetLastError());
     return static_cast<int>(PRNN_OK);
