@@ -237,13 +237,15 @@ constexpr Total kNoTotal{0, ~0ull, ~0u};
 __global__ __launch_bounds__(256) void beam_choose_kernel(BeamArgs A) {
   __shared__ Total s_top[256], s_list[kMost * kRound + kMost], s_carry[kMost], s_bound[4];
   __shared__ int s_count, s_held;
-  __shared__ double s_off[kMost], s_most[kMost];  // a total is (logit - most) + off
+  // A total is ((logit - most) + score) - log(sum): the first two sums are exact for logits and scores of like
+  // size, so that what is equal in a row's candidates, or in equal rows', stays equal.
+  __shared__ double s_most[kMost], s_score[kMost], s_log[kMost];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, b = blockIdx.x;
   const int per = A.S * A.M;  // candidates of a beam; all of kMost beams' are below 2^26
   const bool few = A.M <= kFew;
   if (tid == 0) s_held = 0;
-  // score - log(sum), beams in blocks of kMost, a beam a wave; the largest logit stays apart (masks of
-  // the type's lowest value would swallow the logarithm)
+  // What the beams' totals are made of, beams in blocks of kMost, a beam a wave; the largest logit stays
+  // apart (masks of the type's lowest value would swallow the logarithm)
   for (int k0 = 0; k0 < A.K; k0 += kMost) {
     __syncthreads();
     const int end = min(A.K - k0, kMost) * per;
@@ -278,7 +280,7 @@ __global__ __launch_bounds__(256) void beam_choose_kernel(BeamArgs A) {
       if (base == 0) {
         for (int k = k0 + wave; k < min(A.K, k0 + kMost); k += 4) {
           const int row = b * A.K + k;
-          double off = A.scores[row], most = -static_cast<double>(INFINITY);
+          double score = A.scores[row], most = -static_cast<double>(INFINITY), log_sum = 0.0;
           if (!(A.ended && A.ended[row])) {
             const Slice* x = A.slices + static_cast<size_t>(row) * A.S;
             Slice own = lane < A.S ? x[lane] : Slice{0.0, -INFINITY, 0};
@@ -298,11 +300,13 @@ __global__ __launch_bounds__(256) void beam_choose_kernel(BeamArgs A) {
 #pragma unroll
             for (int m = 1; m < 64; m <<= 1) sum += __shfl_xor(sum, m);
             most = top;
-            off = __any(bad) ? -static_cast<double>(INFINITY) : off - log(sum);
+            if (__any(bad)) score = -static_cast<double>(INFINITY);
+            log_sum = log(sum);
           }
           if (lane == 0) {
-            s_off[k - k0] = off;
             s_most[k - k0] = most;
+            s_score[k - k0] = score;
+            s_log[k - k0] = log_sum;
           }
         }
         __syncthreads();
@@ -314,10 +318,11 @@ __global__ __launch_bounds__(256) void beam_choose_kernel(BeamArgs A) {
         const int k = beam[i];
         if (k < 0) continue;
         if (over[i]) {
-          c[i] = total(s_off[k], k0 + k, 0, A.pad);
+          c[i] = total(s_score[k], k0 + k, 0, A.pad);
         } else {
           const float logit = __uint_as_float(best[i].x & 0x80000000u ? best[i].x & 0x7fffffffu : ~best[i].x);
-          c[i] = total((static_cast<double>(logit) - s_most[k]) + s_off[k], k0 + k, ~best[i].x, best[i].y);
+          const double t = ((static_cast<double>(logit) - s_most[k]) + s_score[k]) - s_log[k];
+          c[i] = total(t, k0 + k, ~best[i].x, best[i].y);
         }
         if (c[i].o && before(c[i], top)) top = c[i];
       }

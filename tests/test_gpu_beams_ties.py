@@ -79,3 +79,18 @@ def test_scores_are_those_of_64_bits(dtype, spread):
     b = torch.arange(B)[:, None].expand(B, K)
     want = total[b, p.long(), t.long()]
     assert ((s.double() - want).abs() <= 2.0 ** -24 * want.abs() + V * 2.0 ** -51).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+def test_totals_that_are_equal_by_their_parts(dtype):
+    """Equal rows whose scores differ by as much as their logits do, all in steps of a quarter: a total is
+    the score and the logit, exactly, less what the rows share.  Equal ones go to the lowest beam."""
+    from pararnn_amd import beam_select
+
+    K, V, M = 12, 700, 100
+    r = torch.Generator().manual_seed(11)
+    row = torch.randint(-40, 40, (V,), generator=r) / 4
+    scores = -torch.randint(0, 40, (K,), generator=r) / 4
+    _, p, t = beam_select(row.to(dtype).expand(1, K, V).contiguous().to(DEV), scores[None].to(DEV), beams=M)
+    want = sorted((-float(scores[k] + row[i]), k, -float(row[i]), i) for k in range(K) for i in range(V))[:M]
+    assert list(zip(p[0].tolist(), t[0].tolist())) == [(k, i) for _, k, _, i in want]
