@@ -14,7 +14,7 @@
 //
 // Eight waves: four for the pairs and dq, four for dk, each with its own code and the same barriers, so
 // that two workgroups a CU (what LDS holds) are four waves a SIMD (four waves that did all took 1.24
-// times as long).  4096 chunks of bf16, D = 64: 158 us for 470 MB, of which 317 reach memory (3 TB/s of all).
+// times as long).  4096 chunks of bf16, D = 64: 158 us for 470 MB, of which 324 reach memory (3 TB/s of all).
 // Vector instructions take half of the time, most of them the splits of fp32 operands into three bf16 parts
 // (125 us with two parts, whose 16 bits showed in the results' last place), the phases' latencies the rest.
 #include "delta_rule_loads.h"

@@ -6,7 +6,7 @@
 //
 // A workgroup takes 32 columns of the state; its four waves take 32 rows each in turn, all operands in
 // three bf16 parts (24 bits), the state handed round through LDS in parts.  Transfers lie in memory as
-// operands (dr_operand_at).  Bound by the chain from piece to piece, 2.4 us each (D = 128, 16 pieces: 38
+// operands (dr_operand_at).  Bound by the chain from piece to piece, 2.6 us each (D = 128, 16 pieces: 40
 // us), of which the next piece's operands, held in registers, and two sums in turn have taken a third.
 #include "delta_rule_loads.h"
 
