@@ -58,7 +58,7 @@ __device__ __forceinline__ double value(uint64_t o) {
 }
 
 // exp(x) for x <= 0 as a whole number of 2^-50: 2^n 2^f with |f| <= 1/2, 2^f = sum (f ln 2)^i / i! to i = 12.
-// Off by half of one, and by 2^-51 relative (what the sum leaves out, and the reduction).
+// Off by half of one, and by (|x| + 2) 2^-53 of itself (the reduction and what the sum leaves out).
 constexpr int kUnit = 50;
 struct Taylor {
   double c[13] = {1.0};

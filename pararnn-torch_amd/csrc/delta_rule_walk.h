@@ -304,10 +304,9 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
     const int q = reg >> 2, r = reg & 3, row = NC == 32 ? 8 * q + r : 16 * (t & 1) + r;
     return std::pair<int, int>{(NC == 32 ? t : t >> 1) * v_steps * 2048, row * 32};
   };
-  // bf16: e and the states are turned by products of its three parts with the unit matrix (their sum is the
-  // value, exactly), so that a lane has four columns of a row and not a row's place in four of them: 16
-  // bytes a store and not 4.
-  constexpr bool kTurned = KIND == kDrKept && kNarrow;  // held_k
+  // bf16: states are turned by products of their three parts with the unit matrix (the sum is the value,
+  // exactly), so that a lane has four columns of a row and not a row's place in four of them: 16 bytes a
+  // store and not 4.
   Op<M, 1> unit[2];
   if constexpr (kNarrow && kKeeps) {
 #pragma unroll
@@ -347,34 +346,10 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
     }
   };
   // A chunk's e, or dv; NaN for the tokens that `stop` tells (behind the walk's direction of it).
-  auto hold_rows = [&](float* v, bool poisoned, int stop) {
-    constexpr float kNan = __builtin_nanf("");
-    if constexpr (kTurned) {
-      A_t d[TT];
+  auto hold_rows = [&](const float* v, int stop) {
 #pragma unroll
-      for (int f = 0; f < TF; ++f) {
-        const auto o = parts_of<M, 3>(v + 8 * f);
-        if constexpr (NC == 32) {
-          turn(d[f >> 1], o, f & 1);
-        } else {
-          turn(d[2 * f], o, 0);
-          turn(d[2 * f + 1], o, 1);
-        }
-      }
-      // (only now: the products' sums with zeros run over tokens)
-#pragma unroll
-      for (int i = 0; i < NC; ++i) {
-        held_k[i] = d[i / RT][i % RT];
-        if (poisoned) {
-          const int r = i % RT, token = NC * (i / RT) + nn, from = __shfl(stop, 4 * G * (r >> 2) + 4 * g + (r & 3));
-          if (token >= from) held_k[i] = kNan;
-        }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < NC; ++i)
-        held_k[i] = (kBack ? at_token(i) <= stop : at_token(i) >= stop) ? kNan : v[i];
-    }
+    for (int i = 0; i < NC; ++i)
+      held_k[i] = (kBack ? at_token(i) <= stop : at_token(i) >= stop) ? __builtin_nanf("") : v[i];
   };
   auto flush = [&]() {
     const int t0 = pc.begin + held_c * kDrC, n = held_n;  // nothing held: 0 tokens
@@ -418,19 +393,11 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
         const size_t row = ((tok0 + t0) * A.H + h) * A.Dv, unit = static_cast<size_t>(row0 + held_c) * A.H + h;
         const rsrc_t r = kBack ? make_rsrc(A.dv + row, (n - 1) * step + A.Dv * 4)
                                : make_rsrc(A.e + unit * elems, static_cast<uint32_t>(elems) * 4);
-        if constexpr (kTurned) {
+        const uint32_t lane_at = kBack ? la_in(col < A.Dv, 4 * g * step + col * 4) : operand_lane;
 #pragma unroll
-          for (int t = 0; t < TT; ++t)
-#pragma unroll
-            for (int q = 0; q < RT / 4; ++q)
-              __builtin_amdgcn_raw_buffer_store_b128(four(held_k + RT * t + 4 * q), r, turned_at(t, q), 0, 0);
-        } else {
-          const uint32_t lane_at = kBack ? la_in(col < A.Dv, 4 * g * step + col * 4) : operand_lane;
-#pragma unroll
-          for (int i = 0; i < NC; ++i) {
-            const auto rest = kBack ? std::pair<int, int>{0, (at_token(i) - 4 * g) * step} : operand_rest(i / RT, i % RT);
-            stb<float>(r, lane_at + rest.second, rest.first, held_k[i]);
-          }
+        for (int i = 0; i < NC; ++i) {
+          const auto rest = kBack ? std::pair<int, int>{0, (at_token(i) - 4 * g) * step} : operand_rest(i / RT, i % RT);
+          stb<float>(r, lane_at + rest.second, rest.first, held_k[i]);
         }
       }
     }
@@ -707,14 +674,11 @@ __global__ __launch_bounds__(64 * (W + L), (dr_pair_waves<M, NC, KD, W, KIND>)) 
       if constexpr (KIND == kDrKept) {
 #pragma unroll
         for (int i = 0; i < NC; ++i) v[i] = Y[i / RT][i % RT];
-        hold_rows(v, poisoned, stop);
+        hold_rows(v, stop);
       }
     }
     if constexpr (KIND == kDrBackward) {
-      float dv[NC];
-#pragma unroll
-      for (int i = 0; i < NC; ++i) dv[i] = u[i];
-      hold_rows(dv, poisoned, stop);
+      hold_rows(u, stop);
     }
     held_n = n;
     held_c = c;
