@@ -13,7 +13,7 @@
 //
 // Bound by this chain: one wave a SIMD goes through some 9500 cycles a chunk (bf16, D = 64; matrix
 // instructions 2700 of them, the rest splits of results into bf16 parts, LDS reads and waits), so 2048
-// tokens of 128 heads take 129 us forwards with what is kept and 116 backwards, and 16384 tokens of 8
+// tokens of 128 heads take 130 us forwards with what is kept and 115 backwards, and 16384 tokens of 8
 // heads, D = 128, in 16 pieces, 74 us.
 //
 // bf16 operands: K, Q and z as they are given; the state, what the tokens write, the system and its right
